@@ -38,7 +38,7 @@ extern "C" {
 #define SLHIP_API __attribute__((visibility("default")))
 #endif
 
-#define SLHIP_ABI_VERSION 5
+#define SLHIP_ABI_VERSION 6
 
 typedef enum slhip_status {
     SLHIP_OK = 0,
@@ -47,7 +47,7 @@ typedef enum slhip_status {
     SLHIP_ERR_HIP = -3,         /* the HIP runtime reported an error */
     SLHIP_ERR_INDEX = -4,       /* a gather index was outside [0, V) (reported by slhip_stream_sync) */
     SLHIP_ERR_NO_DEVICE = -5,   /* no usable device / driver */
-    SLHIP_ERR_CACHE = -6,       /* a KV-cache row outside the cache or block table (at slhip_stream_sync) */
+    SLHIP_ERR_CACHE = -6,       /* a KV-cache row, block or request outside the cache or block table (at slhip_stream_sync) */
     SLHIP_ERR_FORMAT = -7       /* malformed file data: a truncated or inconsistent GGUF file */
 } slhip_status;
 
@@ -437,6 +437,126 @@ SLHIP_API int slhip_gather(int format, const void* table, int64_t V, int64_t D, 
  */
 SLHIP_API int slhip_cache_write(int dtype_in, int dtype_cache, const void* x, int64_t x_stride, int64_t T,
                                 int64_t inner, void* cache, const slhip_cache_rows* rows, slhip_stream stream);
+
+/* ---- paged 8-bit KV cache: tables, write, attention ----------------------------------------------
+ *
+ * A serving step of B requests ("the batch"): request i has past[i] cached tokens and brings the rows starts[i] ..
+ * starts[i+1]-1 of the step's T rows, positions past[i], past[i]+1, ...; its blocks are row slots[i] (NULL: i) of the
+ * block table pages [page_slots, blocks_per_slot]. Rows from starts[B] on are padding: no op reads or writes them.
+ * starts[0] is 0 and starts never falls. All lengths live on the device, so a captured step replays with other lengths.
+ * No op allocates, none keeps anything between calls, and results do not depend on timing (no atomics on data). */
+
+/*
+ * Block tables and slot maps from request lengths.
+ *
+ * slhip_kv_pages_advance: takes the blocks that the step's new tokens need from the free list, a stack of *n_free block
+ *   ids whose top is free_blocks[*n_free - 1], and lays out the step's rows:
+ *     held(i) = ceil(past[i] / block_size), need(i) = ceil((past[i] + count[i]) / block_size) - held(i),
+ *     o(i) = need(0) + .. + need(i-1):
+ *     pages[slot, held(i) + j] = free_blocks[*n_free - 1 - (o(i) + j)] for j < need(i); *n_free_out = *n_free - o(B);
+ *     starts[i] = count[0] + .. + count[i-1] (B + 1 values);
+ *     for row t of request i: pos[t] = past[i] + t - starts[i], seq[t] = (slot, pos[t], i, block of pos[t]): the rows of
+ *     slhip_cache_rows (SLHIP_ROWS_PAGED) and positions of slhip_rope; rows behind the last: seq = (-1,-1,-1,-1), pos = 0.
+ * slhip_kv_pages_release: the blocks of requests that ended, ceil(past[i] / block_size) of slot i each, go back on the
+ *   stack in order (free_blocks[*n_free + ..]; capacity free_capacity), their table entries become -1, and
+ *   *n_free_out = *n_free + the blocks. count, starts, seq, pos and tokens are not used.
+ *
+ * n_free_out may be n_free itself (one counter that the steps of a captured loop advance) or another word (the old count
+ * stays, to step back to). All or nothing: where a length is negative, a context would outgrow its table row or the rows
+ * `tokens`, a slot is outside the table or named twice, or the free list has too few ids (too little room), the tables,
+ * the list and the count stay as they were (*n_free_out = *n_free), starts are 0, every row is padding, and the next
+ * slhip_stream_sync reports SLHIP_ERR_CACHE. Arrays are int32; seq and pos may be NULL.
+ * requests <= 4096, page_slots <= 131072, block_size a power of two, blocks_per_slot * block_size < 2^31, tokens < 2^31.
+ * Sizes of zero are fine (no requests: starts[0] = 0, all rows padding).
+ */
+typedef struct slhip_kv_pages {
+    int64_t requests;             /* B */
+    const int32_t* past;          /* [B] */
+    const int32_t* count;         /* [B] (advance) */
+    const int32_t* slots;         /* [B], or NULL: slot i */
+    int32_t* pages;               /* [page_slots, blocks_per_slot] */
+    int64_t page_slots, blocks_per_slot, block_size;
+    int32_t* free_blocks;         /* [free_capacity]; advance only reads it */
+    int64_t free_capacity;
+    const int32_t* n_free;        /* [1] */
+    int32_t* n_free_out;          /* [1] */
+    int64_t tokens;               /* rows of seq and pos */
+    int32_t* starts;              /* [B + 1] */
+    int32_t* seq;                 /* [tokens, 4] or NULL */
+    int32_t* pos;                 /* [tokens] or NULL */
+} slhip_kv_pages;
+SLHIP_API int slhip_kv_pages_advance(const slhip_kv_pages* p, slhip_stream stream);
+SLHIP_API int slhip_kv_pages_release(const slhip_kv_pages* p, slhip_stream stream);
+
+/*
+ * The cache. Codes of K: [blocks, heads, block_size, head_dim] bytes; of V: [blocks, heads, block_size / 16, head_dim, 16]
+ * bytes (the 16 tokens of a dim next to each other, as the attention's matrix products read them); one f32 scale for each
+ * block and head, [blocks, heads], for K and V apart. value = code * scale, the scale a power of two >= 2^-40:
+ * int8 codes -127 .. 127, or OCP E4M3 codes up to +-448.
+ * k and v 16-byte aligned; block_size 16, 32, 64, 128 or 256; head_dim a multiple of 16 up to 256.
+ */
+typedef enum slhip_kv8_format { SLHIP_KV8_I8 = 0, SLHIP_KV8_E4M3 = 1 } slhip_kv8_format;
+typedef struct slhip_kv8_cache {
+    int32_t format; /* slhip_kv8_format */
+    int32_t reserved;
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int64_t blocks, block_size, heads, head_dim;
+} slhip_kv8_cache;
+typedef struct slhip_kv8_batch {
+    int64_t requests; /* B */
+    int64_t tokens;   /* T: rows of the step's tensors, padding rows included */
+    const int32_t* starts; /* [B + 1] */
+    const int32_t* past;   /* [B] */
+    const int32_t* slots;  /* [B], or NULL: slot i */
+    const int32_t* pages;  /* [page_slots, blocks_per_slot] */
+    int64_t page_slots, blocks_per_slot;
+} slhip_kv8_batch;
+
+/*
+ * Writes the batch's K and V rows [T, heads, head_dim] (f32 or bf16, strides in elements, innermost 1) into the cache.
+ * For each block that the batch writes to, each head, K and V apart: a = the largest |value| of the block's new tokens and
+ * s(a) the smallest power of two >= 2^-40 with a <= 127 s (int8) or 448 s (E4M3). A block whose first token is among the
+ * new ones is begun anew: scale s(a), its other codes 0. Otherwise the scale becomes max(old, s(a)); where it grew, the
+ * codes of the block's earlier tokens are rounded to the new scale. New codes are value / scale, rounded to nearest even.
+ * Powers of two make the division exact, so the codes are the same on every implementation; a scale grows by 2 at least,
+ * so all roundings of an int8 code together stay under one step of the last scale, and E4M3 codes above their subnormal
+ * range move without loss. A non-finite new value, or one beyond 127 (448) * 2^40, makes the scale NaN (its new codes 0):
+ * the block's values are NaN until it is begun again.
+ * A block id outside the cache, or a request that does not fit the batch or the table, is skipped and reported
+ * (SLHIP_ERR_CACHE) by the next slhip_stream_sync. Requests of one batch must not write to the same block.
+ */
+SLHIP_API int slhip_kv8_write(int dtype, const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v,
+                              int64_t v_stride_t, int64_t v_stride_h, const slhip_kv8_cache* cache,
+                              const slhip_kv8_batch* batch, slhip_stream stream);
+
+/*
+ * Causal attention of the batch's query rows q [T, q_heads, head_dim] over the cache, which holds the new tokens already:
+ *   row t of request i, position p, query head h on K/V head h / (q_heads / heads), keys j <= p:
+ *   z_j = scale * (q . K_j); softcap > 0: z_j = softcap * tanh(z_j / softcap); slopes: z_j += slopes[h] * (j - p);
+ *   window > 0: only j > p - window;  y = sum_j softmax(z)_j V_j.
+ * q and y (dtype f32 or bf16, both the same; strides in elements, innermost 1) are [T, q_heads, head_dim]; y may be q.
+ * q_heads a multiple of heads, at most 64 query heads for each. A row that sees no key is 0.
+ * max_new: no request brings more rows (0: unknown); a request that does is reported (SLHIP_ERR_CACHE) and its rows are
+ * left as they were, as are those of a request that does not fit the batch or the table. A block id outside the cache is
+ * reported too, and its keys are not seen.
+ * work: workspace of work_bytes >= slhip_kv8_attention_work_bytes(...), 16-byte aligned, for the sums of key ranges that
+ * are worked on apart; calls that may overlap each need their own. It needs no initialisation and keeps nothing.
+ * Products of f32 activations are exact to 2^-22 (two f16 parts each), those of bf16 with the softmax weights in f16;
+ * sums are f32.
+ */
+typedef struct slhip_kv8_attn {
+    float scale, softcap;
+    int64_t window;
+    const float* slopes; /* [q_heads] or NULL */
+    int64_t max_new;
+} slhip_kv8_attn;
+SLHIP_API int64_t slhip_kv8_attention_work_bytes(int64_t q_heads, const slhip_kv8_cache* cache,
+                                                 const slhip_kv8_batch* batch, int64_t max_new);
+SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t q_heads, void* y,
+                                  int64_t y_stride_t, int64_t y_stride_h, const slhip_kv8_cache* cache,
+                                  const slhip_kv8_batch* batch, const slhip_kv8_attn* cfg, void* work, int64_t work_bytes,
+                                  slhip_stream stream);
 
 /*
  * Element type conversion y = cast(x) of n elements (F32, F16, BF16 in any direction); f32 -> bf16 rounds

@@ -377,7 +377,9 @@ __device__ __forceinline__ void e4m3_group_scale(float m, float& d, float& id)
 
 // ---- device side: errors raised by kernels -----------------------------------------------------------
 
-enum : uint32_t { kErrGatherIndex = 1, kErrCacheSeq = 2, kErrCachePageTable = 3, kErrCacheBlock = 4 };
+enum : uint32_t {
+    kErrGatherIndex = 1, kErrCacheSeq = 2, kErrCachePageTable = 3, kErrCacheBlock = 4, kErrKvRequest = 5, kErrKvPages = 6
+};
 
 // Records an error in the device's error record unless one is already there (the first error wins).
 __device__ __forceinline__ void raise_error(uint32_t* err, uint32_t code, uint32_t a, uint32_t b, uint32_t c,

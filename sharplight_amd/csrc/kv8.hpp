@@ -1,0 +1,86 @@
+// The 8-bit paged KV cache as its kernels take it: requests of a step, blocks, codes.
+#pragma once
+
+#include "common.hpp"
+#include "kv8_map.hpp"
+
+namespace slhip {
+
+struct Kv8Dev {
+    uint8_t *k, *v;
+    float *ks, *vs;
+    int64_t blocks;
+    int32_t shift, heads, D;  // log2(block_size)
+    int32_t B;
+    int64_t T;
+    const int32_t *starts, *past, *slots, *pages;
+    int64_t page_slots, bps;
+    uint32_t* err;
+};
+
+// Checks what the host can see of a cache and a batch (kv8_write.hip) and fills `out`.
+int make_kv8(const char* op, const slhip_kv8_cache* c, const slhip_kv8_batch* b, Kv8Dev* out);
+
+// A request of the step. n = 0 where it has no rows or does not fit (bad).
+struct Kv8Request {
+    int32_t first, n, past, slot;
+    bool bad;
+    const int32_t* table;
+};
+
+__device__ __forceinline__ Kv8Request kv8_request(const Kv8Dev& d, int32_t i)
+{
+    Kv8Request r;
+    const int32_t s0 = d.starts[i], s1 = d.starts[i + 1];
+    r.past = d.past[i];
+    r.slot = d.slots ? d.slots[i] : i;
+    r.bad = !request_fits(s0, s1, d.T, r.past, r.slot, d.page_slots, d.bps << d.shift);
+    r.first = s0;
+    r.n = r.bad ? 0 : s1 - s0;
+    r.table = d.pages + (r.bad ? 0 : r.slot * d.bps);
+    return r;
+}
+
+__device__ __forceinline__ void raise_request(const Kv8Dev& d, int32_t i, const Kv8Request& r)
+{
+    const int64_t n = static_cast<int64_t>(d.starts[i + 1]) - d.starts[i];
+    raise_error(d.err, kErrKvRequest, i, r.slot, r.past, static_cast<uint32_t>(n), static_cast<uint32_t>(static_cast<uint64_t>(n) >> 32), 0);
+}
+
+__device__ __forceinline__ void raise_block(const Kv8Dev& d, int32_t row, int32_t slot, int32_t pos, int32_t block)
+{
+    const int64_t v = block;
+    raise_error(d.err, kErrCacheBlock, row, slot, pos, static_cast<uint32_t>(v), static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32),
+                static_cast<uint32_t>(d.blocks << d.shift));
+}
+
+// item_request by a whole wave: 64 requests are looked at a step, so 4096 take two dependent loads. Wave-uniform.
+__device__ __forceinline__ int32_t kv8_find(const Kv8Dev& d, int64_t item, int64_t tile, int64_t extra)
+{
+    int32_t lo = 0, n = d.B;
+    const int lane = threadIdx.x & 63;
+    for (;;) {
+        const int32_t step = (n + 63) / 64;
+        const int32_t i = lo + lane * step;
+        const bool under = i < lo + n && item_base(d.starts[i < lo + n ? i : lo], i, tile, extra) <= item;
+        const int32_t k = __popcll(__ballot(under));
+        if (k > 0) {
+            lo += (k - 1) * step;
+            n -= (k - 1) * step;
+        }
+        if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
+        n = min(n, step);
+    }
+}
+
+template <int DT> __device__ __forceinline__ float4 load4f(const void* p, int64_t i)
+{
+    if constexpr (DT == SLHIP_F32) {
+        return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+        return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y));
+    }
+}
+
+}  // namespace slhip

@@ -1,0 +1,236 @@
+// Block tables and slot maps of a serving step, from request lengths on the device (slhip_kv_pages_advance / _release).
+//
+// Mathematics: two prefix sums over the requests -- of their new tokens (starts) and of the blocks those need (which ids
+// of the free list are theirs) -- then one write per taken block and one row per token. Nothing here moves enough bytes to
+// matter (20 a token); what a call costs is its launch and the chain load lengths -> scan -> load table -> store. So one
+// block of 1024 threads does it all in one launch, with the sums and the slots seen (a bit each, for the duplicate check)
+// in LDS, and decides over the whole step before it writes anything: all or nothing needs no second pass. From
+// kFusedTokens rows on, the rows go to a second launch over many blocks: one CU stores a row of 20 bytes about every
+// 20 cycles, which by then costs more than a launch.
+#include "common.hpp"
+#include "kv8_map.hpp"
+
+namespace slhip {
+
+constexpr int kPagesThreads = 1024;
+constexpr int kMaxRequests = 4096;
+constexpr int kMaxSlots = 131072;
+constexpr int64_t kFusedTokens = 4096;
+
+struct KvPagesArgs {
+    int32_t B;
+    const int32_t *past, *count, *slots;
+    int32_t* pages;
+    int64_t page_slots, bps;
+    int32_t shift;  // log2(block_size)
+    int32_t* free_blocks;
+    int64_t capacity;
+    const int32_t* n_free;
+    int32_t* n_free_out;
+    int64_t tokens;
+    int32_t *starts, *seq, *pos;
+    bool rows_here;
+    uint32_t* err;
+};
+
+enum : uint32_t { kBadLength = 1, kBadSlot = 2, kBadRows = 3, kBadFree = 4 };
+
+__device__ __forceinline__ int64_t blocks_of(int64_t tokens, int shift) { return (tokens + (int64_t{1} << shift) - 1) >> shift; }
+
+// Row t of the step: request i's token t - starts[i], or padding.
+__device__ __forceinline__ void write_row(const KvPagesArgs& a, int64_t t, bool there, int32_t i, int32_t start)
+{
+    int32_t slot = -1, pos = -1, block = -1;
+    if (there) {
+        slot = a.slots ? a.slots[i] : i;
+        pos = a.past[i] + static_cast<int32_t>(t - start);
+        block = a.pages[slot * a.bps + (pos >> a.shift)];
+    }
+    if (a.seq) {
+        int32_t* s = a.seq + t * 4;
+        if ((reinterpret_cast<uintptr_t>(a.seq) & 15u) == 0) {
+            *reinterpret_cast<int4*>(s) = make_int4(slot, pos, there ? i : -1, block);
+        } else {
+            s[0] = slot;
+            s[1] = pos;
+            s[2] = there ? i : -1;
+            s[3] = block;
+        }
+    }
+    if (a.pos) a.pos[t] = there ? pos : 0;
+}
+
+template <bool RELEASE>
+__global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
+{
+    __shared__ int32_t s_start[kMaxRequests + 1], s_off[kMaxRequests + 1];
+    __shared__ uint32_t s_seen[kMaxSlots / 32];
+    __shared__ int64_t s_wave[2][kPagesThreads / 64];
+    __shared__ uint32_t s_bad;  // the first bad request * 8 + what is wrong with it
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t n_free = *a.n_free;
+    for (int64_t w = tid; w < (a.page_slots + 31) / 32; w += kPagesThreads) s_seen[w] = 0;
+    if (tid == 0) s_bad = 0xFFFFFFFFu;
+    __syncthreads();
+
+    const int per = (a.B + kPagesThreads - 1) / kPagesThreads;
+    const int i0 = min(tid * per, a.B), i1 = min(i0 + per, a.B);
+    const int64_t row_tokens = a.bps << a.shift;
+    int64_t tokens = 0, blocks = 0;
+    for (int i = i0; i < i1; i++) {
+        const int64_t past = a.past[i], count = RELEASE ? 0 : a.count[i], slot = a.slots ? a.slots[i] : i;
+        uint32_t bad = 0;
+        if (slot < 0 || slot >= a.page_slots || (atomicOr(&s_seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1u)) bad = kBadSlot;
+        if (past < 0 || count < 0 || past + count > row_tokens) bad = kBadLength;
+        if (bad) {
+            atomicMin(&s_bad, static_cast<uint32_t>(i) * 8 + bad);
+        } else {
+            tokens += count;
+            blocks += RELEASE ? blocks_of(past, a.shift) : blocks_of(past + count, a.shift) - blocks_of(past, a.shift);
+        }
+    }
+    // exclusive sums over the threads: within waves, then over the waves' totals
+    int64_t st = tokens, so = blocks;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t ut = __shfl_up(st, o, 64), uo = __shfl_up(so, o, 64);
+        if (lane >= o) {
+            st += ut;
+            so += uo;
+        }
+    }
+    if (lane == 63) {
+        s_wave[0][wave] = st;
+        s_wave[1][wave] = so;
+    }
+    __syncthreads();
+    st -= tokens;
+    so -= blocks;
+    int64_t all_tokens = 0, all_blocks = 0;
+    for (int w = 0; w < kPagesThreads / 64; w++) {
+        if (w == wave) {
+            st += all_tokens;
+            so += all_blocks;
+        }
+        all_tokens += s_wave[0][w];
+        all_blocks += s_wave[1][w];
+    }
+    uint32_t bad = s_bad;
+    if (bad == 0xFFFFFFFFu) {
+        const bool room = n_free >= 0 && n_free <= a.capacity && (RELEASE ? n_free + all_blocks <= a.capacity : all_blocks <= n_free);
+        if (!RELEASE && all_tokens > a.tokens) bad = kBadRows;
+        else if (!room) bad = kBadFree;
+    }
+    const bool ok = bad == 0xFFFFFFFFu;
+    if (tid == 0) {
+        if (!ok) {
+            const int i = min(static_cast<int>(bad >> 3), a.B - 1);
+            const int64_t count = RELEASE || i < 0 ? 0 : a.count[i];
+            raise_error(a.err, kErrKvPages, max(i, 0), i < 0 ? 0 : a.slots ? a.slots[i] : i, i < 0 ? 0 : a.past[i],
+                        static_cast<uint32_t>(count), static_cast<uint32_t>(static_cast<uint64_t>(count) >> 32), bad & 7);
+        }
+        *a.n_free_out = static_cast<int32_t>(!ok ? n_free : RELEASE ? n_free + all_blocks : n_free - all_blocks);
+    }
+    if (!ok) all_tokens = all_blocks = 0;
+
+    for (int i = i0; i < i1; i++) {
+        s_start[i] = static_cast<int32_t>(st);
+        s_off[i] = static_cast<int32_t>(so);
+        if (!RELEASE) a.starts[i] = ok ? static_cast<int32_t>(st) : 0;
+        if (!ok) continue;
+        const int64_t past = a.past[i];
+        if (RELEASE) {
+            so += blocks_of(past, a.shift);
+        } else {
+            st += a.count[i];
+            so += blocks_of(past + a.count[i], a.shift) - blocks_of(past, a.shift);
+        }
+    }
+    if (!RELEASE && tid == 0) a.starts[a.B] = static_cast<int32_t>(all_tokens);
+    __syncthreads();
+
+    for (int64_t k = tid; k < all_blocks; k += kPagesThreads) {
+        const int32_t i = static_cast<int32_t>(item_request([&](int64_t r) { return s_off[r]; }, a.B, k, 1, 0));
+        const int64_t slot = a.slots ? a.slots[i] : i;
+        int32_t* row = a.pages + slot * a.bps;
+        if (RELEASE) {
+            int32_t* e = row + (k - s_off[i]);
+            a.free_blocks[n_free + k] = *e;
+            *e = -1;
+        } else {
+            row[blocks_of(a.past[i], a.shift) + (k - s_off[i])] = a.free_blocks[n_free - 1 - k];
+        }
+    }
+    if (RELEASE || !a.rows_here) return;
+    __threadfence_block();
+    __syncthreads();
+    for (int64_t t = tid; t < a.tokens; t += kPagesThreads) {
+        const bool there = t < all_tokens;
+        const int32_t i = there ? static_cast<int32_t>(item_request([&](int64_t r) { return s_start[r]; }, a.B, t, 1, 0)) : 0;
+        write_row(a, t, there, i, there ? s_start[i] : 0);
+    }
+}
+
+__global__ __launch_bounds__(256) void kv_pages_rows(KvPagesArgs a)
+{
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (t >= a.tokens) return;
+    const bool there = t < a.starts[a.B];
+    const int32_t i = there ? static_cast<int32_t>(item_request([&](int64_t r) { return a.starts[r]; }, a.B, t, 1, 0)) : 0;
+    write_row(a, t, there, i, there ? a.starts[i] : 0);
+}
+
+// Checks what the host can see of the arguments.
+static int make_args(const char* op, bool release, const slhip_kv_pages* p, KvPagesArgs* a)
+{
+    if (!p) return fail(SLHIP_ERR_INVALID, "%s: arguments are null", op);
+    if (p->requests < 0 || p->page_slots < 0 || p->blocks_per_slot < 0 || p->free_capacity < 0 || p->tokens < 0)
+        return fail(SLHIP_ERR_INVALID, "%s: negative size", op);
+    if (p->requests > kMaxRequests) return fail(SLHIP_ERR_UNSUPPORTED, "%s: more than %d requests", op, kMaxRequests);
+    if (p->page_slots > kMaxSlots) return fail(SLHIP_ERR_UNSUPPORTED, "%s: more than %d table rows", op, kMaxSlots);
+    if (p->block_size < 1 || p->block_size > (1 << 20) || (p->block_size & (p->block_size - 1)))
+        return fail(SLHIP_ERR_INVALID, "%s: block size %lld is not a power of two up to 2^20", op, static_cast<long long>(p->block_size));
+    if (p->blocks_per_slot > 0x7FFFFFFF / p->block_size)
+        return fail(SLHIP_ERR_UNSUPPORTED, "%s: table rows of 2^31 tokens or more", op);
+    if (p->tokens > 0x7FFFFFFF || p->free_capacity > 0x7FFFFFFF) return fail(SLHIP_ERR_UNSUPPORTED, "%s: 2^31 tokens or blocks or more", op);
+    if (!p->n_free || !p->n_free_out) return fail(SLHIP_ERR_INVALID, "%s: n_free and n_free_out are required", op);
+    if (p->free_capacity > 0 && !p->free_blocks) return fail(SLHIP_ERR_INVALID, "%s: the free list is null", op);
+    if (p->requests > 0 && (!p->past || !p->pages || (!release && !p->count)))
+        return fail(SLHIP_ERR_INVALID, "%s: past, count and pages are required", op);
+    if (!release && !p->starts) return fail(SLHIP_ERR_INVALID, "%s: starts is required", op);
+    int shift = 0;
+    while ((int64_t{1} << shift) < p->block_size) shift++;
+    *a = KvPagesArgs{static_cast<int32_t>(p->requests), p->past, p->count, p->slots, p->pages, p->page_slots, p->blocks_per_slot,
+                     shift, p->free_blocks, p->free_capacity, p->n_free, p->n_free_out, p->tokens, p->starts, p->seq, p->pos,
+                     false, nullptr};
+    return error_word(&a->err);
+}
+
+}  // namespace slhip
+
+using namespace slhip;
+
+extern "C" SLHIP_API int slhip_kv_pages_advance(const slhip_kv_pages* p, slhip_stream stream)
+{
+    KvPagesArgs a;
+    const int e = make_args("kv_pages_advance", false, p, &a);
+    if (e) return e;
+    const bool rows = a.tokens > 0 && (a.seq || a.pos);
+    a.rows_here = rows && a.tokens <= kFusedTokens;
+    kv_pages_tables<false><<<1, kPagesThreads, 0, to_stream(stream)>>>(a);
+    if (rows && !a.rows_here) {
+        const int s = check_launch("kv_pages_tables");
+        if (s) return s;
+        kv_pages_rows<<<dim3(static_cast<unsigned>((a.tokens + 255) / 256)), 256, 0, to_stream(stream)>>>(a);
+        return check_launch("kv_pages_rows");
+    }
+    return check_launch("kv_pages_tables");
+}
+
+extern "C" SLHIP_API int slhip_kv_pages_release(const slhip_kv_pages* p, slhip_stream stream)
+{
+    KvPagesArgs a;
+    const int e = make_args("kv_pages_release", true, p, &a);
+    if (e) return e;
+    kv_pages_tables<true><<<1, kPagesThreads, 0, to_stream(stream)>>>(a);
+    return check_launch("kv_pages_tables");
+}

@@ -132,6 +132,15 @@ static int take_device_error()
     case kErrCacheBlock:
         return fail(SLHIP_ERR_CACHE, "Block %lld of slot %d (position %d) is outside the KV cache of %u rows.", v1,
                     slot, pos, h[6]);
+    case kErrKvRequest:
+        return fail(SLHIP_ERR_CACHE, "Request %u (slot %d, %d cached tokens, %lld new) does not fit the batch's rows, its limit "
+                    "of new tokens or the block table.", h[1], slot, pos, v1);
+    case kErrKvPages: {
+        static const char* const why[] = {"", "its lengths do not fit its table row", "its slot is outside the table or named twice",
+                                          "the step has more tokens than rows", "the free list has too few blocks or too little room"};
+        return fail(SLHIP_ERR_CACHE, "Block tables: request %u (slot %d, %d cached tokens, %lld new): %s.", h[1], slot, pos, v1,
+                    why[h[6] <= 4 ? h[6] : 0]);
+    }
     default: return fail(SLHIP_ERR_HIP, "device error record holds unknown code %u", h[0]);
     }
 }

@@ -89,6 +89,39 @@ class CacheRows(ctypes.Structure):
                 ("block_size", ctypes.c_int64)]
 
 
+class KvPages(ctypes.Structure):
+    """slhip_kv_pages: a step's request lengths, the block table and free list, and the rows that the step gets."""
+    _fields_ = [("requests", ctypes.c_int64), ("past", ctypes.c_void_p), ("count", ctypes.c_void_p),
+                ("slots", ctypes.c_void_p), ("pages", ctypes.c_void_p), ("page_slots", ctypes.c_int64),
+                ("blocks_per_slot", ctypes.c_int64), ("block_size", ctypes.c_int64), ("free_blocks", ctypes.c_void_p),
+                ("free_capacity", ctypes.c_int64), ("n_free", ctypes.c_void_p), ("n_free_out", ctypes.c_void_p),
+                ("tokens", ctypes.c_int64), ("starts", ctypes.c_void_p), ("seq", ctypes.c_void_p),
+                ("pos", ctypes.c_void_p)]
+
+
+class Kv8Cache(ctypes.Structure):
+    """slhip_kv8_cache: the 8-bit paged cache's codes and scales."""
+    _fields_ = [("format", ctypes.c_int32), ("reserved", ctypes.c_int32), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("blocks", ctypes.c_int64),
+                ("block_size", ctypes.c_int64), ("heads", ctypes.c_int64), ("head_dim", ctypes.c_int64)]
+
+
+class Kv8Batch(ctypes.Structure):
+    """slhip_kv8_batch: a step's requests and their block table."""
+    _fields_ = [("requests", ctypes.c_int64), ("tokens", ctypes.c_int64), ("starts", ctypes.c_void_p),
+                ("past", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("pages", ctypes.c_void_p),
+                ("page_slots", ctypes.c_int64), ("blocks_per_slot", ctypes.c_int64)]
+
+
+class Kv8Attn(ctypes.Structure):
+    """slhip_kv8_attn: the attention's scores and bounds."""
+    _fields_ = [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("window", ctypes.c_int64),
+                ("slopes", ctypes.c_void_p), ("max_new", ctypes.c_int64)]
+
+
+KV8_FORMATS = {"i8": 0, "e4m3": 1}
+
+
 class NormCopies(ctypes.Structure):
     """slhip_norm_copies: the f16 and E4M3 GEMM activation copies a row norm writes (either may be NULL)."""
     _fields_ = [("y16", ctypes.c_void_p), ("y16_stride", ctypes.c_int64), ("yq", ctypes.c_void_p),
@@ -226,6 +259,12 @@ SIGNATURES = {
     "slhip_binary": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P]),
     "slhip_unary": (_I, [_I, _I, _I, _P, _P, _I64, _I64, _I64, _I64, _F, _F, _P]),
     "slhip_cache_write": (_I, [_I, _I, _P, _I64, _I64, _I64, _P, ctypes.POINTER(CacheRows), _P]),
+    "slhip_kv_pages_advance": (_I, [ctypes.POINTER(KvPages), _P]),
+    "slhip_kv_pages_release": (_I, [ctypes.POINTER(KvPages), _P]),
+    "slhip_kv8_write": (_I, [_I, _P, _I64, _I64, _P, _I64, _I64, ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8Batch), _P]),
+    "slhip_kv8_attention_work_bytes": (_I64, [_I64, ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8Batch), _I64]),
+    "slhip_kv8_attention": (_I, [_I, _P, _I64, _I64, _I64, _P, _I64, _I64, ctypes.POINTER(Kv8Cache),
+                                 ctypes.POINTER(Kv8Batch), ctypes.POINTER(Kv8Attn), _P, _I64, _P]),
     "slhip_provider_check": (_I, [ctypes.c_char_p, _SZ]),
     "slhip_node_supports": (_I, [ctypes.c_char_p, _I, ctypes.POINTER(_I), ctypes.c_char_p, _SZ]),
     "slhip_segment_compile": (_I, [ctypes.c_char_p, _I64, ctypes.POINTER(_P)]),
@@ -594,6 +633,61 @@ def rope(dtype_in, dtype_out, tensors, pos, T, D, *, dims=0, neox=True, base=100
 def cache_write(dtype_in, dtype_cache, x, T, inner, cache, rows: CacheRows, *, x_stride=None, stream=None):
     call("slhip_cache_write", DTYPES.get(dtype_in, dtype_in), DTYPES.get(dtype_cache, dtype_cache), ptr(x),
          inner if x_stride is None else x_stride, T, inner, ptr(cache), ctypes.byref(rows), stream)
+
+
+def kv_pages(requests, past, count, pages, page_slots, blocks_per_slot, block_size, free_blocks, free_capacity, n_free,
+             n_free_out, tokens=0, starts=None, *, seq=None, pos=None, slots=None) -> KvPages:
+    """The arguments of kv_pages_advance / kv_pages_release (int32 device arrays), to be kept with the buffers."""
+    return KvPages(requests, ptr(past), ptr(count), ptr(slots), ptr(pages), page_slots, blocks_per_slot, block_size,
+                   ptr(free_blocks), free_capacity, ptr(n_free), ptr(n_free_out), tokens, ptr(starts), ptr(seq), ptr(pos))
+
+
+def kv_pages_advance(p: KvPages, stream=None):
+    """Takes the step's blocks from the free list and writes its block table entries, starts, seq and pos."""
+    call("slhip_kv_pages_advance", ctypes.byref(p), stream)
+
+
+def kv_pages_release(p: KvPages, stream=None):
+    """Returns the blocks of requests that ended (slots, past = their lengths) to the free list."""
+    call("slhip_kv_pages_release", ctypes.byref(p), stream)
+
+
+def kv8_cache(fmt, k, v, k_scale, v_scale, blocks, block_size, heads, head_dim) -> Kv8Cache:
+    """An 8-bit cache ("i8" or "e4m3"): codes k, v (blocks * heads * block_size * head_dim bytes each) and f32 scales
+    [blocks, heads]."""
+    return Kv8Cache(KV8_FORMATS.get(fmt, fmt), 0, ptr(k), ptr(v), ptr(k_scale), ptr(v_scale), blocks, block_size, heads,
+                    head_dim)
+
+
+def kv8_batch(requests, tokens, starts, past, pages, page_slots, blocks_per_slot, *, slots=None) -> Kv8Batch:
+    """A step's requests: starts [requests + 1], past and slots [requests], the block table."""
+    return Kv8Batch(requests, tokens, ptr(starts), ptr(past), ptr(slots), ptr(pages), page_slots, blocks_per_slot)
+
+
+def kv8_write(dtype, k, v, cache: Kv8Cache, batch: Kv8Batch, *, k_stride_t=None, k_stride_h=None, v_stride_t=None,
+              v_stride_h=None, stream=None):
+    """Quantises the batch's K and V rows [tokens, heads, head_dim] (f32 / bf16) into the cache."""
+    d, row = cache.head_dim, cache.heads * cache.head_dim
+    call("slhip_kv8_write", DTYPES.get(dtype, dtype), ptr(k), row if k_stride_t is None else k_stride_t,
+         d if k_stride_h is None else k_stride_h, ptr(v), row if v_stride_t is None else v_stride_t,
+         d if v_stride_h is None else v_stride_h, ctypes.byref(cache), ctypes.byref(batch), stream)
+
+
+def kv8_attention_work_bytes(q_heads, cache: Kv8Cache, batch: Kv8Batch, max_new=0) -> int:
+    """Bytes of workspace that kv8_attention wants for such a batch."""
+    return int(lib().slhip_kv8_attention_work_bytes(q_heads, ctypes.byref(cache), ctypes.byref(batch), max_new))
+
+
+def kv8_attention(dtype, q, y, q_heads, cache: Kv8Cache, batch: Kv8Batch, *, scale, softcap=0.0, window=0, slopes=None,
+                  max_new=0, work=None, work_bytes=0, q_stride_t=None, q_stride_h=None, y_stride_t=None, y_stride_h=None,
+                  stream=None):
+    """y [tokens, q_heads, head_dim] = causal attention of q over the cache, which holds the batch's tokens already."""
+    d, row = cache.head_dim, q_heads * cache.head_dim
+    cfg = Kv8Attn(scale, softcap, window, ptr(slopes), max_new)
+    call("slhip_kv8_attention", DTYPES.get(dtype, dtype), ptr(q), row if q_stride_t is None else q_stride_t,
+         d if q_stride_h is None else q_stride_h, q_heads, ptr(y), row if y_stride_t is None else y_stride_t,
+         d if y_stride_h is None else y_stride_h, ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(cfg), ptr(work),
+         work_bytes, stream)
 
 
 def gather(fmt, table, V, D, ids, N, dtype_out, y, *, y_stride=None, stream=None):
