@@ -518,7 +518,7 @@ typedef struct slhip_kv8_batch {
  * For each block that the batch writes to, each head, K and V apart: a = the largest |value| of the block's new tokens and
  * s(a) the smallest power of two >= 2^-40 with a <= 127 s (int8) or 448 s (E4M3). A block whose first token is among the
  * new ones is begun anew: scale s(a), its other codes 0. Otherwise the scale becomes max(old, s(a)); where it grew, the
- * codes of the block's earlier tokens are rounded to the new scale. New codes are value / scale, rounded to nearest even.
+ * block's other codes are rounded to the new scale. New codes are value / scale, rounded to nearest even.
  * Powers of two make the division exact, so the codes are the same on every implementation; a scale grows by 2 at least,
  * so all roundings of an int8 code together stay under one step of the last scale, and E4M3 codes above their subnormal
  * range move without loss. A non-finite new value, or one beyond 127 (448) * 2^40, makes the scale NaN (its new codes 0):

@@ -192,7 +192,7 @@ __global__ __launch_bounds__(1024) void kv8_write(Kv8WriteArgs a)
                 *p = make_uint2(Code8<FMT>::pack(f + 8 * o, inv), Code8<FMT>::pack(f + 8 * o + 4, inv));
             } else if (fresh) {
                 *p = make_uint2(0, 0);
-            } else if (grew && q0 + t < r.past) {
+            } else if (grew) {
                 const uint2 w = *p;
                 float g[8];
                 Code8<FMT>::unpack(w.x, g);
@@ -215,8 +215,7 @@ __global__ __launch_bounds__(1024) void kv8_write(Kv8WriteArgs a)
                     if (grew) {
                         float g[4];
                         Code8<FMT>::unpack(w[j], g);
-                        const uint32_t m = byte_mask(j, 0, min(max(r.past - q0, 0), 16));
-                        w[j] = (Code8<FMT>::pack(g, shrink) & m) | (w[j] & ~m);
+                        w[j] = Code8<FMT>::pack(g, shrink);
                     }
                     const uint32_t m = byte_mask(j, na, nb);
                     w[j] = (nb > na ? Code8<FMT>::pack(f + 32 * o + 16 * e + 4 * j, inv) & m : 0) | (w[j] & ~m);

@@ -103,8 +103,7 @@ def write(cache: Cache, k, v, starts, past, slots, pages):
                     if begun:
                         old[:] = 0
                     elif s1_ > s0_:
-                        seen = slice(0, lo - j * bs)
-                        old[seen] = to_codes(tab[old[seen]] * (float(s0_) / float(s1_)), fmt)
+                        old[:] = to_codes(tab[old] * (float(s0_) / float(s1_)), fmt)
                     old[lo - j * bs:hi - j * bs] = 0 if np.isnan(s1_) else to_codes(new / float(s1_), fmt)
                     codes[block, h] = old.reshape(bs // 16, 16, cache.D).transpose(0, 2, 1) if codes.ndim == 5 else old
                     scales[block, h] = s1_

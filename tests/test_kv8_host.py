@@ -180,8 +180,8 @@ def test_write_by_hand():
     kv8_ref.write(c, k, k, [0, 2], [15], [0], pages)  # again, and the next block's first
     assert c.ks[2, 0] == 2.0 ** -5 and c.ks[0, 0] == 1.0 and c.k[0, 0, 0, 0] == 100
     k[0, 0, 0] = 200.0
-    kv8_ref.write(c, k, k, [0, 1], [1], [0], pages)  # grows: nothing but token 0 is older
-    assert c.ks[2, 0] == 2.0 and c.k[2, 0, 1, 0] == 100 and c.k[2, 0, 15, 0] == 96
+    kv8_ref.write(c, k, k, [0, 1], [1], [0], pages)  # grows by 2^6: 96 steps of before are 1.5 now, and go to 2
+    assert c.ks[2, 0] == 2.0 and c.k[2, 0, 1, 0] == 100 and c.k[2, 0, 15, 0] == 2
 
 
 def test_attention_by_hand():
