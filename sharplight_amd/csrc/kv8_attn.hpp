@@ -35,6 +35,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = 64;
 constexpr float kBias = 8.0f;  // weights are at most 2^kBias in f16
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kLeastRounds = 1;
 constexpr float kNone = -1e30f;  // a maximum of nothing: finite, so that differences with -inf stay numbers
 
 struct Kv8AttnArgs {
@@ -46,11 +47,14 @@ struct Kv8AttnArgs {
     float scale, cap;
     int32_t window;              // 0: none
     const float* slopes;
-    int32_t min_rows, max_rows;  // the launch takes requests of (min_rows, max_rows] query rows a K/V head
-    bool strict;                 // requests above max_rows are an error here (no other launch takes them)
-    int32_t units;               // wave tiles: most units a head's requests are cut into, beyond one for each
-    int32_t tile_tokens, splits; // block tiles: rows' tokens of a tile, key ranges it is cut into
-    float* part;                 // sums of key ranges
+    bool reshaped;               // scores are capped or sloped, or scale is not positive
+    int32_t min_rows, max_rows;    // few-row work: requests of (min_rows, max_rows] query rows a K/V head
+    bool strict;                   // requests above max_rows are an error (nothing else takes them)
+    int32_t block_min, block_max;  // many-row tiles: requests of (block_min, block_max] rows; above is an error
+    int32_t workers;             // few-row thread blocks
+    int32_t tile_tokens, splits; // many-row tiles: tokens of a tile, key ranges it is cut into
+    int64_t items;               // many-row tiles of a head
+    float *part, *part2;         // sums of key ranges: of workers, of splits
 };
 
 // ---- codes ----------------------------------------------------------------------------------------------------
@@ -227,45 +231,48 @@ template <int NP>
 __device__ __forceinline__ float tile_softmax(const Kv8AttnArgs& a, f32x4 (&S)[4], const Row& row, const TileScale& sc, int32_t key0,
                                               int lo, int hi, bool masked, float& m, float& l, f16x8 (&p)[NP][2])
 {
-    const float k2 = row.back * sc.k * kLog2e;
-    float mx = -INFINITY;
-    if (a.cap > 0.0f) {
-        const float in = row.back * sc.k / a.cap, out = a.cap * kLog2e;
+    // t = fma(S, mul, add). Capped or sloped scores, masked tiles and multipliers that are not positive turn S into t first.
+    float mul = row.back * sc.k * kLog2e, add = sc.ev;
+    if (masked || a.reshaped) {
+        if (a.cap > 0.0f) {
+            const float in = row.back * sc.k / a.cap, out = a.cap * kLog2e;
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+            for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) S[t][r] = fmaf(tanh_f(S[t][r] * in), out, sc.ev);
-    } else {
+                for (int r = 0; r < 4; r++) S[t][r] = fmaf(tanh_f(S[t][r] * in), out, add);
+        } else {
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+            for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) S[t][r] = fmaf(S[t][r], k2, sc.ev);
-    }
-    if (a.slopes) {
-        const float first = static_cast<float>(key0 - row.pos);
+                for (int r = 0; r < 4; r++) S[t][r] = fmaf(S[t][r], mul, add);
+        }
+        if (a.slopes) {
+            const float first = static_cast<float>(key0 - row.pos);
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+            for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) S[t][r] = fmaf(row.slope, first + static_cast<float>(4 * t + r), S[t][r]);
-    }
-    if (masked) {
+                for (int r = 0; r < 4; r++) S[t][r] = fmaf(row.slope, first + static_cast<float>(4 * t + r), S[t][r]);
+        }
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int r = 0; r < 4; r++) S[t][r] = 4 * t + r >= lo && 4 * t + r < hi ? S[t][r] : -INFINITY;
+        mul = 1.0f;
+        add = 0.0f;
     }
+    float mx = S[0][0];
 #pragma unroll
     for (int t = 0; t < 4; t++) mx = fmaxf(fmaxf(fmaxf(mx, S[t][0]), fmaxf(S[t][1], S[t][2])), S[t][3]);
     const float was = m;
-    m = fmaxf(m, row_max(mx));
-    const float shift = m - kBias;
+    m = fmaxf(m, row_max(fmaf(mx, mul, add)));
+    const float shift = add - (m - kBias);
     float sum = 0.0f;
 #pragma unroll
     for (int s = 0; s < 2; s++)
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
             const int t = 2 * s + (j >> 2), r = j & 3;
-            const float w0 = __builtin_amdgcn_exp2f(S[t][r] - shift), w1 = __builtin_amdgcn_exp2f(S[t][r + 1] - shift);
+            const float w0 = __builtin_amdgcn_exp2f(fmaf(S[t][r], mul, shift)), w1 = __builtin_amdgcn_exp2f(fmaf(S[t][r + 1], mul, shift));
             sum += w0 + w1;
             const f16x2 hi2 = to_f16x2(w0, w1);
             p[0][s][j] = hi2.x;
@@ -325,310 +332,366 @@ __device__ __forceinline__ void key_range(const Kv8AttnArgs& a, int32_t past, in
 
 // ---- few rows: a wave a key tile ---------------------------------------------------------------------------------
 
-// Which requests are cut into which key ranges, from the lengths alone, so that every thread block of a launch finds its
-// own without a launch before it: ranges of `chunk` tiles, the smallest multiple of four (a tile for each wave) that makes
-// about a.units ranges a head of all requests together, so long requests and short ones give ranges of one size.
-struct Unit {
-    int32_t request;  // -1: none
-    int32_t part;     // which of its ranges
-    int32_t parts;    // how many
-    int32_t base;     // its first slot among the partial sums (requests of one range have none)
+// The work of all requests of a launch, in rounds of four key tiles (one for each wave of a thread block), is one line --
+// request by request, head by head -- that `workers` thread blocks share out in equal pieces, whatever the lengths are. A
+// piece that begins or ends inside a head's keys leaves partial sums, of which a worker has two at most: of its first
+// segment in slot 2 w, of its last in slot 2 w + 1. Where a piece lies follows from the lengths alone, so every worker finds
+// its own without a launch before it, and the join finds the workers of a head by a division.
+struct Line {
+    int64_t each;     // rounds of a worker
+    int64_t total;    // rounds of all
+    int64_t before;   // rounds of a head of the requests before `request`
+    int32_t request;  // the request looked for
+    int32_t rounds;   // its rounds a head
 };
 
-__device__ __forceinline__ int32_t request_tiles(const Kv8AttnArgs& a, int32_t i)
+__device__ __forceinline__ int32_t request_rounds(const Kv8AttnArgs& a, const Kv8Request& r)
 {
-    const Kv8Request r = kv8_request(a.c, i);
     const int64_t rows = static_cast<int64_t>(r.n) * a.G;
     if (r.n == 0 || rows <= a.min_rows || rows > a.max_rows) return 0;
     int32_t first, end;
     key_range(a, r.past, 0, r.n, first, end);
-    return (end - first + kTile - 1) / kTile;
+    return (end - first + 4 * kTile - 1) / (4 * kTile);
 }
 
-__device__ __forceinline__ int32_t ranges_of(int32_t tiles, int32_t chunk) { return (tiles + chunk - 1) / chunk; }
-
-// Finds range `unit` of the launch's requests (FIND_REQUEST: the unit is a request, and all its ranges are asked for).
-// All 256 threads of the block call it.
-template <bool FIND_REQUEST>
-__device__ __forceinline__ Unit find_unit(const Kv8AttnArgs& a, int32_t unit, int32_t& chunk)
+// The line as one wave sees it, 64 requests a step, and on it the request of worker `at` (of request `at` itself if
+// BY_REQUEST). Wave-uniform.
+template <bool BY_REQUEST> __device__ __forceinline__ Line find_line(const Kv8AttnArgs& a, int32_t at)
 {
-    __shared__ int64_t s_tiles[4];
-    __shared__ int32_t s_ranges[4], s_parts[4];
-    __shared__ Unit s_unit;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (a.c.B + 255) / 256, i0 = min(tid * per, a.c.B), i1 = min(i0 + per, a.c.B);
-    int64_t tiles = 0;
-    int32_t kept = 0;  // of the thread's first request: most batches have one a thread
-    for (int i = i0; i < i1; i++) {
-        const int32_t n = request_tiles(a, i);
-        if (i == i0) kept = n;
-        tiles += n;
-    }
-    int64_t sum = tiles;
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) s_tiles[wave] = sum;
-    if (tid == 0) s_unit.request = -1;
-    __syncthreads();
-    sum = s_tiles[0] + s_tiles[1] + s_tiles[2] + s_tiles[3];
-    const int64_t want = (sum + a.units - 1) / a.units;
-    chunk = static_cast<int32_t>((want + 3) / 4 * 4);
-    if (chunk < 4) chunk = 4;
-    int32_t ranges = 0, parts = 0;
-    for (int i = i0; i < i1; i++) {
-        const int32_t n = ranges_of(i == i0 ? kept : request_tiles(a, i), chunk);
-        ranges += n;
-        parts += n > 1 ? n : 0;
-    }
-    int32_t before = ranges, slots = parts;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int32_t u = __shfl_up(before, o, 64), v = __shfl_up(slots, o, 64);
-        if (lane >= o) {
-            before += u;
-            slots += v;
+    const int lane = threadIdx.x & 63;
+    Line f{0, 0, 0, -1, 0};
+    int32_t kept = 0, up = 0;  // of the lane's request in the last step, and its inclusive sum
+    int64_t sum = 0;
+    const auto step = [&](int32_t i0) {
+        kept = i0 + lane < a.c.B ? request_rounds(a, kv8_request(a.c, i0 + lane)) : 0;
+        up = kept;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int32_t v = __shfl_up(up, o, 64);
+            if (lane >= o) up += v;
         }
+    };
+    for (int32_t i0 = 0; i0 < a.c.B; i0 += 64) {
+        step(i0);
+        if (BY_REQUEST && at >= i0 && at < i0 + 64) {
+            f.request = at;
+            f.rounds = __builtin_amdgcn_readlane(kept, at - i0);
+            f.before = sum + __builtin_amdgcn_readlane(up, at - i0) - f.rounds;
+        }
+        sum += __builtin_amdgcn_readlane(up, 63);
     }
-    if (lane == 63) {
-        s_ranges[wave] = before;
-        s_parts[wave] = slots;
+    f.total = sum * a.c.heads;
+    f.each = (f.total + a.workers - 1) / a.workers;
+    if (f.each < kLeastRounds) f.each = kLeastRounds;
+    if (BY_REQUEST || at * f.each >= f.total) return f;
+    sum = 0;
+    for (int32_t i0 = 0; i0 < a.c.B; i0 += 64) {
+        if (a.c.B > 64) step(i0);
+        const uint64_t under = __ballot((sum + up) * a.c.heads <= at * f.each);  // requests that end before the piece begins
+        const int k = __popcll(under);
+        if (k < 64) {
+            f.request = i0 + k;
+            f.rounds = __builtin_amdgcn_readlane(kept, k);
+            f.before = sum + __builtin_amdgcn_readlane(up, k) - f.rounds;
+            break;
+        }
+        sum += __builtin_amdgcn_readlane(up, 63);
     }
-    __syncthreads();
-    before -= ranges;
-    slots -= parts;
-    for (int w = 0; w < wave; w++) {
-        before += s_ranges[w];
-        slots += s_parts[w];
-    }
-    for (int i = i0; i < i1; i++) {
-        const int32_t n = ranges_of(i == i0 ? kept : request_tiles(a, i), chunk);
-        if (FIND_REQUEST ? i == unit : unit >= before && unit < before + n) s_unit = Unit{i, unit - before, n, slots};
-        before += n;
-        slots += n > 1 ? n : 0;
-    }
-    __syncthreads();
-    return s_unit;
+    return f;
 }
 
-// Sums of a key range, lane by lane as the kernel holds them: [n][dt][lane] of 4 dims, then [n][row] of (m, l).
+// Sums of a key range, lane by lane as the kernels hold them: [n][dt][lane] of 4 dims, then [n][row] of (m, l).
 template <int DP, int NT> struct Partial {
     static constexpr int64_t kDims = static_cast<int64_t>(NT) * (DP / 16) * 64 * 4;
     static constexpr int64_t kFloats = kDims + NT * 16 * 2;
 };
 
-template <int FMT, int DP> struct WaveTile {
-    uint4 k[4][DP / 64], v[DP / 16];
-    float ks, vs;
-    SubBlock vb;
-};
-
-// Loads a tile's codes and scales for the wave. kid, vid: the table entries of the lane's two sub-blocks.
-template <int FMT, int DP>
-__device__ __forceinline__ void load_tile(const Kv8AttnArgs& a, int32_t head, int32_t key, int32_t end, int32_t kid, int32_t vid,
-                                          WaveTile<FMT, DP>& w)
-{
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, D = a.c.D;
-    const SubBlock kb = sub_block(a.c, kid, head, key + 16 * (c >> 2), end);
-    w.vb = sub_block(a.c, vid, head, key + 16 * g, end);
-    const uint8_t* k = a.c.k + ((kb.at << a.c.shift) + kb.sub * 16 + (c & 3)) * D;
-#pragma unroll
-    for (int h = 0; h < DP / 64; h++) {
-        const int d = 64 * h + 16 * g < D ? 64 * h + 16 * g : 0;  // dims past D: any codes, q is 0 there
-#pragma unroll
-        for (int t = 0; t < 4; t++) w.k[t][h] = load_nt(k + 4 * t * D + d);
-    }
-    const uint8_t* v = a.c.v + ((w.vb.at << a.c.shift) + w.vb.sub * 16) * D + c * 16;
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; dt++) w.v[dt] = load_nt(v + (16 * dt < D ? 256 * dt : 0));
-    w.ks = a.c.ks[w.vb.at];
-    w.vs = a.c.vs[w.vb.at];
-}
+template <int DP, int NT> constexpr int waves_lds() { return (2 * NT * (DP / 16) * 64 * 4 + 4 * NT * 16 * 2) * 4; }
 
 template <int DT, int FMT, int DP, int NT>
-__global__ __launch_bounds__(256) void kv8_attn_waves(Kv8AttnArgs a)
+__device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t worker, char* lds)
 {
-    constexpr int NP = DT == SLHIP_F32 ? 2 : 1, ND = DP / 16;
-    __shared__ f32x4 s_o[2][NT * ND * 64];
-    __shared__ float s_ml[4][NT * 16][2];
-    const int lane = threadIdx.x & 63, wave = wave_id(), c = lane & 15, g = lane >> 4;
-    const int32_t head = blockIdx.x % a.c.heads;
-    int32_t chunk;
-    const Unit u = find_unit<false>(a, blockIdx.x / a.c.heads, chunk);
-    if (blockIdx.x == 0) {
+    constexpr int NP = DT == SLHIP_F32 ? 2 : 1, ND = DP / 16, NH = DP / 64;
+    f32x4* s_o = reinterpret_cast<f32x4*>(lds);                                       // [2][NT * ND * 64]
+    float2* s_ml = reinterpret_cast<float2*>(lds + 2 * NT * ND * 64 * sizeof(f32x4));  // [4][NT * 16]
+    const int lane = threadIdx.x & 63, wave = wave_id(), c = lane & 15, g = lane >> 4, D = a.c.D;
+    const Line line = find_line<false>(a, worker);
+    if (worker == 0) {
         for (int i = threadIdx.x; i < a.c.B; i += 256) {
             const Kv8Request r = kv8_request(a.c, i);
             if (r.bad || (a.strict && static_cast<int64_t>(r.n) * a.G > a.max_rows)) raise_request(a.c, i, r);
         }
     }
-    if (u.request < 0) return;
-    const Kv8Request r = kv8_request(a.c, u.request);
-    const int32_t rows = r.n * a.G;
-    f16x8 q[NT][NP][DP / 64][2];
-    Row row[NT];
-    float m[NT], l[NT];
-    f32x4 o[NT][ND];
+    if (line.request < 0) return;
+    int64_t pos = worker * line.each;
+    const int64_t stop = min(pos + line.each, line.total);
+    int32_t i = line.request, rounds = line.rounds;
+    const int64_t in = pos - line.before * a.c.heads;
+    int32_t head = static_cast<int32_t>(in / rounds), from = static_cast<int32_t>(in % rounds);
+    Kv8Request r = kv8_request(a.c, i);
+    for (bool opening = true;; opening = false) {
+        const int32_t count = static_cast<int32_t>(min(static_cast<int64_t>(rounds - from), stop - pos));
+        const int32_t rows = r.n * a.G;
+        int32_t first, end;
+        key_range(a, r.past, 0, r.n, first, end);
+        const int32_t k0 = first + (from * 4 + wave) * kTile;
+        const int32_t last = static_cast<int32_t>(min(static_cast<int64_t>(end), first + (static_cast<int64_t>(from) + count) * 4 * kTile));
+        int32_t kid = 0, vid = 0;
+        if (k0 < last) {
+            kid = block_id(a.c, r.table, k0 + 16 * (c >> 2), end);
+            vid = block_id(a.c, r.table, k0 + 16 * g, end);
+        }
+        f16x8 q[NT][NP][NH][2];
+        Row row[NT];
+        float m[NT], l[NT];
+        f32x4 o[NT][ND];
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        row[n] = load_row<DT, DP, NP>(a, r, head, 16 * n + c, 16 * n + c < rows, q[n]);
-        m[n] = kNone;
-        l[n] = 0.0f;
+        for (int n = 0; n < NT; n++) {
+            row[n] = load_row<DT, DP, NP>(a, r, head, 16 * n + c, 16 * n + c < rows, q[n]);
+            m[n] = kNone;
+            l[n] = 0.0f;
 #pragma unroll
-        for (int dt = 0; dt < ND; dt++) o[n][dt] = f32x4{0, 0, 0, 0};
-    }
-    int32_t first, end;
-    key_range(a, r.past, 0, r.n, first, end);
-    const int32_t k0 = first + (u.part * chunk + wave) * kTile;
-    const int32_t stop = min(static_cast<int64_t>(end), first + (static_cast<int64_t>(u.part) + 1) * chunk * kTile);
-    if (k0 < stop) {
-        WaveTile<FMT, DP> w;
-        int32_t kid = block_id(a.c, r.table, k0 + 16 * (c >> 2), end), vid = block_id(a.c, r.table, k0 + 16 * g, end);
-        load_tile<FMT, DP>(a, head, k0, end, kid, vid, w);
-        kid = block_id(a.c, r.table, k0 + 4 * kTile + 16 * (c >> 2), end);
-        vid = block_id(a.c, r.table, k0 + 4 * kTile + 16 * g, end);
-        for (int32_t key = k0; key < stop; key += 4 * kTile) {
-            WaveTile<FMT, DP> x = w;
-            if (key + 4 * kTile < stop) {
-                load_tile<FMT, DP>(a, head, key + 4 * kTile, end, kid, vid, w);
-                kid = block_id(a.c, r.table, key + 8 * kTile + 16 * (c >> 2), end);
-                vid = block_id(a.c, r.table, key + 8 * kTile + 16 * g, end);
-            }
-            if (x.vb.bad) raise_block(a.c, r.first, r.slot, key + 16 * g, x.vb.id);
-            f32x4 S[NT][4];
+            for (int dt = 0; dt < ND; dt++) o[n][dt] = f32x4{0, 0, 0, 0};
+        }
+        if (k0 < last) {
+            // K's codes are loaded again as soon as the first product has used them, V's after the second: each then has
+            // the other product and the softmax to arrive in, and the codes need registers once
+            uint4 k[4][NH], v[ND];
+            float ks, vs;
+            const uint8_t* vp;
+            SubBlock vb;
+            const auto aim = [&](int32_t key) {  // K's codes and the scales of the tile at `key`; where V's codes are
+                const SubBlock kb = sub_block(a.c, kid, head, key + 16 * (c >> 2), end);
+                vb = sub_block(a.c, vid, head, key + 16 * g, end);
+                const uint8_t* kp = a.c.k + ((kb.at << a.c.shift) + kb.sub * 16 + (c & 3)) * D;
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+                for (int h = 0; h < NH; h++) {
+                    const int d = 64 * h + 16 * g < D ? 64 * h + 16 * g : 0;  // dims past D: any codes, q is 0 there
 #pragma unroll
-                for (int t = 0; t < 4; t++) S[n][t] = f32x4{0, 0, 0, 0};
+                    for (int t = 0; t < 4; t++) k[t][h] = load_nt(kp + 4 * t * D + d);
+                }
+                ks = a.c.ks[vb.at];
+                vs = a.c.vs[vb.at];
+                vp = a.c.v + ((vb.at << a.c.shift) + vb.sub * 16) * D + c * 16;
+            };
+            const auto load_v = [&]() {
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+                for (int dt = 0; dt < ND; dt++) v[dt] = load_nt(vp + (16 * dt < D ? 256 * dt : 0));
+            };
+            aim(k0);
+            load_v();
+            kid = block_id(a.c, r.table, k0 + 4 * kTile + 16 * (c >> 2), end);
+            vid = block_id(a.c, r.table, k0 + 4 * kTile + 16 * g, end);
+            for (int32_t key = k0; key < last; key += 4 * kTile) {
+                f32x4 S[NT][4];
 #pragma unroll
-                for (int h = 0; h < DP / 64; h++) {
-                    f16x8 k[2];
-                    codes_f16<FMT>(x.k[t][h], k[0], k[1]);
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int t = 0; t < 4; t++) S[n][t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int h = 0; h < NH; h++) {
+                        f16x8 x[2];
+                        codes_f16<FMT>(k[t][h], x[0], x[1]);
+#pragma unroll
+                        for (int s = 0; s < 2; s++)
+#pragma unroll
+                            for (int n = 0; n < NT; n++)
+#pragma unroll
+                                for (int e = 0; e < NP; e++) S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s], q[n][e][h][s], S[n][t], 0, 0, 0);
+                    }
+                const TileScale sc = tile_scale(a.c, vb, ks, vs);
+                const int32_t keys = vb.keys;
+                if (vb.bad) raise_block(a.c, r.first, r.slot, key + 16 * g, vb.id);
+                const bool more = key + 4 * kTile < last;
+                if (more) {
+                    aim(key + 4 * kTile);
+                    kid = block_id(a.c, r.table, key + 8 * kTile + 16 * (c >> 2), end);
+                    vid = block_id(a.c, r.table, key + 8 * kTile + 16 * g, end);
+                }
+                f16x8 p[NT][NP][2];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const int k0l = key + 16 * g;
+                    const int hi = min(row[n].pos - k0l + 1, keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
+                    const bool masked = __any(hi < 16 || lo > 0);
+                    const float alpha = tile_softmax<NP>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], l[n], p[n]);
+                    if (__any(alpha != 1.0f)) {
+#pragma unroll
+                        for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
+                    }
+                }
+                // keys that are not there have weight 0, but their codes could be NaN
+                if (__any(keys < 16)) {
+#pragma unroll
+                    for (int dt = 0; dt < ND; dt++) v[dt] = first_codes(v[dt], keys);
+                }
+#pragma unroll
+                for (int dt = 0; dt < ND; dt++) {
+                    f16x8 x[2];
+                    codes_f16<FMT>(v[dt], x[0], x[1]);
 #pragma unroll
                     for (int s = 0; s < 2; s++)
 #pragma unroll
                         for (int n = 0; n < NT; n++)
 #pragma unroll
-                            for (int p = 0; p < NP; p++) S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s], q[n][p][h][s], S[n][t], 0, 0, 0);
+                            for (int e = 0; e < NP; e++) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s], p[n][e][s], o[n][dt], 0, 0, 0);
                 }
-            const TileScale sc = tile_scale(a.c, x.vb, x.ks, x.vs);
-            f16x8 p[NT][NP][2];
+                if (more) load_v();
+            }
+        }
+        // the four waves: a common maximum, then the sums of waves 2 and 3 into 0 and 1, and 1 into 0
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            l[n] = row_sum(l[n]);
+            if (g == 0) s_ml[wave * NT * 16 + 16 * n + c] = make_float2(m[n], l[n]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float top = m[n];
+            for (int w = 0; w < 4; w++) top = fmaxf(top, s_ml[w * NT * 16 + 16 * n + c].x);
+            float all = 0.0f;
+            for (int w = 0; w < 4; w++) {
+                const float2 x = s_ml[w * NT * 16 + 16 * n + c];
+                all += x.y * __builtin_amdgcn_exp2f(x.x - top);
+            }
+            const float alpha = __builtin_amdgcn_exp2f(m[n] - top);
+            m[n] = top;
+            l[n] = all;
+#pragma unroll
+            for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
+        }
+        for (int half = 2; half > 0; half >>= 1) {
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int dt = 0; dt < ND; dt++) s_o[((wave - half) * NT * ND + n * ND + dt) * 64 + lane] = o[n][dt];
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int dt = 0; dt < ND; dt++) o[n][dt] += s_o[(wave * NT * ND + n * ND + dt) * 64 + lane];
+            }
+            __syncthreads();
+        }
+        if (wave == 0) {
+            float* part = a.part + (2 * static_cast<int64_t>(worker) + (opening ? 0 : 1)) * Partial<DP, NT>::kFloats;
+            const bool whole = count == rounds;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                const int k0l = key + 16 * g;
-                const int hi = min(row[n].pos - k0l + 1, x.vb.keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
-                const bool masked = __any(hi < 16 || lo > 0);
-                const float alpha = tile_softmax<NP>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], l[n], p[n]);
-                if (__any(alpha != 1.0f)) {
+                const int32_t at = 16 * n + c;
+                if (whole) {
+                    const float inv = row_inverse(l[n]);
+                    if (at < rows) {
 #pragma unroll
-                    for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
+                        for (int dt = 0; dt < ND; dt++) store_dims<DT>(a, r, head, at, dt, o[n][dt], inv);
+                    }
+                } else {
+#pragma unroll
+                    for (int dt = 0; dt < ND; dt++) reinterpret_cast<f32x4*>(part)[(n * ND + dt) * 64 + lane] = o[n][dt];
+                    if (g == 0) reinterpret_cast<float2*>(part + Partial<DP, NT>::kDims)[at] = make_float2(m[n], l[n]);
                 }
             }
-            // keys that are not there have weight 0, but their codes could be NaN
-            if (__any(x.vb.keys < 16)) {
-#pragma unroll
-                for (int dt = 0; dt < ND; dt++) x.v[dt] = first_codes(x.v[dt], x.vb.keys);
-            }
-#pragma unroll
-            for (int dt = 0; dt < ND; dt++) {
-                f16x8 v[2];
-                codes_f16<FMT>(x.v[dt], v[0], v[1]);
-#pragma unroll
-                for (int s = 0; s < 2; s++)
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int e = 0; e < NP; e++) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[s], p[n][e][s], o[n][dt], 0, 0, 0);
-            }
         }
-    }
-    // the block's four waves: a common maximum, then the sums of waves 2 and 3 into 0 and 1, and 1 into 0
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        l[n] = row_sum(l[n]);
-        if (g == 0) {
-            s_ml[wave][16 * n + c][0] = m[n];
-            s_ml[wave][16 * n + c][1] = l[n];
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        float top = m[n];
-        for (int w = 0; w < 4; w++) top = fmaxf(top, s_ml[w][16 * n + c][0]);
-        float all = 0.0f;
-        for (int w = 0; w < 4; w++) all += s_ml[w][16 * n + c][1] * __builtin_amdgcn_exp2f(s_ml[w][16 * n + c][0] - top);
-        const float alpha = __builtin_amdgcn_exp2f(m[n] - top);
-        m[n] = top;
-        l[n] = all;
-#pragma unroll
-        for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
-    }
-    for (int step = 2; step > 0; step >>= 1) {
-        if (wave >= step && wave < 2 * step) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int dt = 0; dt < ND; dt++) s_o[wave - step][(n * ND + dt) * 64 + lane] = o[n][dt];
-        }
-        __syncthreads();
-        if (wave < step) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int dt = 0; dt < ND; dt++) o[n][dt] += s_o[wave][(n * ND + dt) * 64 + lane];
-        }
-        __syncthreads();
-    }
-    if (wave > 0) return;
-    float* part = a.part + (static_cast<int64_t>(u.base + u.part) * a.c.heads + head) * Partial<DP, NT>::kFloats;
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int32_t at = 16 * n + c;
-        if (u.parts == 1) {
-            const float inv = row_inverse(l[n]);
-            if (at < rows) {
-#pragma unroll
-                for (int dt = 0; dt < ND; dt++) store_dims<DT>(a, r, head, at, dt, o[n][dt], inv);
-            }
-        } else {
-#pragma unroll
-            for (int dt = 0; dt < ND; dt++) reinterpret_cast<f32x4*>(part)[(n * ND + dt) * 64 + lane] = o[n][dt];
-            if (g == 0) reinterpret_cast<float2*>(part + Partial<DP, NT>::kDims)[at] = make_float2(m[n], l[n]);
+        pos += count;
+        if (pos >= stop) return;
+        from = 0;
+        if (++head == a.c.heads) {
+            head = 0;
+            do {
+                r = kv8_request(a.c, ++i);  // there is one: rounds are left on the line
+                rounds = request_rounds(a, r);
+            } while (rounds == 0);
         }
     }
 }
 
-// Joins the ranges of a request's head: the common maximum, then the sums relative to it, dims shared out over the waves.
-template <int DT, int DP, int NT>
-__global__ __launch_bounds__(256) void kv8_attn_join(Kv8AttnArgs a)
+// ---- joins ----------------------------------------------------------------------------------------------------------
+
+// Joins `count` partial sums of 16 rows that lie `step` floats apart from `part` on (the first at `first`): the common
+// maximum, then the sums relative to it. The thread block's waves share out the dims, or (BY_PART) the sums of dims `dt0`,
+// which go through LDS then. put(dt, o, l) gets what the wave has of d-tile dt.
+template <int DP, int NT, bool BY_PART, class At, class Put>
+__device__ __forceinline__ void join_rows(const At& at, int32_t count, int n, int dt0, const Put& put)
 {
     constexpr int ND = DP / 16;
     const int lane = threadIdx.x & 63, wave = wave_id(), c = lane & 15;
-    const int32_t head = blockIdx.x % a.c.heads;
-    int32_t chunk;
-    const Unit u = find_unit<true>(a, blockIdx.x / a.c.heads, chunk);
-    if (u.parts <= 1) return;
-    const Kv8Request r = kv8_request(a.c, u.request);
-    const float* part = a.part + (static_cast<int64_t>(u.base) * a.c.heads + head) * Partial<DP, NT>::kFloats;
-    const int64_t step = static_cast<int64_t>(a.c.heads) * Partial<DP, NT>::kFloats;
-    for (int n = 0; n < NT; n++) {
-        if (16 * n >= r.n * a.G) break;
-        const float2* ml = reinterpret_cast<const float2*>(part + Partial<DP, NT>::kDims) + 16 * n + c;
-        float top = kNone;
-        for (int k = 0; k < u.parts; k++) top = fmaxf(top, ml[k * (step / 2)].x);
-        for (int dt = wave; dt < ND; dt += 4) {
-            f32x4 o = {0, 0, 0, 0};
-            float l = 0.0f;
-            for (int k = 0; k < u.parts; k++) {
-                const float2 v = ml[k * (step / 2)];
-                const float by = __builtin_amdgcn_exp2f(v.x - top);
-                l = fmaf(v.y, by, l);
-                const f32x4 x = reinterpret_cast<const f32x4*>(part + k * step)[(n * ND + dt) * 64 + lane];
+    const auto ml = [&](int32_t k) { return reinterpret_cast<const float2*>(at(k) + Partial<DP, NT>::kDims)[16 * n + c]; };
+    float top = kNone;
+#pragma unroll 4
+    for (int32_t k = 0; k < count; k++) top = fmaxf(top, ml(k).x);
+    for (int dt = BY_PART ? dt0 : wave; dt < (BY_PART ? dt0 + 1 : ND); dt += 4) {
+        f32x4 o = {0, 0, 0, 0};
+        float l = 0.0f;
+#pragma unroll 4
+        for (int32_t k = BY_PART ? wave : 0; k < count; k += BY_PART ? 4 : 1) {
+            const float2 v = ml(k);
+            const f32x4 x = reinterpret_cast<const f32x4*>(at(k))[(n * ND + dt) * 64 + lane];
+            const float by = __builtin_amdgcn_exp2f(v.x - top);
+            l = fmaf(v.y, by, l);
 #pragma unroll
-                for (int j = 0; j < 4; j++) o[j] = fmaf(x[j], by, o[j]);
-            }
-            if (16 * n + c < r.n * a.G) store_dims<DT>(a, r, head, 16 * n + c, dt, o, row_inverse(l));
+            for (int j = 0; j < 4; j++) o[j] = fmaf(x[j], by, o[j]);
         }
+        if constexpr (BY_PART) {
+            __shared__ f32x4 s_o[4][64];
+            __shared__ float s_l[4][64];
+            s_o[wave][lane] = o;
+            s_l[wave][lane] = l;
+            __syncthreads();
+            if (wave > 0) return;
+            o = (s_o[0][lane] + s_o[1][lane]) + (s_o[2][lane] + s_o[3][lane]);
+            l = (s_l[0][lane] + s_l[1][lane]) + (s_l[2][lane] + s_l[3][lane]);
+        }
+        put(dt, o, l);
     }
+}
+
+// The sums of a request's head over the workers that share it. index: (request, head, n[, dt]).
+template <int DT, int DP, int NT, bool BY_PART>
+__device__ __forceinline__ void join_waves(const Kv8AttnArgs& a, int64_t index)
+{
+    constexpr int ND = DP / 16;
+    const int dt0 = BY_PART ? static_cast<int>(index % ND) : 0;
+    if (BY_PART) index /= ND;
+    const int n = static_cast<int>(index % NT);
+    index /= NT;
+    const int32_t head = static_cast<int32_t>(index % a.c.heads);
+    const Line f = find_line<true>(a, static_cast<int32_t>(index / a.c.heads));
+    if (f.rounds == 0) return;
+    const int64_t from = f.before * a.c.heads + static_cast<int64_t>(head) * f.rounds;
+    const int64_t w0 = from / f.each, w1 = (from + f.rounds - 1) / f.each;
+    const Kv8Request r = kv8_request(a.c, f.request);
+    const int32_t row = 16 * n + (threadIdx.x & 15);
+    if (w0 == w1 || 16 * n >= r.n * a.G) return;
+    const int64_t slot0 = 2 * w0 + (w0 * f.each < from ? 1 : 0);
+    const auto at = [&](int32_t k) { return a.part + (k == 0 ? slot0 : 2 * (w0 + k)) * Partial<DP, NT>::kFloats; };
+    join_rows<DP, NT, BY_PART>(at, static_cast<int32_t>(w1 - w0 + 1), n, dt0, [&](int dt, const f32x4& o, float l) {
+        if (row < r.n * a.G) store_dims<DT>(a, r, head, row, dt, o, row_inverse(l));
+    });
+}
+
+// The sums of a row tile over its splits. index: (tile from the last, head, n).
+template <int DT, int DP, int NT> __device__ __forceinline__ void join_blocks(const Kv8AttnArgs& a, int64_t index)
+{
+    const int n = static_cast<int>(index % NT);
+    index /= NT;
+    const int32_t head = static_cast<int32_t>(index % a.c.heads);
+    const int64_t back = index / a.c.heads, item = a.items - 1 - back;
+    const int32_t i = kv8_find(a.c, item, a.tile_tokens, 1);
+    const Kv8Request r = kv8_request(a.c, i);
+    const int64_t t0 = (item - item_base(a.c.starts[i], i, a.tile_tokens, 1)) * a.tile_tokens;
+    if (t0 < 0 || t0 >= r.n || static_cast<int64_t>(r.n) * a.G <= a.block_min || static_cast<int64_t>(r.n) * a.G > a.block_max) return;
+    const int32_t row0 = static_cast<int32_t>(t0) * a.G, row1 = static_cast<int32_t>(min(static_cast<int64_t>(r.n), t0 + a.tile_tokens)) * a.G;
+    if (row0 + 16 * n >= row1) return;
+    const int32_t row = row0 + 16 * n + (threadIdx.x & 15);
+    const auto at = [&](int32_t k) { return a.part2 + ((back * a.splits + k) * a.c.heads + head) * Partial<DP, NT>::kFloats; };
+    join_rows<DP, NT, false>(at, a.splits, n, 0, [&](int dt, const f32x4& o, float l) {
+        if (row < row1) store_dims<DT>(a, r, head, row, dt, o, row_inverse(l));
+    });
 }
 
 // ---- many rows: a thread block a tile of rows -----------------------------------------------------------------------
@@ -640,24 +703,26 @@ template <int DP> struct BlockTile {
     static constexpr int kK = 4 * (DP / 32), kV = (DP / 16) * 2;  // fragments of K: t, h, s; of V: dt, s
 };
 
+template <int DP> constexpr int blocks_lds() { return 2 * (BlockTile<DP>::kK + BlockTile<DP>::kV) * 64 * static_cast<int>(sizeof(f16x8)); }
+
 template <int DT, int FMT, int DP, int NT>
-__global__ __launch_bounds__(256) void kv8_attn_blocks(Kv8AttnArgs a)
+__device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t index, char* lds)
 {
     constexpr int NP = DT == SLHIP_F32 ? 2 : 1, ND = DP / 16, NH = DP / 64;
     constexpr int kK = BlockTile<DP>::kK, kV = BlockTile<DP>::kV;
-    extern __shared__ f16x8 s_frag[];  // [2][kK + kV][64]
+    f16x8* s_frag = reinterpret_cast<f16x8*>(lds);  // [2][kK + kV][64]
     const int lane = threadIdx.x & 63, wave = wave_id(), c = lane & 15, g = lane >> 4, D = a.c.D;
-    const int32_t head = blockIdx.x % a.c.heads;
-    const int64_t rest = blockIdx.x / a.c.heads;
+    const int32_t head = static_cast<int32_t>(index % a.c.heads);
+    const int64_t rest = index / a.c.heads;
     const int32_t split = static_cast<int32_t>(rest % a.splits);
     // tiles from the last: their key ranges are the longest, and short ones fill the end
-    const int64_t item = item_count(a.c.T, a.c.B, a.tile_tokens, 1) - 1 - rest / a.splits;
+    const int64_t item = a.items - 1 - rest / a.splits;
     const int32_t i = kv8_find(a.c, item, a.tile_tokens, 1);
     const Kv8Request r = kv8_request(a.c, i);
     const int64_t t0 = (item - item_base(a.c.starts[i], i, a.tile_tokens, 1)) * a.tile_tokens;
     if (r.bad && t0 == 0 && head == 0 && split == 0 && threadIdx.x == 0) raise_request(a.c, i, r);
-    if (t0 < 0 || t0 >= r.n || static_cast<int64_t>(r.n) * a.G <= a.min_rows) return;
-    if (a.strict && static_cast<int64_t>(r.n) * a.G > a.max_rows) {
+    if (t0 < 0 || t0 >= r.n || static_cast<int64_t>(r.n) * a.G <= a.block_min) return;
+    if (static_cast<int64_t>(r.n) * a.G > a.block_max) {
         if (t0 == 0 && head == 0 && split == 0 && threadIdx.x == 0) raise_request(a.c, i, r);
         return;
     }
@@ -796,7 +861,7 @@ __global__ __launch_bounds__(256) void kv8_attn_blocks(Kv8AttnArgs a)
         buf ^= 1;
         if (more) stage(buf);
     }
-    float* part = a.part + blockIdx.x * Partial<DP, 4 * NT>::kFloats;
+    float* part = a.part2 + index * Partial<DP, 4 * NT>::kFloats;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int32_t at = (wave * NT + n) * 16 + c;
@@ -815,89 +880,69 @@ __global__ __launch_bounds__(256) void kv8_attn_blocks(Kv8AttnArgs a)
     }
 }
 
-// Joins the splits of a row tile; a thread block joins 16 rows, dims shared out over its waves.
-template <int DT, int DP, int NT>
-__global__ __launch_bounds__(256) void kv8_attn_blocks_join(Kv8AttnArgs a)
-{
-    constexpr int ND = DP / 16;
-    const int lane = threadIdx.x & 63, wave = wave_id(), c = lane & 15;
-    const int32_t head = blockIdx.x % a.c.heads, n = blockIdx.y;
-    const int64_t back = blockIdx.x / a.c.heads, item = item_count(a.c.T, a.c.B, a.tile_tokens, 1) - 1 - back;
-    const int32_t i = kv8_find(a.c, item, a.tile_tokens, 1);
-    const Kv8Request r = kv8_request(a.c, i);
-    const int64_t t0 = (item - item_base(a.c.starts[i], i, a.tile_tokens, 1)) * a.tile_tokens;
-    if (t0 < 0 || t0 >= r.n || static_cast<int64_t>(r.n) * a.G <= a.min_rows) return;
-    if (a.strict && static_cast<int64_t>(r.n) * a.G > a.max_rows) return;
-    const int32_t t1 = min(static_cast<int64_t>(r.n), t0 + a.tile_tokens);
-    const int32_t row0 = static_cast<int32_t>(t0) * a.G, row1 = t1 * a.G;
-    const float* part = a.part + (back * a.splits * a.c.heads + head) * Partial<DP, 4 * NT>::kFloats;
-    const int64_t step = static_cast<int64_t>(a.c.heads) * Partial<DP, 4 * NT>::kFloats;
-    const float2* ml = reinterpret_cast<const float2*>(part + Partial<DP, 4 * NT>::kDims) + 16 * n + c;
-    if (row0 + 16 * n >= row1) return;
-    float top = kNone;
-    for (int k = 0; k < a.splits; k++) top = fmaxf(top, ml[k * (step / 2)].x);
-    for (int dt = wave; dt < ND; dt += 4) {
-        f32x4 o = {0, 0, 0, 0};
-        float l = 0.0f;
-        for (int k = 0; k < a.splits; k++) {
-            const float2 v = ml[k * (step / 2)];
-            const float by = __builtin_amdgcn_exp2f(v.x - top);
-            l = fmaf(v.y, by, l);
-            const f32x4 x = reinterpret_cast<const f32x4*>(part + k * step)[(n * ND + dt) * 64 + lane];
-#pragma unroll
-            for (int j = 0; j < 4; j++) o[j] = fmaf(x[j], by, o[j]);
-        }
-        if (row0 + 16 * n + c < row1) store_dims<DT>(a, r, head, row0 + 16 * n + c, dt, o, row_inverse(l));
-    }
-}
-
 // ---- launches -----------------------------------------------------------------------------------------------------
 
 // What a call launches, from what the host knows.
 struct Kv8AttnPlan {
-    int32_t wave_rows;    // 0: no few-row launch, else 16 or 32
-    bool blocks;          // the many-row launch
-    int32_t block_rows;   // its rows a tile
-    int64_t wave_grid, block_items, work_bytes;
-    int32_t units, splits, tile_tokens;
+    int32_t wave_tiles;  // few-row launch: 0 none, else matrix tiles of 16 rows (1, 2)
+    bool blocks;         // many-row tiles
+    bool by_part;        // the few-row join shares out the sums of a head, not its dims
 };
+
+// Thread blocks of the few-row work, then of the many-row tiles: one launch, so that neither waits for the other's end.
+template <int DT, int FMT, int DP, int NT, int NB>
+__global__ __launch_bounds__(256, DP == 256 || NT == 2 ? 1 : 2) void kv8_attn(Kv8AttnArgs a)
+{
+    extern __shared__ __align__(16) char lds[];
+    if constexpr (NT > 0 && NB > 0) {
+        if (blockIdx.x < static_cast<unsigned>(a.workers)) attn_waves<DT, FMT, DP, NT>(a, blockIdx.x, lds);
+        else attn_blocks<DT, FMT, DP, NB>(a, blockIdx.x - a.workers, lds);
+    } else if constexpr (NT > 0) {
+        attn_waves<DT, FMT, DP, NT>(a, blockIdx.x, lds);
+    } else {
+        attn_blocks<DT, FMT, DP, NB>(a, blockIdx.x, lds);
+    }
+}
+
+template <int DT, int DP, int NT, int NB, bool BY_PART>
+__global__ __launch_bounds__(256) void kv8_attn_join(Kv8AttnArgs a, int64_t wave_joins)
+{
+    if (blockIdx.x < wave_joins) join_waves<DT, DP, NT, BY_PART>(a, blockIdx.x);
+    else join_blocks<DT, DP, 4 * NB>(a, blockIdx.x - wave_joins);
+}
 
 template <int DT, int FMT> int kv8_attn_launch(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st);
 
-template <int DT, int FMT, int DP> static int kv8_attn_run(const Kv8AttnArgs& args, const Kv8AttnPlan& p, hipStream_t st)
+template <int DT, int FMT, int DP, int NT, int NB> static int kv8_attn_start(const Kv8AttnArgs& a, hipStream_t st)
 {
-    Kv8AttnArgs a = args;
-    if (p.wave_rows) {
-        a.min_rows = 0;
-        a.max_rows = p.blocks ? p.wave_rows : args.max_rows;
-        a.strict = !p.blocks;
-        a.units = p.units;
-        const unsigned grid = static_cast<unsigned>(p.wave_grid), joins = static_cast<unsigned>(a.c.B) * a.c.heads;
-        constexpr int NT2 = DP <= 128 ? 2 : 1;  // 32 rows (make_plan asks for them up to 128 dims)
-        if (p.wave_rows == 16) kv8_attn_waves<DT, FMT, DP, 1><<<grid, 256, 0, st>>>(a);
-        else kv8_attn_waves<DT, FMT, DP, NT2><<<grid, 256, 0, st>>>(a);
-        const int e = check_launch("kv8_attn_waves");
-        if (e) return e;
-        if (p.wave_rows == 16) kv8_attn_join<DT, DP, 1><<<joins, 256, 0, st>>>(a);
-        else kv8_attn_join<DT, DP, NT2><<<joins, 256, 0, st>>>(a);
-        const int s = check_launch("kv8_attn_join");
-        if (s) return s;
-    }
-    if (!p.blocks) return SLHIP_OK;
-    constexpr int NT = DT == SLHIP_F32 || DP == 256 ? 1 : 2;
-    a.min_rows = p.wave_rows;
-    a.max_rows = args.max_rows;
-    a.strict = args.strict;
-    a.tile_tokens = p.tile_tokens;
-    a.splits = p.splits;
-    const unsigned lds = 2 * (BlockTile<DP>::kK + BlockTile<DP>::kV) * 64 * sizeof(f16x8);
-    const auto kernel = kv8_attn_blocks<DT, FMT, DP, NT>;
+    constexpr int waves = NT > 0 ? waves_lds<DP, NT ? NT : 1>() : 0, blocks = NB > 0 ? blocks_lds<DP>() : 0, lds = waves > blocks ? waves : blocks;
+    const auto kernel = kv8_attn<DT, FMT, DP, NT, NB>;
     if (lds > 65536) SLHIP_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    kernel<<<static_cast<unsigned>(p.block_items * p.splits * a.c.heads), 256, lds, st>>>(a);
-    const int s = check_launch("kv8_attn_blocks");
-    if (s || p.splits == 1) return s;
-    kv8_attn_blocks_join<DT, DP, NT><<<dim3(static_cast<unsigned>(p.block_items * a.c.heads), 4 * NT), 256, 0, st>>>(a);
-    return check_launch("kv8_attn_blocks_join");
+    const int64_t grid = (NT > 0 ? a.workers : 0) + (NB > 0 ? a.items * a.splits * a.c.heads : 0);
+    kernel<<<static_cast<unsigned>(grid), 256, lds, st>>>(a);
+    return check_launch("kv8_attn");
+}
+
+template <int DT, int FMT, int DP> static int kv8_attn_run(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
+{
+    constexpr int NB = DT == SLHIP_F32 || DP == 256 ? 1 : 2, NT2 = DP <= 128 ? 2 : 1;  // make_plan asks for two tiles up to 128 dims
+    int e;
+    if (p.blocks) e = p.wave_tiles ? kv8_attn_start<DT, FMT, DP, 1, NB>(a, st) : kv8_attn_start<DT, FMT, DP, 0, NB>(a, st);
+    else e = p.wave_tiles == 1 ? kv8_attn_start<DT, FMT, DP, 1, 0>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0>(a, st);
+    if (e) return e;
+    const int64_t waves = p.wave_tiles ? static_cast<int64_t>(a.c.B) * a.c.heads * p.wave_tiles * (p.by_part ? DP / 16 : 1) : 0;
+    const int64_t blocks = p.blocks && a.splits > 1 ? a.items * a.c.heads * 4 * NB : 0;
+    if (waves + blocks == 0) return SLHIP_OK;
+    if (waves + blocks > 0x7FFFFFFF) return fail(SLHIP_ERR_UNSUPPORTED, "kv8_attention: too many tiles");
+    const unsigned grid = static_cast<unsigned>(waves + blocks);
+    if (p.wave_tiles == 2) {
+        if (p.by_part) kv8_attn_join<DT, DP, NT2, NB, true><<<grid, 256, 0, st>>>(a, waves);
+        else kv8_attn_join<DT, DP, NT2, NB, false><<<grid, 256, 0, st>>>(a, waves);
+    } else {
+        if (p.by_part) kv8_attn_join<DT, DP, 1, NB, true><<<grid, 256, 0, st>>>(a, waves);
+        else kv8_attn_join<DT, DP, 1, NB, false><<<grid, 256, 0, st>>>(a, waves);
+    }
+    return check_launch("kv8_attn_join");
 }
 
 template <int DT, int FMT> int kv8_attn_by_dim(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
