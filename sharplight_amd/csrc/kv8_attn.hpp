@@ -123,7 +123,7 @@ struct SubBlock {
     int32_t id;
 };
 
-// The table entry of the sub-block at `key` (any address in the table where the key is behind `end`).
+// The table entry of the sub-block at `key` (another of the request's where the key is behind `end`).
 __device__ __forceinline__ int32_t block_id(const Kv8Dev& c, const int32_t* table, int32_t key, int32_t end)
 {
     return table[min(key, end - 1) >> c.shift];
@@ -135,7 +135,7 @@ __device__ __forceinline__ SubBlock sub_block(const Kv8Dev& c, int32_t id, int32
     const bool here = key < end, fine = id >= 0 && id < c.blocks;
     s.id = id;
     s.bad = here && !fine;
-    s.at = static_cast<int64_t>(fine ? id : 0) * c.heads + head;
+    s.at = static_cast<int64_t>(here && fine ? id : 0) * c.heads + head;
     s.sub = (key >> 4) & ((1 << (c.shift - 4)) - 1);
     s.keys = here && fine ? min(end - key, 16) : 0;
     return s;
@@ -437,8 +437,8 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
         const int32_t last = static_cast<int32_t>(min(static_cast<int64_t>(end), first + (static_cast<int64_t>(from) + count) * 4 * kTile));
         int32_t kid = 0, vid = 0;
         if (k0 < last) {
-            kid = block_id(a.c, r.table, k0 + 16 * (c >> 2), end);
-            vid = block_id(a.c, r.table, k0 + 16 * g, end);
+            kid = block_id(a.c, r.table, k0 + 16 * (c >> 2), last);
+            vid = block_id(a.c, r.table, k0 + 16 * g, last);
         }
         f16x8 q[NT][NP][NH][2];
         Row row[NT];
@@ -459,19 +459,22 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
             float ks, vs;
             const uint8_t* vp;
             SubBlock vb;
+            // Past the piece's last tile the loads go on, from block 0 (they are in its XCD's L2 after the first one): a branch
+            // around them would leave the compiler waiting for all of them where its paths meet.
             const auto aim = [&](int32_t key) {  // K's codes and the scales of the tile at `key`; where V's codes are
-                const SubBlock kb = sub_block(a.c, kid, head, key + 16 * (c >> 2), end);
-                vb = sub_block(a.c, vid, head, key + 16 * g, end);
+                const SubBlock kb = sub_block(a.c, kid, head, key + 16 * (c >> 2), last);
+                vb = sub_block(a.c, vid, head, key + 16 * g, last);
                 const uint8_t* kp = a.c.k + ((kb.at << a.c.shift) + kb.sub * 16 + (c & 3)) * D;
 #pragma unroll
-                for (int h = 0; h < NH; h++) {
-                    const int d = 64 * h + 16 * g < D ? 64 * h + 16 * g : 0;  // dims past D: any codes, q is 0 there
+                for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int t = 0; t < 4; t++) k[t][h] = load_nt(kp + 4 * t * D + d);
-                }
+                    for (int h = 0; h < NH; h++)  // dims past D: any codes, q is 0 there
+                        k[t][h] = *reinterpret_cast<const uint4*>(kp + 4 * t * D + (64 * h + 16 * g < D ? 64 * h + 16 * g : 0));
                 ks = a.c.ks[vb.at];
                 vs = a.c.vs[vb.at];
                 vp = a.c.v + ((vb.at << a.c.shift) + vb.sub * 16) * D + c * 16;
+                kid = block_id(a.c, r.table, key + 4 * kTile + 16 * (c >> 2), last);
+                vid = block_id(a.c, r.table, key + 4 * kTile + 16 * g, last);
             };
             const auto load_v = [&]() {
 #pragma unroll
@@ -479,8 +482,6 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
             };
             aim(k0);
             load_v();
-            kid = block_id(a.c, r.table, k0 + 4 * kTile + 16 * (c >> 2), end);
-            vid = block_id(a.c, r.table, k0 + 4 * kTile + 16 * g, end);
             for (int32_t key = k0; key < last; key += 4 * kTile) {
                 f32x4 S[NT][4];
 #pragma unroll
@@ -500,15 +501,14 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
 #pragma unroll
                                 for (int e = 0; e < NP; e++) S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s], q[n][e][h][s], S[n][t], 0, 0, 0);
                     }
-                const TileScale sc = tile_scale(a.c, vb, ks, vs);
+                TileScale sc = tile_scale(a.c, vb, ks, vs);
                 const int32_t keys = vb.keys;
                 if (vb.bad) raise_block(a.c, r.first, r.slot, key + 16 * g, vb.id);
-                const bool more = key + 4 * kTile < last;
-                if (more) {
-                    aim(key + 4 * kTile);
-                    kid = block_id(a.c, r.table, key + 8 * kTile + 16 * (c >> 2), end);
-                    vid = block_id(a.c, r.table, key + 8 * kTile + 16 * g, end);
-                }
+                // registers of their own, or the next scales' arrival is waited for to move them
+                asm volatile("" : "+v"(sc.k), "+v"(sc.ev), "+v"(sc.down));
+                __builtin_amdgcn_sched_barrier(0);
+                aim(key + 4 * kTile);
+                __builtin_amdgcn_sched_barrier(0);
                 f16x8 p[NT][NP][2];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
@@ -537,7 +537,8 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
 #pragma unroll
                             for (int e = 0; e < NP; e++) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s], p[n][e][s], o[n][dt], 0, 0, 0);
                 }
-                if (more) load_v();
+                __builtin_amdgcn_sched_barrier(0);
+                load_v();
             }
         }
         // the four waves: a common maximum, then the sums of waves 2 and 3 into 0 and 1, and 1 into 0
