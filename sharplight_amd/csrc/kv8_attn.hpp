@@ -24,6 +24,8 @@
 // The dims of the first product are taken in the order of the lanes' 16-byte loads (dim 64h + 16g + 8s + j at step h, s).
 #pragma once
 
+#include <type_traits>
+
 #include "kv8.hpp"
 
 namespace slhip {
@@ -150,34 +152,51 @@ struct Row {
     float slope;  // slopes[h] * log2(e)
 };
 
-// Loads NP f16 parts of the row's lane share: q[p][h][s] holds dims 64h + 16g + 8s + (0..7). Dims past D are 0.
-template <int DT, int DP, int NP>
-__device__ __forceinline__ Row load_row(const Kv8AttnArgs& a, const Kv8Request& r, int32_t head, int32_t row, bool valid,
-                                        f16x8 (&q)[NP][DP / 64][2])
+// The lane's share of a row as it lies in memory: dims 64h + 16g + (0..15) of step h.
+template <int DT, int DP> struct RawRow {
+    static constexpr int kVecs = DT == SLHIP_F32 ? 4 : 2;
+    uint4 w[DP / 64][kVecs];
+};
+
+template <int DT, int DP>
+__device__ __forceinline__ void fetch_row(const Kv8AttnArgs& a, const Kv8Request& r, int32_t head, int32_t row, bool valid, RawRow<DT, DP>& raw)
 {
+    constexpr int kVecs = RawRow<DT, DP>::kVecs, per = Vec<DT>::N;
     const int g = (threadIdx.x & 63) >> 4;
-    const int32_t tok = valid ? row / a.G : 0, qh = head * a.G + (valid ? row % a.G : 0);
-    const int64_t base = (static_cast<int64_t>(r.first) + tok) * a.qt + qh * a.qh;
-    const bool vec = reinterpret_cast<uintptr_t>(a.q) % (DT == SLHIP_F32 ? 16 : 8) == 0 && (a.qt | a.qh) % 4 == 0;
-    float f[DP / 64][16];
-    uint32_t top = 0;
+    const int64_t base = (static_cast<int64_t>(r.first) + row / a.G) * a.qt + (head * a.G + row % a.G) * a.qh;
+    const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.qt | a.qh) % per == 0;
 #pragma unroll
     for (int h = 0; h < DP / 64; h++) {
         const int d = 64 * h + 16 * g;
         const bool in = valid && d < a.c.D;
 #pragma unroll
-        for (int j = 0; j < 16; j += 4) {
-            float4 w = make_float4(0, 0, 0, 0);
-            if (in) {
-                if (vec) {
-                    w = load4f<DT>(a.q, base + d + j);
-                } else {
-                    w = make_float4(Vec<DT>::load1(a.q, base + d + j), Vec<DT>::load1(a.q, base + d + j + 1),
-                                    Vec<DT>::load1(a.q, base + d + j + 2), Vec<DT>::load1(a.q, base + d + j + 3));
-                }
+        for (int i = 0; i < kVecs; i++) {
+            raw.w[h][i] = make_uint4(0, 0, 0, 0);
+            const int64_t at = base + d + i * per;
+            if (in && vec) {
+                raw.w[h][i] = *reinterpret_cast<const uint4*>(static_cast<const char*>(a.q) + at * Vec<DT>::BYTES);
+            } else if (in) {
+                float f[per];
+                for (int j = 0; j < per; j++) f[j] = Vec<DT>::load1(a.q, at + j);
+                raw.w[h][i] = Vec<DT>::pack(f);  // the same bits again
             }
-            f[h][j] = w.x; f[h][j + 1] = w.y; f[h][j + 2] = w.z; f[h][j + 3] = w.w;
         }
+    }
+}
+
+// NP f16 parts of the row's lane share: q[p][h][s] holds dims 64h + 16g + 8s + (0..7). Dims past D are 0.
+template <int DT, int DP, int NP>
+__device__ __forceinline__ Row make_row(const Kv8AttnArgs& a, const Kv8Request& r, int32_t head, int32_t row, bool valid,
+                                        const RawRow<DT, DP>& raw, f16x8 (&q)[NP][DP / 64][2])
+{
+    constexpr int kVecs = RawRow<DT, DP>::kVecs, per = Vec<DT>::N;
+    const int32_t tok = valid ? row / a.G : 0, qh = head * a.G + (valid ? row % a.G : 0);
+    float f[DP / 64][16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int h = 0; h < DP / 64; h++) {
+#pragma unroll
+        for (int i = 0; i < kVecs; i++) Vec<DT>::unpack(raw.w[h][i], &f[h][i * per]);
 #pragma unroll
         for (int j = 0; j < 16; j++) top = max(top, __float_as_uint(f[h][j]) & 0x7FFFFFFFu);
     }
@@ -343,7 +362,15 @@ struct Line {
     int64_t before;   // rounds of a head of the requests before `request`
     int32_t request;  // the request looked for
     int32_t rounds;   // its rounds a head
+    Kv8Request r;
 };
+
+// Quotients of numbers that fit 32 bits in all but the longest batches.
+__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d)
+{
+    if (((n | d) >> 32) == 0) return static_cast<uint32_t>(n) / static_cast<uint32_t>(d);
+    return n / d;
+}
 
 __device__ __forceinline__ int32_t request_rounds(const Kv8AttnArgs& a, const Kv8Request& r)
 {
@@ -359,28 +386,38 @@ __device__ __forceinline__ int32_t request_rounds(const Kv8AttnArgs& a, const Kv
 template <bool BY_REQUEST> __device__ __forceinline__ Line find_line(const Kv8AttnArgs& a, int32_t at)
 {
     const int lane = threadIdx.x & 63;
-    Line f{0, 0, 0, -1, 0};
-    int32_t kept = 0, up = 0;  // of the lane's request in the last step, and its inclusive sum
+    Line f{0, 0, 0, -1, 0, {}};
+    Kv8Request mine{};         // the lane's request in the last step
+    int32_t kept = 0, up = 0;  // its rounds, and their inclusive sum
     int64_t sum = 0;
     const auto step = [&](int32_t i0) {
-        kept = i0 + lane < a.c.B ? request_rounds(a, kv8_request(a.c, i0 + lane)) : 0;
+        const bool there = i0 + lane < a.c.B;
+        mine = kv8_request(a.c, there ? i0 + lane : 0);
+        kept = there ? request_rounds(a, mine) : 0;
         up = kept;
         for (int o = 1; o < 64; o <<= 1) {
             const int32_t v = __shfl_up(up, o, 64);
             if (lane >= o) up += v;
         }
     };
+    const auto take = [&](int32_t i0, int k) {
+        f.request = i0 + k;
+        f.rounds = __builtin_amdgcn_readlane(kept, k);
+        f.before = sum + __builtin_amdgcn_readlane(up, k) - f.rounds;
+        f.r.first = __builtin_amdgcn_readlane(mine.first, k);
+        f.r.n = __builtin_amdgcn_readlane(mine.n, k);
+        f.r.past = __builtin_amdgcn_readlane(mine.past, k);
+        f.r.slot = __builtin_amdgcn_readlane(mine.slot, k);
+        f.r.bad = f.r.n == 0;
+        f.r.table = a.c.pages + (f.r.bad ? 0 : f.r.slot * a.c.bps);
+    };
     for (int32_t i0 = 0; i0 < a.c.B; i0 += 64) {
         step(i0);
-        if (BY_REQUEST && at >= i0 && at < i0 + 64) {
-            f.request = at;
-            f.rounds = __builtin_amdgcn_readlane(kept, at - i0);
-            f.before = sum + __builtin_amdgcn_readlane(up, at - i0) - f.rounds;
-        }
+        if (BY_REQUEST && at >= i0 && at < i0 + 64) take(i0, at - i0);
         sum += __builtin_amdgcn_readlane(up, 63);
     }
     f.total = sum * a.c.heads;
-    f.each = (f.total + a.workers - 1) / a.workers;
+    f.each = quotient(f.total + a.workers - 1, a.workers);
     if (f.each < kLeastRounds) f.each = kLeastRounds;
     if (BY_REQUEST || at * f.each >= f.total) return f;
     sum = 0;
@@ -389,9 +426,7 @@ template <bool BY_REQUEST> __device__ __forceinline__ Line find_line(const Kv8At
         const uint64_t under = __ballot((sum + up) * a.c.heads <= at * f.each);  // requests that end before the piece begins
         const int k = __popcll(under);
         if (k < 64) {
-            f.request = i0 + k;
-            f.rounds = __builtin_amdgcn_readlane(kept, k);
-            f.before = sum + __builtin_amdgcn_readlane(up, k) - f.rounds;
+            take(i0, k);
             break;
         }
         sum += __builtin_amdgcn_readlane(up, 63);
@@ -415,7 +450,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
     float2* s_ml = reinterpret_cast<float2*>(lds + 2 * NT * ND * 64 * sizeof(f32x4));  // [4][NT * 16]
     const int lane = threadIdx.x & 63, wave = wave_id(), c = lane & 15, g = lane >> 4, D = a.c.D;
     const Line line = find_line<false>(a, worker);
-    if (worker == 0) {
+    if (worker == a.workers - 1) {  // the one with the least to do
         for (int i = threadIdx.x; i < a.c.B; i += 256) {
             const Kv8Request r = kv8_request(a.c, i);
             if (r.bad || (a.strict && static_cast<int64_t>(r.n) * a.G > a.max_rows)) raise_request(a.c, i, r);
@@ -426,8 +461,8 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
     const int64_t stop = min(pos + line.each, line.total);
     int32_t i = line.request, rounds = line.rounds;
     const int64_t in = pos - line.before * a.c.heads;
-    int32_t head = static_cast<int32_t>(in / rounds), from = static_cast<int32_t>(in % rounds);
-    Kv8Request r = kv8_request(a.c, i);
+    int32_t head = static_cast<int32_t>(quotient(in, rounds)), from = static_cast<int32_t>(in - static_cast<int64_t>(head) * rounds);
+    Kv8Request r = line.r;
     for (bool opening = true;; opening = false) {
         const int32_t count = static_cast<int32_t>(min(static_cast<int64_t>(rounds - from), stop - pos));
         const int32_t rows = r.n * a.G;
@@ -437,8 +472,40 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
         const int32_t last = static_cast<int32_t>(min(static_cast<int64_t>(end), first + (static_cast<int64_t>(from) + count) * 4 * kTile));
         int32_t kid = 0, vid = 0;
         if (k0 < last) {
-            kid = block_id(a.c, r.table, k0 + 16 * (c >> 2), last);
-            vid = block_id(a.c, r.table, k0 + 16 * g, last);
+            kid = block_id(a.c, r.table, k0 + 16 * (c >> 2), end);
+            vid = block_id(a.c, r.table, k0 + 16 * g, end);
+        }
+        RawRow<DT, DP> raw[NT];
+#pragma unroll
+        for (int n = 0; n < NT; n++) fetch_row<DT, DP>(a, r, head, 16 * n + c, 16 * n + c < rows, raw[n]);
+        // K's codes are loaded again as soon as the first product has used them, V's after the second: each then has the other
+        // product and the softmax to arrive in, and the codes need registers once
+        uint4 k[4][NH], v[ND];
+        float ks, vs;
+        const uint8_t* vp;
+        SubBlock vb;
+        const auto aim = [&](int32_t key) __attribute__((always_inline)) {  // K's codes and the scales of the tile at `key`; where V's codes are
+            const SubBlock kb = sub_block(a.c, kid, head, key + 16 * (c >> 2), end);
+            vb = sub_block(a.c, vid, head, key + 16 * g, end);
+            const uint8_t* kp = a.c.k + ((kb.at << a.c.shift) + kb.sub * 16 + (c & 3)) * D;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int h = 0; h < NH; h++)  // dims past D: any codes, q is 0 there
+                    k[t][h] = *reinterpret_cast<const uint4*>(kp + 4 * t * D + (64 * h + 16 * g < D ? 64 * h + 16 * g : 0));
+            ks = a.c.ks[vb.at];
+            vs = a.c.vs[vb.at];
+            vp = a.c.v + ((vb.at << a.c.shift) + vb.sub * 16) * D + c * 16;
+            kid = block_id(a.c, r.table, key + 4 * kTile + 16 * (c >> 2), end);
+            vid = block_id(a.c, r.table, key + 4 * kTile + 16 * g, end);
+        };
+        const auto load_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int dt = 0; dt < ND; dt++) v[dt] = load_nt(vp + (16 * dt < D ? 256 * dt : 0));
+        };
+        if (k0 < last) {
+            aim(k0);
+            load_v();
         }
         f16x8 q[NT][NP][NH][2];
         Row row[NT];
@@ -446,100 +513,80 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
         f32x4 o[NT][ND];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            row[n] = load_row<DT, DP, NP>(a, r, head, 16 * n + c, 16 * n + c < rows, q[n]);
+            row[n] = make_row<DT, DP, NP>(a, r, head, 16 * n + c, 16 * n + c < rows, raw[n], q[n]);
             m[n] = kNone;
             l[n] = 0.0f;
 #pragma unroll
             for (int dt = 0; dt < ND; dt++) o[n][dt] = f32x4{0, 0, 0, 0};
         }
-        if (k0 < last) {
-            // K's codes are loaded again as soon as the first product has used them, V's after the second: each then has
-            // the other product and the softmax to arrive in, and the codes need registers once
-            uint4 k[4][NH], v[ND];
-            float ks, vs;
-            const uint8_t* vp;
-            SubBlock vb;
-            // Past the piece's last tile the loads go on, from block 0 (they are in its XCD's L2 after the first one): a branch
-            // around them would leave the compiler waiting for all of them where its paths meet.
-            const auto aim = [&](int32_t key) {  // K's codes and the scales of the tile at `key`; where V's codes are
-                const SubBlock kb = sub_block(a.c, kid, head, key + 16 * (c >> 2), last);
-                vb = sub_block(a.c, vid, head, key + 16 * g, last);
-                const uint8_t* kp = a.c.k + ((kb.at << a.c.shift) + kb.sub * 16 + (c & 3)) * D;
+        // One tile; `more`: the next one is loaded meanwhile. (Without a branch: where the paths of one meet, the compiler would
+        // wait for what was loaded on either.)
+        const auto tile = [&](int32_t key, auto more) __attribute__((always_inline)) {
+            f32x4 S[NT][4];
 #pragma unroll
-                for (int t = 0; t < 4; t++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int h = 0; h < NH; h++)  // dims past D: any codes, q is 0 there
-                        k[t][h] = *reinterpret_cast<const uint4*>(kp + 4 * t * D + (64 * h + 16 * g < D ? 64 * h + 16 * g : 0));
-                ks = a.c.ks[vb.at];
-                vs = a.c.vs[vb.at];
-                vp = a.c.v + ((vb.at << a.c.shift) + vb.sub * 16) * D + c * 16;
-                kid = block_id(a.c, r.table, key + 4 * kTile + 16 * (c >> 2), last);
-                vid = block_id(a.c, r.table, key + 4 * kTile + 16 * g, last);
-            };
-            const auto load_v = [&]() {
+                for (int t = 0; t < 4; t++) S[n][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int dt = 0; dt < ND; dt++) v[dt] = load_nt(vp + (16 * dt < D ? 256 * dt : 0));
-            };
-            aim(k0);
-            load_v();
-            for (int32_t key = k0; key < last; key += 4 * kTile) {
-                f32x4 S[NT][4];
+            for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int t = 0; t < 4; t++) S[n][t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int h = 0; h < NH; h++) {
-                        f16x8 x[2];
-                        codes_f16<FMT>(k[t][h], x[0], x[1]);
-#pragma unroll
-                        for (int s = 0; s < 2; s++)
-#pragma unroll
-                            for (int n = 0; n < NT; n++)
-#pragma unroll
-                                for (int e = 0; e < NP; e++) S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s], q[n][e][h][s], S[n][t], 0, 0, 0);
-                    }
-                TileScale sc = tile_scale(a.c, vb, ks, vs);
-                const int32_t keys = vb.keys;
-                if (vb.bad) raise_block(a.c, r.first, r.slot, key + 16 * g, vb.id);
-                // registers of their own, or the next scales' arrival is waited for to move them
-                asm volatile("" : "+v"(sc.k), "+v"(sc.ev), "+v"(sc.down));
-                __builtin_amdgcn_sched_barrier(0);
-                aim(key + 4 * kTile);
-                __builtin_amdgcn_sched_barrier(0);
-                f16x8 p[NT][NP][2];
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const int k0l = key + 16 * g;
-                    const int hi = min(row[n].pos - k0l + 1, keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
-                    const bool masked = __any(hi < 16 || lo > 0);
-                    const float alpha = tile_softmax<NP>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], l[n], p[n]);
-                    if (__any(alpha != 1.0f)) {
-#pragma unroll
-                        for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
-                    }
-                }
-                // keys that are not there have weight 0, but their codes could be NaN
-                if (__any(keys < 16)) {
-#pragma unroll
-                    for (int dt = 0; dt < ND; dt++) v[dt] = first_codes(v[dt], keys);
-                }
-#pragma unroll
-                for (int dt = 0; dt < ND; dt++) {
+                for (int h = 0; h < NH; h++) {
                     f16x8 x[2];
-                    codes_f16<FMT>(v[dt], x[0], x[1]);
+                    codes_f16<FMT>(k[t][h], x[0], x[1]);
 #pragma unroll
                     for (int s = 0; s < 2; s++)
 #pragma unroll
                         for (int n = 0; n < NT; n++)
 #pragma unroll
-                            for (int e = 0; e < NP; e++) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s], p[n][e][s], o[n][dt], 0, 0, 0);
+                            for (int e = 0; e < NP; e++) S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s], q[n][e][h][s], S[n][t], 0, 0, 0);
                 }
+            TileScale sc = tile_scale(a.c, vb, ks, vs);
+            const int32_t keys = vb.keys;
+            if (vb.bad) raise_block(a.c, r.first, r.slot, key + 16 * g, vb.id);
+            if constexpr (more) {
+                // scales in registers of their own, or the next ones' arrival is waited for to move them
+                asm volatile("" : "+v"(sc.k), "+v"(sc.ev), "+v"(sc.down));
+                __builtin_amdgcn_sched_barrier(0);
+                aim(key + 4 * kTile);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            f16x8 p[NT][NP][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const int k0l = key + 16 * g;
+                const int hi = min(row[n].pos - k0l + 1, keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
+                const bool masked = __any(hi < 16 || lo > 0);
+                const float alpha = tile_softmax<NP>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], l[n], p[n]);
+                if (__any(alpha != 1.0f)) {
+#pragma unroll
+                    for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
+                }
+            }
+            // keys that are not there have weight 0, but their codes could be NaN
+            if (__any(keys < 16)) {
+#pragma unroll
+                for (int dt = 0; dt < ND; dt++) v[dt] = first_codes(v[dt], keys);
+            }
+#pragma unroll
+            for (int dt = 0; dt < ND; dt++) {
+                f16x8 x[2];
+                codes_f16<FMT>(v[dt], x[0], x[1]);
+#pragma unroll
+                for (int s = 0; s < 2; s++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int e = 0; e < NP; e++) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s], p[n][e][s], o[n][dt], 0, 0, 0);
+            }
+            if constexpr (more) {
                 __builtin_amdgcn_sched_barrier(0);
                 load_v();
             }
+        };
+        if (k0 < last) {
+            int32_t key = k0;
+            for (; key + 4 * kTile < last; key += 4 * kTile) tile(key, std::true_type{});
+            tile(key, std::false_type{});
         }
         // the four waves: a common maximum, then the sums of waves 2 and 3 into 0 and 1, and 1 into 0
 #pragma unroll
@@ -664,8 +711,8 @@ __device__ __forceinline__ void join_waves(const Kv8AttnArgs& a, int64_t index)
     const Line f = find_line<true>(a, static_cast<int32_t>(index / a.c.heads));
     if (f.rounds == 0) return;
     const int64_t from = f.before * a.c.heads + static_cast<int64_t>(head) * f.rounds;
-    const int64_t w0 = from / f.each, w1 = (from + f.rounds - 1) / f.each;
-    const Kv8Request r = kv8_request(a.c, f.request);
+    const int64_t w0 = quotient(from, f.each), w1 = quotient(from + f.rounds - 1, f.each);
+    const Kv8Request& r = f.r;
     const int32_t row = 16 * n + (threadIdx.x & 15);
     if (w0 == w1 || 16 * n >= r.n * a.G) return;
     const int64_t slot0 = 2 * w0 + (w0 * f.each < from ? 1 : 0);
@@ -745,7 +792,9 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int32_t at = row0 + (wave * NT + n) * 16 + c;
-        row[n] = load_row<DT, DP, NP>(a, r, head, at, at < row1, q[n]);
+        RawRow<DT, DP> raw;
+        fetch_row<DT, DP>(a, r, head, at, at < row1, raw);
+        row[n] = make_row<DT, DP, NP>(a, r, head, at, at < row1, raw, q[n]);
         if (at < row1) {
             low = min(low, row[n].pos);
             high = max(high, row[n].pos);
