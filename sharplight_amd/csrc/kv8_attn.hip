@@ -1,5 +1,6 @@
 // Entry points of the attention over the 8-bit paged cache: checks, and what a call launches (kernels: kv8_attn.hpp).
 #include "kv8_attn.hpp"
+#include <stdlib.h>
 
 namespace slhip {
 
@@ -33,17 +34,19 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
     a->block_max = static_cast<int32_t>(limit);
     int64_t bytes = 0;
     if (p->wave_tiles) {
-        a->workers = dp == 256 ? 256 : 512;
+        a->workers = getenv("KV8_W") ? atoi(getenv("KV8_W")) : dp == 256 ? 256 : 512;
+        a->start = getenv("KV8_S") ? atoi(getenv("KV8_S")) : kStart;
         p->by_part = B * heads < 256;
         bytes += 2 * a->workers * (few * dp + few * 2) * 4;
     }
     a->splits = 1;
     if (p->blocks) {
-        const int64_t tile = dtype == SLHIP_F32 || dp == 256 ? 64 : 128;
+        const int64_t tile = 64 * block_tiles(dtype == SLHIP_F32, static_cast<int>(dp));
         a->tile_tokens = static_cast<int32_t>(tile / G);
         a->items = item_count(T, B, a->tile_tokens, 1);
         const int64_t pairs = a->items * heads, longest = (c.bps << c.shift) / (4 * kTile) + 1;
-        int64_t s = pairs < kBlockUnits ? (kBlockUnits + pairs - 1) / pairs : 1;
+        const int64_t BU = getenv("KV8_BU") ? atoi(getenv("KV8_BU")) : kBlockUnits;
+        int64_t s = pairs < BU ? (BU + pairs - 1) / pairs : 1;
         if (s > kMaxSplits) s = kMaxSplits;
         if (s > longest) s = longest;
         a->splits = static_cast<int32_t>(s);
@@ -107,7 +110,7 @@ extern "C" SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q
     a.window = cfg->window > 0x7FFFFFFF ? 0 : static_cast<int32_t>(cfg->window);  // no context is that long
     a.slopes = cfg->slopes;
     a.part = static_cast<float*>(work);
-    a.reshaped = a.cap > 0.0f || a.slopes || !(a.scale > 0.0f);
+    a.cap_inverse = 1.0f / a.cap;
     Kv8AttnPlan p;
     const int64_t need = make_plan(dtype, a.G, cfg->max_new, &a, &p);
     if (need > 0 && (!work || !aligned16(work) || work_bytes < need))

@@ -37,7 +37,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = 64;
 constexpr float kBias = 8.0f;  // weights are at most 2^kBias in f16
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr int kLeastRounds = 1;
+constexpr int kStart = 2;
 constexpr float kNone = -1e30f;  // a maximum of nothing: finite, so that differences with -inf stay numbers
 
 struct Kv8AttnArgs {
@@ -46,14 +46,14 @@ struct Kv8AttnArgs {
     void* y;
     int64_t qt, qh, yt, yh;
     int32_t G;                   // query heads of a K/V head
-    float scale, cap;
+    float scale, cap, cap_inverse;
     int32_t window;              // 0: none
     const float* slopes;
-    bool reshaped;               // scores are capped or sloped, or scale is not positive
     int32_t min_rows, max_rows;    // few-row work: requests of (min_rows, max_rows] query rows a K/V head
     bool strict;                   // requests above max_rows are an error (nothing else takes them)
     int32_t block_min, block_max;  // many-row tiles: requests of (block_min, block_max] rows; above is an error
     int32_t workers;             // few-row thread blocks
+    int32_t start;
     int32_t tile_tokens, splits; // many-row tiles: tokens of a tile, key ranges it is cut into
     int64_t items;               // many-row tiles of a head
     float *part, *part2;         // sums of key ranges: of workers, of splits
@@ -247,41 +247,40 @@ struct TileScale {
 };
 
 template <int NP>
-__device__ __forceinline__ float tile_softmax(const Kv8AttnArgs& a, f32x4 (&S)[4], const Row& row, const TileScale& sc, int32_t key0,
+__device__ __forceinline__ float tile_softmax(const Kv8AttnArgs& a, const f32x4 (&products)[4], const Row& row, const TileScale& sc, int32_t key0,
                                               int lo, int hi, bool masked, float& m, float& l, f16x8 (&p)[NP][2])
 {
-    // t = fma(S, mul, add). Capped or sloped scores, masked tiles and multipliers that are not positive turn S into t first.
-    float mul = row.back * sc.k * kLog2e, add = sc.ev;
-    if (masked || a.reshaped) {
-        if (a.cap > 0.0f) {
-            const float in = row.back * sc.k / a.cap, out = a.cap * kLog2e;
+    // t = fma(S, mul, add): S is turned into t first only where it has to be, for caps and slopes, in tiles that are masked
+    // and where a multiplier that is not positive would make the smallest S the largest t.
+    float S[16], mul = row.back * sc.k * kLog2e, add = sc.ev;
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+    for (int j = 0; j < 16; j++) S[j] = products[j >> 2][j & 3];
+    if (a.cap > 0.0f) {
+        const float in = row.back * sc.k * a.cap_inverse, out = a.cap * kLog2e;
 #pragma unroll
-                for (int r = 0; r < 4; r++) S[t][r] = fmaf(tanh_f(S[t][r] * in), out, add);
-        } else {
+        for (int j = 0; j < 16; j++) S[j] = tanh_f(S[j] * in) * out;
+        mul = 1.0f;
+    }
+    if (a.slopes) {
+        add = fmaf(row.slope, static_cast<float>(key0 - row.pos), add);
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+        for (int j = 0; j < 16; j++) S[j] = fmaf(S[j], mul, fmaf(row.slope, static_cast<float>(j), add));
+        mul = 1.0f;
+        add = 0.0f;
+    } else if (masked || !(a.scale > 0.0f)) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) S[t][r] = fmaf(S[t][r], mul, add);
-        }
-        if (a.slopes) {
-            const float first = static_cast<float>(key0 - row.pos);
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) S[t][r] = fmaf(row.slope, first + static_cast<float>(4 * t + r), S[t][r]);
-        }
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) S[t][r] = 4 * t + r >= lo && 4 * t + r < hi ? S[t][r] : -INFINITY;
+        for (int j = 0; j < 16; j++) S[j] = fmaf(S[j], mul, add);
         mul = 1.0f;
         add = 0.0f;
     }
-    float mx = S[0][0];
+    if (masked) {
 #pragma unroll
-    for (int t = 0; t < 4; t++) mx = fmaxf(fmaxf(fmaxf(mx, S[t][0]), fmaxf(S[t][1], S[t][2])), S[t][3]);
+        for (int j = 0; j < 16; j++) S[j] = j >= lo && j < hi ? S[j] : -INFINITY;
+    }
+    float mx = S[0];
+#pragma unroll
+    for (int j = 1; j < 15; j += 2) mx = fmaxf(fmaxf(mx, S[j]), S[j + 1]);
+    mx = fmaxf(mx, S[15]);
     const float was = m;
     m = fmaxf(m, row_max(fmaf(mx, mul, add)));
     const float shift = add - (m - kBias);
@@ -290,14 +289,15 @@ __device__ __forceinline__ float tile_softmax(const Kv8AttnArgs& a, f32x4 (&S)[4
     for (int s = 0; s < 2; s++)
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
-            const int t = 2 * s + (j >> 2), r = j & 3;
-            const float w0 = __builtin_amdgcn_exp2f(fmaf(S[t][r], mul, shift)), w1 = __builtin_amdgcn_exp2f(fmaf(S[t][r + 1], mul, shift));
+            const int i = 8 * s + j;
+            const float w0 = __builtin_amdgcn_exp2f(fmaf(S[i], mul, shift)), w1 = __builtin_amdgcn_exp2f(fmaf(S[i + 1], mul, shift));
             sum += w0 + w1;
             const f16x2 hi2 = to_f16x2(w0, w1);
             p[0][s][j] = hi2.x;
             p[0][s][j + 1] = hi2.y;
             if constexpr (NP == 2) {
-                const f16x2 lo2 = to_f16x2(w0 - static_cast<float>(hi2.x), w1 - static_cast<float>(hi2.y));
+                // (as fused multiply-adds, which take the f16 part as it is)
+                const f16x2 lo2 = to_f16x2(fmaf(-static_cast<float>(hi2.x), 1.0f, w0), fmaf(-static_cast<float>(hi2.y), 1.0f, w1));
                 p[1][s][j] = lo2.x;
                 p[1][s][j + 1] = lo2.y;
             }
@@ -353,15 +353,18 @@ __device__ __forceinline__ void key_range(const Kv8AttnArgs& a, int32_t past, in
 
 // The work of all requests of a launch, in rounds of four key tiles (one for each wave of a thread block), is one line --
 // request by request, head by head -- that `workers` thread blocks share out in equal pieces, whatever the lengths are. A
-// piece that begins or ends inside a head's keys leaves partial sums, of which a worker has two at most: of its first
-// segment in slot 2 w, of its last in slot 2 w + 1. Where a piece lies follows from the lengths alone, so every worker finds
-// its own without a launch before it, and the join finds the workers of a head by a division.
+// piece that begins or ends inside a head's keys leaves partial sums, of which a worker has two at most: of the head that it
+// goes on with in slot 2 w, of one that it begins in slot 2 w + 1. Where a piece lies follows from the lengths alone, so every
+// worker finds its own without a launch before it, and the join finds the workers of a head by a division.
+// Beginning a head costs as much as kStart rounds (query and table loads, the join of the four waves), which stand on the
+// line before its rounds: without them the workers of short requests end last (64 sequences of 1 to 4095 tokens: KSTART0
+// us, with them KSTART1).
 struct Line {
-    int64_t each;     // rounds of a worker
-    int64_t total;    // rounds of all
-    int64_t before;   // rounds of a head of the requests before `request`
+    int64_t each;     // steps of a worker
+    int64_t total;    // steps of all
+    int64_t before;   // steps of a head of the requests before `request`
     int32_t request;  // the request looked for
-    int32_t rounds;   // its rounds a head
+    int32_t steps;    // its steps a head: kStart and its rounds (0: it is not the launch's)
     Kv8Request r;
 };
 
@@ -372,13 +375,13 @@ __device__ __forceinline__ int64_t quotient(int64_t n, int64_t d)
     return n / d;
 }
 
-__device__ __forceinline__ int32_t request_rounds(const Kv8AttnArgs& a, const Kv8Request& r)
+__device__ __forceinline__ int32_t request_steps(const Kv8AttnArgs& a, const Kv8Request& r)
 {
     const int64_t rows = static_cast<int64_t>(r.n) * a.G;
     if (r.n == 0 || rows <= a.min_rows || rows > a.max_rows) return 0;
     int32_t first, end;
     key_range(a, r.past, 0, r.n, first, end);
-    return (end - first + 4 * kTile - 1) / (4 * kTile);
+    return (end - first + 4 * kTile - 1) / (4 * kTile) + a.start;
 }
 
 // The line as one wave sees it, 64 requests a step, and on it the request of worker `at` (of request `at` itself if
@@ -388,12 +391,12 @@ template <bool BY_REQUEST> __device__ __forceinline__ Line find_line(const Kv8At
     const int lane = threadIdx.x & 63;
     Line f{0, 0, 0, -1, 0, {}};
     Kv8Request mine{};         // the lane's request in the last step
-    int32_t kept = 0, up = 0;  // its rounds, and their inclusive sum
+    int32_t kept = 0, up = 0;  // its steps, and their inclusive sum
     int64_t sum = 0;
     const auto step = [&](int32_t i0) {
         const bool there = i0 + lane < a.c.B;
         mine = kv8_request(a.c, there ? i0 + lane : 0);
-        kept = there ? request_rounds(a, mine) : 0;
+        kept = there ? request_steps(a, mine) : 0;
         up = kept;
         for (int o = 1; o < 64; o <<= 1) {
             const int32_t v = __shfl_up(up, o, 64);
@@ -402,8 +405,8 @@ template <bool BY_REQUEST> __device__ __forceinline__ Line find_line(const Kv8At
     };
     const auto take = [&](int32_t i0, int k) {
         f.request = i0 + k;
-        f.rounds = __builtin_amdgcn_readlane(kept, k);
-        f.before = sum + __builtin_amdgcn_readlane(up, k) - f.rounds;
+        f.steps = __builtin_amdgcn_readlane(kept, k);
+        f.before = sum + __builtin_amdgcn_readlane(up, k) - f.steps;
         f.r.first = __builtin_amdgcn_readlane(mine.first, k);
         f.r.n = __builtin_amdgcn_readlane(mine.n, k);
         f.r.past = __builtin_amdgcn_readlane(mine.past, k);
@@ -418,7 +421,7 @@ template <bool BY_REQUEST> __device__ __forceinline__ Line find_line(const Kv8At
     }
     f.total = sum * a.c.heads;
     f.each = quotient(f.total + a.workers - 1, a.workers);
-    if (f.each < kLeastRounds) f.each = kLeastRounds;
+    if (f.each < a.start + 1) f.each = a.start + 1;
     if (BY_REQUEST || at * f.each >= f.total) return f;
     sum = 0;
     for (int32_t i0 = 0; i0 < a.c.B; i0 += 64) {
@@ -459,12 +462,16 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
     if (line.request < 0) return;
     int64_t pos = worker * line.each;
     const int64_t stop = min(pos + line.each, line.total);
-    int32_t i = line.request, rounds = line.rounds;
+    int32_t i = line.request, steps = line.steps;
     const int64_t in = pos - line.before * a.c.heads;
-    int32_t head = static_cast<int32_t>(quotient(in, rounds)), from = static_cast<int32_t>(in - static_cast<int64_t>(head) * rounds);
+    int32_t head = static_cast<int32_t>(quotient(in, steps)), step = static_cast<int32_t>(in - static_cast<int64_t>(head) * steps);
     Kv8Request r = line.r;
-    for (bool opening = true;; opening = false) {
-        const int32_t count = static_cast<int32_t>(min(static_cast<int64_t>(rounds - from), stop - pos));
+    for (;;) {
+        const int32_t until = static_cast<int32_t>(min(static_cast<int64_t>(steps), step + (stop - pos)));
+        pos += until - step;
+        const bool goes_on = step >= a.start && pos - (until - step) == worker * line.each;
+        const int32_t from = max(step - a.start, 0), count = until - a.start - from;  // its rounds
+        if (count > 0) {
         const int32_t rows = r.n * a.G;
         int32_t first, end;
         key_range(a, r.past, 0, r.n, first, end);
@@ -627,8 +634,8 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
             __syncthreads();
         }
         if (wave == 0) {
-            float* part = a.part + (2 * static_cast<int64_t>(worker) + (opening ? 0 : 1)) * Partial<DP, NT>::kFloats;
-            const bool whole = count == rounds;
+            float* part = a.part + (2 * static_cast<int64_t>(worker) + (goes_on ? 0 : 1)) * Partial<DP, NT>::kFloats;
+            const bool whole = count == steps - a.start;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const int32_t at = 16 * n + c;
@@ -645,15 +652,15 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
                 }
             }
         }
-        pos += count;
+        }
         if (pos >= stop) return;
-        from = 0;
+        step = 0;
         if (++head == a.c.heads) {
             head = 0;
             do {
-                r = kv8_request(a.c, ++i);  // there is one: rounds are left on the line
-                rounds = request_rounds(a, r);
-            } while (rounds == 0);
+                r = kv8_request(a.c, ++i);  // there is one: steps are left on the line
+                steps = request_steps(a, r);
+            } while (steps == 0);
         }
     }
 }
@@ -709,9 +716,9 @@ __device__ __forceinline__ void join_waves(const Kv8AttnArgs& a, int64_t index)
     index /= NT;
     const int32_t head = static_cast<int32_t>(index % a.c.heads);
     const Line f = find_line<true>(a, static_cast<int32_t>(index / a.c.heads));
-    if (f.rounds == 0) return;
-    const int64_t from = f.before * a.c.heads + static_cast<int64_t>(head) * f.rounds;
-    const int64_t w0 = quotient(from, f.each), w1 = quotient(from + f.rounds - 1, f.each);
+    if (f.steps == 0) return;
+    const int64_t from = f.before * a.c.heads + static_cast<int64_t>(head) * f.steps + a.start;  // its first round
+    const int64_t w0 = quotient(from, f.each), w1 = quotient(from + f.steps - a.start - 1, f.each);
     const Kv8Request& r = f.r;
     const int32_t row = 16 * n + (threadIdx.x & 15);
     if (w0 == w1 || 16 * n >= r.n * a.G) return;
@@ -812,29 +819,34 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
     high = __builtin_amdgcn_readfirstlane(high);
     const int32_t all = r.past + r.n;  // keys of the request: codes behind them are not read as keys
 
-    // staging: wave w loads the codes of K's product t = w and of V's dims 16 (w + 4 j)
+    // staging: wave w loads the codes of K's product t = w and of V's dims 16 (w + 4 j). Table entries are a tile ahead of the
+    // codes that they lead to, codes a tile ahead of the products.
     constexpr int VJ = ND / 4;
     uint4 ck[NH], cv[VJ];
-    float ks = 0, vs = 0;
-    SubBlock vb{}, vnext{};
-    float ksn = 0, vsn = 0;
-    const auto load = [&](int32_t key) {
-        const int32_t kid = block_id(a.c, r.table, key + 16 * (c >> 2), all), vid = block_id(a.c, r.table, key + 16 * g, all);
+    SubBlock next;
+    float ksn, vsn;
+    int32_t kid = 0, vid = 0;
+    const auto look = [&](int32_t key) __attribute__((always_inline)) {
+        kid = block_id(a.c, r.table, key + 16 * (c >> 2), all);
+        vid = block_id(a.c, r.table, key + 16 * g, all);
+    };
+    const auto load = [&](int32_t key) __attribute__((always_inline)) {
         const SubBlock kb = sub_block(a.c, kid, head, key + 16 * (c >> 2), all);
-        vnext = sub_block(a.c, vid, head, key + 16 * g, all);
+        next = sub_block(a.c, vid, head, key + 16 * g, all);
         const uint8_t* k = a.c.k + ((kb.at << a.c.shift) + kb.sub * 16 + 4 * wave + (c & 3)) * D;
 #pragma unroll
         for (int h = 0; h < NH; h++) ck[h] = *reinterpret_cast<const uint4*>(k + (64 * h + 16 * g < D ? 64 * h + 16 * g : 0));
-        const uint8_t* v = a.c.v + ((vnext.at << a.c.shift) + vnext.sub * 16) * D + c * 16;
+        const uint8_t* v = a.c.v + ((next.at << a.c.shift) + next.sub * 16) * D + c * 16;
 #pragma unroll
         for (int j = 0; j < VJ; j++) {
             const int dt = wave + 4 * j;
             cv[j] = *reinterpret_cast<const uint4*>(v + (16 * dt < D ? 256 * dt : 0));
         }
-        ksn = a.c.ks[vnext.at];
-        vsn = a.c.vs[vnext.at];
+        ksn = a.c.ks[next.at];
+        vsn = a.c.vs[next.at];
+        look(key + kTile);
     };
-    const auto stage = [&](int buf) {
+    const auto stage = [&](int buf) __attribute__((always_inline)) {
         f16x8* f = s_frag + buf * (kK + kV) * 64 + lane;
 #pragma unroll
         for (int h = 0; h < NH; h++) {
@@ -843,73 +855,88 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
             f[((wave * NH + h) * 2) * 64] = x;
             f[((wave * NH + h) * 2 + 1) * 64] = z;
         }
+        if (__any(next.keys < 16)) {
+#pragma unroll
+            for (int j = 0; j < VJ; j++) cv[j] = first_codes(cv[j], next.keys);
+        }
 #pragma unroll
         for (int j = 0; j < VJ; j++) {
             f16x8 x, z;
-            codes_f16<FMT>(vnext.keys < 16 ? first_codes(cv[j], vnext.keys) : cv[j], x, z);
+            codes_f16<FMT>(cv[j], x, z);
             f[(kK + (wave + 4 * j) * 2) * 64] = x;
             f[(kK + (wave + 4 * j) * 2 + 1) * 64] = z;
         }
-        vb = vnext;
-        ks = ksn;
-        vs = vsn;
     };
-    int buf = 0;
-    if (first < end) {
-        load(first);
-        stage(0);
-    }
-    for (int32_t key = first; key < end; key += kTile) {
-        const bool more = key + kTile < end;
-        const SubBlock b = vb;
-        const TileScale sc = tile_scale(a.c, b, ks, vs);
-        if (more) load(key + kTile);
-        __syncthreads();
-        if (b.bad && wave == 0) raise_block(a.c, r.first, r.slot, key + 16 * g, b.id);
-        if (key <= high && (a.window <= 0 || key + kTile > low - a.window + 1)) {
-            const f16x8* f = s_frag + buf * (kK + kV) * 64 + lane;
-            f32x4 S[NT][4];
+    const auto compute = [&](int32_t key, int buf, const TileScale& sc, int32_t keys) __attribute__((always_inline)) {
+        if (key > high || (a.window > 0 && key + kTile <= low - a.window + 1)) return;  // nothing that the wave's rows see
+        const f16x8* f = s_frag + buf * (kK + kV) * 64 + lane;
+        f32x4 S[NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int t = 0; t < 4; t++) S[n][t] = f32x4{0, 0, 0, 0};
+            for (int t = 0; t < 4; t++) S[n][t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+        for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int h = 0; h < NH; h++)
-#pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        const f16x8 k = f[((t * NH + h) * 2 + s) * 64];
-#pragma unroll
-                        for (int n = 0; n < NT; n++)
-#pragma unroll
-                            for (int p = 0; p < NP; p++) S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][p][h][s], S[n][t], 0, 0, 0);
-                    }
-            f16x8 p[NT][NP][2];
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const int k0l = key + 16 * g;
-                const int hi = min(row[n].pos - k0l + 1, b.keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
-                const bool masked = __any(hi < 16 || lo > 0);
-                const float alpha = tile_softmax<NP>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], l[n], p[n]);
-                if (__any(alpha != 1.0f)) {
-#pragma unroll
-                    for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
-                }
-            }
-#pragma unroll
-            for (int dt = 0; dt < ND; dt++)
+            for (int h = 0; h < NH; h++)
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
-                    const f16x8 v = f[(kK + dt * 2 + s) * 64];
+                    const f16x8 k = f[((t * NH + h) * 2 + s) * 64];
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int e = 0; e < NP; e++) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[n][e][s], o[n][dt], 0, 0, 0);
+                        for (int p = 0; p < NP; p++) S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][p][h][s], S[n][t], 0, 0, 0);
                 }
+        f16x8 p[NT][NP][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int k0l = key + 16 * g;
+            const int hi = min(row[n].pos - k0l + 1, keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
+            const bool masked = __any(hi < 16 || lo > 0);
+            const float alpha = tile_softmax<NP>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], l[n], p[n]);
+            if (__any(alpha != 1.0f)) {
+#pragma unroll
+                for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
+            }
         }
-        buf ^= 1;
-        if (more) stage(buf);
+#pragma unroll
+        for (int dt = 0; dt < ND; dt++)
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const f16x8 v = f[(kK + dt * 2 + s) * 64];
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < NP; e++) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[n][e][s], o[n][dt], 0, 0, 0);
+            }
+    };
+    if (first < end) {
+        int buf = 0;
+        int32_t key = first;
+        look(key);
+        load(key);
+        stage(0);
+        const auto scales = [&](int32_t at) __attribute__((always_inline)) {
+            TileScale sc = tile_scale(a.c, next, ksn, vsn);
+            // in registers of their own, or the next scales' arrival is waited for to move them
+            asm volatile("" : "+v"(sc.k), "+v"(sc.ev), "+v"(sc.down));
+            if (next.bad && wave == 0) raise_block(a.c, r.first, r.slot, at + 16 * g, next.id);
+            return sc;
+        };
+        for (; key + kTile < end; key += kTile) {
+            const TileScale sc = scales(key);
+            const int32_t keys = next.keys;
+            __builtin_amdgcn_sched_barrier(0);
+            load(key + kTile);
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+            compute(key, buf, sc, keys);
+            buf ^= 1;
+            stage(buf);
+        }
+        const TileScale sc = scales(key);
+        __syncthreads();
+        compute(key, buf, sc, next.keys);
     }
     float* part = a.part2 + index * Partial<DP, 4 * NT>::kFloats;
 #pragma unroll
@@ -932,6 +959,9 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
 
 // ---- launches -----------------------------------------------------------------------------------------------------
 
+// Matrix tiles of 16 rows that a wave of a many-row tile works on: two where two waves a SIMD find registers for them.
+constexpr int block_tiles(bool f32, int dp) { return dp == 256 || (f32 && dp == 128) ? 1 : 2; }
+
 // What a call launches, from what the host knows.
 struct Kv8AttnPlan {
     int32_t wave_tiles;  // few-row launch: 0 none, else matrix tiles of 16 rows (1, 2)
@@ -939,14 +969,15 @@ struct Kv8AttnPlan {
     bool by_part;        // the few-row join shares out the sums of a head, not its dims
 };
 
-// Thread blocks of the few-row work, then of the many-row tiles: one launch, so that neither waits for the other's end.
+// Thread blocks of the many-row tiles, then of the few-row work: one launch, so that neither waits for the other's end.
 template <int DT, int FMT, int DP, int NT, int NB>
 __global__ __launch_bounds__(256, DP == 256 || NT == 2 ? 1 : 2) void kv8_attn(Kv8AttnArgs a)
 {
     extern __shared__ __align__(16) char lds[];
     if constexpr (NT > 0 && NB > 0) {
-        if (blockIdx.x < static_cast<unsigned>(a.workers)) attn_waves<DT, FMT, DP, NT>(a, blockIdx.x, lds);
-        else attn_blocks<DT, FMT, DP, NB>(a, blockIdx.x - a.workers, lds);
+        const unsigned blocks = gridDim.x - a.workers;
+        if (blockIdx.x < blocks) attn_blocks<DT, FMT, DP, NB>(a, blockIdx.x, lds);
+        else attn_waves<DT, FMT, DP, NT>(a, blockIdx.x - blocks, lds);
     } else if constexpr (NT > 0) {
         attn_waves<DT, FMT, DP, NT>(a, blockIdx.x, lds);
     } else {
@@ -975,7 +1006,7 @@ template <int DT, int FMT, int DP, int NT, int NB> static int kv8_attn_start(con
 
 template <int DT, int FMT, int DP> static int kv8_attn_run(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
 {
-    constexpr int NB = DT == SLHIP_F32 || DP == 256 ? 1 : 2, NT2 = DP <= 128 ? 2 : 1;  // make_plan asks for two tiles up to 128 dims
+    constexpr int NB = block_tiles(DT == SLHIP_F32, DP), NT2 = DP <= 128 ? 2 : 1;  // make_plan asks for two up to 128 dims
     int e;
     if (p.blocks) e = p.wave_tiles ? kv8_attn_start<DT, FMT, DP, 1, NB>(a, st) : kv8_attn_start<DT, FMT, DP, 0, NB>(a, st);
     else e = p.wave_tiles == 1 ? kv8_attn_start<DT, FMT, DP, 1, 0>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0>(a, st);
