@@ -35,7 +35,6 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
     int64_t bytes = 0;
     if (p->wave_tiles) {
         a->workers = getenv("KV8_W") ? atoi(getenv("KV8_W")) : dp == 256 ? 256 : 512;
-        a->start = getenv("KV8_S") ? atoi(getenv("KV8_S")) : kStart;
         p->by_part = B * heads < 256;
         bytes += 2 * a->workers * (few * dp + few * 2) * 4;
     }

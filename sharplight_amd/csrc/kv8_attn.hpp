@@ -53,7 +53,6 @@ struct Kv8AttnArgs {
     bool strict;                   // requests above max_rows are an error (nothing else takes them)
     int32_t block_min, block_max;  // many-row tiles: requests of (block_min, block_max] rows; above is an error
     int32_t workers;             // few-row thread blocks
-    int32_t start;
     int32_t tile_tokens, splits; // many-row tiles: tokens of a tile, key ranges it is cut into
     int64_t items;               // many-row tiles of a head
     float *part, *part2;         // sums of key ranges: of workers, of splits
@@ -381,7 +380,7 @@ __device__ __forceinline__ int32_t request_steps(const Kv8AttnArgs& a, const Kv8
     if (r.n == 0 || rows <= a.min_rows || rows > a.max_rows) return 0;
     int32_t first, end;
     key_range(a, r.past, 0, r.n, first, end);
-    return (end - first + 4 * kTile - 1) / (4 * kTile) + a.start;
+    return (end - first + 4 * kTile - 1) / (4 * kTile) + kStart;
 }
 
 // The line as one wave sees it, 64 requests a step, and on it the request of worker `at` (of request `at` itself if
@@ -421,7 +420,7 @@ template <bool BY_REQUEST> __device__ __forceinline__ Line find_line(const Kv8At
     }
     f.total = sum * a.c.heads;
     f.each = quotient(f.total + a.workers - 1, a.workers);
-    if (f.each < a.start + 1) f.each = a.start + 1;
+    if (f.each < 1) f.each = 1;
     if (BY_REQUEST || at * f.each >= f.total) return f;
     sum = 0;
     for (int32_t i0 = 0; i0 < a.c.B; i0 += 64) {
@@ -460,60 +459,105 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
         }
     }
     if (line.request < 0) return;
+
+    // A head's share of the piece, and what its loads go by.
+    struct Segment {
+        const int32_t* table;
+        int32_t row0, n, past, slot;  // of the request
+        int32_t i, steps, head;
+        int32_t end, k0, last;  // the request's keys; the wave's first tile; where its tiles end
+        int32_t whole, goes_on;
+        __device__ __forceinline__ void take(const Kv8Request& r) { table = r.table; row0 = r.first; n = r.n; past = r.past; slot = r.slot; }
+        __device__ __forceinline__ Kv8Request request() const { return {row0, n, past, slot, false, table}; }
+    } cur, next;
     int64_t pos = worker * line.each;
-    const int64_t stop = min(pos + line.each, line.total);
-    int32_t i = line.request, steps = line.steps;
-    const int64_t in = pos - line.before * a.c.heads;
-    int32_t head = static_cast<int32_t>(quotient(in, steps)), step = static_cast<int32_t>(in - static_cast<int64_t>(head) * steps);
-    Kv8Request r = line.r;
-    for (;;) {
-        const int32_t until = static_cast<int32_t>(min(static_cast<int64_t>(steps), step + (stop - pos)));
+    const int64_t begin = pos, stop = min(pos + line.each, line.total);
+    int32_t step;
+    // The share of the head that cur points at from `step` on; false if the piece ends before its rounds.
+    const auto share = [&](Segment& s) __attribute__((always_inline)) {
+        const int32_t until = static_cast<int32_t>(min(static_cast<int64_t>(s.steps), step + (stop - pos)));
+        s.goes_on = pos == begin && step >= kStart;
         pos += until - step;
-        const bool goes_on = step >= a.start && pos - (until - step) == worker * line.each;
-        const int32_t from = max(step - a.start, 0), count = until - a.start - from;  // its rounds
-        if (count > 0) {
-        const int32_t rows = r.n * a.G;
-        int32_t first, end;
-        key_range(a, r.past, 0, r.n, first, end);
-        const int32_t k0 = first + (from * 4 + wave) * kTile;
-        const int32_t last = static_cast<int32_t>(min(static_cast<int64_t>(end), first + (static_cast<int64_t>(from) + count) * 4 * kTile));
-        int32_t kid = 0, vid = 0;
-        if (k0 < last) {
-            kid = block_id(a.c, r.table, k0 + 16 * (c >> 2), end);
-            vid = block_id(a.c, r.table, k0 + 16 * g, end);
+        const int32_t from = max(step - kStart, 0), count = until - kStart - from;
+        if (count <= 0) return false;
+        int32_t first;
+        key_range(a, s.past, 0, s.n, first, s.end);
+        s.k0 = first + (from * 4 + wave) * kTile;
+        s.last = static_cast<int32_t>(min(static_cast<int64_t>(s.end), first + (static_cast<int64_t>(from) + count) * 4 * kTile));
+        s.whole = count == s.steps - kStart;
+        return true;
+    };
+    const auto advance = [&](Segment& s) __attribute__((always_inline)) {  // to the next head on the line, while the piece lasts
+        step = 0;
+        for (;;) {
+            if (pos >= stop) return false;
+            if (++s.head == a.c.heads) {
+                s.head = 0;
+                do {
+                    const Kv8Request r = kv8_request(a.c, ++s.i);  // there is one: steps are left on the line
+                    s.take(r);
+                    s.steps = request_steps(a, r);
+                } while (s.steps == 0);
+            }
+            if (share(s)) return true;
         }
-        RawRow<DT, DP> raw[NT];
+    };
+    cur.take(line.r);
+    cur.i = line.request;
+    cur.steps = line.steps;
+    const int64_t in = pos - line.before * a.c.heads;
+    cur.head = static_cast<int32_t>(quotient(in, cur.steps));
+    step = static_cast<int32_t>(in - static_cast<int64_t>(cur.head) * cur.steps);
+    if (!share(cur) && !advance(cur)) return;
+
+    constexpr bool kEarly = DT != SLHIP_F32 && DP <= 128;  // (f32 queries and 256 dims leave no registers for that)
+    // K's codes are loaded again as soon as the first product has used them, V's after the second: each then has the other
+    // product and the softmax to arrive in, and the codes need registers once. The next head's first tile and queries are on
+    // their way while the four waves join this one's sums.
+    RawRow<DT, DP> raw[NT];
+    uint4 k[4][NH], v[ND];
+    float ks, vs;
+    const uint8_t* vp;
+    SubBlock vb;
+    int32_t kid, vid;
+    const auto look = [&](const Segment& s, int32_t key) __attribute__((always_inline)) {
+        kid = block_id(a.c, s.table, key + 16 * (c >> 2), s.end);
+        vid = block_id(a.c, s.table, key + 16 * g, s.end);
+    };
+    const auto aim = [&](const Segment& s, int32_t key) __attribute__((always_inline)) {  // K's codes and the scales of the tile at `key`; where V's codes are
+        const SubBlock kb = sub_block(a.c, kid, s.head, key + 16 * (c >> 2), s.end);
+        vb = sub_block(a.c, vid, s.head, key + 16 * g, s.end);
+        const uint8_t* kp = a.c.k + ((kb.at << a.c.shift) + kb.sub * 16 + (c & 3)) * D;
 #pragma unroll
-        for (int n = 0; n < NT; n++) fetch_row<DT, DP>(a, r, head, 16 * n + c, 16 * n + c < rows, raw[n]);
-        // K's codes are loaded again as soon as the first product has used them, V's after the second: each then has the other
-        // product and the softmax to arrive in, and the codes need registers once
-        uint4 k[4][NH], v[ND];
-        float ks, vs;
-        const uint8_t* vp;
-        SubBlock vb;
-        const auto aim = [&](int32_t key) __attribute__((always_inline)) {  // K's codes and the scales of the tile at `key`; where V's codes are
-            const SubBlock kb = sub_block(a.c, kid, head, key + 16 * (c >> 2), end);
-            vb = sub_block(a.c, vid, head, key + 16 * g, end);
-            const uint8_t* kp = a.c.k + ((kb.at << a.c.shift) + kb.sub * 16 + (c & 3)) * D;
+        for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+            for (int h = 0; h < NH; h++)  // dims past D: any codes, q is 0 there
+                k[t][h] = *reinterpret_cast<const uint4*>(kp + 4 * t * D + (64 * h + 16 * g < D ? 64 * h + 16 * g : 0));
+        ks = a.c.ks[vb.at];
+        vs = a.c.vs[vb.at];
+        vp = a.c.v + ((vb.at << a.c.shift) + vb.sub * 16) * D + c * 16;
+        look(s, key + 4 * kTile);
+    };
+    const auto load_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
-                for (int h = 0; h < NH; h++)  // dims past D: any codes, q is 0 there
-                    k[t][h] = *reinterpret_cast<const uint4*>(kp + 4 * t * D + (64 * h + 16 * g < D ? 64 * h + 16 * g : 0));
-            ks = a.c.ks[vb.at];
-            vs = a.c.vs[vb.at];
-            vp = a.c.v + ((vb.at << a.c.shift) + vb.sub * 16) * D + c * 16;
-            kid = block_id(a.c, r.table, key + 4 * kTile + 16 * (c >> 2), end);
-            vid = block_id(a.c, r.table, key + 4 * kTile + 16 * g, end);
-        };
-        const auto load_v = [&]() __attribute__((always_inline)) {
+        for (int dt = 0; dt < ND; dt++) v[dt] = load_nt(vp + (16 * dt < D ? 256 * dt : 0));
+    };
+    // Queries first (they are used first), then the first tile, if the wave has one.
+    const auto open = [&](const Segment& s) __attribute__((always_inline)) {
 #pragma unroll
-            for (int dt = 0; dt < ND; dt++) v[dt] = load_nt(vp + (16 * dt < D ? 256 * dt : 0));
-        };
-        if (k0 < last) {
-            aim(k0);
+        for (int n = 0; n < NT; n++) fetch_row<DT, DP>(a, s.request(), s.head, 16 * n + c, 16 * n + c < s.n * a.G, raw[n]);
+        if (s.k0 < s.last) {
+            aim(s, s.k0);
             load_v();
         }
+    };
+    look(cur, min(cur.k0, cur.end - 1));
+    open(cur);
+    for (;;) {
+        const Kv8Request r = cur.request();
+        const int32_t rows = r.n * a.G, head = cur.head;
+        next = cur;
+        const bool another = advance(next);
         f16x8 q[NT][NP][NH][2];
         Row row[NT];
         float m[NT], l[NT];
@@ -554,7 +598,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
                 // scales in registers of their own, or the next ones' arrival is waited for to move them
                 asm volatile("" : "+v"(sc.k), "+v"(sc.ev), "+v"(sc.down));
                 __builtin_amdgcn_sched_barrier(0);
-                aim(key + 4 * kTile);
+                aim(cur, key + 4 * kTile);
                 __builtin_amdgcn_sched_barrier(0);
             }
             f16x8 p[NT][NP][2];
@@ -590,11 +634,16 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
                 load_v();
             }
         };
-        if (k0 < last) {
-            int32_t key = k0;
-            for (; key + 4 * kTile < last; key += 4 * kTile) tile(key, std::true_type{});
+        if (cur.k0 < cur.last) {
+            int32_t key = cur.k0;
+            for (; key + 4 * kTile < cur.last; key += 4 * kTile) tile(key, std::true_type{});
             tile(key, std::false_type{});
         }
+        if (another) {
+            look(next, min(next.k0, next.end - 1));
+            if (kEarly) open(next);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         // the four waves: a common maximum, then the sums of waves 2 and 3 into 0 and 1, and 1 into 0
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -634,12 +683,11 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
             __syncthreads();
         }
         if (wave == 0) {
-            float* part = a.part + (2 * static_cast<int64_t>(worker) + (goes_on ? 0 : 1)) * Partial<DP, NT>::kFloats;
-            const bool whole = count == steps - a.start;
+            float* part = a.part + (2 * static_cast<int64_t>(worker) + (cur.goes_on ? 0 : 1)) * Partial<DP, NT>::kFloats;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const int32_t at = 16 * n + c;
-                if (whole) {
+                if (cur.whole) {
                     const float inv = row_inverse(l[n]);
                     if (at < rows) {
 #pragma unroll
@@ -652,16 +700,9 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
                 }
             }
         }
-        }
-        if (pos >= stop) return;
-        step = 0;
-        if (++head == a.c.heads) {
-            head = 0;
-            do {
-                r = kv8_request(a.c, ++i);  // there is one: steps are left on the line
-                steps = request_steps(a, r);
-            } while (steps == 0);
-        }
+        if (!another) return;
+        if (!kEarly) open(next);
+        cur = next;
     }
 }
 
@@ -717,8 +758,8 @@ __device__ __forceinline__ void join_waves(const Kv8AttnArgs& a, int64_t index)
     const int32_t head = static_cast<int32_t>(index % a.c.heads);
     const Line f = find_line<true>(a, static_cast<int32_t>(index / a.c.heads));
     if (f.steps == 0) return;
-    const int64_t from = f.before * a.c.heads + static_cast<int64_t>(head) * f.steps + a.start;  // its first round
-    const int64_t w0 = quotient(from, f.each), w1 = quotient(from + f.steps - a.start - 1, f.each);
+    const int64_t from = f.before * a.c.heads + static_cast<int64_t>(head) * f.steps + kStart;  // its first round
+    const int64_t w0 = quotient(from, f.each), w1 = quotient(from + f.steps - kStart - 1, f.each);
     const Kv8Request& r = f.r;
     const int32_t row = 16 * n + (threadIdx.x & 15);
     if (w0 == w1 || 16 * n >= r.n * a.G) return;
