@@ -383,56 +383,79 @@ __device__ __forceinline__ int32_t request_steps(const Kv8AttnArgs& a, const Kv8
     return (end - first + 4 * kTile - 1) / (4 * kTile) + kStart;
 }
 
-// The line as one wave sees it, 64 requests a step, and on it the request of worker `at` (of request `at` itself if
-// BY_REQUEST). Wave-uniform.
+// Inclusive sums over the wave: shifts within rows of 16 lanes, then each row's total into those after it.
+__device__ __forceinline__ int32_t wave_scan(int32_t v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);  // row_shr:8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31
+    return v;
+}
+
+constexpr int kMaxGroups = 65536 / 64;  // of 64 requests
+
+// The line, and on it the request of worker `at` (of request `at` itself if BY_REQUEST). The requests are taken in groups of
+// 64, a lane each; the waves of the thread block share out the groups' sums, and each then looks again at the one group that
+// holds the request. Wave-uniform; all 256 threads call it.
 template <bool BY_REQUEST> __device__ __forceinline__ Line find_line(const Kv8AttnArgs& a, int32_t at)
 {
-    const int lane = threadIdx.x & 63;
+    __shared__ int32_t s_group[kMaxGroups];
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const int32_t groups = (a.c.B + 63) / 64;
     Line f{0, 0, 0, -1, 0, {}};
-    Kv8Request mine{};         // the lane's request in the last step
+    Kv8Request mine{};         // the lane's request in the group looked at
     int32_t kept = 0, up = 0;  // its steps, and their inclusive sum
-    int64_t sum = 0;
-    const auto step = [&](int32_t i0) {
-        const bool there = i0 + lane < a.c.B;
-        mine = kv8_request(a.c, there ? i0 + lane : 0);
-        kept = there ? request_steps(a, mine) : 0;
-        up = kept;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int32_t v = __shfl_up(up, o, 64);
-            if (lane >= o) up += v;
+    const auto look = [&](int32_t group) {
+        const int32_t i = group * 64 + lane;
+        mine = kv8_request(a.c, i < a.c.B ? i : 0);
+        kept = i < a.c.B ? request_steps(a, mine) : 0;
+        up = wave_scan(kept);
+    };
+    int32_t group = 0;
+    int64_t sum = 0, before = 0;  // steps of all requests, of those before the group
+    if (groups == 1) {
+        look(0);
+        sum = __builtin_amdgcn_readlane(up, 63);
+    } else {
+        for (int32_t j = wave; j < groups; j += 4) {
+            look(j);
+            if (lane == 63) s_group[j] = up;
         }
-    };
-    const auto take = [&](int32_t i0, int k) {
-        f.request = i0 + k;
-        f.steps = __builtin_amdgcn_readlane(kept, k);
-        f.before = sum + __builtin_amdgcn_readlane(up, k) - f.steps;
-        f.r.first = __builtin_amdgcn_readlane(mine.first, k);
-        f.r.n = __builtin_amdgcn_readlane(mine.n, k);
-        f.r.past = __builtin_amdgcn_readlane(mine.past, k);
-        f.r.slot = __builtin_amdgcn_readlane(mine.slot, k);
-        f.r.bad = f.r.n == 0;
-        f.r.table = a.c.pages + (f.r.bad ? 0 : f.r.slot * a.c.bps);
-    };
-    for (int32_t i0 = 0; i0 < a.c.B; i0 += 64) {
-        step(i0);
-        if (BY_REQUEST && at >= i0 && at < i0 + 64) take(i0, at - i0);
-        sum += __builtin_amdgcn_readlane(up, 63);
+        __syncthreads();
+        for (int32_t j = 0; j < groups; j += 64) sum += __builtin_amdgcn_readlane(wave_scan(j + lane < groups ? s_group[j + lane] : 0), 63);
     }
     f.total = sum * a.c.heads;
     f.each = quotient(f.total + a.workers - 1, a.workers);
     if (f.each < 1) f.each = 1;
-    if (BY_REQUEST || at * f.each >= f.total) return f;
-    sum = 0;
-    for (int32_t i0 = 0; i0 < a.c.B; i0 += 64) {
-        if (a.c.B > 64) step(i0);
-        const uint64_t under = __ballot((sum + up) * a.c.heads <= at * f.each);  // requests that end before the piece begins
-        const int k = __popcll(under);
-        if (k < 64) {
-            take(i0, k);
-            break;
+    if (!BY_REQUEST && at * f.each >= f.total) return f;
+    // requests that end before the piece begins, in whole groups and then in the group
+    const auto under = [&](int64_t end) { return end * a.c.heads <= at * f.each; };
+    if (groups > 1) {
+        for (int32_t j = 0; j < groups; j += 64) {
+            const int32_t g = wave_scan(j + lane < groups ? s_group[j + lane] : 0);
+            const int32_t k = BY_REQUEST ? at / 64 - j : __popcll(__ballot(j + lane < groups && under(before + g)));
+            if (k < 64) {
+                group = j + k;
+                if (k > 0) before += __builtin_amdgcn_readlane(g, k - 1);
+                break;
+            }
+            before += __builtin_amdgcn_readlane(g, 63);
         }
-        sum += __builtin_amdgcn_readlane(up, 63);
+        look(group);
     }
+    const int k = BY_REQUEST ? at & 63 : __popcll(__ballot(under(before + up)));  // below 64: the piece begins in the group
+    f.request = group * 64 + k;
+    f.steps = __builtin_amdgcn_readlane(kept, k);
+    f.before = before + __builtin_amdgcn_readlane(up, k) - f.steps;
+    f.r.first = __builtin_amdgcn_readlane(mine.first, k);
+    f.r.n = __builtin_amdgcn_readlane(mine.n, k);
+    f.r.past = __builtin_amdgcn_readlane(mine.past, k);
+    f.r.slot = __builtin_amdgcn_readlane(mine.slot, k);
+    f.r.bad = f.r.n == 0;
+    f.r.table = a.c.pages + (f.r.bad ? 0 : f.r.slot * a.c.bps);
     return f;
 }
 
@@ -708,39 +731,57 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
 
 // ---- joins ----------------------------------------------------------------------------------------------------------
 
-// Joins `count` partial sums of 16 rows that lie `step` floats apart from `part` on (the first at `first`): the common
-// maximum, then the sums relative to it. The thread block's waves share out the dims, or (BY_PART) the sums of dims `dt0`,
-// which go through LDS then. put(dt, o, l) gets what the wave has of d-tile dt.
+// Joins `count` partial sums of 16 rows, the k-th at at(k): four at a time, relative to the largest maximum so far. The
+// thread block's waves share out the dims, or (BY_PART) the sums of d-tile dt0, which they then join through LDS.
+// put(dt, o, l) gets what the wave has of d-tile dt.
 template <int DP, int NT, bool BY_PART, class At, class Put>
 __device__ __forceinline__ void join_rows(const At& at, int32_t count, int n, int dt0, const Put& put)
 {
     constexpr int ND = DP / 16;
     const int lane = threadIdx.x & 63, wave = wave_id(), c = lane & 15;
-    const auto ml = [&](int32_t k) { return reinterpret_cast<const float2*>(at(k) + Partial<DP, NT>::kDims)[16 * n + c]; };
-    float top = kNone;
-#pragma unroll 4
-    for (int32_t k = 0; k < count; k++) top = fmaxf(top, ml(k).x);
     for (int dt = BY_PART ? dt0 : wave; dt < (BY_PART ? dt0 + 1 : ND); dt += 4) {
         f32x4 o = {0, 0, 0, 0};
-        float l = 0.0f;
-#pragma unroll 4
-        for (int32_t k = BY_PART ? wave : 0; k < count; k += BY_PART ? 4 : 1) {
-            const float2 v = ml(k);
-            const f32x4 x = reinterpret_cast<const f32x4*>(at(k))[(n * ND + dt) * 64 + lane];
-            const float by = __builtin_amdgcn_exp2f(v.x - top);
-            l = fmaf(v.y, by, l);
+        float l = 0.0f, top = kNone;
+        for (int32_t k = BY_PART ? wave : 0; k < count; k += BY_PART ? 16 : 4) {
+            float2 ml[4];
+            f32x4 x[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[j] = fmaf(x[j], by, o[j]);
+            for (int u = 0; u < 4; u++) {
+                const int32_t j = k + u * (BY_PART ? 4 : 1);
+                const float* p = at(min(j, count - 1));
+                ml[u] = reinterpret_cast<const float2*>(p + Partial<DP, NT>::kDims)[16 * n + c];
+                x[u] = reinterpret_cast<const f32x4*>(p)[(n * ND + dt) * 64 + lane];
+                if (j >= count) ml[u].x = -INFINITY;  // the last one again, with no weight
+            }
+            const float was = top;
+#pragma unroll
+            for (int u = 0; u < 4; u++) top = fmaxf(top, ml[u].x);
+            const float alpha = __builtin_amdgcn_exp2f(was - top);
+            l *= alpha;
+            o *= alpha;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float by = __builtin_amdgcn_exp2f(ml[u].x - top);
+                l = fmaf(ml[u].y, by, l);
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j] = fmaf(x[u][j], by, o[j]);
+            }
         }
         if constexpr (BY_PART) {
             __shared__ f32x4 s_o[4][64];
-            __shared__ float s_l[4][64];
+            __shared__ float2 s_ml[4][64];
             s_o[wave][lane] = o;
-            s_l[wave][lane] = l;
+            s_ml[wave][lane] = make_float2(top, l);
             __syncthreads();
             if (wave > 0) return;
-            o = (s_o[0][lane] + s_o[1][lane]) + (s_o[2][lane] + s_o[3][lane]);
-            l = (s_l[0][lane] + s_l[1][lane]) + (s_l[2][lane] + s_l[3][lane]);
+            for (int w = 1; w < 4; w++) top = fmaxf(top, s_ml[w][lane].x);
+            o = f32x4{0, 0, 0, 0};
+            l = 0.0f;
+            for (int w = 0; w < 4; w++) {
+                const float by = __builtin_amdgcn_exp2f(s_ml[w][lane].x - top);
+                l = fmaf(s_ml[w][lane].y, by, l);
+                o += s_o[w][lane] * by;
+            }
         }
         put(dt, o, l);
     }
