@@ -601,18 +601,22 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int t = 0; t < 4; t++) S[n][t] = f32x4{0, 0, 0, 0};
+            // two 16-key products (and two dim tiles below) take turns, so that none waits for its own last product
 #pragma unroll
-            for (int t = 0; t < 4; t++)
+            for (int t = 0; t < 4; t += 2)
 #pragma unroll
                 for (int h = 0; h < NH; h++) {
-                    f16x8 x[2];
-                    codes_f16<FMT>(k[t][h], x[0], x[1]);
+                    f16x8 x[2][2];
+                    codes_f16<FMT>(k[t][h], x[0][0], x[0][1]);
+                    codes_f16<FMT>(k[t + 1][h], x[1][0], x[1][1]);
 #pragma unroll
                     for (int s = 0; s < 2; s++)
 #pragma unroll
-                        for (int n = 0; n < NT; n++)
+                        for (int e = 0; e < NP; e++)
 #pragma unroll
-                            for (int e = 0; e < NP; e++) S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s], q[n][e][h][s], S[n][t], 0, 0, 0);
+                            for (int u = 0; u < 2; u++)
+#pragma unroll
+                                for (int n = 0; n < NT; n++) S[n][t + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[u][s], q[n][e][h][s], S[n][t + u], 0, 0, 0);
                 }
             TileScale sc = tile_scale(a.c, vb, ks, vs);
             const int32_t keys = vb.keys;
@@ -642,15 +646,18 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
                 for (int dt = 0; dt < ND; dt++) v[dt] = first_codes(v[dt], keys);
             }
 #pragma unroll
-            for (int dt = 0; dt < ND; dt++) {
-                f16x8 x[2];
-                codes_f16<FMT>(v[dt], x[0], x[1]);
+            for (int dt = 0; dt < ND; dt += 2) {
+                f16x8 x[2][2];
+                codes_f16<FMT>(v[dt], x[0][0], x[0][1]);
+                codes_f16<FMT>(v[dt + 1], x[1][0], x[1][1]);
 #pragma unroll
                 for (int s = 0; s < 2; s++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+                    for (int e = 0; e < NP; e++)
 #pragma unroll
-                        for (int e = 0; e < NP; e++) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s], p[n][e][s], o[n][dt], 0, 0, 0);
+                        for (int u = 0; u < 2; u++)
+#pragma unroll
+                            for (int n = 0; n < NT; n++) o[n][dt + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[u][s], p[n][e][s], o[n][dt + u], 0, 0, 0);
             }
             if constexpr (more) {
                 __builtin_amdgcn_sched_barrier(0);
@@ -957,18 +964,34 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int t = 0; t < 4; t++) S[n][t] = f32x4{0, 0, 0, 0};
+        // Fragments are read four ahead of the products that take them, so that LDS answers meanwhile; the four are of two
+        // 16-key products (of two dim tiles), so that 2 NT sums take turns and none waits for its own last product.
+        f16x8 frag[2][4];
+        const auto fetch = [&](int j) __attribute__((always_inline)) {  // group j: K's [t pair][h], then V's [dt pair]
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+            for (int u = 0; u < 4; u++) {
+                const int at = j < kK / 4 ? ((2 * (j / NH) + (u >> 1)) * NH + j % NH) * 2 + (u & 1) : 4 * j + u;
+                frag[j & 1][u] = f[at * 64];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        fetch(0);
 #pragma unroll
-            for (int h = 0; h < NH; h++)
+        for (int j = 0; j < kK / 4; j++) {
+            if (j + 1 < kK / 4) fetch(j + 1);
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    const f16x8 k = f[((t * NH + h) * 2 + s) * 64];
+            for (int s = 0; s < 2; s++)
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+                for (int p = 0; p < NP; p++)
 #pragma unroll
-                        for (int p = 0; p < NP; p++) S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[n][p][h][s], S[n][t], 0, 0, 0);
-                }
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            const int t = 2 * (j / NH) + u;
+                            S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(frag[j & 1][2 * u + s], q[n][p][j % NH][s], S[n][t], 0, 0, 0);
+                        }
+            __builtin_amdgcn_sched_barrier(0);
+        }
         f16x8 p[NT][NP][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -981,16 +1004,23 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
                 for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
             }
         }
+        fetch(kK / 4);
 #pragma unroll
-        for (int dt = 0; dt < ND; dt++)
+        for (int j = kK / 4; j < (kK + kV) / 4; j++) {
+            if (j + 1 < (kK + kV) / 4) fetch(j + 1);
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
-                const f16x8 v = f[(kK + dt * 2 + s) * 64];
+            for (int s = 0; s < 2; s++)
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int e = 0; e < NP; e++)
 #pragma unroll
-                    for (int e = 0; e < NP; e++) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[n][e][s], o[n][dt], 0, 0, 0);
-            }
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int n = 0; n < NT; n++) {
+                            const int dt = 2 * (j - kK / 4) + u;
+                            o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(frag[j & 1][2 * u + s], p[n][e][s], o[n][dt], 0, 0, 0);
+                        }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     if (first < end) {
         int buf = 0;
