@@ -4,10 +4,20 @@
 
 namespace slhip {
 
-template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_I8>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
-template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_E4M3>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
-template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_I8>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
-template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_E4M3>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_I8, false>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_E4M3, false>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_I8, false>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_E4M3, false>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_I8, true>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_E4M3, true>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_I8, true>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_E4M3, true>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+
+template <int DT, int FMT> static int launch(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
+{
+    const bool reshaped = a.cap > 0.0f || a.slopes || !(a.scale > 0.0f);
+    return reshaped ? kv8_attn_launch<DT, FMT, true>(a, p, st) : kv8_attn_launch<DT, FMT, false>(a, p, st);
+}
 
 constexpr int64_t kBlockUnits = 512;  // row tiles and key ranges of the many-row work, over all heads
 constexpr int64_t kMaxSplits = 64;
@@ -120,9 +130,9 @@ extern "C" SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q
     if (e) return e;
     hipStream_t st = to_stream(stream);
     if (dtype == SLHIP_F32) {
-        if (cache->format == SLHIP_KV8_I8) return kv8_attn_launch<SLHIP_F32, SLHIP_KV8_I8>(a, p, st);
-        return kv8_attn_launch<SLHIP_F32, SLHIP_KV8_E4M3>(a, p, st);
+        if (cache->format == SLHIP_KV8_I8) return launch<SLHIP_F32, SLHIP_KV8_I8>(a, p, st);
+        return launch<SLHIP_F32, SLHIP_KV8_E4M3>(a, p, st);
     }
-    if (cache->format == SLHIP_KV8_I8) return kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_I8>(a, p, st);
-    return kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_E4M3>(a, p, st);
+    if (cache->format == SLHIP_KV8_I8) return launch<SLHIP_BF16, SLHIP_KV8_I8>(a, p, st);
+    return launch<SLHIP_BF16, SLHIP_KV8_E4M3>(a, p, st);
 }

@@ -238,43 +238,55 @@ __device__ __forceinline__ float tanh_f(float y)
     return copysignf(u < 0.15f ? small : big, y);
 }
 
-// The softmax of one tile and row: S (codes' products of the lane's 16 keys, key 4t + r at S[t][r]) becomes weights.
-// lo <= key < hi of the sub-block are seen. m, l: the row's running maximum, the lane's part of its sum.
 struct TileScale {
     float k;         // ks
     float ev, down;  // log2(vs), 1 / vs
 };
 
-template <int NP>
-__device__ __forceinline__ float tile_softmax(const Kv8AttnArgs& a, const f32x4 (&products)[4], const Row& row, const TileScale& sc, int32_t key0,
-                                              int lo, int hi, bool masked, float& m, float& l, f16x8 (&p)[NP][2])
+// The softmax of one tile and row, in two steps. A lane has the row's products with its sub-block's 16 keys.
+struct TileRow {
+    float S[16];       // scores: weight j is 2^(S[j] * mul + shift)
+    float mul, shift;
+    float sum;         // of the weights so far
+};
+
+// Scores and the row's new maximum m (in TileRow's terms); returns what the row's sums so far are to be multiplied by.
+// lo <= j < hi are the keys that are seen.
+template <bool RESHAPED>
+__device__ __forceinline__ float tile_max(const Kv8AttnArgs& a, const f32x4 (&products)[4], const Row& row, const TileScale& sc, int32_t key0,
+                                          int lo, int hi, bool masked, float& m, TileRow& t)
 {
-    // t = fma(S, mul, add): S is turned into t first only where it has to be, for caps and slopes, in tiles that are masked
-    // and where a multiplier that is not positive would make the smallest S the largest t.
-    float S[16], mul = row.back * sc.k * kLog2e, add = sc.ev;
+    // t = fma(S, mul, add) with mul > 0, so the largest S is the largest t. Capped or sloped scores, and those of a scale that
+    // is not positive (RESHAPED), are turned into t themselves.
+    float (&S)[16] = t.S;
+    float mul = fmaxf(row.back * sc.k * kLog2e, 1.17549435e-38f), add = sc.ev;  // (a masked S is -inf: not times 0)
 #pragma unroll
     for (int j = 0; j < 16; j++) S[j] = products[j >> 2][j & 3];
-    if (a.cap > 0.0f) {
-        const float in = row.back * sc.k * a.cap_inverse, out = a.cap * kLog2e;
+    if constexpr (RESHAPED) {
+        if (a.cap > 0.0f) {
+            const float in = row.back * sc.k * a.cap_inverse, out = a.cap * kLog2e;
 #pragma unroll
-        for (int j = 0; j < 16; j++) S[j] = tanh_f(S[j] * in) * out;
-        mul = 1.0f;
-    }
-    if (a.slopes) {
-        add = fmaf(row.slope, static_cast<float>(key0 - row.pos), add);
+            for (int j = 0; j < 16; j++) S[j] = fmaf(tanh_f(S[j] * in), out, add);
+        } else {
+            mul = row.back * sc.k * kLog2e;
 #pragma unroll
-        for (int j = 0; j < 16; j++) S[j] = fmaf(S[j], mul, fmaf(row.slope, static_cast<float>(j), add));
-        mul = 1.0f;
-        add = 0.0f;
-    } else if (masked || !(a.scale > 0.0f)) {
+            for (int j = 0; j < 16; j++) S[j] = fmaf(S[j], mul, add);
+        }
+        if (a.slopes) {
+            const float far = row.slope * static_cast<float>(key0 - row.pos);
 #pragma unroll
-        for (int j = 0; j < 16; j++) S[j] = fmaf(S[j], mul, add);
+            for (int j = 0; j < 16; j++) S[j] += fmaf(row.slope, static_cast<float>(j), far);
+        }
         mul = 1.0f;
         add = 0.0f;
     }
     if (masked) {
 #pragma unroll
         for (int j = 0; j < 16; j++) S[j] = j >= lo && j < hi ? S[j] : -INFINITY;
+        if (hi <= max(lo, 0)) {  // none is seen: the block's scales, which may be no numbers, do not count
+            mul = 1.0f;
+            add = 0.0f;
+        }
     }
     float mx = S[0];
 #pragma unroll
@@ -282,38 +294,36 @@ __device__ __forceinline__ float tile_softmax(const Kv8AttnArgs& a, const f32x4 
     mx = fmaxf(mx, S[15]);
     const float was = m;
     m = fmaxf(m, row_max(fmaf(mx, mul, add)));
-    const float shift = add - (m - kBias);
-    float sum = 0.0f;
-#pragma unroll
-    for (int s = 0; s < 2; s++)
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-            const int i = 8 * s + j;
-            const float w0 = __builtin_amdgcn_exp2f(fmaf(S[i], mul, shift)), w1 = __builtin_amdgcn_exp2f(fmaf(S[i + 1], mul, shift));
-            sum += w0 + w1;
-            const f16x2 hi2 = to_f16x2(w0, w1);
-            p[0][s][j] = hi2.x;
-            p[0][s][j + 1] = hi2.y;
-            if constexpr (NP == 2) {
-                // (as fused multiply-adds, which take the f16 part as it is)
-                const f16x2 lo2 = to_f16x2(fmaf(-static_cast<float>(hi2.x), 1.0f, w0), fmaf(-static_cast<float>(hi2.y), 1.0f, w1));
-                p[1][s][j] = lo2.x;
-                p[1][s][j + 1] = lo2.y;
-            }
-        }
-    const float alpha = __builtin_amdgcn_exp2f(was - m);
-    l = fmaf(sum, sc.down, l * alpha);
-    return alpha;
+    t.mul = mul;
+    t.shift = add - (m - kBias);
+    t.sum = 0.0f;
+    return __builtin_amdgcn_exp2f(was - m);
+}
+
+// Weights 8 s + j and 8 s + j + 1 (j even), into P's parts.
+template <int NP> __device__ __forceinline__ void tile_weights(TileRow& t, int s, int j, f16x8 (&p)[NP][2])
+{
+    const float w0 = __builtin_amdgcn_exp2f(fmaf(t.S[8 * s + j], t.mul, t.shift));
+    const float w1 = __builtin_amdgcn_exp2f(fmaf(t.S[8 * s + j + 1], t.mul, t.shift));
+    t.sum += w0 + w1;
+    const f16x2 hi = to_f16x2(w0, w1);
+    p[0][s][j] = hi.x;
+    p[0][s][j + 1] = hi.y;
+    if constexpr (NP == 2) {  // (as fused multiply-adds, which take the f16 part as it is)
+        const f16x2 lo = to_f16x2(fmaf(-static_cast<float>(hi.x), 1.0f, w0), fmaf(-static_cast<float>(hi.y), 1.0f, w1));
+        p[1][s][j] = lo.x;
+        p[1][s][j + 1] = lo.y;
+    }
 }
 
 __device__ __forceinline__ TileScale tile_scale(const Kv8Dev& c, const SubBlock& s, float ks, float vs)
 {
     // a scale that is NaN makes the weights of the keys that are seen NaN, and must not reach l through those that are not
     const int e = static_cast<int>(__float_as_uint(vs) >> 23 & 0xFF) - 127;
-    const bool fine = e <= 126 && e >= -126;
+    const bool fine = e <= 126;
     TileScale o;
     o.k = ks;
-    o.ev = fine ? static_cast<float>(e) : vs;
+    o.ev = fine && ks == ks ? static_cast<float>(e) : __uint_as_float(0x7FC00000u);
     o.down = fine ? __uint_as_float(static_cast<uint32_t>(127 - e) << 23) : 1.0f;
     return o;
 }
@@ -467,7 +477,7 @@ template <int DP, int NT> struct Partial {
 
 template <int DP, int NT> constexpr int waves_lds() { return (2 * NT * (DP / 16) * 64 * 4 + 4 * NT * 16 * 2) * 4; }
 
-template <int DT, int FMT, int DP, int NT>
+template <int DT, int FMT, int DP, int NT, bool RESHAPED>
 __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t worker, char* lds)
 {
     constexpr int NP = DT == SLHIP_F32 ? 2 : 1, ND = DP / 16, NH = DP / 64;
@@ -634,11 +644,15 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
                 const int k0l = key + 16 * g;
                 const int hi = min(row[n].pos - k0l + 1, keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
                 const bool masked = __any(hi < 16 || lo > 0);
-                const float alpha = tile_softmax<NP>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], l[n], p[n]);
+                TileRow t;
+                const float alpha = tile_max<RESHAPED>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], t);
                 if (__any(alpha != 1.0f)) {
 #pragma unroll
                     for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
                 }
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) tile_weights<NP>(t, j >> 3, j & 7, p[n]);
+                l[n] = fmaf(t.sum, sc.down, l[n] * alpha);
             }
             // keys that are not there have weight 0, but their codes could be NaN
             if (__any(keys < 16)) {
@@ -849,7 +863,7 @@ template <int DP> struct BlockTile {
 
 template <int DP> constexpr int blocks_lds() { return 2 * (BlockTile<DP>::kK + BlockTile<DP>::kV) * 64 * static_cast<int>(sizeof(f16x8)); }
 
-template <int DT, int FMT, int DP, int NT>
+template <int DT, int FMT, int DP, int NT, bool RESHAPED>
 __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t index, char* lds)
 {
     constexpr int NP = DT == SLHIP_F32 ? 2 : 1, ND = DP / 16, NH = DP / 64;
@@ -884,44 +898,37 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
     Row row[NT];
     float m[NT], l[NT];
     f32x4 o[NT][ND];
-    int32_t low = 0x7FFFFFFF, high = -1;  // positions of the wave's rows
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int32_t at = row0 + (wave * NT + n) * 16 + c;
         RawRow<DT, DP> raw;
         fetch_row<DT, DP>(a, r, head, at, at < row1, raw);
         row[n] = make_row<DT, DP, NP>(a, r, head, at, at < row1, raw, q[n]);
-        if (at < row1) {
-            low = min(low, row[n].pos);
-            high = max(high, row[n].pos);
-        }
         m[n] = kNone;
         l[n] = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < ND; dt++) o[n][dt] = f32x4{0, 0, 0, 0};
     }
-    for (int x = 1; x < 16; x <<= 1) {
-        low = min(low, __shfl_xor(low, x, 64));
-        high = max(high, __shfl_xor(high, x, 64));
-    }
-    low = __builtin_amdgcn_readfirstlane(low);
-    high = __builtin_amdgcn_readfirstlane(high);
     const int32_t all = r.past + r.n;  // keys of the request: codes behind them are not read as keys
 
-    // staging: wave w loads the codes of K's product t = w and of V's dims 16 (w + 4 j). Table entries are a tile ahead of the
-    // codes that they lead to, codes a tile ahead of the products.
+    // Staging: wave w takes the codes of K's product t = w and of V's dims 16 (w + 4 j). Table entries are a tile ahead of
+    // the codes that they lead to, codes are loaded two tiles ahead of the products that take them and converted one tile
+    // ahead. Past the range's last tile that one is loaded again.
     constexpr int VJ = ND / 4;
     uint4 ck[NH], cv[VJ];
     SubBlock next;
     float ksn, vsn;
-    int32_t kid = 0, vid = 0;
+    int32_t kid, vid;
+    const int32_t border = first + ((end - first - 1) & ~(kTile - 1));  // the last tile
     const auto look = [&](int32_t key) __attribute__((always_inline)) {
+        key = min(key, border);
         kid = block_id(a.c, r.table, key + 16 * (c >> 2), all);
         vid = block_id(a.c, r.table, key + 16 * g, all);
     };
     const auto load = [&](int32_t key) __attribute__((always_inline)) {
-        const SubBlock kb = sub_block(a.c, kid, head, key + 16 * (c >> 2), all);
-        next = sub_block(a.c, vid, head, key + 16 * g, all);
+        const int32_t at = min(key, border);
+        const SubBlock kb = sub_block(a.c, kid, head, at + 16 * (c >> 2), all);
+        next = sub_block(a.c, vid, head, at + 16 * g, all);
         const uint8_t* k = a.c.k + ((kb.at << a.c.shift) + kb.sub * 16 + 4 * wave + (c & 3)) * D;
 #pragma unroll
         for (int h = 0; h < NH; h++) ck[h] = *reinterpret_cast<const uint4*>(k + (64 * h + 16 * g < D ? 64 * h + 16 * g : 0));
@@ -935,120 +942,117 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
         vsn = a.c.vs[next.at];
         look(key + kTile);
     };
-    const auto stage = [&](int buf) __attribute__((always_inline)) {
-        f16x8* f = s_frag + buf * (kK + kV) * 64 + lane;
-#pragma unroll
-        for (int h = 0; h < NH; h++) {
-            f16x8 x, z;
-            codes_f16<FMT>(ck[h], x, z);
-            f[((wave * NH + h) * 2) * 64] = x;
-            f[((wave * NH + h) * 2 + 1) * 64] = z;
-        }
+    const auto clip = [&]() __attribute__((always_inline)) {  // V's codes of keys that are not there
         if (__any(next.keys < 16)) {
 #pragma unroll
             for (int j = 0; j < VJ; j++) cv[j] = first_codes(cv[j], next.keys);
         }
-#pragma unroll
-        for (int j = 0; j < VJ; j++) {
-            f16x8 x, z;
-            codes_f16<FMT>(cv[j], x, z);
-            f[(kK + (wave + 4 * j) * 2) * 64] = x;
-            f[(kK + (wave + 4 * j) * 2 + 1) * 64] = z;
-        }
     };
-    const auto compute = [&](int32_t key, int buf, const TileScale& sc, int32_t keys) __attribute__((always_inline)) {
-        if (key > high || (a.window > 0 && key + kTile <= low - a.window + 1)) return;  // nothing that the wave's rows see
-        const f16x8* f = s_frag + buf * (kK + kV) * 64 + lane;
-        f32x4 S[NT][4];
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int t = 0; t < 4; t++) S[n][t] = f32x4{0, 0, 0, 0};
-        // Fragments are read four ahead of the products that take them, so that LDS answers meanwhile; the four are of two
-        // 16-key products (of two dim tiles), so that 2 NT sums take turns and none waits for its own last product.
-        f16x8 frag[2][4];
-        const auto fetch = [&](int j) __attribute__((always_inline)) {  // group j: K's [t pair][h], then V's [dt pair]
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int at = j < kK / 4 ? ((2 * (j / NH) + (u >> 1)) * NH + j % NH) * 2 + (u & 1) : 4 * j + u;
-                frag[j & 1][u] = f[at * 64];
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        fetch(0);
-#pragma unroll
-        for (int j = 0; j < kK / 4; j++) {
-            if (j + 1 < kK / 4) fetch(j + 1);
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int p = 0; p < NP; p++)
-#pragma unroll
-                    for (int u = 0; u < 2; u++)
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            const int t = 2 * (j / NH) + u;
-                            S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(frag[j & 1][2 * u + s], q[n][p][j % NH][s], S[n][t], 0, 0, 0);
-                        }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        f16x8 p[NT][NP][2];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int k0l = key + 16 * g;
-            const int hi = min(row[n].pos - k0l + 1, keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
-            const bool masked = __any(hi < 16 || lo > 0);
-            const float alpha = tile_softmax<NP>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], l[n], p[n]);
-            if (__any(alpha != 1.0f)) {
-#pragma unroll
-                for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
-            }
-        }
-        fetch(kK / 4);
-#pragma unroll
-        for (int j = kK / 4; j < (kK + kV) / 4; j++) {
-            if (j + 1 < (kK + kV) / 4) fetch(j + 1);
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int e = 0; e < NP; e++)
-#pragma unroll
-                    for (int u = 0; u < 2; u++)
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            const int dt = 2 * (j - kK / 4) + u;
-                            o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(frag[j & 1][2 * u + s], p[n][e][s], o[n][dt], 0, 0, 0);
-                        }
-            __builtin_amdgcn_sched_barrier(0);
-        }
+    const auto stage = [&](f16x8* f, int i) __attribute__((always_inline)) {  // load i of the NH + VJ
+        f16x8 x, z;
+        const int at = i < NH ? (wave * NH + i) * 2 : kK + (wave + 4 * (i - NH)) * 2;
+        codes_f16<FMT>(i < NH ? ck[i < NH ? i : 0] : cv[i < NH ? 0 : i - NH], x, z);
+        f[at * 64] = x;
+        f[(at + 1) * 64] = z;
     };
     if (first < end) {
-        int buf = 0;
-        int32_t key = first;
-        look(key);
-        load(key);
-        stage(0);
-        const auto scales = [&](int32_t at) __attribute__((always_inline)) {
+        const auto scales = [&](int32_t key) __attribute__((always_inline)) {
             TileScale sc = tile_scale(a.c, next, ksn, vsn);
             // in registers of their own, or the next scales' arrival is waited for to move them
             asm volatile("" : "+v"(sc.k), "+v"(sc.ev), "+v"(sc.down));
-            if (next.bad && wave == 0) raise_block(a.c, r.first, r.slot, at + 16 * g, next.id);
+            if (next.bad && wave == 0) raise_block(a.c, r.first, r.slot, min(key, border) + 16 * g, next.id);
             return sc;
         };
-        for (; key + kTile < end; key += kTile) {
-            const TileScale sc = scales(key);
-            const int32_t keys = next.keys;
-            __builtin_amdgcn_sched_barrier(0);
-            load(key + kTile);
-            __builtin_amdgcn_sched_barrier(0);
+        look(first);
+        load(first);
+        clip();
+#pragma unroll
+        for (int i = 0; i < NH + VJ; i++) stage(s_frag + lane, i);
+        TileScale sc = scales(first);
+        int32_t keys = next.keys;
+        load(first + kTile);
+        int buf = 0;
+        for (int32_t key = first; key < end; key += kTile, buf ^= 1) {
+            const f16x8* f = s_frag + buf * (kK + kV) * 64 + lane;
+            f16x8* g2 = s_frag + (buf ^ 1) * (kK + kV) * 64 + lane;
+            clip();
             __syncthreads();
-            compute(key, buf, sc, keys);
-            buf ^= 1;
-            stage(buf);
+            // Matrix and vector instructions are put in turns by hand: a wave issues in order, and while one product runs,
+            // a few conversions (of the next tile) or exponentials (of the second half of the keys) fit in its shadow.
+            // Fragments are read four ahead of their products, of two 16-key products (of all dim tiles) in turns, so that no
+            // sum waits for its own last product.
+            f32x4 S[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int t = 0; t < 4; t++) S[n][t] = f32x4{0, 0, 0, 0};
+            constexpr int R = 5;  // fragments held: the one in use and four on their way
+            f16x8 ring[R];
+            const auto fetch = [&](int i) __attribute__((always_inline)) {  // K's [t pair][h][s][t], then V's [s][dt]
+                const int j = i / 4, v = i - kK;
+                const int at = i < kK ? ((2 * (j / NH) + (i & 1)) * NH + j % NH) * 2 + ((i >> 1) & 1) : kK + v % ND * 2 + v / ND;
+                ring[i % R] = f[at * 64];
+            };
+#pragma unroll
+            for (int i = 0; i < R - 1; i++) fetch(i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < kK; i++) {
+                const int j = i / 4, t = 2 * (j / NH) + (i & 1), s = (i >> 1) & 1;
+                if (i + R - 1 < kK) fetch(i + R - 1);
+#pragma unroll
+                for (int p = 0; p < NP; p++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[i % R], q[n][p][j % NH][s], S[n][t], 0, 0, 0);
+                if (i % (kK / (NH + VJ)) == 0 && i / (kK / (NH + VJ)) < NH + VJ) stage(g2, i / (kK / (NH + VJ)));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const TileScale sn = scales(key + kTile);
+            const int32_t keys_next = next.keys;
+            __builtin_amdgcn_sched_barrier(0);
+            load(key + 2 * kTile);
+            __builtin_amdgcn_sched_barrier(0);
+            TileRow t[NT];
+            float alpha[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const int k0l = key + 16 * g;
+                const int hi = min(row[n].pos - k0l + 1, keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
+                const bool masked = __any(hi < 16 || lo > 0);
+                alpha[n] = tile_max<RESHAPED>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], t[n]);
+                if (__any(alpha[n] != 1.0f)) {
+#pragma unroll
+                    for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha[n];
+                }
+            }
+            f16x8 p[NT][NP][2];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < R - 1; i++) fetch(kK + i);
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) tile_weights<NP>(t[n], 0, j, p[n]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < kV; i++) {
+                const int s = i / ND, dt = i % ND;
+                if (i + R - 1 < kV) fetch(kK + i + R - 1);
+#pragma unroll
+                for (int e = 0; e < NP; e++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) o[n][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[(kK + i) % R], p[n][e][s], o[n][dt], 0, 0, 0);
+                // the other half's weights, 4 NT pairs over the turns of the first half
+#pragma unroll
+                for (int w = 0; w < 4 * NT; w++)
+                    if (s == 0 && w * ND / (4 * NT) == dt) tile_weights<NP>(t[w % NT], 1, 2 * (w / NT), p[w % NT]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) l[n] = fmaf(t[n].sum, sc.down, l[n] * alpha[n]);
+            sc = sn;
+            keys = keys_next;
         }
-        const TileScale sc = scales(key);
-        __syncthreads();
-        compute(key, buf, sc, next.keys);
     }
     float* part = a.part2 + index * Partial<DP, 4 * NT>::kFloats;
 #pragma unroll
@@ -1082,18 +1086,18 @@ struct Kv8AttnPlan {
 };
 
 // Thread blocks of the many-row tiles, then of the few-row work: one launch, so that neither waits for the other's end.
-template <int DT, int FMT, int DP, int NT, int NB>
+template <int DT, int FMT, int DP, int NT, int NB, bool RESHAPED>
 __global__ __launch_bounds__(256, DP == 256 || NT == 2 ? 1 : 2) void kv8_attn(Kv8AttnArgs a)
 {
     extern __shared__ __align__(16) char lds[];
     if constexpr (NT > 0 && NB > 0) {
         const unsigned blocks = gridDim.x - a.workers;
-        if (blockIdx.x < blocks) attn_blocks<DT, FMT, DP, NB>(a, blockIdx.x, lds);
-        else attn_waves<DT, FMT, DP, NT>(a, blockIdx.x - blocks, lds);
+        if (blockIdx.x < blocks) attn_blocks<DT, FMT, DP, NB, RESHAPED>(a, blockIdx.x, lds);
+        else attn_waves<DT, FMT, DP, NT, RESHAPED>(a, blockIdx.x - blocks, lds);
     } else if constexpr (NT > 0) {
-        attn_waves<DT, FMT, DP, NT>(a, blockIdx.x, lds);
+        attn_waves<DT, FMT, DP, NT, RESHAPED>(a, blockIdx.x, lds);
     } else {
-        attn_blocks<DT, FMT, DP, NB>(a, blockIdx.x, lds);
+        attn_blocks<DT, FMT, DP, NB, RESHAPED>(a, blockIdx.x, lds);
     }
 }
 
@@ -1104,24 +1108,24 @@ __global__ __launch_bounds__(256) void kv8_attn_join(Kv8AttnArgs a, int64_t wave
     else join_blocks<DT, DP, 4 * NB>(a, blockIdx.x - wave_joins);
 }
 
-template <int DT, int FMT> int kv8_attn_launch(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st);
+template <int DT, int FMT, bool RESHAPED> int kv8_attn_launch(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st);
 
-template <int DT, int FMT, int DP, int NT, int NB> static int kv8_attn_start(const Kv8AttnArgs& a, hipStream_t st)
+template <int DT, int FMT, int DP, int NT, int NB, bool RESHAPED> static int kv8_attn_start(const Kv8AttnArgs& a, hipStream_t st)
 {
     constexpr int waves = NT > 0 ? waves_lds<DP, NT ? NT : 1>() : 0, blocks = NB > 0 ? blocks_lds<DP>() : 0, lds = waves > blocks ? waves : blocks;
-    const auto kernel = kv8_attn<DT, FMT, DP, NT, NB>;
+    const auto kernel = kv8_attn<DT, FMT, DP, NT, NB, RESHAPED>;
     if (lds > 65536) SLHIP_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     const int64_t grid = (NT > 0 ? a.workers : 0) + (NB > 0 ? a.items * a.splits * a.c.heads : 0);
     kernel<<<static_cast<unsigned>(grid), 256, lds, st>>>(a);
     return check_launch("kv8_attn");
 }
 
-template <int DT, int FMT, int DP> static int kv8_attn_run(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
+template <int DT, int FMT, int DP, bool RESHAPED> static int kv8_attn_run(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
 {
     constexpr int NB = block_tiles(DT == SLHIP_F32, DP), NT2 = DP <= 128 ? 2 : 1;  // make_plan asks for two up to 128 dims
     int e;
-    if (p.blocks) e = p.wave_tiles ? kv8_attn_start<DT, FMT, DP, 1, NB>(a, st) : kv8_attn_start<DT, FMT, DP, 0, NB>(a, st);
-    else e = p.wave_tiles == 1 ? kv8_attn_start<DT, FMT, DP, 1, 0>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0>(a, st);
+    if (p.blocks) e = p.wave_tiles ? kv8_attn_start<DT, FMT, DP, 1, NB, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, 0, NB, RESHAPED>(a, st);
+    else e = p.wave_tiles == 1 ? kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED>(a, st);
     if (e) return e;
     const int64_t waves = p.wave_tiles ? static_cast<int64_t>(a.c.B) * a.c.heads * p.wave_tiles * (p.by_part ? DP / 16 : 1) : 0;
     const int64_t blocks = p.blocks && a.splits > 1 ? a.items * a.c.heads * 4 * NB : 0;
@@ -1138,11 +1142,11 @@ template <int DT, int FMT, int DP> static int kv8_attn_run(const Kv8AttnArgs& a,
     return check_launch("kv8_attn_join");
 }
 
-template <int DT, int FMT> int kv8_attn_by_dim(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
+template <int DT, int FMT, bool RESHAPED> int kv8_attn_by_dim(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
 {
-    if (a.c.D <= 64) return kv8_attn_run<DT, FMT, 64>(a, p, st);
-    if (a.c.D <= 128) return kv8_attn_run<DT, FMT, 128>(a, p, st);
-    return kv8_attn_run<DT, FMT, 256>(a, p, st);
+    if (a.c.D <= 64) return kv8_attn_run<DT, FMT, 64, RESHAPED>(a, p, st);
+    if (a.c.D <= 128) return kv8_attn_run<DT, FMT, 128, RESHAPED>(a, p, st);
+    return kv8_attn_run<DT, FMT, 256, RESHAPED>(a, p, st);
 }
 
 }  // namespace slhip
