@@ -9,8 +9,7 @@ namespace slhip {
 struct Kv8Dev {
     uint8_t *k, *v;
     float *ks, *vs;
-    int64_t blocks;
-    int32_t shift, heads, D;  // log2(block_size)
+    int32_t blocks, shift, heads, D;  // shift: log2(block_size)
     int32_t B;
     int64_t T;
     const int32_t *starts, *past, *slots, *pages;
@@ -51,26 +50,46 @@ __device__ __forceinline__ void raise_block(const Kv8Dev& d, int32_t row, int32_
 {
     const int64_t v = block;
     raise_error(d.err, kErrCacheBlock, row, slot, pos, static_cast<uint32_t>(v), static_cast<uint32_t>(static_cast<uint64_t>(v) >> 32),
-                static_cast<uint32_t>(d.blocks << d.shift));
+                static_cast<uint32_t>(static_cast<int64_t>(d.blocks) << d.shift));
 }
 
-// item_request by a whole wave: 64 requests are looked at a step, so 4096 take two dependent loads. Wave-uniform.
-__device__ __forceinline__ int32_t kv8_find(const Kv8Dev& d, int64_t item, int64_t tile, int64_t extra)
+// The request of an item, and which of its items that is.
+struct Kv8Item {
+    int32_t i;
+    int64_t piece;  // below 0 or past the request's pieces where there is nothing to do
+    Kv8Request r;
+};
+
+// item_request by a whole wave: 64 requests are looked at a step, and the last step brings the request itself, so up to 64
+// take one memory latency and 4096 two. Wave-uniform.
+__device__ __forceinline__ Kv8Item kv8_find(const Kv8Dev& d, int64_t item, int64_t tile, int64_t extra)
 {
     int32_t lo = 0, n = d.B;
     const int lane = threadIdx.x & 63;
-    for (;;) {
-        const int32_t step = (n + 63) / 64;
-        const int32_t i = lo + lane * step;
+    while (n > 64) {
+        const int32_t step = (n + 63) / 64, i = lo + lane * step;
         const bool under = i < lo + n && item_base(d.starts[i < lo + n ? i : lo], i, tile, extra) <= item;
         const int32_t k = __popcll(__ballot(under));
         if (k > 0) {
             lo += (k - 1) * step;
             n -= (k - 1) * step;
         }
-        if (step == 1) return __builtin_amdgcn_readfirstlane(lo);
         n = min(n, step);
     }
+    const int32_t i = lo + (lane < n ? lane : 0);
+    const Kv8Request mine = kv8_request(d, i);
+    const int32_t start = d.starts[i];
+    const int32_t k = max(__popcll(__ballot(lane < n && item_base(start, i, tile, extra) <= item)) - 1, 0);
+    Kv8Item f;
+    f.i = __builtin_amdgcn_readfirstlane(lo) + k;
+    f.piece = item - item_base(__builtin_amdgcn_readlane(start, k), f.i, tile, extra);
+    f.r.first = __builtin_amdgcn_readlane(mine.first, k);
+    f.r.n = __builtin_amdgcn_readlane(mine.n, k);
+    f.r.past = __builtin_amdgcn_readlane(mine.past, k);
+    f.r.slot = __builtin_amdgcn_readlane(mine.slot, k);
+    f.r.bad = __builtin_amdgcn_readlane(static_cast<int>(mine.bad), k) != 0;
+    f.r.table = d.pages + (f.r.bad ? 0 : f.r.slot * d.bps);
+    return f;
 }
 
 template <int DT> __device__ __forceinline__ float4 load4f(const void* p, int64_t i)

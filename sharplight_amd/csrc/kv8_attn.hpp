@@ -115,31 +115,58 @@ __device__ __forceinline__ float row_sum(float v)
 
 // ---- a lane's key blocks -----------------------------------------------------------------------------------------
 
-// A sub-block of 16 keys from `key`: its block, or block 0 and no keys where there is none to see.
+// A sub-block of 16 keys: where its codes are in the cache, or block 0's and no keys where there is none to see.
 struct SubBlock {
-    int64_t at;    // (block * heads + head) of the scales
-    int32_t sub;   // which 16 keys of the block
+    uint32_t id;   // the block
+    int32_t sub;   // which 16 keys of it
     int32_t keys;  // how many are below `end`
-    int32_t bad;   // a block id outside the cache (0 where it is fine: -1 is bad, too)
-    int32_t id;
+    int32_t bad;   // the table's entry is no block of the cache (it is in `entry`)
+    int32_t entry;
 };
 
 // The table entry of the sub-block at `key` (another of the request's where the key is behind `end`).
 __device__ __forceinline__ int32_t block_id(const Kv8Dev& c, const int32_t* table, int32_t key, int32_t end)
 {
-    return table[min(key, end - 1) >> c.shift];
+    return table[static_cast<uint32_t>(min(key, end - 1)) >> c.shift];
 }
 
-__device__ __forceinline__ SubBlock sub_block(const Kv8Dev& c, int32_t id, int32_t head, int32_t key, int32_t end)
+__device__ __forceinline__ SubBlock sub_block(const Kv8Dev& c, int32_t entry, int32_t key, int32_t end)
 {
     SubBlock s;
-    const bool here = key < end, fine = id >= 0 && id < c.blocks;
-    s.id = id;
+    const bool here = key < end, fine = static_cast<uint32_t>(entry) < static_cast<uint32_t>(c.blocks);
+    s.entry = entry;
     s.bad = here && !fine;
-    s.at = static_cast<int64_t>(here && fine ? id : 0) * c.heads + head;
+    s.id = here && fine ? entry : 0;
     s.sub = (key >> 4) & ((1 << (c.shift - 4)) - 1);
     s.keys = here && fine ? min(end - key, 16) : 0;
     return s;
+}
+
+// A K/V head's codes and scales of block 0, and the bytes from a block to the next.
+struct HeadBase {
+    const uint8_t *k, *v, *ks, *vs;
+    uint32_t codes, scales;
+    uint32_t slab;  // bytes of 16 keys
+};
+
+__device__ __forceinline__ HeadBase head_base(const Kv8Dev& c, int32_t head)
+{
+    HeadBase h;
+    h.slab = 16 * c.D;
+    const uint32_t codes = h.slab << (c.shift - 4);  // of a block's head: at most 2^16
+    h.k = c.k + static_cast<int64_t>(head) * codes;
+    h.v = c.v + static_cast<int64_t>(head) * codes;
+    h.ks = reinterpret_cast<const uint8_t*>(c.ks + head);
+    h.vs = reinterpret_cast<const uint8_t*>(c.vs + head);
+    h.codes = c.heads * codes;
+    h.scales = c.heads * 4;
+    return h;
+}
+
+// Byte offset of a sub-block's codes from HeadBase::k or ::v.
+__device__ __forceinline__ uint64_t codes_at(const HeadBase& h, const SubBlock& s)
+{
+    return static_cast<uint64_t>(s.id) * h.codes + __umul24(s.sub, h.slab);
 }
 
 // ---- rows -------------------------------------------------------------------------------------------------------
@@ -558,17 +585,19 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
         vid = block_id(a.c, s.table, key + 16 * g, s.end);
     };
     const auto aim = [&](const Segment& s, int32_t key) __attribute__((always_inline)) {  // K's codes and the scales of the tile at `key`; where V's codes are
-        const SubBlock kb = sub_block(a.c, kid, s.head, key + 16 * (c >> 2), s.end);
-        vb = sub_block(a.c, vid, s.head, key + 16 * g, s.end);
-        const uint8_t* kp = a.c.k + ((kb.at << a.c.shift) + kb.sub * 16 + (c & 3)) * D;
+        const HeadBase base = head_base(a.c, s.head);
+        const SubBlock kb = sub_block(a.c, kid, key + 16 * (c >> 2), s.end);
+        vb = sub_block(a.c, vid, key + 16 * g, s.end);
+        const uint8_t* kp = base.k + codes_at(base, kb) + (c & 3) * D;
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int h = 0; h < NH; h++)  // dims past D: any codes, q is 0 there
                 k[t][h] = *reinterpret_cast<const uint4*>(kp + 4 * t * D + (64 * h + 16 * g < D ? 64 * h + 16 * g : 0));
-        ks = a.c.ks[vb.at];
-        vs = a.c.vs[vb.at];
-        vp = a.c.v + ((vb.at << a.c.shift) + vb.sub * 16) * D + c * 16;
+        const uint64_t at = static_cast<uint64_t>(vb.id) * base.scales;
+        ks = *reinterpret_cast<const float*>(base.ks + at);
+        vs = *reinterpret_cast<const float*>(base.vs + at);
+        vp = base.v + codes_at(base, vb) + c * 16;
         look(s, key + 4 * kTile);
     };
     const auto load_v = [&]() __attribute__((always_inline)) {
@@ -630,7 +659,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
                 }
             TileScale sc = tile_scale(a.c, vb, ks, vs);
             const int32_t keys = vb.keys;
-            if (vb.bad) raise_block(a.c, r.first, r.slot, key + 16 * g, vb.id);
+            if (vb.bad) raise_block(a.c, r.first, r.slot, key + 16 * g, vb.entry);
             if constexpr (more) {
                 // scales in registers of their own, or the next ones' arrival is waited for to move them
                 asm volatile("" : "+v"(sc.k), "+v"(sc.ev), "+v"(sc.down));
@@ -839,9 +868,9 @@ template <int DT, int DP, int NT> __device__ __forceinline__ void join_blocks(co
     index /= NT;
     const int32_t head = static_cast<int32_t>(index % a.c.heads);
     const int64_t back = index / a.c.heads, item = a.items - 1 - back;
-    const int32_t i = kv8_find(a.c, item, a.tile_tokens, 1);
-    const Kv8Request r = kv8_request(a.c, i);
-    const int64_t t0 = (item - item_base(a.c.starts[i], i, a.tile_tokens, 1)) * a.tile_tokens;
+    const Kv8Item it = kv8_find(a.c, item, a.tile_tokens, 1);
+    const Kv8Request& r = it.r;
+    const int64_t t0 = it.piece * a.tile_tokens;
     if (t0 < 0 || t0 >= r.n || static_cast<int64_t>(r.n) * a.G <= a.block_min || static_cast<int64_t>(r.n) * a.G > a.block_max) return;
     const int32_t row0 = static_cast<int32_t>(t0) * a.G, row1 = static_cast<int32_t>(min(static_cast<int64_t>(r.n), t0 + a.tile_tokens)) * a.G;
     if (row0 + 16 * n >= row1) return;
@@ -875,13 +904,13 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
     const int32_t split = static_cast<int32_t>(rest % a.splits);
     // tiles from the last: their key ranges are the longest, and short ones fill the end
     const int64_t item = a.items - 1 - rest / a.splits;
-    const int32_t i = kv8_find(a.c, item, a.tile_tokens, 1);
-    const Kv8Request r = kv8_request(a.c, i);
-    const int64_t t0 = (item - item_base(a.c.starts[i], i, a.tile_tokens, 1)) * a.tile_tokens;
-    if (r.bad && t0 == 0 && head == 0 && split == 0 && threadIdx.x == 0) raise_request(a.c, i, r);
+    const Kv8Item it = kv8_find(a.c, item, a.tile_tokens, 1);
+    const Kv8Request& r = it.r;
+    const int64_t t0 = it.piece * a.tile_tokens;
+    if (r.bad && t0 == 0 && head == 0 && split == 0 && threadIdx.x == 0) raise_request(a.c, it.i, r);
     if (t0 < 0 || t0 >= r.n || static_cast<int64_t>(r.n) * a.G <= a.block_min) return;
     if (static_cast<int64_t>(r.n) * a.G > a.block_max) {
-        if (t0 == 0 && head == 0 && split == 0 && threadIdx.x == 0) raise_request(a.c, i, r);
+        if (t0 == 0 && head == 0 && split == 0 && threadIdx.x == 0) raise_request(a.c, it.i, r);
         return;
     }
     const int32_t t1 = min(static_cast<int64_t>(r.n), t0 + a.tile_tokens);
@@ -919,6 +948,10 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
     SubBlock next;
     float ksn, vsn;
     int32_t kid, vid;
+    const HeadBase base = head_base(a.c, head);
+    // the lane's first codes in a sub-block (dims past D: any codes, q is 0 there and the sums are not stored)
+    const uint8_t* const kbase = base.k + (4 * wave + (c & 3)) * D + (16 * g < D ? 16 * g : 0);
+    const uint8_t* const vbase = base.v + (16 * wave < D ? 256 * wave : 0) + c * 16;
     const int32_t border = first + ((end - first - 1) & ~(kTile - 1));  // the last tile
     const auto look = [&](int32_t key) __attribute__((always_inline)) {
         key = min(key, border);
@@ -927,19 +960,17 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
     };
     const auto load = [&](int32_t key) __attribute__((always_inline)) {
         const int32_t at = min(key, border);
-        const SubBlock kb = sub_block(a.c, kid, head, at + 16 * (c >> 2), all);
-        next = sub_block(a.c, vid, head, at + 16 * g, all);
-        const uint8_t* k = a.c.k + ((kb.at << a.c.shift) + kb.sub * 16 + 4 * wave + (c & 3)) * D;
+        const SubBlock kb = sub_block(a.c, kid, at + 16 * (c >> 2), all);
+        next = sub_block(a.c, vid, at + 16 * g, all);
+        const uint8_t* k = kbase + codes_at(base, kb);
 #pragma unroll
-        for (int h = 0; h < NH; h++) ck[h] = *reinterpret_cast<const uint4*>(k + (64 * h + 16 * g < D ? 64 * h + 16 * g : 0));
-        const uint8_t* v = a.c.v + ((next.at << a.c.shift) + next.sub * 16) * D + c * 16;
+        for (int h = 0; h < NH; h++) ck[h] = *reinterpret_cast<const uint4*>(k + (64 * h + 16 * g < D ? 64 * h : 0));
+        const uint8_t* v = vbase + codes_at(base, next);
 #pragma unroll
-        for (int j = 0; j < VJ; j++) {
-            const int dt = wave + 4 * j;
-            cv[j] = *reinterpret_cast<const uint4*>(v + (16 * dt < D ? 256 * dt : 0));
-        }
-        ksn = a.c.ks[next.at];
-        vsn = a.c.vs[next.at];
+        for (int j = 0; j < VJ; j++) cv[j] = *reinterpret_cast<const uint4*>(v + (16 * (wave + 4 * j) < D ? 1024 * j : 0));
+        const uint64_t scales = static_cast<uint64_t>(next.id) * base.scales;
+        ksn = *reinterpret_cast<const float*>(base.ks + scales);
+        vsn = *reinterpret_cast<const float*>(base.vs + scales);
         look(key + kTile);
     };
     const auto clip = [&]() __attribute__((always_inline)) {  // V's codes of keys that are not there
@@ -960,7 +991,7 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
             TileScale sc = tile_scale(a.c, next, ksn, vsn);
             // in registers of their own, or the next scales' arrival is waited for to move them
             asm volatile("" : "+v"(sc.k), "+v"(sc.ev), "+v"(sc.down));
-            if (next.bad && wave == 0) raise_block(a.c, r.first, r.slot, min(key, border) + 16 * g, next.id);
+            if (next.bad && wave == 0) raise_block(a.c, r.first, r.slot, min(key, border) + 16 * g, next.entry);
             return sc;
         };
         look(first);

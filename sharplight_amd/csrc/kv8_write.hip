@@ -88,20 +88,15 @@ __global__ __launch_bounds__(1024) void kv8_write(Kv8WriteArgs a)
     __shared__ uint32_t s_max[16];
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int bs = 1 << c.shift, wpi = bs >> 4;  // waves per item
-    const int32_t i = kv8_find(c, blockIdx.x, a.tile, a.extra);
-    const Kv8Request r = kv8_request(c, i);
-    const int64_t piece = blockIdx.x - item_base(c.starts[i], i, a.tile, a.extra);
+    const Kv8Item it = kv8_find(c, blockIdx.x, a.tile, a.extra);
+    const Kv8Request& r = it.r;
     const int pair = static_cast<int>(blockIdx.y) * (static_cast<int>(blockDim.x >> 6) / wpi) + wave / wpi, sub = wave % wpi;
-    if (r.bad && piece == 0 && blockIdx.y == 0 && threadIdx.x == 0) raise_request(c, i, r);
+    if (r.bad && it.piece == 0 && blockIdx.y == 0 && threadIdx.x == 0) raise_request(c, it.i, r);
     // everything above is the same for all of the thread block: nothing is left waiting at the barrier below
     const int b0 = r.past >> c.shift;
-    if (r.n == 0 || piece < 0 || piece > ((r.past + r.n - 1) >> c.shift) - b0) return;
-    const int tb = b0 + static_cast<int>(piece), p0 = tb << c.shift;  // the block's place in the table, its first position
-    const int32_t block = r.table[tb];
-    if (block < 0 || block >= c.blocks) {
-        if (threadIdx.x == 0 && blockIdx.y == 0) raise_block(c, r.first, r.slot, max(p0, r.past), block);
-        return;
-    }
+    if (r.n == 0 || it.piece < 0 || it.piece > ((r.past + r.n - 1) >> c.shift) - b0) return;
+    const int tb = b0 + static_cast<int>(it.piece), p0 = tb << c.shift;  // the block's place in the table, its first position
+    const int32_t block = r.table[tb];  // (on its way while the values are)
     const bool mine = pair < 2 * c.heads;
     const int kv = pair & 1, head = mine ? pair >> 1 : 0, D = c.D;
     const bool fresh = r.past <= p0;
@@ -117,6 +112,7 @@ __global__ __launch_bounds__(1024) void kv8_write(Kv8WriteArgs a)
     uint32_t top = 0;
     if (mine && nb > na) {
         if (kv == 0) {
+#pragma unroll
             for (int o = 0; o < KR; o++) {
                 const int at = (lane + 64 * o) * 8, t = at / D, d = at % D;  // D values a token, 16 tokens
                 const bool in = t >= na && t < nb;
@@ -135,11 +131,12 @@ __global__ __launch_bounds__(1024) void kv8_write(Kv8WriteArgs a)
                     }
                     f[8 * o + j] = w.x; f[8 * o + j + 1] = w.y; f[8 * o + j + 2] = w.z; f[8 * o + j + 3] = w.w;
                 }
-                for (int j = 0; j < 8; j++) top = max(top, abs_bits(f[8 * o + j]));
             }
         } else {
+#pragma unroll
             for (int o = 0; o < VR; o++) {
                 const int d = 2 * (lane + 64 * o);
+#pragma unroll
                 for (int t = 0; t < 16; t++) {
                     float lo = 0, hi = 0;
                     if (d < D && t >= na && t < nb) {
@@ -159,14 +156,30 @@ __global__ __launch_bounds__(1024) void kv8_write(Kv8WriteArgs a)
                     }
                     f[32 * o + t] = lo;
                     f[32 * o + 16 + t] = hi;
-                    top = max(top, max(abs_bits(lo), abs_bits(hi)));
                 }
             }
         }
     }
+    if (block < 0 || block >= c.blocks) {  // the same for all of the thread block
+        if (threadIdx.x == 0 && blockIdx.y == 0) raise_block(c, r.first, r.slot, max(p0, r.past), block);
+        return;
+    }
     float* sp = (kv ? c.vs : c.ks) + static_cast<int64_t>(block) * c.heads + head;
     const float s0 = fresh ? 0.0f : *sp;
-    top = wave_umax(top);
+    uint8_t* base = (kv ? c.v : c.k) + ((static_cast<int64_t>(block) * c.heads + head) * bs + sub * 16) * D;
+    uint4 was[VR][2];  // V's codes that are there already
+    if (mine && kv == 1 && !fresh) {
+#pragma unroll
+        for (int o = 0; o < VR; o++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) was[o][e] = *reinterpret_cast<const uint4*>(base + (2 * (lane + 64 * o) < D ? 2 * (lane + 64 * o) + e : 0) * 16);
+    }
+    if (mine && nb > na) {
+#pragma unroll
+        for (int j = 0; j < static_cast<int>(sizeof f / sizeof f[0]); j++)
+            if (j < (kv == 0 ? KR * 8 : VR * 32)) top = max(top, abs_bits(f[j]));
+        top = wave_umax(top);
+    }
     if (wpi > 1) {
         if (lane == 0) s_max[wave] = top;
         __syncthreads();
@@ -182,8 +195,8 @@ __global__ __launch_bounds__(1024) void kv8_write(Kv8WriteArgs a)
     if (!fresh && !grew && nb <= na) return;
     if (lost)
         for (float& v : f) v = 0.0f;
-    uint8_t* base = (kv ? c.v : c.k) + ((static_cast<int64_t>(block) * c.heads + head) * bs + sub * 16) * D;
     if (kv == 0) {
+#pragma unroll
         for (int o = 0; o < KR; o++) {
             const int at = (lane + 64 * o) * 8, t = at / D;
             if (t >= 16) continue;
@@ -201,15 +214,16 @@ __global__ __launch_bounds__(1024) void kv8_write(Kv8WriteArgs a)
             }
         }
     } else {
+#pragma unroll
         for (int o = 0; o < VR; o++) {
             const int d = 2 * (lane + 64 * o);
             if (d >= D) continue;
+#pragma unroll
             for (int e = 0; e < 2; e++) {
                 uint4* p = reinterpret_cast<uint4*>(base + (d + e) * 16);
                 uint32_t w[4] = {0, 0, 0, 0};
                 if (!fresh) {
-                    const uint4 was = *p;
-                    w[0] = was.x; w[1] = was.y; w[2] = was.z; w[3] = was.w;
+                    w[0] = was[o][e].x; w[1] = was[o][e].y; w[2] = was[o][e].z; w[3] = was[o][e].w;
                 }
                 for (int j = 0; j < 4; j++) {
                     if (grew) {
@@ -248,7 +262,7 @@ int make_kv8(const char* op, const slhip_kv8_cache* c, const slhip_kv8_batch* b,
         if (!aligned16(c->k) || !aligned16(c->v)) return fail(SLHIP_ERR_INVALID, "%s: codes must be 16-byte aligned", op);
         if (c->blocks == 0) return fail(SLHIP_ERR_INVALID, "%s: the cache has no blocks", op);
     }
-    *out = Kv8Dev{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), c->k_scale, c->v_scale, c->blocks, shift,
+    *out = Kv8Dev{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), c->k_scale, c->v_scale, static_cast<int32_t>(c->blocks), shift,
                   static_cast<int32_t>(c->heads), static_cast<int32_t>(c->head_dim), static_cast<int32_t>(b->requests), b->tokens,
                   b->starts, b->past, b->slots, b->pages, b->page_slots, b->blocks_per_slot, nullptr};
     return SLHIP_OK;
