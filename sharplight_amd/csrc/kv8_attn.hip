@@ -19,6 +19,8 @@ template <int DT, int FMT> static int launch(const Kv8AttnArgs& a, const Kv8Attn
     return reshaped ? kv8_attn_launch<DT, FMT, true>(a, p, st) : kv8_attn_launch<DT, FMT, false>(a, p, st);
 }
 
+constexpr int64_t kWorkers = 512;     // two thread blocks a CU (one of 256 dims)
+constexpr int64_t kDirectRounds = 4;
 constexpr int64_t kBlockUnits = 512;  // row tiles and key ranges of the many-row work, over all heads
 constexpr int64_t kMaxSplits = 64;
 
@@ -43,10 +45,14 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
     a->block_min = static_cast<int32_t>(few);
     a->block_max = static_cast<int32_t>(limit);
     int64_t bytes = 0;
+    a->direct = false;
     if (p->wave_tiles) {
-        a->workers = getenv("KV8_W") ? atoi(getenv("KV8_W")) : dp == 256 ? 256 : 512;
+        // Contexts that cannot be longer than kDirectRounds rounds are not worth a second launch: a few of them get a thread
+        // block for each head.
+        a->direct = B * heads <= kWorkers && c.bps << c.shift <= kDirectRounds * 4 * kTile;
+        a->workers = static_cast<int32_t>(a->direct ? B * heads : dp == 256 ? kWorkers / 2 : kWorkers);
         p->by_part = B * heads < 256;
-        bytes += 2 * a->workers * (few * dp + few * 2) * 4;
+        if (!a->direct) bytes += 2 * a->workers * (few * dp + few * 2) * 4;
     }
     a->splits = 1;
     if (p->blocks) {

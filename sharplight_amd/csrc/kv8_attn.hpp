@@ -53,6 +53,7 @@ struct Kv8AttnArgs {
     bool strict;                   // requests above max_rows are an error (nothing else takes them)
     int32_t block_min, block_max;  // many-row tiles: requests of (block_min, block_max] rows; above is an error
     int32_t workers;             // few-row thread blocks
+    bool direct;                 // one for each request's head, which share nothing
     int32_t tile_tokens, splits; // many-row tiles: tokens of a tile, key ranges it is cut into
     int64_t items;               // many-row tiles of a head
     float *part, *part2;         // sums of key ranges: of workers, of splits
@@ -420,18 +421,6 @@ __device__ __forceinline__ int32_t request_steps(const Kv8AttnArgs& a, const Kv8
     return (end - first + 4 * kTile - 1) / (4 * kTile) + kStart;
 }
 
-// Inclusive sums over the wave: shifts within rows of 16 lanes, then each row's total into those after it.
-__device__ __forceinline__ int32_t wave_scan(int32_t v)
-{
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);  // row_shr:8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31
-    return v;
-}
-
 constexpr int kMaxGroups = 65536 / 64;  // of 64 requests
 
 // The line, and on it the request of worker `at` (of request `at` itself if BY_REQUEST). The requests are taken in groups of
@@ -511,14 +500,12 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
     f32x4* s_o = reinterpret_cast<f32x4*>(lds);                                       // [2][NT * ND * 64]
     float2* s_ml = reinterpret_cast<float2*>(lds + 2 * NT * ND * 64 * sizeof(f32x4));  // [4][NT * 16]
     const int lane = threadIdx.x & 63, wave = wave_id(), c = lane & 15, g = lane >> 4, D = a.c.D;
-    const Line line = find_line<false>(a, worker);
-    if (worker == a.workers - 1) {  // the one with the least to do
+    if (worker == a.workers - 1) {  // (of a shared line, the one with the least to do)
         for (int i = threadIdx.x; i < a.c.B; i += 256) {
             const Kv8Request r = kv8_request(a.c, i);
             if (r.bad || (a.strict && static_cast<int64_t>(r.n) * a.G > a.max_rows)) raise_request(a.c, i, r);
         }
     }
-    if (line.request < 0) return;
 
     // A head's share of the piece, and what its loads go by.
     struct Segment {
@@ -530,9 +517,29 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
         __device__ __forceinline__ void take(const Kv8Request& r) { table = r.table; row0 = r.first; n = r.n; past = r.past; slot = r.slot; }
         __device__ __forceinline__ Kv8Request request() const { return {row0, n, past, slot, false, table}; }
     } cur, next;
-    int64_t pos = worker * line.each;
-    const int64_t begin = pos, stop = min(pos + line.each, line.total);
-    int32_t step;
+    int64_t pos = 0, stop;  // on the line
+    int32_t step = 0;
+    if (a.direct) {
+        cur.i = worker / a.c.heads;
+        cur.head = worker - cur.i * a.c.heads;
+        const Kv8Request r = kv8_request(a.c, cur.i);
+        cur.take(r);
+        cur.steps = request_steps(a, r);
+        stop = cur.steps;
+    } else {
+        const Line line = find_line<false>(a, worker);
+        if (line.request < 0) return;
+        pos = worker * line.each;
+        stop = min(pos + line.each, line.total);
+        cur.i = line.request;
+        cur.take(line.r);
+        cur.steps = line.steps;
+        const int64_t in = pos - line.before * a.c.heads;
+        cur.head = static_cast<int32_t>(quotient(in, cur.steps));
+        step = static_cast<int32_t>(in - static_cast<int64_t>(cur.head) * cur.steps);
+    }
+    if (cur.steps == 0) return;
+    const int64_t begin = pos;
     // The share of the head that cur points at from `step` on; false if the piece ends before its rounds.
     const auto share = [&](Segment& s) __attribute__((always_inline)) {
         const int32_t until = static_cast<int32_t>(min(static_cast<int64_t>(s.steps), step + (stop - pos)));
@@ -562,12 +569,6 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
             if (share(s)) return true;
         }
     };
-    cur.take(line.r);
-    cur.i = line.request;
-    cur.steps = line.steps;
-    const int64_t in = pos - line.before * a.c.heads;
-    cur.head = static_cast<int32_t>(quotient(in, cur.steps));
-    step = static_cast<int32_t>(in - static_cast<int64_t>(cur.head) * cur.steps);
     if (!share(cur) && !advance(cur)) return;
 
     constexpr bool kEarly = DT != SLHIP_F32 && DP <= 128;  // (f32 queries and 256 dims leave no registers for that)
@@ -1158,7 +1159,7 @@ template <int DT, int FMT, int DP, bool RESHAPED> static int kv8_attn_run(const 
     if (p.blocks) e = p.wave_tiles ? kv8_attn_start<DT, FMT, DP, 1, NB, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, 0, NB, RESHAPED>(a, st);
     else e = p.wave_tiles == 1 ? kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED>(a, st);
     if (e) return e;
-    const int64_t waves = p.wave_tiles ? static_cast<int64_t>(a.c.B) * a.c.heads * p.wave_tiles * (p.by_part ? DP / 16 : 1) : 0;
+    const int64_t waves = p.wave_tiles && !a.direct ? static_cast<int64_t>(a.c.B) * a.c.heads * p.wave_tiles * (p.by_part ? DP / 16 : 1) : 0;
     const int64_t blocks = p.blocks && a.splits > 1 ? a.items * a.c.heads * 4 * NB : 0;
     if (waves + blocks == 0) return SLHIP_OK;
     if (waves + blocks > 0x7FFFFFFF) return fail(SLHIP_ERR_UNSUPPORTED, "kv8_attention: too many tiles");

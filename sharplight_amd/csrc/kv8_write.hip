@@ -21,6 +21,8 @@ struct Kv8WriteArgs {
     const void* x[2];
     int64_t st[2], sh[2];
     int64_t tile, extra;  // items by blocks (block_size, 2) or by tokens (1, 0)
+    int32_t chunks;       // D / 8, and its reciprocal: n / chunks = n * inverse >> 16 for n < 512
+    int32_t inverse;
 };
 
 constexpr int kLeastExp = -40, kMostExp = 40;
@@ -30,7 +32,13 @@ template <int FMT> struct Code8;
 template <> struct Code8<SLHIP_KV8_E4M3> {
     static constexpr uint32_t kLead = 0x600000u;  // fraction bits of 1.75
     static constexpr int kTop = 8;
-    __device__ static __forceinline__ uint32_t pack(const float* v, float inv) { return e4m3_pack4(v, inv); }
+    // |v * inv| <= 448 by the choice of the scale, so nothing is clamped; + 0 turns -0 into +0.
+    __device__ static __forceinline__ uint32_t pack(const float* v, float inv)
+    {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(fmaf(v[0], inv, 0.0f), fmaf(v[1], inv, 0.0f), 0, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(fmaf(v[2], inv, 0.0f), fmaf(v[3], inv, 0.0f), w, true);
+        return static_cast<uint32_t>(w);
+    }
     __device__ static __forceinline__ void unpack(uint32_t w, float* f)
     {
         const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
@@ -43,9 +51,11 @@ template <> struct Code8<SLHIP_KV8_I8> {
     static constexpr int kTop = 6;
     __device__ static __forceinline__ uint32_t pack(const float* v, float inv)
     {
-        uint32_t w = 0;
-        for (int i = 0; i < 4; i++) w |= (static_cast<uint32_t>(static_cast<int>(rintf(v[i] * inv))) & 0xFFu) << (8 * i);
-        return w;
+        // 1.5 * 2^23 + code: the sum rounds to a whole number, ties to even, whose low byte is the code
+        uint32_t u[4];
+        for (int i = 0; i < 4; i++) u[i] = __float_as_uint(fmaf(v[i], inv, 12582912.0f));
+        const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000C0Cu);
+        return lo | hi;
     }
     __device__ static __forceinline__ void unpack(uint32_t w, float* f)
     {
@@ -64,10 +74,16 @@ template <int FMT> __device__ __forceinline__ float scale_of(uint32_t amax)
 // 1 / s of a power of two.
 __device__ __forceinline__ float inverse(float s) { return __uint_as_float(0x7F000000u - __float_as_uint(s)); }
 
+// Largest of the wave, in lane 63's view made wave-uniform: within rows of 16 lanes, then row by row.
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v)
 {
-    for (int o = 32; o > 0; o >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o, 64)));
-    return v;
+    v = dpp_umax_step<0xB1>(v);   // quad_perm [1,0,3,2]
+    v = dpp_umax_step<0x4E>(v);   // quad_perm [2,3,0,1]
+    v = dpp_umax_step<0x141>(v);  // row_half_mirror
+    v = dpp_umax_step<0x140>(v);  // row_mirror
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x142, 0xA, 0xF, false)));  // row_bcast:15
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x143, 0xC, 0xF, false)));  // row_bcast:31
+    return __builtin_amdgcn_readlane(static_cast<int>(v), 63);
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7FFFFFFFu; }
@@ -79,6 +95,39 @@ __device__ __forceinline__ uint32_t byte_mask(int j, int a, int b)
     const uint32_t upto_hi = hi == 4 ? 0xFFFFFFFFu : (1u << (8 * hi)) - 1, upto_lo = lo == 4 ? 0xFFFFFFFFu : (1u << (8 * lo)) - 1;
     return upto_hi & ~upto_lo;
 }
+
+// 16 bytes of values from element i on; VEC: they may be loaded at once.
+template <int DT, bool VEC> __device__ __forceinline__ uint4 load_word(const void* p, int64_t i)
+{
+    if constexpr (VEC) return *reinterpret_cast<const uint4*>(static_cast<const char*>(p) + i * Vec<DT>::BYTES);
+    float f[Vec<DT>::N];
+#pragma unroll
+    for (int j = 0; j < Vec<DT>::N; j++) f[j] = Vec<DT>::load1(p, i + j);
+    return Vec<DT>::pack(f);  // the same bits again (a NaN's may change: it stays one)
+}
+
+// Two values next to each other.
+template <int DT> struct Pair;
+template <> struct Pair<SLHIP_F32> {
+    typedef float2 T;
+    template <bool VEC> __device__ static __forceinline__ T load(const void* p, int64_t i)
+    {
+        const float* f = static_cast<const float*>(p) + i;
+        if constexpr (VEC) return *reinterpret_cast<const float2*>(f);
+        return make_float2(f[0], f[1]);
+    }
+    __device__ static __forceinline__ float2 unpack(T v) { return v; }
+};
+template <> struct Pair<SLHIP_BF16> {
+    typedef uint32_t T;
+    template <bool VEC> __device__ static __forceinline__ T load(const void* p, int64_t i)
+    {
+        const uint16_t* f = static_cast<const uint16_t*>(p) + i;
+        if constexpr (VEC) return *reinterpret_cast<const uint32_t*>(f);
+        return f[0] | static_cast<uint32_t>(f[1]) << 16;
+    }
+    __device__ static __forceinline__ float2 unpack(T v) { return make_float2(bf16_lo(v), bf16_hi(v)); }
+};
 
 // DP: head dims up to 64, 128 or 256; VEC: rows that 16-byte (K) and pair (V) loads can read.
 template <int DT, int FMT, int DP, bool VEC>
@@ -109,57 +158,47 @@ __global__ __launch_bounds__(1024) void kv8_write(Kv8WriteArgs a)
 
     constexpr int KR = DP / 32, VR = (DP + 127) / 128;  // rounds of a lane: 8 values of K, 2 x 16 of V
     float f[KR * 8 > VR * 32 ? KR * 8 : VR * 32];
-    uint32_t top = 0;
+#pragma unroll
+    for (float& v : f) v = 0.0f;
+    // All loads go out before the first value is used: rows that are not the request's are read as one of its rows and dropped.
     if (mine && nb > na) {
         if (kv == 0) {
+            constexpr int W = Vec<DT>::BYTES / 2;  // 16-byte words of 8 values
+            uint4 raw[KR][W];
 #pragma unroll
             for (int o = 0; o < KR; o++) {
-                const int at = (lane + 64 * o) * 8, t = at / D, d = at % D;  // D values a token, 16 tokens
-                const bool in = t >= na && t < nb;
-                const int64_t e = (row0 + t) * xs + xh + d;
-                for (int j = 0; j < 8; j += 4) {
-                    float4 w = make_float4(0, 0, 0, 0);
-                    if (in) {
-                        if constexpr (VEC) {
-                            w = load4f<DT>(x, e + j);
-                        } else {
-                            w.x = Vec<DT>::load1(x, e + j);
-                            w.y = Vec<DT>::load1(x, e + j + 1);
-                            w.z = Vec<DT>::load1(x, e + j + 2);
-                            w.w = Vec<DT>::load1(x, e + j + 3);
-                        }
-                    }
-                    f[8 * o + j] = w.x; f[8 * o + j + 1] = w.y; f[8 * o + j + 2] = w.z; f[8 * o + j + 3] = w.w;
-                }
+                const int i = lane + 64 * o, row = i * a.inverse >> 16, t = min(max(row, na), nb - 1);  // 16 tokens of a.chunks
+                const int64_t e = (row0 + t) * xs + xh + (i - row * a.chunks) * 8;
+#pragma unroll
+                for (int w = 0; w < W; w++) raw[o][w] = load_word<DT, VEC>(x, e + w * Vec<DT>::N);
+            }
+#pragma unroll
+            for (int o = 0; o < KR; o++) {
+                const int t = (lane + 64 * o) * a.inverse >> 16;
+#pragma unroll
+                for (int w = 0; w < W; w++) Vec<DT>::unpack(raw[o][w], f + 8 * o + w * Vec<DT>::N);
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[8 * o + j] = t >= na && t < nb ? f[8 * o + j] : 0.0f;
             }
         } else {
+            typename Pair<DT>::T raw[VR][16];
 #pragma unroll
             for (int o = 0; o < VR; o++) {
-                const int d = 2 * (lane + 64 * o);
+                const int d = min(2 * (lane + 64 * o), D - 2);
+#pragma unroll
+                for (int t = 0; t < 16; t++) raw[o][t] = Pair<DT>::template load<VEC>(x, (row0 + min(max(t, na), nb - 1)) * xs + xh + d);
+            }
+#pragma unroll
+            for (int o = 0; o < VR; o++)
 #pragma unroll
                 for (int t = 0; t < 16; t++) {
-                    float lo = 0, hi = 0;
-                    if (d < D && t >= na && t < nb) {
-                        const int64_t e = (row0 + t) * xs + xh + d;
-                        if constexpr (VEC && DT == SLHIP_F32) {
-                            const float2 w = *reinterpret_cast<const float2*>(static_cast<const float*>(x) + e);
-                            lo = w.x;
-                            hi = w.y;
-                        } else if constexpr (VEC) {
-                            const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(x) + e);
-                            lo = bf16_lo(w);
-                            hi = bf16_hi(w);
-                        } else {
-                            lo = Vec<DT>::load1(x, e);
-                            hi = Vec<DT>::load1(x, e + 1);
-                        }
-                    }
-                    f[32 * o + t] = lo;
-                    f[32 * o + 16 + t] = hi;
+                    const float2 w = Pair<DT>::unpack(raw[o][t]);
+                    f[32 * o + t] = t >= na && t < nb ? w.x : 0.0f;
+                    f[32 * o + 16 + t] = t >= na && t < nb ? w.y : 0.0f;
                 }
-            }
         }
     }
+    uint32_t top = 0;
     if (block < 0 || block >= c.blocks) {  // the same for all of the thread block
         if (threadIdx.x == 0 && blockIdx.y == 0) raise_block(c, r.first, r.slot, max(p0, r.past), block);
         return;
@@ -198,7 +237,7 @@ __global__ __launch_bounds__(1024) void kv8_write(Kv8WriteArgs a)
     if (kv == 0) {
 #pragma unroll
         for (int o = 0; o < KR; o++) {
-            const int at = (lane + 64 * o) * 8, t = at / D;
+            const int at = (lane + 64 * o) * 8, t = (lane + 64 * o) * a.inverse >> 16;
             if (t >= 16) continue;
             uint2* p = reinterpret_cast<uint2*>(base + at);
             if (t >= na && t < nb) {
@@ -298,14 +337,17 @@ extern "C" SLHIP_API int slhip_kv8_write(int dtype, const void* k, int64_t k_str
     if (!k || !v) return fail(SLHIP_ERR_INVALID, "kv8_write: k and v are required");
     const int64_t size = dtype == SLHIP_F32 ? 4 : 2, D = a.c.D;
     if (k_stride_h < D || v_stride_h < D || k_stride_t < 0 || v_stride_t < 0) return fail(SLHIP_ERR_INVALID, "kv8_write: a head stride is smaller than the head, or a stride is negative");
+    a.chunks = a.c.D / 8;
+    a.inverse = (65536 + a.chunks - 1) / a.chunks;  // off by less than chunks / 65536 each: 512 * 32 of them stay below one
     a.x[0] = k;
     a.x[1] = v;
     a.st[0] = k_stride_t;
     a.st[1] = v_stride_t;
     a.sh[0] = k_stride_h;
     a.sh[1] = v_stride_h;
-    const bool vec = reinterpret_cast<uintptr_t>(k) % (4 * size) == 0 && reinterpret_cast<uintptr_t>(v) % (2 * size) == 0 &&
-                     k_stride_t % 4 == 0 && k_stride_h % 4 == 0 && v_stride_t % 2 == 0 && v_stride_h % 2 == 0;
+    const int64_t n16 = 16 / size;  // values of 16 bytes
+    const bool vec = aligned16(k) && reinterpret_cast<uintptr_t>(v) % (2 * size) == 0 && k_stride_t % n16 == 0 &&
+                     k_stride_h % n16 == 0 && v_stride_t % 2 == 0 && v_stride_h % 2 == 0;
     // Items by blocks, or by rows where that is fewer: a decode step has one row and one block a request.
     const int64_t bs = int64_t{1} << a.c.shift;
     const bool by_block = item_count(a.c.T, a.c.B, bs, 2) < a.c.T;

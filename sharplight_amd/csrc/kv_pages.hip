@@ -2,11 +2,13 @@
 //
 // Mathematics: two prefix sums over the requests -- of their new tokens (starts) and of the blocks those need (which ids
 // of the free list are theirs) -- then one write per taken block and one row per token. Nothing here moves enough bytes to
-// matter (20 a token); what a call costs is its launch and the chain load lengths -> scan -> load table -> store. So one
-// block of 1024 threads does it all in one launch, with the sums and the slots seen (a bit each, for the duplicate check)
-// in LDS, and decides over the whole step before it writes anything: all or nothing needs no second pass. From
-// kFusedTokens rows on, the rows go to a second launch over many blocks: one CU stores a row of 20 bytes about every
-// 20 cycles, which by then costs more than a launch.
+// matter (20 a token); what a call costs is its launch and the chain load lengths -> scan -> load table -> store. So a
+// thread block of 1024 does it all, with the sums and the slots seen (a bit each, for the duplicate check) in LDS, and
+// decides over the whole step before it writes anything: all or nothing needs no second pass. Steps of more rows than it
+// writes in the time of a launch (kBlockRows) take more thread blocks, each of which scans the lengths again and takes its
+// share of the rows; the first one alone writes the tables. A new block's id comes from the free list, an old one's from the
+// table, so no thread block waits for another's stores. Only the free list's count can be written where it is read (in
+// place); a step of many rows then has its rows in a second launch.
 #include "common.hpp"
 #include "kv8_map.hpp"
 
@@ -15,7 +17,7 @@ namespace slhip {
 constexpr int kPagesThreads = 1024;
 constexpr int kMaxRequests = 4096;
 constexpr int kMaxSlots = 131072;
-constexpr int64_t kFusedTokens = 4096;
+constexpr int64_t kBlockRows = 1024;
 
 struct KvPagesArgs {
     int32_t B;
@@ -29,7 +31,7 @@ struct KvPagesArgs {
     int32_t* n_free_out;
     int64_t tokens;
     int32_t *starts, *seq, *pos;
-    bool rows_here;
+    int64_t block_rows;  // rows of a thread block (0: none here)
     uint32_t* err;
 };
 
@@ -37,27 +39,26 @@ enum : uint32_t { kBadLength = 1, kBadSlot = 2, kBadRows = 3, kBadFree = 4 };
 
 __device__ __forceinline__ int64_t blocks_of(int64_t tokens, int shift) { return (tokens + (int64_t{1} << shift) - 1) >> shift; }
 
-// Row t of the step: request i's token t - starts[i], or padding.
-__device__ __forceinline__ void write_row(const KvPagesArgs& a, int64_t t, bool there, int32_t i, int32_t start)
+__device__ __forceinline__ void store_row(const KvPagesArgs& a, int64_t t, int32_t slot, int32_t pos, int32_t i, int32_t block)
 {
-    int32_t slot = -1, pos = -1, block = -1;
-    if (there) {
-        slot = a.slots ? a.slots[i] : i;
-        pos = a.past[i] + static_cast<int32_t>(t - start);
-        block = a.pages[slot * a.bps + (pos >> a.shift)];
-    }
     if (a.seq) {
         int32_t* s = a.seq + t * 4;
         if ((reinterpret_cast<uintptr_t>(a.seq) & 15u) == 0) {
-            *reinterpret_cast<int4*>(s) = make_int4(slot, pos, there ? i : -1, block);
+            *reinterpret_cast<int4*>(s) = make_int4(slot, pos, i, block);
         } else {
             s[0] = slot;
             s[1] = pos;
-            s[2] = there ? i : -1;
+            s[2] = i;
             s[3] = block;
         }
     }
-    if (a.pos) a.pos[t] = there ? pos : 0;
+    if (a.pos) a.pos[t] = max(pos, 0);
+}
+
+// Inclusive sums over the wave of numbers below 2^31, in 64 bits: the halves of 16 bits apart.
+__device__ __forceinline__ int64_t wave_scan_wide(int32_t v)
+{
+    return (static_cast<int64_t>(wave_scan(static_cast<uint32_t>(v) >> 16)) << 16) + wave_scan(v & 0xFFFF);
 }
 
 template <bool RELEASE>
@@ -67,18 +68,22 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     __shared__ uint32_t s_seen[kMaxSlots / 32];
     __shared__ int64_t s_wave[2][kPagesThreads / 64];
     __shared__ uint32_t s_bad;  // the first bad request * 8 + what is wrong with it
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const int64_t n_free = *a.n_free;
+    const int per = (a.B + kPagesThreads - 1) / kPagesThreads;
+    const int i0 = min(tid * per, a.B), i1 = min(i0 + per, a.B);
+    const int64_t row_tokens = a.bps << a.shift;
+    const auto slot_of = [&](int i) { return a.slots ? a.slots[i] : i; };
+    // the thread's first request: most steps have no more than one a thread
+    const int32_t past0 = i0 < i1 ? a.past[i0] : 0, count0 = i0 < i1 && !RELEASE ? a.count[i0] : 0, slot0 = i0 < i1 ? slot_of(i0) : 0;
     for (int64_t w = tid; w < (a.page_slots + 31) / 32; w += kPagesThreads) s_seen[w] = 0;
     if (tid == 0) s_bad = 0xFFFFFFFFu;
     __syncthreads();
 
-    const int per = (a.B + kPagesThreads - 1) / kPagesThreads;
-    const int i0 = min(tid * per, a.B), i1 = min(i0 + per, a.B);
-    const int64_t row_tokens = a.bps << a.shift;
+    // sums of the thread's requests: at most four of below 2^31 each, so they are kept below that by what the step may have
     int64_t tokens = 0, blocks = 0;
     for (int i = i0; i < i1; i++) {
-        const int64_t past = a.past[i], count = RELEASE ? 0 : a.count[i], slot = a.slots ? a.slots[i] : i;
+        const int64_t past = i == i0 ? past0 : a.past[i], count = RELEASE ? 0 : i == i0 ? count0 : a.count[i], slot = i == i0 ? slot0 : slot_of(i);
         uint32_t bad = 0;
         if (slot < 0 || slot >= a.page_slots || (atomicOr(&s_seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1u)) bad = kBadSlot;
         if (past < 0 || count < 0 || past + count > row_tokens) bad = kBadLength;
@@ -89,22 +94,16 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
             blocks += RELEASE ? blocks_of(past, a.shift) : blocks_of(past + count, a.shift) - blocks_of(past, a.shift);
         }
     }
-    // exclusive sums over the threads: within waves, then over the waves' totals
-    int64_t st = tokens, so = blocks;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t ut = __shfl_up(st, o, 64), uo = __shfl_up(so, o, 64);
-        if (lane >= o) {
-            st += ut;
-            so += uo;
-        }
-    }
+    const int64_t most = 0x7FFFFFFF;  // more than any step has rows or any list has room for
+    const int64_t ct = min(tokens, most), co = min(blocks, most);
+    int64_t st = wave_scan_wide(static_cast<int32_t>(ct)), so = wave_scan_wide(static_cast<int32_t>(co));
     if (lane == 63) {
         s_wave[0][wave] = st;
         s_wave[1][wave] = so;
     }
     __syncthreads();
-    st -= tokens;
-    so -= blocks;
+    st -= ct;
+    so -= co;
     int64_t all_tokens = 0, all_blocks = 0;
     for (int w = 0; w < kPagesThreads / 64; w++) {
         if (w == wave) {
@@ -120,13 +119,13 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
         if (!RELEASE && all_tokens > a.tokens) bad = kBadRows;
         else if (!room) bad = kBadFree;
     }
-    const bool ok = bad == 0xFFFFFFFFu;
-    if (tid == 0) {
+    const bool ok = bad == 0xFFFFFFFFu, first = blockIdx.x == 0;
+    if (first && tid == 0) {
         if (!ok) {
             const int i = min(static_cast<int>(bad >> 3), a.B - 1);
             const int64_t count = RELEASE || i < 0 ? 0 : a.count[i];
-            raise_error(a.err, kErrKvPages, max(i, 0), i < 0 ? 0 : a.slots ? a.slots[i] : i, i < 0 ? 0 : a.past[i],
-                        static_cast<uint32_t>(count), static_cast<uint32_t>(static_cast<uint64_t>(count) >> 32), bad & 7);
+            raise_error(a.err, kErrKvPages, max(i, 0), i < 0 ? 0 : slot_of(i), i < 0 ? 0 : a.past[i], static_cast<uint32_t>(count),
+                        static_cast<uint32_t>(static_cast<uint64_t>(count) >> 32), bad & 7);
         }
         *a.n_free_out = static_cast<int32_t>(!ok ? n_free : RELEASE ? n_free + all_blocks : n_free - all_blocks);
     }
@@ -135,48 +134,55 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     for (int i = i0; i < i1; i++) {
         s_start[i] = static_cast<int32_t>(st);
         s_off[i] = static_cast<int32_t>(so);
-        if (!RELEASE) a.starts[i] = ok ? static_cast<int32_t>(st) : 0;
+        if (!RELEASE && first) a.starts[i] = ok ? static_cast<int32_t>(st) : 0;
         if (!ok) continue;
-        const int64_t past = a.past[i];
-        if (RELEASE) {
-            so += blocks_of(past, a.shift);
-        } else {
-            st += a.count[i];
-            so += blocks_of(past + a.count[i], a.shift) - blocks_of(past, a.shift);
-        }
+        const int64_t past = i == i0 ? past0 : a.past[i], count = RELEASE ? 0 : i == i0 ? count0 : a.count[i];
+        st += count;
+        so += RELEASE ? blocks_of(past, a.shift) : blocks_of(past + count, a.shift) - blocks_of(past, a.shift);
     }
-    if (!RELEASE && tid == 0) a.starts[a.B] = static_cast<int32_t>(all_tokens);
+    if (!RELEASE && first && tid == 0) a.starts[a.B] = static_cast<int32_t>(all_tokens);
     __syncthreads();
 
-    for (int64_t k = tid; k < all_blocks; k += kPagesThreads) {
-        const int32_t i = static_cast<int32_t>(item_request([&](int64_t r) { return s_off[r]; }, a.B, k, 1, 0));
-        const int64_t slot = a.slots ? a.slots[i] : i;
-        int32_t* row = a.pages + slot * a.bps;
-        if (RELEASE) {
-            int32_t* e = row + (k - s_off[i]);
-            a.free_blocks[n_free + k] = *e;
-            *e = -1;
-        } else {
-            row[blocks_of(a.past[i], a.shift) + (k - s_off[i])] = a.free_blocks[n_free - 1 - k];
+    if (first) {
+        for (int64_t k = tid; k < all_blocks; k += kPagesThreads) {
+            const int32_t i = static_cast<int32_t>(item_request([&](int64_t r) { return s_off[r]; }, a.B, k, 1, 0));
+            int32_t* row = a.pages + slot_of(i) * a.bps;
+            if (RELEASE) {
+                int32_t* e = row + (k - s_off[i]);
+                a.free_blocks[n_free + k] = *e;
+                *e = -1;
+            } else {
+                row[blocks_of(a.past[i], a.shift) + (k - s_off[i])] = a.free_blocks[n_free - 1 - k];
+            }
         }
     }
-    if (RELEASE || !a.rows_here) return;
-    __threadfence_block();
-    __syncthreads();
-    for (int64_t t = tid; t < a.tokens; t += kPagesThreads) {
-        const bool there = t < all_tokens;
-        const int32_t i = there ? static_cast<int32_t>(item_request([&](int64_t r) { return s_start[r]; }, a.B, t, 1, 0)) : 0;
-        write_row(a, t, there, i, there ? s_start[i] : 0);
+    if (RELEASE) return;
+    const int64_t t1 = min((static_cast<int64_t>(blockIdx.x) + 1) * a.block_rows, a.tokens);
+    for (int64_t t = blockIdx.x * a.block_rows + tid; t < t1; t += kPagesThreads) {
+        if (t >= all_tokens) {
+            store_row(a, t, -1, -1, -1, -1);
+            continue;
+        }
+        const int32_t i = static_cast<int32_t>(item_request([&](int64_t r) { return s_start[r]; }, a.B, t, 1, 0));
+        const int32_t past = a.past[i], slot = slot_of(i), pos = past + static_cast<int32_t>(t - s_start[i]);
+        const int64_t j = pos >> a.shift, taken = j - blocks_of(past, a.shift);  // a new block's number among the request's
+        const int32_t block = taken < 0 ? a.pages[slot * a.bps + j] : a.free_blocks[n_free - 1 - (s_off[i] + taken)];
+        store_row(a, t, slot, pos, i, block);
     }
 }
 
+// The rows after the tables: a step of many rows whose free list counts in place.
 __global__ __launch_bounds__(256) void kv_pages_rows(KvPagesArgs a)
 {
     const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (t >= a.tokens) return;
-    const bool there = t < a.starts[a.B];
-    const int32_t i = there ? static_cast<int32_t>(item_request([&](int64_t r) { return a.starts[r]; }, a.B, t, 1, 0)) : 0;
-    write_row(a, t, there, i, there ? a.starts[i] : 0);
+    if (t >= a.starts[a.B]) {
+        store_row(a, t, -1, -1, -1, -1);
+        return;
+    }
+    const int32_t i = static_cast<int32_t>(item_request([&](int64_t r) { return a.starts[r]; }, a.B, t, 1, 0));
+    const int32_t slot = a.slots ? a.slots[i] : i, pos = a.past[i] + static_cast<int32_t>(t - a.starts[i]);
+    store_row(a, t, slot, pos, i, a.pages[slot * a.bps + (pos >> a.shift)]);
 }
 
 // Checks what the host can see of the arguments.
@@ -201,7 +207,7 @@ static int make_args(const char* op, bool release, const slhip_kv_pages* p, KvPa
     while ((int64_t{1} << shift) < p->block_size) shift++;
     *a = KvPagesArgs{static_cast<int32_t>(p->requests), p->past, p->count, p->slots, p->pages, p->page_slots, p->blocks_per_slot,
                      shift, p->free_blocks, p->free_capacity, p->n_free, p->n_free_out, p->tokens, p->starts, p->seq, p->pos,
-                     false, nullptr};
+                     0, nullptr};
     return error_word(&a->err);
 }
 
@@ -214,16 +220,14 @@ extern "C" SLHIP_API int slhip_kv_pages_advance(const slhip_kv_pages* p, slhip_s
     KvPagesArgs a;
     const int e = make_args("kv_pages_advance", false, p, &a);
     if (e) return e;
-    const bool rows = a.tokens > 0 && (a.seq || a.pos);
-    a.rows_here = rows && a.tokens <= kFusedTokens;
-    kv_pages_tables<false><<<1, kPagesThreads, 0, to_stream(stream)>>>(a);
-    if (rows && !a.rows_here) {
-        const int s = check_launch("kv_pages_tables");
-        if (s) return s;
-        kv_pages_rows<<<dim3(static_cast<unsigned>((a.tokens + 255) / 256)), 256, 0, to_stream(stream)>>>(a);
-        return check_launch("kv_pages_rows");
-    }
-    return check_launch("kv_pages_tables");
+    const bool rows = a.tokens > 0 && (a.seq || a.pos), apart = rows && a.tokens > kBlockRows && a.n_free == a.n_free_out;
+    a.block_rows = rows && !apart ? kBlockRows : 0;
+    const int64_t grid = a.block_rows ? (a.tokens + kBlockRows - 1) / kBlockRows : 1;
+    kv_pages_tables<false><<<static_cast<unsigned>(grid), kPagesThreads, 0, to_stream(stream)>>>(a);
+    const int s = check_launch("kv_pages_tables");
+    if (s || !apart) return s;
+    kv_pages_rows<<<static_cast<unsigned>((a.tokens + 255) / 256), 256, 0, to_stream(stream)>>>(a);
+    return check_launch("kv_pages_rows");
 }
 
 extern "C" SLHIP_API int slhip_kv_pages_release(const slhip_kv_pages* p, slhip_stream stream)

@@ -385,14 +385,14 @@ CASES = [  # D, heads, G, bs, new, past: one token to long, few rows and many, o
 @pytest.mark.parametrize("fmt,dtype", [("i8", "f32"), ("e4m3", "f32"), ("i8", "bf16"), ("e4m3", "bf16")])
 @pytest.mark.parametrize("D,heads,G,bs,new,past", CASES)
 def test_attention(device, fmt, dtype, D, heads, G, bs, new, past):
-    rng = _rng("attn", fmt, dtype, D, heads, G, bs, tuple(new))
-    st = Step(rng, new, past, bs, padding=3)
-    c = kv8_ref.Cache(fmt, st.blocks, bs, heads, D, fill=rng)
-    q, q64 = _put(rng.standard_normal((st.T, heads * G, D)) * 3, dtype)
-    scale = 1 / np.sqrt(D)
-    for max_new in (0, max(new)):
+    for max_new, wide in ((0, 500), (max(new), 1)):  # long table rows: contexts may be long, and heads are shared out
+        rng = _rng("attn", fmt, dtype, D, heads, G, bs, tuple(new))
+        st = Step(rng, new, past, bs, padding=3, wide=wide)
+        c = kv8_ref.Cache(fmt, st.blocks, bs, heads, D, fill=rng)
+        q, q64 = _put(rng.standard_normal((st.T, heads * G, D)) * 3, dtype)
+        scale = 1 / np.sqrt(D)
         with Dev() as d:
-            log(f"kv8_attention {dtype} {fmt} D={D} heads={heads}x{G} bs={bs} new={new} past={past} max_new={max_new}")
+            log(f"kv8_attention {dtype} {fmt} D={D} heads={heads}x{G} bs={bs} new={new} past={past} max_new={max_new} wide={wide}")
             y = _attend(d, dtype, st, c, q, G, max_new=max_new, scale=scale)
             native.synchronize()
             got = _from(d.get(y, q.shape, NP[dtype]), dtype)
@@ -407,7 +407,7 @@ def test_attention(device, fmt, dtype, D, heads, G, bs, new, past):
 def test_attention_scores(device, fmt, dtype, kw, D, heads, G, bs, new, past):
     """Caps, windows (of one key, inside a tile, at its border) and distance slopes."""
     rng = _rng("scores", fmt, dtype, str(kw), D)
-    st = Step(rng, new, past, bs)
+    st = Step(rng, new, past, bs, wide=1 if dtype == "f32" else 200)
     c = kv8_ref.Cache(fmt, st.blocks, bs, heads, D, fill=rng)
     q, q64 = _put(rng.standard_normal((st.T, heads * G, D)) * 3, dtype)
     kw = {"scale": 0.125, **kw}
@@ -467,7 +467,7 @@ def test_attention_does_not_see_what_is_not_there(device, fmt, dtype, new, past)
     """Codes behind a request's last token, blocks of nobody and their scales may hold anything; a poisoned block gives NaN
     to the rows that see it and to no others."""
     rng = _rng("unseen", fmt, dtype, len(new))
-    st = Step(rng, new, past, 16)
+    st = Step(rng, new, past, 16, wide=1 if dtype == "f32" else 300)
     c = kv8_ref.Cache(fmt, st.blocks, 16, 2, 64, fill=rng)
     want, bound = None, None
     q, q64 = _put(rng.standard_normal((st.T, 4, 64)), dtype)
@@ -511,7 +511,7 @@ def test_attention_does_not_see_what_is_not_there(device, fmt, dtype, new, past)
 def test_attention_of_what_does_not_fit(device, new, bad):
     """Keys of blocks outside the cache are not seen (a row without keys is 0); rows of requests that do not fit stay."""
     rng = _rng("unfit", bad, len(new))
-    st = Step(rng, new, [40, 50, 20], 16)
+    st = Step(rng, new, [40, 50, 20], 16, wide=1 if bad == "slot" else 300)
     max_new = 0
     if bad == "block":
         st.pages[st.slots[1], 1] = -1

@@ -118,7 +118,7 @@ def test_write_refusals():
 
 def test_attention_refusals():
     go = lambda q_heads=4, dtype="f32", q=FAKE, y=FAKE, work=FAKE, work_bytes=1 << 40, cache=None, **kw: native.kv8_attention(  # noqa: E731
-        dtype, q, y, q_heads, cache or _cache(), _batch(), scale=kw.pop("scale", 1.0), work=work, work_bytes=work_bytes, **kw)
+        dtype, q, y, q_heads, cache or _cache(), _batch(blocks_per_slot=1000), scale=kw.pop("scale", 1.0), work=work, work_bytes=work_bytes, **kw)
     with pytest.raises(ValueError, match="multiple of 2"):
         go(q_heads=3)
     with pytest.raises(NotImplementedError, match="64 query heads"):
@@ -142,8 +142,9 @@ def test_attention_refusals():
 
 
 def test_work_bytes():
-    need = native.kv8_attention_work_bytes(4, _cache(), _batch(), 1)
+    need = native.kv8_attention_work_bytes(4, _cache(), _batch(blocks_per_slot=1000), 1)
     assert 0 < need < 1 << 28
+    assert native.kv8_attention_work_bytes(4, _cache(), _batch(), 1) == 0  # contexts of 64 tokens at most: one launch
     assert native.kv8_attention_work_bytes(4, _cache(), _batch(requests=0), 1) == 0
     assert native.kv8_attention_work_bytes(3, _cache(), _batch(), 1) == -1
     for tokens in (1, 31, 512, 100000):
