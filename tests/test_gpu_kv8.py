@@ -440,6 +440,35 @@ def test_attention_long(device, fmt, dtype, D, heads, G, bs, new, past):
     _check_y(got, want, bound, "long")
 
 
+@pytest.mark.parametrize("fmt,dtype,G,most", [("i8", "f32", 2, 1), ("e4m3", "bf16", 4, 7), ("e4m3", "bf16", 1, 40)])
+@pytest.mark.parametrize("B,wide", [(64, 80), (65, 1), (70, 80), (300, 80), (4500, 1)])
+def test_many_requests(device, fmt, dtype, G, most, B, wide):
+    """More requests than lanes of a wave, and than its square: the write and the attention find theirs. Some bring nothing."""
+    rng = _rng("many", fmt, dtype, B)
+    new = rng.integers(0, 3, B)
+    new[rng.integers(0, B, 20)] = most
+    new = np.minimum(new, most)
+    st = Step(rng, new.tolist(), rng.integers(0, 60, B) * (rng.random(B) < 0.8), 16, padding=2, wide=wide)
+    c = kv8_ref.Cache(fmt, st.blocks, 16, 2, 32, fill=rng)
+    q, q64 = _put(rng.standard_normal((st.T, 2 * G, 32)) * 3, dtype)
+    k, k64 = _put(_values(rng, (st.T, 2, 32)), dtype)
+    v, v64 = _put(_values(rng, (st.T, 2, 32)), dtype)
+    with Dev() as d:
+        cache, at = _cache(d, c)
+        batch = st.batch(d)
+        log(f"{B} requests, {dtype} {fmt} G={G} most={most} wide={wide}")
+        native.kv8_write(dtype, d.put(k), d.put(v), cache, batch)
+        native.synchronize()
+        kv8_ref.write(c, k64, v64, st.starts, st.past, st.slots, st.pages)
+        _check_write(d, c, at, B)
+        for max_new in (0, most):
+            y = _attend(d, dtype, st, c, q, G, batch=batch, cache=cache, scale=0.125, max_new=max_new)
+            native.synchronize()
+            got = _from(d.get(y, q.shape, NP[dtype]), dtype)
+            want, bound = kv8_ref.attention(c, q64, st.starts, st.past, st.slots, st.pages, scale=0.125, dtype=dtype)
+            _check_y(got, want, bound, f"max_new={max_new}", _pattern(dtype))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("new,past", [([1, 2, 1], [40, 100, 3]), ([60, 70], [40, 10])])
 def test_attention_scales_far_apart(device, dtype, new, past):

@@ -141,6 +141,14 @@ def test_attention_refusals():
         go(work=FAKE + 4)
 
 
+def test_attention_refuses_more_keys_than_its_sums_hold():
+    batch = lambda requests: _batch(requests=requests, page_slots=1 << 16, tokens=1 << 16, blocks_per_slot=(1 << 23) // 16)  # noqa: E731
+    with pytest.raises(NotImplementedError, match="are too many"):
+        native.kv8_attention("f32", FAKE, FAKE, 4, _cache(), batch(1 << 16), scale=1.0, max_new=1, work=FAKE, work_bytes=1 << 40)
+    assert native.kv8_attention_work_bytes(4, _cache(), batch(1 << 16), 1) == -1
+    assert native.kv8_attention_work_bytes(4, _cache(), batch(1 << 15), 1) > 0
+
+
 def test_work_bytes():
     need = native.kv8_attention_work_bytes(4, _cache(), _batch(blocks_per_slot=1000), 1)
     assert 0 < need < 1 << 28
