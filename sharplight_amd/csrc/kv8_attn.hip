@@ -49,9 +49,10 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
     int64_t bytes = 0;
     a->direct = false;
     if (p->wave_tiles) {
-        // Contexts that cannot be longer than kDirectRounds rounds are not worth a second launch: a few of them get a thread
-        // block for each head.
-        a->direct = B * heads <= kWorkers && c.bps << c.shift <= kDirectRounds * 4 * kTile;
+        // Contexts that cannot be longer than kDirectRounds rounds are not worth a second launch: each of their heads gets a
+        // thread block. (One query row each, 8 K/V heads: 128 of 1001 tokens 38 us on a line, 33 us so; 400 of up to 701 89
+        // and 79 us. 150 of up to 401 tokens, 4 heads of 256 dims, at one thread block a CU: 37 and 43 us.)
+        a->direct = c.bps << c.shift <= kDirectRounds * 4 * kTile && (dp < 256 || B * heads <= kWorkers);
         a->workers = static_cast<int32_t>(a->direct ? B * heads : dp == 256 ? kWorkers / 2 : kWorkers);
         p->by_part = B * heads < 256;
         if (!a->direct) bytes += 2 * a->workers * (few * dp + few * 2) * 4;
@@ -134,7 +135,9 @@ extern "C" SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q
     if (need > 0 && (!work || !aligned16(work) || work_bytes < need))
         return fail(SLHIP_ERR_INVALID, "kv8_attention: the workspace has %lld bytes, %lld are needed (16-byte aligned)",
                     static_cast<long long>(work ? work_bytes : 0), static_cast<long long>(need));
-    if (a.items * a.splits * a.c.heads > 0x7FFFFFFF - 4096) return fail(SLHIP_ERR_UNSUPPORTED, "kv8_attention: too many tiles");
+    // a launch has less than 2^32 threads; the join has two thread blocks a head at most, besides those of few tiles
+    if (a.items * a.splits * a.c.heads + a.workers >= 1 << 24 || static_cast<int64_t>(a.c.B) * a.c.heads * 2 >= (1 << 24) - kBlockUnits * 32)
+        return fail(SLHIP_ERR_UNSUPPORTED, "kv8_attention: too many tiles");
     e = error_word(&a.c.err);
     if (e) return e;
     hipStream_t st = to_stream(stream);

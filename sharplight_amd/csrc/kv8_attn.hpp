@@ -1171,7 +1171,6 @@ template <int DT, int FMT, int DP, bool RESHAPED> static int kv8_attn_run(const 
     const int64_t waves = p.wave_tiles && !a.direct ? static_cast<int64_t>(a.c.B) * a.c.heads * p.wave_tiles * (p.by_part ? DP / 16 : 1) : 0;
     const int64_t blocks = p.blocks && a.splits > 1 ? a.items * a.c.heads * 4 * NB : 0;
     if (waves + blocks == 0) return SLHIP_OK;
-    if (waves + blocks > 0x7FFFFFFF) return fail(SLHIP_ERR_UNSUPPORTED, "kv8_attention: too many tiles");
     const unsigned grid = static_cast<unsigned>(waves + blocks);
     if (p.wave_tiles == 2) {
         if (p.by_part) kv8_attn_join<DT, DP, NT2, NB, true><<<grid, 256, 0, st>>>(a, waves);

@@ -355,6 +355,7 @@ extern "C" SLHIP_API int slhip_kv8_write(int dtype, const void* k, int64_t k_str
     a.extra = by_block ? 2 : 0;
     const int64_t items = by_block ? item_count(a.c.T, a.c.B, bs, 2) : a.c.T;
     const unsigned wpi = static_cast<unsigned>(bs >> 4), threads = 64 * (wpi < 4 ? 4 : wpi), per = threads / 64 / wpi;
+    if (items * threads > 0xFFFFFFFFll) return fail(SLHIP_ERR_UNSUPPORTED, "kv8_write: too many rows");  // a launch's threads
     const dim3 grid(static_cast<unsigned>(items), (2 * a.c.heads + per - 1) / per);
     const int w = error_word(&a.c.err);
     if (w) return w;

@@ -149,6 +149,20 @@ def test_attention_refuses_more_keys_than_its_sums_hold():
     assert native.kv8_attention_work_bytes(4, _cache(), batch(1 << 15), 1) > 0
 
 
+def test_launches_past_their_limits_are_refused():
+    """A launch has less than 2^32 threads."""
+    most = _batch(tokens=(1 << 31) - (1 << 17), blocks_per_slot=1000)
+    with pytest.raises(NotImplementedError, match="too many rows"):
+        native.kv8_write("bf16", FAKE, FAKE, _cache(), most)
+    go = lambda cache, batch, q_heads, **kw: native.kv8_attention("bf16", FAKE, FAKE, q_heads, cache, batch, scale=1.0, work=FAKE,  # noqa: E731
+                                                                  work_bytes=1 << 40, **kw)
+    with pytest.raises(NotImplementedError, match="too many tiles"):
+        go(_cache(), most, 4)
+    for slots in (4, 1000):  # short contexts, and such that are shared out
+        with pytest.raises(NotImplementedError, match="too many tiles"):
+            go(_cache(heads=4096), _batch(requests=65536, page_slots=65536, tokens=65536, blocks_per_slot=slots), 4096, max_new=1)
+
+
 def test_work_bytes():
     need = native.kv8_attention_work_bytes(4, _cache(), _batch(blocks_per_slot=1000), 1)
     assert 0 < need < 1 << 28
