@@ -728,6 +728,51 @@ def test_serving_steps(device, captured, fmt, dtype):
         graph = None
 
 
+@pytest.mark.parametrize("dtype,D,max_new", [("bf16", 256, 0), ("f32", 128, 0), ("bf16", 128, 8)])
+def test_captured_attention_with_other_lengths(device, dtype, D, max_new):
+    """One captured call of room for many rows and long contexts, replayed with other lengths, among them none at all, and the
+    program's own work in between: what an eager call gives, and the statement's values."""
+    rng = _rng("captured", dtype, D, max_new)
+    B, heads, G, bs, rows = 3, 2, 4, 16, 120
+    top = Step(rng, [rows, rows, rows], [2000, 2000, 2000], bs)
+    c = kv8_ref.Cache("i8", top.blocks, bs, heads, D, fill=rng)
+    lengths = [([1, 1, 1], [1700, 3, 900]), ([8, 5, 1], [0, 1999, 64]), ([0, 0, 0], [5, 6, 7]), ([1, 8, 0], [31, 32, 33])]
+    if not max_new:
+        lengths += [([100, 3, 17], [0, 2000, 300]), ([1, 40, 60], [2000, 10, 0])]
+    st = native.Stream()
+    with Dev() as d:
+        cache, batch = _cache(d, c)[0], top.batch(d)
+        starts, past = top.dev[:2]
+        batch = native.kv8_batch(B, rows, starts, past, top.dev[2], top.pages.shape[0], top.pages.shape[1], slots=top.dev[3])
+        q, q64 = _put(rng.standard_normal((rows, heads * G, D)) * 2, dtype)
+        pq, y, eager = d.put(q), d.empty(q.nbytes), d.empty(q.nbytes)
+        need = native.kv8_attention_work_bytes(heads * G, cache, batch, max_new)
+        work = d.empty(max(need, 16), fill=0xFF)
+
+        def run(out=y, stream=st.handle):
+            native.kv8_attention(dtype, pq, out, heads * G, cache, batch, scale=0.0625, max_new=max_new, work=work, work_bytes=need, stream=stream)
+
+        graph = native.Graph(st, run)
+        for turn, (new, old) in enumerate(lengths * 2):
+            s = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+            for at, x in ((starts, s), (past, np.int32(old))):
+                native.call("slhip_memcpy_h2d", at, np.ascontiguousarray(x).ctypes.data, x.nbytes, st.handle)
+            for out in (y, eager):
+                native.call("slhip_memset", out, 0x5A, q.nbytes, st.handle)
+            st.sync()
+            log(f"captured attention {dtype} D={D} turn {turn}: new={new} past={old}")
+            graph.launch(st)
+            st.sync()
+            run(eager)
+            st.sync()
+            got = d.get(y, q.shape, NP[dtype])
+            assert np.array_equal(got, d.get(eager, q.shape, NP[dtype])), turn
+            if turn < len(lengths):
+                want, bound = kv8_ref.attention(c, q64, s, np.int32(old), top.slots, top.pages, scale=0.0625, dtype=dtype)
+                _check_y(_from(got, dtype), want, bound, turn, _pattern(dtype))
+        graph = None
+
+
 def test_two_streams_at_once(device):
     """Overlapping calls with workspaces of their own, on two streams, several times: the same bits as one after another."""
     rng = _rng("streams")
