@@ -12,6 +12,9 @@
 // stores 8 codes. V goes [D][16 tokens]: a lane takes a pair of dims of all 16 tokens (4-byte loads that cover a token's
 // row between them) and stores 16 + 16 bytes, so neither needs a transpose. What bounds it: HBM for a prompt, launch and
 // the chain starts -> table -> scale for a decode step.
+// Measured, 8 heads of 128, bf16 to E4M3: a prompt of 8192 tokens 12.5 us (50 MB, 4.0 TB/s), one token of 64 requests 5.0 us.
+// All of an item's loads are issued before the first value is used (before that 15.2 us): the table entry and the old codes
+// and scale wait behind them.
 #include "kv8.hpp"
 
 namespace slhip {
