@@ -415,8 +415,8 @@ class DeviceBuffer:
 
 def ptr(x) -> int | None:
     """Device address of a DeviceBuffer / int / None."""
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     if isinstance(x, DeviceBuffer):
         return x.ptr
     return int(x)
@@ -644,12 +644,12 @@ def kv_pages(requests, past, count, pages, page_slots, blocks_per_slot, block_si
 
 def kv_pages_advance(p: KvPages, stream=None):
     """Takes the step's blocks from the free list and writes its block table entries, starts, seq and pos."""
-    call("slhip_kv_pages_advance", ctypes.byref(p), stream)
+    call("slhip_kv_pages_advance", p, stream)
 
 
 def kv_pages_release(p: KvPages, stream=None):
     """Returns the blocks of requests that ended (slots, past = their lengths) to the free list."""
-    call("slhip_kv_pages_release", ctypes.byref(p), stream)
+    call("slhip_kv_pages_release", p, stream)
 
 
 def kv8_cache(fmt, k, v, k_scale, v_scale, blocks, block_size, heads, head_dim) -> Kv8Cache:
@@ -670,7 +670,7 @@ def kv8_write(dtype, k, v, cache: Kv8Cache, batch: Kv8Batch, *, k_stride_t=None,
     d, row = cache.head_dim, cache.heads * cache.head_dim
     call("slhip_kv8_write", DTYPES.get(dtype, dtype), ptr(k), row if k_stride_t is None else k_stride_t,
          d if k_stride_h is None else k_stride_h, ptr(v), row if v_stride_t is None else v_stride_t,
-         d if v_stride_h is None else v_stride_h, ctypes.byref(cache), ctypes.byref(batch), stream)
+         d if v_stride_h is None else v_stride_h, cache, batch, stream)
 
 
 def kv8_attention_work_bytes(q_heads, cache: Kv8Cache, batch: Kv8Batch, max_new=0) -> int:
@@ -686,8 +686,7 @@ def kv8_attention(dtype, q, y, q_heads, cache: Kv8Cache, batch: Kv8Batch, *, sca
     cfg = Kv8Attn(scale, softcap, window, ptr(slopes), max_new)
     call("slhip_kv8_attention", DTYPES.get(dtype, dtype), ptr(q), row if q_stride_t is None else q_stride_t,
          d if q_stride_h is None else q_stride_h, q_heads, ptr(y), row if y_stride_t is None else y_stride_t,
-         d if y_stride_h is None else y_stride_h, ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(cfg), ptr(work),
-         work_bytes, stream)
+         d if y_stride_h is None else y_stride_h, cache, batch, cfg, ptr(work), work_bytes, stream)
 
 
 def gather(fmt, table, V, D, ids, N, dtype_out, y, *, y_stride=None, stream=None):
