@@ -342,7 +342,7 @@ template <int NP> __device__ __forceinline__ void tile_weights(TileRow& t, int s
 {
     const float w0 = __builtin_amdgcn_exp2f(fmaf(t.S[8 * s + j], t.mul, t.shift));
     const float w1 = __builtin_amdgcn_exp2f(fmaf(t.S[8 * s + j + 1], t.mul, t.shift));
-    t.sum += w0 + w1;
+    t.sum += w0 + w1;  // not of the f16 parts: l weighs them by 1 / vs, and a block of tiny values has no f16 weights left
     const f16x2 hi = to_f16x2(w0, w1);
     p[0][s][j] = hi.x;
     p[0][s][j + 1] = hi.y;
