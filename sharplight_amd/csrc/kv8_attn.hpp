@@ -35,7 +35,9 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 64;
-constexpr float kBias = 8.0f;  // weights are at most 2^kBias in f16
+constexpr float kBias = 8.0f;   // weights are 2^kBias in f16 for t_j = M
+constexpr float kSlack = 7.0f;  // and at most 2^(kBias + kSlack), below f16's largest
+constexpr float kExact = 0x1p20f;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kStart = 2;
 constexpr float kNone = -1e30f;  // a maximum of nothing: finite, so that differences with -inf stay numbers
@@ -278,11 +280,12 @@ struct TileRow {
     float sum;         // of the weights so far
 };
 
-// Scores and the row's new maximum m (in TileRow's terms); returns what the row's sums so far are to be multiplied by.
-// lo <= j < hi are the keys that are seen.
-template <int DT, bool RESHAPED>
-__device__ __forceinline__ float tile_max(const Kv8AttnArgs& a, const f32x4 (&products)[4], const Row& row, const TileScale& sc, int32_t key0,
-                                          int lo, int hi, bool masked, float& m, TileRow& t)
+// Scores, and the row's M (m, in TileRow's terms). M need not be the maximum: it moves up to it only where the maximum is above
+// it by more than kSlack, so that the sums so far are seldom multiplied (rescale; a row's maximum moves in every second tile
+// of the first 64, and 32 or 64 products a tile are as many as its exponentials). lo <= j < hi are the keys that are seen.
+template <int DT, bool RESHAPED, class Rescale>
+__device__ __forceinline__ void tile_max(const Kv8AttnArgs& a, const f32x4 (&products)[4], const Row& row, const TileScale& sc, int32_t key0,
+                                         int lo, int hi, bool masked, float& m, TileRow& t, const Rescale& rescale)
 {
     // t = fma(S, mul, add) with mul > 0, so the largest S is the largest t. Capped or sloped scores, and those of a scale that
     // is not positive (RESHAPED), are turned into t themselves.
@@ -329,12 +332,22 @@ __device__ __forceinline__ float tile_max(const Kv8AttnArgs& a, const f32x4 (&pr
 #pragma unroll
     for (int j = 1; j < 15; j += 2) mx = fmaxf(fmaxf(mx, S[j]), S[j + 1]);
     mx = fmaxf(mx, S[15]);
-    const float was = m;
-    m = fmaxf(m, row_max(fmaf(mx, mul, add)));
+    const float top = row_max(fmaf(mx, mul, add));
+    const bool up = top - m > kSlack;
+    if (__any(up)) {
+        const float to = up ? top : m;
+        rescale(__builtin_amdgcn_exp2f(m - to));
+        m = to;
+    }
     t.mul = mul;
     t.shift = add - (m - kBias);
     t.sum = 0.0f;
-    return __builtin_amdgcn_exp2f(was - m);
+    if (__any(fabsf(m) > kExact)) {  // the roundings of S * mul + shift could add up to a weight past f16: t first, then t - M
+#pragma unroll
+        for (int j = 0; j < 16; j++) S[j] = fmaf(S[j], mul, add) - m;
+        t.mul = 1.0f;
+        t.shift = kBias;
+    }
 }
 
 // Weights 8 s + j and 8 s + j + 1 (j even), into P's parts.
@@ -690,14 +703,14 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
                 const int hi = min(row[n].pos - k0l + 1, keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
                 const bool masked = __any(hi < 16 || lo > 0);
                 TileRow t;
-                const float alpha = tile_max<DT, RESHAPED>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], t);
-                if (__any(alpha != 1.0f)) {
+                tile_max<DT, RESHAPED>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], t, [&](float alpha) __attribute__((always_inline)) {
+                    l[n] *= alpha;
 #pragma unroll
                     for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
-                }
+                });
 #pragma unroll
                 for (int j = 0; j < 16; j += 2) tile_weights<NP>(t, j >> 3, j & 7, p[n]);
-                l[n] = fmaf(t.sum, sc.down, l[n] * alpha);
+                l[n] = fmaf(t.sum, sc.down, l[n]);
             }
             // keys that are not there have weight 0, but their codes could be NaN
             if (__any(keys < 16)) {
@@ -1062,17 +1075,16 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
             load(key + 2 * kTile);
             __builtin_amdgcn_sched_barrier(0);
             TileRow t[NT];
-            float alpha[NT];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 const int k0l = key + 16 * g;
                 const int hi = min(row[n].pos - k0l + 1, keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
                 const bool masked = __any(hi < 16 || lo > 0);
-                alpha[n] = tile_max<DT, RESHAPED>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], t[n]);
-                if (__any(alpha[n] != 1.0f)) {
+                tile_max<DT, RESHAPED>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], t[n], [&](float alpha) __attribute__((always_inline)) {
+                    l[n] *= alpha;
 #pragma unroll
-                    for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha[n];
-                }
+                    for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
+                });
             }
             f16x8 p[NT][NP][2];
             __builtin_amdgcn_sched_barrier(0);
@@ -1098,7 +1110,7 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
-            for (int n = 0; n < NT; n++) l[n] = fmaf(t[n].sum, sc.down, l[n] * alpha[n]);
+            for (int n = 0; n < NT; n++) l[n] = fmaf(t[n].sum, sc.down, l[n]);
             sc = sn;
             keys = keys_next;
         }

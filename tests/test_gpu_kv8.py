@@ -490,6 +490,36 @@ def test_attention_scales_far_apart(device, dtype, new, past):
     _check_y(got, want, bound, "far apart")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("new,past", [([1, 2], [130, 500]), ([40, 50], [130, 500])])
+def test_attention_of_large_scores(device, dtype, slopes, new, past):
+    """Scores of up to 2^60: far past where f32 tells neighbours apart, but the largest of a row is larger by a third, so its
+    key's value is the answer. (Weights of e^-1000 and less for the others: the rest is y's rounding, and 2^-11 or 2^-22 of it for
+    the weight, which cancels.)"""
+    rng = _rng("large", dtype, slopes, len(new))
+    st = Step(rng, new, past, 16)
+    D, heads, G = 64, 2, 2
+    c = kv8_ref.Cache("i8", st.blocks, 16, heads, D, fill=rng)
+    c.k[:], c.ks[:], c.vs[:] = 0, 1.0, 1.0
+    c.k[..., 0] = 90
+    best = [int(rng.integers(0, p + 1)) for p in past]  # every row of the request sees it
+    for i, s in enumerate(st.slots):
+        c.k[st.pages[s, best[i] // 16], :, best[i] % 16, 0] = 120
+    q = np.zeros((st.T, heads * G, D))
+    q[..., 0] = np.exp2(rng.integers(5, 54, (st.T, heads * G)))
+    bits, _ = _put(q, dtype)
+    with Dev() as d:
+        log(f"kv8_attention large scores {dtype} slopes={slopes} new={new}")
+        y = _attend(d, dtype, st, c, bits, G, scale=1.0, slopes=d.put(np.full(heads * G, 0.25, np.float32)) if slopes else None)
+        native.synchronize()
+        got = _from(d.get(y, bits.shape, NP[dtype]), dtype)
+    for i, s in enumerate(st.slots):
+        v = c.v.view(np.int8)[st.pages[s, best[i] // 16], :, 0, :, best[i] % 16].astype(np.float64)  # [heads, D]
+        rows = got[st.starts[i]:st.starts[i + 1]].reshape(-1, heads, G, D)
+        assert (np.abs(rows - v[None, :, None]) <= np.abs(v[None, :, None]) * 2.0 ** (-20 if dtype == "f32" else -7)).all(), i
+
+
 @pytest.mark.parametrize("fmt,dtype", [("e4m3", "f32"), ("e4m3", "bf16"), ("i8", "bf16")])
 @pytest.mark.parametrize("new,past", [([1, 1], [70, 10]), ([40, 50], [70, 0])])
 def test_attention_does_not_see_what_is_not_there(device, fmt, dtype, new, past):
