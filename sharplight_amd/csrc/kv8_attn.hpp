@@ -3,10 +3,10 @@
 // Mathematics. For a query row q with position p and keys j <= p (and j > p - window):
 //   z_j = scale * ks_b * (q . k_j)  (capped, slopes added), ks_b and vs_b = 2^ev_b the scales of key j's block b,
 //   y   = sum_j e^z_j vs_b c_j / sum_j e^z_j,  k_j and c_j the codes.
-// With t_j = z_j log2(e) + ev_b and M the running maximum of t_j, w_j = 2^(t_j - M) <= 1 holds the whole weight of code
-// c_j, the block's scale included: o = sum_j w_j c_j, l = sum_j w_j 2^-ev_b, y = o / l. So V's codes go to the matrix
-// cores as they are, the scale costs nothing (it rides in the addition of the exponent), and what is rounded to f16, w_j,
-// is rounded relative to the largest contribution, whatever the scales of the blocks are.
+// With t_j = z_j log2(e) + ev_b and M the running maximum of t_j (or a little less: tile_max), w_j = 2^(t_j - M) holds the
+// whole weight of code c_j, the block's scale included: o = sum_j w_j c_j, l = sum_j w_j 2^-ev_b, y = o / l. So V's codes go
+// to the matrix cores as they are, the scale costs nothing (it rides in the addition of the exponent), and what is rounded
+// to f16, w_j, is rounded relative to the largest contribution, whatever the scales of the blocks are.
 //
 // Numbers. int8 and E4M3 codes are exact in f16. A query row is multiplied by the power of two that brings its largest
 // value to [2^14, 2^15): bf16 values are then exact in f16 down to 2^-29 of the row's largest (below that they round to
@@ -915,8 +915,9 @@ template <int DT, int DP, int NT> __device__ __forceinline__ void join_blocks(co
 // Four waves of NT * 16 rows each share a key tile's codes, converted to f16 once and held in LDS in the order in which
 // the matrix instructions take them (a fragment is 64 lanes of 16 bytes: reads and writes without conflicts), two tiles
 // deep, the next tile's codes loading meanwhile: one barrier a tile. The vector unit (exponentials, f16 conversions) bounds
-// it next to the matrix cores. Measured: a prompt of 8192, 32 query heads of 128 on 8, bf16 and E4M3, 569 us (970 TFLOP/s of
-// the 1310 that a large bf16 product reaches; vector unit 69% and matrix cores 41% of the time).
+// it next to the matrix cores. Measured: a prompt of 8192, 32 query heads of 128 on 8, bf16 and E4M3, 557 us (990 TFLOP/s of
+// the 1310 that a large bf16 product reaches) at 2.25 GHz, 612 us at the 2.05 that the clock falls to under a long load;
+// vector unit 66% and matrix cores 42% of the cycles.
 template <int DP> struct BlockTile {
     static constexpr int kK = 4 * (DP / 32), kV = (DP / 16) * 2;  // fragments of K: t, h, s; of V: dt, s
 };
