@@ -126,6 +126,29 @@ def test_pages_advance(device, B, bs, most_past, most_new, padding, in_place):
         assert np.array_equal(d.get(at["free"], free.shape, np.int32), free)
 
 
+def test_pages_of_the_largest_table(device):
+    """4096 requests in a table of 131072 rows, the last row among them, and rows over hundreds of thread blocks."""
+    rng = _rng("largest")
+    B, bs, slots = 4096, 64, 131072
+    past = rng.integers(0, 128, B).astype(np.int32)
+    count = np.where(rng.random(B) < 0.1, rng.integers(0, 129, B), 1).astype(np.int32)
+    slot = rng.permutation(slots)[:B].astype(np.int32)
+    slot[7] = slots - 1 if (slot != slots - 1).all() else slot[7]
+    pages = np.full((slots, 4), -1, np.int32)
+    for i in range(B):
+        n = -(-int(past[i]) // bs)
+        pages[slot[i], :n] = 10 * i + np.arange(n)
+    need = int(sum(-(-(int(p) + int(c)) // bs) - -(-int(p) // bs) for p, c in zip(past, count)))
+    free, tokens = (100000 + rng.permutation(need + 9)).astype(np.int32), int(count.sum()) + 100
+    for in_place in (False, True):
+        with Dev() as d:
+            log(f"kv_pages_advance of {B} requests, {tokens} rows, in place: {in_place}")
+            p, at = _advance(d, past, count, slot, pages, bs, free, len(free), tokens, in_place)
+            native.kv_pages_advance(p)
+            native.synchronize()
+            _check_advance(d, at, kv8_ref.advance(past, count, slot, pages, bs, free, len(free), tokens), B, tokens)
+
+
 def test_pages_identity_slots_no_rows_and_no_requests(device):
     rng = _rng("identity")
     past, count, slot, pages, free, need = _tables(rng, 9, 16, 60, 20, 9)
@@ -488,6 +511,32 @@ def test_attention_scales_far_apart(device, dtype, new, past):
         got = _from(d.get(y, q.shape, NP[dtype]), dtype)
     want, bound = kv8_ref.attention(c, q64, st.starts, st.past, st.slots, st.pages, scale=float(np.float32(0.2)), dtype=dtype)
     _check_y(got, want, bound, "far apart")
+
+
+def test_as_many_requests_as_there_may_be(device):
+    """65536 requests, of which a few hundred bring rows, the first and the last among them."""
+    rng = _rng("most")
+    B = 65536
+    new, past = np.zeros(B, int), np.zeros(B, int)
+    at = np.concatenate([[0, 63, 64, 4095, 4096, B - 1], rng.integers(0, B, 300)])
+    new[at], past[at] = rng.integers(1, 4, len(at)), rng.integers(0, 100, len(at))
+    st = Step(rng, new.tolist(), past, 16, padding=1, wide=80)
+    c = kv8_ref.Cache("i8", st.blocks, 16, 1, 32, fill=rng)
+    q, q64 = _put(rng.standard_normal((st.T, 4, 32)) * 2, "bf16")
+    k, k64 = _put(_values(rng, (st.T, 1, 32)), "bf16")
+    with Dev() as d:
+        cache, where = _cache(d, c)
+        batch = st.batch(d)
+        log(f"{B} requests, {st.T} rows")
+        native.kv8_write("bf16", d.put(k), d.put(k), cache, batch)
+        native.synchronize()
+        kv8_ref.write(c, k64, k64, st.starts, st.past, st.slots, st.pages)
+        _check_write(d, c, where, B)
+        y = _attend(d, "bf16", st, c, q, 4, batch=batch, cache=cache, scale=0.125, max_new=3)
+        native.synchronize()
+        got = _from(d.get(y, q.shape, np.uint16), "bf16")
+    want, bound = kv8_ref.attention(c, q64, st.starts, st.past, st.slots, st.pages, scale=0.125, dtype="bf16")
+    _check_y(got, want, bound, B, _pattern("bf16"))
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
