@@ -955,20 +955,11 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
         first = static_cast<int32_t>(min(from, static_cast<int64_t>(end)));
         end = static_cast<int32_t>(min(to, static_cast<int64_t>(end)));
     }
-    f16x8 q[NT][NP][NH][2];
-    Row row[NT];
-    float m[NT], l[NT];
-    f32x4 o[NT][ND];
+    RawRow<DT, DP> raw[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int32_t at = row0 + (wave * NT + n) * 16 + c;
-        RawRow<DT, DP> raw;
-        fetch_row<DT, DP>(a, r, head, at, at < row1, raw);
-        row[n] = make_row<DT, DP, NP>(a, r, head, at, at < row1, raw, q[n]);
-        m[n] = kNone;
-        l[n] = 0.0f;
-#pragma unroll
-        for (int dt = 0; dt < ND; dt++) o[n][dt] = f32x4{0, 0, 0, 0};
+        fetch_row<DT, DP>(a, r, head, at, at < row1, raw[n]);
     }
     const int32_t all = r.past + r.n;  // keys of the request: codes behind them are not read as keys
 
@@ -984,7 +975,7 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
     // the lane's first codes in a sub-block (dims past D: any codes, q is 0 there and the sums are not stored)
     const uint8_t* const kbase = base.k + (4 * wave + (c & 3)) * D + (16 * g < D ? 16 * g : 0);
     const uint8_t* const vbase = base.v + (16 * wave < D ? 256 * wave : 0) + c * 16;
-    const int32_t border = first + ((end - first - 1) & ~(kTile - 1));  // the last tile
+    const int32_t border = max(first + ((end - first - 1) & ~(kTile - 1)), 0);  // the last tile
     const auto look = [&](int32_t key) __attribute__((always_inline)) {
         key = min(key, border);
         kid = block_id(a.c, r.table, key + 16 * (c >> 2), all);
@@ -1018,6 +1009,23 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
         f[at * 64] = x;
         f[(at + 1) * 64] = z;
     };
+    // The first codes are on their way while the queries become f16 parts. (A range of no tiles loads others of the request.)
+    look(first);
+    load(first);
+    __builtin_amdgcn_sched_barrier(0);
+    f16x8 q[NT][NP][NH][2];
+    Row row[NT];
+    float m[NT], l[NT];
+    f32x4 o[NT][ND];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int32_t at = row0 + (wave * NT + n) * 16 + c;
+        row[n] = make_row<DT, DP, NP>(a, r, head, at, at < row1, raw[n], q[n]);
+        m[n] = kNone;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < ND; dt++) o[n][dt] = f32x4{0, 0, 0, 0};
+    }
     if (first < end) {
         const auto scales = [&](int32_t key) __attribute__((always_inline)) {
             TileScale sc = tile_scale(a.c, next, ksn, vsn);
@@ -1026,8 +1034,6 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
             if (next.bad && wave == 0) raise_block(a.c, r.first, r.slot, min(key, border) + 16 * g, next.entry);
             return sc;
         };
-        look(first);
-        load(first);
         clip();
 #pragma unroll
         for (int i = 0; i < NH + VJ; i++) stage(s_frag + lane, i);
