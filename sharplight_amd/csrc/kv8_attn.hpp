@@ -322,7 +322,11 @@ __device__ __forceinline__ void tile_max(const Kv8AttnArgs& a, const f32x4 (&pro
     }
     if (masked) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) S[j] = j >= lo && j < hi ? S[j] : -INFINITY;
+        for (int j = 0; j < 16; j++) S[j] = j < hi ? S[j] : -INFINITY;
+        if (__any(lo > 0)) {  // at a window's border only
+#pragma unroll
+            for (int j = 0; j < 16; j++) S[j] = j >= lo ? S[j] : -INFINITY;
+        }
         if (hi <= max(lo, 0)) {  // none is seen: the block's scales, which may be no numbers, do not count
             mul = 1.0f;
             add = 0.0f;
