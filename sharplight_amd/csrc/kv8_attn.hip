@@ -24,7 +24,10 @@ constexpr int64_t kDirectRounds = 4;
 // up to 1500 older ones, 12 heads of 64, f32 67, 54, 52 us; a prompt of 1024, 32 query heads of 128 on 8, bf16 34, 32, 42 us;
 // 128 tokens on 30000, the same heads 118, 99, 111 us.
 constexpr int64_t kBlockUnits = 512;
-constexpr int64_t kMaxSplits = 64;
+// Up to here (and up to 64 requests) the cuts go by the lengths, whose scan costs some 3 us in the kernel and in the join: 128
+// tokens on 30000, as above, 103 us with equal cuts and 95 so, 7 requests of up to 74700 82 and 65 us; but the prompt of 1024 33
+// and 37 us, the 5 requests 53 and 60.
+constexpr int64_t kFewTiles = kBlockUnits / 4;
 
 // What a call over T rows of B requests launches. Few-row work takes a request whose rows fit one or two matrix tiles (16
 // or 32 rows a K/V head): its keys are then read once by single waves. Everything else goes to thread blocks that share
@@ -58,17 +61,21 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
         if (!a->direct) bytes += 2 * a->workers * (few * dp + few * 2) * 4;
     }
     a->splits = 1;
+    a->share = 0;
     if (p->blocks) {
-        const int64_t tile = 64 * block_tiles(dtype == SLHIP_F32, static_cast<int>(dp));
+        const int64_t tile = 64 * block_tiles(dtype == SLHIP_F32, static_cast<int>(dp)), floats = tile * dp + tile * 2;
         a->tile_tokens = static_cast<int32_t>(tile / G);
         a->items = item_count(T, B, a->tile_tokens, 1);
-        const int64_t pairs = a->items * heads, longest = (c.bps << c.shift) / (4 * kTile) + 1;
-        int64_t s = pairs < kBlockUnits ? (kBlockUnits + pairs - 1) / pairs : 1;
-        if (s > kMaxSplits) s = kMaxSplits;
-        if (s > longest) s = longest;
-        a->splits = static_cast<int32_t>(s);
         a->part2 = a->part + bytes / 4;
-        if (s > 1) bytes += pairs * s * (tile * dp + tile * 2) * 4;
+        const int64_t pairs = a->items * heads, longest = (c.bps << c.shift) / (kLeastCut * kTile) + 1;
+        if (pairs <= kFewTiles && B <= 64 && a->items * longest < 1 << 27) {
+            a->share = static_cast<int32_t>((kBlockUnits + heads - 1) / heads);
+            bytes += (a->items + a->share) * heads * floats * 4;
+        } else if (pairs < kBlockUnits) {
+            const int64_t s = (kBlockUnits + pairs - 1) / pairs;
+            a->splits = static_cast<int32_t>(s < longest ? s : longest);
+            if (a->splits > 1) bytes += pairs * a->splits * floats * 4;
+        }
     }
     return bytes;
 }
@@ -136,7 +143,7 @@ extern "C" SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q
         return fail(SLHIP_ERR_INVALID, "kv8_attention: the workspace has %lld bytes, %lld are needed (16-byte aligned)",
                     static_cast<long long>(work ? work_bytes : 0), static_cast<long long>(need));
     // a launch has less than 2^32 threads; the join has two thread blocks a head at most, besides those of few tiles
-    if (a.items * a.splits * a.c.heads + a.workers >= 1 << 24 || static_cast<int64_t>(a.c.B) * a.c.heads * 2 >= (1 << 24) - kBlockUnits * 32)
+    if ((a.items * a.splits + a.share) * a.c.heads + a.workers >= 1 << 24 || static_cast<int64_t>(a.c.B) * a.c.heads * 2 >= (1 << 24) - kBlockUnits * 32)
         return fail(SLHIP_ERR_UNSUPPORTED, "kv8_attention: too many tiles");
     e = error_word(&a.c.err);
     if (e) return e;

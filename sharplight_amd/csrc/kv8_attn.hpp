@@ -38,6 +38,7 @@ constexpr int kTile = 64;
 constexpr float kBias = 8.0f;   // weights are 2^kBias in f16 for t_j = M
 constexpr float kSlack = 7.0f;  // and at most 2^(kBias + kSlack), below f16's largest
 constexpr float kExact = 0x1p20f;
+constexpr int kLeastCut = 4;  // key tiles of a many-row tile that are worth a thread block of their own
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kStart = 2;
 constexpr float kNone = -1e30f;  // a maximum of nothing: finite, so that differences with -inf stay numbers
@@ -56,9 +57,10 @@ struct Kv8AttnArgs {
     int32_t block_min, block_max;  // many-row tiles: requests of (block_min, block_max] rows; above is an error
     int32_t workers;             // few-row thread blocks
     bool direct;                 // one for each request's head, which share nothing
-    int32_t tile_tokens, splits; // many-row tiles: tokens of a tile, key ranges it is cut into
-    int64_t items;               // many-row tiles of a head
-    float *part, *part2;         // sums of key ranges: of workers, of splits
+    int32_t tile_tokens;         // many-row tiles: tokens of a tile
+    int64_t items;               // of a head
+    int32_t splits, share;       // key ranges that each is cut into; or (share > 0) how many more than tiles a head has of them
+    float *part, *part2;         // sums of key ranges: of workers, of tiles
 };
 
 // ---- codes ----------------------------------------------------------------------------------------------------
@@ -894,22 +896,84 @@ __device__ __forceinline__ void join_waves(const Kv8AttnArgs& a, int64_t index)
     });
 }
 
-// The sums of a row tile over its splits. index: (tile from the last, head, n).
+// A key range of a row tile: number `split` of the `cuts` that the tile is cut into; their sums are parts first + 0 .. of the
+// head. cuts = 0: there is none.
+struct Cut {
+    Kv8Request r;
+    int32_t tile, split, cuts;
+    int64_t first;
+};
+
+// The row tiles of a request that is of the many-row work.
+__device__ __forceinline__ int32_t request_tiles(const Kv8AttnArgs& a, const Kv8Request& r)
+{
+    const int64_t rows = static_cast<int64_t>(r.n) * a.G;
+    return rows <= a.block_min || rows > a.block_max ? 0 : (r.n + a.tile_tokens - 1) / a.tile_tokens;
+}
+
+// Range `index` of a head, or the first one of row tile `index` (BY_TILE). Tiles that fill the machine are not cut; of up to 64
+// requests, whose lengths a wave has at once, those with longer contexts are cut into more ranges (all tiles of a request into
+// as many as its last), so that `share` ranges besides the tiles are about as long as each other; of more requests all
+// tiles are cut alike. Whole row tiles come from the last: their key ranges are the longest, and short ones fill the end.
+// Wave-uniform.
+template <bool BY_TILE> __device__ __forceinline__ Cut find_cut(const Kv8AttnArgs& a, int64_t index, bool raise)
+{
+    Cut f{};
+    if (a.share == 0) {
+        const int64_t back = BY_TILE ? index : index / a.splits;
+        const Kv8Item it = kv8_find(a.c, a.items - 1 - back, a.tile_tokens, 1);
+        if (raise && (threadIdx.x & 63) == 0 && it.piece == 0 && (it.r.bad || static_cast<int64_t>(it.r.n) * a.G > a.block_max)) raise_request(a.c, it.i, it.r);
+        if (it.piece < 0 || it.piece >= request_tiles(a, it.r)) return f;
+        f.r = it.r;
+        f.tile = static_cast<int32_t>(it.piece);
+        f.first = back * a.splits;
+        f.split = BY_TILE ? 0 : static_cast<int32_t>(index - f.first);
+        f.cuts = a.splits;
+        return f;
+    }
+    const int lane = threadIdx.x & 63, i = min(lane, a.c.B - 1);
+    const Kv8Request mine = kv8_request(a.c, i);
+    const int32_t tiles = lane < a.c.B ? request_tiles(a, mine) : 0;
+    if (raise && index == 0 && lane < a.c.B && (mine.bad || static_cast<int64_t>(mine.n) * a.G > a.block_max)) raise_request(a.c, i, mine);
+    int32_t first, end;
+    key_range(a, mine.past, (tiles - 1) * a.tile_tokens, mine.n, first, end);
+    const int32_t length = (end - first + kTile - 1) / kTile;
+    const int32_t all = __builtin_amdgcn_readlane(wave_scan(tiles * length), 63), each = max((all + a.share - 1) / a.share, kLeastCut);
+    const int32_t cuts = (length + each - 1) / each, up = wave_scan(tiles * cuts);
+    const int k = BY_TILE ? max(__popcll(__ballot(lane < a.c.B && item_base(a.c.starts[i], i, a.tile_tokens, 1) <= index)) - 1, 0)
+                          : __popcll(__ballot(up <= index));
+    if (k >= a.c.B) return f;
+    const int32_t t = __builtin_amdgcn_readlane(tiles, k), cut = __builtin_amdgcn_readlane(cuts, k);
+    const int64_t from = __builtin_amdgcn_readlane(up, k) - static_cast<int64_t>(t) * cut;
+    const int64_t piece = BY_TILE ? index - item_base(__builtin_amdgcn_readlane(mine.first, k), k, a.tile_tokens, 1) : quotient(index - from, max(cut, 1));
+    if (piece < 0 || piece >= t || from < 0 || from + static_cast<int64_t>(t) * cut > a.items + a.share) return f;
+    f.r.first = __builtin_amdgcn_readlane(mine.first, k);
+    f.r.n = __builtin_amdgcn_readlane(mine.n, k);
+    f.r.past = __builtin_amdgcn_readlane(mine.past, k);
+    f.r.slot = __builtin_amdgcn_readlane(mine.slot, k);
+    f.r.bad = false;
+    f.r.table = a.c.pages + f.r.slot * a.c.bps;
+    f.tile = static_cast<int32_t>(piece);
+    f.first = from + piece * cut;
+    f.split = BY_TILE ? 0 : static_cast<int32_t>(index - f.first);
+    f.cuts = cut;
+    return f;
+}
+
+// The sums of a row tile over its key ranges. index: (tile, head, n).
 template <int DT, int DP, int NT> __device__ __forceinline__ void join_blocks(const Kv8AttnArgs& a, int64_t index)
 {
     const int n = static_cast<int>(index % NT);
     index /= NT;
     const int32_t head = static_cast<int32_t>(index % a.c.heads);
-    const int64_t back = index / a.c.heads, item = a.items - 1 - back;
-    const Kv8Item it = kv8_find(a.c, item, a.tile_tokens, 1);
-    const Kv8Request& r = it.r;
-    const int64_t t0 = it.piece * a.tile_tokens;
-    if (t0 < 0 || t0 >= r.n || static_cast<int64_t>(r.n) * a.G <= a.block_min || static_cast<int64_t>(r.n) * a.G > a.block_max) return;
-    const int32_t row0 = static_cast<int32_t>(t0) * a.G, row1 = static_cast<int32_t>(min(static_cast<int64_t>(r.n), t0 + a.tile_tokens)) * a.G;
+    const Cut f = find_cut<true>(a, index / a.c.heads, false);
+    if (f.cuts < 2) return;
+    const Kv8Request& r = f.r;
+    const int32_t row0 = f.tile * a.tile_tokens * a.G, row1 = min(r.n, (f.tile + 1) * a.tile_tokens) * a.G;
     if (row0 + 16 * n >= row1) return;
     const int32_t row = row0 + 16 * n + (threadIdx.x & 15);
-    const auto at = [&](int32_t k) { return a.part2 + ((back * a.splits + k) * a.c.heads + head) * Partial<DP, NT>::kFloats; };
-    join_rows<DP, NT, false>(at, a.splits, n, 0, [&](int dt, const f32x4& o, float l) {
+    const auto at = [&](int32_t k) { return a.part2 + ((f.first + k) * a.c.heads + head) * Partial<DP, NT>::kFloats; };
+    join_rows<DP, NT, false>(at, f.cuts, n, 0, [&](int dt, const f32x4& o, float l) {
         if (row < row1) store_dims<DT>(a, r, head, row, dt, o, row_inverse(l));
     });
 }
@@ -936,26 +1000,16 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
     f16x8* s_frag = reinterpret_cast<f16x8*>(lds);  // [2][kK + kV][64]
     const int lane = threadIdx.x & 63, wave = wave_id(), c = lane & 15, g = lane >> 4, D = a.c.D;
     const int32_t head = static_cast<int32_t>(index % a.c.heads);
-    const int64_t rest = index / a.c.heads;
-    const int32_t split = static_cast<int32_t>(rest % a.splits);
-    // tiles from the last: their key ranges are the longest, and short ones fill the end
-    const int64_t item = a.items - 1 - rest / a.splits;
-    const Kv8Item it = kv8_find(a.c, item, a.tile_tokens, 1);
-    const Kv8Request& r = it.r;
-    const int64_t t0 = it.piece * a.tile_tokens;
-    if (r.bad && t0 == 0 && head == 0 && split == 0 && threadIdx.x == 0) raise_request(a.c, it.i, r);
-    if (t0 < 0 || t0 >= r.n || static_cast<int64_t>(r.n) * a.G <= a.block_min) return;
-    if (static_cast<int64_t>(r.n) * a.G > a.block_max) {
-        if (t0 == 0 && head == 0 && split == 0 && threadIdx.x == 0) raise_request(a.c, it.i, r);
-        return;
-    }
-    const int32_t t1 = min(static_cast<int64_t>(r.n), t0 + a.tile_tokens);
-    const int32_t row0 = static_cast<int32_t>(t0) * a.G, row1 = t1 * a.G;  // rows of the tile
+    const Cut cut = find_cut<false>(a, index / a.c.heads, head == 0 && wave == 0);
+    if (cut.cuts == 0) return;
+    const Kv8Request& r = cut.r;
+    const int32_t t0 = cut.tile * a.tile_tokens, t1 = min(r.n, t0 + a.tile_tokens);
+    const int32_t row0 = t0 * a.G, row1 = t1 * a.G;  // rows of the tile
     int32_t first, end;
-    key_range(a, r.past, static_cast<int32_t>(t0), t1, first, end);
-    {   // this split's part of the range
-        const int32_t tiles = (end - first + kTile - 1) / kTile, each = (tiles + a.splits - 1) / a.splits;
-        const int64_t from = first + static_cast<int64_t>(split) * each * kTile, to = from + static_cast<int64_t>(each) * kTile;
+    key_range(a, r.past, t0, t1, first, end);
+    {   // this part of the range
+        const int32_t tiles = (end - first + kTile - 1) / kTile, each = (tiles + cut.cuts - 1) / cut.cuts;
+        const int64_t from = first + static_cast<int64_t>(cut.split) * each * kTile, to = from + static_cast<int64_t>(each) * kTile;
         first = static_cast<int32_t>(min(from, static_cast<int64_t>(end)));
         end = static_cast<int32_t>(min(to, static_cast<int64_t>(end)));
     }
@@ -1126,12 +1180,12 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
             keys = keys_next;
         }
     }
-    float* part = a.part2 + index * Partial<DP, 4 * NT>::kFloats;
+    float* part = a.part2 + ((cut.first + cut.split) * a.c.heads + head) * Partial<DP, 4 * NT>::kFloats;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int32_t at = (wave * NT + n) * 16 + c;
         l[n] = row_sum(l[n]);
-        if (a.splits == 1) {
+        if (cut.cuts == 1) {
             const float inv = row_inverse(l[n]);
             if (row0 + at < row1) {
 #pragma unroll
@@ -1187,7 +1241,7 @@ template <int DT, int FMT, int DP, int NT, int NB, bool RESHAPED> static int kv8
     constexpr int waves = NT > 0 ? waves_lds<DP, NT ? NT : 1>() : 0, blocks = NB > 0 ? blocks_lds<DP>() : 0, lds = waves > blocks ? waves : blocks;
     const auto kernel = kv8_attn<DT, FMT, DP, NT, NB, RESHAPED>;
     if (lds > 65536) SLHIP_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    const int64_t grid = (NT > 0 ? a.workers : 0) + (NB > 0 ? a.items * a.splits * a.c.heads : 0);
+    const int64_t grid = (NT > 0 ? a.workers : 0) + (NB > 0 ? (a.share ? a.items + a.share : a.items * a.splits) * a.c.heads : 0);
     kernel<<<static_cast<unsigned>(grid), 256, lds, st>>>(a);
     return check_launch("kv8_attn");
 }
@@ -1200,7 +1254,7 @@ template <int DT, int FMT, int DP, bool RESHAPED> static int kv8_attn_run(const 
     else e = p.wave_tiles == 1 ? kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED>(a, st);
     if (e) return e;
     const int64_t waves = p.wave_tiles && !a.direct ? static_cast<int64_t>(a.c.B) * a.c.heads * p.wave_tiles * (p.by_part ? DP / 16 : 1) : 0;
-    const int64_t blocks = p.blocks && a.splits > 1 ? a.items * a.c.heads * 4 * NB : 0;
+    const int64_t blocks = p.blocks && (a.share || a.splits > 1) ? a.items * a.c.heads * 4 * NB : 0;
     if (waves + blocks == 0) return SLHIP_OK;
     const unsigned grid = static_cast<unsigned>(waves + blocks);
     if (p.wave_tiles == 2) {
