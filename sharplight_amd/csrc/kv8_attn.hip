@@ -55,7 +55,8 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
         // Contexts that cannot be longer than kDirectRounds rounds are not worth a second launch: each of their heads gets a
         // thread block. (One query row each, 8 K/V heads: 128 of 1001 tokens 38 us on a line, 33 us so; 400 of up to 701 89
         // and 79 us. 150 of up to 401 tokens, 4 heads of 256 dims, at one thread block a CU: 37 and 43 us.)
-        a->direct = c.bps << c.shift <= kDirectRounds * 4 * kTile && (dp < 256 || B * heads <= kWorkers);
+        const bool two = dp < 256 || (!p->blocks && lean(dtype == SLHIP_F32, static_cast<int>(dp)));  // thread blocks a CU
+        a->direct = c.bps << c.shift <= kDirectRounds * 4 * kTile && (two || B * heads <= kWorkers);
         a->workers = static_cast<int32_t>(a->direct ? B * heads : dp == 256 ? kWorkers / 2 : kWorkers);
         p->by_part = B * heads < 256;
         if (!a->direct) bytes += 2 * a->workers * (few * dp + few * 2) * 4;

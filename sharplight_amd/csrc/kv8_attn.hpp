@@ -527,7 +527,7 @@ template <int DP, int NT> struct Partial {
 
 template <int DP, int NT> constexpr int waves_lds() { return (2 * NT * (DP / 16) * 64 * 4 + 4 * NT * 16 * 2) * 4; }
 
-template <int DT, int FMT, int DP, int NT, bool RESHAPED>
+template <int DT, int FMT, int DP, int NT, bool LEAN, bool RESHAPED>
 __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t worker, char* lds)
 {
     constexpr int NP = DT == SLHIP_F32 ? 2 : 1, ND = DP / 16, NH = DP / 64;
@@ -553,7 +553,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
     } cur, next;
     int64_t pos = 0, stop;  // on the line
     int32_t step = 0;
-    if (a.direct) {
+    if (LEAN || a.direct) {
         cur.i = worker / a.c.heads;
         cur.head = worker - cur.i * a.c.heads;
         const Kv8Request r = kv8_request(a.c, cur.i);
@@ -645,7 +645,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
         for (int n = 0; n < NT; n++) fetch_row<DT, DP>(a, s.request(), s.head, 16 * n + c, 16 * n + c < s.n * a.G, raw[n]);
         if (s.k0 < s.last) {
             aim(s, s.k0);
-            load_v();
+            if (!LEAN) load_v();
         }
     };
     look(cur, min(cur.k0, cur.end - 1));
@@ -654,7 +654,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
         const Kv8Request r = cur.request();
         const int32_t rows = r.n * a.G, head = cur.head;
         next = cur;
-        const bool another = advance(next);
+        const bool another = !LEAN && advance(next);
         f16x8 q[NT][NP][NH][2];
         Row row[NT];
         float m[NT], l[NT];
@@ -695,7 +695,11 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
             TileScale sc = tile_scale(a.c, vb, ks, vs);
             const int32_t keys = vb.keys;
             if (vb.bad) raise_block(a.c, r.first, r.slot, key + 16 * g, vb.entry);
-            if constexpr (more) {
+            if constexpr (LEAN) {
+                __builtin_amdgcn_sched_barrier(0);
+                load_v();
+                __builtin_amdgcn_sched_barrier(0);
+            } else if constexpr (more) {
                 // scales in registers of their own, or the next ones' arrival is waited for to move them
                 asm volatile("" : "+v"(sc.k), "+v"(sc.ev), "+v"(sc.down));
                 __builtin_amdgcn_sched_barrier(0);
@@ -739,7 +743,8 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
             }
             if constexpr (more) {
                 __builtin_amdgcn_sched_barrier(0);
-                load_v();
+                if constexpr (LEAN) aim(cur, key + 4 * kTile);
+                else load_v();
             }
         };
         if (cur.k0 < cur.last) {
@@ -1204,6 +1209,12 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
 // Matrix tiles of 16 rows that a wave of a many-row tile works on: two where two waves a SIMD find registers for them.
 constexpr int block_tiles(bool f32, int dp) { return dp == 256 || (f32 && dp == 128) ? 1 : 2; }
 
+// Whether direct few-row work has a kernel that holds K's and V's codes in the same registers, one after the other, so that two
+// waves a SIMD find room: heads of short contexts are all latency, of which two thread blocks a CU hide each other's. (289
+// requests of up to 19 tokens, 2 K/V heads of 256: LEAN1 us, by the other kernel LEAN0. Long contexts want the loads in
+// flight: 32 of up to 8000 100 us, so 120.)
+constexpr bool lean(bool f32, int dp) { return dp == 256 && !f32; }
+
 // What a call launches, from what the host knows.
 struct Kv8AttnPlan {
     int32_t wave_tiles;  // few-row launch: 0 none, else matrix tiles of 16 rows (1, 2)
@@ -1212,16 +1223,16 @@ struct Kv8AttnPlan {
 };
 
 // Thread blocks of the many-row tiles, then of the few-row work: one launch, so that neither waits for the other's end.
-template <int DT, int FMT, int DP, int NT, int NB, bool RESHAPED>
-__global__ __launch_bounds__(256, DP == 256 || NT == 2 ? 1 : 2) void kv8_attn(Kv8AttnArgs a)
+template <int DT, int FMT, int DP, int NT, int NB, bool LEAN, bool RESHAPED>
+__global__ __launch_bounds__(256, (DP == 256 && !LEAN) || NT == 2 ? 1 : 2) void kv8_attn(Kv8AttnArgs a)
 {
     extern __shared__ __align__(16) char lds[];
     if constexpr (NT > 0 && NB > 0) {
         const unsigned blocks = gridDim.x - a.workers;
         if (blockIdx.x < blocks) attn_blocks<DT, FMT, DP, NB, RESHAPED>(a, blockIdx.x, lds);
-        else attn_waves<DT, FMT, DP, NT, RESHAPED>(a, blockIdx.x - blocks, lds);
+        else attn_waves<DT, FMT, DP, NT, false, RESHAPED>(a, blockIdx.x - blocks, lds);
     } else if constexpr (NT > 0) {
-        attn_waves<DT, FMT, DP, NT, RESHAPED>(a, blockIdx.x, lds);
+        attn_waves<DT, FMT, DP, NT, LEAN, RESHAPED>(a, blockIdx.x, lds);
     } else {
         attn_blocks<DT, FMT, DP, NB, RESHAPED>(a, blockIdx.x, lds);
     }
@@ -1236,10 +1247,11 @@ __global__ __launch_bounds__(256) void kv8_attn_join(Kv8AttnArgs a, int64_t wave
 
 template <int DT, int FMT, bool RESHAPED> int kv8_attn_launch(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st);
 
-template <int DT, int FMT, int DP, int NT, int NB, bool RESHAPED> static int kv8_attn_start(const Kv8AttnArgs& a, hipStream_t st)
+template <int DT, int FMT, int DP, int NT, int NB, bool RESHAPED, bool LEAN = false>
+static int kv8_attn_start(const Kv8AttnArgs& a, hipStream_t st)
 {
     constexpr int waves = NT > 0 ? waves_lds<DP, NT ? NT : 1>() : 0, blocks = NB > 0 ? blocks_lds<DP>() : 0, lds = waves > blocks ? waves : blocks;
-    const auto kernel = kv8_attn<DT, FMT, DP, NT, NB, RESHAPED>;
+    const auto kernel = kv8_attn<DT, FMT, DP, NT, NB, LEAN, RESHAPED>;
     if (lds > 65536) SLHIP_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     const int64_t grid = (NT > 0 ? a.workers : 0) + (NB > 0 ? (a.share ? a.items + a.share : a.items * a.splits) * a.c.heads : 0);
     kernel<<<static_cast<unsigned>(grid), 256, lds, st>>>(a);
@@ -1250,7 +1262,9 @@ template <int DT, int FMT, int DP, bool RESHAPED> static int kv8_attn_run(const 
 {
     constexpr int NB = block_tiles(DT == SLHIP_F32, DP), NT2 = DP <= 128 ? 2 : 1;  // make_plan asks for two up to 128 dims
     int e;
-    if (p.blocks) e = p.wave_tiles ? kv8_attn_start<DT, FMT, DP, 1, NB, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, 0, NB, RESHAPED>(a, st);
+    constexpr bool kLean = lean(DT == SLHIP_F32, DP);
+    if (kLean && !p.blocks && a.direct) e = kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED, kLean>(a, st);
+    else if (p.blocks) e = p.wave_tiles ? kv8_attn_start<DT, FMT, DP, 1, NB, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, 0, NB, RESHAPED>(a, st);
     else e = p.wave_tiles == 1 ? kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED>(a, st);
     if (e) return e;
     const int64_t waves = p.wave_tiles && !a.direct ? static_cast<int64_t>(a.c.B) * a.c.heads * p.wave_tiles * (p.by_part ? DP / 16 : 1) : 0;
