@@ -19,7 +19,6 @@ template <int DT, int FMT> static int launch(const Kv8AttnArgs& a, const Kv8Attn
 }
 
 constexpr int64_t kWorkers = 512;     // two thread blocks a CU (one of 256 dims)
-constexpr int64_t kDirectRounds = 4;
 // Row tiles and key ranges of the many-row work, over all heads. With 256, 512, 1024: 5 requests of 77 to 611 new tokens and
 // up to 1500 older ones, 12 heads of 64, f32 67, 54, 52 us; a prompt of 1024, 32 query heads of 128 on 8, bf16 34, 32, 42 us;
 // 128 tokens on 30000, the same heads 118, 99, 111 us.
@@ -52,11 +51,13 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
     int64_t bytes = 0;
     a->direct = false;
     if (p->wave_tiles) {
-        // Contexts that cannot be longer than kDirectRounds rounds are not worth a second launch: each of their heads gets a
-        // thread block. (One query row each, 8 K/V heads: 128 of 1001 tokens 38 us on a line, 33 us so; 400 of up to 701 89
-        // and 79 us. 150 of up to 401 tokens, 4 heads of 256 dims, at one thread block a CU: 37 and 43 us.)
-        const bool two = dp < 256 || (!p->blocks && lean(dtype == SLHIP_F32, static_cast<int>(dp)));  // thread blocks a CU
-        a->direct = c.bps << c.shift <= kDirectRounds * 4 * kTile && (two || B * heads <= kWorkers);
+        // Each head gets a thread block of its own, and no second launch, where contexts cannot be long: up to 4 rounds (1024
+        // tokens), and the more the more heads there are to fill the machine while the longest run. (8 K/V heads of 128, on
+        // the line and so: 8 requests of up to 2001 tokens 15 and 16 us, 64 of them 34 and 30, 256 of up to 4001 208 and 198, of
+        // up to 8001 367 and 394.)
+        const int64_t rounds = p->blocks || B * heads < kWorkers ? 4 : B * heads < 2 * kWorkers ? 8 : 16;
+        a->direct = c.bps << c.shift <= rounds * 4 * kTile && (dp < 256 || !p->blocks || B * heads <= kWorkers);
+        p->few_heads = B * heads <= kWorkers;
         a->workers = static_cast<int32_t>(a->direct ? B * heads : dp == 256 ? kWorkers / 2 : kWorkers);
         p->by_part = B * heads < 256;
         if (!a->direct) bytes += 2 * a->workers * (few * dp + few * 2) * 4;

@@ -416,6 +416,14 @@ __device__ __forceinline__ void key_range(const Kv8AttnArgs& a, int32_t past, in
 
 // ---- few rows: a wave a key tile ---------------------------------------------------------------------------------
 
+// How heads come to thread blocks: kShared, by the line below (or directly, where the launch holds many-row tiles too); kDirect,
+// a thread block a head, with nothing carried from one to the next, which takes 60 registers less; kLean, that with K's and V's
+// codes in the same registers one after the other, for three waves a SIMD (two of 256 dims or 32 rows): many short contexts are all
+// latency, of which the waves hide each other's. Times by kShared, kDirect and kLean, 8 K/V heads of 128, a row each: one
+// request of 501 tokens 9.4, 7.7 and 8.5 us; 256 of up to 251 33, 28 and 24 us; 400 of up to 701 81, 74 and 67 us. 100 of up to
+// 401, 4 heads of 256: 30 us shared, 17 lean.
+constexpr int kShared = 0, kDirect = 1, kLean = 2;
+
 // Every wave takes key tiles of its own, with all of a K/V head's rows: codes go from memory into registers and from there to
 // the matrix cores, nothing through LDS, and no wave waits for another before a head's end. HBM bounds it, and the latency
 // of a head's beginning (lengths, table, codes) and end (the four waves' join). Measured, 8 K/V heads of 128: 64 sequences of
@@ -527,7 +535,7 @@ template <int DP, int NT> struct Partial {
 
 template <int DP, int NT> constexpr int waves_lds() { return (2 * NT * (DP / 16) * 64 * 4 + 4 * NT * 16 * 2) * 4; }
 
-template <int DT, int FMT, int DP, int NT, bool LEAN, bool RESHAPED>
+template <int DT, int FMT, int DP, int NT, int DIRECT, bool RESHAPED>
 __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t worker, char* lds)
 {
     constexpr int NP = DT == SLHIP_F32 ? 2 : 1, ND = DP / 16, NH = DP / 64;
@@ -553,7 +561,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
     } cur, next;
     int64_t pos = 0, stop;  // on the line
     int32_t step = 0;
-    if (LEAN || a.direct) {
+    if (DIRECT != kShared || a.direct) {
         cur.i = worker / a.c.heads;
         cur.head = worker - cur.i * a.c.heads;
         const Kv8Request r = kv8_request(a.c, cur.i);
@@ -605,6 +613,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
     };
     if (!share(cur) && !advance(cur)) return;
 
+    constexpr bool LEAN = DIRECT == kLean;
     constexpr bool kEarly = DT != SLHIP_F32 && DP <= 128;  // (f32 queries and 256 dims leave no registers for that)
     // K's codes are loaded again as soon as the first product has used them, V's after the second: each then has the other
     // product and the softmax to arrive in, and the codes need registers once. The next head's first tile and queries are on
@@ -654,7 +663,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
         const Kv8Request r = cur.request();
         const int32_t rows = r.n * a.G, head = cur.head;
         next = cur;
-        const bool another = !LEAN && advance(next);
+        const bool another = DIRECT == kShared && advance(next);
         f16x8 q[NT][NP][NH][2];
         Row row[NT];
         float m[NT], l[NT];
@@ -1209,30 +1218,25 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
 // Matrix tiles of 16 rows that a wave of a many-row tile works on: two where two waves a SIMD find registers for them.
 constexpr int block_tiles(bool f32, int dp) { return dp == 256 || (f32 && dp == 128) ? 1 : 2; }
 
-// Whether direct few-row work has a kernel that holds K's and V's codes in the same registers, one after the other, so that two
-// waves a SIMD find room: heads of short contexts are all latency, of which two thread blocks a CU hide each other's. (289
-// requests of up to 19 tokens, 2 K/V heads of 256: LEAN1 us, by the other kernel LEAN0. Long contexts want the loads in
-// flight: 32 of up to 8000 100 us, so 120.)
-constexpr bool lean(bool f32, int dp) { return dp == 256 && !f32; }
-
 // What a call launches, from what the host knows.
 struct Kv8AttnPlan {
     int32_t wave_tiles;  // few-row launch: 0 none, else matrix tiles of 16 rows (1, 2)
     bool blocks;         // many-row tiles
     bool by_part;        // the few-row join shares out the sums of a head, not its dims
+    bool few_heads;      // of direct work: all have a place at once
 };
 
 // Thread blocks of the many-row tiles, then of the few-row work: one launch, so that neither waits for the other's end.
-template <int DT, int FMT, int DP, int NT, int NB, bool LEAN, bool RESHAPED>
-__global__ __launch_bounds__(256, (DP == 256 && !LEAN) || NT == 2 ? 1 : 2) void kv8_attn(Kv8AttnArgs a)
+template <int DT, int FMT, int DP, int NT, int NB, int DIRECT, bool RESHAPED>
+__global__ __launch_bounds__(256, DIRECT == kShared && (DP == 256 || NT == 2) ? 1 : 2) void kv8_attn(Kv8AttnArgs a)
 {
     extern __shared__ __align__(16) char lds[];
     if constexpr (NT > 0 && NB > 0) {
         const unsigned blocks = gridDim.x - a.workers;
         if (blockIdx.x < blocks) attn_blocks<DT, FMT, DP, NB, RESHAPED>(a, blockIdx.x, lds);
-        else attn_waves<DT, FMT, DP, NT, false, RESHAPED>(a, blockIdx.x - blocks, lds);
+        else attn_waves<DT, FMT, DP, NT, kShared, RESHAPED>(a, blockIdx.x - blocks, lds);
     } else if constexpr (NT > 0) {
-        attn_waves<DT, FMT, DP, NT, LEAN, RESHAPED>(a, blockIdx.x, lds);
+        attn_waves<DT, FMT, DP, NT, DIRECT, RESHAPED>(a, blockIdx.x, lds);
     } else {
         attn_blocks<DT, FMT, DP, NB, RESHAPED>(a, blockIdx.x, lds);
     }
@@ -1247,11 +1251,11 @@ __global__ __launch_bounds__(256) void kv8_attn_join(Kv8AttnArgs a, int64_t wave
 
 template <int DT, int FMT, bool RESHAPED> int kv8_attn_launch(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st);
 
-template <int DT, int FMT, int DP, int NT, int NB, bool RESHAPED, bool LEAN = false>
+template <int DT, int FMT, int DP, int NT, int NB, bool RESHAPED, int DIRECT = kShared>
 static int kv8_attn_start(const Kv8AttnArgs& a, hipStream_t st)
 {
     constexpr int waves = NT > 0 ? waves_lds<DP, NT ? NT : 1>() : 0, blocks = NB > 0 ? blocks_lds<DP>() : 0, lds = waves > blocks ? waves : blocks;
-    const auto kernel = kv8_attn<DT, FMT, DP, NT, NB, LEAN, RESHAPED>;
+    const auto kernel = kv8_attn<DT, FMT, DP, NT, NB, DIRECT, RESHAPED>;
     if (lds > 65536) SLHIP_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     const int64_t grid = (NT > 0 ? a.workers : 0) + (NB > 0 ? (a.share ? a.items + a.share : a.items * a.splits) * a.c.heads : 0);
     kernel<<<static_cast<unsigned>(grid), 256, lds, st>>>(a);
@@ -1262,8 +1266,11 @@ template <int DT, int FMT, int DP, bool RESHAPED> static int kv8_attn_run(const 
 {
     constexpr int NB = block_tiles(DT == SLHIP_F32, DP), NT2 = DP <= 128 ? 2 : 1;  // make_plan asks for two up to 128 dims
     int e;
-    constexpr bool kLean = lean(DT == SLHIP_F32, DP);
-    if (kLean && !p.blocks && a.direct) e = kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED, kLean>(a, st);
+    constexpr int kOne = DP <= 128 ? kDirect : kLean;
+    if (!p.blocks && a.direct) {
+        if (p.wave_tiles == 2) e = kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED, kLean>(a, st);
+        else e = p.few_heads ? kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED, kOne>(a, st) : kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED, kLean>(a, st);
+    }
     else if (p.blocks) e = p.wave_tiles ? kv8_attn_start<DT, FMT, DP, 1, NB, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, 0, NB, RESHAPED>(a, st);
     else e = p.wave_tiles == 1 ? kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED>(a, st);
     if (e) return e;
