@@ -51,12 +51,13 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
     int64_t bytes = 0;
     a->direct = false;
     if (p->wave_tiles) {
-        // Each head gets a thread block of its own, and no second launch, where contexts cannot be long: up to 4 rounds (1024
+        // Each head gets a thread block of its own, and no second launch, where no row can see far: up to 4 rounds (1024
         // tokens), and the more the more heads there are to fill the machine while the longest run. (8 K/V heads of 128, on
         // the line and so: 8 requests of up to 2001 tokens 15 and 16 us, 64 of them 34 and 30, 256 of up to 4001 208 and 198, of
         // up to 8001 367 and 394.)
+        const int64_t tokens = c.bps << c.shift, seen = a->window > 0 && a->window + most + kTile < tokens ? a->window + most + kTile : tokens;
         const int64_t rounds = p->blocks || B * heads < kWorkers ? 4 : B * heads < 2 * kWorkers ? 8 : 16;
-        a->direct = c.bps << c.shift <= rounds * 4 * kTile && (dp < 256 || !p->blocks || B * heads <= kWorkers);
+        a->direct = seen <= rounds * 4 * kTile && (dp < 256 || !p->blocks || B * heads <= kWorkers);
         p->few_heads = B * heads <= kWorkers;
         a->workers = static_cast<int32_t>(a->direct ? B * heads : dp == 256 ? kWorkers / 2 : kWorkers);
         p->by_part = B * heads < 256;

@@ -463,6 +463,46 @@ def test_attention_long(device, fmt, dtype, D, heads, G, bs, new, past):
     _check_y(got, want, bound, "long")
 
 
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", "f32"), ("i8", "bf16")])
+@pytest.mark.parametrize("window", [64, 1000, 1500, 2049, 3900])
+@pytest.mark.parametrize("D,heads,G,new,past", [(64, 2, 4, [1, 2, 1], [4000, 1600, 5]), (128, 1, 2, [12, 16, 3], [3000, 0, 1501]),
+                                                (256, 2, 2, [1, 8], [4100, 2000]), (64, 1, 2, [40, 1, 130], [4000, 3000, 1400])])
+def test_attention_long_windows(device, fmt, dtype, window, D, heads, G, new, past):
+    """Windows of many key tiles in longer contexts, whose borders lie inside tiles, ranges and blocks."""
+    rng = _rng("windows", fmt, dtype, window, D)
+    st = Step(rng, new, past, 32)
+    c = kv8_ref.Cache(fmt, st.blocks, 32, heads, D, fill=rng)
+    q, q64 = _put(rng.standard_normal((st.T, heads * G, D)) * 2, dtype)
+    for max_new in (0, max(new)):
+        with Dev() as d:
+            log(f"kv8_attention long windows {dtype} {fmt} D={D} new={new} past={past} window={window} max_new={max_new}")
+            y = _attend(d, dtype, st, c, q, G, scale=0.125, window=window, max_new=max_new)
+            native.synchronize()
+            got = _from(d.get(y, q.shape, NP[dtype]), dtype)
+        want, bound = kv8_ref.attention(c, q64, st.starts, st.past, st.slots, st.pages, scale=0.125, window=window, dtype=dtype)
+        _check_y(got, want, bound, f"max_new={max_new}")
+
+
+@pytest.mark.parametrize("fmt,dtype", [("i8", "bf16"), ("e4m3", "f32")])
+@pytest.mark.parametrize("B,heads,longest,wide", [(40, 16, 1900, 1), (70, 16, 3000, 1), (20, 4, 900, 1), (20, 4, 900, 200)])
+@pytest.mark.parametrize("D,G,new", [(64, 4, 1), (128, 2, 12), (256, 3, 2)])
+def test_attention_of_uneven_contexts(device, fmt, dtype, B, heads, longest, wide, D, G, new):
+    """Steps of many heads with a thread block each, and with a shared line; one context is as long as may be."""
+    rng = _rng("uneven", fmt, dtype, B, D)
+    past = np.where(rng.random(B) < 0.1, longest, rng.integers(0, 100, B))
+    past[3] = longest
+    st = Step(rng, [new] * B, past, 16, wide=wide)
+    c = kv8_ref.Cache(fmt, st.blocks, 16, heads, D, fill=rng)
+    q, q64 = _put(rng.standard_normal((st.T, heads * G, D)) * 2, dtype)
+    with Dev() as d:
+        log(f"kv8_attention uneven {dtype} {fmt} B={B} heads={heads} D={D} G={G} new={new} longest={longest} wide={wide}")
+        y = _attend(d, dtype, st, c, q, G, scale=0.125, max_new=new)
+        native.synchronize()
+        got = _from(d.get(y, q.shape, NP[dtype]), dtype)
+    want, bound = kv8_ref.attention(c, q64, st.starts, st.past, st.slots, st.pages, scale=0.125, dtype=dtype)
+    _check_y(got, want, bound, "uneven")
+
+
 @pytest.mark.parametrize("fmt,dtype,G,most", [("i8", "f32", 2, 1), ("e4m3", "bf16", 4, 7), ("e4m3", "bf16", 1, 40)])
 @pytest.mark.parametrize("B,wide", [(64, 80), (65, 1), (70, 80), (300, 80), (4500, 1)])
 def test_many_requests(device, fmt, dtype, G, most, B, wide):
