@@ -48,6 +48,8 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
     a->strict = !p->blocks;
     a->block_min = static_cast<int32_t>(few);
     a->block_max = static_cast<int32_t>(limit);
+    // tokens that a row can see at most, and the others of its tile or request
+    const int64_t tokens = c.bps << c.shift, seen = a->window > 0 && a->window + most + kTile < tokens ? a->window + most + kTile : tokens;
     int64_t bytes = 0;
     a->direct = false;
     if (p->wave_tiles) {
@@ -55,7 +57,6 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
         // tokens), and the more the more heads there are to fill the machine while the longest run. (8 K/V heads of 128, on
         // the line and so: 8 requests of up to 2001 tokens 15 and 16 us, 64 of them 34 and 30, 256 of up to 4001 208 and 198, of
         // up to 8001 367 and 394.)
-        const int64_t tokens = c.bps << c.shift, seen = a->window > 0 && a->window + most + kTile < tokens ? a->window + most + kTile : tokens;
         const int64_t rounds = p->blocks || B * heads < kWorkers ? 4 : B * heads < 2 * kWorkers ? 8 : 16;
         a->direct = seen <= rounds * 4 * kTile && (dp < 256 || !p->blocks || B * heads <= kWorkers);
         p->few_heads = B * heads <= kWorkers;
@@ -70,14 +71,16 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
         a->tile_tokens = static_cast<int32_t>(tile / G);
         a->items = item_count(T, B, a->tile_tokens, 1);
         a->part2 = a->part + bytes / 4;
-        const int64_t pairs = a->items * heads, longest = (c.bps << c.shift) / (kLeastCut * kTile) + 1;
-        if (pairs <= kFewTiles && B <= 64 && a->items * longest < 1 << 27) {
+        // A range of less than 8 key tiles does not earn its partial sums and the join (a prompt of 400, 32 query heads of 128 on
+        // 8, bf16: whole 20 us, in two 22; of 700 27 and 25; 5 requests of 250 to 433, 16 heads of 96 on 2: 22 and 34).
+        const int64_t pairs = a->items * heads, most_cuts = seen / (8 * kTile);
+        if (most_cuts >= 2 && pairs <= kFewTiles && B <= 64 && a->items * tokens / kTile < 1 << 28) {
             a->share = static_cast<int32_t>((kBlockUnits + heads - 1) / heads);
             bytes += (a->items + a->share) * heads * floats * 4;
-        } else if (pairs < kBlockUnits) {
+        } else if (most_cuts >= 2 && pairs < kBlockUnits) {
             const int64_t s = (kBlockUnits + pairs - 1) / pairs;
-            a->splits = static_cast<int32_t>(s < longest ? s : longest);
-            if (a->splits > 1) bytes += pairs * a->splits * floats * 4;
+            a->splits = static_cast<int32_t>(s < most_cuts ? s : most_cuts);
+            bytes += pairs * a->splits * floats * 4;
         }
     }
     return bytes;
