@@ -58,7 +58,7 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
         // the line and so: 8 requests of up to 2001 tokens 15 and 16 us, 64 of them 34 and 30, 256 of up to 4001 208 and 198, of
         // up to 8001 367 and 394.)
         const int64_t rounds = p->blocks || B * heads < kWorkers ? 4 : B * heads < 2 * kWorkers ? 8 : 16;
-        a->direct = seen <= rounds * 4 * kTile && (dp < 256 || !p->blocks || B * heads <= kWorkers);
+        a->direct = seen <= rounds * 4 * kTile;
         p->few_heads = B * heads <= kWorkers;
         a->workers = static_cast<int32_t>(a->direct ? B * heads : dp == 256 ? kWorkers / 2 : kWorkers);
         p->by_part = B * heads < 256;
@@ -67,7 +67,7 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
     a->splits = 1;
     a->share = 0;
     if (p->blocks) {
-        const int64_t tile = 64 * block_tiles(dtype == SLHIP_F32, static_cast<int>(dp)), floats = tile * dp + tile * 2;
+        const int64_t tile = 16 * block_waves(static_cast<int>(dp)) * block_tiles(dtype == SLHIP_F32, static_cast<int>(dp)), floats = tile * dp + tile * 2;
         a->tile_tokens = static_cast<int32_t>(tile / G);
         a->items = item_count(T, B, a->tile_tokens, 1);
         a->part2 = a->part + bytes / 4;

@@ -1000,6 +1000,10 @@ template <int DT, int DP, int NT> __device__ __forceinline__ void join_blocks(co
 // it next to the matrix cores. Measured: a prompt of 8192, 32 query heads of 128 on 8, bf16 and E4M3, 557 us (990 TFLOP/s of
 // the 1310 that a large bf16 product reaches) at 2.25 GHz, 612 us at the 2.05 that the clock falls to under a long load;
 // vector unit 66% and matrix cores 42% of the cycles.
+// Of 256 dims the tiles take most of a CU's LDS; there one thread block has eight waves, for two on each SIMD. (A prompt of
+// 4096, 16 query heads of 256 on 4, bf16: 276 us with four waves, 170 with eight; 150 of 30 to 574, 16 on 8, f32: 1048 and 757.)
+constexpr int block_waves(int dp) { return dp == 256 ? 8 : 4; }
+
 template <int DP> struct BlockTile {
     static constexpr int kK = 4 * (DP / 32), kV = (DP / 16) * 2;  // fragments of K: t, h, s; of V: dt, s
 };
@@ -1010,7 +1014,7 @@ template <int DT, int FMT, int DP, int NT, bool RESHAPED>
 __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t index, char* lds)
 {
     constexpr int NP = DT == SLHIP_F32 ? 2 : 1, ND = DP / 16, NH = DP / 64;
-    constexpr int kK = BlockTile<DP>::kK, kV = BlockTile<DP>::kV;
+    constexpr int kK = BlockTile<DP>::kK, kV = BlockTile<DP>::kV, W = block_waves(DP);
     f16x8* s_frag = reinterpret_cast<f16x8*>(lds);  // [2][kK + kV][64]
     const int lane = threadIdx.x & 63, wave = wave_id(), c = lane & 15, g = lane >> 4, D = a.c.D;
     const int32_t head = static_cast<int32_t>(index % a.c.heads);
@@ -1035,17 +1039,18 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
     }
     const int32_t all = r.past + r.n;  // keys of the request: codes behind them are not read as keys
 
-    // Staging: wave w takes the codes of K's product t = w and of V's dims 16 (w + 4 j). Table entries are a tile ahead of
+    // Staging: wave w takes codes of K's product t = w % 4 (of eight waves, half its dims) and of V's dims 16 (w + W j). Table entries are a tile ahead of
     // the codes that they lead to, codes are loaded two tiles ahead of the products that take them and converted one tile
     // ahead. Past the range's last tile that one is loaded again.
-    constexpr int VJ = ND / 4;
-    uint4 ck[NH], cv[VJ];
+    constexpr int KJ = 4 * NH / W, VJ = ND / W;
+    const int h0 = (wave >> 2) * KJ;
+    uint4 ck[KJ], cv[VJ];
     SubBlock next;
     float ksn, vsn;
     int32_t kid, vid;
     const HeadBase base = head_base(a.c, head);
     // the lane's first codes in a sub-block (dims past D: any codes, q is 0 there and the sums are not stored)
-    const uint8_t* const kbase = base.k + (4 * wave + (c & 3)) * D + (16 * g < D ? 16 * g : 0);
+    const uint8_t* const kbase = base.k + (4 * (wave & 3) + (c & 3)) * D + (16 * g < D ? 16 * g : 0);
     const uint8_t* const vbase = base.v + (16 * wave < D ? 256 * wave : 0) + c * 16;
     const int32_t border = max(first + ((end - first - 1) & ~(kTile - 1)), 0);  // the last tile
     const auto look = [&](int32_t key) __attribute__((always_inline)) {
@@ -1059,10 +1064,10 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
         next = sub_block(a.c, vid, at + 16 * g, all);
         const uint8_t* k = kbase + codes_at(base, kb);
 #pragma unroll
-        for (int h = 0; h < NH; h++) ck[h] = *reinterpret_cast<const uint4*>(k + (64 * h + 16 * g < D ? 64 * h : 0));
+        for (int h = 0; h < KJ; h++) ck[h] = *reinterpret_cast<const uint4*>(k + (64 * (h0 + h) + 16 * g < D ? 64 * (h0 + h) : 0));
         const uint8_t* v = vbase + codes_at(base, next);
 #pragma unroll
-        for (int j = 0; j < VJ; j++) cv[j] = *reinterpret_cast<const uint4*>(v + (16 * (wave + 4 * j) < D ? 1024 * j : 0));
+        for (int j = 0; j < VJ; j++) cv[j] = *reinterpret_cast<const uint4*>(v + (16 * (wave + W * j) < D ? 256 * W * j : 0));
         const uint64_t scales = static_cast<uint64_t>(next.id) * base.scales;
         ksn = *reinterpret_cast<const float*>(base.ks + scales);
         vsn = *reinterpret_cast<const float*>(base.vs + scales);
@@ -1074,10 +1079,10 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
             for (int j = 0; j < VJ; j++) cv[j] = first_codes(cv[j], next.keys);
         }
     };
-    const auto stage = [&](f16x8* f, int i) __attribute__((always_inline)) {  // load i of the NH + VJ
+    const auto stage = [&](f16x8* f, int i) __attribute__((always_inline)) {  // load i of the KJ + VJ
         f16x8 x, z;
-        const int at = i < NH ? (wave * NH + i) * 2 : kK + (wave + 4 * (i - NH)) * 2;
-        codes_f16<FMT>(i < NH ? ck[i < NH ? i : 0] : cv[i < NH ? 0 : i - NH], x, z);
+        const int at = i < KJ ? ((wave & 3) * NH + h0 + i) * 2 : kK + (wave + W * (i - KJ)) * 2;
+        codes_f16<FMT>(i < KJ ? ck[i < KJ ? i : 0] : cv[i < KJ ? 0 : i - KJ], x, z);
         f[at * 64] = x;
         f[(at + 1) * 64] = z;
     };
@@ -1108,7 +1113,7 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
         };
         clip();
 #pragma unroll
-        for (int i = 0; i < NH + VJ; i++) stage(s_frag + lane, i);
+        for (int i = 0; i < KJ + VJ; i++) stage(s_frag + lane, i);
         TileScale sc = scales(first);
         int32_t keys = next.keys;
         load(first + kTile);
@@ -1145,7 +1150,7 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
                 for (int p = 0; p < NP; p++)
 #pragma unroll
                     for (int n = 0; n < NT; n++) S[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[i % R], q[n][p][j % NH][s], S[n][t], 0, 0, 0);
-                if (i % (kK / (NH + VJ)) == 0 && i / (kK / (NH + VJ)) < NH + VJ) stage(g2, i / (kK / (NH + VJ)));
+                if (i % (kK / (KJ + VJ)) == 0 && i / (kK / (KJ + VJ)) < KJ + VJ) stage(g2, i / (kK / (KJ + VJ)));
                 __builtin_amdgcn_sched_barrier(0);
             }
             const TileScale sn = scales(key + kTile);
@@ -1194,7 +1199,7 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
             keys = keys_next;
         }
     }
-    float* part = a.part2 + ((cut.first + cut.split) * a.c.heads + head) * Partial<DP, 4 * NT>::kFloats;
+    float* part = a.part2 + ((cut.first + cut.split) * a.c.heads + head) * Partial<DP, W * NT>::kFloats;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int32_t at = (wave * NT + n) * 16 + c;
@@ -1208,7 +1213,7 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
         } else {
 #pragma unroll
             for (int dt = 0; dt < ND; dt++) reinterpret_cast<f32x4*>(part)[((wave * NT + n) * ND + dt) * 64 + lane] = o[n][dt];
-            if (g == 0) reinterpret_cast<float2*>(part + Partial<DP, 4 * NT>::kDims)[at] = make_float2(m[n], l[n]);
+            if (g == 0) reinterpret_cast<float2*>(part + Partial<DP, W * NT>::kDims)[at] = make_float2(m[n], l[n]);
         }
     }
 }
@@ -1226,9 +1231,11 @@ struct Kv8AttnPlan {
     bool few_heads;      // of direct work: all have a place at once
 };
 
+constexpr int block_threads(int dp, int nb) { return nb > 0 ? 64 * block_waves(dp) : 256; }
+
 // Thread blocks of the many-row tiles, then of the few-row work: one launch, so that neither waits for the other's end.
 template <int DT, int FMT, int DP, int NT, int NB, int DIRECT, bool RESHAPED>
-__global__ __launch_bounds__(256, DIRECT == kShared && (DP == 256 || NT == 2) ? 1 : 2) void kv8_attn(Kv8AttnArgs a)
+__global__ __launch_bounds__(block_threads(DP, NB), DIRECT == kShared && (NB == 0 && DP == 256 || NT == 2) ? 1 : 2) void kv8_attn(Kv8AttnArgs a)
 {
     extern __shared__ __align__(16) char lds[];
     if constexpr (NT > 0 && NB > 0) {
@@ -1246,7 +1253,7 @@ template <int DT, int DP, int NT, int NB, bool BY_PART>
 __global__ __launch_bounds__(256) void kv8_attn_join(Kv8AttnArgs a, int64_t wave_joins)
 {
     if (blockIdx.x < wave_joins) join_waves<DT, DP, NT, BY_PART>(a, blockIdx.x);
-    else join_blocks<DT, DP, 4 * NB>(a, blockIdx.x - wave_joins);
+    else join_blocks<DT, DP, block_waves(DP) * NB>(a, blockIdx.x - wave_joins);
 }
 
 template <int DT, int FMT, bool RESHAPED> int kv8_attn_launch(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st);
@@ -1258,24 +1265,29 @@ static int kv8_attn_start(const Kv8AttnArgs& a, hipStream_t st)
     const auto kernel = kv8_attn<DT, FMT, DP, NT, NB, DIRECT, RESHAPED>;
     if (lds > 65536) SLHIP_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     const int64_t grid = (NT > 0 ? a.workers : 0) + (NB > 0 ? (a.share ? a.items + a.share : a.items * a.splits) * a.c.heads : 0);
-    kernel<<<static_cast<unsigned>(grid), 256, lds, st>>>(a);
+    kernel<<<static_cast<unsigned>(grid), block_threads(DP, NB), lds, st>>>(a);
     return check_launch("kv8_attn");
 }
 
 template <int DT, int FMT, int DP, bool RESHAPED> static int kv8_attn_run(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
 {
     constexpr int NB = block_tiles(DT == SLHIP_F32, DP), NT2 = DP <= 128 ? 2 : 1;  // make_plan asks for two up to 128 dims
-    int e;
     constexpr int kOne = DP <= 128 ? kDirect : kLean;
-    if (!p.blocks && a.direct) {
-        if (p.wave_tiles == 2) e = kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED, kLean>(a, st);
+    int e = SLHIP_OK;
+    if constexpr (DP <= 128) {
+        if (p.blocks && p.wave_tiles) e = kv8_attn_start<DT, FMT, DP, 1, NB, RESHAPED>(a, st);
+    }
+    const bool both = DP <= 128 && p.blocks && p.wave_tiles;  // (of 256 dims the two want different thread blocks: two launches)
+    if (p.blocks && !both) e = kv8_attn_start<DT, FMT, DP, 0, NB, RESHAPED>(a, st);
+    if (e) return e;
+    if (p.wave_tiles && !both) {
+        if (p.wave_tiles == 2) e = a.direct ? kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED, kLean>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED>(a, st);
+        else if (!a.direct) e = kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED>(a, st);
         else e = p.few_heads ? kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED, kOne>(a, st) : kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED, kLean>(a, st);
     }
-    else if (p.blocks) e = p.wave_tiles ? kv8_attn_start<DT, FMT, DP, 1, NB, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, 0, NB, RESHAPED>(a, st);
-    else e = p.wave_tiles == 1 ? kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED>(a, st);
     if (e) return e;
     const int64_t waves = p.wave_tiles && !a.direct ? static_cast<int64_t>(a.c.B) * a.c.heads * p.wave_tiles * (p.by_part ? DP / 16 : 1) : 0;
-    const int64_t blocks = p.blocks && (a.share || a.splits > 1) ? a.items * a.c.heads * 4 * NB : 0;
+    const int64_t blocks = p.blocks && (a.share || a.splits > 1) ? a.items * a.c.heads * block_waves(DP) * NB : 0;
     if (waves + blocks == 0) return SLHIP_OK;
     const unsigned grid = static_cast<unsigned>(waves + blocks);
     if (p.wave_tiles == 2) {
