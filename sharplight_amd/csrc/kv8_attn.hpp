@@ -428,7 +428,7 @@ constexpr int kShared = 0, kDirect = 1, kLean = 2;
 // the matrix cores, nothing through LDS, and no wave waits for another before a head's end. HBM bounds it, and the latency
 // of a head's beginning (lengths, table, codes) and end (the four waves' join). Measured, 8 K/V heads of 128: 64 sequences of
 // 1 to 4095 tokens, bf16 and E4M3, 61 us with the join (264 MB, 4.3 TB/s); 2 of up to 131000, f32 and int8, 66 us (337 MB,
-// 5.1 TB/s). Of 4 heads of 256, whose codes leave registers for one wave a SIMD: 16 windows of 4096 tokens 33 us (2.8 TB/s).
+// 5.1 TB/s). Of 4 heads of 256, whose codes leave registers for one wave a SIMD: 16 windows of 4096 tokens 31 us (2.9 TB/s).
 
 // The work of all requests of a launch, in rounds of four key tiles (one for each wave of a thread block), is one line --
 // request by request, head by head -- that `workers` thread blocks share out in equal pieces, whatever the lengths are. A
