@@ -372,7 +372,7 @@ template <int NP> __device__ __forceinline__ void tile_weights(TileRow& t, int s
     }
 }
 
-__device__ __forceinline__ TileScale tile_scale(const Kv8Dev& c, const SubBlock& s, float ks, float vs)
+__device__ __forceinline__ TileScale tile_scale(float ks, float vs)
 {
     // a scale that is NaN makes the weights of the keys that are seen NaN, and must not reach l through those that are not
     const int e = static_cast<int>(__float_as_uint(vs) >> 23 & 0xFF) - 127;
@@ -701,7 +701,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
 #pragma unroll
                                 for (int n = 0; n < NT; n++) S[n][t + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[u][s], q[n][e][h][s], S[n][t + u], 0, 0, 0);
                 }
-            TileScale sc = tile_scale(a.c, vb, ks, vs);
+            TileScale sc = tile_scale(ks, vs);
             const int32_t keys = vb.keys;
             if (vb.bad) raise_block(a.c, r.first, r.slot, key + 16 * g, vb.entry);
             if constexpr (LEAN) {
@@ -1105,7 +1105,7 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
     }
     if (first < end) {
         const auto scales = [&](int32_t key) __attribute__((always_inline)) {
-            TileScale sc = tile_scale(a.c, next, ksn, vsn);
+            TileScale sc = tile_scale(ksn, vsn);
             // in registers of their own, or the next scales' arrival is waited for to move them
             asm volatile("" : "+v"(sc.k), "+v"(sc.ev), "+v"(sc.down));
             if (next.bad && wave == 0) raise_block(a.c, r.first, r.slot, min(key, border) + 16 * g, next.entry);
