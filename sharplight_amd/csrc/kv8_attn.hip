@@ -31,7 +31,7 @@ constexpr int64_t kFewTiles = kBlockUnits / 4;
 // What a call over T rows of B requests launches. Few-row work takes a request whose rows fit one or two matrix tiles (16
 // or 32 rows a K/V head): its keys are then read once by single waves. Everything else goes to thread blocks that share
 // key tiles among 64 or 128 rows. Where the host cannot tell (max_new unknown or large, several requests) one launch holds
-// both and each leaves the other's requests alone. Fills what of `a` the kernels go by; returns the workspace's bytes.
+// both (of 256 dims two do) and each leaves the other's requests alone. Fills what of `a` the kernels go by; returns the workspace's bytes.
 static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, Kv8AttnPlan* p)
 {
     const Kv8Dev& c = a->c;
