@@ -3,19 +3,24 @@
 
 namespace slhip {
 
-template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_I8, false>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
-template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_E4M3, false>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
-template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_I8, false>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
-template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_E4M3, false>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
-template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_I8, true>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
-template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_E4M3, true>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
-template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_I8, true>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
-template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_E4M3, true>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_I8, kPlain>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_E4M3, kPlain>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_I8, kPlain>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_E4M3, kPlain>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_I8, kReshaped>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_E4M3, kReshaped>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_I8, kReshaped>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_E4M3, kReshaped>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_I8, kFarCap>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
+template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_E4M3, kFarCap>(const Kv8AttnArgs&, const Kv8AttnPlan&, hipStream_t);
 
 template <int DT, int FMT> static int launch(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
 {
+    if constexpr (DT == SLHIP_BF16) {
+        if (a.cap > kFastCap) return kv8_attn_launch<DT, FMT, kFarCap>(a, p, st);
+    }
     const bool reshaped = a.cap > 0.0f || a.slopes || !(a.scale > 0.0f);
-    return reshaped ? kv8_attn_launch<DT, FMT, true>(a, p, st) : kv8_attn_launch<DT, FMT, false>(a, p, st);
+    return reshaped ? kv8_attn_launch<DT, FMT, kReshaped>(a, p, st) : kv8_attn_launch<DT, FMT, kPlain>(a, p, st);
 }
 
 constexpr int64_t kWorkers = 512;     // two thread blocks a CU (one of 256 dims)

@@ -41,6 +41,16 @@ constexpr float kExact = 0x1p20f;
 constexpr int kLeastCut = 4;  // key tiles of a many-row tile that are worth a thread block of their own
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kStart = 2;
+
+// What becomes of a score before its exponential: nothing but the scale; a cap, slopes or a scale that is not positive; or a cap
+// above kFastCap, for bf16 activations in kernels of their own (f32 ones cap all scores alike).
+// Up to kFastCap the scores of bf16 activations are capped by tanh y = 1 - 2 / (1 + e^(2 y)), off by up to 2^-22 whatever y is: a
+// score by 2^-22 of the cap, its weight by 2^-14 of itself at most (2^-16 with a cap of 50), whose f16 part is off by 2^-11.
+// It takes half of tanh_f's instructions: prompts of 188 to 1978, 64 query heads of 64, 255 us, with tanh_f 349. (As a branch in one
+// kernel tanh_f costs the others two registers more, and a third wave a SIMD: a prompt of 4096, 32 heads of 64, int8: 162 us, 176.)
+constexpr int kPlain = 0, kReshaped = 1, kFarCap = 2;
+constexpr float kFastCap = 256.0f;
+
 constexpr float kNone = -1e30f;  // a maximum of nothing: finite, so that differences with -inf stay numbers
 
 struct Kv8AttnArgs {
@@ -285,25 +295,23 @@ struct TileRow {
 // Scores, and the row's M (m, in TileRow's terms). M need not be the maximum: it moves up to it only where the maximum is above
 // it by more than kSlack, so that the sums so far are seldom multiplied (rescale; a row's maximum moves in every second tile
 // of the first 64, and 32 or 64 products a tile are as many as its exponentials). lo <= j < hi are the keys that are seen.
-template <int DT, bool RESHAPED, class Rescale>
+template <int DT, int SCORES, class Rescale>
 __device__ __forceinline__ void tile_max(const Kv8AttnArgs& a, const f32x4 (&products)[4], const Row& row, const TileScale& sc, int32_t key0,
                                          int lo, int hi, bool masked, float& m, TileRow& t, const Rescale& rescale)
 {
     // t = fma(S, mul, add) with mul > 0, so the largest S is the largest t. Capped or sloped scores, and those of a scale that
-    // is not positive (RESHAPED), are turned into t themselves.
+    // is not positive, are turned into t themselves.
     float (&S)[16] = t.S;
     float mul = fmaxf(row.back * sc.k * kLog2e, 1.17549435e-38f), add = sc.ev;  // (a masked S is -inf: not times 0)
 #pragma unroll
     for (int j = 0; j < 16; j++) S[j] = products[j >> 2][j & 3];
-    if constexpr (RESHAPED) {
+    if constexpr (SCORES != kPlain) {
         if (a.cap > 0.0f) {
             const float in = row.back * sc.k * a.cap_inverse, out = a.cap * kLog2e;
-            if constexpr (DT == SLHIP_F32) {
+            if constexpr (DT == SLHIP_F32 || SCORES == kFarCap) {
 #pragma unroll
                 for (int j = 0; j < 16; j++) S[j] = fmaf(tanh_f(S[j] * in), out, add);
             } else {
-                // tanh y = 1 - 2 / (1 + e^(2 y)), off by up to 2^-22: 2^-16 of a weight with a cap of 50, whose f16 part is
-                // off by 2^-11. (Half of tanh_f's instructions: prompts of 188 to 1978, 64 query heads of 64: 255 us, with tanh_f 349.)
                 const float twice = in * (2.0f * kLog2e), both = out + add;
 #pragma unroll
                 for (int j = 0; j < 16; j++)
@@ -535,7 +543,7 @@ template <int DP, int NT> struct Partial {
 
 template <int DP, int NT> constexpr int waves_lds() { return (2 * NT * (DP / 16) * 64 * 4 + 4 * NT * 16 * 2) * 4; }
 
-template <int DT, int FMT, int DP, int NT, int DIRECT, bool RESHAPED>
+template <int DT, int FMT, int DP, int NT, int DIRECT, int SCORES>
 __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t worker, char* lds)
 {
     constexpr int NP = DT == SLHIP_F32 ? 2 : 1, ND = DP / 16, NH = DP / 64;
@@ -722,7 +730,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
                 const int hi = min(row[n].pos - k0l + 1, keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
                 const bool masked = __any(hi < 16 || lo > 0);
                 TileRow t;
-                tile_max<DT, RESHAPED>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], t, [&](float alpha) __attribute__((always_inline)) {
+                tile_max<DT, SCORES>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], t, [&](float alpha) __attribute__((always_inline)) {
                     l[n] *= alpha;
 #pragma unroll
                     for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
@@ -1010,7 +1018,7 @@ template <int DP> struct BlockTile {
 
 template <int DP> constexpr int blocks_lds() { return 2 * (BlockTile<DP>::kK + BlockTile<DP>::kV) * 64 * static_cast<int>(sizeof(f16x8)); }
 
-template <int DT, int FMT, int DP, int NT, bool RESHAPED>
+template <int DT, int FMT, int DP, int NT, int SCORES>
 __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t index, char* lds)
 {
     constexpr int NP = DT == SLHIP_F32 ? 2 : 1, ND = DP / 16, NH = DP / 64;
@@ -1164,7 +1172,7 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
                 const int k0l = key + 16 * g;
                 const int hi = min(row[n].pos - k0l + 1, keys), lo = a.window > 0 ? row[n].pos - a.window + 1 - k0l : 0;
                 const bool masked = __any(hi < 16 || lo > 0);
-                tile_max<DT, RESHAPED>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], t[n], [&](float alpha) __attribute__((always_inline)) {
+                tile_max<DT, SCORES>(a, S[n], row[n], sc, k0l, lo, hi, masked, m[n], t[n], [&](float alpha) __attribute__((always_inline)) {
                     l[n] *= alpha;
 #pragma unroll
                     for (int dt = 0; dt < ND; dt++) o[n][dt] *= alpha;
@@ -1234,18 +1242,18 @@ struct Kv8AttnPlan {
 constexpr int block_threads(int dp, int nb) { return nb > 0 ? 64 * block_waves(dp) : 256; }
 
 // Thread blocks of the many-row tiles, then of the few-row work: one launch, so that neither waits for the other's end.
-template <int DT, int FMT, int DP, int NT, int NB, int DIRECT, bool RESHAPED>
+template <int DT, int FMT, int DP, int NT, int NB, int DIRECT, int SCORES>
 __global__ __launch_bounds__(block_threads(DP, NB), DIRECT == kShared && (NB == 0 && DP == 256 || NT == 2) ? 1 : 2) void kv8_attn(Kv8AttnArgs a)
 {
     extern __shared__ __align__(16) char lds[];
     if constexpr (NT > 0 && NB > 0) {
         const unsigned blocks = gridDim.x - a.workers;
-        if (blockIdx.x < blocks) attn_blocks<DT, FMT, DP, NB, RESHAPED>(a, blockIdx.x, lds);
-        else attn_waves<DT, FMT, DP, NT, kShared, RESHAPED>(a, blockIdx.x - blocks, lds);
+        if (blockIdx.x < blocks) attn_blocks<DT, FMT, DP, NB, SCORES>(a, blockIdx.x, lds);
+        else attn_waves<DT, FMT, DP, NT, kShared, SCORES>(a, blockIdx.x - blocks, lds);
     } else if constexpr (NT > 0) {
-        attn_waves<DT, FMT, DP, NT, DIRECT, RESHAPED>(a, blockIdx.x, lds);
+        attn_waves<DT, FMT, DP, NT, DIRECT, SCORES>(a, blockIdx.x, lds);
     } else {
-        attn_blocks<DT, FMT, DP, NB, RESHAPED>(a, blockIdx.x, lds);
+        attn_blocks<DT, FMT, DP, NB, SCORES>(a, blockIdx.x, lds);
     }
 }
 
@@ -1256,34 +1264,34 @@ __global__ __launch_bounds__(256) void kv8_attn_join(Kv8AttnArgs a, int64_t wave
     else join_blocks<DT, DP, block_waves(DP) * NB>(a, blockIdx.x - wave_joins);
 }
 
-template <int DT, int FMT, bool RESHAPED> int kv8_attn_launch(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st);
+template <int DT, int FMT, int SCORES> int kv8_attn_launch(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st);
 
-template <int DT, int FMT, int DP, int NT, int NB, bool RESHAPED, int DIRECT = kShared>
+template <int DT, int FMT, int DP, int NT, int NB, int SCORES, int DIRECT = kShared>
 static int kv8_attn_start(const Kv8AttnArgs& a, hipStream_t st)
 {
     constexpr int waves = NT > 0 ? waves_lds<DP, NT ? NT : 1>() : 0, blocks = NB > 0 ? blocks_lds<DP>() : 0, lds = waves > blocks ? waves : blocks;
-    const auto kernel = kv8_attn<DT, FMT, DP, NT, NB, DIRECT, RESHAPED>;
+    const auto kernel = kv8_attn<DT, FMT, DP, NT, NB, DIRECT, SCORES>;
     if (lds > 65536) SLHIP_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     const int64_t grid = (NT > 0 ? a.workers : 0) + (NB > 0 ? (a.share ? a.items + a.share : a.items * a.splits) * a.c.heads : 0);
     kernel<<<static_cast<unsigned>(grid), block_threads(DP, NB), lds, st>>>(a);
     return check_launch("kv8_attn");
 }
 
-template <int DT, int FMT, int DP, bool RESHAPED> static int kv8_attn_run(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
+template <int DT, int FMT, int DP, int SCORES> static int kv8_attn_run(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
 {
     constexpr int NB = block_tiles(DT == SLHIP_F32, DP), NT2 = DP <= 128 ? 2 : 1;  // make_plan asks for two up to 128 dims
     constexpr int kOne = DP <= 128 ? kDirect : kLean;
     int e = SLHIP_OK;
     if constexpr (DP <= 128) {
-        if (p.blocks && p.wave_tiles) e = kv8_attn_start<DT, FMT, DP, 1, NB, RESHAPED>(a, st);
+        if (p.blocks && p.wave_tiles) e = kv8_attn_start<DT, FMT, DP, 1, NB, SCORES>(a, st);
     }
     const bool both = DP <= 128 && p.blocks && p.wave_tiles;  // (of 256 dims the two want different thread blocks: two launches)
-    if (p.blocks && !both) e = kv8_attn_start<DT, FMT, DP, 0, NB, RESHAPED>(a, st);
+    if (p.blocks && !both) e = kv8_attn_start<DT, FMT, DP, 0, NB, SCORES>(a, st);
     if (e) return e;
     if (p.wave_tiles && !both) {
-        if (p.wave_tiles == 2) e = a.direct ? kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED, kLean>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0, RESHAPED>(a, st);
-        else if (!a.direct) e = kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED>(a, st);
-        else e = p.few_heads ? kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED, kOne>(a, st) : kv8_attn_start<DT, FMT, DP, 1, 0, RESHAPED, kLean>(a, st);
+        if (p.wave_tiles == 2) e = a.direct ? kv8_attn_start<DT, FMT, DP, NT2, 0, SCORES, kLean>(a, st) : kv8_attn_start<DT, FMT, DP, NT2, 0, SCORES>(a, st);
+        else if (!a.direct) e = kv8_attn_start<DT, FMT, DP, 1, 0, SCORES>(a, st);
+        else e = p.few_heads ? kv8_attn_start<DT, FMT, DP, 1, 0, SCORES, kOne>(a, st) : kv8_attn_start<DT, FMT, DP, 1, 0, SCORES, kLean>(a, st);
     }
     if (e) return e;
     const int64_t waves = p.wave_tiles && !a.direct ? static_cast<int64_t>(a.c.B) * a.c.heads * p.wave_tiles * (p.by_part ? DP / 16 : 1) : 0;
@@ -1300,11 +1308,11 @@ template <int DT, int FMT, int DP, bool RESHAPED> static int kv8_attn_run(const 
     return check_launch("kv8_attn_join");
 }
 
-template <int DT, int FMT, bool RESHAPED> int kv8_attn_by_dim(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
+template <int DT, int FMT, int SCORES> int kv8_attn_by_dim(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
 {
-    if (a.c.D <= 64) return kv8_attn_run<DT, FMT, 64, RESHAPED>(a, p, st);
-    if (a.c.D <= 128) return kv8_attn_run<DT, FMT, 128, RESHAPED>(a, p, st);
-    return kv8_attn_run<DT, FMT, 256, RESHAPED>(a, p, st);
+    if (a.c.D <= 64) return kv8_attn_run<DT, FMT, 64, SCORES>(a, p, st);
+    if (a.c.D <= 128) return kv8_attn_run<DT, FMT, 128, SCORES>(a, p, st);
+    return kv8_attn_run<DT, FMT, 256, SCORES>(a, p, st);
 }
 
 }  // namespace slhip

@@ -3,9 +3,9 @@
 
 namespace slhip {
 
-template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_E4M3, false>(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
+template <> int kv8_attn_launch<SLHIP_BF16, SLHIP_KV8_E4M3, kPlain>(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
 {
-    return kv8_attn_by_dim<SLHIP_BF16, SLHIP_KV8_E4M3, false>(a, p, st);
+    return kv8_attn_by_dim<SLHIP_BF16, SLHIP_KV8_E4M3, kPlain>(a, p, st);
 }
 
 }  // namespace slhip

@@ -3,9 +3,9 @@
 
 namespace slhip {
 
-template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_I8, true>(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
+template <> int kv8_attn_launch<SLHIP_F32, SLHIP_KV8_I8, kReshaped>(const Kv8AttnArgs& a, const Kv8AttnPlan& p, hipStream_t st)
 {
-    return kv8_attn_by_dim<SLHIP_F32, SLHIP_KV8_I8, true>(a, p, st);
+    return kv8_attn_by_dim<SLHIP_F32, SLHIP_KV8_I8, kReshaped>(a, p, st);
 }
 
 }  // namespace slhip

@@ -1,0 +1,67 @@
+"""GPU tests of the paged 8-bit cache at the limits of what its calls take."""
+import numpy as np
+import pytest
+
+from sharplight_amd import native
+from tests import kv8_ref
+from tests.devutil import Dev, log
+from tests.test_gpu_kv8 import NP, Step, _attend, _cache, _check_y, _from, _pattern, _put, _rng
+
+pytestmark = pytest.mark.gpu
+
+# new, past, wide: a thread block a head; a shared line; row tiles; row tiles beside few rows
+SHAPES = [([1, 1, 3], [0, 300, 65], 1), ([1, 1, 3], [0, 300, 65], 200), ([150], [90], 1), ([150, 20, 1], [0, 90, 333], 200)]
+
+
+def _scores(c, st, q, G, scale):
+    """The largest |z| that some row sees, before a cap."""
+    top = 0.0
+    for i, s in enumerate(st.slots):
+        n = int(st.past[i]) + st.new[i]
+        for h in range(c.heads):
+            k = c.keys(st.pages[s, :-(-n // st.bs)], h)[0][:n]
+            rows = q[st.starts[i]:st.starts[i + 1], h * G:(h + 1) * G].reshape(-1, c.D)
+            top = max(top, float(np.abs(scale * (rows @ k.T)).max(initial=0)))
+    return top
+
+
+# ---- caps ------------------------------------------------------------------------------------------------------------
+
+def _capped(fmt, dtype, cap, new, past, wide, D):
+    """A cap far above the scores changes them by |z|^3 / (3 cap^2) at most, so y lies within the bound of uncapped attention and what
+    the cap's arithmetic adds (below 1000, where it changes more, within the statement's bound, which grants 2^-22 of the cap). That is relative to z: the products by 1 / cap and by cap log2(e) and their factors, eight roundings
+    of 2^-24, and 2^-21 for tanh (2^-22 of itself, of an argument off by 2^-22). A score that is off by d moves y by 2 d max|v| at most."""
+    rng = _rng("caps", fmt, dtype, cap, len(new))
+    heads, G, bs = 2, 2, 16
+    st = Step(rng, new, past, bs, wide=wide)
+    c = kv8_ref.Cache(fmt, st.blocks, bs, heads, D, fill=rng)
+    q, q64 = _put(rng.standard_normal((st.T, heads * G, D)) * 3, dtype)
+    scale = 0.125
+    with Dev() as d:
+        log(f"kv8_attention cap={cap} {dtype} {fmt} D={D} new={new} wide={wide}")
+        y = _attend(d, dtype, st, c, q, G, scale=scale, softcap=cap)
+        native.synchronize()
+        got = _from(d.get(y, q.shape, NP[dtype]), dtype)
+    cap = float(np.float32(cap))
+    want, _ = kv8_ref.attention(c, q64, st.starts, st.past, st.slots, st.pages, scale=scale, softcap=cap, dtype=dtype)
+    if cap < 1e3:
+        _, bound = kv8_ref.attention(c, q64, st.starts, st.past, st.slots, st.pages, scale=scale, softcap=cap, dtype=dtype)
+        return _check_y(got, want, bound, cap, _pattern(dtype))
+    _, bound = kv8_ref.attention(c, q64, st.starts, st.past, st.slots, st.pages, scale=scale, dtype=dtype)
+    z = _scores(c, st, q64, G, scale)
+    most = kv8_ref.QMAX[fmt] * float(c.vs.max())
+    _check_y(got, want, bound + 2 * most * ((8 * 2.0 ** -24 + 2.0 ** -21) * z + z ** 3 / (3 * cap * cap)), cap, _pattern(dtype))
+
+
+@pytest.mark.parametrize("fmt,dtype", [("i8", "f32"), ("e4m3", "f32"), ("i8", "bf16"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("cap", [4e3, 1e5, 1e7, 1e9])
+@pytest.mark.parametrize("new,past,wide", SHAPES)
+def test_caps_above_the_scores(device, fmt, dtype, cap, new, past, wide):
+    _capped(fmt, dtype, cap, new, past, wide, 64)
+
+
+@pytest.mark.parametrize("cap", [255.0, 256.0, 257.0, 1e6])
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("new,past,wide", SHAPES[1:3])
+def test_caps_above_the_scores_of_wider_heads(device, cap, D, new, past, wide):
+    _capped("i8", "bf16", cap, new, past, wide, D)
