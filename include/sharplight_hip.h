@@ -545,7 +545,7 @@ SLHIP_API int slhip_kv8_write(int dtype, const void* k, int64_t k_stride_t, int6
  * work: workspace of work_bytes >= slhip_kv8_attention_work_bytes(...), 16-byte aligned, for the sums of key ranges that
  * are worked on apart; calls that may overlap each need their own. It needs no initialisation and keeps nothing.
  * Products of f32 activations are exact to 2^-22 (two f16 parts each), those of bf16 with the softmax weights in f16;
- * sums are f32. A cap adds 2^-21 of z; for bf16 activations and caps of up to 256, 2^-22 of the cap.
+ * sums are f32. A cap adds 2^-21 of z; for bf16 activations and caps of up to 256, 2^-22 of the cap. One above 2^60 counts as none.
  */
 typedef struct slhip_kv8_attn {
     float scale, softcap;

@@ -143,11 +143,14 @@ extern "C" SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q
     a.yh = y_stride_h;
     a.G = static_cast<int32_t>(q_heads / a.c.heads);
     a.scale = cfg->scale;
-    a.cap = cfg->softcap;
+    // A cap above 2^60 counts as none: scores below 2^49 differ by less than 2^-24 of themselves from capped ones, and above that
+    // (up to the cap) the largest is alone either way. Of a cap below 2^-60 its inverse counts as 2^60: all scores are 0 to 2^-60.
+    // In between 1 / cap times a score's factor stays a normal number.
+    a.cap = cfg->softcap > 0x1p60f ? 0.0f : cfg->softcap;
     a.window = cfg->window > 0x7FFFFFFF ? 0 : static_cast<int32_t>(cfg->window);  // no context is that long
     a.slopes = cfg->slopes;
     a.part = static_cast<float*>(work);
-    a.cap_inverse = 1.0f / a.cap;
+    a.cap_inverse = a.cap < 0x1p-60f ? 0x1p60f : 1.0f / a.cap;
     Kv8AttnPlan p;
     const int64_t need = make_plan(dtype, a.G, cfg->max_new, &a, &p);
     if (need > 0 && (!work || !aligned16(work) || work_bytes < need))

@@ -307,7 +307,8 @@ __device__ __forceinline__ void tile_max(const Kv8AttnArgs& a, const f32x4 (&pro
     for (int j = 0; j < 16; j++) S[j] = products[j >> 2][j & 3];
     if constexpr (SCORES != kPlain) {
         if (a.cap > 0.0f) {
-            const float in = row.back * sc.k * a.cap_inverse, out = a.cap * kLog2e;
+            // (in: no infinity times a product of 0)
+            const float in = __builtin_amdgcn_fmed3f(row.back * sc.k * a.cap_inverse, -0x1p126f, 0x1p126f), out = a.cap * kLog2e;
             if constexpr (DT == SLHIP_F32 || SCORES == kFarCap) {
 #pragma unroll
                 for (int j = 0; j < 16; j++) S[j] = fmaf(tanh_f(S[j] * in), out, add);

@@ -65,3 +65,32 @@ def test_caps_above_the_scores(device, fmt, dtype, cap, new, past, wide):
 @pytest.mark.parametrize("new,past,wide", SHAPES[1:3])
 def test_caps_above_the_scores_of_wider_heads(device, cap, D, new, past, wide):
     _capped("i8", "bf16", cap, new, past, wide, D)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("i8", "f32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("cap", [1e30, 1e38, 3.4e38])
+@pytest.mark.parametrize("new,past,wide", SHAPES)
+def test_caps_at_the_end_of_the_range(device, fmt, dtype, cap, new, past, wide):
+    _capped(fmt, dtype, cap, new, past, wide, 64)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("i8", "f32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("cap", [1e-6, 1.5e-38, 1e-39, 1e-45])
+@pytest.mark.parametrize("new,past,wide", SHAPES)
+def test_caps_near_zero(device, fmt, dtype, cap, new, past, wide):
+    """Every score is about 0, that of a key of zeros among them: y is the mean of what a row sees. (The statement's bound counts the
+    products before the cap too, so the capped scores' own error, at most the cap, is far inside it.)"""
+    rng = _rng("tiny caps", fmt, dtype, cap, len(new))
+    st = Step(rng, new, past, 16, wide=wide)
+    c = kv8_ref.Cache(fmt, st.blocks, 16, 2, 64, fill=rng)
+    c.k[:, :, 3::5] = 0
+    q, q64 = _put(rng.standard_normal((st.T, 4, 64)) * np.exp2(rng.integers(0, 40, (st.T, 4, 1))), dtype)
+    with Dev() as d:
+        log(f"kv8_attention cap={cap} {dtype} {fmt} new={new} wide={wide}")
+        y = _attend(d, dtype, st, c, q, 2, scale=0.125, softcap=cap)
+        native.synchronize()
+        got = _from(d.get(y, q.shape, NP[dtype]), dtype)
+    cap = float(np.float32(cap))
+    want, _ = kv8_ref.attention(c, q64, st.starts, st.past, st.slots, st.pages, scale=0.125, softcap=cap, dtype=dtype)
+    _, bound = kv8_ref.attention(c, q64 * 2.0 ** -40, st.starts, st.past, st.slots, st.pages, scale=0.125, dtype=dtype)
+    _check_y(got, want, bound + 4 * cap * kv8_ref.QMAX[fmt] * float(c.vs.max()), cap, _pattern(dtype))
