@@ -51,7 +51,7 @@ constexpr int kStart = 2;
 constexpr int kPlain = 0, kReshaped = 1, kFarCap = 2;
 constexpr float kFastCap = 256.0f;
 
-constexpr float kNone = -1e30f;  // a maximum of nothing: finite, so that differences with -inf stay numbers
+constexpr float kNone = -3.40282347e38f;  // a maximum of nothing: the least number, so that differences with -inf stay numbers
 
 struct Kv8AttnArgs {
     Kv8Dev c;

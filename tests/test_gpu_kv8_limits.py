@@ -94,3 +94,35 @@ def test_caps_near_zero(device, fmt, dtype, cap, new, past, wide):
     want, _ = kv8_ref.attention(c, q64, st.starts, st.past, st.slots, st.pages, scale=0.125, softcap=cap, dtype=dtype)
     _, bound = kv8_ref.attention(c, q64 * 2.0 ** -40, st.starts, st.past, st.slots, st.pages, scale=0.125, dtype=dtype)
     _check_y(got, want, bound + 4 * cap * kv8_ref.QMAX[fmt] * float(c.vs.max()), cap, _pattern(dtype))
+
+
+# ---- scores and queries at the end of the range ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kw", [dict(), dict(slopes=True), dict(window=200)])
+@pytest.mark.parametrize("new,past,wide", [([1, 2], [130, 500], 1), ([1, 2], [130, 500], 200), ([40, 50], [130, 500], 1), ([60, 1], [130, 500], 200)])
+def test_scores_far_below_zero(device, dtype, kw, new, past, wide):
+    """Scores of -2^108 to -2^125, of which a row's highest is higher by a quarter, so its key's value is the answer. (The others' weights
+    are 0: the rest is y's rounding and 2^-11 or 2^-22 of it for the weight, which cancels.)"""
+    rng = _rng("far below", dtype, str(kw), len(new), new[0])
+    st = Step(rng, new, past, 16, wide=wide)
+    D, heads, G = 64, 2, 2
+    c = kv8_ref.Cache("i8", st.blocks, 16, heads, D, fill=rng)
+    c.k[:], c.ks[:], c.vs[:] = 0, 1.0, 1.0
+    c.k[..., 0] = 256 - 120
+    best = [p - 5 for p in past]  # every row of the request sees it, inside a window too
+    for i, s in enumerate(st.slots):
+        c.k[st.pages[s, best[i] // 16], :, best[i] % 16, 0] = 256 - 90
+    q = np.zeros((st.T, heads * G, D))
+    q[..., 0] = np.exp2(rng.integers(102, 118, (st.T, heads * G)))
+    bits, _ = _put(q, dtype)
+    with Dev() as d:
+        log(f"kv8_attention scores far below zero {dtype} {kw} new={new} wide={wide}")
+        slopes = d.put(np.full(heads * G, 0.25, np.float32)) if "slopes" in kw else None
+        y = _attend(d, dtype, st, c, bits, G, scale=1.0, slopes=slopes, window=kw.get("window", 0))
+        native.synchronize()
+        got = _from(d.get(y, bits.shape, NP[dtype]), dtype)
+    for i, s in enumerate(st.slots):
+        v = c.v.view(np.int8)[st.pages[s, best[i] // 16], :, 0, :, best[i] % 16].astype(np.float64)  # [heads, D]
+        rows = got[st.starts[i]:st.starts[i + 1]].reshape(-1, heads, G, D)
+        assert (np.abs(rows - v[None, :, None]) <= np.abs(v[None, :, None]) * 2.0 ** (-20 if dtype == "f32" else -7)).all(), i
