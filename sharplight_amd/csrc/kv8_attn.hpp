@@ -243,9 +243,11 @@ __device__ __forceinline__ Row make_row(const Kv8AttnArgs& a, const Kv8Request& 
     }
     top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
     top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
-    // multiply by 2^(14 - e): biased exponents; rows that are tiny, or not finite, by a power that stays in range
-    const int e = static_cast<int>(top >> 23) - 127, up = e > 127 ? 0 : 14 - max(e, -100);
-    const float mul = __uint_as_float(static_cast<uint32_t>(127 + min(up, 114)) << 23);
+    // multiply by 2^(14 - e): biased exponents; rows that are tiny by a power that stays in range. A row that is not finite is NaN;
+    // under a cap an infinity is more than the largest number (and has one f16 part).
+    const bool finite = top < 0x7F800000u;
+    const int e = static_cast<int>(top >> 23) - 127, up = 14 - max(min(e, 127), -100);
+    const float mul = finite || a.cap > 0.0f ? __uint_as_float(static_cast<uint32_t>(127 + up) << 23) : __uint_as_float(0x7FC00000u);
 #pragma unroll
     for (int h = 0; h < DP / 64; h++)
 #pragma unroll
@@ -257,7 +259,7 @@ __device__ __forceinline__ Row make_row(const Kv8AttnArgs& a, const Kv8Request& 
                 q[0][h][s][j] = hi.x;
                 q[0][h][s][j + 1] = hi.y;
                 if constexpr (NP == 2) {
-                    const f16x2 lo = to_f16x2(x0 - static_cast<float>(hi.x), x1 - static_cast<float>(hi.y));
+                    const f16x2 lo = to_f16x2(finite ? x0 - static_cast<float>(hi.x) : 0.0f, finite ? x1 - static_cast<float>(hi.y) : 0.0f);
                     q[1][h][s][j] = lo.x;
                     q[1][h][s][j + 1] = lo.y;
                 }

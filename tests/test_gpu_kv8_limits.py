@@ -126,3 +126,43 @@ def test_scores_far_below_zero(device, dtype, kw, new, past, wide):
         v = c.v.view(np.int8)[st.pages[s, best[i] // 16], :, 0, :, best[i] % 16].astype(np.float64)  # [heads, D]
         rows = got[st.starts[i]:st.starts[i + 1]].reshape(-1, heads, G, D)
         assert (np.abs(rows - v[None, :, None]) <= np.abs(v[None, :, None]) * 2.0 ** (-20 if dtype == "f32" else -7)).all(), i
+
+
+@pytest.mark.parametrize("fmt,dtype", [("i8", "f32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("new,past,wide", [([1, 1, 3], [0, 300, 65], 1), ([1, 1, 3], [0, 300, 65], 200), ([150, 20, 1], [0, 90, 333], 200)])
+def test_queries_that_are_not_finite(device, fmt, dtype, new, past, wide):
+    """A row with an infinity or a NaN has no softmax: it is NaN, also where all its scores are -infinity, and no other row is. Under a cap
+    an infinity counts as the cap."""
+    rng = _rng("not finite", fmt, dtype, len(new), new[0])
+    st = Step(rng, new, past, 16, wide=wide)
+    c = kv8_ref.Cache(fmt, st.blocks, 16, 2, 64, fill=rng)
+    one = 0x38 if fmt == "e4m3" else 1
+    minus = 0xB8 if fmt == "e4m3" else 0xFF
+    c.k[..., 0], c.k[..., 1], c.k[..., 2] = one, minus, np.where(rng.random(c.k.shape[:-1]) < 0.5, one, minus)
+    x = rng.standard_normal((st.T, 4, 64)) * 3
+    kind = rng.integers(0, 6, (st.T, 4))  # 0: -inf to all keys, 1: the same by a negative value, 2: either sign, 3: NaN, others finite
+    kind[0] = [0, 1, 2, 4]
+    x[kind == 0, 1], x[kind == 1, 0], x[kind == 2, 2], x[kind == 3, 9] = np.inf, -np.inf, np.inf, np.nan
+    x[kind == 2, 5] = 1e30  # far beyond the others, and nothing beside an infinity
+    q, q64 = _put(x, dtype)
+    fine = np.where((kind > 3)[..., None], q64, 0.0)
+    cap, scale = 4.0, 0.125
+    for softcap in (0.0, cap):
+        with Dev() as d:
+            log(f"kv8_attention queries not finite {dtype} {fmt} new={new} wide={wide} cap={softcap}")
+            y = _attend(d, dtype, st, c, q, 2, scale=scale, softcap=softcap)
+            native.synchronize()
+            got = _from(d.get(y, q.shape, NP[dtype]), dtype)
+        want, bound = kv8_ref.attention(c, fine, st.starts, st.past, st.slots, st.pages, scale=scale, softcap=softcap, dtype=dtype)
+        lost = kind <= 3 if softcap == 0 else kind == 3
+        assert np.isnan(got[lost]).all(), np.argwhere(lost & ~np.isnan(got).all(-1))[:4].tolist()
+        if softcap:  # the scores of an infinity: +-cap, as a query of that size along the one dim gives them without a cap
+            sure = np.zeros(q64.shape)
+            for k, dim, sign in ((0, 1, 1), (1, 0, -1), (2, 2, 1)):
+                sure[kind == k, dim] = sign
+            flat = c.copy()
+            flat.ks[:] = 1.0
+            w2, b2 = kv8_ref.attention(flat, sure, st.starts, st.past, st.slots, st.pages, scale=cap, dtype=dtype)
+            turned = (kind <= 2)[..., None]
+            want, bound = np.where(turned, w2, want), np.where(turned, b2 + 2 * 2.0 ** -22 * cap * kv8_ref.QMAX[fmt] * float(c.vs.max()), bound)
+        _check_y(np.where(lost[..., None], want, got), want, bound, softcap)
