@@ -189,7 +189,7 @@ __device__ __forceinline__ uint64_t codes_at(const HeadBase& h, const SubBlock& 
 // Query row `row` (token * G + head of the group) of a request, or none.
 struct Row {
     int32_t pos;
-    float back;   // scale of the scores: scale / the power of two that the row was multiplied by
+    float back;   // scale of the scores (under a cap, of what the cap takes): scale / the power of two that the row was multiplied by
     float slope;  // slopes[h] * log2(e)
 };
 
@@ -226,7 +226,7 @@ __device__ __forceinline__ void fetch_row(const Kv8AttnArgs& a, const Kv8Request
 }
 
 // NP f16 parts of the row's lane share: q[p][h][s] holds dims 64h + 16g + 8s + (0..7). Dims past D are 0.
-template <int DT, int DP, int NP>
+template <int DT, int DP, int NP, int SCORES>
 __device__ __forceinline__ Row make_row(const Kv8AttnArgs& a, const Kv8Request& r, int32_t head, int32_t row, bool valid,
                                         const RawRow<DT, DP>& raw, f16x8 (&q)[NP][DP / 64][2])
 {
@@ -245,9 +245,9 @@ __device__ __forceinline__ Row make_row(const Kv8AttnArgs& a, const Kv8Request& 
     top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
     // multiply by 2^(14 - e): biased exponents; rows that are tiny by a power that stays in range. A row that is not finite is NaN;
     // under a cap an infinity is more than the largest number (and has one f16 part).
-    const bool finite = top < 0x7F800000u;
+    const bool capped = SCORES != kPlain && a.cap > 0.0f, finite = top < 0x7F800000u;
     const int e = static_cast<int>(top >> 23) - 127, up = 14 - max(min(e, 127), -100);
-    const float mul = finite || a.cap > 0.0f ? __uint_as_float(static_cast<uint32_t>(127 + up) << 23) : __uint_as_float(0x7FC00000u);
+    const float mul = finite || capped ? __uint_as_float(static_cast<uint32_t>(127 + up) << 23) : __uint_as_float(0x7FC00000u);
 #pragma unroll
     for (int h = 0; h < DP / 64; h++)
 #pragma unroll
@@ -267,6 +267,9 @@ __device__ __forceinline__ Row make_row(const Kv8AttnArgs& a, const Kv8Request& 
     Row o;
     o.pos = r.past + tok;
     o.back = a.scale / mul;
+    // Finite after a block's scale too, or a product of 0 would be no number. (Products are multiples of 2^-33, scales at least
+    // 2^-40: what is not 0 is past the cap with 2^86 already.)
+    if (capped) o.back = __builtin_amdgcn_fmed3f(o.back * a.cap_inverse, -0x1p86f, 0x1p86f);
     o.slope = a.slopes ? a.slopes[qh] * kLog2e : 0.0f;
     return o;
 }
@@ -309,8 +312,7 @@ __device__ __forceinline__ void tile_max(const Kv8AttnArgs& a, const f32x4 (&pro
     for (int j = 0; j < 16; j++) S[j] = products[j >> 2][j & 3];
     if constexpr (SCORES != kPlain) {
         if (a.cap > 0.0f) {
-            // (in: no infinity times a product of 0)
-            const float in = __builtin_amdgcn_fmed3f(row.back * sc.k * a.cap_inverse, -0x1p126f, 0x1p126f), out = a.cap * kLog2e;
+            const float in = row.back * sc.k, out = a.cap * kLog2e;
             if constexpr (DT == SLHIP_F32 || SCORES == kFarCap) {
 #pragma unroll
                 for (int j = 0; j < 16; j++) S[j] = fmaf(tanh_f(S[j] * in), out, add);
@@ -681,7 +683,7 @@ __device__ __forceinline__ void attn_waves(const Kv8AttnArgs& a, const int32_t w
         f32x4 o[NT][ND];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            row[n] = make_row<DT, DP, NP>(a, r, head, 16 * n + c, 16 * n + c < rows, raw[n], q[n]);
+            row[n] = make_row<DT, DP, NP, SCORES>(a, r, head, 16 * n + c, 16 * n + c < rows, raw[n], q[n]);
             m[n] = kNone;
             l[n] = 0.0f;
 #pragma unroll
@@ -1108,7 +1110,7 @@ __device__ __forceinline__ void attn_blocks(const Kv8AttnArgs& a, const int64_t 
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int32_t at = row0 + (wave * NT + n) * 16 + c;
-        row[n] = make_row<DT, DP, NP>(a, r, head, at, at < row1, raw[n], q[n]);
+        row[n] = make_row<DT, DP, NP, SCORES>(a, r, head, at, at < row1, raw[n], q[n]);
         m[n] = kNone;
         l[n] = 0.0f;
 #pragma unroll
