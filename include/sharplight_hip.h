@@ -537,7 +537,8 @@ SLHIP_API int slhip_kv8_write(int dtype, const void* k, int64_t k_stride_t, int6
  *   z_j = scale * (q . K_j); softcap > 0: z_j = softcap * tanh(z_j / softcap); slopes: z_j += slopes[h] * (j - p);
  *   window > 0: only j > p - window;  y = sum_j softmax(z)_j V_j.
  * q and y (dtype f32 or bf16, both the same; strides in elements, innermost 1) are [T, q_heads, head_dim]; y may be q.
- * q_heads a multiple of heads, at most 64 query heads for each. A row that sees no key is 0. requests *
+ * q_heads a multiple of heads, at most 64 query heads for each. A row that sees no key is 0, one that holds an
+ * infinity or a NaN and sees one NaN (under a cap an infinity is past it). requests *
  * (blocks_per_slot * block_size / 256 + 3) < 2^31.
  * max_new: no request brings more rows (0: unknown); a request that does is reported (SLHIP_ERR_CACHE) and its rows are
  * left as they were, as are those of a request that does not fit the batch or the table. A block id outside the cache is

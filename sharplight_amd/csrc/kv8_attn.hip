@@ -1,4 +1,7 @@
 // Entry points of the attention over the 8-bit paged cache: checks, and what a call launches (kernels: kv8_attn.hpp).
+#include <float.h>
+#include <math.h>
+
 #include "kv8_attn.hpp"
 
 namespace slhip {
@@ -19,7 +22,7 @@ template <int DT, int FMT> static int launch(const Kv8AttnArgs& a, const Kv8Attn
     if constexpr (DT == SLHIP_BF16) {
         if (a.cap > kFastCap) return kv8_attn_launch<DT, FMT, kFarCap>(a, p, st);
     }
-    const bool reshaped = a.cap > 0.0f || a.slopes || !(a.scale > 0.0f);
+    const bool reshaped = a.cap > 0.0f || a.slopes || !(a.factor > 0.0f);
     return reshaped ? kv8_attn_launch<DT, FMT, kReshaped>(a, p, st) : kv8_attn_launch<DT, FMT, kPlain>(a, p, st);
 }
 
@@ -142,7 +145,6 @@ extern "C" SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q
     a.yt = y_stride_t;
     a.yh = y_stride_h;
     a.G = static_cast<int32_t>(q_heads / a.c.heads);
-    a.scale = cfg->scale;
     // A cap above 2^60 counts as none: scores below 2^49 differ by less than 2^-24 of themselves from capped ones, and above that
     // (up to the cap) the largest is alone either way. Of a cap below 2^-60 its inverse counts as 2^60: all scores are 0 to 2^-60.
     // In between 1 / cap times a score's factor stays a normal number.
@@ -150,7 +152,10 @@ extern "C" SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q
     a.window = cfg->window > 0x7FFFFFFF ? 0 : static_cast<int32_t>(cfg->window);  // no context is that long
     a.slopes = cfg->slopes;
     a.part = static_cast<float*>(work);
-    a.cap_inverse = a.cap < 0x1p-60f ? 0x1p60f : 1.0f / a.cap;
+    const bool capped = a.cap > 0.0f;
+    a.factor = cfg->scale * (!capped ? 1.0f : a.cap < 0x1p-60f ? 0x1p60f : 1.0f / a.cap);
+    a.most = capped ? 0x1p86f : FLT_MAX;
+    a.lost = capped ? 0x1p-113f : NAN;  // under a cap an infinity is more than the largest number, which is multiplied by that
     Kv8AttnPlan p;
     const int64_t need = make_plan(dtype, a.G, cfg->max_new, &a, &p);
     if (need > 0 && (!work || !aligned16(work) || work_bytes < need))

@@ -59,7 +59,9 @@ struct Kv8AttnArgs {
     void* y;
     int64_t qt, qh, yt, yh;
     int32_t G;                   // query heads of a K/V head
-    float scale, cap, cap_inverse;
+    float cap;
+    float factor, most;          // of what the cap takes (scale / cap), or of the scores; its largest size in a row
+    float lost;                  // what a row that is not finite is multiplied by
     int32_t window;              // 0: none
     const float* slopes;
     int32_t min_rows, max_rows;    // few-row work: requests of (min_rows, max_rows] query rows a K/V head
@@ -189,7 +191,7 @@ __device__ __forceinline__ uint64_t codes_at(const HeadBase& h, const SubBlock& 
 // Query row `row` (token * G + head of the group) of a request, or none.
 struct Row {
     int32_t pos;
-    float back;   // scale of the scores (under a cap, of what the cap takes): scale / the power of two that the row was multiplied by
+    float back;   // factor / the power of two that the row was multiplied by
     float slope;  // slopes[h] * log2(e)
 };
 
@@ -245,9 +247,10 @@ __device__ __forceinline__ Row make_row(const Kv8AttnArgs& a, const Kv8Request& 
     top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
     // multiply by 2^(14 - e): biased exponents; rows that are tiny by a power that stays in range. A row that is not finite is NaN;
     // under a cap an infinity is more than the largest number (and has one f16 part).
-    const bool capped = SCORES != kPlain && a.cap > 0.0f, finite = top < 0x7F800000u;
-    const int e = static_cast<int>(top >> 23) - 127, up = 14 - max(min(e, 127), -100);
-    const float mul = finite || capped ? __uint_as_float(static_cast<uint32_t>(127 + up) << 23) : __uint_as_float(0x7FC00000u);
+    const bool finite = top < 0x7F800000u;
+    const int e = static_cast<int>(top >> 23) - 127;
+    const float power = __uint_as_float(static_cast<uint32_t>(127 + 14 - max(e, -100)) << 23);
+    const float mul = finite ? power : SCORES == kPlain ? __uint_as_float(0x7FC00000u) : a.lost;
 #pragma unroll
     for (int h = 0; h < DP / 64; h++)
 #pragma unroll
@@ -259,17 +262,18 @@ __device__ __forceinline__ Row make_row(const Kv8AttnArgs& a, const Kv8Request& 
                 q[0][h][s][j] = hi.x;
                 q[0][h][s][j + 1] = hi.y;
                 if constexpr (NP == 2) {
-                    const f16x2 lo = to_f16x2(finite ? x0 - static_cast<float>(hi.x) : 0.0f, finite ? x1 - static_cast<float>(hi.y) : 0.0f);
+                    const bool two = SCORES == kPlain || finite;
+                    const f16x2 lo = to_f16x2(two ? x0 - static_cast<float>(hi.x) : 0.0f, two ? x1 - static_cast<float>(hi.y) : 0.0f);
                     q[1][h][s][j] = lo.x;
                     q[1][h][s][j + 1] = lo.y;
                 }
             }
     Row o;
     o.pos = r.past + tok;
-    o.back = a.scale / mul;
-    // Finite after a block's scale too, or a product of 0 would be no number. (Products are multiples of 2^-33, scales at least
-    // 2^-40: what is not 0 is past the cap with 2^86 already.)
-    if (capped) o.back = __builtin_amdgcn_fmed3f(o.back * a.cap_inverse, -0x1p86f, 0x1p86f);
+    o.back = a.factor / mul;
+    // Finite after a block's scale too, or a product of 0 would be no number under a cap. (Products are multiples of 2^-33, scales
+    // at least 2^-40: what is not 0 is past the cap with 2^86 already.)
+    if (SCORES != kPlain) o.back = __builtin_amdgcn_fmed3f(o.back, -a.most, a.most);
     o.slope = a.slopes ? a.slopes[qh] * kLog2e : 0.0f;
     return o;
 }
