@@ -24,6 +24,7 @@ struct Kv8WriteArgs {
     const void* x[2];
     int64_t st[2], sh[2];
     int64_t tile, extra;  // items by blocks (block_size, 2) or by tokens (1, 0)
+    int64_t items;        // thread blocks behind them look for requests that do not fit
     int32_t chunks;       // D / 8, and its reciprocal: n / chunks = n * inverse >> 16 for n < 512
     int32_t inverse;
 };
@@ -140,10 +141,19 @@ __global__ __launch_bounds__(1024) void kv8_write(Kv8WriteArgs a)
     __shared__ uint32_t s_max[16];
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int bs = 1 << c.shift, wpi = bs >> 4;  // waves per item
+    // A request that does not fit may have no item: one that begins behind the last row, or brings none. So each is looked at here,
+    // by a thread.
+    if (blockIdx.x >= a.items) {
+        const int64_t i = (blockIdx.x - a.items) * blockDim.x + threadIdx.x;
+        if (blockIdx.y == 0 && i < c.B) {
+            const Kv8Request r = kv8_request(c, static_cast<int32_t>(i));
+            if (r.bad) raise_request(c, static_cast<int32_t>(i), r);
+        }
+        return;
+    }
     const Kv8Item it = kv8_find(c, blockIdx.x, a.tile, a.extra);
     const Kv8Request& r = it.r;
     const int pair = static_cast<int>(blockIdx.y) * (static_cast<int>(blockDim.x >> 6) / wpi) + wave / wpi, sub = wave % wpi;
-    if (r.bad && it.piece == 0 && blockIdx.y == 0 && threadIdx.x == 0) raise_request(c, it.i, r);
     // everything above is the same for all of the thread block: nothing is left waiting at the barrier below
     const int b0 = r.past >> c.shift;
     if (r.n == 0 || it.piece < 0 || it.piece > ((r.past + r.n - 1) >> c.shift) - b0) return;
@@ -358,8 +368,10 @@ extern "C" SLHIP_API int slhip_kv8_write(int dtype, const void* k, int64_t k_str
     a.extra = by_block ? 2 : 0;
     const int64_t items = by_block ? item_count(a.c.T, a.c.B, bs, 2) : a.c.T;
     const unsigned wpi = static_cast<unsigned>(bs >> 4), threads = 64 * (wpi < 4 ? 4 : wpi), per = threads / 64 / wpi;
-    if (items * threads > 0xFFFFFFFFll) return fail(SLHIP_ERR_UNSUPPORTED, "kv8_write: too many rows");  // a launch's threads
-    const dim3 grid(static_cast<unsigned>(items), (2 * a.c.heads + per - 1) / per);
+    a.items = items;
+    const int64_t blocks = items + (a.c.B + threads - 1) / threads;
+    if (blocks * threads > 0xFFFFFFFFll) return fail(SLHIP_ERR_UNSUPPORTED, "kv8_write: too many rows");  // a launch's threads
+    const dim3 grid(static_cast<unsigned>(blocks), (2 * a.c.heads + per - 1) / per);
     const int w = error_word(&a.c.err);
     if (w) return w;
     hipStream_t st = to_stream(stream);

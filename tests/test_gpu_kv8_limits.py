@@ -5,7 +5,7 @@ import pytest
 from sharplight_amd import native
 from tests import kv8_ref
 from tests.devutil import Dev, log
-from tests.test_gpu_kv8 import NP, Step, _attend, _cache, _check_y, _from, _pattern, _put, _rng
+from tests.test_gpu_kv8 import NP, Step, _attend, _cache, _check_write, _check_y, _from, _pattern, _put, _rng, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -166,3 +166,36 @@ def test_queries_that_are_not_finite(device, fmt, dtype, new, past, wide):
             turned = (kind <= 2)[..., None]
             want, bound = np.where(turned, w2, want), np.where(turned, b2 + 2 * 2.0 ** -22 * cap * kv8_ref.QMAX[fmt] * float(c.vs.max()), bound)
         _check_y(np.where(lost[..., None], want, got), want, bound, softcap)
+
+
+# ---- requests and tables that do not fit ---------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("B", [3, 64, 70, 5000])
+@pytest.mark.parametrize("bad", ["a row too many", "slot of no rows", "past of no rows"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_write_reports_requests_without_rows_of_their_own(device, B, bad, new):
+    """A request that begins behind the step's last row, and one that brings nothing but does not fit: reported like any other, and the
+    others are written."""
+    if new > 1 and B > 100:
+        B = 130
+    rng = _rng("reports", B, bad, new)
+    counts, past = np.full(B, new), rng.integers(0, 40, B)
+    at = B - 1 if bad == "a row too many" else int(rng.integers(0, B))
+    counts[at] = 1 if bad == "a row too many" else 0
+    st = Step(rng, counts.tolist(), past, 16)
+    if bad == "a row too many":
+        st.T -= 1
+    elif bad == "slot of no rows":
+        st.slots[at] = len(st.pages) + 5
+    else:
+        st.past[at] = st.pages.shape[1] * 16 + 1
+    c = kv8_ref.Cache("i8", st.blocks, 16, 2, 32, fill=rng)
+    k, k64 = _put(_values(rng, (st.T, 2, 32)), "f32")
+    with Dev() as d:
+        cache, where = _cache(d, c)
+        log(f"kv8_write of {B} requests, {bad}")
+        native.kv8_write("f32", d.put(k), d.put(k), cache, st.batch(d))
+        with pytest.raises(native.SlhipCacheError, match=f"Request {at} .*does not fit"):
+            native.synchronize()
+        kv8_ref.write(c, k64, k64, st.starts, st.past, st.slots, st.pages)
+        _check_write(d, c, where, bad)
