@@ -463,9 +463,10 @@ SLHIP_API int slhip_cache_write(int dtype_in, int dtype_cache, const void* x, in
  *
  * n_free_out may be n_free itself (one counter that the steps of a captured loop advance) or another word (the old count
  * stays, to step back to). All or nothing: where a length is negative, a context would outgrow its table row or the rows
- * `tokens`, a slot is outside the table or named twice, or the free list has too few ids (too little room), the tables,
- * the list and the count stay as they were (*n_free_out = *n_free), starts are 0, every row is padding, and the next
- * slhip_stream_sync reports SLHIP_ERR_CACHE. Arrays are int32; seq and pos may be NULL.
+ * `tokens`, a slot is outside the table or named twice, the free list has too few ids (too little room), or a block to be
+ * released is not in the table (its entry is negative: it was released before), the tables, the list and the count stay as
+ * they were (*n_free_out = *n_free), starts are 0, every row is padding, and the next slhip_stream_sync reports
+ * SLHIP_ERR_CACHE. Arrays are int32; seq and pos may be NULL.
  * requests <= 4096, page_slots <= 131072, block_size a power of two, blocks_per_slot * block_size < 2^31, tokens < 2^31.
  * Sizes of zero are fine (no requests: starts[0] = 0, all rows padding).
  */

@@ -10,7 +10,8 @@
 // table, so no thread block waits for another's stores. Only the free list's count can be written where it is read (in
 // place); a step of many rows then has its rows in a second launch.
 // Measured: 64 requests of a token 4.4 us, 333 requests of 1 to 200 tokens (some 33000 rows) 6.2 us; an empty launch takes 2.5.
-// With kBlockRows = 4096 the latter took 10.4 us, and with the rows in a second launch 10.0.
+// With kBlockRows = 4096 the latter took 10.4 us, and with the rows in a second launch 10.0. A release is one thread block's too: 64
+// requests of 256 blocks 19 us, of 8192 432.
 #include "common.hpp"
 #include "kv8_map.hpp"
 
@@ -37,7 +38,7 @@ struct KvPagesArgs {
     uint32_t* err;
 };
 
-enum : uint32_t { kBadLength = 1, kBadSlot = 2, kBadRows = 3, kBadFree = 4 };
+enum : uint32_t { kBadLength = 1, kBadSlot = 2, kBadRows = 3, kBadFree = 4, kBadEntry = 5 };
 
 __device__ __forceinline__ int64_t blocks_of(int64_t tokens, int shift) { return (tokens + (int64_t{1} << shift) - 1) >> shift; }
 
@@ -121,18 +122,9 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
         if (!RELEASE && all_tokens > a.tokens) bad = kBadRows;
         else if (!room) bad = kBadFree;
     }
-    const bool ok = bad == 0xFFFFFFFFu, first = blockIdx.x == 0;
-    if (first && tid == 0) {
-        if (!ok) {
-            const int i = min(static_cast<int>(bad >> 3), a.B - 1);
-            const int64_t count = RELEASE || i < 0 ? 0 : a.count[i];
-            raise_error(a.err, kErrKvPages, max(i, 0), i < 0 ? 0 : slot_of(i), i < 0 ? 0 : a.past[i], static_cast<uint32_t>(count),
-                        static_cast<uint32_t>(static_cast<uint64_t>(count) >> 32), bad & 7);
-        }
-        *a.n_free_out = static_cast<int32_t>(!ok ? n_free : RELEASE ? n_free + all_blocks : n_free - all_blocks);
-    }
+    const bool first = blockIdx.x == 0;
+    bool ok = bad == 0xFFFFFFFFu;
     if (!ok) all_tokens = all_blocks = 0;
-
     for (int i = i0; i < i1; i++) {
         s_start[i] = static_cast<int32_t>(st);
         s_off[i] = static_cast<int32_t>(so);
@@ -144,28 +136,84 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     }
     if (!RELEASE && first && tid == 0) a.starts[a.B] = static_cast<int32_t>(all_tokens);
     __syncthreads();
-
+    const auto request_of = [&](const int32_t* sums, int64_t k) {
+        return static_cast<int32_t>(item_request([&](int64_t r) { return sums[r]; }, a.B, k, 1, 0));
+    };
+    // What goes back has to be there (a request that was released before has no entries), so all entries are looked at before one is
+    // moved. Up to kHeld a thread are looked up once, all searches and loads on their way together; of more, a request is searched
+    // for only where the last one's blocks end.
+    constexpr int kHeld = 16;
+    const bool held = all_blocks <= kHeld * kPagesThreads;
+    int32_t *at[kHeld], entry[kHeld];
+    const auto entry_of = [&](int64_t k, int32_t& i) {
+        if (i + 1 < a.B && k >= s_off[i + 1]) i = request_of(s_off, k);
+        return a.pages + slot_of(i) * a.bps + (k - s_off[i]);
+    };
+    if (RELEASE && ok) {
+        int64_t none = all_blocks;  // the thread's first block that is not there
+        if (held) {
+#pragma unroll
+            for (int u = 0; u < kHeld; u++) {
+                if (u * kPagesThreads >= all_blocks) break;
+                const int64_t k = min(static_cast<int64_t>(tid + u * kPagesThreads), all_blocks - 1);
+                const int32_t i = request_of(s_off, k);
+                at[u] = a.pages + slot_of(i) * a.bps + (k - s_off[i]);
+                entry[u] = *at[u];
+            }
+#pragma unroll
+            for (int u = kHeld - 1; u >= 0; u--)
+                if (tid + u * kPagesThreads < all_blocks && entry[u] < 0) none = tid + u * kPagesThreads;
+        } else {
+            int32_t i = 0;
+            for (int64_t k = tid; k < all_blocks; k += kPagesThreads)
+                if (*entry_of(k, i) < 0) none = min(none, k);
+        }
+        if (none < all_blocks) atomicMin(&s_bad, static_cast<uint32_t>(request_of(s_off, none)) * 8 + kBadEntry);
+        __syncthreads();
+        bad = s_bad;
+        ok = bad == 0xFFFFFFFFu;
+    }
+    if (first && tid == 0) {
+        if (!ok) {
+            const int i = min(static_cast<int>(bad >> 3), a.B - 1);
+            const int64_t count = RELEASE || i < 0 ? 0 : a.count[i];
+            raise_error(a.err, kErrKvPages, max(i, 0), i < 0 ? 0 : slot_of(i), i < 0 ? 0 : a.past[i], static_cast<uint32_t>(count),
+                        static_cast<uint32_t>(static_cast<uint64_t>(count) >> 32), bad & 7);
+        }
+        *a.n_free_out = static_cast<int32_t>(!ok ? n_free : RELEASE ? n_free + all_blocks : n_free - all_blocks);
+    }
+    if (RELEASE) {
+        if (!ok) return;
+        if (held) {
+#pragma unroll
+            for (int u = 0; u < kHeld; u++) {
+                if (tid + u * kPagesThreads >= all_blocks) break;
+                a.free_blocks[n_free + tid + u * kPagesThreads] = entry[u];
+                *at[u] = -1;
+            }
+            return;
+        }
+        int32_t i = 0;
+        for (int64_t k = tid; k < all_blocks; k += kPagesThreads) {
+            int32_t* e = entry_of(k, i);
+            a.free_blocks[n_free + k] = *e;
+            *e = -1;
+        }
+        return;
+    }
     if (first) {
         for (int64_t k = tid; k < all_blocks; k += kPagesThreads) {
-            const int32_t i = static_cast<int32_t>(item_request([&](int64_t r) { return s_off[r]; }, a.B, k, 1, 0));
-            int32_t* row = a.pages + slot_of(i) * a.bps;
-            if (RELEASE) {
-                int32_t* e = row + (k - s_off[i]);
-                a.free_blocks[n_free + k] = *e;
-                *e = -1;
-            } else {
-                row[blocks_of(a.past[i], a.shift) + (k - s_off[i])] = a.free_blocks[n_free - 1 - k];
-            }
+            const int32_t i = request_of(s_off, k);
+            a.pages[slot_of(i) * a.bps + blocks_of(a.past[i], a.shift) + (k - s_off[i])] = a.free_blocks[n_free - 1 - k];
         }
     }
-    if (RELEASE) return;
     const int64_t t1 = min((static_cast<int64_t>(blockIdx.x) + 1) * a.block_rows, a.tokens);
     for (int64_t t = blockIdx.x * a.block_rows + tid; t < t1; t += kPagesThreads) {
         if (t >= all_tokens) {
             store_row(a, t, -1, -1, -1, -1);
             continue;
         }
-        const int32_t i = static_cast<int32_t>(item_request([&](int64_t r) { return s_start[r]; }, a.B, t, 1, 0));
+        const int32_t i = request_of(s_start, t);
         const int32_t past = a.past[i], slot = slot_of(i), pos = past + static_cast<int32_t>(t - s_start[i]);
         const int64_t j = pos >> a.shift, taken = j - blocks_of(past, a.shift);  // a new block's number among the request's
         const int32_t block = taken < 0 ? a.pages[slot * a.bps + j] : a.free_blocks[n_free - 1 - (s_off[i] + taken)];

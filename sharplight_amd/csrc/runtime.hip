@@ -137,9 +137,10 @@ static int take_device_error()
                     "of new tokens or the block table.", h[1], slot, pos, v1);
     case kErrKvPages: {
         static const char* const why[] = {"", "its lengths do not fit its table row", "its slot is outside the table or named twice",
-                                          "the step has more tokens than rows", "the free list has too few blocks or too little room"};
+                                          "the step has more tokens than rows", "the free list has too few blocks or too little room",
+                                          "its table row does not hold its blocks"};
         return fail(SLHIP_ERR_CACHE, "Block tables: request %u (slot %d, %d cached tokens, %lld new): %s.", h[1], slot, pos, v1,
-                    why[h[6] <= 4 ? h[6] : 0]);
+                    why[h[6] <= 5 ? h[6] : 0]);
     }
     default: return fail(SLHIP_ERR_HIP, "device error record holds unknown code %u", h[0]);
     }

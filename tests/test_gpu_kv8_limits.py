@@ -199,3 +199,43 @@ def test_write_reports_requests_without_rows_of_their_own(device, B, bad, new):
             native.synchronize()
         kv8_ref.write(c, k64, k64, st.starts, st.past, st.slots, st.pages)
         _check_write(d, c, where, bad)
+
+
+@pytest.mark.parametrize("B,most", [(1, 100), (40, 100), (1030, 100), (30, 20000), (4096, 100)])
+@pytest.mark.parametrize("bad", ["", "twice", "longer", "last"])
+def test_release_of_blocks_that_are_not_held(device, B, most, bad):
+    """A request that was released before, or with fewer blocks than its length says: nothing changes, and the next sync says why. Up to
+    some 20000 blocks."""
+    rng = _rng("held", B, bad, most)
+    bs, bps = 16, -(-most // 16) + 2
+    past = rng.integers(1, most, B).astype(np.int32)
+    slots = rng.permutation(B + 2)[:B].astype(np.int32)
+    pages, ids = np.full((B + 2, bps), -1, np.int32), iter(rng.permutation(B * bps).astype(np.int32))
+    for s, p in zip(slots, past):
+        for j in range(-(-int(p) // bs)):
+            pages[s, j] = next(ids)
+    at = B - 1 if bad == "last" else int(rng.integers(0, B))
+    if bad == "twice":
+        pages[slots[at]] = -1
+    elif bad == "longer":  # ends within the row
+        past[at] = -(-int(past[at]) // bs) * bs + 1
+    elif bad == "last":
+        pages[slots[at], -(-int(past[at]) // bs) - 1] = -1
+    free = np.arange(9000, 9000 + B * bps + 9, dtype=np.int32)
+    with Dev() as d:
+        where = {"pages": d.put(pages), "free": d.put(free), "n": d.put(np.int32([5])), "out": d.put(np.int32([77]))}
+        p = native.kv_pages(B, d.put(past), None, where["pages"], pages.shape[0], bps, bs, where["free"], len(free), where["n"], where["out"],
+                            slots=d.put(slots))
+        log(f"kv_pages_release of {B} requests, {bad}")
+        native.kv_pages_release(p)
+        n_free = 5
+        if bad:
+            with pytest.raises(native.SlhipCacheError, match=f"request {at} .*does not hold"):
+                native.synchronize()
+        else:
+            native.synchronize()
+            ok, pages, free, n_free = kv8_ref.release(past, slots, pages, bs, free, 5)
+            assert ok
+        assert np.array_equal(d.get(where["pages"], pages.shape, np.int32), pages)
+        assert np.array_equal(d.get(where["free"], free.shape, np.int32), free)
+        assert d.get(where["out"], (1,), np.int32)[0] == n_free
