@@ -58,10 +58,10 @@ __device__ __forceinline__ void store_row(const KvPagesArgs& a, int64_t t, int32
     if (a.pos) a.pos[t] = max(pos, 0);
 }
 
-// Inclusive sums over the wave of numbers below 2^31, in 64 bits: the halves of 16 bits apart.
-__device__ __forceinline__ int64_t wave_scan_wide(int32_t v)
+// Inclusive sums over the wave of numbers below 2^32, in 64 bits: the halves of 16 bits apart.
+__device__ __forceinline__ int64_t wave_scan_wide(uint32_t v)
 {
-    return (static_cast<int64_t>(wave_scan(static_cast<uint32_t>(v) >> 16)) << 16) + wave_scan(v & 0xFFFF);
+    return (static_cast<int64_t>(wave_scan(v >> 16)) << 16) + wave_scan(v & 0xFFFF);
 }
 
 template <bool RELEASE>
@@ -83,7 +83,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     if (tid == 0) s_bad = 0xFFFFFFFFu;
     __syncthreads();
 
-    // sums of the thread's requests: at most four of below 2^31 each, so they are kept below that by what the step may have
+    // sums of the thread's requests: four of below 2^31 each at most, cut off below at 2^32 - 1, which no step takes
     int64_t tokens = 0, blocks = 0;
     for (int i = i0; i < i1; i++) {
         const int64_t past = i == i0 ? past0 : a.past[i], count = RELEASE ? 0 : i == i0 ? count0 : a.count[i], slot = i == i0 ? slot0 : slot_of(i);
@@ -97,9 +97,9 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
             blocks += RELEASE ? blocks_of(past, a.shift) : blocks_of(past + count, a.shift) - blocks_of(past, a.shift);
         }
     }
-    const int64_t most = 0x7FFFFFFF;  // more than any step has rows or any list has room for
+    const int64_t most = 0xFFFFFFFF;  // more than any step has rows or any list has room for
     const int64_t ct = min(tokens, most), co = min(blocks, most);
-    int64_t st = wave_scan_wide(static_cast<int32_t>(ct)), so = wave_scan_wide(static_cast<int32_t>(co));
+    int64_t st = wave_scan_wide(static_cast<uint32_t>(ct)), so = wave_scan_wide(static_cast<uint32_t>(co));
     if (lane == 63) {
         s_wave[0][wave] = st;
         s_wave[1][wave] = so;

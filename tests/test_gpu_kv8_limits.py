@@ -5,7 +5,7 @@ import pytest
 from sharplight_amd import native
 from tests import kv8_ref
 from tests.devutil import Dev, log
-from tests.test_gpu_kv8 import NP, Step, _attend, _cache, _check_write, _check_y, _from, _pattern, _put, _rng, _values
+from tests.test_gpu_kv8 import NP, Step, _advance, _attend, _cache, _check_advance, _check_write, _check_y, _from, _pattern, _put, _rng, _values
 
 pytestmark = pytest.mark.gpu
 
@@ -239,3 +239,20 @@ def test_release_of_blocks_that_are_not_held(device, B, most, bad):
         assert np.array_equal(d.get(where["pages"], pages.shape, np.int32), pages)
         assert np.array_equal(d.get(where["free"], free.shape, np.int32), free)
         assert d.get(where["out"], (1,), np.int32)[0] == n_free
+
+
+@pytest.mark.parametrize("tokens", [(1 << 31) - 1, (1 << 31) - 2])
+def test_advance_of_more_tokens_than_any_step_has(device, tokens):
+    """Two requests of neighbouring places whose tokens together pass 2^31, in a step without rows: refused."""
+    B, bs, bps = 1500, 1 << 20, 1600
+    past, count, slot = np.zeros(B, np.int32), np.zeros(B, np.int32), np.arange(B, dtype=np.int32)
+    count[:2] = 1600 << 20
+    pages, free = np.full((B, bps), -1, np.int32), np.arange(4000, dtype=np.int32)
+    with Dev() as d:
+        p, at = _advance(d, past, count, slot, pages, bs, free, len(free), 1, False, rows=False)
+        p.tokens = tokens
+        log(f"kv_pages_advance of {2 * int(count[0])} tokens")
+        native.kv_pages_advance(p)
+        with pytest.raises(native.SlhipCacheError, match="more tokens than rows"):
+            native.synchronize()
+        _check_advance(d, at, (False, pages, len(free), np.zeros(B + 1, np.int32), None, None), B, 0, rows=False)
