@@ -545,7 +545,9 @@ SLHIP_API int slhip_kv8_write(int dtype, const void* k, int64_t k_stride_t, int6
  * left as they were, as are those of a request that does not fit the batch or the table. A block id outside the cache is
  * reported too, and its keys are not seen.
  * work: workspace of work_bytes >= slhip_kv8_attention_work_bytes(...), 16-byte aligned, for the sums of key ranges that
- * are worked on apart; calls that may overlap each need their own. It needs no initialisation and keeps nothing.
+ * are worked on apart; calls that may overlap each need their own. It needs no initialisation and keeps nothing. The size that
+ * a batch is given is enough for every batch of the same heads with no more requests, tokens, blocks_per_slot * block_size and
+ * new tokens a request (max_new, or tokens where it is 0), whatever the call's scores and window are: a long prompt alone may need none.
  * Products of f32 activations are exact to 2^-22 (two f16 parts each), those of bf16 with the softmax weights in f16;
  * sums are f32. A cap adds 2^-21 of z; for bf16 activations and caps of up to 256, 2^-22 of the cap. One above 2^60 counts as none.
  */

@@ -36,6 +36,21 @@ constexpr int64_t kBlockUnits = 512;
 // and 37 us, the 5 requests 53 and 60.
 constexpr int64_t kFewTiles = kBlockUnits / 4;
 
+// Floats of the sums of `rows` rows; workers of the line; rows of a row tile; ranges of a head besides its tiles, and of a tile (cut
+// into no ranges of less than 8 key tiles, see below).
+static int64_t part_floats(int64_t dp, int64_t rows) { return rows * dp + rows * 2; }
+static int64_t workers_of(int64_t dp) { return dp == 256 ? kWorkers / 2 : kWorkers; }
+static int64_t tile_rows(int dtype, int64_t dp)
+{
+    return 16 * block_waves(static_cast<int>(dp)) * block_tiles(dtype == SLHIP_F32, static_cast<int>(dp));
+}
+static int64_t share_of(int64_t heads) { return (kBlockUnits + heads - 1) / heads; }
+static int64_t splits_of(int64_t pairs, int64_t seen)
+{
+    const int64_t s = (kBlockUnits + pairs - 1) / pairs, most = seen / (8 * kTile);
+    return s < most ? s : most;
+}
+
 // What a call over T rows of B requests launches. Few-row work takes a request whose rows fit one or two matrix tiles (16
 // or 32 rows a K/V head): its keys are then read once by single waves. Everything else goes to thread blocks that share
 // key tiles among 64 or 128 rows. Where the host cannot tell (max_new unknown or large, several requests) one launch holds
@@ -68,14 +83,14 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
         const int64_t rounds = p->blocks || B * heads < kWorkers ? 4 : B * heads < 2 * kWorkers ? 8 : 16;
         a->direct = seen <= rounds * 4 * kTile;
         p->few_heads = B * heads <= kWorkers;
-        a->workers = static_cast<int32_t>(a->direct ? B * heads : dp == 256 ? kWorkers / 2 : kWorkers);
+        a->workers = static_cast<int32_t>(a->direct ? B * heads : workers_of(dp));
         p->by_part = B * heads < 256;
-        if (!a->direct) bytes += 2 * a->workers * (few * dp + few * 2) * 4;
+        if (!a->direct) bytes += 2 * a->workers * part_floats(dp, few) * 4;
     }
     a->splits = 1;
     a->share = 0;
     if (p->blocks) {
-        const int64_t tile = 16 * block_waves(static_cast<int>(dp)) * block_tiles(dtype == SLHIP_F32, static_cast<int>(dp)), floats = tile * dp + tile * 2;
+        const int64_t tile = tile_rows(dtype, dp), floats = part_floats(dp, tile);
         a->tile_tokens = static_cast<int32_t>(tile / G);
         a->items = item_count(T, B, a->tile_tokens, 1);
         a->part2 = a->part + bytes / 4;
@@ -83,15 +98,34 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
         // 8, bf16: whole 20 us, in two 22; of 700 27 and 25; 5 requests of 250 to 433, 16 heads of 96 on 2: 22 and 34).
         const int64_t pairs = a->items * heads, most_cuts = seen / (8 * kTile);
         if (most_cuts >= 2 && pairs <= kFewTiles && B <= 64 && a->items * tokens / kTile < 1 << 28) {
-            a->share = static_cast<int32_t>((kBlockUnits + heads - 1) / heads);
+            a->share = static_cast<int32_t>(share_of(heads));
             bytes += (a->items + a->share) * heads * floats * 4;
         } else if (most_cuts >= 2 && pairs < kBlockUnits) {
-            const int64_t s = (kBlockUnits + pairs - 1) / pairs;
-            a->splits = static_cast<int32_t>(s < most_cuts ? s : most_cuts);
+            a->splits = static_cast<int32_t>(splits_of(pairs, seen));
             bytes += pairs * a->splits * floats * 4;
         }
     }
     return bytes;
+}
+
+// The most that a call needs whose requests, rows, new tokens and table rows are no more than these: a long prompt fills the machine
+// and needs nothing, its shorter end is cut along the keys. Every kind of plan that make_plan may choose, each at its largest.
+static int64_t most_work(int dtype, int64_t G, int64_t max_new, const Kv8Dev& c)
+{
+    const int64_t heads = c.heads, rows = (max_new > 0 && max_new < c.T ? max_new : c.T) * G, tokens = c.bps << c.shift;
+    const int64_t dp = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
+    const auto few = [&](int64_t tiles) { return tokens <= 4 * 4 * kTile ? 0 : 2 * workers_of(dp) * part_floats(dp, 16 * tiles) * 4; };
+    int64_t most = G <= 16 ? few(1) : 0;
+    if (dp <= 128 && G <= 32 && rows > 16 && few(2) > most) most = few(2);
+    if (rows <= (dp <= 128 ? 32 : 16)) return most;
+    const int64_t tile = tile_rows(dtype, dp), all = item_count(c.T, c.B, tile / G, 1);
+    const int64_t beside = G <= 16 && c.B > 1 ? few(1) : 0;
+    for (int64_t items = 1; items <= all && items * heads < kBlockUnits; items++) {
+        const int64_t pairs = items * heads, whole = pairs <= kFewTiles ? pairs + share_of(heads) * heads : 0, cut = pairs * splits_of(pairs, tokens);
+        const int64_t bytes = tokens / (8 * kTile) < 2 ? 0 : (whole > cut ? whole : cut) * part_floats(dp, tile) * 4;
+        if (bytes + beside > most) most = bytes + beside;
+    }
+    return most > beside ? most : beside;
 }
 
 static int check_sizes(int64_t q_heads, const Kv8Dev& c)
@@ -111,12 +145,10 @@ using namespace slhip;
 extern "C" SLHIP_API int64_t slhip_kv8_attention_work_bytes(int64_t q_heads, const slhip_kv8_cache* cache,
                                                             const slhip_kv8_batch* batch, int64_t max_new)
 {
-    Kv8AttnArgs a{};
-    Kv8AttnPlan p;
-    if (make_kv8("kv8_attention", cache, batch, &a.c) || check_sizes(q_heads, a.c)) return -1;
-    if (a.c.B == 0 || a.c.T == 0) return 0;
-    const int64_t f32 = make_plan(SLHIP_F32, q_heads / a.c.heads, max_new, &a, &p);
-    const int64_t bf16 = make_plan(SLHIP_BF16, q_heads / a.c.heads, max_new, &a, &p);
+    Kv8Dev c;
+    if (make_kv8("kv8_attention", cache, batch, &c) || check_sizes(q_heads, c)) return -1;
+    if (c.B == 0 || c.T == 0) return 0;
+    const int64_t f32 = most_work(SLHIP_F32, q_heads / c.heads, max_new, c), bf16 = most_work(SLHIP_BF16, q_heads / c.heads, max_new, c);
     return f32 > bf16 ? f32 : bf16;
 }
 

@@ -674,7 +674,7 @@ def kv8_write(dtype, k, v, cache: Kv8Cache, batch: Kv8Batch, *, k_stride_t=None,
 
 
 def kv8_attention_work_bytes(q_heads, cache: Kv8Cache, batch: Kv8Batch, max_new=0) -> int:
-    """Bytes of workspace that kv8_attention wants for such a batch."""
+    """Bytes of workspace that are enough for kv8_attention of such a batch and of every smaller one (-1: refused)."""
     return int(lib().slhip_kv8_attention_work_bytes(q_heads, ctypes.byref(cache), ctypes.byref(batch), max_new))
 
 

@@ -256,3 +256,33 @@ def test_advance_of_more_tokens_than_any_step_has(device, tokens):
         with pytest.raises(native.SlhipCacheError, match="more tokens than rows"):
             native.synchronize()
         _check_advance(d, at, (False, pages, len(free), np.zeros(B + 1, np.int32), None, None), B, 0, rows=False)
+
+
+# ---- workspace -------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 128), ("f32", 64), ("bf16", 256)])
+def test_one_workspace_for_every_smaller_step(device, dtype, D):
+    """A workspace of the size that the largest batch asks for takes all smaller steps: fewer requests, rows and new tokens, shorter tables."""
+    heads, G, bs = 2, 4, 16
+    steps = [([700, 600, 500, 40], [2500, 0, 900, 5], 150, 0), ([300], [2000], 150, 0), ([128], [3300], 0, 128), ([20, 9], [3000, 100], 20, 0),
+             ([4, 1, 3], [3000, 100, 2600], 0, 4), ([8], [1500], 0, 8), ([1], [100], 150, 1), ([40], [600], 0, 0)]
+    with Dev() as d:
+        sizes = []
+        for k, (new, past, wide, max_new) in enumerate(steps):
+            rng = _rng("workspace", dtype, D, k)
+            st = Step(rng, new, past, bs, wide=wide)
+            c = kv8_ref.Cache("i8", st.blocks, bs, heads, D, fill=rng)
+            q, q64 = _put(rng.standard_normal((st.T, heads * G, D)) * 2, dtype)
+            cache, batch = _cache(d, c)[0], st.batch(d)
+            if k == 0:  # the table's rows as long as any, and more rows than the step has
+                largest = native.kv8_batch(4, 9000, *st.dev[:3], 8, 360)
+                need = native.kv8_attention_work_bytes(heads * G, cache, largest, 0)
+                work = d.empty(need, fill=0xFF)
+            sizes.append(native.kv8_attention_work_bytes(heads * G, cache, batch, max_new))
+            y = d.empty(q.nbytes, fill=0x5A)
+            log(f"kv8_attention {dtype} D={D} new={new} past={past} of a workspace of {need} bytes")
+            native.kv8_attention(dtype, d.put(q), y, heads * G, cache, batch, scale=0.125, max_new=max_new, work=work, work_bytes=need)
+            native.synchronize()
+            want, bound = kv8_ref.attention(c, q64, st.starts, st.past, st.slots, st.pages, scale=0.125, dtype=dtype)
+            _check_y(_from(d.get(y, q.shape, NP[dtype]), dtype), want, bound, new, _pattern(dtype))
+        assert max(sizes) <= need
