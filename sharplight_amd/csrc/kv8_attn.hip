@@ -193,8 +193,13 @@ extern "C" SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q
     if (need > 0 && (!work || !aligned16(work) || work_bytes < need))
         return fail(SLHIP_ERR_INVALID, "kv8_attention: the workspace has %lld bytes, %lld are needed (16-byte aligned)",
                     static_cast<long long>(work ? work_bytes : 0), static_cast<long long>(need));
-    // a launch has less than 2^32 threads; the join has two thread blocks a head at most, besides those of few tiles
-    if ((a.items * a.splits + a.share) * a.c.heads + a.workers >= 1 << 24 || static_cast<int64_t>(a.c.B) * a.c.heads * 2 >= (1 << 24) - kBlockUnits * 32)
+    // A launch has less than 2^32 threads. Row tiles and few-row work are one launch, of 256 dims two (of different thread blocks); the
+    // join has two thread blocks a head, or up to 16 for each of fewer than 256 heads and of fewer than kBlockUnits row tiles.
+    const int64_t tiles = p.blocks ? (a.items * a.splits + a.share) * a.c.heads : 0, few = p.wave_tiles ? a.workers : 0;
+    const bool apart = a.c.D > 128;
+    const int64_t threads = tiles * block_threads(apart ? 256 : 128, p.blocks ? 1 : 0) + (apart ? 0 : few * 256);
+    const int64_t joins = static_cast<int64_t>(a.c.B) * a.c.heads * 2 + kBlockUnits * 32;
+    if (threads > 0xFFFFFFFFll || few * 256 > 0xFFFFFFFFll || joins * 256 > 0xFFFFFFFFll)
         return fail(SLHIP_ERR_UNSUPPORTED, "kv8_attention: too many tiles");
     e = error_word(&a.c.err);
     if (e) return e;

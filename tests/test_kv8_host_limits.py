@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from sharplight_amd import native
-from tests.test_kv8_host import _batch, _cache
+from tests.test_kv8_host import FAKE, _batch, _cache
 
 
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
@@ -30,3 +30,11 @@ def test_a_prompt_and_its_last_chunk():
     """A long prompt fills the machine without a workspace; the shorter step after it does not."""
     need = lambda t: native.kv8_attention_work_bytes(32, _cache(heads=8, head_dim=128), _batch(requests=1, tokens=t, blocks_per_slot=512), 0)  # noqa: E731
     assert need(8192) >= need(1024) >= need(128) > 0
+
+
+def test_launches_of_wide_heads_past_their_limits_are_refused():
+    """Row tiles of 256 dims have 512 threads: 2^23 of them are a launch of 2^32."""
+    for tokens in (300 << 20, 500 << 20):
+        with pytest.raises(NotImplementedError, match="too many tiles"):
+            native.kv8_attention("bf16", FAKE, FAKE, 4, _cache(head_dim=256), _batch(tokens=tokens, blocks_per_slot=1000), scale=1.0,
+                                 work=FAKE, work_bytes=1 << 40)
