@@ -92,14 +92,4 @@ __device__ __forceinline__ Kv8Item kv8_find(const Kv8Dev& d, int64_t item, int64
     return f;
 }
 
-template <int DT> __device__ __forceinline__ float4 load4f(const void* p, int64_t i)
-{
-    if constexpr (DT == SLHIP_F32) {
-        return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-        return make_float4(bf16_lo(v.x), bf16_hi(v.x), bf16_lo(v.y), bf16_hi(v.y));
-    }
-}
-
 }  // namespace slhip

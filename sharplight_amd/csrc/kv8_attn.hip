@@ -26,7 +26,9 @@ template <int DT, int FMT> static int launch(const Kv8AttnArgs& a, const Kv8Attn
     return reshaped ? kv8_attn_launch<DT, FMT, kReshaped>(a, p, st) : kv8_attn_launch<DT, FMT, kPlain>(a, p, st);
 }
 
-constexpr int64_t kWorkers = 512;     // two thread blocks a CU (one of 256 dims)
+// Two thread blocks a CU: the registers of the line's kernels leave places for so many. Those of 256 dims have one, and half the
+// workers; those of 32 rows (296 to 430 registers) have one too, and take the line's pieces in two rounds.
+constexpr int64_t kWorkers = 512;
 // Row tiles and key ranges of the many-row work, over all heads. With 256, 512, 1024: 5 requests of 77 to 611 new tokens and
 // up to 1500 older ones, 12 heads of 64, f32 67, 54, 52 us; a prompt of 1024, 32 query heads of 128 on 8, bf16 34, 32, 42 us;
 // 128 tokens on 30000, the same heads 118, 99, 111 us.
@@ -66,7 +68,6 @@ static int64_t make_plan(int dtype, int64_t G, int64_t max_new, Kv8AttnArgs* a, 
     else p->blocks = true;
     if (p->blocks && G <= 16 && B > 1) p->wave_tiles = 1;
     const int64_t limit = rows < 0x7FFFFFFF ? rows : 0x7FFFFFFF, few = 16 * p->wave_tiles;
-    a->min_rows = 0;
     a->max_rows = static_cast<int32_t>(p->blocks && few < limit ? few : limit);
     a->strict = !p->blocks;
     a->block_min = static_cast<int32_t>(few);

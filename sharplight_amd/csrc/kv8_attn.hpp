@@ -64,7 +64,7 @@ struct Kv8AttnArgs {
     float lost;                  // what a row that is not finite is multiplied by
     int32_t window;              // 0: none
     const float* slopes;
-    int32_t min_rows, max_rows;    // few-row work: requests of (min_rows, max_rows] query rows a K/V head
+    int32_t max_rows;              // few-row work: requests of up to so many query rows a K/V head
     bool strict;                   // requests above max_rows are an error (nothing else takes them)
     int32_t block_min, block_max;  // many-row tiles: requests of (block_min, block_max] rows; above is an error
     int32_t workers;             // few-row thread blocks
@@ -474,7 +474,7 @@ __device__ __forceinline__ int64_t quotient(int64_t n, int64_t d)
 __device__ __forceinline__ int32_t request_steps(const Kv8AttnArgs& a, const Kv8Request& r)
 {
     const int64_t rows = static_cast<int64_t>(r.n) * a.G;
-    if (r.n == 0 || rows <= a.min_rows || rows > a.max_rows) return 0;
+    if (r.n == 0 || rows > a.max_rows) return 0;
     int32_t first, end;
     key_range(a, r.past, 0, r.n, first, end);
     return (end - first + 4 * kTile - 1) / (4 * kTile) + kStart;
