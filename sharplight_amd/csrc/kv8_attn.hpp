@@ -46,8 +46,8 @@ constexpr int kStart = 2;
 // above kFastCap, for bf16 activations in kernels of their own (f32 ones cap all scores alike).
 // Up to kFastCap the scores of bf16 activations are capped by tanh y = 1 - 2 / (1 + e^(2 y)), off by up to 2^-22 whatever y is: a
 // score by 2^-22 of the cap, its weight by 2^-14 of itself at most (2^-16 with a cap of 50), whose f16 part is off by 2^-11.
-// It takes half of tanh_f's instructions: prompts of 188 to 1978, 64 query heads of 64, 255 us, with tanh_f 349. (As a branch in one
-// kernel tanh_f costs the others two registers more, and a third wave a SIMD: a prompt of 4096, 32 heads of 64, int8: 162 us, 176.)
+// It takes half of tanh_f's instructions: a prompt of 4096, 32 query heads of 64 on 8, int8 codes, 163 us, with tanh_f 249. (As a branch
+// in one kernel tanh_f costs smaller caps two registers more, and with them a third wave a SIMD: 176 us.)
 constexpr int kPlain = 0, kReshaped = 1, kFarCap = 2;
 constexpr float kFastCap = 256.0f;
 
@@ -436,7 +436,8 @@ __device__ __forceinline__ void key_range(const Kv8AttnArgs& a, int32_t past, in
 // How heads come to thread blocks: kShared, by the line below (or directly, where the launch holds many-row tiles too); kDirect,
 // a thread block a head, with nothing carried from one to the next, which takes 60 registers less; kLean, that with K's and V's
 // codes in the same registers one after the other, for three waves a SIMD (two of 256 dims or 32 rows): many short contexts are all
-// latency, of which the waves hide each other's. Times by kShared, kDirect and kLean, 8 K/V heads of 128, a row each: one
+// latency, of which the waves hide each other's. (Of f32 and 256 dims, or 32 rows of 128 with reshaped scores, 4 to 20 registers
+// go to scratch for that.) Times by kShared, kDirect and kLean, 8 K/V heads of 128, a row each: one
 // request of 501 tokens 9.4, 7.7 and 8.5 us; 256 of up to 251 33, 28 and 24 us; 400 of up to 701 81, 74 and 67 us. 100 of up to
 // 401, 4 heads of 256: 30 us shared, 17 lean.
 constexpr int kShared = 0, kDirect = 1, kLean = 2;
