@@ -538,18 +538,19 @@ SLHIP_API int slhip_kv8_write(int dtype, const void* k, int64_t k_stride_t, int6
  *   z_j = scale * (q . K_j); softcap > 0: z_j = softcap * tanh(z_j / softcap); slopes: z_j += slopes[h] * (j - p);
  *   window > 0: only j > p - window;  y = sum_j softmax(z)_j V_j.
  * q and y (dtype f32 or bf16, both the same; strides in elements, innermost 1) are [T, q_heads, head_dim]; y may be q.
- * q_heads a multiple of heads, at most 64 query heads for each. A row that sees no key is 0, one that holds an
- * infinity or a NaN and sees one NaN (under a cap an infinity is past it). requests *
- * (blocks_per_slot * block_size / 256 + 3) < 2^31.
+ * q_heads a multiple of heads, at most 64 query heads for each. A row that sees no key is 0; one that holds an infinity or a
+ * NaN and sees a key is NaN (under a cap an infinity is past it). requests * (blocks_per_slot * block_size / 256 + 3) < 2^31.
  * max_new: no request brings more rows (0: unknown); a request that does is reported (SLHIP_ERR_CACHE) and its rows are
  * left as they were, as are those of a request that does not fit the batch or the table. A block id outside the cache is
  * reported too, and its keys are not seen.
  * work: workspace of work_bytes >= slhip_kv8_attention_work_bytes(...), 16-byte aligned, for the sums of key ranges that
  * are worked on apart; calls that may overlap each need their own. It needs no initialisation and keeps nothing. The size that
- * a batch is given is enough for every batch of the same heads with no more requests, tokens, blocks_per_slot * block_size and
- * new tokens a request (max_new, or tokens where it is 0), whatever the call's scores and window are: a long prompt alone may need none.
- * Products of f32 activations are exact to 2^-22 (two f16 parts each), those of bf16 with the softmax weights in f16;
- * sums are f32. A cap adds 2^-21 of z; for bf16 activations and caps of up to 256, 2^-22 of the cap. One above 2^60 counts as none.
+ * a batch is given is enough for every batch of the same heads with no more requests, tokens, blocks_per_slot * block_size
+ * and new tokens a request (max_new, or tokens where it is 0), whatever the scores and window: a long prompt may need less than
+ * its end.
+ * Products of f32 activations are exact to 2^-22 (two f16 parts each), those of bf16 with the softmax weights in f16; a weight
+ * of less than 2^-33 of the row's largest, each times its block's V scale, counts as 0 there; sums are f32. A cap adds 2^-21
+ * of z; for bf16 activations and caps of up to 256, 2^-22 of the cap. One above 2^60 counts as none.
  */
 typedef struct slhip_kv8_attn {
     float scale, softcap;

@@ -6,12 +6,13 @@
 // With t_j = z_j log2(e) + ev_b and M the running maximum of t_j (or a little less: tile_max), w_j = 2^(t_j - M) holds the
 // whole weight of code c_j, the block's scale included: o = sum_j w_j c_j, l = sum_j w_j 2^-ev_b, y = o / l. So V's codes go
 // to the matrix cores as they are, the scale costs nothing (it rides in the addition of the exponent), and what is rounded
-// to f16, w_j, is rounded relative to the largest contribution, whatever the scales of the blocks are.
+// to f16, w_j, is rounded relative to the largest one, whatever the scales of the blocks are (and whatever the codes: beside a key
+// of zeros that has all but 2^-33 of the weight, the others' values are lost).
 //
 // Numbers. int8 and E4M3 codes are exact in f16. A query row is multiplied by the power of two that brings its largest
 // value to [2^14, 2^15): bf16 values are then exact in f16 down to 2^-29 of the row's largest (below that they round to
 // 2^-40 of it), f32 values are the sum of two f16 parts to 2^-22 (or 2^-40 of the largest). w_j goes to the matrix cores
-// scaled by 2^kBias, in f16 (2^-11 of itself, 2^-33 of the largest contribution at least) for bf16 activations, whose
+// scaled by 2^kBias, in f16 (2^-11 of itself, or 2^-33 of the largest) for bf16 activations, whose
 // output is rounded to 2^-8 anyway, and as two f16 parts (2^-22) for f32. Products are exact, sums, maxima and l are f32.
 //
 // Layout. A tile is 64 keys, four 16-key sub-blocks, and a wave works on NT * 16 query rows of one K/V head: rows are
