@@ -38,14 +38,14 @@ extern "C" {
 #define SLHIP_API __attribute__((visibility("default")))
 #endif
 
-#define SLHIP_ABI_VERSION 6
+#define SLHIP_ABI_VERSION 7
 
 typedef enum slhip_status {
     SLHIP_OK = 0,
     SLHIP_ERR_INVALID = -1,     /* bad argument: null pointer, size, stride, dtype combination */
     SLHIP_ERR_UNSUPPORTED = -2, /* valid request this library has no kernel for */
     SLHIP_ERR_HIP = -3,         /* the HIP runtime reported an error */
-    SLHIP_ERR_INDEX = -4,       /* a gather index was outside [0, V) (reported by slhip_stream_sync) */
+    SLHIP_ERR_INDEX = -4,       /* a gather index, drafted token or adapter out of its range (reported by slhip_stream_sync) */
     SLHIP_ERR_NO_DEVICE = -5,   /* no usable device / driver */
     SLHIP_ERR_CACHE = -6,       /* a KV-cache row, block or request outside the cache or block table (at slhip_stream_sync) */
     SLHIP_ERR_FORMAT = -7       /* malformed file data: a truncated or inconsistent GGUF file */
@@ -460,9 +460,14 @@ SLHIP_API int slhip_cache_write(int dtype_in, int dtype_cache, const void* x, in
  * slhip_kv_pages_release: the blocks of requests that ended, ceil(past[i] / block_size) of slot i each, go back on the
  *   stack in order (free_blocks[*n_free + ..]; capacity free_capacity), their table entries become -1, and
  *   *n_free_out = *n_free + the blocks. count, starts, seq, pos and tokens are not used.
+ * slhip_kv_pages_trim: requests step back from past[i] + count[i] tokens to past[i]: the blocks behind their first
+ *   keep(i) = ceil(past[i] / block_size), back(i) = ceil((past[i] + count[i]) / block_size) - keep(i) of them, o(i) = back(0) + ..
+ *   + back(i-1), go back on the stack: free_blocks[*n_free + o(B) - 1 - (o(i) + j)] = pages[slot, keep(i) + j] for j < back(i),
+ *   their table entries become -1, and *n_free_out = *n_free + o(B). Where all that an advance took goes back in the same
+ *   order of requests, the free list is as it was before. starts, seq, pos and tokens are not used.
  *
  * n_free_out may be n_free itself (one counter that the steps of a captured loop advance) or another word (the old count
- * stays, to step back to). All or nothing: where a length is negative, a context would outgrow its table row or the rows
+ * stays, to step back to). All or nothing, for each of the three: where a length is negative, a context would outgrow its table row or the rows
  * `tokens`, a slot is outside the table or named twice, the free list has too few ids (too little room), or a block to be
  * released is not in the table (its entry is negative: it was released before), the tables, the list and the count stay as
  * they were (*n_free_out = *n_free), starts are 0, every row is padding, and the next slhip_stream_sync reports
@@ -473,7 +478,7 @@ SLHIP_API int slhip_cache_write(int dtype_in, int dtype_cache, const void* x, in
 typedef struct slhip_kv_pages {
     int64_t requests;             /* B */
     const int32_t* past;          /* [B] */
-    const int32_t* count;         /* [B] (advance) */
+    const int32_t* count;         /* [B] (advance, trim) */
     const int32_t* slots;         /* [B], or NULL: slot i */
     int32_t* pages;               /* [page_slots, blocks_per_slot] */
     int64_t page_slots, blocks_per_slot, block_size;
@@ -488,6 +493,7 @@ typedef struct slhip_kv_pages {
 } slhip_kv_pages;
 SLHIP_API int slhip_kv_pages_advance(const slhip_kv_pages* p, slhip_stream stream);
 SLHIP_API int slhip_kv_pages_release(const slhip_kv_pages* p, slhip_stream stream);
+SLHIP_API int slhip_kv_pages_trim(const slhip_kv_pages* p, slhip_stream stream);
 
 /*
  * The cache. Codes of K: [blocks, heads, block_size, head_dim] bytes; of V: [blocks, heads, block_size / 16, head_dim, 16]
@@ -564,6 +570,87 @@ SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q_stride_t, 
                                   int64_t y_stride_t, int64_t y_stride_h, const slhip_kv8_cache* cache,
                                   const slhip_kv8_batch* batch, const slhip_kv8_attn* cfg, void* work, int64_t work_bytes,
                                   slhip_stream stream);
+
+/*
+ * Verification of drafted tokens against the target's probabilities, from given random numbers, and the draw of the token
+ * behind the accepted ones. Request i has rows starts[i] .. starts[i+1]-1 of the step's T: row t's logits (target) give the
+ * probabilities of the token behind ids[t], and ids[t + 1] is the draft for it, but for the request's last row, which has none.
+ * One row and no draft: a token is drawn from the row.
+ *   p_t(v) = softmax(target[t] / tau_i)_v, q_t likewise from draft[t] and draft_temperature: the probabilities that the draft was
+ *   drawn from. Without draft logits, or where draft_temperature[i] <= 0, the draft was chosen: q_t is 1 there.
+ *   Draft x of row t is accepted while accept[t] * q_t(x) < p_t(x). Behind the accepted ones comes one more token, from the row
+ *   of the first refused draft or the last row: of weights max(p - q, 0) (the last row, or weights that are all 0: p) it is the
+ *   first v whose sum over 0 .. v is above sample[i] times the sum of all, or the last one with a weight.
+ *   temperature[i] <= 0: a draft is accepted while it is the lowest v with the largest logit, and that is the token behind; no random
+ *   number and no draft logits count. Logits of -inf have the probability 0. Temperatures count as 2^-40 .. 2^40.
+ *   out[i, 0 ..]: the accepted drafts and the token, then -1 up to out_stride; n_out[i] their number (0 for a request of no rows);
+ *   logp (NULL: none): the logarithms of their p (greedy: at temperature 1), then 0. kept[i] = past[i] + n_out[i], the tokens that
+ *   the cache keeps of past[i] and the step's; dropped[i] = the request's rows - n_out[i]: what slhip_kv_pages_trim takes as past and count.
+ * Where a row's target logits hold a NaN or +inf, or nothing above -inf, or a temperature is NaN, its draft is refused and its
+ * token is -1 with a NaN; where its draft logits do, the draft is refused and the token drawn from p. A draft outside the vocabulary
+ * that is reached is refused and reported (SLHIP_ERR_INDEX) by the next slhip_stream_sync. A request that does not fit the rows, or has more of them
+ * than out_stride, gets no tokens and is reported (SLHIP_ERR_CACHE).
+ * target, draft: f32 or bf16 (dtype), rows of `vocab` logits with a stride; a row's sum is of f32 exponentials, of which e
+ * is off by (2 + |log2 e|) 2^-23 of itself at most; all that follows is f64. ids, starts, past, out, n_out, kept, dropped: int32.
+ * work: workspace of work_bytes >= slhip_draft_verify_work_bytes(...) (enough for every smaller batch too), 16-byte aligned; calls that
+ * may overlap each need their own. It needs no initialisation and keeps nothing. requests <= 65536, vocab <= 2^24,
+ * tokens * ceil(vocab / 4096) < 2^23, requests * ceil(vocab / 4096) < 2^24. out, n_out, kept, dropped and logp overlap no input.
+ */
+typedef struct slhip_drafts {
+    int64_t requests;               /* B */
+    int64_t tokens;                 /* T: rows of target, draft, ids and accept, padding rows included */
+    int64_t vocab;
+    const int32_t* starts;          /* [B + 1] */
+    const int32_t* ids;             /* [T] */
+    const float* temperature;       /* [B] or NULL: 1 */
+    const float* draft_temperature; /* [B] or NULL: temperature */
+    const float* accept;            /* [T], each in [0, 1) */
+    const float* sample;            /* [B], each in [0, 1) */
+    int32_t* out;                   /* [B, out_stride] */
+    int64_t out_stride;
+    int32_t* n_out;                 /* [B] */
+    const int32_t* past;            /* [B] or NULL: 0 */
+    int32_t *kept, *dropped;        /* [B] or NULL */
+    float* logp;                    /* [B, out_stride] or NULL */
+} slhip_drafts;
+SLHIP_API int64_t slhip_draft_verify_work_bytes(int64_t requests, int64_t tokens, int64_t vocab);
+SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64_t target_stride, const void* draft, int64_t draft_stride,
+                                 const slhip_drafts* d, void* work, int64_t work_bytes, slhip_stream stream);
+
+/*
+ * Low-rank adapters of many requests at once beside a shared projection:
+ *   y[t] = add[t] + scale[a] * B_a (A_a x[t]) for the rows starts[i] .. starts[i+1]-1 of request i, a = adapter[i];
+ *   y[t] = add[t] where adapter[i] is -1.
+ * A_a [max_rank, K] and B_a [N, max_rank] (rows dense) lie a_stride and b_stride elements after one another; of adapter a only the
+ * first rank[a] ranks count (of fewer than max_rank, the others are not read). x [T, K] f32 or bf16 (dtype_x), add and y [T, N] (dtype_y), row strides
+ * in elements; add may be y (in place: rows without an adapter are then not touched) or NULL (0). Rows from starts[B] on are padding: neither
+ * read nor written. starts[0] is 0 and starts never falls; starts, adapter and rank are int32 on the device.
+ * A x is summed and held in f32 (for bf16 y and adapters B takes it in two bf16 parts, to 2^-17 of itself); y is rounded once.
+ * An adapter outside [-1, adapters) counts as -1 and is reported (SLHIP_ERR_INDEX) by the next slhip_stream_sync; a request
+ * that does not fit the rows is left as it was and reported (SLHIP_ERR_CACHE).
+ * work: workspace of work_bytes >= slhip_lora_work_bytes(tokens, max_rank) (enough for fewer tokens and ranks too), 16-byte
+ * aligned; calls that may overlap each need their own. It needs no initialisation and keeps nothing.
+ * max_rank <= 256, K and N <= 2^24, requests <= 4096. Any alignment; rows and adapters of 16-byte steps are fastest.
+ */
+typedef struct slhip_lora_set {
+    int32_t dtype; /* of a and b: F32, F16 or BF16 */
+    int32_t reserved;
+    const void *a, *b;
+    int64_t adapters, max_rank, K, N;
+    int64_t a_stride, b_stride; /* elements from an adapter to the next */
+    const int32_t* rank;        /* [adapters] or NULL: max_rank */
+    const float* scale;         /* [adapters] or NULL: 1 */
+} slhip_lora_set;
+typedef struct slhip_lora_rows {
+    int64_t requests;       /* B */
+    int64_t tokens;         /* T: rows of x, add and y, padding rows included */
+    const int32_t* starts;  /* [B + 1] */
+    const int32_t* adapter; /* [B] */
+} slhip_lora_rows;
+SLHIP_API int64_t slhip_lora_work_bytes(int64_t tokens, int64_t max_rank);
+SLHIP_API int slhip_lora(int dtype_x, int dtype_y, const void* x, int64_t x_stride, const void* add, int64_t add_stride, void* y,
+                         int64_t y_stride, const slhip_lora_set* set, const slhip_lora_rows* rows, void* work, int64_t work_bytes,
+                         slhip_stream stream);
 
 /*
  * Element type conversion y = cast(x) of n elements (F32, F16, BF16 in any direction); f32 -> bf16 rounds

@@ -390,7 +390,8 @@ __device__ __forceinline__ void e4m3_group_scale(float m, float& d, float& id)
 // ---- device side: errors raised by kernels -----------------------------------------------------------
 
 enum : uint32_t {
-    kErrGatherIndex = 1, kErrCacheSeq = 2, kErrCachePageTable = 3, kErrCacheBlock = 4, kErrKvRequest = 5, kErrKvPages = 6
+    kErrGatherIndex = 1, kErrCacheSeq = 2, kErrCachePageTable = 3, kErrCacheBlock = 4, kErrKvRequest = 5, kErrKvPages = 6,
+    kErrDraftToken = 7, kErrAdapter = 8
 };
 
 // Records an error in the device's error record unless one is already there (the first error wins).

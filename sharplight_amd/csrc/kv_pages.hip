@@ -1,4 +1,4 @@
-// Block tables and slot maps of a serving step, from request lengths on the device (slhip_kv_pages_advance / _release).
+// Block tables and slot maps of a serving step, from request lengths on the device (slhip_kv_pages_advance / _trim / _release).
 //
 // Mathematics: two prefix sums over the requests -- of their new tokens (starts) and of the blocks those need (which ids
 // of the free list are theirs) -- then one write per taken block and one row per token. Nothing here moves enough bytes to
@@ -12,6 +12,8 @@
 // Measured: 64 requests of a token 4.4 us, 333 requests of 1 to 200 tokens (some 33000 rows) 6.2 us; an empty launch takes 2.5.
 // With kBlockRows = 4096 the latter took 10.4 us, and with the rows in a second launch 10.0. A release is one thread block's too: 64
 // requests of 256 blocks 19 us, of 8192 432.
+// A trim is a release that leaves each request's first blocks, and it fills the stack from the other end, so that it undoes an
+// advance. Its few blocks' chain is the release's: lengths -> scan -> table entries -> stores.
 #include "common.hpp"
 #include "kv8_map.hpp"
 
@@ -64,9 +66,12 @@ __device__ __forceinline__ int64_t wave_scan_wide(uint32_t v)
     return (static_cast<int64_t>(wave_scan(v >> 16)) << 16) + wave_scan(v & 0xFFFF);
 }
 
-template <bool RELEASE>
+enum { kAdvance = 0, kRelease = 1, kTrim = 2 };
+
+template <int OP>
 __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
 {
+    constexpr bool RELEASE = OP != kAdvance, COUNTS = OP != kRelease;  // blocks go back; requests have a count
     __shared__ int32_t s_start[kMaxRequests + 1], s_off[kMaxRequests + 1];
     __shared__ uint32_t s_seen[kMaxSlots / 32];
     __shared__ int64_t s_wave[2][kPagesThreads / 64];
@@ -78,15 +83,19 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     const int64_t row_tokens = a.bps << a.shift;
     const auto slot_of = [&](int i) { return a.slots ? a.slots[i] : i; };
     // the thread's first request: most steps have no more than one a thread
-    const int32_t past0 = i0 < i1 ? a.past[i0] : 0, count0 = i0 < i1 && !RELEASE ? a.count[i0] : 0, slot0 = i0 < i1 ? slot_of(i0) : 0;
+    const int32_t past0 = i0 < i1 ? a.past[i0] : 0, count0 = i0 < i1 && COUNTS ? a.count[i0] : 0, slot0 = i0 < i1 ? slot_of(i0) : 0;
     for (int64_t w = tid; w < (a.page_slots + 31) / 32; w += kPagesThreads) s_seen[w] = 0;
     if (tid == 0) s_bad = 0xFFFFFFFFu;
     __syncthreads();
 
+    // the blocks that a request takes or gives back
+    const auto moved = [&](int64_t past, int64_t count) {
+        return OP == kRelease ? blocks_of(past, a.shift) : blocks_of(past + count, a.shift) - blocks_of(past, a.shift);
+    };
     // sums of the thread's requests: four of below 2^31 each at most, cut off below at 2^32 - 1, which no step takes
     int64_t tokens = 0, blocks = 0;
     for (int i = i0; i < i1; i++) {
-        const int64_t past = i == i0 ? past0 : a.past[i], count = RELEASE ? 0 : i == i0 ? count0 : a.count[i], slot = i == i0 ? slot0 : slot_of(i);
+        const int64_t past = i == i0 ? past0 : a.past[i], count = !COUNTS ? 0 : i == i0 ? count0 : a.count[i], slot = i == i0 ? slot0 : slot_of(i);
         uint32_t bad = 0;
         if (slot < 0 || slot >= a.page_slots || (atomicOr(&s_seen[slot >> 5], 1u << (slot & 31)) >> (slot & 31) & 1u)) bad = kBadSlot;
         if (past < 0 || count < 0 || past + count > row_tokens) bad = kBadLength;
@@ -94,7 +103,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
             atomicMin(&s_bad, static_cast<uint32_t>(i) * 8 + bad);
         } else {
             tokens += count;
-            blocks += RELEASE ? blocks_of(past, a.shift) : blocks_of(past + count, a.shift) - blocks_of(past, a.shift);
+            blocks += moved(past, count);
         }
     }
     const int64_t most = 0xFFFFFFFF;  // more than any step has rows or any list has room for
@@ -130,9 +139,9 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
         s_off[i] = static_cast<int32_t>(so);
         if (!RELEASE && first) a.starts[i] = ok ? static_cast<int32_t>(st) : 0;
         if (!ok) continue;
-        const int64_t past = i == i0 ? past0 : a.past[i], count = RELEASE ? 0 : i == i0 ? count0 : a.count[i];
+        const int64_t past = i == i0 ? past0 : a.past[i], count = !COUNTS ? 0 : i == i0 ? count0 : a.count[i];
         st += count;
-        so += RELEASE ? blocks_of(past, a.shift) : blocks_of(past + count, a.shift) - blocks_of(past, a.shift);
+        so += moved(past, count);
     }
     if (!RELEASE && first && tid == 0) a.starts[a.B] = static_cast<int32_t>(all_tokens);
     __syncthreads();
@@ -145,9 +154,14 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     constexpr int kHeld = 16;
     const bool held = all_blocks <= kHeld * kPagesThreads;
     int32_t *at[kHeld], entry[kHeld];
+    const auto row_of = [&](int32_t i) {  // the first table entry that the request gives back
+        return a.pages + slot_of(i) * a.bps + (OP == kTrim ? blocks_of(a.past[i], a.shift) : 0);
+    };
+    // where block k of all goes on the stack
+    const auto place = [&](int64_t k) { return n_free + (OP == kTrim ? all_blocks - 1 - k : k); };
     const auto entry_of = [&](int64_t k, int32_t& i) {
         if (i + 1 < a.B && k >= s_off[i + 1]) i = request_of(s_off, k);
-        return a.pages + slot_of(i) * a.bps + (k - s_off[i]);
+        return row_of(i) + (k - s_off[i]);
     };
     if (RELEASE && ok) {
         int64_t none = all_blocks;  // the thread's first block that is not there
@@ -157,7 +171,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
                 if (u * kPagesThreads >= all_blocks) break;
                 const int64_t k = min(static_cast<int64_t>(tid + u * kPagesThreads), all_blocks - 1);
                 const int32_t i = request_of(s_off, k);
-                at[u] = a.pages + slot_of(i) * a.bps + (k - s_off[i]);
+                at[u] = row_of(i) + (k - s_off[i]);
                 entry[u] = *at[u];
             }
 #pragma unroll
@@ -176,7 +190,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     if (first && tid == 0) {
         if (!ok) {
             const int i = min(static_cast<int>(bad >> 3), a.B - 1);
-            const int64_t count = RELEASE || i < 0 ? 0 : a.count[i];
+            const int64_t count = !COUNTS || i < 0 ? 0 : a.count[i];
             raise_error(a.err, kErrKvPages, max(i, 0), i < 0 ? 0 : slot_of(i), i < 0 ? 0 : a.past[i], static_cast<uint32_t>(count),
                         static_cast<uint32_t>(static_cast<uint64_t>(count) >> 32), bad & 7);
         }
@@ -188,7 +202,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
 #pragma unroll
             for (int u = 0; u < kHeld; u++) {
                 if (tid + u * kPagesThreads >= all_blocks) break;
-                a.free_blocks[n_free + tid + u * kPagesThreads] = entry[u];
+                a.free_blocks[place(tid + u * kPagesThreads)] = entry[u];
                 *at[u] = -1;
             }
             return;
@@ -196,7 +210,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
         int32_t i = 0;
         for (int64_t k = tid; k < all_blocks; k += kPagesThreads) {
             int32_t* e = entry_of(k, i);
-            a.free_blocks[n_free + k] = *e;
+            a.free_blocks[place(k)] = *e;
             *e = -1;
         }
         return;
@@ -236,7 +250,7 @@ __global__ __launch_bounds__(256) void kv_pages_rows(KvPagesArgs a)
 }
 
 // Checks what the host can see of the arguments.
-static int make_args(const char* op, bool release, const slhip_kv_pages* p, KvPagesArgs* a)
+static int make_args(const char* op, int kind, const slhip_kv_pages* p, KvPagesArgs* a)
 {
     if (!p) return fail(SLHIP_ERR_INVALID, "%s: arguments are null", op);
     if (p->requests < 0 || p->page_slots < 0 || p->blocks_per_slot < 0 || p->free_capacity < 0 || p->tokens < 0)
@@ -250,9 +264,9 @@ static int make_args(const char* op, bool release, const slhip_kv_pages* p, KvPa
     if (p->tokens > 0x7FFFFFFF || p->free_capacity > 0x7FFFFFFF) return fail(SLHIP_ERR_UNSUPPORTED, "%s: 2^31 tokens or blocks or more", op);
     if (!p->n_free || !p->n_free_out) return fail(SLHIP_ERR_INVALID, "%s: n_free and n_free_out are required", op);
     if (p->free_capacity > 0 && !p->free_blocks) return fail(SLHIP_ERR_INVALID, "%s: the free list is null", op);
-    if (p->requests > 0 && (!p->past || !p->pages || (!release && !p->count)))
+    if (p->requests > 0 && (!p->past || !p->pages || (kind != kRelease && !p->count)))
         return fail(SLHIP_ERR_INVALID, "%s: past, count and pages are required", op);
-    if (!release && !p->starts) return fail(SLHIP_ERR_INVALID, "%s: starts is required", op);
+    if (kind == kAdvance && !p->starts) return fail(SLHIP_ERR_INVALID, "%s: starts is required", op);
     int shift = 0;
     while ((int64_t{1} << shift) < p->block_size) shift++;
     *a = KvPagesArgs{static_cast<int32_t>(p->requests), p->past, p->count, p->slots, p->pages, p->page_slots, p->blocks_per_slot,
@@ -268,12 +282,12 @@ using namespace slhip;
 extern "C" SLHIP_API int slhip_kv_pages_advance(const slhip_kv_pages* p, slhip_stream stream)
 {
     KvPagesArgs a;
-    const int e = make_args("kv_pages_advance", false, p, &a);
+    const int e = make_args("kv_pages_advance", kAdvance, p, &a);
     if (e) return e;
     const bool rows = a.tokens > 0 && (a.seq || a.pos), apart = rows && a.tokens > kBlockRows && a.n_free == a.n_free_out;
     a.block_rows = rows && !apart ? kBlockRows : 0;
     const int64_t grid = a.block_rows ? (a.tokens + kBlockRows - 1) / kBlockRows : 1;
-    kv_pages_tables<false><<<static_cast<unsigned>(grid), kPagesThreads, 0, to_stream(stream)>>>(a);
+    kv_pages_tables<kAdvance><<<static_cast<unsigned>(grid), kPagesThreads, 0, to_stream(stream)>>>(a);
     const int s = check_launch("kv_pages_tables");
     if (s || !apart) return s;
     kv_pages_rows<<<static_cast<unsigned>((a.tokens + 255) / 256), 256, 0, to_stream(stream)>>>(a);
@@ -283,8 +297,17 @@ extern "C" SLHIP_API int slhip_kv_pages_advance(const slhip_kv_pages* p, slhip_s
 extern "C" SLHIP_API int slhip_kv_pages_release(const slhip_kv_pages* p, slhip_stream stream)
 {
     KvPagesArgs a;
-    const int e = make_args("kv_pages_release", true, p, &a);
+    const int e = make_args("kv_pages_release", kRelease, p, &a);
     if (e) return e;
-    kv_pages_tables<true><<<1, kPagesThreads, 0, to_stream(stream)>>>(a);
+    kv_pages_tables<kRelease><<<1, kPagesThreads, 0, to_stream(stream)>>>(a);
+    return check_launch("kv_pages_tables");
+}
+
+extern "C" SLHIP_API int slhip_kv_pages_trim(const slhip_kv_pages* p, slhip_stream stream)
+{
+    KvPagesArgs a;
+    const int e = make_args("kv_pages_trim", kTrim, p, &a);
+    if (e) return e;
+    kv_pages_tables<kTrim><<<1, kPagesThreads, 0, to_stream(stream)>>>(a);
     return check_launch("kv_pages_tables");
 }

@@ -142,6 +142,9 @@ static int take_device_error()
         return fail(SLHIP_ERR_CACHE, "Block tables: request %u (slot %d, %d cached tokens, %lld new): %s.", h[1], slot, pos, v1,
                     why[h[6] <= 5 ? h[6] : 0]);
     }
+    case kErrDraftToken:
+        return fail(SLHIP_ERR_INDEX, "Drafted token %d (number %u of request %u) out of range [0,%u).", pos, h[2], h[1], h[4]);
+    case kErrAdapter: return fail(SLHIP_ERR_INDEX, "Adapter %d of request %u out of range [-1,%u).", slot, h[1], h[3]);
     default: return fail(SLHIP_ERR_HIP, "device error record holds unknown code %u", h[0]);
     }
 }

@@ -122,6 +122,27 @@ class Kv8Attn(ctypes.Structure):
 KV8_FORMATS = {"i8": 0, "e4m3": 1}
 
 
+class Drafts(ctypes.Structure):
+    """slhip_drafts: a step's drafted tokens and random numbers, and where the accepted ones go."""
+    _fields_ = [("requests", ctypes.c_int64), ("tokens", ctypes.c_int64), ("vocab", ctypes.c_int64), ("starts", ctypes.c_void_p),
+                ("ids", ctypes.c_void_p), ("temperature", ctypes.c_void_p), ("draft_temperature", ctypes.c_void_p),
+                ("accept", ctypes.c_void_p), ("sample", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64),
+                ("n_out", ctypes.c_void_p), ("past", ctypes.c_void_p), ("kept", ctypes.c_void_p), ("dropped", ctypes.c_void_p),
+                ("logp", ctypes.c_void_p)]
+
+
+class LoraSet(ctypes.Structure):
+    """slhip_lora_set: the low-rank adapters of one projection."""
+    _fields_ = [("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
+                ("adapters", ctypes.c_int64), ("max_rank", ctypes.c_int64), ("K", ctypes.c_int64), ("N", ctypes.c_int64),
+                ("a_stride", ctypes.c_int64), ("b_stride", ctypes.c_int64), ("rank", ctypes.c_void_p), ("scale", ctypes.c_void_p)]
+
+
+class LoraRows(ctypes.Structure):
+    """slhip_lora_rows: a step's requests and the adapter of each."""
+    _fields_ = [("requests", ctypes.c_int64), ("tokens", ctypes.c_int64), ("starts", ctypes.c_void_p), ("adapter", ctypes.c_void_p)]
+
+
 class NormCopies(ctypes.Structure):
     """slhip_norm_copies: the f16 and E4M3 GEMM activation copies a row norm writes (either may be NULL)."""
     _fields_ = [("y16", ctypes.c_void_p), ("y16_stride", ctypes.c_int64), ("yq", ctypes.c_void_p),
@@ -261,6 +282,11 @@ SIGNATURES = {
     "slhip_cache_write": (_I, [_I, _I, _P, _I64, _I64, _I64, _P, ctypes.POINTER(CacheRows), _P]),
     "slhip_kv_pages_advance": (_I, [ctypes.POINTER(KvPages), _P]),
     "slhip_kv_pages_release": (_I, [ctypes.POINTER(KvPages), _P]),
+    "slhip_kv_pages_trim": (_I, [ctypes.POINTER(KvPages), _P]),
+    "slhip_draft_verify_work_bytes": (_I64, [_I64, _I64, _I64]),
+    "slhip_draft_verify": (_I, [_I, _P, _I64, _P, _I64, ctypes.POINTER(Drafts), _P, _I64, _P]),
+    "slhip_lora_work_bytes": (_I64, [_I64, _I64]),
+    "slhip_lora": (_I, [_I, _I, _P, _I64, _P, _I64, _P, _I64, ctypes.POINTER(LoraSet), ctypes.POINTER(LoraRows), _P, _I64, _P]),
     "slhip_kv8_write": (_I, [_I, _P, _I64, _I64, _P, _I64, _I64, ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8Batch), _P]),
     "slhip_kv8_attention_work_bytes": (_I64, [_I64, ctypes.POINTER(Kv8Cache), ctypes.POINTER(Kv8Batch), _I64]),
     "slhip_kv8_attention": (_I, [_I, _P, _I64, _I64, _I64, _P, _I64, _I64, ctypes.POINTER(Kv8Cache),
@@ -637,7 +663,7 @@ def cache_write(dtype_in, dtype_cache, x, T, inner, cache, rows: CacheRows, *, x
 
 def kv_pages(requests, past, count, pages, page_slots, blocks_per_slot, block_size, free_blocks, free_capacity, n_free,
              n_free_out, tokens=0, starts=None, *, seq=None, pos=None, slots=None) -> KvPages:
-    """The arguments of kv_pages_advance / kv_pages_release (int32 device arrays), to be kept with the buffers."""
+    """The arguments of kv_pages_advance / kv_pages_release / kv_pages_trim (int32 device arrays), to be kept with the buffers."""
     return KvPages(requests, ptr(past), ptr(count), ptr(slots), ptr(pages), page_slots, blocks_per_slot, block_size,
                    ptr(free_blocks), free_capacity, ptr(n_free), ptr(n_free_out), tokens, ptr(starts), ptr(seq), ptr(pos))
 
@@ -650,6 +676,11 @@ def kv_pages_advance(p: KvPages, stream=None):
 def kv_pages_release(p: KvPages, stream=None):
     """Returns the blocks of requests that ended (slots, past = their lengths) to the free list."""
     call("slhip_kv_pages_release", p, stream)
+
+
+def kv_pages_trim(p: KvPages, stream=None):
+    """Requests step back from past + count tokens to past; the blocks behind go back to the free list."""
+    call("slhip_kv_pages_trim", p, stream)
 
 
 def kv8_cache(fmt, k, v, k_scale, v_scale, blocks, block_size, heads, head_dim) -> Kv8Cache:
@@ -687,6 +718,49 @@ def kv8_attention(dtype, q, y, q_heads, cache: Kv8Cache, batch: Kv8Batch, *, sca
     call("slhip_kv8_attention", DTYPES.get(dtype, dtype), ptr(q), row if q_stride_t is None else q_stride_t,
          d if q_stride_h is None else q_stride_h, q_heads, ptr(y), row if y_stride_t is None else y_stride_t,
          d if y_stride_h is None else y_stride_h, cache, batch, cfg, ptr(work), work_bytes, stream)
+
+
+def drafts(requests, tokens, vocab, starts, ids, accept, sample, out, out_stride, n_out, *, temperature=None,
+           draft_temperature=None, past=None, kept=None, dropped=None, logp=None) -> Drafts:
+    """The arguments of draft_verify (int32 and f32 device arrays), to be kept with the buffers."""
+    return Drafts(requests, tokens, vocab, ptr(starts), ptr(ids), ptr(temperature), ptr(draft_temperature), ptr(accept),
+                  ptr(sample), ptr(out), out_stride, ptr(n_out), ptr(past), ptr(kept), ptr(dropped), ptr(logp))
+
+
+def draft_verify_work_bytes(requests, tokens, vocab) -> int:
+    """Bytes of workspace that are enough for draft_verify of such a batch and of every smaller one (-1: refused)."""
+    return int(lib().slhip_draft_verify_work_bytes(requests, tokens, vocab))
+
+
+def draft_verify(dtype, target, draft, d: Drafts, *, target_stride=None, draft_stride=None, work=None, work_bytes=0, stream=None):
+    """Accepts drafted tokens by the target's logits (and those that they were drawn from; None: they were chosen) and draws
+    the token behind them."""
+    call("slhip_draft_verify", DTYPES.get(dtype, dtype), ptr(target), d.vocab if target_stride is None else target_stride, ptr(draft),
+         d.vocab if draft_stride is None else draft_stride, d, ptr(work), work_bytes, stream)
+
+
+def lora_set(dtype, a, b, adapters, max_rank, K, N, *, rank=None, scale=None, a_stride=None, b_stride=None) -> LoraSet:
+    """The adapters of a projection: a [adapters, max_rank, K], b [adapters, N, max_rank], rank and scale [adapters]."""
+    return LoraSet(DTYPES.get(dtype, dtype), 0, ptr(a), ptr(b), adapters, max_rank, K, N, max_rank * K if a_stride is None else a_stride,
+                   N * max_rank if b_stride is None else b_stride, ptr(rank), ptr(scale))
+
+
+def lora_rows(requests, tokens, starts, adapter) -> LoraRows:
+    """A step's requests: starts [requests + 1], adapter [requests] (-1: none)."""
+    return LoraRows(requests, tokens, ptr(starts), ptr(adapter))
+
+
+def lora_work_bytes(tokens, max_rank) -> int:
+    """Bytes of workspace that are enough for lora of so many rows and ranks, and of fewer (-1: refused)."""
+    return int(lib().slhip_lora_work_bytes(tokens, max_rank))
+
+
+def lora(dtype_x, dtype_y, x, add, y, adapters: LoraSet, rows: LoraRows, *, x_stride=None, add_stride=None, y_stride=None, work=None,
+         work_bytes=0, stream=None):
+    """y [tokens, N] = add + scale * B (A x) with each request's adapter; add may be y, or None for 0."""
+    call("slhip_lora", DTYPES.get(dtype_x, dtype_x), DTYPES.get(dtype_y, dtype_y), ptr(x), adapters.K if x_stride is None else x_stride,
+         ptr(add), adapters.N if add_stride is None else add_stride, ptr(y), adapters.N if y_stride is None else y_stride, adapters,
+         rows, ptr(work), work_bytes, stream)
 
 
 def gather(fmt, table, V, D, ids, N, dtype_out, y, *, y_stride=None, stream=None):
