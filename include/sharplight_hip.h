@@ -625,7 +625,8 @@ SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64_t target_s
  * first rank[a] ranks count (of fewer than max_rank, the others are not read). x [T, K] f32 or bf16 (dtype_x), add and y [T, N] (dtype_y), row strides
  * in elements; add may be y (in place: rows without an adapter are then not touched) or NULL (0). Rows from starts[B] on are padding: neither
  * read nor written. starts[0] is 0 and starts never falls; starts, adapter and rank are int32 on the device.
- * A x is summed and held in f32 (for bf16 y and adapters B takes it in two bf16 parts, to 2^-17 of itself); y is rounded once.
+ * A x is summed and held in f32 (for bf16 y B takes it in two bf16 parts, to 2^-17 of itself); y is rounded once. A row
+ * that holds an infinity or a NaN gives no finite values; no other row's change.
  * An adapter outside [-1, adapters) counts as -1 and is reported (SLHIP_ERR_INDEX) by the next slhip_stream_sync; a request
  * that does not fit the rows is left as it was and reported (SLHIP_ERR_CACHE).
  * work: workspace of work_bytes >= slhip_lora_work_bytes(tokens, max_rank) (enough for fewer tokens and ranks too), 16-byte

@@ -6,24 +6,22 @@
 //
 // Every row's S is needed for its p(x), so the rows are read once for their sums (HBM bounds it), in chunks that lie in
 // registers: a chunk's maximum first, then one exponential a logit, no running rescale. Which row is drawn from follows from all
-// of a request's sums; that row alone is read again, for sums of weights chunk by chunk, and one chunk a third time, for the
-// place in it.
+// of a request's sums. The sums of p's chunks are there already; those of max(p - q, 0) take that one row of both a second time. The
+// place in a chunk takes it once more.
 //
 // Numbers. A choice changes where a sum passes a random number, so what two implementations may differ in is kept small: chunk
 // sums are f32 exponentials of arguments with one rounding (log2(e) / tau in two parts, or all terms of a sum would be off the same
 // way), everything behind them f64: the rows' sums, p(x), q(x), and the drawn row's weights, whose differences p - q cancel.
-#include <float.h>
 #include <math.h>
 
 #include "step.hpp"
 
 namespace slhip {
 
-constexpr int kChunk = 4096;       // logits of a chunk
-constexpr int kThreads = 256;
-constexpr int kEach = kChunk / kThreads;
-constexpr int kDecide = 1024;      // threads of draft_decide
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kVecs = 4;  // 16-byte vectors of a thread: a chunk is 16 KB
 constexpr int64_t kMaxVocab = 1 << 24;
+template <int DT> constexpr int kChunk = kThreads * kVecs * Vec<DT>::N;  // logits of a chunk
 
 struct ChunkStat {
     float m;      // the largest logit; NaN where the chunk holds a NaN or an infinity above
@@ -74,35 +72,73 @@ __device__ __forceinline__ Heat heat_of(const float* tau, int32_t i)
 // A thread's logits of a chunk: vectors of 16 bytes, a block's threads side by side, in the order of the vocabulary from one step
 // to the next. Places past the vocabulary are -inf.
 template <int DT> struct Logits {
-    static constexpr int N = Vec<DT>::N, kVecs = kEach / N;
-    float z[kEach];
-    __device__ static __forceinline__ int32_t place(int32_t chunk, int j) { return chunk * kChunk + (j * kThreads + static_cast<int>(threadIdx.x)) * N; }
+    static constexpr int N = Vec<DT>::N, kEach = kVecs * N;
+    uint4 w[kVecs];
+    __device__ static __forceinline__ int32_t place(int32_t chunk, int j) { return chunk * kChunk<DT> + (j * kThreads + static_cast<int>(threadIdx.x)) * N; }
     __device__ __forceinline__ void load(const void* rows, int64_t row, int64_t stride, int32_t V, int32_t chunk)
     {
         const char* p = static_cast<const char*>(rows) + row * stride * Vec<DT>::BYTES;
-        uint4 w[kVecs];
+        if ((chunk + 1) * kChunk<DT> <= V) {  // whole: no branch between the loads
 #pragma unroll
-        for (int j = 0; j < kVecs; j++) {
-            const int32_t v = place(chunk, j);
-            w[j] = make_uint4(0, 0, 0, 0);
-            if (v + N <= V) w[j] = load_any(p + static_cast<int64_t>(v) * Vec<DT>::BYTES);
+            for (int j = 0; j < kVecs; j++) w[j] = load_any(p + static_cast<int64_t>(place(chunk, j)) * Vec<DT>::BYTES);
+            return;
         }
 #pragma unroll
         for (int j = 0; j < kVecs; j++) {
             const int32_t v = place(chunk, j);
-            Vec<DT>::unpack(w[j], &z[j * N]);
-            if (v + N > V) {
-                for (int k = 0; k < N; k++) z[j * N + k] = v + k < V ? Vec<DT>::load1(p, v + k) : -INFINITY;
+            if (v + N <= V) {
+                w[j] = load_any(p + static_cast<int64_t>(v) * Vec<DT>::BYTES);
+            } else {
+                float z[N];
+                for (int k = 0; k < N; k++) z[k] = v + k < V ? Vec<DT>::load1(p, v + k) : -INFINITY;
+                w[j] = Vec<DT>::pack(z);  // the same bits again
             }
         }
     }
+    __device__ __forceinline__ void vec(int j, float (&z)[N]) const { Vec<DT>::unpack(w[j], z); }
 };
 
+// v of another lane by a DPP move, 0 where there is none.
+template <int CTRL, int ROWS = 0xF> __device__ __forceinline__ double dpp64(double v)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROWS, 0xF, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+__device__ __forceinline__ double lane64(double v, int lane)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(u), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Over 16 lanes, in every lane (swaps in quads, then mirrors: group_sum).
+__device__ __forceinline__ double row_sum64(double v)
+{
+    v += dpp64<0xB1>(v);
+    v += dpp64<0x4E>(v);
+    v += dpp64<0x141>(v);
+    return v + dpp64<0x140>(v);
+}
+
+// Over the wave, wave-uniform.
 __device__ __forceinline__ double wave_sum64(double v)
 {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-    return v;
+    v = row_sum64(v);
+    return (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
+}
+
+// Inclusive sums over the wave (wave_scan's steps).
+__device__ __forceinline__ double wave_scan64(double v)
+{
+    v += dpp64<0x111>(v);
+    v += dpp64<0x112>(v);
+    v += dpp64<0x114>(v);
+    v += dpp64<0x118>(v);
+    v += dpp64<0x142, 0xA>(v);
+    return v + dpp64<0x143, 0xC>(v);
 }
 
 // 2^y to 2^-40 of itself for y <= 0 (0 below -1000): the series of 2^f, |f| <= 1/2.
@@ -132,11 +168,11 @@ __device__ __forceinline__ double share_of(float z, double m, double c) { return
 
 template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_stats(DraftArgs a)
 {
-    __shared__ float s_m[kThreads / 64];
-    __shared__ double s_s[kThreads / 64];
-    __shared__ int32_t s_arg[kThreads / 64];
+    __shared__ float s_m[kWaves];
+    __shared__ double s_s[kWaves];
+    __shared__ int32_t s_arg[kWaves];
+    constexpr int N = Logits<DT>::N, kMats = DRAFT ? 2 : 1;
     const int lane = threadIdx.x & 63, wave = wave_id();
-    constexpr int kMats = DRAFT ? 2 : 1;
     const int64_t item = blockIdx.x, t = item / (a.chunks * kMats);
     const int32_t rest = static_cast<int32_t>(item - t * (a.chunks * kMats)), mat = rest / a.chunks, chunk = rest - mat * a.chunks;
     Logits<DT> x;
@@ -148,33 +184,36 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
         if (target.greedy || h.greedy || t == a.starts[i + 1] - 1) return;
         x.load(a.draft, t, a.qs, a.V, chunk);
     }
+    float z[Logits<DT>::kEach];
+#pragma unroll
+    for (int j = 0; j < kVecs; j++) Vec<DT>::unpack(x.w[j], &z[j * N]);
     float m = -INFINITY;
     bool bad = false;
 #pragma unroll
-    for (int j = 0; j < kEach; j++) {
-        m = fmaxf(m, x.z[j]);
-        bad |= !(x.z[j] < INFINITY);
+    for (int j = 0; j < kVecs * N; j++) {
+        m = fmaxf(m, z[j]);
+        bad |= !(z[j] < INFINITY);
     }
     m = group_max<64>(m);
     if (__any(bad)) m = INFINITY;
     if (lane == 0) s_m[wave] = m;
     __syncthreads();
     m = s_m[0];
-    for (int w = 1; w < kThreads / 64; w++) m = fmaxf(m, s_m[w]);
+    for (int w = 1; w < kWaves; w++) m = fmaxf(m, s_m[w]);
     const double c = kLog2e64 / h.tau;
     const float hi = static_cast<float>(c), lo = static_cast<float>(c - hi);
     float s = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kEach; j++) {
-        const float d = fmaxf(x.z[j] - m, -0x1p60f);
+    for (int j = 0; j < kVecs * N; j++) {
+        const float d = fmaxf(z[j] - m, -0x1p60f);
         s += __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo));
     }
     const double sum = wave_sum64(s);
     int32_t arg = 0x7FFFFFFF;
     if (target.greedy) {
 #pragma unroll
-        for (int j = kEach - 1; j >= 0; j--)
-            if (x.z[j] == m) arg = Logits<DT>::place(chunk, j / Logits<DT>::N) + j % Logits<DT>::N;
+        for (int j = kVecs * N - 1; j >= 0; j--)
+            if (z[j] == m) arg = Logits<DT>::place(chunk, j / N) + j % N;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) arg = min(arg, __shfl_xor(arg, o, 64));
     }
@@ -185,7 +224,7 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
     __syncthreads();
     if (threadIdx.x == 0) {
         ChunkStat o{m == INFINITY ? NAN : m, s_arg[0], s_s[0]};
-        for (int w = 1; w < kThreads / 64; w++) {
+        for (int w = 1; w < kWaves; w++) {
             o.s += s_s[w];
             o.arg = min(o.arg, s_arg[w]);
         }
@@ -196,297 +235,366 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
 
 // ---- what is accepted ----------------------------------------------------------------------------------------------
 
+// A row of a matrix: its maximum and sum, the lowest place of the maximum, whether it can be used; and its draft's logit and share.
 struct RowStat {
-    double m, s;
+    double m, s, share;
     int32_t arg;
     bool fine;
+    float z;
 };
 
-// The chunks of a row together, by a whole wave.
-__device__ __forceinline__ RowStat row_stat(const DraftArgs& a, int64_t t, int mat, double c)
+// The chunks of a row together, by 16 lanes. The first 64 chunks are looked at once.
+__device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks, double c, bool arg)
 {
-    const ChunkStat* st = a.stats + (t * 2 + mat) * a.chunks;
-    const int lane = threadIdx.x & 63;
+    constexpr int kHeld = 4;
+    const int lane = threadIdx.x & 15;
+    ChunkStat x[kHeld];
+#pragma unroll
+    for (int j = 0; j < kHeld; j++) {
+        x[j] = st[min(lane + 16 * j, chunks - 1)];
+        if (lane + 16 * j >= chunks) x[j].m = -INFINITY;
+    }
     float m = -INFINITY;
     bool bad = false;
-    for (int32_t k = lane; k < a.chunks; k += 64) {
-        const float x = st[k].m;
-        bad |= x != x;
-        m = fmaxf(m, x);
-    }
-    m = group_max<64>(m);
+    const auto look = [&](float v) {
+        bad |= v != v;
+        m = fmaxf(m, v);
+    };
+#pragma unroll
+    for (int j = 0; j < kHeld; j++) look(x[j].m);
+    for (int32_t k = lane + 16 * kHeld; k < chunks; k += 16) look(st[k].m);
+    m = group_max_dpp<16>(bad ? INFINITY : m);
     RowStat r;
-    r.fine = !__any(bad) && m > -INFINITY;
+    r.fine = m < INFINITY && m > -INFINITY;
     r.m = m;
     double s = 0.0;
-    int32_t arg = 0x7FFFFFFF;
-    for (int32_t k = lane; k < a.chunks; k += 64) {
-        const ChunkStat x = st[k];
-        if (x.m > -INFINITY) s += x.s * exp2_64((static_cast<double>(x.m) - r.m) * c);
-        if (x.m == m) arg = min(arg, x.arg);
-    }
-    r.s = wave_sum64(s);
+    int32_t first = 0x7FFFFFFF;
+    const auto take = [&](const ChunkStat& v) {
+        if (v.m > -INFINITY) s += v.s * exp2_64((static_cast<double>(v.m) - r.m) * c);
+        if (v.m == m) first = min(first, v.arg);
+    };
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) arg = min(arg, __shfl_xor(arg, o, 64));
-    r.arg = arg;
+    for (int j = 0; j < kHeld; j++) take(x[j]);
+    for (int32_t k = lane + 16 * kHeld; k < chunks; k += 16) take(st[k]);
+    r.s = row_sum64(s);
+    if (arg) {
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) first = min(first, __shfl_xor(first, o, 64));
+    }
+    r.arg = first;
     return r;
 }
 
-template <int DT> __global__ __launch_bounds__(kDecide) void draft_decide(DraftArgs a)
+struct DecideLds {
+    RowStat row[16];  // of a pass: target's rows, or target's and draft's in turns
+};
+
+// What request i's accepted drafts are, and what is drawn behind them, by the whole block; into the outputs too.
+template <int DT> __device__ __forceinline__ Pick decide(const DraftArgs& a, int32_t i, DecideLds& lds)
 {
-    constexpr int kWaves = kDecide / 64, kRows = kWaves / 2;  // rows of a pass: a wave for the target's sums, one for the draft's
-    __shared__ RowStat s_row[kRows][2];
-    __shared__ int32_t s_stop;
-    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
-    const int32_t i = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, group = tid >> 4;
     const int64_t s0 = a.starts[i], s1 = a.starts[i + 1];
     const bool fits = s0 >= 0 && s1 >= s0 && s1 <= a.T && s1 - s0 <= a.out_stride;
     const int32_t n = fits ? static_cast<int32_t>(s1 - s0) : 0;
     const Heat hp = heat_of(a.tau, i), hq = a.tau_q ? heat_of(a.tau_q, i) : hp;
     const double cp = kLog2e64 / hp.tau, cq = kLog2e64 / hq.tau;
     const bool drawn = a.draft && !hp.greedy && !hq.greedy;  // else the drafts were chosen: q is 1 there
+    const int mats = drawn ? 2 : 1, rows = 16 / mats;
     int32_t* out = a.out + i * a.out_stride;
     float* logp = a.logp ? a.logp + i * a.out_stride : nullptr;
-    int32_t stop = n;  // the place of the token behind the accepted drafts
-    for (int32_t first = 0; first < n && stop == n; first += kRows) {
-        const int32_t count = min(n - first, kRows), j = wave >> 1;
-        if (j < count && ((wave & 1) == 0 || (drawn && first + j < n - 1))) {
-            const RowStat r = row_stat(a, s0 + first + j, wave & 1, wave & 1 ? cq : cp);
-            if (lane == 0) s_row[j][wave & 1] = r;
-        }
-        __syncthreads();
-        if (wave == 0) {
-            const int32_t place = first + lane;
+    int32_t stop = n, first = 0;  // the place of the token behind the accepted drafts; the pass's first row
+    for (; first < n; first += rows) {
+        const int32_t count = min(n - first, rows), place = first + group / mats, mat = group & (mats - 1);
+        if (place < n && (mat == 0 || place < n - 1)) {
             const int64_t t = s0 + place;
-            const bool row = lane < count && place < n - 1;  // it has a draft
-            const RowStat &p = s_row[lane & (kRows - 1)][0], &q = s_row[lane & (kRows - 1)][1];
-            const int32_t x = row ? a.ids[t + 1] : 0;
-            const bool fine = row && p.fine && !hp.bad, known = x >= 0 && x < a.V;
-            bool good = false;
-            float z = 0.0f;
-            if (fine && known) {
-                z = Vec<DT>::load1(a.target, t * a.zs + x);
-                if (hp.greedy) {
-                    good = x == p.arg;
-                } else if (!drawn || (q.fine && !hq.bad)) {
-                    const double qx = drawn ? share_of(Vec<DT>::load1(a.draft, t * a.qs + x), q.m, cq) / q.s : 1.0;
-                    good = static_cast<double>(a.accept[t]) * qx < share_of(z, p.m, cp) / p.s;
-                }
-            }
-            const uint64_t refused = ~__ballot(good) & ((uint64_t{1} << count) - 1);
-            const int32_t to = refused ? first + __ffsll(static_cast<long long>(refused)) - 1 : n;
-            if (good && place < to) {
-                out[place] = x;
-                if (logp) logp[place] = static_cast<float>((static_cast<double>(z) - p.m) * (cp / kLog2e64) - log(p.s));
-            }
-            if (fine && !known && place == to)
-                raise_error(a.err, kErrDraftToken, static_cast<uint32_t>(i), static_cast<uint32_t>(place), static_cast<uint32_t>(x), static_cast<uint32_t>(a.V), 0, 0);
-            if (lane == 0) s_stop = to;
+            const int32_t x = place < n - 1 ? a.ids[t + 1] : 0;
+            float z = -INFINITY;
+            if (x >= 0 && x < a.V) z = Vec<DT>::load1(mat ? a.draft : a.target, t * (mat ? a.qs : a.zs) + x);
+            const double c = mat ? cq : cp;
+            RowStat r = row_stat(a.stats + (t * 2 + mat) * a.chunks, a.chunks, c, hp.greedy);
+            r.fine &= !(mat ? hq.bad : hp.bad);
+            r.z = z;
+            r.share = share_of(z, r.m, c) / r.s;
+            if ((tid & 15) == 0) lds.row[group] = r;
         }
         __syncthreads();
-        stop = s_stop;
-        if (stop == n) __syncthreads();  // the next pass writes s_row
-    }
-    if (wave != 0) return;
-    if (lane == 0) {
-        Pick k{};
-        k.kind = kDone;
-        if (n > 0) {
-            const int32_t j = stop % kRows;
-            const RowStat &p = s_row[j][0], &q = s_row[j][1];
-            const int64_t t = s0 + stop;
-            const bool last = stop == n - 1;
-            k.row = static_cast<int32_t>(t);
-            k.place = stop;
-            if (!p.fine || hp.bad) {
-                out[stop] = -1;
-                if (logp) logp[stop] = NAN;
-            } else if (hp.greedy) {
-                out[stop] = p.arg;
-                if (logp) logp[stop] = static_cast<float>(-log(p.s));
-            } else {
-                k.token = last ? -1 : a.ids[t + 1];
-                k.kind = last ? kFromTarget : !drawn ? kFromOthers : q.fine && !hq.bad ? kFromRest : kFromTarget;
-                k.mp = p.m;
-                k.cp = cp;
-                k.ip = 1.0 / p.s;
-                k.mq = q.m;
-                k.cq = cq;
-                k.iq = 1.0 / q.s;
-            }
-            a.n_out[i] = stop + 1;
-        } else {
-            a.n_out[i] = 0;
-            if (!fits)
-                raise_error(a.err, kErrKvRequest, static_cast<uint32_t>(i), static_cast<uint32_t>(i), a.past ? static_cast<uint32_t>(a.past[i]) : 0,
-                            static_cast<uint32_t>(s1 - s0), static_cast<uint32_t>(static_cast<uint64_t>(s1 - s0) >> 32), 0);
+        // each wave looks at all rows of the pass, a lane each
+        const int32_t mine = first + lane;
+        const bool row = lane < count && mine < n - 1;  // it has a draft
+        const RowStat &p = lds.row[(lane & (rows - 1)) * mats], &q = lds.row[(lane & (rows - 1)) * mats + mats - 1];
+        const int32_t x = row ? a.ids[s0 + mine + 1] : 0;
+        const bool known = x >= 0 && x < a.V;
+        bool good = false;
+        if (row && p.fine && known) {
+            if (hp.greedy) good = x == p.arg;
+            else if (!drawn || q.fine) good = static_cast<double>(a.accept[s0 + mine]) * (drawn ? q.share : 1.0) < p.share;
         }
-        a.picks[i] = k;
+        const uint64_t refused = ~__ballot(good) & ((uint64_t{1} << count) - 1);
+        if (refused) stop = first + __ffsll(static_cast<long long>(refused)) - 1;
+        if (tid < 64) {
+            if (good && mine < stop) {
+                out[mine] = x;
+                if (logp) logp[mine] = static_cast<float>((static_cast<double>(p.z) - p.m) * (cp / kLog2e64) - log(p.s));
+            }
+            if (row && p.fine && !known && mine == stop)
+                raise_error(a.err, kErrDraftToken, static_cast<uint32_t>(i), static_cast<uint32_t>(mine), static_cast<uint32_t>(x), static_cast<uint32_t>(a.V), 0, 0);
+        }
+        if (stop < n) break;
+        __syncthreads();  // the next pass writes the rows
+    }
+    Pick k{};
+    k.kind = kDone;
+    int32_t token = -1;
+    float lp = NAN;
+    if (n > 0) {
+        const RowStat &p = lds.row[(stop - first) * mats], &q = lds.row[(stop - first) * mats + mats - 1];
+        const bool last = stop == n - 1;
+        k.row = static_cast<int32_t>(s0) + stop;
+        k.place = stop;
+        if (p.fine && hp.greedy) {
+            token = p.arg;
+            lp = static_cast<float>(-log(p.s));
+        } else if (p.fine) {
+            k.token = last ? -1 : a.ids[k.row + 1];
+            k.kind = last ? kFromTarget : !drawn ? kFromOthers : q.fine ? kFromRest : kFromTarget;
+            k.mp = p.m;
+            k.cp = cp;
+            k.ip = 1.0 / p.s;
+            k.mq = q.m;
+            k.cq = cq;
+            k.iq = 1.0 / q.s;
+        }
+    }
+    if (tid == 0) {
+        if (n > 0 && k.kind == kDone) {
+            out[stop] = token;
+            if (logp) logp[stop] = lp;
+        }
+        a.n_out[i] = n > 0 ? stop + 1 : 0;
         if (a.kept) a.kept[i] = (a.past ? a.past[i] : 0) + (n > 0 ? stop + 1 : 0);
         if (a.dropped) a.dropped[i] = n > 0 ? n - stop - 1 : 0;
+        if (!fits)
+            raise_error(a.err, kErrKvRequest, static_cast<uint32_t>(i), static_cast<uint32_t>(i), a.past ? static_cast<uint32_t>(a.past[i]) : 0,
+                        static_cast<uint32_t>(s1 - s0), static_cast<uint32_t>(static_cast<uint64_t>(s1 - s0) >> 32), 0);
     }
-    for (int64_t j = (n > 0 ? stop + 1 : 0) + lane; j < a.out_stride; j += 64) {
+    for (int64_t j = (n > 0 ? stop + 1 : 0) + tid; j < a.out_stride; j += kThreads) {
         out[j] = -1;
         if (logp) logp[j] = 0.0f;
     }
+    return k;
 }
 
 // ---- the draw ------------------------------------------------------------------------------------------------------
 
-// The weights of a thread's logits of a chunk. `all`: p, whatever the pick's kind is.
-template <int DT> __device__ __forceinline__ void weights(const DraftArgs& a, const Pick& k, int32_t chunk, bool all, double (&w)[kEach])
+// e^((z - m) / tau): as f32 where it is below 2^-12 (its roundings are then below those of the sums), f64 above.
+struct Share {
+    double m, c;
+    float mf, hi, lo;
+    __device__ __forceinline__ Share(double m_, double c_) : m(m_), c(c_), mf(static_cast<float>(m_)), hi(static_cast<float>(c_)), lo(static_cast<float>(c_ - hi)) {}
+    template <int N> __device__ __forceinline__ void of(const float (&z)[N], double (&w)[N]) const
+    {
+        bool large = false;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const float d = fmaxf(z[e] - mf, -0x1p60f), y = fmaf(d, hi, d * lo);
+            w[e] = static_cast<double>(__builtin_amdgcn_exp2f(y));
+            large |= y > -12.0f;
+        }
+        if (__any(large)) {
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const float d = fmaxf(z[e] - mf, -0x1p60f);
+                if (fmaf(d, hi, d * lo) > -12.0f) w[e] = exp2_64((static_cast<double>(z[e]) - m) * c);
+            }
+        }
+    }
+};
+
+// The weights of a thread's logits of a chunk, as the pick's kind says, vector by vector: put(j, w).
+template <int DT, class Put> __device__ __forceinline__ void weights(const DraftArgs& a, const Pick& k, int32_t kind, int32_t chunk, const Put& put)
 {
 #pragma clang fp contract(off)  // p - q of equal numbers is 0, not the rounding of a product
-    Logits<DT> x;
+    constexpr int N = Logits<DT>::N;
+    Logits<DT> x, y;
     x.load(a.target, k.row, a.zs, a.V, chunk);
+    if (kind == kFromRest) y.load(a.draft, k.row, a.qs, a.V, chunk);
+    const Share p(k.mp, k.cp), q(k.mq, k.cq);
 #pragma unroll
-    for (int j = 0; j < kEach; j++) w[j] = share_of(x.z[j], k.mp, k.cp) * k.ip;
-    if (all || k.kind == kFromTarget) return;
-    if (k.kind == kFromOthers) {
+    for (int j = 0; j < kVecs; j++) {
+        float z[N];
+        double w[N];
+        x.vec(j, z);
+        p.of(z, w);
 #pragma unroll
-        for (int j = 0; j < kEach; j++)
-            if (Logits<DT>::place(chunk, j / Logits<DT>::N) + j % Logits<DT>::N == k.token) w[j] = 0.0;
-        return;
+        for (int e = 0; e < N; e++) w[e] *= k.ip;
+        const int32_t at = Logits<DT>::place(chunk, j);
+        if (kind == kFromOthers) {
+#pragma unroll
+            for (int e = 0; e < N; e++) w[e] = at + e == k.token ? 0.0 : w[e];
+        } else if (kind == kFromRest) {
+            double u[N];
+            y.vec(j, z);
+            q.of(z, u);
+#pragma unroll
+            for (int e = 0; e < N; e++) w[e] = fmax(w[e] - u[e] * k.iq, 0.0);
+        }
+        put(j, w);
     }
-    x.load(a.draft, k.row, a.qs, a.V, chunk);
-#pragma unroll
-    for (int j = 0; j < kEach; j++) w[j] = fmax(w[j] - share_of(x.z[j], k.mq, k.cq) * k.iq, 0.0);
 }
 
-// The sum over the thread block, in every thread.
-__device__ __forceinline__ double block_sum(double v, double* lds)
+// The sum over the thread block, in every thread. lds: of this sum alone.
+__device__ __forceinline__ double block_sum(double v, double (&lds)[kWaves])
 {
     v = wave_sum64(v);
     if ((threadIdx.x & 63) == 0) lds[wave_id()] = v;
     __syncthreads();
-    double s = 0.0;
-    for (int w = 0; w < kThreads / 64; w++) s += lds[w];
-    __syncthreads();
-    return s;
+    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
-template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a, const Pick& k, int32_t chunk, bool all, double* lds)
+template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a, const Pick& k, int32_t chunk, double (&lds)[kWaves])
 {
-    double w[kEach], s = 0.0;
-    weights<DT>(a, k, chunk, all, w);
+    double s = 0.0;
+    weights<DT>(a, k, k.kind, chunk, [&](int, const double (&w)[Logits<DT>::N]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < kEach; j++) s += w[j];
+        for (int e = 0; e < Logits<DT>::N; e++) s += w[e];
+    });
     return block_sum(s, lds);
 }
 
-template <int DT> __global__ __launch_bounds__(kThreads) void draft_sums(DraftArgs a)
+// The draw itself, by the whole block. Chunk c's weight is sums[c], or where there are none p's, of the target's chunk sums.
+template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32_t i, const Pick& k, const double* sums)
 {
-    __shared__ double lds[kThreads / 64];
-    const int32_t i = blockIdx.x / a.chunks, chunk = blockIdx.x - i * a.chunks;
-    const Pick k = a.picks[i];
-    if (k.kind == kDone) return;
-    const double s = chunk_sum<DT>(a, k, chunk, false, lds);
-    if (threadIdx.x == 0) a.sums[static_cast<int64_t>(i) * a.chunks + chunk] = s;
-}
-
-// Inclusive sums over the thread block.
-__device__ __forceinline__ double block_scan(double v, double* lds)
-{
-    const int lane = threadIdx.x & 63, wave = wave_id();
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double u = __shfl_up(v, o, 64);
-        if (lane >= o) v += u;
-    }
-    if (lane == 63) lds[wave] = v;
-    __syncthreads();
-    for (int w = 0; w < wave; w++) v += lds[w];
-    __syncthreads();
-    return v;
-}
-
-template <int DT> __global__ __launch_bounds__(kThreads) void draft_pick(DraftArgs a)
-{
-    __shared__ double lds[kThreads / 64];
-    __shared__ int32_t s_place, s_last;
-    __shared__ double s_before;
     constexpr int N = Logits<DT>::N;
-    const int32_t i = blockIdx.x, tid = threadIdx.x;
-    const Pick k = a.picks[i];
-    if (k.kind == kDone) return;
-    double* sums = a.sums + static_cast<int64_t>(i) * a.chunks;
+    __shared__ double s_total[kWaves], s_other[kWaves], s_up[2][kWaves], s_part[kVecs][kWaves], s_before;
+    __shared__ int32_t s_chunk, s_last, s_place;
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+    const ChunkStat* st = a.stats + static_cast<int64_t>(k.row) * 2 * a.chunks;
+    if (tid == 0) s_chunk = s_place = 0x7FFFFFFF;
+    if (tid == 0) s_last = 0;
+    // the draft's chunk without it
+    int32_t kind = k.kind;
+    const int32_t other = kind == kFromOthers && k.token >= 0 && k.token < a.V ? k.token / kChunk<DT> : -1;
+    double others = 0.0;
+    if (other >= 0) others = chunk_sum<DT>(a, k, other, s_other);
+    const auto target = [&](int32_t c) { return st[c].m > -INFINITY ? st[c].s * exp2_64((static_cast<double>(st[c].m) - k.mp) * k.cp) * k.ip : 0.0; };
+    const auto weight = [&](int32_t c) { return c == other ? others : sums ? sums[c] : target(c); };
     double mine = 0.0;
-    for (int32_t c = tid; c < a.chunks; c += kThreads) mine += sums[c];
-    double total = block_sum(mine, lds);
-    const bool all = !(total > 0.0);  // p and q are equal: p
-    if (all) {
-        for (int32_t c = 0; c < a.chunks; c++) {
-            const double s = chunk_sum<DT>(a, k, c, true, lds);
-            if (tid == 0) sums[c] = s;
-        }
-        __syncthreads();
+    for (int32_t c = tid; c < a.chunks; c += kThreads) mine += weight(c);
+    double total = block_sum(mine, s_total);
+    const bool none = !(total > 0.0);  // p and q are equal, or the draft has all of p: p
+    if (none) {
+        kind = kFromTarget;
         mine = 0.0;
-        for (int32_t c = tid; c < a.chunks; c += kThreads) mine += sums[c];
-        total = block_sum(mine, lds);
+        for (int32_t c = tid; c < a.chunks; c += kThreads) mine += target(c);
+        __syncthreads();
+        total = block_sum(mine, s_total);
     }
     const float u = a.sample[i];
     const double r = total * (u > 0.0f ? u : 0.0f);
     // the chunk: the first whose inclusive sum is above r, or the last one with a weight
-    if (tid == 0) {
-        s_place = 0x7FFFFFFF;
-        s_last = 0;
-    }
-    double before = 0.0;
-    int32_t chunk = -1;
-    __syncthreads();
-    for (int32_t c0 = 0; c0 < a.chunks && chunk < 0; c0 += kThreads) {
+    double base = 0.0;
+    int32_t chunk = 0x7FFFFFFF;
+    for (int32_t c0 = 0, turn = 0; c0 < a.chunks && chunk == 0x7FFFFFFF; c0 += kThreads, turn ^= 1) {
         const int32_t c = c0 + tid;
-        const double v = c < a.chunks ? sums[c] : 0.0, up = before + block_scan(v, lds);
-        if (v > 0.0) {
-            atomicMax(&s_last, c);
-            if (up > r) atomicMin(&s_place, c);
+        const double v = c >= a.chunks ? 0.0 : none ? target(c) : weight(c);
+        double up = wave_scan64(v);
+        if (lane == 63) s_up[turn][wave] = up;
+        __syncthreads();
+        for (int w = 0; w < kWaves; w++) {
+            if (w == wave) up += base;
+            base += s_up[turn][w];
         }
+        const uint64_t some = __ballot(v > 0.0), above = __ballot(v > 0.0 && up > r);
+        if (lane == 0 && some) atomicMax(&s_last, c + 63 - __clzll(static_cast<long long>(some)));
+        if (lane == 0 && above) atomicMin(&s_chunk, c + __ffsll(static_cast<long long>(above)) - 1);
         __syncthreads();
-        if (s_place != 0x7FFFFFFF) chunk = s_place;
+        chunk = s_chunk;
         if (c == chunk) s_before = up - v;
-        if (tid == kThreads - 1) lds[0] = up;
-        __syncthreads();
-        before = chunk < 0 ? lds[0] : s_before;
-        __syncthreads();
-    }
-    const bool end = chunk < 0;  // rounding: the last weight of all
-    if (end) chunk = s_last;
-    if (tid == 0) {
-        s_place = 0x7FFFFFFF;
-        s_last = 0;
     }
     __syncthreads();
-    double w[kEach];
-    weights<DT>(a, k, chunk, all, w);
-#pragma unroll
-    for (int j = 0; j < kEach; j += N) {
+    const bool end = chunk == 0x7FFFFFFF;  // rounding: the last weight of all
+    if (end) chunk = s_last;
+    base = end ? 0.0 : s_before;
+    __syncthreads();
+    if (tid == 0) s_last = 0;
+    double w[kVecs][N], up[kVecs];
+    weights<DT>(a, k, kind, chunk, [&](int j, const double (&v)[N]) __attribute__((always_inline)) {
         double s = 0.0;
-        for (int e = 0; e < N; e++) s += w[j + e];
-        const double up = before + block_scan(s, lds);
-        double c = up - s;
-        const int32_t at = Logits<DT>::place(chunk, j / N);
-        int32_t last = -1, place = -1;
+#pragma unroll
         for (int e = 0; e < N; e++) {
-            c += w[j + e];
-            if (w[j + e] > 0.0) {
+            w[j][e] = v[e];
+            s += v[e];
+        }
+        up[j] = wave_scan64(s);
+        if (lane == 63) s_part[j][wave] = up[j];
+        up[j] -= s;
+    });
+    __syncthreads();
+    int32_t last = -1, place = 0x7FFFFFFF;
+#pragma unroll
+    for (int j = 0; j < kVecs; j++) {
+        double c = base;
+        for (int v = 0; v < kWaves; v++) {
+            if (v == wave) c = base + up[j];
+            base += s_part[j][v];
+        }
+        const int32_t at = Logits<DT>::place(chunk, j);
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            c += w[j][e];
+            if (w[j][e] > 0.0) {
                 last = at + e;
-                if (place < 0 && c > r) place = at + e;
+                if (c > r && place == 0x7FFFFFFF) place = at + e;
             }
         }
-        if (last >= 0) atomicMax(&s_last, last);
-        if (place >= 0 && !end) atomicMin(&s_place, place);
-        if (tid == kThreads - 1) lds[0] = up;
-        __syncthreads();
-        before = lds[0];
-        __syncthreads();
     }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        last = max(last, __shfl_xor(last, o, 64));
+        place = min(place, __shfl_xor(place, o, 64));
+    }
+    if (lane == 0 && last >= 0) atomicMax(&s_last, last);
+    if (lane == 0) atomicMin(&s_place, place);
+    __syncthreads();
     if (tid == 0) {
-        const int32_t token = s_place != 0x7FFFFFFF ? s_place : s_last;
+        const int32_t token = !end && s_place != 0x7FFFFFFF ? s_place : s_last;
         a.out[i * a.out_stride + k.place] = token;
         if (a.logp)
             a.logp[i * a.out_stride + k.place] =
                 static_cast<float>((static_cast<double>(Vec<DT>::load1(a.target, k.row * a.zs + token)) - k.mp) * (k.cp / kLog2e64) + log(k.ip));
     }
+}
+
+// Drafts that were chosen, or none: the sums of p are there, a thread block a request does the rest.
+template <int DT> __global__ __launch_bounds__(kThreads) void draft_choose(DraftArgs a)
+{
+    __shared__ DecideLds lds;
+    const Pick k = decide<DT>(a, blockIdx.x, lds);
+    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, nullptr);
+}
+
+// Drafts that were drawn: what is accepted, then a thread block for each chunk of the row that is drawn from.
+template <int DT> __global__ __launch_bounds__(kThreads) void draft_decide(DraftArgs a)
+{
+    __shared__ DecideLds lds;
+    const Pick k = decide<DT>(a, blockIdx.x, lds);
+    if (threadIdx.x == 0) a.picks[blockIdx.x] = k;
+}
+
+template <int DT> __global__ __launch_bounds__(kThreads) void draft_sums(DraftArgs a)
+{
+    __shared__ double s_sum[kWaves];
+    const int32_t i = blockIdx.x / a.chunks, chunk = blockIdx.x - i * a.chunks;
+    const Pick k = a.picks[i];
+    if (k.kind != kFromRest) return;
+    const double s = chunk_sum<DT>(a, k, chunk, s_sum);
+    if (threadIdx.x == 0) a.sums[static_cast<int64_t>(i) * a.chunks + chunk] = s;
+}
+
+template <int DT> __global__ __launch_bounds__(kThreads) void draft_pick(DraftArgs a)
+{
+    const Pick k = a.picks[blockIdx.x];
+    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, k.kind == kFromRest ? a.sums + static_cast<int64_t>(blockIdx.x) * a.chunks : nullptr);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
@@ -499,33 +607,39 @@ static int64_t work_of(int64_t B, int64_t T, int64_t chunks)
     return T * 2 * chunks * static_cast<int64_t>(sizeof(ChunkStat)) + round16(B * static_cast<int64_t>(sizeof(Pick))) + round16(B * chunks * 8);
 }
 
-static int check_sizes(int64_t B, int64_t T, int64_t V)
+// chunks: of the smaller kind, f32's.
+static int check_sizes(int64_t B, int64_t T, int64_t V, int64_t* chunks)
 {
     if (B < 0 || T < 0 || V < 1) return fail(SLHIP_ERR_INVALID, "draft_verify: bad size");
-    const int64_t chunks = (V + kChunk - 1) / kChunk;
-    if (B > 65536 || V > kMaxVocab || T * chunks * 2 > 0xFFFFFF || B * chunks > 0xFFFFFF)
+    *chunks = (V + kChunk<SLHIP_F32> - 1) / kChunk<SLHIP_F32>;
+    if (B > 65536 || V > kMaxVocab || T * *chunks * 2 > 0xFFFFFF || B * *chunks > 0xFFFFFF)
         return fail(SLHIP_ERR_UNSUPPORTED, "draft_verify: too many requests, rows or tokens of the vocabulary");
     return SLHIP_OK;
 }
 
-template <int DT> static int launch(const DraftArgs& a, hipStream_t st)
+template <int DT> static int launch(DraftArgs& a, hipStream_t st)
 {
-    const int64_t rows = a.T * a.chunks;
+    a.chunks = (a.V + kChunk<DT> - 1) / kChunk<DT>;
+    const unsigned rows = static_cast<unsigned>(a.T * a.chunks), B = static_cast<unsigned>(a.B);
     if (rows > 0) {
         if (a.draft)
-            draft_stats<DT, true><<<static_cast<unsigned>(rows * 2), kThreads, 0, st>>>(a);
+            draft_stats<DT, true><<<rows * 2, kThreads, 0, st>>>(a);
         else
-            draft_stats<DT, false><<<static_cast<unsigned>(rows), kThreads, 0, st>>>(a);
+            draft_stats<DT, false><<<rows, kThreads, 0, st>>>(a);
         const int e = check_launch("draft_stats");
         if (e) return e;
     }
-    draft_decide<DT><<<static_cast<unsigned>(a.B), kDecide, 0, st>>>(a);
+    if (!a.draft) {
+        draft_choose<DT><<<B, kThreads, 0, st>>>(a);
+        return check_launch("draft_choose");
+    }
+    draft_decide<DT><<<B, kThreads, 0, st>>>(a);
     int e = check_launch("draft_decide");
     if (e) return e;
-    draft_sums<DT><<<static_cast<unsigned>(a.B * a.chunks), kThreads, 0, st>>>(a);
+    draft_sums<DT><<<B * a.chunks, kThreads, 0, st>>>(a);
     e = check_launch("draft_sums");
     if (e) return e;
-    draft_pick<DT><<<static_cast<unsigned>(a.B), kThreads, 0, st>>>(a);
+    draft_pick<DT><<<B, kThreads, 0, st>>>(a);
     return check_launch("draft_pick");
 }
 
@@ -535,8 +649,9 @@ using namespace slhip;
 
 extern "C" SLHIP_API int64_t slhip_draft_verify_work_bytes(int64_t requests, int64_t tokens, int64_t vocab)
 {
-    if (check_sizes(requests, tokens, vocab)) return -1;
-    return work_of(requests, tokens, (vocab + kChunk - 1) / kChunk);
+    int64_t chunks;
+    if (check_sizes(requests, tokens, vocab, &chunks)) return -1;
+    return work_of(requests, tokens, chunks);
 }
 
 extern "C" SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64_t target_stride, const void* draft, int64_t draft_stride,
@@ -544,7 +659,8 @@ extern "C" SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64
 {
     if (!d) return fail(SLHIP_ERR_INVALID, "draft_verify: arguments are null");
     if (dtype != SLHIP_F32 && dtype != SLHIP_BF16) return fail(SLHIP_ERR_UNSUPPORTED, "draft_verify: dtype %d not supported", dtype);
-    int e = check_sizes(d->requests, d->tokens, d->vocab);
+    int64_t chunks;
+    int e = check_sizes(d->requests, d->tokens, d->vocab, &chunks);
     if (e) return e;
     if (d->out_stride < 0 || d->out_stride > 0x7FFFFFFF) return fail(SLHIP_ERR_INVALID, "draft_verify: bad stride of the tokens");
     if (target_stride < d->vocab || (draft && draft_stride < d->vocab))
@@ -553,7 +669,7 @@ extern "C" SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64
     if (!d->starts || !d->n_out || (d->out_stride > 0 && !d->out)) return fail(SLHIP_ERR_INVALID, "draft_verify: starts, out and n_out are required");
     if (d->tokens > 0 && (!target || !d->ids || !d->accept || !d->sample))
         return fail(SLHIP_ERR_INVALID, "draft_verify: target, ids, accept and sample are required");
-    const int64_t chunks = (d->vocab + kChunk - 1) / kChunk, need = work_of(d->requests, d->tokens, chunks);
+    const int64_t need = work_of(d->requests, d->tokens, chunks);
     if (!work || !aligned16(work) || work_bytes < need)
         return fail(SLHIP_ERR_INVALID, "draft_verify: the workspace has %lld bytes, %lld are needed (16-byte aligned)",
                     static_cast<long long>(work ? work_bytes : 0), static_cast<long long>(need));
@@ -565,7 +681,6 @@ extern "C" SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64
     a.T = d->tokens;
     a.B = static_cast<int32_t>(d->requests);
     a.V = static_cast<int32_t>(d->vocab);
-    a.chunks = static_cast<int32_t>(chunks);
     a.starts = d->starts;
     a.ids = d->ids;
     a.tau = d->temperature;

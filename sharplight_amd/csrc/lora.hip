@@ -11,9 +11,10 @@
 // With mfma 16x16x32 (A[m][8g+j], B[8g+j][n], C[4g+r][n] in lane (n or m) + 16 g) adapters are the first operand and rows the
 // second one, so that a lane's sums are four neighbours of one row: h is stored and y made without an exchange.
 //
-// Numbers. bf16 rows and adapters go to the bf16 matrix cores as they are (products exact, sums f32). h stays f32; for bf16
-// results of bf16 adapters it goes on as two bf16 parts (2^-17 of itself, against the result's 2^-8), which fill the two halves of one
-// instruction's 32 products for 16 ranks. All else takes f32 matrix cores with every operand widened.
+// Numbers. All products are of bf16 numbers on the matrix cores, with f32 sums. A number of another type is the sum of bf16 ones, exactly:
+// f16 of two, f32 of three, each the last one's remainder cut to 8 bits; a product takes all pairs. h stays f32; for f32
+// results it goes on in three parts, for bf16 ones in two (2^-17 of itself, against the result's 2^-8). Two parts of 16 ranks fill the two
+// halves of one instruction's 32 products.
 #include "kv8_map.hpp"
 #include "step.hpp"
 
@@ -77,12 +78,36 @@ __device__ __forceinline__ int32_t block_scan(int32_t v, int32_t* lds, int32_t& 
     return v;
 }
 
+// The same for up to 64 requests, a lane each: one memory latency, and nothing but the rows goes through LDS.
+template <int TM> __device__ __forceinline__ int32_t find_tile_64(const LoraArgs& a, int64_t item, int32_t* s_rows)
+{
+    const int lane = threadIdx.x & 63, j = min(lane, a.B - 1);
+    const int32_t s0 = a.starts[j], mine = lane < a.B ? rows_of(a, j) : 0, own = adapter_of(a, j);
+    const int k = max(__popcll(__ballot(lane < a.B && item_base(s0, j, TM, 1) <= item)) - 1, 0);
+    const int32_t n = __builtin_amdgcn_readlane(mine, k), key = __builtin_amdgcn_readlane(own, k), at = __builtin_amdgcn_readlane(s0, k);
+    const int64_t piece = item - item_base(at, k, TM, 1);
+    if (piece < 0 || piece * TM >= n) return kNoTile;
+    const int32_t match = own == key ? mine : 0, up = wave_scan(match) - match, before = __builtin_amdgcn_readlane(up, k);
+    const int64_t first = ((static_cast<int64_t>(before) + TM - 1) / TM + piece) * TM, off = first - before;
+    if (off < 0 || off >= n) return kNoTile;  // (below 0 where requests overlap, which none may)
+    if (threadIdx.x < 64) {
+        const int32_t have = static_cast<int32_t>(min(static_cast<int64_t>(TM), n - off));
+        if (lane < TM) s_rows[lane] = lane < have ? at + static_cast<int32_t>(off) + lane : -1;
+        if (lane > k && up >= static_cast<int64_t>(before) + n) {
+            for (int32_t r = 0; r < match && up + r - first < TM; r++) s_rows[up + r - first] = s0 + r;
+        }
+    }
+    __syncthreads();
+    return key;
+}
+
 // The rows of tile `item` into s_rows (-1 behind the last), and their adapter; kNoTile where there is none.
 template <int TM> __device__ __forceinline__ int32_t find_tile(const LoraArgs& a, int64_t item, int32_t* s_rows, int32_t* lds)
 {
     const int lane = threadIdx.x & 63, tid = threadIdx.x;
+    if (a.B <= 64) return find_tile_64<TM>(a, item, s_rows);
     int32_t i = 0;
-    if (a.B > 1) {  // as row_request, by the requests' first items
+    {   // as row_request, by the requests' first items
         int32_t lo = 0, n = a.B;
         while (n > 64) {
             const int32_t step = (n + 63) / 64, j = lo + lane * step;
@@ -103,11 +128,7 @@ template <int TM> __device__ __forceinline__ int32_t find_tile(const LoraArgs& a
     int32_t before = 0;
     for (int32_t j = tid; j < i; j += kThreads)
         if (adapter_of(a, j) == key) before += rows_of(a, j);
-    if (a.B > 1) {
-        int32_t total;
-        block_scan(before, lds, total);
-        before = total;
-    }
+    block_scan(before, lds, before);
     const int64_t off = ((static_cast<int64_t>(before) + TM - 1) / TM + piece) * TM - before;
     if (off < 0 || off >= n) return kNoTile;  // (below 0 where requests overlap, which none may)
     int32_t have = static_cast<int32_t>(min(static_cast<int64_t>(TM), n - off));
@@ -132,11 +153,36 @@ __device__ __forceinline__ int32_t rank_of(const LoraArgs& a, int32_t adapter)
 
 // ---- loads ---------------------------------------------------------------------------------------------------------
 
-// N neighbours (4, 8 or 16) of which the first n are there; the others are 0.
+template <int DT> constexpr int kParts = DT == SLHIP_BF16 ? 1 : DT == SLHIP_F16 ? 2 : 3;
+
+// v as P bf16 numbers that add up to it (all of its bits are in them). An infinity leaves a NaN behind.
+template <int P> __device__ __forceinline__ void cut(const float (&v)[8], bf16x8 (&p)[P])
+{
+    float r[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) r[e] = v[e];
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(__float_as_uint(r[2 * e + 1]), __float_as_uint(r[2 * e]), 0x07060302u);  // upper halves
+        p[i] = __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+        for (int e = 0; e < 8; e++) r[e] -= __uint_as_float(__float_as_uint(r[e]) & 0xFFFF0000u);
+    }
+}
+
+// N neighbours (8 or 16) of which the first n are there; the others are 0.
 template <int DT, int N> struct Run {
     static constexpr int kVecs = N * Vec<DT>::BYTES / 16, kPer = Vec<DT>::N;
     uint4 w[kVecs];
-    __device__ __forceinline__ void load(const void* p, int64_t at, int64_t n)
+    __device__ __forceinline__ void load(const void* p, int64_t at)
+    {
+        const char* c = static_cast<const char*>(p) + at * Vec<DT>::BYTES;
+#pragma unroll
+        for (int i = 0; i < kVecs; i++) w[i] = load_any(c + 16 * i);
+    }
+    __device__ __forceinline__ void load_some(const void* p, int64_t at, int64_t n)
     {
         const char* c = static_cast<const char*>(p) + at * Vec<DT>::BYTES;
 #pragma unroll
@@ -152,40 +198,26 @@ template <int DT, int N> struct Run {
             }
         }
     }
-    __device__ __forceinline__ void floats(float (&f)[N]) const
+    // Eight of them as bf16 parts.
+    template <int P> __device__ __forceinline__ void parts(int half, bf16x8 (&p)[P]) const
     {
+        if constexpr (DT == SLHIP_BF16) {
+            p[0] = __builtin_bit_cast(bf16x8, w[half]);
+        } else {
+            float f[8];
 #pragma unroll
-        for (int i = 0; i < kVecs; i++) Vec<DT>::unpack(w[i], &f[i * kPer]);
+            for (int i = 0; i < 8 / kPer; i++) Vec<DT>::unpack(w[half * (8 / kPer) + i], &f[i * kPer]);
+            cut(f, p);
+        }
     }
 };
-
-// Four neighbours, the first n of them, as f32.
-template <int DT> __device__ __forceinline__ f32x4 four(const void* p, int64_t at, int64_t n)
-{
-    f32x4 f = {0, 0, 0, 0};
-    if (n >= 4) {
-        if constexpr (DT == SLHIP_F32) {
-            __builtin_memcpy(&f, static_cast<const float*>(p) + at, 16);
-        } else {
-            uint2 w;
-            __builtin_memcpy(&w, static_cast<const uint16_t*>(p) + at, 8);
-            f = DT == SLHIP_BF16 ? f32x4{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)}
-                                 : f32x4{f16_lo(w.x), f16_hi(w.x), f16_lo(w.y), f16_hi(w.y)};
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (j < n) f[j] = Vec<DT>::load1(p, at + j);
-    }
-    return f;
-}
 
 // ---- h = A x -------------------------------------------------------------------------------------------------------
 
 template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads) void lora_shrink(LoraArgs a)
 {
-    constexpr bool BF = XT == SLHIP_BF16 && WT == SLHIP_BF16;
-    constexpr int TM = 16 * MT, U = BF ? 2 : 1;
+    constexpr int TM = 16 * MT, PX = kParts<XT>, PW = kParts<WT>;
+    constexpr int U = MT * RB == 1 ? 4 : MT == 1 || XT == SLHIP_BF16 ? 2 : 1;  // units whose loads are on their way together
     __shared__ int32_t s_rows[TM], lds[kWaves];
     __shared__ f32x4 s_acc[kWaves / 2][MT * RB][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), c = lane & 15, g = lane >> 4;
@@ -205,61 +237,67 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
     if (r0 >= rank) return;
     const int32_t units = (a.K + kUnit - 1) / kUnit, each = (units + a.splits - 1) / a.splits;
     const int32_t u0 = split * each, u1 = min(u0 + each, units);
+    // rows and ranks that are not there: others, whose sums nothing takes
     int64_t xp[MT], ap[RB];
-    bool xin[MT], ain[RB];
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int32_t row = s_rows[16 * m + c];
-        xin[m] = row >= 0;
-        xp[m] = (row >= 0 ? row : 0) * a.xs + 16 * g;
+        xp[m] = (row >= 0 ? row : s_rows[0]) * a.xs + 16 * g;
     }
 #pragma unroll
-    for (int q = 0; q < RB; q++) {
-        const int32_t r = r0 + 16 * q + c;
-        ain[q] = r < rank;
-        ap[q] = key * a.sa + static_cast<int64_t>(ain[q] ? r : 0) * a.K + 16 * g;
-    }
+    for (int q = 0; q < RB; q++) ap[q] = key * a.sa + static_cast<int64_t>(min(r0 + 16 * q + c, rank - 1)) * a.K + 16 * g;
     f32x4 acc[MT][RB];
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int q = 0; q < RB; q++) acc[m][q] = f32x4{0, 0, 0, 0};
-    for (int32_t u = u0 + wave; u < u1; u += kWaves * U) {
+    const int32_t ranks = (min(rank - r0, RB * 16) + 15) / 16;
+    const auto multiply = [&](const Run<XT, 16> (&x)[MT], const Run<WT, 16> (&w)[RB]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            bf16x8 px[MT][PX];
+#pragma unroll
+            for (int m = 0; m < MT; m++) x[m].parts(s, px[m]);
+#pragma unroll
+            for (int q = 0; q < RB; q++) {
+                if (q > 0 && q >= ranks) break;
+                bf16x8 pw[PW];
+                w[q].parts(s, pw);
+#pragma unroll
+                for (int i = PX - 1; i >= 0; i--)  // small ones first
+#pragma unroll
+                    for (int j = PW - 1; j >= 0; j--)
+#pragma unroll
+                        for (int m = 0; m < MT; m++) acc[m][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pw[j], px[m][i], acc[m][q], 0, 0, 0);
+            }
+        }
+    };
+    int32_t u = u0 + wave;
+    const int32_t whole = min(u1, a.K / kUnit);  // (the last unit may not be)
+    for (; u + (U - 1) * kWaves < whole; u += kWaves * U) {
         Run<XT, 16> x[U][MT];
         Run<WT, 16> w[U][RB];
 #pragma unroll
         for (int v = 0; v < U; v++) {
-            const int64_t k = static_cast<int64_t>(u + v * kWaves) * kUnit, n = u + v * kWaves < u1 ? a.K - k - 16 * g : 0;
+            const int64_t k = static_cast<int64_t>(u + v * kWaves) * kUnit;
 #pragma unroll
-            for (int q = 0; q < RB; q++) w[v][q].load(a.a, ap[q] + k, ain[q] ? n : 0);
+            for (int q = 0; q < RB; q++)
+                if (q == 0 || q < ranks) w[v][q].load(a.a, ap[q] + k);
 #pragma unroll
-            for (int m = 0; m < MT; m++) x[v][m].load(a.x, xp[m] + k, xin[m] ? n : 0);
+            for (int m = 0; m < MT; m++) x[v][m].load(a.x, xp[m] + k);
         }
 #pragma unroll
-        for (int v = 0; v < U; v++) {
-            if constexpr (BF) {
+        for (int v = 0; v < U; v++) multiply(x[v], w[v]);
+    }
+    for (; u < u1; u += kWaves) {
+        Run<XT, 16> x[MT];
+        Run<WT, 16> w[RB];
+        const int64_t k = static_cast<int64_t>(u) * kUnit, n = a.K - k - 16 * g;
 #pragma unroll
-                for (int s = 0; s < 2; s++)
+        for (int q = 0; q < RB; q++) w[q].load_some(a.a, ap[q] + k, n);
 #pragma unroll
-                    for (int m = 0; m < MT; m++)
-#pragma unroll
-                        for (int q = 0; q < RB; q++)
-                            acc[m][q] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[v][q].w[s]), __builtin_bit_cast(bf16x8, x[v][m].w[s]), acc[m][q], 0, 0, 0);
-            } else {
-                float fw[RB][16];
-#pragma unroll
-                for (int q = 0; q < RB; q++) w[v][q].floats(fw[q]);
-#pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    float fx[16];
-                    x[v][m].floats(fx);
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-#pragma unroll
-                        for (int q = 0; q < RB; q++) acc[m][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(fw[q][e], fx[e], acc[m][q], 0, 0, 0);
-                }
-            }
-        }
+        for (int m = 0; m < MT; m++) x[m].load_some(a.x, xp[m] + k, n);
+        multiply(x, w);
     }
     // the sums of waves 2 and 3 into 0 and 1, and 1 into 0
     for (int half = kWaves / 2; half > 0; half >>= 1) {
@@ -292,24 +330,39 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
 
 // ---- y = add + s B h -----------------------------------------------------------------------------------------------
 
-// Eight neighbours of a row of add or y.
+// Eight neighbours of a row of add or y, the first n of them.
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 template <int DT> struct Eight {
-    static constexpr int kVecs = 8 * Vec<DT>::BYTES / 16;
-    __device__ static __forceinline__ void load(const void* p, int64_t at, int32_t n, float (&f)[8])
+    static constexpr int kVecs = 8 * Vec<DT>::BYTES / 16, kPer = Vec<DT>::N;
+    u32x4 w[kVecs];
+    __device__ __forceinline__ void load(const void* p, int64_t at)
     {
         const char* c = static_cast<const char*>(p) + at * Vec<DT>::BYTES;
-        if (n >= 8) {
 #pragma unroll
-            for (int i = 0; i < kVecs; i++) {
-                const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(c + 16 * i));
-                Vec<DT>::unpack(make_uint4(w.x, w.y, w.z, w.w), &f[i * Vec<DT>::N]);
+        for (int i = 0; i < kVecs; i++) w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(c + 16 * i));
+    }
+    __device__ __forceinline__ void load_some(const void* p, int64_t at, int32_t n)
+    {
+        const char* c = static_cast<const char*>(p) + at * Vec<DT>::BYTES;
+#pragma unroll
+        for (int i = 0; i < kVecs; i++) {
+            w[i] = u32x4{0, 0, 0, 0};
+            if (n >= 8) {
+                w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(c + 16 * i));
+            } else if (n > i * kPer) {
+                float f[kPer] = {};
+                for (int j = 0; j < kPer; j++)
+                    if (i * kPer + j < n) f[j] = Vec<DT>::load1(c, i * kPer + j);
+                const uint4 v = Vec<DT>::pack(f);  // the same bits again
+                w[i] = u32x4{v.x, v.y, v.z, v.w};
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) f[j] = j < n ? Vec<DT>::load1(c, j) : 0.0f;
         }
+    }
+    __device__ __forceinline__ void floats(float (&f)[8]) const
+    {
+#pragma unroll
+        for (int i = 0; i < kVecs; i++) Vec<DT>::unpack(make_uint4(w[i].x, w[i].y, w[i].z, w[i].w), &f[i * kPer]);
     }
     __device__ static __forceinline__ void store(void* p, int64_t at, int32_t n, const float (&f)[8])
     {
@@ -317,7 +370,7 @@ template <int DT> struct Eight {
         if (n >= 8) {
 #pragma unroll
             for (int i = 0; i < kVecs; i++) {
-                const uint4 w = Vec<DT>::pack(&f[i * Vec<DT>::N]);
+                const uint4 w = Vec<DT>::pack(&f[i * kPer]);
                 const u32x4 t = {w.x, w.y, w.z, w.w};
                 __builtin_nontemporal_store(t, reinterpret_cast<u32x4_any*>(c + 16 * i));
             }
@@ -329,99 +382,132 @@ template <int DT> struct Eight {
     }
 };
 
-// The two bf16 parts of v: what is left of an infinity is 0.
+// The two bf16 parts of v, rounded: what is left of an infinity is 0.
 __device__ __forceinline__ float low_part(float v, float hi) { return fabsf(hi) < INFINITY ? v - hi : 0.0f; }
 
 template <int YT, int WT, int MT> __global__ __launch_bounds__(kThreads) void lora_expand(LoraArgs a)
 {
-    constexpr bool BF = YT == SLHIP_BF16 && WT == SLHIP_BF16;
-    constexpr int TM = 16 * MT;
+    constexpr int TM = 16 * MT, PW = kParts<WT>;
+    constexpr int H = YT == SLHIP_BF16 ? 1 : 2;  // instructions that take h's parts of 16 ranks
     __shared__ int32_t s_rows[TM], lds[kWaves];
-    extern __shared__ uint4 s_h[];  // [MT][ranks / 16][64]: the second operand of 16 ranks
+    extern __shared__ uint4 s_h[];  // [MT][ranks / 16][H][64]: the second operand of 16 ranks
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), c = lane & 15, g = lane >> 4;
     const int32_t cb = blockIdx.x % a.col_blocks;
     const int32_t key = find_tile<TM>(a, blockIdx.x / a.col_blocks, s_rows, lds);
     if (key == kNoTile || (key < 0 && a.add == a.y)) return;
     const int32_t rank = key < 0 ? 0 : rank_of(a, key), tiles = (rank + 15) / 16;
     const float scale = key < 0 || !a.scale ? 1.0f : a.scale[key];
-    for (int t = tid; t < MT * tiles * 64; t += kThreads) {
-        const int m = t / (tiles * 64), q = t / 64 - m * tiles, l = t & 63;
-        const int32_t row = s_rows[16 * m + (l & 15)];
-        constexpr int E = BF ? 8 : 4;
-        const int32_t r = 16 * q + (BF ? 8 * (l >> 4 & 1) : 4 * (l >> 4));
-        float f[E] = {};
-        if (row >= 0) {
-            for (int s = 0; s < a.splits; s++) {
-                const f32x4* p = reinterpret_cast<const f32x4*>(a.h + (static_cast<int64_t>(s) * a.T + row) * a.R16 + r);
-#pragma unroll
-                for (int e = 0; e < E; e++) f[e] += p[e >> 2][e & 3];
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < E; e++) f[e] = r + e < rank ? f[e] * scale : 0.0f;
-        if constexpr (BF) {
-            float hi[8], lo[8];
-            const uint4 w = Vec<SLHIP_BF16>::pack(f);
-            Vec<SLHIP_BF16>::unpack(w, hi);
-#pragma unroll
-            for (int e = 0; e < 8; e++) lo[e] = low_part(f[e], hi[e]);
-            s_h[t] = l < 32 ? w : Vec<SLHIP_BF16>::pack(lo);
-        } else {
-            s_h[t] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-        }
-    }
-    __syncthreads();
     int32_t row[MT];
 #pragma unroll
     for (int m = 0; m < MT; m++) row[m] = s_rows[16 * m + c];
     const int64_t base = key < 0 ? 0 : key * a.sb;
+    // Columns of a product u: a lane gets four in a row, with u + 1 (u even) eight. Those behind the last are others, which are not stored.
+    const auto column = [&](int32_t n0, int u) { return min(n0 + 32 * (u >> 1) + 8 * (c >> 2) + 4 * (u & 1) + (c & 3), a.N - 1); };
+    Eight<YT> add[MT][2];
+    Run<WT, 8> w[4];
+    const auto fetch_w = [&](int32_t n0, int q) __attribute__((always_inline)) {
+        const int32_t r = 16 * q + 8 * (g & 1);
+        if (16 * q + 16 <= rank) {
+#pragma unroll
+            for (int u = 0; u < 4; u++) w[u].load(a.b, base + static_cast<int64_t>(column(n0, u)) * a.R + r);
+        } else {  // ranks behind the last are not read
+#pragma unroll
+            for (int u = 0; u < 4; u++) w[u].load_some(a.b, base + static_cast<int64_t>(column(n0, u)) * a.R + r, rank - r);
+        }
+    };
+    const auto fetch = [&](int32_t n0) __attribute__((always_inline)) {
+        if (tiles > 0) fetch_w(n0, 0);
+        if (a.add && n0 + 64 <= a.N) {
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int p = 0; p < 2; p++) add[m][p].load(a.add, (row[m] >= 0 ? row[m] : s_rows[0]) * a.as + n0 + 32 * p + 8 * g);
+        } else {
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    const int32_t n = n0 + 32 * p + 8 * g;
+                    add[m][p].load_some(a.add, row[m] * a.as + n, a.add && row[m] >= 0 ? a.N - n : 0);
+                }
+        }
+    };
+    const int32_t first = (cb * a.col_steps * kWaves + wave) * 64;
+    if (first < a.N) fetch(first);
+    for (int t = tid; t < MT * tiles * 32; t += kThreads) {  // eight ranks of a row
+        const int m = t / (tiles * 32), q = t / 32 - m * tiles, l = t & 31;
+        const int32_t at = s_rows[16 * m + (l & 15)], r = 16 * q + 8 * (l >> 4);
+        float f[8] = {};
+        if (at >= 0) {
+            const float* h = a.h + static_cast<int64_t>(at) * a.R16 + r;
+            const int64_t step = a.T * a.R16;
+            for (int s0 = 0; s0 < a.splits; s0 += 8) {
+                f32x4 x[8][2];
+#pragma unroll
+                for (int s = 0; s < 8; s++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) x[s][e] = s0 + s < a.splits ? reinterpret_cast<const f32x4*>(h + (s0 + s) * step)[e] : f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < 8; s++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) f[e] += x[s][e >> 2][e & 3];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = r + e < rank ? f[e] * scale : 0.0f;
+        uint4* to = s_h + ((m * tiles + q) * H) * 64 + l;  // the parts of a row's 16 ranks: lanes l and l + 32
+        if constexpr (H == 1) {
+            float lo[8];
+            to[0] = Vec<SLHIP_BF16>::pack(f);
+            Vec<SLHIP_BF16>::unpack(to[0], lo);
+#pragma unroll
+            for (int e = 0; e < 8; e++) lo[e] = low_part(f[e], lo[e]);
+            to[32] = Vec<SLHIP_BF16>::pack(lo);
+        } else {
+            bf16x8 p[3];
+            cut(f, p);
+#pragma unroll
+            for (int i = 0; i < 3; i++) to[32 * i] = __builtin_bit_cast(uint4, p[i]);
+            to[96] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    __syncthreads();
     for (int j = 0; j < a.col_steps; j++) {
-        const int32_t n0 = ((cb * a.col_steps + j) * kWaves + wave) * 64;
+        const int32_t n0 = first + j * kWaves * 64;
         if (n0 >= a.N) break;
+        if (j > 0) fetch(n0);
         f32x4 acc[MT][4];
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
             for (int u = 0; u < 4; u++) acc[m][u] = f32x4{0, 0, 0, 0};
         for (int q = 0; q < tiles; q++) {
-            // product u has the columns of which a lane gets four in a row: with u + 1 (u even) eight
+            bf16x8 pw[4][PW];
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int32_t n = n0 + 32 * (u >> 1) + 8 * (c >> 2) + 4 * (u & 1) + (c & 3);
-                const int64_t at = base + static_cast<int64_t>(n < a.N ? n : 0) * a.R;
-                if constexpr (BF) {
-                    const int32_t r = 16 * q + 8 * (g & 1);
-                    Run<WT, 8> w;
-                    w.load(a.b, at + r, n < a.N ? rank - r : 0);
+            for (int u = 0; u < 4; u++) w[u].parts(0, pw[u]);
+            if (q + 1 < tiles) fetch_w(n0, q + 1);
 #pragma unroll
-                    for (int m = 0; m < MT; m++)
-                        acc[m][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w.w[0]), __builtin_bit_cast(bf16x8, s_h[(m * tiles + q) * 64 + lane]), acc[m][u], 0, 0, 0);
-                } else {
-                    const int32_t r = 16 * q + 4 * g;
-                    const f32x4 w = four<WT>(a.b, at + r, n < a.N ? rank - r : 0);
+            for (int m = 0; m < MT; m++)
 #pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        const f32x4 h = __builtin_bit_cast(f32x4, s_h[(m * tiles + q) * 64 + lane]);
+                for (int h = H - 1; h >= 0; h--) {
+                    const bf16x8 x = __builtin_bit_cast(bf16x8, s_h[((m * tiles + q) * H + h) * 64 + lane]);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) acc[m][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e], h[e], acc[m][u], 0, 0, 0);
-                    }
+                    for (int i = PW - 1; i >= 0; i--)
+#pragma unroll
+                        for (int u = 0; u < 4; u++) acc[m][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pw[u][i], x, acc[m][u], 0, 0, 0);
                 }
-            }
         }
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            if (row[m] < 0) continue;
+        for (int m = 0; m < MT; m++)
 #pragma unroll
             for (int p = 0; p < 2; p++) {
                 const int32_t n = n0 + 32 * p + 8 * g;
-                if (n >= a.N) continue;
-                float f[8] = {};
-                if (a.add) Eight<YT>::load(a.add, row[m] * a.as + n, a.N - n, f);
+                float f[8];
+                add[m][p].floats(f);
 #pragma unroll
                 for (int e = 0; e < 8; e++) f[e] += acc[m][2 * p + (e >> 2)][e & 3];
-                Eight<YT>::store(a.y, row[m] * a.ys + n, a.N - n, f);
+                if (row[m] >= 0 && n < a.N) Eight<YT>::store(a.y, row[m] * a.ys + n, a.N - n, f);
             }
-        }
     }
 }
 
@@ -437,16 +523,14 @@ static int64_t work_of(int64_t T, int64_t R)
 
 template <int XT, int WT, int MT> static int shrink(const LoraArgs& a, int64_t blocks, hipStream_t st)
 {
-    if (a.R16 <= 16)
-        lora_shrink<XT, WT, MT, 1><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
-    else
-        lora_shrink<XT, WT, MT, 4><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
+    const auto kernel = a.R16 <= 16 ? lora_shrink<XT, WT, MT, 1> : a.R16 <= 32 ? lora_shrink<XT, WT, MT, 2> : lora_shrink<XT, WT, MT, 4>;
+    kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
     return check_launch("lora_shrink");
 }
 
 template <int YT, int WT, int MT> static int expand(const LoraArgs& a, int64_t blocks, hipStream_t st)
 {
-    const int lds = MT * a.R16 * 64;
+    const int lds = MT * a.R16 * (YT == SLHIP_BF16 ? 64 : 128);
     if (lds > 60000)
         SLHIP_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&lora_expand<YT, WT, MT>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     lora_expand<YT, WT, MT><<<static_cast<unsigned>(blocks), kThreads, lds, st>>>(a);
@@ -456,9 +540,9 @@ template <int YT, int WT, int MT> static int expand(const LoraArgs& a, int64_t b
 template <int WT, int MT> static int launch(int dtype_x, int dtype_y, LoraArgs& a, hipStream_t st)
 {
     const int64_t items = item_count(a.T, a.B, 16 * MT, 1);
-    a.rank_blocks = a.R16 <= 16 ? 1 : (a.R16 + 63) / 64;
+    a.rank_blocks = a.R16 <= 32 ? 1 : (a.R16 + 63) / 64;
     // ranges of K: enough thread blocks for the machine, of 512 inputs at least
-    int64_t splits = 1024 / (items * a.rank_blocks), most = a.K / 512;
+    int64_t splits = 4096 / (items * a.rank_blocks), most = a.K / 512;
     if (splits > most) splits = most;
     if (splits > kMostSplits) splits = kMostSplits;
     if (splits > kSplitRows / a.T) splits = kSplitRows / a.T;

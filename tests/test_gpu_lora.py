@@ -60,7 +60,7 @@ class Case:
 
     def expected(self):
         return step_ref.lora(self.vx, self.vadd, self.va, self.vb, self.starts, self.adapter, self.ranks, self.scale,
-                             bf16_parts=self.dy == "bf16" and self.dw == "bf16")
+                             bf16_parts=self.dy == "bf16")
 
     def put(self, d, in_place=False, shift=0, x_stride=None, add_stride=None, y_stride=None, a_pad=0, b_pad=0):
         """The call's arguments; strides, shifts (elements) and gaps as asked, every gap a NaN."""
