@@ -622,7 +622,7 @@ SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64_t target_s
  *   y[t] = add[t] + scale[a] * B_a (A_a x[t]) for the rows starts[i] .. starts[i+1]-1 of request i, a = adapter[i];
  *   y[t] = add[t] where adapter[i] is -1.
  * A_a [max_rank, K] and B_a [N, max_rank] (rows dense) lie a_stride and b_stride elements after one another; of adapter a only the
- * first rank[a] ranks count (of fewer than max_rank, the others are not read). x [T, K] f32 or bf16 (dtype_x), add and y [T, N] (dtype_y), row strides
+ * first rank[a] ranks count (the others may hold anything). x [T, K] f32 or bf16 (dtype_x), add and y [T, N] (dtype_y), row strides
  * in elements; add may be y (in place: rows without an adapter are then not touched) or NULL (0). Rows from starts[B] on are padding: neither
  * read nor written. starts[0] is 0 and starts never falls; starts, adapter and rank are int32 on the device.
  * A x is summed and held in f32 (for bf16 y B takes it in two bf16 parts, to 2^-17 of itself); y is rounded once. A row
@@ -631,7 +631,7 @@ SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64_t target_s
  * that does not fit the rows is left as it was and reported (SLHIP_ERR_CACHE).
  * work: workspace of work_bytes >= slhip_lora_work_bytes(tokens, max_rank) (enough for fewer tokens and ranks too), 16-byte
  * aligned; calls that may overlap each need their own. It needs no initialisation and keeps nothing.
- * max_rank <= 256, K and N <= 2^24, requests <= 4096. Any alignment; rows and adapters of 16-byte steps are fastest.
+ * max_rank <= 256, K and N 8 .. 2^24, a matrix of an adapter less than 2^31 bytes, requests <= 4096. Any alignment; rows and adapters of 16-byte steps are fastest.
  */
 typedef struct slhip_lora_set {
     int32_t dtype; /* of a and b: F32, F16 or BF16 */

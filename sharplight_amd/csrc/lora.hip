@@ -15,6 +15,8 @@
 // f16 of two, f32 of three, each the last one's remainder cut to 8 bits; a product takes all pairs. h stays f32; for f32
 // results it goes on in three parts, for bf16 ones in two (2^-17 of itself, against the result's 2^-8). Two parts of 16 ranks fill the two
 // halves of one instruction's 32 products.
+#include <type_traits>
+
 #include "kv8_map.hpp"
 #include "step.hpp"
 
@@ -43,7 +45,8 @@ struct LoraArgs {
     int64_t T;
     const int32_t *starts, *adapter;
     float* h;  // [splits][T][R16]
-    int32_t splits, rank_blocks, col_blocks, col_steps;
+    int32_t splits, rank_blocks, col_blocks;
+    int32_t spare;  // columns that the last 16 ranks of one may reach into
     uint32_t* err;
 };
 
@@ -101,11 +104,79 @@ template <int TM> __device__ __forceinline__ int32_t find_tile_64(const LoraArgs
     return key;
 }
 
+// The same for up to kHeld * 256 requests: a thread holds kHeld of them, so there is one memory latency.
+constexpr int kHeld = 4;
+
+template <int TM> __device__ __forceinline__ int32_t find_tile_held(const LoraArgs& a, int64_t item, int32_t* s_rows)
+{
+    __shared__ int32_t s_at[kWaves], s_one[3], s_before[kWaves], s_sum[kHeld][kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+    int32_t s0[kHeld], n[kHeld], key[kHeld], begun = 0;
+#pragma unroll
+    for (int e = 0; e < kHeld; e++) {
+        const int32_t j = tid + e * kThreads, at = min(j, a.B - 1);
+        s0[e] = a.starts[at];
+        n[e] = j < a.B ? rows_of(a, at) : 0;
+        key[e] = adapter_of(a, at);
+    }
+#pragma unroll
+    for (int e = 0; e < kHeld; e++) {
+        const int32_t j = tid + e * kThreads;
+        begun += __popcll(__ballot(j < a.B && item_base(s0[e], j, TM, 1) <= item));
+    }
+    if (lane == 0) s_at[wave] = begun;
+    if (tid < TM) s_rows[tid] = -1;
+    __syncthreads();
+    const int32_t i = max((s_at[0] + s_at[1]) + (s_at[2] + s_at[3]) - 1, 0);
+#pragma unroll
+    for (int e = 0; e < kHeld; e++)
+        if (tid + e * kThreads == i) {
+            s_one[0] = s0[e];
+            s_one[1] = n[e];
+            s_one[2] = key[e];
+        }
+    __syncthreads();
+    const int32_t at = s_one[0], rows = s_one[1], mine = s_one[2];
+    const int64_t piece = item - item_base(at, i, TM, 1);
+    if (piece < 0 || piece * TM >= rows) return kNoTile;
+    int32_t up[kHeld], before = 0;
+#pragma unroll
+    for (int e = 0; e < kHeld; e++) {
+        if (key[e] != mine) n[e] = 0;
+        up[e] = wave_scan(n[e]);
+        if (lane == 63) s_sum[e][wave] = up[e];
+        up[e] -= n[e];
+        before += tid + e * kThreads < i ? n[e] : 0;
+    }
+    before = wave_scan(before);
+    if (lane == 63) s_before[wave] = before;
+    __syncthreads();
+    before = (s_before[0] + s_before[1]) + (s_before[2] + s_before[3]);
+    const int64_t first = ((static_cast<int64_t>(before) + TM - 1) / TM + piece) * TM, off = first - before;
+    if (off < 0 || off >= rows) return kNoTile;  // (below 0 where requests overlap, which none may)
+    if (tid < min(static_cast<int64_t>(TM), rows - off)) s_rows[tid] = at + static_cast<int32_t>(off) + tid;
+    int64_t base = -first;  // of the wave's requests
+#pragma unroll
+    for (int e = 0; e < kHeld; e++) {
+        int64_t to = base + up[e];
+        for (int w = 0; w < kWaves; w++) {
+            to += w < wave ? s_sum[e][w] : 0;
+            base += s_sum[e][w];
+        }
+        if (tid + e * kThreads > i && to >= 1) {
+            for (int32_t r = 0; r < n[e] && to + r < TM; r++) s_rows[to + r] = s0[e] + r;
+        }
+    }
+    __syncthreads();
+    return mine;
+}
+
 // The rows of tile `item` into s_rows (-1 behind the last), and their adapter; kNoTile where there is none.
 template <int TM> __device__ __forceinline__ int32_t find_tile(const LoraArgs& a, int64_t item, int32_t* s_rows, int32_t* lds)
 {
     const int lane = threadIdx.x & 63, tid = threadIdx.x;
     if (a.B <= 64) return find_tile_64<TM>(a, item, s_rows);
+    if (a.B <= kHeld * kThreads) return find_tile_held<TM>(a, item, s_rows);
     int32_t i = 0;
     {   // as row_request, by the requests' first items
         int32_t lo = 0, n = a.B;
@@ -172,31 +243,55 @@ template <int P> __device__ __forceinline__ void cut(const float (&v)[8], bf16x8
     }
 }
 
-// N neighbours (8 or 16) of which the first n are there; the others are 0.
+// v's bytes from `bytes` (0 .. 16, even) on, zeros behind them.
+__device__ __forceinline__ uint4 shift_down(uint4 v, int32_t bytes)
+{
+    if (bytes & 16) v = make_uint4(0, 0, 0, 0);
+    if (bytes & 8) v = make_uint4(v.z, v.w, 0, 0);
+    if (bytes & 4) v = make_uint4(v.y, v.z, v.w, 0);
+    const uint32_t s = (bytes & 2) * 8;
+    return make_uint4(__builtin_amdgcn_alignbit(v.y, v.x, s), __builtin_amdgcn_alignbit(v.z, v.y, s), __builtin_amdgcn_alignbit(v.w, v.z, s), v.w >> s);
+}
+
+// 16 bytes of an array that ends at element `end` (and has 16 bytes at least): zeros behind its end.
+template <int DT> __device__ __forceinline__ uint4 load_end(const void* p, int64_t at, int64_t end)
+{
+    constexpr int E = Vec<DT>::N;
+    const int64_t in = min(at, end - E);
+    return shift_down(load_any(static_cast<const char*>(p) + in * Vec<DT>::BYTES), static_cast<int32_t>(min(at - in, static_cast<int64_t>(E))) * Vec<DT>::BYTES);
+}
+
+// The first n elements of v; the others become 0.
+template <int DT> __device__ __forceinline__ uint4 keep(const uint4& v, int32_t n)
+{
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if constexpr (DT == SLHIP_F32) w[j] = n > j ? w[j] : 0;
+        else w[j] = n > 2 * j + 1 ? w[j] : n > 2 * j ? w[j] & 0xFFFF : 0;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// N neighbours (8 or 16).
 template <int DT, int N> struct Run {
     static constexpr int kVecs = N * Vec<DT>::BYTES / 16, kPer = Vec<DT>::N;
     uint4 w[kVecs];
-    __device__ __forceinline__ void load(const void* p, int64_t at)
+    __device__ __forceinline__ void load(const char* p)
     {
-        const char* c = static_cast<const char*>(p) + at * Vec<DT>::BYTES;
 #pragma unroll
-        for (int i = 0; i < kVecs; i++) w[i] = load_any(c + 16 * i);
+        for (int i = 0; i < kVecs; i++) w[i] = load_any(p + 16 * i);
     }
-    __device__ __forceinline__ void load_some(const void* p, int64_t at, int64_t n)
+    // Of an array that ends at `end`.
+    __device__ __forceinline__ void load_end(const void* p, int64_t at, int64_t end)
     {
-        const char* c = static_cast<const char*>(p) + at * Vec<DT>::BYTES;
 #pragma unroll
-        for (int i = 0; i < kVecs; i++) {
-            w[i] = make_uint4(0, 0, 0, 0);
-            if (n >= (i + 1) * kPer) {
-                w[i] = load_any(c + 16 * i);
-            } else if (n > i * kPer) {
-                float f[kPer] = {};
-                for (int j = 0; j < kPer; j++)
-                    if (i * kPer + j < n) f[j] = Vec<DT>::load1(c, i * kPer + j);
-                w[i] = Vec<DT>::pack(f);  // the same bits again
-            }
-        }
+        for (int i = 0; i < kVecs; i++) w[i] = slhip::load_end<DT>(p, at + i * kPer, end);
+    }
+    __device__ __forceinline__ void keep(int32_t n)
+    {
+#pragma unroll
+        for (int i = 0; i < kVecs; i++) w[i] = slhip::keep<DT>(w[i], n - i * kPer);
     }
     // Eight of them as bf16 parts.
     template <int P> __device__ __forceinline__ void parts(int half, bf16x8 (&p)[P]) const
@@ -238,14 +333,16 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
     const int32_t units = (a.K + kUnit - 1) / kUnit, each = (units + a.splits - 1) / a.splits;
     const int32_t u0 = split * each, u1 = min(u0 + each, units);
     // rows and ranks that are not there: others, whose sums nothing takes
-    int64_t xp[MT], ap[RB];
+    const char* xp[MT];
+    uint32_t ap[RB];
+    const char* const ad = static_cast<const char*>(a.a) + key * a.sa * Vec<WT>::BYTES;
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         const int32_t row = s_rows[16 * m + c];
-        xp[m] = (row >= 0 ? row : s_rows[0]) * a.xs + 16 * g;
+        xp[m] = static_cast<const char*>(a.x) + ((row >= 0 ? row : s_rows[0]) * a.xs + 16 * g) * Vec<XT>::BYTES;
     }
 #pragma unroll
-    for (int q = 0; q < RB; q++) ap[q] = key * a.sa + static_cast<int64_t>(min(r0 + 16 * q + c, rank - 1)) * a.K + 16 * g;
+    for (int q = 0; q < RB; q++) ap[q] = static_cast<uint32_t>(min(r0 + 16 * q + c, rank - 1) * a.K + 16 * g) * Vec<WT>::BYTES;
     f32x4 acc[MT][RB];
 #pragma unroll
     for (int m = 0; m < MT; m++)
@@ -279,12 +376,12 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
         Run<WT, 16> w[U][RB];
 #pragma unroll
         for (int v = 0; v < U; v++) {
-            const int64_t k = static_cast<int64_t>(u + v * kWaves) * kUnit;
+            const uint32_t k = static_cast<uint32_t>(u + v * kWaves) * kUnit;
 #pragma unroll
             for (int q = 0; q < RB; q++)
-                if (q == 0 || q < ranks) w[v][q].load(a.a, ap[q] + k);
+                if (q == 0 || q < ranks) w[v][q].load(ad + (ap[q] + k * Vec<WT>::BYTES));
 #pragma unroll
-            for (int m = 0; m < MT; m++) x[v][m].load(a.x, xp[m] + k);
+            for (int m = 0; m < MT; m++) x[v][m].load(xp[m] + k * Vec<XT>::BYTES);
         }
 #pragma unroll
         for (int v = 0; v < U; v++) multiply(x[v], w[v]);
@@ -292,11 +389,18 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
     for (; u < u1; u += kWaves) {
         Run<XT, 16> x[MT];
         Run<WT, 16> w[RB];
-        const int64_t k = static_cast<int64_t>(u) * kUnit, n = a.K - k - 16 * g;
+        const int32_t k = u * kUnit + 16 * g, n = a.K - k;
 #pragma unroll
-        for (int q = 0; q < RB; q++) w[q].load_some(a.a, ap[q] + k, n);
+        for (int q = 0; q < RB; q++) {
+            w[q].load_end(ad, min(r0 + 16 * q + c, rank - 1) * a.K + k, a.R * a.K);
+            w[q].keep(n);
+        }
 #pragma unroll
-        for (int m = 0; m < MT; m++) x[m].load_some(a.x, xp[m] + k, n);
+        for (int m = 0; m < MT; m++) {
+            const int32_t row = s_rows[16 * m + c];
+            x[m].load_end(a.x, (row >= 0 ? row : s_rows[0]) * a.xs + k, (a.T - 1) * a.xs + a.K);
+            x[m].keep(n);
+        }
         multiply(x, w);
     }
     // the sums of waves 2 and 3 into 0 and 1, and 1 into 0
@@ -330,57 +434,29 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
 
 // ---- y = add + s B h -----------------------------------------------------------------------------------------------
 
-// Eight neighbours of a row of add or y, the first n of them.
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
-template <int DT> struct Eight {
-    static constexpr int kVecs = 8 * Vec<DT>::BYTES / 16, kPer = Vec<DT>::N;
-    u32x4 w[kVecs];
-    __device__ __forceinline__ void load(const void* p, int64_t at)
-    {
-        const char* c = static_cast<const char*>(p) + at * Vec<DT>::BYTES;
-#pragma unroll
-        for (int i = 0; i < kVecs; i++) w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(c + 16 * i));
-    }
-    __device__ __forceinline__ void load_some(const void* p, int64_t at, int32_t n)
-    {
-        const char* c = static_cast<const char*>(p) + at * Vec<DT>::BYTES;
-#pragma unroll
-        for (int i = 0; i < kVecs; i++) {
-            w[i] = u32x4{0, 0, 0, 0};
-            if (n >= 8) {
-                w[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(c + 16 * i));
-            } else if (n > i * kPer) {
-                float f[kPer] = {};
-                for (int j = 0; j < kPer; j++)
-                    if (i * kPer + j < n) f[j] = Vec<DT>::load1(c, i * kPer + j);
-                const uint4 v = Vec<DT>::pack(f);  // the same bits again
-                w[i] = u32x4{v.x, v.y, v.z, v.w};
-            }
-        }
-    }
-    __device__ __forceinline__ void floats(float (&f)[8]) const
-    {
-#pragma unroll
-        for (int i = 0; i < kVecs; i++) Vec<DT>::unpack(make_uint4(w[i].x, w[i].y, w[i].z, w[i].w), &f[i * kPer]);
-    }
-    __device__ static __forceinline__ void store(void* p, int64_t at, int32_t n, const float (&f)[8])
-    {
-        char* c = static_cast<char*>(p) + at * Vec<DT>::BYTES;
-        if (n >= 8) {
-#pragma unroll
-            for (int i = 0; i < kVecs; i++) {
-                const uint4 w = Vec<DT>::pack(&f[i * kPer]);
-                const u32x4 t = {w.x, w.y, w.z, w.w};
-                __builtin_nontemporal_store(t, reinterpret_cast<u32x4_any*>(c + 16 * i));
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j < n) Vec<DT>::store1(c, j, f[j]);
-        }
-    }
-};
+__device__ __forceinline__ void store_any(char* p, const uint4& v)
+{
+    const u32x4 t = {v.x, v.y, v.z, v.w};
+    __builtin_nontemporal_store(t, reinterpret_cast<u32x4_any*>(p));
+}
+
+// Two 16-byte pieces of each of 16 rows, by lanes c + 16 g: with both pieces of row c in lane c (a of columns before b's), or as memory
+// takes them best, eight lanes a line: a of row c % 8 and b of row 8 + c % 8, of the first piece in lanes c < 8, of the second above.
+// One goes over into the other by an exchange of lanes c and c +- 8.
+__device__ __forceinline__ void swap_halves(uint4& a, uint4& b)
+{
+    const auto one = [](uint32_t& x, uint32_t& y) {
+        const uint32_t t = __builtin_amdgcn_update_dpp(static_cast<int>(y), static_cast<int>(x), 0x128, 0xF, 0x3, false);  // row_ror:8 into c < 8
+        x = __builtin_amdgcn_update_dpp(static_cast<int>(x), static_cast<int>(y), 0x128, 0xF, 0xC, false);                 // and into c >= 8
+        y = t;
+    };
+    one(a.x, b.x);
+    one(a.y, b.y);
+    one(a.z, b.z);
+    one(a.w, b.w);
+}
 
 // The two bf16 parts of v, rounded: what is left of an infinity is 0.
 __device__ __forceinline__ float low_part(float v, float hi) { return fabsf(hi) < INFINITY ? v - hi : 0.0f; }
@@ -397,42 +473,71 @@ template <int YT, int WT, int MT> __global__ __launch_bounds__(kThreads) void lo
     if (key == kNoTile || (key < 0 && a.add == a.y)) return;
     const int32_t rank = key < 0 ? 0 : rank_of(a, key), tiles = (rank + 15) / 16;
     const float scale = key < 0 || !a.scale ? 1.0f : a.scale[key];
-    int32_t row[MT];
+    const char* const ad = static_cast<const char*>(a.b) + (key < 0 ? 0 : key * a.sb * Vec<WT>::BYTES);
+    // 64 columns of a row are kPieces of 16 bytes a lane. Product u has those of 16 columns of which a lane (c, g) gets four in a row,
+    // row c's: f32 4 g of the u-th 16, bf16 eight with those of u + 1 (u even), 8 g of the u-th 16.
+    constexpr int E = Vec<YT>::N, kPieces = 16 / E;
+    const auto column = [&](int32_t n0, int u) {
+        return min(n0 + (YT == SLHIP_F32 ? 16 * u + c : 32 * (u >> 1) + 8 * (c >> 2) + 4 * (u & 1) + (c & 3)), a.N - 1);  // behind the last: not stored
+    };
+    // Where a lane loads and stores (swap_halves): rows c % 8 and 8 + c % 8 of each 16, of pieces 2 p + c / 8.
+    const int32_t in = (c >> 3) * 4 * E + g * E;
+    const char* from[MT][2];
+    char* to[MT][2];
+    bool there[MT][2];
 #pragma unroll
-    for (int m = 0; m < MT; m++) row[m] = s_rows[16 * m + c];
-    const int64_t base = key < 0 ? 0 : key * a.sb;
-    // Columns of a product u: a lane gets four in a row, with u + 1 (u even) eight. Those behind the last are others, which are not stored.
-    const auto column = [&](int32_t n0, int u) { return min(n0 + 32 * (u >> 1) + 8 * (c >> 2) + 4 * (u & 1) + (c & 3), a.N - 1); };
-    Eight<YT> add[MT][2];
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int32_t row = s_rows[16 * m + 8 * h + (c & 7)];
+            there[m][h] = row >= 0;
+            from[m][h] = static_cast<const char*>(a.add) + ((row >= 0 ? row : s_rows[0]) * a.as + in) * Vec<YT>::BYTES;
+            to[m][h] = static_cast<char*>(a.y) + ((row >= 0 ? row : 0) * a.ys + in) * Vec<YT>::BYTES;
+        }
+    uint4 add[MT][kPieces];
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int i = 0; i < kPieces; i++) add[m][i] = make_uint4(0, 0, 0, 0);
     Run<WT, 8> w[4];
-    const auto fetch_w = [&](int32_t n0, int q) __attribute__((always_inline)) {
-        const int32_t r = 16 * q + 8 * (g & 1);
-        if (16 * q + 16 <= rank) {
+    uint32_t wp[4];
 #pragma unroll
-            for (int u = 0; u < 4; u++) w[u].load(a.b, base + static_cast<int64_t>(column(n0, u)) * a.R + r);
-        } else {  // ranks behind the last are not read
+    for (int u = 0; u < 4; u++) wp[u] = static_cast<uint32_t>(column(0, u) * a.R + 8 * (g & 1)) * Vec<WT>::BYTES;
+    // whole: 64 columns, whose last 16 ranks end inside the adapter
+    const auto is_whole = [&](int32_t n0) { return n0 + 64 + a.spare <= a.N; };
+    const auto fetch_w = [&](int32_t n0, int q, bool whole) __attribute__((always_inline)) {
+        if (whole) {
+            const char* const at = ad + (static_cast<int64_t>(n0) * a.R + 16 * q) * Vec<WT>::BYTES;
 #pragma unroll
-            for (int u = 0; u < 4; u++) w[u].load_some(a.b, base + static_cast<int64_t>(column(n0, u)) * a.R + r, rank - r);
+            for (int u = 0; u < 4; u++) w[u].load(at + wp[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; u++) w[u].load_end(ad, column(n0, u) * a.R + 16 * q + 8 * (g & 1), a.N * a.R);
         }
     };
     const auto fetch = [&](int32_t n0) __attribute__((always_inline)) {
-        if (tiles > 0) fetch_w(n0, 0);
-        if (a.add && n0 + 64 <= a.N) {
+        const bool whole = is_whole(n0);
+        if (tiles > 0) fetch_w(n0, 0, whole);
+        if (!a.add) return;
+        if (whole) {
+            const int64_t at = static_cast<int64_t>(n0) * Vec<YT>::BYTES;
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int p = 0; p < 2; p++) add[m][p].load(a.add, (row[m] >= 0 ? row[m] : s_rows[0]) * a.as + n0 + 32 * p + 8 * g);
+                for (int i = 0; i < kPieces; i++) {
+                    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(from[m][i & 1] + at + (i >> 1) * 128));
+                    add[m][i] = make_uint4(v.x, v.y, v.z, v.w);
+                }
         } else {
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int p = 0; p < 2; p++) {
-                    const int32_t n = n0 + 32 * p + 8 * g;
-                    add[m][p].load_some(a.add, row[m] * a.as + n, a.add && row[m] >= 0 ? a.N - n : 0);
-                }
+                for (int i = 0; i < kPieces; i++)
+                    add[m][i] = load_end<YT>(a.add, (from[m][i & 1] - static_cast<const char*>(a.add)) / Vec<YT>::BYTES + n0 + (i >> 1) * 8 * E, (a.T - 1) * a.as + a.N);
         }
     };
-    const int32_t first = (cb * a.col_steps * kWaves + wave) * 64;
+    // thread blocks that run together take neighbouring columns: the same columns of many rows lie in few memory channels
+    const int32_t first = (cb * kWaves + wave) * 64, step = a.col_blocks * kWaves * 64;
     if (first < a.N) fetch(first);
     for (int t = tid; t < MT * tiles * 32; t += kThreads) {  // eight ranks of a row
         const int m = t / (tiles * 32), q = t / 32 - m * tiles, l = t & 31;
@@ -472,20 +577,19 @@ template <int YT, int WT, int MT> __global__ __launch_bounds__(kThreads) void lo
         }
     }
     __syncthreads();
-    for (int j = 0; j < a.col_steps; j++) {
-        const int32_t n0 = first + j * kWaves * 64;
-        if (n0 >= a.N) break;
-        if (j > 0) fetch(n0);
+    for (int32_t n0 = first; n0 < a.N; n0 += step) {
+        if (n0 > first) fetch(n0);
+        const bool whole = is_whole(n0);
         f32x4 acc[MT][4];
+        const auto multiply = [&](int q, auto begins) __attribute__((always_inline)) {
+            if (16 * q + 16 > rank) {  // ranks behind the last may hold anything
 #pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int u = 0; u < 4; u++) acc[m][u] = f32x4{0, 0, 0, 0};
-        for (int q = 0; q < tiles; q++) {
+                for (int u = 0; u < 4; u++) w[u].keep(rank - 16 * q - 8 * (g & 1));
+            }
             bf16x8 pw[4][PW];
 #pragma unroll
             for (int u = 0; u < 4; u++) w[u].parts(0, pw[u]);
-            if (q + 1 < tiles) fetch_w(n0, q + 1);
+            if (q + 1 < tiles) fetch_w(n0, q + 1, whole);
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -494,19 +598,49 @@ template <int YT, int WT, int MT> __global__ __launch_bounds__(kThreads) void lo
 #pragma unroll
                     for (int i = PW - 1; i >= 0; i--)
 #pragma unroll
-                        for (int u = 0; u < 4; u++) acc[m][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pw[u][i], x, acc[m][u], 0, 0, 0);
+                        for (int u = 0; u < 4; u++)
+                            acc[m][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pw[u][i], x, begins && h == H - 1 && i == PW - 1 ? f32x4{0, 0, 0, 0} : acc[m][u], 0, 0, 0);
                 }
+        };
+        if (tiles > 0) {
+            multiply(0, std::true_type{});
+            for (int q = 1; q < tiles; q++) multiply(q, std::false_type{});
+        } else {
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int u = 0; u < 4; u++) acc[m][u] = f32x4{0, 0, 0, 0};
         }
+        const int64_t at = static_cast<int64_t>(n0) * Vec<YT>::BYTES;
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
-            for (int p = 0; p < 2; p++) {
-                const int32_t n = n0 + 32 * p + 8 * g;
-                float f[8];
-                add[m][p].floats(f);
+            for (int p = 0; p < kPieces; p += 2) {
+                uint4 v[2] = {add[m][p], add[m][p + 1]};
+                swap_halves(v[0], v[1]);
 #pragma unroll
-                for (int e = 0; e < 8; e++) f[e] += acc[m][2 * p + (e >> 2)][e & 3];
-                if (row[m] >= 0 && n < a.N) Eight<YT>::store(a.y, row[m] * a.ys + n, a.N - n, f);
+                for (int i = 0; i < 2; i++) {
+                    float f[E];
+                    Vec<YT>::unpack(v[i], f);
+#pragma unroll
+                    for (int e = 0; e < E; e++) f[e] += acc[m][(p + i) * E / 4 + e / 4][e & 3];
+                    v[i] = Vec<YT>::pack(f);
+                }
+                swap_halves(v[0], v[1]);
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    char* const place = to[m][i] + at + p * 64;
+                    const int32_t n = a.N - (n0 + p * 4 * E + in);
+                    if (whole || n >= E) {
+                        if (there[m][i]) store_any(place, v[i]);
+                    } else if (there[m][i]) {  // the last ones of a row
+                        float f[E];
+                        Vec<YT>::unpack(v[i], f);
+#pragma unroll
+                        for (int e = 0; e < E; e++)
+                            if (e < n) Vec<YT>::store1(place, e, f[e]);
+                    }
+                }
             }
     }
 }
@@ -523,7 +657,8 @@ static int64_t work_of(int64_t T, int64_t R)
 
 template <int XT, int WT, int MT> static int shrink(const LoraArgs& a, int64_t blocks, hipStream_t st)
 {
-    const auto kernel = a.R16 <= 16 ? lora_shrink<XT, WT, MT, 1> : a.R16 <= 32 ? lora_shrink<XT, WT, MT, 2> : lora_shrink<XT, WT, MT, 4>;
+    constexpr int few = MT == 1 ? 1 : 2;
+    const auto kernel = a.R16 <= 16 ? lora_shrink<XT, WT, few, 1> : a.R16 <= 32 ? lora_shrink<XT, WT, few, 2> : lora_shrink<XT, WT, MT, 4>;
     kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
     return check_launch("lora_shrink");
 }
@@ -537,29 +672,32 @@ template <int YT, int WT, int MT> static int expand(const LoraArgs& a, int64_t b
     return check_launch("lora_expand");
 }
 
-template <int WT, int MT> static int launch(int dtype_x, int dtype_y, LoraArgs& a, hipStream_t st)
+template <int WT> static int launch(int dtype_x, int dtype_y, LoraArgs& a, hipStream_t st)
 {
-    const int64_t items = item_count(a.T, a.B, 16 * MT, 1);
+    const bool few = a.T <= 32 * static_cast<int64_t>(a.B);
+    const int first_tile = few ? 16 : a.R16 <= 32 ? 32 : 64, second_tile = few ? 16 : a.R16 <= 32 ? 32 : 64;
+    const int64_t first_items = item_count(a.T, a.B, first_tile, 1), items = item_count(a.T, a.B, second_tile, 1);
     a.rank_blocks = a.R16 <= 32 ? 1 : (a.R16 + 63) / 64;
-    // ranges of K: enough thread blocks for the machine, of 512 inputs at least
-    int64_t splits = 4096 / (items * a.rank_blocks), most = a.K / 512;
+    // ranges of K: enough thread blocks for the machine, of 256 inputs at least
+    int64_t splits = (few ? 4096 : 1024) / (first_items * a.rank_blocks), most = a.K / 256;
     if (splits > most) splits = most;
     if (splits > kMostSplits) splits = kMostSplits;
     if (splits > kSplitRows / a.T) splits = kSplitRows / a.T;
     a.splits = splits < 1 ? 1 : static_cast<int32_t>(splits);
     const int64_t cols = (a.N + 64 * kWaves - 1) / (64 * kWaves);
-    a.col_steps = items * cols > 4096 ? 4 : 1;
-    a.col_blocks = static_cast<int32_t>((cols + a.col_steps - 1) / a.col_steps);
-    const int64_t first = items * a.splits * a.rank_blocks, second = items * a.col_blocks;
+    int64_t steps = few && a.B > 64 ? 1 : (items * cols + 2047) / 2048;
+    if (steps > 8) steps = 8;
+    a.col_blocks = static_cast<int32_t>((cols + steps - 1) / steps);
+    const int64_t first = first_items * a.splits * a.rank_blocks, second = items * a.col_blocks;
     if (first > 0xFFFFFF || second > 0xFFFFFF) return fail(SLHIP_ERR_UNSUPPORTED, "lora: too many rows");
-    const int e = dtype_x == SLHIP_F32 ? shrink<SLHIP_F32, WT, MT>(a, first, st) : shrink<SLHIP_BF16, WT, MT>(a, first, st);
+    const bool f32 = dtype_x == SLHIP_F32;
+    const int e = few ? f32 ? shrink<SLHIP_F32, WT, 1>(a, first, st) : shrink<SLHIP_BF16, WT, 1>(a, first, st)
+                      : f32 ? shrink<SLHIP_F32, WT, 4>(a, first, st) : shrink<SLHIP_BF16, WT, 4>(a, first, st);
     if (e) return e;
-    return dtype_y == SLHIP_F32 ? expand<SLHIP_F32, WT, MT>(a, second, st) : expand<SLHIP_BF16, WT, MT>(a, second, st);
-}
-
-template <int WT> static int launch(int dtype_x, int dtype_y, LoraArgs& a, hipStream_t st)
-{
-    return a.T > 32 * static_cast<int64_t>(a.B) ? launch<WT, 4>(dtype_x, dtype_y, a, st) : launch<WT, 1>(dtype_x, dtype_y, a, st);
+    const bool out32 = dtype_y == SLHIP_F32;
+    if (second_tile == 16) return out32 ? expand<SLHIP_F32, WT, 1>(a, second, st) : expand<SLHIP_BF16, WT, 1>(a, second, st);
+    if (second_tile == 32) return out32 ? expand<SLHIP_F32, WT, 2>(a, second, st) : expand<SLHIP_BF16, WT, 2>(a, second, st);
+    return out32 ? expand<SLHIP_F32, WT, 4>(a, second, st) : expand<SLHIP_BF16, WT, 4>(a, second, st);
 }
 
 }  // namespace slhip
@@ -586,10 +724,12 @@ extern "C" SLHIP_API int slhip_lora(int dtype_x, int dtype_y, const void* x, int
         return fail(SLHIP_ERR_UNSUPPORTED, "lora: adapters of dtype %d not supported", set->dtype);
     if (set->adapters < 0 || set->max_rank < 1 || set->K < 1 || set->N < 1 || rows->requests < 0 || rows->tokens < 0)
         return fail(SLHIP_ERR_INVALID, "lora: bad size");
+    if (set->K < 8 || set->N < 8) return fail(SLHIP_ERR_UNSUPPORTED, "lora: less than 8 inputs or outputs");  // a 16-byte load of bf16
     if (set->max_rank > kMaxRank) return fail(SLHIP_ERR_UNSUPPORTED, "lora: more than %d ranks", kMaxRank);
     if (rows->requests > kMaxRequests) return fail(SLHIP_ERR_UNSUPPORTED, "lora: more than %d requests", kMaxRequests);
-    if (set->adapters > 0x7FFFFFFF || set->K > (1 << 24) || set->N > (1 << 24) || rows->tokens > 0x7FFFFFFFll - 65536)
-        return fail(SLHIP_ERR_UNSUPPORTED, "lora: too many adapters, inputs, outputs or rows");
+    const int64_t widest = (set->K > set->N ? set->K : set->N) * set->max_rank * (set->dtype == SLHIP_F32 ? 4 : 2);
+    if (set->adapters > 0x7FFFFFFF || widest > 0x7FFFFFFF || set->K > (1 << 24) || set->N > (1 << 24) || rows->tokens > 0x7FFFFFFFll - 65536)
+        return fail(SLHIP_ERR_UNSUPPORTED, "lora: too many adapters, inputs, outputs or rows (a matrix of an adapter has less than 2^31 bytes)");
     if (x_stride < set->K || y_stride < set->N || (add && add_stride < set->N))
         return fail(SLHIP_ERR_INVALID, "lora: a row stride is smaller than the row");
     if (set->a_stride < set->max_rank * set->K || set->b_stride < set->max_rank * set->N)
@@ -616,6 +756,7 @@ extern "C" SLHIP_API int slhip_lora(int dtype_x, int dtype_y, const void* x, int
     a.adapters = static_cast<int32_t>(set->adapters);
     a.R = static_cast<int32_t>(set->max_rank);
     a.R16 = static_cast<int32_t>(round16(set->max_rank));
+    a.spare = static_cast<int32_t>((a.R16 - 1) / a.R);
     a.K = static_cast<int32_t>(set->K);
     a.N = static_cast<int32_t>(set->N);
     a.rank = set->rank;

@@ -113,7 +113,7 @@ TYPES = [("bf16", "bf16", "bf16"), ("f32", "bf16", "f32"), ("f32", "f32", "f32")
 
 @pytest.mark.parametrize("x,w,y", TYPES)
 @pytest.mark.parametrize("new,rank,K,N", [
-    ([1], 16, 512, 256), ([1], 1, 1, 1), ([5], 8, 64, 64), ([17], 16, 100, 70), ([70], 24, 257, 131), ([200], 64, 320, 300), ([40], 100, 130, 65),
+    ([1], 16, 512, 256), ([1], 1, 8, 8), ([2], 3, 9, 11), ([5], 8, 64, 64), ([17], 16, 100, 70), ([70], 24, 257, 131), ([200], 64, 320, 300), ([40], 100, 130, 65),
     ([64], 256, 192, 257)])
 def test_one_request(device, new, rank, K, N, x, w, y):
     with Dev() as d:

@@ -59,7 +59,8 @@ def _rows(**kw):
     (dict(dtype=7), {}, {}, NotImplementedError, "dtype"), ({}, {}, dict(dtype_x="f16"), NotImplementedError, "dtypes"),
     ({}, {}, dict(dtype_y="f16"), NotImplementedError, "dtypes"), (dict(max_rank=257), {}, {}, NotImplementedError, "256 ranks"),
     (dict(max_rank=0), {}, {}, ValueError, "bad size"), (dict(K=0), {}, {}, ValueError, "bad size"), (dict(N=0), {}, {}, ValueError, "bad size"),
-    (dict(adapters=-1), {}, {}, ValueError, "bad size"), (dict(K=1 << 25), {}, {}, NotImplementedError, "too many"),
+    (dict(adapters=-1), {}, {}, ValueError, "bad size"), (dict(K=7), {}, {}, NotImplementedError, "less than 8"),
+    (dict(N=7), {}, {}, NotImplementedError, "less than 8"), (dict(N=1 << 24, max_rank=64), {}, {}, NotImplementedError, "2\\^31 bytes"), (dict(K=1 << 25), {}, {}, NotImplementedError, "too many"),
     ({}, dict(requests=4097), {}, NotImplementedError, "4096 requests"), ({}, dict(requests=-1), {}, ValueError, "bad size"),
     ({}, dict(tokens=1 << 31), {}, NotImplementedError, "too many"), ({}, dict(starts=None), {}, ValueError, "starts"),
     ({}, dict(adapter=None), {}, ValueError, "adapter"), ({}, {}, dict(x=None), ValueError, "x, y"), ({}, {}, dict(y=None), ValueError, "x, y"),
