@@ -631,7 +631,8 @@ SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64_t target_s
  * that does not fit the rows is left as it was and reported (SLHIP_ERR_CACHE).
  * work: workspace of work_bytes >= slhip_lora_work_bytes(tokens, max_rank) (enough for fewer tokens and ranks too), 16-byte
  * aligned; calls that may overlap each need their own. It needs no initialisation and keeps nothing.
- * max_rank <= 256, K and N 8 .. 2^24, a matrix of an adapter less than 2^31 bytes, requests <= 4096. Any alignment; rows and adapters of 16-byte steps are fastest.
+ * max_rank <= 256, K and N 8 .. 2^24, a matrix of an adapter less than 2^31 bytes, strides of add and y
+ * below 2^30, requests <= 4096. Any alignment; rows and adapters of 16-byte steps are fastest.
  */
 typedef struct slhip_lora_set {
     int32_t dtype; /* of a and b: F32, F16 or BF16 */

@@ -6,8 +6,9 @@
 //
 // Layout. Rows that share an adapter are taken together whatever requests they are of: the rows of an adapter, in the requests'
 // order, are one list, which is cut into tiles of TM rows. Request i works on the tiles that begin in its part of the list
-// (no more than its rows alone would make), so a launch is sized from rows and requests (item_base), and a thread block finds its
-// rows by one look at all requests.
+// (no more than its rows alone would make), so a launch is sized from rows and requests (item_base). Up to 64
+// requests a wave looks at all of them at once, a lane each, and every thread block finds its rows so; of more, a launch before (lora_plan)
+// lists the tiles, and the others share out what there is: 256 requests that share 8 adapters are 17 tiles, of 272 that there might be.
 // With mfma 16x16x32 (A[m][8g+j], B[8g+j][n], C[4g+r][n] in lane (n or m) + 16 g) adapters are the first operand and rows the
 // second one, so that a lane's sums are four neighbours of one row: h is stored and y made without an exchange.
 //
@@ -32,6 +33,10 @@ constexpr int kUnit = 64;          // inputs that a wave takes together: a line 
 constexpr int kMostSplits = 16;
 constexpr int64_t kSplitRows = 65536;  // rows times ranges are at most so many, or the rows
 
+struct Plan {
+    int32_t tiles, splits, col_blocks, reserved;
+};
+
 struct LoraArgs {
     const void *x, *add;
     void* y;
@@ -45,8 +50,11 @@ struct LoraArgs {
     int64_t T;
     const int32_t *starts, *adapter;
     float* h;  // [splits][T][R16]
-    int32_t splits, rank_blocks, col_blocks;
-    int32_t spare;  // columns that the last 16 ranks of one may reach into
+    int32_t splits, rank_blocks, col_blocks;  // ranges of K, of the ranks; thread blocks that share a tile's columns
+    int32_t cols;                             // that there could be
+    Plan* plan;                               // of more than 64 requests
+    int32_t *plan_key, *plan_rows;            // [tiles], [tiles][TM]
+    int32_t spare;  // columns that the load of a column's last ranks may reach into
     uint32_t* err;
 };
 
@@ -67,21 +75,7 @@ __device__ __forceinline__ int32_t rows_of(const LoraArgs& a, int32_t i)
     return s0 >= 0 && s1 >= s0 && s1 <= a.T ? s1 - s0 : 0;
 }
 
-__device__ __forceinline__ int32_t block_scan(int32_t v, int32_t* lds, int32_t& total)
-{
-    v = wave_scan(v);
-    if ((threadIdx.x & 63) == 63) lds[wave_id()] = v;
-    __syncthreads();
-    total = 0;
-    for (int w = 0; w < kWaves; w++) {
-        if (w == wave_id()) v += total;
-        total += lds[w];
-    }
-    __syncthreads();
-    return v;
-}
-
-// The same for up to 64 requests, a lane each: one memory latency, and nothing but the rows goes through LDS.
+// A tile of up to 64 requests, a lane each: one memory latency, and nothing but the rows goes through LDS.
 template <int TM> __device__ __forceinline__ int32_t find_tile_64(const LoraArgs& a, int64_t item, int32_t* s_rows)
 {
     const int lane = threadIdx.x & 63, j = min(lane, a.B - 1);
@@ -104,115 +98,96 @@ template <int TM> __device__ __forceinline__ int32_t find_tile_64(const LoraArgs
     return key;
 }
 
-// The same for up to kHeld * 256 requests: a thread holds kHeld of them, so there is one memory latency.
-constexpr int kHeld = 4;
+// Lists the tiles of more than 64 requests, by one thread block: the rows of each adapter in a hash table of adapters, in any
+// order (no row's result depends on the others of its tile), then the adapters' first tiles by a sum over the table.
+constexpr int kPlanThreads = 1024, kSlots = 2 * kMaxRequests, kEach = kMaxRequests / kPlanThreads;
+constexpr int32_t kEmpty = -0x7FFFFFFF;
+constexpr int kPlanLds = (2 * kSlots + kPlanThreads / 64) * 4;
 
-template <int TM> __device__ __forceinline__ int32_t find_tile_held(const LoraArgs& a, int64_t item, int32_t* s_rows)
+template <int TM> __global__ __launch_bounds__(kPlanThreads) void lora_plan(LoraArgs a, int32_t blocks1, int32_t blocks2)
 {
-    __shared__ int32_t s_at[kWaves], s_one[3], s_before[kWaves], s_sum[kHeld][kWaves];
+    extern __shared__ int32_t s_slots[];
+    int32_t *s_key = s_slots, *s_count = s_slots + kSlots, *s_wave = s_slots + 2 * kSlots;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
-    int32_t s0[kHeld], n[kHeld], key[kHeld], begun = 0;
-#pragma unroll
-    for (int e = 0; e < kHeld; e++) {
-        const int32_t j = tid + e * kThreads, at = min(j, a.B - 1);
-        s0[e] = a.starts[at];
-        n[e] = j < a.B ? rows_of(a, at) : 0;
-        key[e] = adapter_of(a, at);
+    int slots = 256;
+    while (slots < 2 * a.B) slots *= 2;  // a power of two, at most kSlots
+    for (int i = tid; i < slots; i += kPlanThreads) {
+        s_key[i] = kEmpty;
+        s_count[i] = 0;
     }
-#pragma unroll
-    for (int e = 0; e < kHeld; e++) {
-        const int32_t j = tid + e * kThreads;
-        begun += __popcll(__ballot(j < a.B && item_base(s0[e], j, TM, 1) <= item));
-    }
-    if (lane == 0) s_at[wave] = begun;
-    if (tid < TM) s_rows[tid] = -1;
+    __shared__ unsigned long long s_all;
+    if (tid == 0) s_all = 0;
     __syncthreads();
-    const int32_t i = max((s_at[0] + s_at[1]) + (s_at[2] + s_at[3]) - 1, 0);
+    int32_t s0[kEach], n[kEach], slot[kEach], at[kEach];
+    unsigned long long rows_mine = 0;
 #pragma unroll
-    for (int e = 0; e < kHeld; e++)
-        if (tid + e * kThreads == i) {
-            s_one[0] = s0[e];
-            s_one[1] = n[e];
-            s_one[2] = key[e];
+    for (int e = 0; e < kEach; e++) {
+        const int32_t j = tid + e * kPlanThreads;
+        const bool in = j < a.B;
+        s0[e] = in ? a.starts[j] : 0;
+        n[e] = in ? rows_of(a, j) : 0;
+        rows_mine += n[e];
+        const int32_t key = in ? adapter_of(a, j) : -1;
+        if (n[e] == 0) continue;
+        int32_t h = static_cast<uint32_t>(key) * 2654435761u >> 16 & (slots - 1);
+        for (;;) {  // there are fewer keys than slots
+            const int32_t was = atomicCAS(&s_key[h], kEmpty, key);
+            if (was == kEmpty || was == key) break;
+            h = (h + 1) & (slots - 1);
         }
-    __syncthreads();
-    const int32_t at = s_one[0], rows = s_one[1], mine = s_one[2];
-    const int64_t piece = item - item_base(at, i, TM, 1);
-    if (piece < 0 || piece * TM >= rows) return kNoTile;
-    int32_t up[kHeld], before = 0;
-#pragma unroll
-    for (int e = 0; e < kHeld; e++) {
-        if (key[e] != mine) n[e] = 0;
-        up[e] = wave_scan(n[e]);
-        if (lane == 63) s_sum[e][wave] = up[e];
-        up[e] -= n[e];
-        before += tid + e * kThreads < i ? n[e] : 0;
+        slot[e] = h;
+        at[e] = atomicAdd(&s_count[h], n[e]);
     }
-    before = wave_scan(before);
-    if (lane == 63) s_before[wave] = before;
+    if (rows_mine > 0) atomicAdd(&s_all, rows_mine);
     __syncthreads();
-    before = (s_before[0] + s_before[1]) + (s_before[2] + s_before[3]);
-    const int64_t first = ((static_cast<int64_t>(before) + TM - 1) / TM + piece) * TM, off = first - before;
-    if (off < 0 || off >= rows) return kNoTile;  // (below 0 where requests overlap, which none may)
-    if (tid < min(static_cast<int64_t>(TM), rows - off)) s_rows[tid] = at + static_cast<int32_t>(off) + tid;
-    int64_t base = -first;  // of the wave's requests
-#pragma unroll
-    for (int e = 0; e < kHeld; e++) {
-        int64_t to = base + up[e];
-        for (int w = 0; w < kWaves; w++) {
-            to += w < wave ? s_sum[e][w] : 0;
-            base += s_sum[e][w];
-        }
-        if (tid + e * kThreads > i && to >= 1) {
-            for (int32_t r = 0; r < n[e] && to + r < TM; r++) s_rows[to + r] = s0[e] + r;
-        }
+    if (s_all > static_cast<unsigned long long>(a.T)) {  // requests overlap, so starts falls, which is reported: there is no list for that
+        if (tid == 0) *a.plan = Plan{0, 1, 1, 0};
+        return;
+    }
+    const int each = slots <= kPlanThreads ? 1 : slots / kPlanThreads;
+    int32_t mine = 0;
+    for (int i = tid * each; i < min((tid + 1) * each, slots); i++) mine += (s_count[i] + TM - 1) / TM;
+    int32_t up = wave_scan(mine);
+    if (lane == 63) s_wave[wave] = up;
+    up -= mine;
+    __syncthreads();
+    int32_t tiles = 0;
+    for (int w = 0; w < kPlanThreads / 64; w++) {
+        if (w == wave) up += tiles;
+        tiles += s_wave[w];
+    }
+    for (int i = tid * each; i < min((tid + 1) * each, slots); i++) {
+        const int32_t rows = s_count[i], some = (rows + TM - 1) / TM;
+        for (int32_t t = 0; t < some; t++) a.plan_key[up + t] = s_key[i];
+        for (int32_t r = rows; r < some * TM; r++) a.plan_rows[up * TM + r] = -1;
+        s_count[i] = up;
+        up += some;
     }
     __syncthreads();
-    return mine;
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        const int32_t to = n[e] > 0 ? s_count[slot[e]] * TM + at[e] : 0;
+        if (n[e] <= 4) {
+            for (int32_t r = 0; r < n[e]; r++) a.plan_rows[to + r] = s0[e] + r;
+        }
+        for (uint64_t many = __ballot(n[e] > 4); many; many &= many - 1) {  // by the whole wave
+            const int k = __ffsll(static_cast<long long>(many)) - 1;
+            const int32_t rows = __builtin_amdgcn_readlane(n[e], k), p = __builtin_amdgcn_readlane(to, k), s = __builtin_amdgcn_readlane(s0[e], k);
+            for (int32_t r = lane; r < rows; r += 64) a.plan_rows[p + r] = s + r;
+        }
+    }
+    if (tid == 0) {  // the tiles share out the thread blocks that there are
+        const int32_t some = max(tiles, 1);
+        *a.plan = Plan{tiles, max(min(a.splits, blocks1 / (some * a.rank_blocks)), 1), max(min(a.cols, blocks2 / some), 1), 0};
+    }
 }
 
 // The rows of tile `item` into s_rows (-1 behind the last), and their adapter; kNoTile where there is none.
-template <int TM> __device__ __forceinline__ int32_t find_tile(const LoraArgs& a, int64_t item, int32_t* s_rows, int32_t* lds)
+template <int TM> __device__ __forceinline__ int32_t find_tile(const LoraArgs& a, int64_t item, int32_t* s_rows)
 {
-    const int lane = threadIdx.x & 63, tid = threadIdx.x;
-    if (a.B <= 64) return find_tile_64<TM>(a, item, s_rows);
-    if (a.B <= kHeld * kThreads) return find_tile_held<TM>(a, item, s_rows);
-    int32_t i = 0;
-    {   // as row_request, by the requests' first items
-        int32_t lo = 0, n = a.B;
-        while (n > 64) {
-            const int32_t step = (n + 63) / 64, j = lo + lane * step;
-            const int32_t k = __popcll(__ballot(j < lo + n && item_base(a.starts[j < lo + n ? j : lo], j, TM, 1) <= item));
-            if (k > 0) {
-                lo += (k - 1) * step;
-                n -= (k - 1) * step;
-            }
-            n = min(n, step);
-        }
-        const int32_t j = lo + (lane < n ? lane : 0);
-        const int32_t k = __popcll(__ballot(lane < n && item_base(a.starts[j], j, TM, 1) <= item));
-        i = __builtin_amdgcn_readfirstlane(lo + max(k - 1, 0));
-    }
-    const int32_t s0 = a.starts[i], n = rows_of(a, i), key = adapter_of(a, i);
-    const int64_t piece = item - item_base(s0, i, TM, 1);
-    if (piece < 0 || piece * TM >= n) return kNoTile;
-    int32_t before = 0;
-    for (int32_t j = tid; j < i; j += kThreads)
-        if (adapter_of(a, j) == key) before += rows_of(a, j);
-    block_scan(before, lds, before);
-    const int64_t off = ((static_cast<int64_t>(before) + TM - 1) / TM + piece) * TM - before;
-    if (off < 0 || off >= n) return kNoTile;  // (below 0 where requests overlap, which none may)
-    int32_t have = static_cast<int32_t>(min(static_cast<int64_t>(TM), n - off));
-    if (tid < have) s_rows[tid] = s0 + static_cast<int32_t>(off) + tid;
-    for (int32_t w = i + 1; have < TM && w < a.B; w += kThreads) {
-        const int32_t j = w + tid;
-        const int32_t count = j < a.B && adapter_of(a, j) == key ? min(rows_of(a, j), TM) : 0;
-        int32_t total;
-        const int32_t at = have + block_scan(count, lds, total) - count;
-        for (int32_t r = 0; r < count && at + r < TM; r++) s_rows[at + r] = a.starts[j] + r;
-        have = min(have + total, TM);
-    }
-    if (tid >= have && tid < TM) s_rows[tid] = -1;
+    if (!a.plan) return find_tile_64<TM>(a, item, s_rows);
+    const int32_t key = a.plan_key[item];
+    if (threadIdx.x < TM) s_rows[threadIdx.x] = a.plan_rows[item * TM + threadIdx.x];
     __syncthreads();
     return key;
 }
@@ -313,7 +288,7 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
 {
     constexpr int TM = 16 * MT, PX = kParts<XT>, PW = kParts<WT>;
     constexpr int U = MT * RB == 1 ? 4 : MT == 1 || XT == SLHIP_BF16 ? 2 : 1;  // units whose loads are on their way together
-    __shared__ int32_t s_rows[TM], lds[kWaves];
+    __shared__ int32_t s_rows[TM];
     __shared__ f32x4 s_acc[kWaves / 2][MT * RB][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), c = lane & 15, g = lane >> 4;
     if (blockIdx.x == 0) {
@@ -325,12 +300,14 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
                 raise_error(a.err, kErrAdapter, static_cast<uint32_t>(i), static_cast<uint32_t>(a.adapter[i]), static_cast<uint32_t>(a.adapters), 0, 0, 0);
         }
     }
-    const int32_t rb = blockIdx.x % a.rank_blocks, rest = blockIdx.x / a.rank_blocks, split = rest % a.splits;
-    const int32_t key = find_tile<TM>(a, rest / a.splits, s_rows, lds);
+    const int32_t splits = a.plan ? a.plan->splits : a.splits, work = a.plan ? a.plan->tiles * splits * a.rank_blocks : gridDim.x;
+    const auto piece = [&](int32_t item) __attribute__((always_inline)) {
+    const int32_t rb = item % a.rank_blocks, rest = item / a.rank_blocks, split = rest % splits;
+    const int32_t key = find_tile<TM>(a, rest / splits, s_rows);
     if (key < 0) return;
     const int32_t rank = rank_of(a, key), r0 = rb * RB * 16;
     if (r0 >= rank) return;
-    const int32_t units = (a.K + kUnit - 1) / kUnit, each = (units + a.splits - 1) / a.splits;
+    const int32_t units = (a.K + kUnit - 1) / kUnit, each = (units + splits - 1) / splits;
     const int32_t u0 = split * each, u1 = min(u0 + each, units);
     // rows and ranks that are not there: others, whose sums nothing takes
     const char* xp[MT];
@@ -430,6 +407,11 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
         for (int q = 0; q < RB; q++)
             if (r0 + 16 * q < rank) *reinterpret_cast<f32x4*>(h + 16 * q) = acc[m][q];
     }
+    };
+    for (int32_t item = blockIdx.x; item < work; item += gridDim.x) {
+        piece(item);
+        if (item + gridDim.x < work) __syncthreads();  // the next piece's rows
+    }
 }
 
 // ---- y = add + s B h -----------------------------------------------------------------------------------------------
@@ -442,164 +424,98 @@ __device__ __forceinline__ void store_any(char* p, const uint4& v)
     __builtin_nontemporal_store(t, reinterpret_cast<u32x4_any*>(p));
 }
 
-// Two 16-byte pieces of each of 16 rows, by lanes c + 16 g: with both pieces of row c in lane c (a of columns before b's), or as memory
-// takes them best, eight lanes a line: a of row c % 8 and b of row 8 + c % 8, of the first piece in lanes c < 8, of the second above.
-// One goes over into the other by an exchange of lanes c and c +- 8.
-__device__ __forceinline__ void swap_halves(uint4& a, uint4& b)
-{
-    const auto one = [](uint32_t& x, uint32_t& y) {
-        const uint32_t t = __builtin_amdgcn_update_dpp(static_cast<int>(y), static_cast<int>(x), 0x128, 0xF, 0x3, false);  // row_ror:8 into c < 8
-        x = __builtin_amdgcn_update_dpp(static_cast<int>(x), static_cast<int>(y), 0x128, 0xF, 0xC, false);                 // and into c >= 8
-        y = t;
-    };
-    one(a.x, b.x);
-    one(a.y, b.y);
-    one(a.z, b.z);
-    one(a.w, b.w);
-}
-
 // The two bf16 parts of v, rounded: what is left of an infinity is 0.
 __device__ __forceinline__ float low_part(float v, float hi) { return fabsf(hi) < INFINITY ? v - hi : 0.0f; }
 
-template <int YT, int WT, int MT> __global__ __launch_bounds__(kThreads) void lora_expand(LoraArgs a)
+// Rows are the first operand here and columns the second. A wave has 16 E columns of its rows, E = 16 bytes of y: product u the
+// columns E c + u, so that a lane's sums of E products are 16 bytes of a row, 16 lanes 256 of it. Row 4 r + g of 16 stands in the operand's
+// place 4 g + r: lane (c, g) has it in element r, and of up to four rows (a decode step's, most often one) all lie in element 0.
+template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThreads) void lora_expand(LoraArgs a)
 {
-    constexpr int TM = 16 * MT, PW = kParts<WT>;
-    constexpr int H = YT == SLHIP_BF16 ? 1 : 2;  // instructions that take h's parts of 16 ranks
-    __shared__ int32_t s_rows[TM], lds[kWaves];
-    extern __shared__ uint4 s_h[];  // [MT][ranks / 16][H][64]: the second operand of 16 ranks
+    constexpr int TM = 16 * MT, PW = kParts<WT>, E = Vec<YT>::N, kColumns = 16 * E;
+    // h's parts of RC ranks are the first operands of H instructions: up to 16 ranks two parts share one, more have one each
+    constexpr int P = YT == SLHIP_BF16 ? 2 : 3, H = WIDE ? P : P - 1, RC = WIDE ? 32 : 16;
+    __shared__ int32_t s_rows[TM];
+    extern __shared__ uint4 s_h[];  // [MT][all][H][64]
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), c = lane & 15, g = lane >> 4;
-    const int32_t cb = blockIdx.x % a.col_blocks;
-    const int32_t key = find_tile<TM>(a, blockIdx.x / a.col_blocks, s_rows, lds);
+    const int32_t col_blocks = a.plan ? a.plan->col_blocks : a.col_blocks, work = a.plan ? a.plan->tiles * col_blocks : gridDim.x;
+    const auto piece = [&](int32_t item) __attribute__((always_inline)) {
+    const int32_t cb = item % col_blocks;
+    const int32_t key = find_tile<TM>(a, item / col_blocks, s_rows);
     if (key == kNoTile || (key < 0 && a.add == a.y)) return;
-    const int32_t rank = key < 0 ? 0 : rank_of(a, key), tiles = (rank + 15) / 16;
-    const float scale = key < 0 || !a.scale ? 1.0f : a.scale[key];
     const char* const ad = static_cast<const char*>(a.b) + (key < 0 ? 0 : key * a.sb * Vec<WT>::BYTES);
-    // 64 columns of a row are kPieces of 16 bytes a lane. Product u has those of 16 columns of which a lane (c, g) gets four in a row,
-    // row c's: f32 4 g of the u-th 16, bf16 eight with those of u + 1 (u even), 8 g of the u-th 16.
-    constexpr int E = Vec<YT>::N, kPieces = 16 / E;
-    const auto column = [&](int32_t n0, int u) {
-        return min(n0 + (YT == SLHIP_F32 ? 16 * u + c : 32 * (u >> 1) + 8 * (c >> 2) + 4 * (u & 1) + (c & 3)), a.N - 1);  // behind the last: not stored
-    };
-    // Where a lane loads and stores (swap_halves): rows c % 8 and 8 + c % 8 of each 16, of pieces 2 p + c / 8.
-    const int32_t in = (c >> 3) * 4 * E + g * E;
-    const char* from[MT][2];
-    char* to[MT][2];
-    bool there[MT][2];
+    const char* const from = static_cast<const char*>(a.add) + E * c * Vec<YT>::BYTES;
+    char* const to = static_cast<char*>(a.y) + E * c * Vec<YT>::BYTES;
+    const uint32_t as = static_cast<uint32_t>(a.as * Vec<YT>::BYTES), ys = static_cast<uint32_t>(a.ys * Vec<YT>::BYTES);
+    uint32_t row[MT][4];
+    bool there[MT][4];
+    int most = 0;  // rows' elements that hold one
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int32_t row = s_rows[16 * m + 8 * h + (c & 7)];
-            there[m][h] = row >= 0;
-            from[m][h] = static_cast<const char*>(a.add) + ((row >= 0 ? row : s_rows[0]) * a.as + in) * Vec<YT>::BYTES;
-            to[m][h] = static_cast<char*>(a.y) + ((row >= 0 ? row : 0) * a.ys + in) * Vec<YT>::BYTES;
+        for (int r = 0; r < 4; r++) {
+            const int32_t v = s_rows[16 * m + 4 * r + g];
+            there[m][r] = v >= 0;
+            row[m][r] = v >= 0 ? v : s_rows[0];
+            if (__any(v >= 0)) most = 4 * m + r + 1;
         }
-    uint4 add[MT][kPieces];
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int i = 0; i < kPieces; i++) add[m][i] = make_uint4(0, 0, 0, 0);
-    Run<WT, 8> w[4];
-    uint32_t wp[4];
-#pragma unroll
-    for (int u = 0; u < 4; u++) wp[u] = static_cast<uint32_t>(column(0, u) * a.R + 8 * (g & 1)) * Vec<WT>::BYTES;
-    // whole: 64 columns, whose last 16 ranks end inside the adapter
-    const auto is_whole = [&](int32_t n0) { return n0 + 64 + a.spare <= a.N; };
+    uint4 add[MT][4];
+    Run<WT, 8> w[E];
+    const int rl = 8 * (WIDE ? g : g & 1);  // the lane's ranks of RC
+    const uint32_t wp = static_cast<uint32_t>(E * c * a.R + rl) * Vec<WT>::BYTES;
+    // whole: all columns, whose last ranks' loads end inside the adapter
+    const auto is_whole = [&](int32_t n0) { return n0 + kColumns + a.spare <= a.N; };
     const auto fetch_w = [&](int32_t n0, int q, bool whole) __attribute__((always_inline)) {
         if (whole) {
-            const char* const at = ad + (static_cast<int64_t>(n0) * a.R + 16 * q) * Vec<WT>::BYTES;
+            const char* const at = ad + (static_cast<int64_t>(n0) * a.R + RC * q) * Vec<WT>::BYTES;
 #pragma unroll
-            for (int u = 0; u < 4; u++) w[u].load(at + wp[u]);
+            for (int u = 0; u < E; u++) w[u].load(at + (wp + static_cast<uint32_t>(u * a.R) * Vec<WT>::BYTES));
         } else {
 #pragma unroll
-            for (int u = 0; u < 4; u++) w[u].load_end(ad, column(n0, u) * a.R + 16 * q + 8 * (g & 1), a.N * a.R);
+            for (int u = 0; u < E; u++) w[u].load_end(ad, min(n0 + E * c + u, a.N - 1) * a.R + RC * q + rl, a.N * a.R);
         }
     };
-    const auto fetch = [&](int32_t n0) __attribute__((always_inline)) {
-        const bool whole = is_whole(n0);
-        if (tiles > 0) fetch_w(n0, 0, whole);
-        if (!a.add) return;
-        if (whole) {
-            const int64_t at = static_cast<int64_t>(n0) * Vec<YT>::BYTES;
+    const auto fetch = [&](int32_t n0, bool whole) __attribute__((always_inline)) {
+        if (key >= 0) fetch_w(n0, 0, whole);
+        const int64_t at = static_cast<int64_t>(n0) * Vec<YT>::BYTES;
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+        for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int i = 0; i < kPieces; i++) {
-                    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(from[m][i & 1] + at + (i >> 1) * 128));
-                    add[m][i] = make_uint4(v.x, v.y, v.z, v.w);
+            for (int r = 0; r < 4; r++) {
+                if (m + r > 0 && 4 * m + r >= most) break;
+                const char* const p = from + at + static_cast<uint64_t>(row[m][r]) * as;
+                if (!a.add) {
+                    add[m][r] = make_uint4(0, 0, 0, 0);
+                } else if (whole) {
+                    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+                    add[m][r] = make_uint4(v.x, v.y, v.z, v.w);
+                } else {
+                    add[m][r] = load_end<YT>(a.add, (p - static_cast<const char*>(a.add)) / Vec<YT>::BYTES, (a.T - 1) * a.as + a.N);
                 }
-        } else {
-#pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-                for (int i = 0; i < kPieces; i++)
-                    add[m][i] = load_end<YT>(a.add, (from[m][i & 1] - static_cast<const char*>(a.add)) / Vec<YT>::BYTES + n0 + (i >> 1) * 8 * E, (a.T - 1) * a.as + a.N);
-        }
+            }
     };
-    // thread blocks that run together take neighbouring columns: the same columns of many rows lie in few memory channels
-    const int32_t first = (cb * kWaves + wave) * 64, step = a.col_blocks * kWaves * 64;
-    if (first < a.N) fetch(first);
-    for (int t = tid; t < MT * tiles * 32; t += kThreads) {  // eight ranks of a row
-        const int m = t / (tiles * 32), q = t / 32 - m * tiles, l = t & 31;
-        const int32_t at = s_rows[16 * m + (l & 15)], r = 16 * q + 8 * (l >> 4);
-        float f[8] = {};
-        if (at >= 0) {
-            const float* h = a.h + static_cast<int64_t>(at) * a.R16 + r;
-            const int64_t step = a.T * a.R16;
-            for (int s0 = 0; s0 < a.splits; s0 += 8) {
-                f32x4 x[8][2];
-#pragma unroll
-                for (int s = 0; s < 8; s++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) x[s][e] = s0 + s < a.splits ? reinterpret_cast<const f32x4*>(h + (s0 + s) * step)[e] : f32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int s = 0; s < 8; s++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) f[e] += x[s][e >> 2][e & 3];
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) f[e] = r + e < rank ? f[e] * scale : 0.0f;
-        uint4* to = s_h + ((m * tiles + q) * H) * 64 + l;  // the parts of a row's 16 ranks: lanes l and l + 32
-        if constexpr (H == 1) {
-            float lo[8];
-            to[0] = Vec<SLHIP_BF16>::pack(f);
-            Vec<SLHIP_BF16>::unpack(to[0], lo);
-#pragma unroll
-            for (int e = 0; e < 8; e++) lo[e] = low_part(f[e], lo[e]);
-            to[32] = Vec<SLHIP_BF16>::pack(lo);
-        } else {
-            bf16x8 p[3];
-            cut(f, p);
-#pragma unroll
-            for (int i = 0; i < 3; i++) to[32 * i] = __builtin_bit_cast(uint4, p[i]);
-            to[96] = make_uint4(0, 0, 0, 0);
-        }
-    }
-    __syncthreads();
-    for (int32_t n0 = first; n0 < a.N; n0 += step) {
-        if (n0 > first) fetch(n0);
-        const bool whole = is_whole(n0);
-        f32x4 acc[MT][4];
+    const int32_t rank = key < 0 ? 0 : rank_of(a, key), tiles = (rank + RC - 1) / RC, all = (a.R + RC - 1) / RC;
+    const auto finish = [&](int32_t n0, bool whole) __attribute__((always_inline)) {
+        f32x4 acc[MT][E];
         const auto multiply = [&](int q, auto begins) __attribute__((always_inline)) {
-            if (16 * q + 16 > rank) {  // ranks behind the last may hold anything
+            if (RC * q + RC > rank) {  // ranks behind the last may hold anything
 #pragma unroll
-                for (int u = 0; u < 4; u++) w[u].keep(rank - 16 * q - 8 * (g & 1));
+                for (int u = 0; u < E; u++) w[u].keep(rank - RC * q - rl);
             }
-            bf16x8 pw[4][PW];
+            bf16x8 pw[E][PW];
 #pragma unroll
-            for (int u = 0; u < 4; u++) w[u].parts(0, pw[u]);
+            for (int u = 0; u < E; u++) w[u].parts(0, pw[u]);
             if (q + 1 < tiles) fetch_w(n0, q + 1, whole);
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
                 for (int h = H - 1; h >= 0; h--) {
-                    const bf16x8 x = __builtin_bit_cast(bf16x8, s_h[((m * tiles + q) * H + h) * 64 + lane]);
+                    const bf16x8 x = __builtin_bit_cast(bf16x8, s_h[((m * all + q) * H + h) * 64 + lane]);
 #pragma unroll
                     for (int i = PW - 1; i >= 0; i--)
 #pragma unroll
-                        for (int u = 0; u < 4; u++)
-                            acc[m][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pw[u][i], x, begins && h == H - 1 && i == PW - 1 ? f32x4{0, 0, 0, 0} : acc[m][u], 0, 0, 0);
+                        for (int u = 0; u < E; u++)
+                            acc[m][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pw[u][i], begins && h == H - 1 && i == PW - 1 ? f32x4{0, 0, 0, 0} : acc[m][u], 0, 0, 0);
                 }
         };
         if (tiles > 0) {
@@ -609,39 +525,90 @@ template <int YT, int WT, int MT> __global__ __launch_bounds__(kThreads) void lo
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int u = 0; u < 4; u++) acc[m][u] = f32x4{0, 0, 0, 0};
+                for (int u = 0; u < E; u++) acc[m][u] = f32x4{0, 0, 0, 0};
         }
         const int64_t at = static_cast<int64_t>(n0) * Vec<YT>::BYTES;
+        const int32_t n = a.N - (n0 + E * c);
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
-            for (int p = 0; p < kPieces; p += 2) {
-                uint4 v[2] = {add[m][p], add[m][p + 1]};
-                swap_halves(v[0], v[1]);
+            for (int r = 0; r < 4; r++) {
+                if (m + r > 0 && 4 * m + r >= most) break;
+                float f[E];
+                Vec<YT>::unpack(add[m][r], f);
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    float f[E];
-                    Vec<YT>::unpack(v[i], f);
+                for (int u = 0; u < E; u++) f[u] += acc[m][u][r];
+                char* const p = to + at + static_cast<uint64_t>(row[m][r]) * ys;
+                if (whole || n >= E) {
+                    if (there[m][r]) store_any(p, Vec<YT>::pack(f));
+                } else if (there[m][r]) {  // the last ones of a row
 #pragma unroll
-                    for (int e = 0; e < E; e++) f[e] += acc[m][(p + i) * E / 4 + e / 4][e & 3];
-                    v[i] = Vec<YT>::pack(f);
-                }
-                swap_halves(v[0], v[1]);
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    char* const place = to[m][i] + at + p * 64;
-                    const int32_t n = a.N - (n0 + p * 4 * E + in);
-                    if (whole || n >= E) {
-                        if (there[m][i]) store_any(place, v[i]);
-                    } else if (there[m][i]) {  // the last ones of a row
-                        float f[E];
-                        Vec<YT>::unpack(v[i], f);
-#pragma unroll
-                        for (int e = 0; e < E; e++)
-                            if (e < n) Vec<YT>::store1(place, e, f[e]);
-                    }
+                    for (int u = 0; u < E; u++)
+                        if (u < n) Vec<YT>::store1(p, u, f[u]);
                 }
             }
+    };
+    // thread blocks that run together take neighbouring columns: the same columns of many rows lie in few memory channels
+    const int32_t first = (cb * kWaves + wave) * kColumns, step = col_blocks * kWaves * kColumns;
+    if (first < a.N) fetch(first, is_whole(first));
+    const float scale = key < 0 || !a.scale ? 1.0f : a.scale[key];
+    const int32_t splits = a.plan ? a.plan->splits : a.splits;
+    // h, ranges of K added up: `parts` lanes share eight ranks of a row
+    const int32_t units = key < 0 ? 0 : MT * all * 2 * RC, parts = units <= 32 ? 8 : units <= 64 ? 4 : units <= 128 ? 2 : 1;
+    for (int t = tid; t < units * parts; t += kThreads) {
+        const int part = t & (parts - 1), unit = t / parts, m = unit / (all * 2 * RC), q = unit / (2 * RC) - m * all, l = unit & (2 * RC - 1);
+        const int32_t at = s_rows[16 * m + 4 * (l & 3) + (l >> 2 & 3)], r = RC * q + 8 * (l >> 4);
+        float f[8] = {};
+        if (at >= 0 && r < rank) {
+            const float* h = a.h + static_cast<int64_t>(at) * a.R16 + r;
+            const int64_t range = a.T * a.R16;
+            for (int s = part; s < splits; s += 2 * parts) {
+                f32x4 x[2][2];
+#pragma unroll
+                for (int v = 0; v < 2; v++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) x[v][e] = reinterpret_cast<const f32x4*>(h + min(s + v * parts, splits - 1) * range)[e];
+#pragma unroll
+                for (int v = 0; v < 2; v++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) f[e] += s + v * parts < splits ? x[v][e >> 2][e & 3] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (parts > 1) f[e] += dpp_f32<0xB1>(f[e]);
+            if (parts > 2) f[e] += dpp_f32<0x4E>(f[e]);
+            if (parts > 4) f[e] += dpp_f32<0x141>(f[e]);
+            f[e] = r + e < rank ? f[e] * scale : 0.0f;
+        }
+        if (part > 0) continue;
+        uint4* const put = s_h + ((m * all + q) * H) * 64 + l;  // WIDE: an operand a part, else lanes l and l + 32 of one
+        constexpr int kNext = WIDE ? 64 : 32;
+        if constexpr (P == 2) {
+            float lo[8];
+            put[0] = Vec<SLHIP_BF16>::pack(f);
+            Vec<SLHIP_BF16>::unpack(put[0], lo);
+#pragma unroll
+            for (int e = 0; e < 8; e++) lo[e] = low_part(f[e], lo[e]);
+            put[kNext] = Vec<SLHIP_BF16>::pack(lo);
+        } else {
+            bf16x8 p[3];
+            cut(f, p);
+#pragma unroll
+            for (int i = 0; i < 3; i++) put[kNext * i] = __builtin_bit_cast(uint4, p[i]);
+            if (!WIDE) put[96] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    __syncthreads();
+    for (int32_t n0 = first; n0 < a.N; n0 += step) {
+        const bool whole = is_whole(n0);
+        if (n0 > first) fetch(n0, whole);
+        finish(n0, whole);
+    }
+    };
+    for (int32_t item = blockIdx.x; item < work; item += gridDim.x) {
+        piece(item);
+        if (item + gridDim.x < work) __syncthreads();  // the next piece's rows and h
     }
 }
 
@@ -649,55 +616,75 @@ template <int YT, int WT, int MT> __global__ __launch_bounds__(kThreads) void lo
 
 static int64_t round16(int64_t n) { return (n + 15) & ~int64_t{15}; }
 
+// Tiles that T rows can make, and what their list takes: key and rows each.
+static int64_t most_tiles(int64_t T, int64_t tile) { return T / tile + (T < kMaxRequests ? T : kMaxRequests); }
+static int64_t plan_of(int64_t T) { return 16 + round16(4 * 33 * most_tiles(T, 16)); }
+
 static int64_t work_of(int64_t T, int64_t R)
 {
     const int64_t most = T > kSplitRows ? T : kSplitRows;
-    return (T * kMostSplits < most ? T * kMostSplits : most) * round16(R) * 4;
+    return (T * kMostSplits < most ? T * kMostSplits : most) * round16(R) * 4 + plan_of(T);
 }
 
 template <int XT, int WT, int MT> static int shrink(const LoraArgs& a, int64_t blocks, hipStream_t st)
 {
-    constexpr int few = MT == 1 ? 1 : 2;
-    const auto kernel = a.R16 <= 16 ? lora_shrink<XT, WT, few, 1> : a.R16 <= 32 ? lora_shrink<XT, WT, few, 2> : lora_shrink<XT, WT, MT, 4>;
+    const auto kernel = a.R16 <= 16 ? lora_shrink<XT, WT, MT, 1> : a.R16 <= 32 ? lora_shrink<XT, WT, MT, 2> : lora_shrink<XT, WT, MT, 4>;
     kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
     return check_launch("lora_shrink");
 }
 
 template <int YT, int WT, int MT> static int expand(const LoraArgs& a, int64_t blocks, hipStream_t st)
 {
-    const int lds = MT * a.R16 * (YT == SLHIP_BF16 ? 64 : 128);
-    if (lds > 60000)
-        SLHIP_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&lora_expand<YT, WT, MT>), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    lora_expand<YT, WT, MT><<<static_cast<unsigned>(blocks), kThreads, lds, st>>>(a);
+    constexpr int P = YT == SLHIP_BF16 ? 2 : 3;
+    const int lds = MT * 1024 * (a.R16 <= 16 ? P - 1 : (a.R + 31) / 32 * P);  // at most 48 KB
+    const auto kernel = a.R16 <= 16 ? lora_expand<YT, WT, MT, false> : lora_expand<YT, WT, MT, true>;
+    kernel<<<static_cast<unsigned>(blocks), kThreads, lds, st>>>(a);
     return check_launch("lora_expand");
 }
 
-template <int WT> static int launch(int dtype_x, int dtype_y, LoraArgs& a, hipStream_t st)
+template <int MT> static int plan(const LoraArgs& a, int64_t blocks1, int64_t blocks2, hipStream_t st)
 {
-    const bool few = a.T <= 32 * static_cast<int64_t>(a.B);
-    const int first_tile = few ? 16 : a.R16 <= 32 ? 32 : 64, second_tile = few ? 16 : a.R16 <= 32 ? 32 : 64;
-    const int64_t first_items = item_count(a.T, a.B, first_tile, 1), items = item_count(a.T, a.B, second_tile, 1);
+    SLHIP_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&lora_plan<16 * MT>), hipFuncAttributeMaxDynamicSharedMemorySize, kPlanLds));
+    lora_plan<16 * MT><<<1, kPlanThreads, kPlanLds, st>>>(a, static_cast<int32_t>(blocks1), static_cast<int32_t>(blocks2));
+    return check_launch("lora_plan");
+}
+
+template <int WT, int MT> static int launch(int dtype_x, int dtype_y, LoraArgs& a, hipStream_t st)
+{
+    const bool planned = a.B > 64;
+    const int64_t tiles = planned ? most_tiles(a.T, 16 * MT) : item_count(a.T, a.B, 16 * MT, 1);
+    const int64_t wide = kWaves * (dtype_y == SLHIP_F32 ? 64 : 128);
     a.rank_blocks = a.R16 <= 32 ? 1 : (a.R16 + 63) / 64;
-    // ranges of K: enough thread blocks for the machine, of 256 inputs at least
-    int64_t splits = (few ? 4096 : 1024) / (first_items * a.rank_blocks), most = a.K / 256;
-    if (splits > most) splits = most;
+    a.cols = static_cast<int32_t>((a.N + wide - 1) / wide);
+    // ranges of K of 512 inputs at least, as far as they give the machine work
+    int64_t splits = a.K / 512;
     if (splits > kMostSplits) splits = kMostSplits;
     if (splits > kSplitRows / a.T) splits = kSplitRows / a.T;
+    if (!planned && splits > 1024 / (tiles * a.rank_blocks)) splits = 1024 / (tiles * a.rank_blocks);
     a.splits = splits < 1 ? 1 : static_cast<int32_t>(splits);
-    const int64_t cols = (a.N + 64 * kWaves - 1) / (64 * kWaves);
-    int64_t steps = few && a.B > 64 ? 1 : (items * cols + 2047) / 2048;
-    if (steps > 8) steps = 8;
-    a.col_blocks = static_cast<int32_t>((cols + steps - 1) / steps);
-    const int64_t first = first_items * a.splits * a.rank_blocks, second = items * a.col_blocks;
+    // a thread block's steps along the columns: a tile's beginning costs as much as some
+    const int64_t blocks2 = MT == 1 ? 512 : 1024;
+    const int64_t most = blocks2 / tiles;
+    a.col_blocks = planned || most >= a.cols ? a.cols : most < 1 ? 1 : static_cast<int32_t>(most);
+    int64_t first = tiles * a.splits * a.rank_blocks, second = tiles * a.col_blocks;
+    if (planned) {
+        if (first > 1024) first = 1024;
+        if (second > blocks2) second = blocks2;
+        const int e = plan<MT>(a, first, second, st);
+        if (e) return e;
+    } else {
+        a.plan = nullptr;
+    }
     if (first > 0xFFFFFF || second > 0xFFFFFF) return fail(SLHIP_ERR_UNSUPPORTED, "lora: too many rows");
-    const bool f32 = dtype_x == SLHIP_F32;
-    const int e = few ? f32 ? shrink<SLHIP_F32, WT, 1>(a, first, st) : shrink<SLHIP_BF16, WT, 1>(a, first, st)
-                      : f32 ? shrink<SLHIP_F32, WT, 4>(a, first, st) : shrink<SLHIP_BF16, WT, 4>(a, first, st);
+    const int e = dtype_x == SLHIP_F32 ? shrink<SLHIP_F32, WT, MT>(a, first, st) : shrink<SLHIP_BF16, WT, MT>(a, first, st);
     if (e) return e;
-    const bool out32 = dtype_y == SLHIP_F32;
-    if (second_tile == 16) return out32 ? expand<SLHIP_F32, WT, 1>(a, second, st) : expand<SLHIP_BF16, WT, 1>(a, second, st);
-    if (second_tile == 32) return out32 ? expand<SLHIP_F32, WT, 2>(a, second, st) : expand<SLHIP_BF16, WT, 2>(a, second, st);
-    return out32 ? expand<SLHIP_F32, WT, 4>(a, second, st) : expand<SLHIP_BF16, WT, 4>(a, second, st);
+    return dtype_y == SLHIP_F32 ? expand<SLHIP_F32, WT, MT>(a, second, st) : expand<SLHIP_BF16, WT, MT>(a, second, st);
+}
+
+// Tiles of 16 rows where requests have few (a decode step), of 32 where they have many.
+template <int WT> static int launch(int dtype_x, int dtype_y, LoraArgs& a, hipStream_t st)
+{
+    return a.T <= 32 * static_cast<int64_t>(a.B) ? launch<WT, 1>(dtype_x, dtype_y, a, st) : launch<WT, 2>(dtype_x, dtype_y, a, st);
 }
 
 }  // namespace slhip
@@ -732,6 +719,7 @@ extern "C" SLHIP_API int slhip_lora(int dtype_x, int dtype_y, const void* x, int
         return fail(SLHIP_ERR_UNSUPPORTED, "lora: too many adapters, inputs, outputs or rows (a matrix of an adapter has less than 2^31 bytes)");
     if (x_stride < set->K || y_stride < set->N || (add && add_stride < set->N))
         return fail(SLHIP_ERR_INVALID, "lora: a row stride is smaller than the row");
+    if (y_stride >= int64_t{1} << 30 || (add && add_stride >= int64_t{1} << 30)) return fail(SLHIP_ERR_UNSUPPORTED, "lora: rows 2^30 values apart or more");
     if (set->a_stride < set->max_rank * set->K || set->b_stride < set->max_rank * set->N)
         return fail(SLHIP_ERR_INVALID, "lora: an adapter stride is smaller than the adapter");
     if (rows->requests == 0 || rows->tokens == 0) return SLHIP_OK;
@@ -756,7 +744,7 @@ extern "C" SLHIP_API int slhip_lora(int dtype_x, int dtype_y, const void* x, int
     a.adapters = static_cast<int32_t>(set->adapters);
     a.R = static_cast<int32_t>(set->max_rank);
     a.R16 = static_cast<int32_t>(round16(set->max_rank));
-    a.spare = static_cast<int32_t>((a.R16 - 1) / a.R);
+    a.spare = a.R <= 16 ? 15 / a.R : ((a.R + 31) / 32 * 32 - 1) / a.R;
     a.K = static_cast<int32_t>(set->K);
     a.N = static_cast<int32_t>(set->N);
     a.rank = set->rank;
@@ -765,7 +753,10 @@ extern "C" SLHIP_API int slhip_lora(int dtype_x, int dtype_y, const void* x, int
     a.T = rows->tokens;
     a.starts = rows->starts;
     a.adapter = rows->adapter;
-    a.h = static_cast<float*>(work);
+    a.plan = static_cast<Plan*>(work);
+    a.plan_key = reinterpret_cast<int32_t*>(a.plan + 1);
+    a.plan_rows = a.plan_key + most_tiles(a.T, 16);
+    a.h = reinterpret_cast<float*>(static_cast<char*>(work) + plan_of(a.T));
     int e = error_word(&a.err);
     if (e) return e;
     hipStream_t st = to_stream(stream);

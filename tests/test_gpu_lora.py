@@ -136,6 +136,31 @@ def test_many_requests(device, B, most, adapters, rank, K, N, x, w, y):
         run(d, Case("many", new, adapter, adapters, rank, K, N, x, w, y, ranks=ranks, scale=rng.standard_normal(adapters), padding=int(rng.integers(0, 20))))
 
 
+@pytest.mark.parametrize("B,most,adapters,share", [(65, 1, 70, 0.0), (66, 700, 3, 0.8), (130, 40, 1, 0.3), (1000, 3, 400, 0.0), (2500, 2, 900, 0.5)])
+def test_lists_of_tiles(device, B, most, adapters, share):
+    """More than 64 requests: few and many adapters, long and empty requests."""
+    rng = rng_of("lists", B, most, adapters)
+    new = np.where(rng.random(B) < share, 0, rng.integers(1, most + 1, B))
+    if most == 700:
+        new = np.where(rng.random(B) < 0.9, np.minimum(new, 5), new)
+    with Dev() as d:
+        run(d, Case("lists", new, rng.integers(-1, adapters, B), adapters, 20, 72, 80, "bf16", "bf16", "f32", padding=3))
+
+
+def test_requests_that_overlap_are_reported(device):
+    """More than 64 requests whose starts fall: nothing is listed for them."""
+    c = Case("overlap", [2] * 80, [0] * 80, 1, 8, 64, 32)
+    c.starts[1:80:2] = 160
+    with Dev() as d:
+        args, more = c.put(d)
+        log("lora of requests that overlap")
+        native.lora(*args, **more)
+        with pytest.raises(native.SlhipCacheError):
+            native.synchronize()
+        native.synchronize()
+        assert (d.get(c.py, (c.T, c.N), np.float32) == -777.25).all()
+
+
 @pytest.mark.parametrize("x,w,y", TYPES[:2])
 def test_4096_requests(device, x, w, y):
     rng = rng_of("4096")
