@@ -228,12 +228,22 @@ __device__ __forceinline__ uint4 shift_down(uint4 v, int32_t bytes)
     return make_uint4(__builtin_amdgcn_alignbit(v.y, v.x, s), __builtin_amdgcn_alignbit(v.z, v.y, s), __builtin_amdgcn_alignbit(v.w, v.z, s), v.w >> s);
 }
 
-// 16 bytes of an array that ends at element `end` (and has 16 bytes at least): zeros behind its end.
-template <int DT> __device__ __forceinline__ uint4 load_end(const void* p, int64_t at, int64_t end)
+// 16 bytes from element `at` of a row of n (16 bytes or more): zeros behind its end.
+template <int DT> __device__ __forceinline__ uint4 load_end(const char* row, int32_t at, int32_t n)
 {
     constexpr int E = Vec<DT>::N;
-    const int64_t in = min(at, end - E);
-    return shift_down(load_any(static_cast<const char*>(p) + in * Vec<DT>::BYTES), static_cast<int32_t>(min(at - in, static_cast<int64_t>(E))) * Vec<DT>::BYTES);
+    const int32_t in = min(at, n - E);
+    return shift_down(load_any(row + static_cast<uint32_t>(in) * Vec<DT>::BYTES), min(at - in, E) * Vec<DT>::BYTES);
+}
+
+// v's bytes moved up by `bytes` (0 .. 16, even), zeros below them.
+__device__ __forceinline__ uint4 shift_up(uint4 v, int32_t bytes)
+{
+    if (bytes & 16) v = make_uint4(0, 0, 0, 0);
+    if (bytes & 8) v = make_uint4(0, 0, v.x, v.y);
+    if (bytes & 4) v = make_uint4(0, v.x, v.y, v.z);
+    if (bytes & 2) v = make_uint4(v.x << 16, __builtin_amdgcn_alignbit(v.y, v.x, 16), __builtin_amdgcn_alignbit(v.z, v.y, 16), __builtin_amdgcn_alignbit(v.w, v.z, 16));
+    return v;
 }
 
 // The first n elements of v; the others become 0.
@@ -257,11 +267,27 @@ template <int DT, int N> struct Run {
 #pragma unroll
         for (int i = 0; i < kVecs; i++) w[i] = load_any(p + 16 * i);
     }
-    // Of an array that ends at `end`.
-    __device__ __forceinline__ void load_end(const void* p, int64_t at, int64_t end)
+    __device__ __forceinline__ void load_end(const char* row, int32_t at, int32_t n)
     {
 #pragma unroll
-        for (int i = 0; i < kVecs; i++) w[i] = slhip::load_end<DT>(p, at + i * kPer, end);
+        for (int i = 0; i < kVecs; i++) w[i] = slhip::load_end<DT>(row, at + i * kPer, n);
+    }
+    // The elements from the k-th on, zeros behind them.
+    __device__ __forceinline__ void shift(int32_t k)
+    {
+#pragma unroll
+        for (int i = 0; i < kVecs; i++) {  // (of two vectors the second one's first come behind the first one's last)
+            const int32_t by = min(k, kPer) * Vec<DT>::BYTES;
+            if (kVecs == 2 && i == 0 && k > 0) {
+                const uint4 a = shift_down(w[0], by), b = w[1];
+                const uint4 up = shift_up(b, 16 - by);
+                w[0] = k >= kPer ? shift_down(b, min(k - kPer, kPer) * Vec<DT>::BYTES) : make_uint4(a.x | up.x, a.y | up.y, a.z | up.z, a.w | up.w);
+            } else if (kVecs == 2 && i == 1) {
+                w[1] = shift_down(w[1], by);
+            } else {
+                w[i] = shift_down(w[i], by);
+            }
+        }
     }
     __device__ __forceinline__ void keep(int32_t n)
     {
@@ -366,18 +392,11 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
     for (; u < u1; u += kWaves) {
         Run<XT, 16> x[MT];
         Run<WT, 16> w[RB];
-        const int32_t k = u * kUnit + 16 * g, n = a.K - k;
+        const int32_t k = u * kUnit + 16 * g;
 #pragma unroll
-        for (int q = 0; q < RB; q++) {
-            w[q].load_end(ad, min(r0 + 16 * q + c, rank - 1) * a.K + k, a.R * a.K);
-            w[q].keep(n);
-        }
+        for (int q = 0; q < RB; q++) w[q].load_end(ad + (ap[q] - 16 * g * Vec<WT>::BYTES), k, a.K);
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
-            const int32_t row = s_rows[16 * m + c];
-            x[m].load_end(a.x, (row >= 0 ? row : s_rows[0]) * a.xs + k, (a.T - 1) * a.xs + a.K);
-            x[m].keep(n);
-        }
+        for (int m = 0; m < MT; m++) x[m].load_end(xp[m] - 16 * g * Vec<XT>::BYTES, k, a.K);
         multiply(x, w);
     }
     // the sums of waves 2 and 3 into 0 and 1, and 1 into 0
@@ -416,23 +435,47 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
 
 // ---- y = add + s B h -----------------------------------------------------------------------------------------------
 
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
-
-__device__ __forceinline__ void store_any(char* p, const uint4& v)
-{
-    const u32x4 t = {v.x, v.y, v.z, v.w};
-    __builtin_nontemporal_store(t, reinterpret_cast<u32x4_any*>(p));
-}
+// E neighbours of a row of add or y, 8 or 16 bytes.
+template <int DT, int E> struct Piece {
+    static constexpr int kWords = E * Vec<DT>::BYTES / 4;
+    typedef uint32_t words __attribute__((ext_vector_type(kWords)));
+    typedef words words_any __attribute__((aligned(2)));
+    words w;
+    __device__ __forceinline__ void load(const char* p) { w = __builtin_nontemporal_load(reinterpret_cast<const words_any*>(p)); }
+    __device__ __forceinline__ void store(char* p) const { __builtin_nontemporal_store(w, reinterpret_cast<words_any*>(p)); }
+    __device__ __forceinline__ void floats(float (&f)[E]) const
+    {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) {
+            if constexpr (DT == SLHIP_F32) {
+                f[i] = __uint_as_float(w[i]);
+            } else {
+                f[2 * i] = bf16_lo(w[i]);
+                f[2 * i + 1] = bf16_hi(w[i]);
+            }
+        }
+    }
+    __device__ __forceinline__ void pack(const float (&f)[E])
+    {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) {
+            if constexpr (DT == SLHIP_F32) w[i] = __float_as_uint(f[i]);
+            else w[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+        }
+    }
+};
 
 // The two bf16 parts of v, rounded: what is left of an infinity is 0.
 __device__ __forceinline__ float low_part(float v, float hi) { return fabsf(hi) < INFINITY ? v - hi : 0.0f; }
 
-// Rows are the first operand here and columns the second. A wave has 16 E columns of its rows, E = 16 bytes of y: product u the
-// columns E c + u, so that a lane's sums of E products are 16 bytes of a row, 16 lanes 256 of it. Row 4 r + g of 16 stands in the operand's
+constexpr int kLane = 4;  // columns of a lane: 8 of bf16 take 256 registers with their sums, and two waves a SIMD are too few
+
+// Rows are the first operand here and columns the second. A wave has 64 columns of its rows: product u the columns 4 c + u, so that a
+// lane's sums of the four products are neighbours in a row, and 16 lanes load and store whole lines of it. Row 4 r + g of 16 stands in the operand's
 // place 4 g + r: lane (c, g) has it in element r, and of up to four rows (a decode step's, most often one) all lie in element 0.
 template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThreads) void lora_expand(LoraArgs a)
 {
-    constexpr int TM = 16 * MT, PW = kParts<WT>, E = Vec<YT>::N, kColumns = 16 * E;
+    constexpr int TM = 16 * MT, PW = kParts<WT>, E = kLane, kColumns = 16 * E;
     // h's parts of RC ranks are the first operands of H instructions: up to 16 ranks two parts share one, more have one each
     constexpr int P = YT == SLHIP_BF16 ? 2 : 3, H = WIDE ? P : P - 1, RC = WIDE ? 32 : 16;
     __shared__ int32_t s_rows[TM];
@@ -444,8 +487,6 @@ template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThrea
     const int32_t key = find_tile<TM>(a, item / col_blocks, s_rows);
     if (key == kNoTile || (key < 0 && a.add == a.y)) return;
     const char* const ad = static_cast<const char*>(a.b) + (key < 0 ? 0 : key * a.sb * Vec<WT>::BYTES);
-    const char* const from = static_cast<const char*>(a.add) + E * c * Vec<YT>::BYTES;
-    char* const to = static_cast<char*>(a.y) + E * c * Vec<YT>::BYTES;
     const uint32_t as = static_cast<uint32_t>(a.as * Vec<YT>::BYTES), ys = static_cast<uint32_t>(a.ys * Vec<YT>::BYTES);
     uint32_t row[MT][4];
     bool there[MT][4];
@@ -459,45 +500,40 @@ template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThrea
             row[m][r] = v >= 0 ? v : s_rows[0];
             if (__any(v >= 0)) most = 4 * m + r + 1;
         }
-    uint4 add[MT][4];
+    Piece<YT, E> add[MT][4];
     Run<WT, 8> w[E];
     const int rl = 8 * (WIDE ? g : g & 1);  // the lane's ranks of RC
-    const uint32_t wp = static_cast<uint32_t>(E * c * a.R + rl) * Vec<WT>::BYTES;
-    // whole: all columns, whose last ranks' loads end inside the adapter
-    const auto is_whole = [&](int32_t n0) { return n0 + kColumns + a.spare <= a.N; };
-    const auto fetch_w = [&](int32_t n0, int q, bool whole) __attribute__((always_inline)) {
-        if (whole) {
-            const char* const at = ad + (static_cast<int64_t>(n0) * a.R + RC * q) * Vec<WT>::BYTES;
+    // The lane's columns from n0 on: of lanes behind the last column those before it once more. Of a column's last ranks the loads reach into the
+    // next one's; those that would leave the adapter begin before, and what they brought is moved down (fix).
+    const auto column = [&](int32_t n0) { return min(n0 + E * c, a.N - E); };
+    const auto whole = [&](int32_t n0) { return n0 + kColumns + a.spare <= a.N; };
+    const auto fetch_w = [&](int32_t n0, int q) __attribute__((always_inline)) {
+        const int32_t at = column(n0) * a.R + RC * q + rl, last = a.N * a.R - 8;
 #pragma unroll
-            for (int u = 0; u < E; u++) w[u].load(at + (wp + static_cast<uint32_t>(u * a.R) * Vec<WT>::BYTES));
-        } else {
-#pragma unroll
-            for (int u = 0; u < E; u++) w[u].load_end(ad, min(n0 + E * c + u, a.N - 1) * a.R + RC * q + rl, a.N * a.R);
-        }
+        for (int u = 0; u < E; u++) w[u].load(ad + static_cast<uint32_t>(min(at + u * a.R, last)) * Vec<WT>::BYTES);
     };
-    const auto fetch = [&](int32_t n0, bool whole) __attribute__((always_inline)) {
-        if (key >= 0) fetch_w(n0, 0, whole);
-        const int64_t at = static_cast<int64_t>(n0) * Vec<YT>::BYTES;
+    const auto fix = [&](int32_t n0, int q) __attribute__((always_inline)) {
+        const int32_t at = column(n0) * a.R + RC * q + rl, last = a.N * a.R - 8;
+#pragma unroll
+        for (int u = 0; u < E; u++) w[u].shift(max(at + u * a.R - last, 0));
+    };
+    const auto fetch = [&](int32_t n0) __attribute__((always_inline)) {
+        if (key >= 0) fetch_w(n0, 0);
+        const char* const at = static_cast<const char*>(a.add) + static_cast<uint32_t>(column(n0)) * Vec<YT>::BYTES;
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 if (m + r > 0 && 4 * m + r >= most) break;
-                const char* const p = from + at + static_cast<uint64_t>(row[m][r]) * as;
-                if (!a.add) {
-                    add[m][r] = make_uint4(0, 0, 0, 0);
-                } else if (whole) {
-                    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
-                    add[m][r] = make_uint4(v.x, v.y, v.z, v.w);
-                } else {
-                    add[m][r] = load_end<YT>(a.add, (p - static_cast<const char*>(a.add)) / Vec<YT>::BYTES, (a.T - 1) * a.as + a.N);
-                }
+                if (a.add) add[m][r].load(at + static_cast<uint64_t>(row[m][r]) * as);
+                else add[m][r].w = 0;
             }
     };
     const int32_t rank = key < 0 ? 0 : rank_of(a, key), tiles = (rank + RC - 1) / RC, all = (a.R + RC - 1) / RC;
-    const auto finish = [&](int32_t n0, bool whole) __attribute__((always_inline)) {
+    const auto finish = [&](int32_t n0) __attribute__((always_inline)) {
         f32x4 acc[MT][E];
         const auto multiply = [&](int q, auto begins) __attribute__((always_inline)) {
+            if (!whole(n0)) fix(n0, q);
             if (RC * q + RC > rank) {  // ranks behind the last may hold anything
 #pragma unroll
                 for (int u = 0; u < E; u++) w[u].keep(rank - RC * q - rl);
@@ -505,52 +541,56 @@ template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThrea
             bf16x8 pw[E][PW];
 #pragma unroll
             for (int u = 0; u < E; u++) w[u].parts(0, pw[u]);
-            if (q + 1 < tiles) fetch_w(n0, q + 1, whole);
+            if (WIDE && q + 1 < tiles) fetch_w(n0, q + 1);
+            bf16x8 x[MT][H];
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int h = H - 1; h >= 0; h--) {
-                    const bf16x8 x = __builtin_bit_cast(bf16x8, s_h[((m * all + q) * H + h) * 64 + lane]);
+                for (int h = 0; h < H; h++) x[m][h] = __builtin_bit_cast(bf16x8, s_h[((m * all + q) * H + h) * 64 + lane]);
+#pragma unroll
+            for (int u = 0; u < E; u++)
+#pragma unroll
+                for (int h = H - 1; h >= 0; h--)
 #pragma unroll
                     for (int i = PW - 1; i >= 0; i--)
 #pragma unroll
-                        for (int u = 0; u < E; u++)
-                            acc[m][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, pw[u][i], begins && h == H - 1 && i == PW - 1 ? f32x4{0, 0, 0, 0} : acc[m][u], 0, 0, 0);
-                }
+                        for (int m = 0; m < MT; m++)
+                            acc[m][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[m][h], pw[u][i], begins && h == H - 1 && i == PW - 1 ? f32x4{0, 0, 0, 0} : acc[m][u], 0, 0, 0);
         };
         if (tiles > 0) {
             multiply(0, std::true_type{});
-            for (int q = 1; q < tiles; q++) multiply(q, std::false_type{});
+            for (int q = 1; WIDE && q < tiles; q++) multiply(q, std::false_type{});
         } else {
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
                 for (int u = 0; u < E; u++) acc[m][u] = f32x4{0, 0, 0, 0};
         }
-        const int64_t at = static_cast<int64_t>(n0) * Vec<YT>::BYTES;
-        const int32_t n = a.N - (n0 + E * c);
+        const int32_t n = column(n0), mine = n0 + E * c;  // a lane's columns from `mine` on are its own
+        char* const to = static_cast<char*>(a.y) + static_cast<uint32_t>(n) * Vec<YT>::BYTES;
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 if (m + r > 0 && 4 * m + r >= most) break;
                 float f[E];
-                Vec<YT>::unpack(add[m][r], f);
+                add[m][r].floats(f);
 #pragma unroll
                 for (int u = 0; u < E; u++) f[u] += acc[m][u][r];
-                char* const p = to + at + static_cast<uint64_t>(row[m][r]) * ys;
-                if (whole || n >= E) {
-                    if (there[m][r]) store_any(p, Vec<YT>::pack(f));
-                } else if (there[m][r]) {  // the last ones of a row
+                char* const p = to + static_cast<uint64_t>(row[m][r]) * ys;
+                if (n == mine) {
+                    add[m][r].pack(f);
+                    if (there[m][r]) add[m][r].store(p);
+                } else if (there[m][r] && mine < a.N) {
 #pragma unroll
-                    for (int u = 0; u < E; u++)
-                        if (u < n) Vec<YT>::store1(p, u, f[u]);
+                    for (int u = 1; u < E; u++)
+                        if (n + u >= mine) Vec<YT>::store1(p, u, f[u]);
                 }
             }
     };
     // thread blocks that run together take neighbouring columns: the same columns of many rows lie in few memory channels
     const int32_t first = (cb * kWaves + wave) * kColumns, step = col_blocks * kWaves * kColumns;
-    if (first < a.N) fetch(first, is_whole(first));
+    if (first < a.N) fetch(first);
     const float scale = key < 0 || !a.scale ? 1.0f : a.scale[key];
     const int32_t splits = a.plan ? a.plan->splits : a.splits;
     // h, ranges of K added up: `parts` lanes share eight ranks of a row
@@ -601,9 +641,8 @@ template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThrea
     }
     __syncthreads();
     for (int32_t n0 = first; n0 < a.N; n0 += step) {
-        const bool whole = is_whole(n0);
-        if (n0 > first) fetch(n0, whole);
-        finish(n0, whole);
+        if (n0 > first) fetch(n0);
+        finish(n0);
     }
     };
     for (int32_t item = blockIdx.x; item < work; item += gridDim.x) {
@@ -653,7 +692,7 @@ template <int WT, int MT> static int launch(int dtype_x, int dtype_y, LoraArgs& 
 {
     const bool planned = a.B > 64;
     const int64_t tiles = planned ? most_tiles(a.T, 16 * MT) : item_count(a.T, a.B, 16 * MT, 1);
-    const int64_t wide = kWaves * (dtype_y == SLHIP_F32 ? 64 : 128);
+    constexpr int64_t wide = kWaves * 16 * kLane;
     a.rank_blocks = a.R16 <= 32 ? 1 : (a.R16 + 63) / 64;
     a.cols = static_cast<int32_t>((a.N + wide - 1) / wide);
     // ranges of K of 512 inputs at least, as far as they give the machine work
@@ -662,8 +701,11 @@ template <int WT, int MT> static int launch(int dtype_x, int dtype_y, LoraArgs& 
     if (splits > kSplitRows / a.T) splits = kSplitRows / a.T;
     if (!planned && splits > 1024 / (tiles * a.rank_blocks)) splits = 1024 / (tiles * a.rank_blocks);
     a.splits = splits < 1 ? 1 : static_cast<int32_t>(splits);
-    // a thread block's steps along the columns: a tile's beginning costs as much as some
-    const int64_t blocks2 = MT == 1 ? 512 : 1024;
+    // How many thread blocks share out the columns of all tiles. A tile's beginning (its rows, h) costs a thread block as much as some of its
+    // steps, the more the more ranks there are; many thread blocks end more evenly. (64 requests of an adapter each, 16 ranks, 14336 outputs: 512
+    // thread blocks 18.7 us with the first product, 2048 22.5, 4096 26.9; a prompt of 8192: 512 140 us, 1024 119, 4096 110; of 64 ranks
+    // 768 178, 4096 192.)
+    const int64_t blocks2 = MT == 1 ? 512 : a.R16 <= 16 ? 4096 : 768;
     const int64_t most = blocks2 / tiles;
     a.col_blocks = planned || most >= a.cols ? a.cols : most < 1 ? 1 : static_cast<int32_t>(most);
     int64_t first = tiles * a.splits * a.rank_blocks, second = tiles * a.col_blocks;
