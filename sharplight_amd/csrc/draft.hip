@@ -34,6 +34,8 @@ enum : int32_t { kDone = 0, kFromTarget = 1, kFromRest = 2, kFromOthers = 3 };  
 struct Pick {
     int32_t kind, row, place, token;  // the row, its place in the request, its draft
     double mp, cp, ip, mq, cq, iq;    // maxima, log2(e) / tau, 1 / sums
+    double px;                        // p of the draft
+    int32_t held, reserved;           // where its chunks' shares are held in LDS (-1: nowhere)
 };
 
 struct DraftArgs {
@@ -141,13 +143,11 @@ __device__ __forceinline__ double wave_scan64(double v)
     return v + dpp64<0x143, 0xC>(v);
 }
 
-// 2^y to 2^-40 of itself for y <= 0 (0 below -1000): the series of 2^f, |f| <= 1/2.
+// 2^y to 2^-36 of itself for y <= 0 (0 below -1000): the series of 2^f, |f| <= 1/2.
 __device__ __forceinline__ double exp2_64(double y)
 {
     const double n = rint(y), f = (y - n) * 0.693147180559945309417;
-    double r = 1.0 / 39916800.0;
-    r = fma(r, f, 1.0 / 3628800.0);
-    r = fma(r, f, 1.0 / 362880.0);
+    double r = 1.0 / 362880.0;
     r = fma(r, f, 1.0 / 40320.0);
     r = fma(r, f, 1.0 / 5040.0);
     r = fma(r, f, 1.0 / 720.0);
@@ -161,6 +161,19 @@ __device__ __forceinline__ double exp2_64(double y)
 }
 
 constexpr double kLog2e64 = 1.44269504088896340736;
+
+// log2(e) / tau as f32 parts, the second one positive: -inf times it is -inf.
+struct Factor {
+    float hi, lo;
+    __device__ __forceinline__ explicit Factor(double c)
+    {
+        const float near = static_cast<float>(c);
+        hi = near > c ? __uint_as_float(__float_as_uint(near) - 1) : near;
+        lo = fmaxf(static_cast<float>(c - hi), 0x1p-60f);
+    }
+    // 2^(d c) for d <= 0, -inf included.
+    __device__ __forceinline__ float power(float d) const { return __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo)); }
+};
 
 __device__ __forceinline__ double share_of(float z, double m, double c) { return z == -INFINITY ? 0.0 : exp2_64((static_cast<double>(z) - m) * c); }
 
@@ -187,27 +200,20 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
     float z[Logits<DT>::kEach];
 #pragma unroll
     for (int j = 0; j < kVecs; j++) Vec<DT>::unpack(x.w[j], &z[j * N]);
-    float m = -INFINITY;
-    bool bad = false;
+    float m = z[0];
 #pragma unroll
-    for (int j = 0; j < kVecs * N; j++) {
-        m = fmaxf(m, z[j]);
-        bad |= !(z[j] < INFINITY);
-    }
+    for (int j = 1; j < kVecs * N; j++) m = __builtin_elementwise_maximum(m, z[j]);  // a NaN stays
+    const bool bad = !(m < INFINITY);
     m = group_max<64>(m);
     if (__any(bad)) m = INFINITY;
     if (lane == 0) s_m[wave] = m;
     __syncthreads();
     m = s_m[0];
     for (int w = 1; w < kWaves; w++) m = fmaxf(m, s_m[w]);
-    const double c = kLog2e64 / h.tau;
-    const float hi = static_cast<float>(c), lo = static_cast<float>(c - hi);
+    const Factor c(kLog2e64 / h.tau);
     float s = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kVecs * N; j++) {
-        const float d = fmaxf(z[j] - m, -0x1p60f);
-        s += __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo));
-    }
+    for (int j = 0; j < kVecs * N; j++) s += c.power(z[j] - m);
     const double sum = wave_sum64(s);
     int32_t arg = 0x7FFFFFFF;
     if (target.greedy) {
@@ -243,10 +249,11 @@ struct RowStat {
     float z;
 };
 
-// The chunks of a row together, by 16 lanes. The first 64 chunks are looked at once.
-__device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks, double c, bool arg)
+constexpr int kHeld = 4;  // chunks of a lane that it looks at once: a vocabulary of 262144
+
+// The chunks of a row together, by 16 lanes. shares: of the first 64 chunks, in units of the row's sum before its division.
+__device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks, double c, bool arg, double* shares)
 {
-    constexpr int kHeld = 4;
     const int lane = threadIdx.x & 15;
     ChunkStat x[kHeld];
 #pragma unroll
@@ -270,11 +277,16 @@ __device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks,
     double s = 0.0;
     int32_t first = 0x7FFFFFFF;
     const auto take = [&](const ChunkStat& v) {
-        if (v.m > -INFINITY) s += v.s * exp2_64((static_cast<double>(v.m) - r.m) * c);
+        const double part = v.m > -INFINITY ? v.s * exp2_64((static_cast<double>(v.m) - r.m) * c) : 0.0;
+        s += part;
         if (v.m == m) first = min(first, v.arg);
+        return part;
     };
 #pragma unroll
-    for (int j = 0; j < kHeld; j++) take(x[j]);
+    for (int j = 0; j < kHeld; j++) {
+        const double part = take(x[j]);
+        if (shares) shares[lane + 16 * j] = part;
+    }
     for (int32_t k = lane + 16 * kHeld; k < chunks; k += 16) take(st[k]);
     r.s = row_sum64(s);
     if (arg) {
@@ -286,11 +298,12 @@ __device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks,
 }
 
 struct DecideLds {
-    RowStat row[16];  // of a pass: target's rows, or target's and draft's in turns
+    RowStat row[16];        // of a pass: target's rows, or target's and draft's in turns
+    double shares[16][64];  // of their first chunks, target's rows where no drafts were drawn
 };
 
-// What request i's accepted drafts are, and what is drawn behind them, by the whole block; into the outputs too.
-template <int DT> __device__ __forceinline__ Pick decide(const DraftArgs& a, int32_t i, DecideLds& lds)
+// What request i's accepted drafts are, and what is drawn behind them, by the whole block. `write`: into the outputs too.
+template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const DraftArgs& a, int32_t i, bool write, DecideLds& lds)
 {
     const int tid = threadIdx.x, lane = tid & 63, group = tid >> 4;
     const int64_t s0 = a.starts[i], s1 = a.starts[i + 1];
@@ -302,16 +315,20 @@ template <int DT> __device__ __forceinline__ Pick decide(const DraftArgs& a, int
     const int mats = drawn ? 2 : 1, rows = 16 / mats;
     int32_t* out = a.out + i * a.out_stride;
     float* logp = a.logp ? a.logp + i * a.out_stride : nullptr;
-    int32_t stop = n, first = 0;  // the place of the token behind the accepted drafts; the pass's first row
+    int32_t stop = n, first = 0, draft = -1;  // the place of the token behind the accepted drafts; the pass's first row; the refused draft
     for (; first < n; first += rows) {
         const int32_t count = min(n - first, rows), place = first + group / mats, mat = group & (mats - 1);
+        const int32_t mine = first + lane;
+        const bool row = lane < count && mine < n - 1;  // the lane's row has a draft
+        const int32_t x = row ? a.ids[s0 + mine + 1] : 0;
+        const double u = row ? a.accept[s0 + mine] : 0.0;
         if (place < n && (mat == 0 || place < n - 1)) {
             const int64_t t = s0 + place;
-            const int32_t x = place < n - 1 ? a.ids[t + 1] : 0;
+            const int32_t v = place < n - 1 ? a.ids[t + 1] : 0;
             float z = -INFINITY;
-            if (x >= 0 && x < a.V) z = Vec<DT>::load1(mat ? a.draft : a.target, t * (mat ? a.qs : a.zs) + x);
+            if (v >= 0 && v < a.V) z = Vec<DT>::load1(mat ? a.draft : a.target, t * (mat ? a.qs : a.zs) + v);
             const double c = mat ? cq : cp;
-            RowStat r = row_stat(a.stats + (t * 2 + mat) * a.chunks, a.chunks, c, hp.greedy);
+            RowStat r = row_stat(a.stats + (t * 2 + mat) * a.chunks, a.chunks, c, hp.greedy, SHARES ? lds.shares[group] : nullptr);
             r.fine &= !(mat ? hq.bad : hp.bad);
             r.z = z;
             r.share = share_of(z, r.m, c) / r.s;
@@ -319,19 +336,17 @@ template <int DT> __device__ __forceinline__ Pick decide(const DraftArgs& a, int
         }
         __syncthreads();
         // each wave looks at all rows of the pass, a lane each
-        const int32_t mine = first + lane;
-        const bool row = lane < count && mine < n - 1;  // it has a draft
         const RowStat &p = lds.row[(lane & (rows - 1)) * mats], &q = lds.row[(lane & (rows - 1)) * mats + mats - 1];
-        const int32_t x = row ? a.ids[s0 + mine + 1] : 0;
         const bool known = x >= 0 && x < a.V;
         bool good = false;
         if (row && p.fine && known) {
             if (hp.greedy) good = x == p.arg;
-            else if (!drawn || q.fine) good = static_cast<double>(a.accept[s0 + mine]) * (drawn ? q.share : 1.0) < p.share;
+            else if (!drawn || q.fine) good = u * (drawn ? q.share : 1.0) < p.share;
         }
         const uint64_t refused = ~__ballot(good) & ((uint64_t{1} << count) - 1);
         if (refused) stop = first + __ffsll(static_cast<long long>(refused)) - 1;
-        if (tid < 64) {
+        if (stop < n) draft = __builtin_amdgcn_readlane(x, stop - first);
+        if (write && tid < 64) {
             if (good && mine < stop) {
                 out[mine] = x;
                 if (logp) logp[mine] = static_cast<float>((static_cast<double>(p.z) - p.m) * (cp / kLog2e64) - log(p.s));
@@ -344,6 +359,7 @@ template <int DT> __device__ __forceinline__ Pick decide(const DraftArgs& a, int
     }
     Pick k{};
     k.kind = kDone;
+    k.held = -1;
     int32_t token = -1;
     float lp = NAN;
     if (n > 0) {
@@ -355,7 +371,7 @@ template <int DT> __device__ __forceinline__ Pick decide(const DraftArgs& a, int
             token = p.arg;
             lp = static_cast<float>(-log(p.s));
         } else if (p.fine) {
-            k.token = last ? -1 : a.ids[k.row + 1];
+            k.token = last ? -1 : draft;
             k.kind = last ? kFromTarget : !drawn ? kFromOthers : q.fine ? kFromRest : kFromTarget;
             k.mp = p.m;
             k.cp = cp;
@@ -363,8 +379,11 @@ template <int DT> __device__ __forceinline__ Pick decide(const DraftArgs& a, int
             k.mq = q.m;
             k.cq = cq;
             k.iq = 1.0 / q.s;
+            k.px = p.share;
+            k.held = SHARES ? (stop - first) * mats : -1;
         }
     }
+    if (!write) return k;
     if (tid == 0) {
         if (n > 0 && k.kind == kDone) {
             out[stop] = token;
@@ -386,25 +405,27 @@ template <int DT> __device__ __forceinline__ Pick decide(const DraftArgs& a, int
 
 // ---- the draw ------------------------------------------------------------------------------------------------------
 
-// e^((z - m) / tau): as f32 where it is below 2^-12 (its roundings are then below those of the sums), f64 above.
+// e^((z - m) / tau): as f32 where it is below 2^-6 (its roundings are then below those of the sums), f64 above, where p - q may cancel.
+// (A vector of four takes 160 instructions more for f64: with a border of 2^-12 the sums of 38 chunks took 8 us.)
 struct Share {
     double m, c;
-    float mf, hi, lo;
-    __device__ __forceinline__ Share(double m_, double c_) : m(m_), c(c_), mf(static_cast<float>(m_)), hi(static_cast<float>(c_)), lo(static_cast<float>(c_ - hi)) {}
+    float mf;
+    Factor f;
+    __device__ __forceinline__ Share(double m_, double c_) : m(m_), c(c_), mf(static_cast<float>(m_)), f(c_) {}
     template <int N> __device__ __forceinline__ void of(const float (&z)[N], double (&w)[N]) const
     {
-        bool large = false;
+        float e[N], most = 0.0f;
 #pragma unroll
-        for (int e = 0; e < N; e++) {
-            const float d = fmaxf(z[e] - mf, -0x1p60f), y = fmaf(d, hi, d * lo);
-            w[e] = static_cast<double>(__builtin_amdgcn_exp2f(y));
-            large |= y > -12.0f;
+        for (int j = 0; j < N; j++) {
+            e[j] = f.power(z[j] - mf);
+            most = fmaxf(most, e[j]);
+            w[j] = e[j];
         }
-        if (__any(large)) {
+        if (__any(most > 0x1p-6f)) {
 #pragma unroll
-            for (int e = 0; e < N; e++) {
-                const float d = fmaxf(z[e] - mf, -0x1p60f);
-                if (fmaf(d, hi, d * lo) > -12.0f) w[e] = exp2_64((static_cast<double>(z[e]) - m) * c);
+            for (int j = 0; j < N; j++) {  // (all of them: a lane's powers take turns then)
+                const double v = exp2_64((static_cast<double>(z[j]) - m) * c);
+                w[j] = e[j] > 0x1p-6f ? v : w[j];
             }
         }
     }
@@ -461,25 +482,29 @@ template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a
     return block_sum(s, lds);
 }
 
-// The draw itself, by the whole block. Chunk c's weight is sums[c], or where there are none p's, of the target's chunk sums.
-template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32_t i, const Pick& k, const double* sums)
+// The draw itself, by the whole block. Chunk c's weight is sums[c], or where there are none p's, of the target's chunk sums: of the chunk that
+// holds the refused draft without that. (Which is off by 2^-24 of the draft's p at most, as are the sums themselves.)
+template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32_t i, const Pick& k, const double* sums, const double* shares)
 {
     constexpr int N = Logits<DT>::N;
-    __shared__ double s_total[kWaves], s_other[kWaves], s_up[2][kWaves], s_part[kVecs][kWaves], s_before;
+    __shared__ double s_total[kWaves], s_up[2][kWaves], s_part[kVecs][kWaves], s_before;
     __shared__ int32_t s_chunk, s_last, s_place;
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const ChunkStat* st = a.stats + static_cast<int64_t>(k.row) * 2 * a.chunks;
+    const float u = a.sample[i];
     if (tid == 0) s_chunk = s_place = 0x7FFFFFFF;
     if (tid == 0) s_last = 0;
-    // the draft's chunk without it
     int32_t kind = k.kind;
     const int32_t other = kind == kFromOthers && k.token >= 0 && k.token < a.V ? k.token / kChunk<DT> : -1;
-    double others = 0.0;
-    if (other >= 0) others = chunk_sum<DT>(a, k, other, s_other);
-    const auto target = [&](int32_t c) { return st[c].m > -INFINITY ? st[c].s * exp2_64((static_cast<double>(st[c].m) - k.mp) * k.cp) * k.ip : 0.0; };
-    const auto weight = [&](int32_t c) { return c == other ? others : sums ? sums[c] : target(c); };
-    double mine = 0.0;
-    for (int32_t c = tid; c < a.chunks; c += kThreads) mine += weight(c);
+    const auto target = [&](int32_t c) {
+        if (shares && c < 16 * kHeld) return shares[c] * k.ip;
+        const ChunkStat x = st[c];
+        return x.m > -INFINITY ? x.s * exp2_64((static_cast<double>(x.m) - k.mp) * k.cp) * k.ip : 0.0;
+    };
+    const auto weight = [&](int32_t c) { return c >= a.chunks ? 0.0 : sums ? sums[c] : c == other ? fmax(target(c) - k.px, 0.0) : target(c); };
+    const double first = weight(tid);  // of the thread's first chunk, mostly the only one
+    double mine = first;
+    for (int32_t c = tid + kThreads; c < a.chunks; c += kThreads) mine += weight(c);
     double total = block_sum(mine, s_total);
     const bool none = !(total > 0.0);  // p and q are equal, or the draft has all of p: p
     if (none) {
@@ -489,14 +514,13 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
         __syncthreads();
         total = block_sum(mine, s_total);
     }
-    const float u = a.sample[i];
     const double r = total * (u > 0.0f ? u : 0.0f);
     // the chunk: the first whose inclusive sum is above r, or the last one with a weight
     double base = 0.0;
     int32_t chunk = 0x7FFFFFFF;
     for (int32_t c0 = 0, turn = 0; c0 < a.chunks && chunk == 0x7FFFFFFF; c0 += kThreads, turn ^= 1) {
         const int32_t c = c0 + tid;
-        const double v = c >= a.chunks ? 0.0 : none ? target(c) : weight(c);
+        const double v = c >= a.chunks ? 0.0 : none ? target(c) : c0 == 0 ? first : weight(c);
         double up = wave_scan64(v);
         if (lane == 63) s_up[turn][wave] = up;
         __syncthreads();
@@ -569,23 +593,33 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
 template <int DT> __global__ __launch_bounds__(kThreads) void draft_choose(DraftArgs a)
 {
     __shared__ DecideLds lds;
-    const Pick k = decide<DT>(a, blockIdx.x, lds);
-    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, nullptr);
+    const Pick k = decide<DT, true>(a, blockIdx.x, true, lds);
+    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, nullptr, lds.shares[k.held]);
 }
 
-// Drafts that were drawn: what is accepted, then a thread block for each chunk of the row that is drawn from.
+// Drafts that were drawn: what is accepted, then a thread block for each chunk of the row that is drawn from. Few chunks in all (kDecides) are
+// a latency: each then decides for itself, in one launch.
 template <int DT> __global__ __launch_bounds__(kThreads) void draft_decide(DraftArgs a)
 {
     __shared__ DecideLds lds;
-    const Pick k = decide<DT>(a, blockIdx.x, lds);
+    const Pick k = decide<DT, false>(a, blockIdx.x, true, lds);
     if (threadIdx.x == 0) a.picks[blockIdx.x] = k;
 }
 
-template <int DT> __global__ __launch_bounds__(kThreads) void draft_sums(DraftArgs a)
+constexpr int64_t kDecides = 512;
+
+template <int DT, bool DECIDES> __global__ __launch_bounds__(kThreads) void draft_sums(DraftArgs a)
 {
     __shared__ double s_sum[kWaves];
     const int32_t i = blockIdx.x / a.chunks, chunk = blockIdx.x - i * a.chunks;
-    const Pick k = a.picks[i];
+    Pick k;
+    if constexpr (DECIDES) {
+        __shared__ DecideLds lds;
+        k = decide<DT, false>(a, i, chunk == 0, lds);
+        if (chunk == 0 && threadIdx.x == 0) a.picks[i] = k;
+    } else {
+        k = a.picks[i];
+    }
     if (k.kind != kFromRest) return;
     const double s = chunk_sum<DT>(a, k, chunk, s_sum);
     if (threadIdx.x == 0) a.sums[static_cast<int64_t>(i) * a.chunks + chunk] = s;
@@ -594,7 +628,7 @@ template <int DT> __global__ __launch_bounds__(kThreads) void draft_sums(DraftAr
 template <int DT> __global__ __launch_bounds__(kThreads) void draft_pick(DraftArgs a)
 {
     const Pick k = a.picks[blockIdx.x];
-    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, k.kind == kFromRest ? a.sums + static_cast<int64_t>(blockIdx.x) * a.chunks : nullptr);
+    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, k.kind == kFromRest ? a.sums + static_cast<int64_t>(blockIdx.x) * a.chunks : nullptr, nullptr);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
@@ -633,11 +667,15 @@ template <int DT> static int launch(DraftArgs& a, hipStream_t st)
         draft_choose<DT><<<B, kThreads, 0, st>>>(a);
         return check_launch("draft_choose");
     }
-    draft_decide<DT><<<B, kThreads, 0, st>>>(a);
-    int e = check_launch("draft_decide");
-    if (e) return e;
-    draft_sums<DT><<<B * a.chunks, kThreads, 0, st>>>(a);
-    e = check_launch("draft_sums");
+    if (static_cast<int64_t>(B) * a.chunks <= kDecides) {
+        draft_sums<DT, true><<<B * a.chunks, kThreads, 0, st>>>(a);
+    } else {
+        draft_decide<DT><<<B, kThreads, 0, st>>>(a);
+        const int e = check_launch("draft_decide");
+        if (e) return e;
+        draft_sums<DT, false><<<B * a.chunks, kThreads, 0, st>>>(a);
+    }
+    const int e = check_launch("draft_sums");
     if (e) return e;
     draft_pick<DT><<<B, kThreads, 0, st>>>(a);
     return check_launch("draft_pick");
