@@ -14,6 +14,8 @@
 // requests of 256 blocks 19 us, of 8192 432.
 // A trim is a release that leaves each request's first blocks, and it fills the stack from the other end, so that it undoes an
 // advance. Its few blocks' chain is the release's: lengths -> scan -> table entries -> stores.
+#include <type_traits>
+
 #include "common.hpp"
 #include "kv8_map.hpp"
 
@@ -148,46 +150,21 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     const auto request_of = [&](const int32_t* sums, int64_t k) {
         return static_cast<int32_t>(item_request([&](int64_t r) { return sums[r]; }, a.B, k, 1, 0));
     };
-    // What goes back has to be there (a request that was released before has no entries), so all entries are looked at before one is
-    // moved. Up to kHeld a thread are looked up once, all searches and loads on their way together; of more, a request is searched
-    // for only where the last one's blocks end.
-    constexpr int kHeld = 16;
-    const bool held = all_blocks <= kHeld * kPagesThreads;
-    int32_t *at[kHeld], entry[kHeld];
     const auto row_of = [&](int32_t i) {  // the first table entry that the request gives back
         return a.pages + slot_of(i) * a.bps + (OP == kTrim ? blocks_of(a.past[i], a.shift) : 0);
     };
     // where block k of all goes on the stack
     const auto place = [&](int64_t k) { return n_free + (OP == kTrim ? all_blocks - 1 - k : k); };
-    const auto entry_of = [&](int64_t k, int32_t& i) {
-        if (i + 1 < a.B && k >= s_off[i + 1]) i = request_of(s_off, k);
-        return row_of(i) + (k - s_off[i]);
-    };
-    if (RELEASE && ok) {
-        int64_t none = all_blocks;  // the thread's first block that is not there
-        if (held) {
-#pragma unroll
-            for (int u = 0; u < kHeld; u++) {
-                if (u * kPagesThreads >= all_blocks) break;
-                const int64_t k = min(static_cast<int64_t>(tid + u * kPagesThreads), all_blocks - 1);
-                const int32_t i = request_of(s_off, k);
-                at[u] = row_of(i) + (k - s_off[i]);
-                entry[u] = *at[u];
-            }
-#pragma unroll
-            for (int u = kHeld - 1; u >= 0; u--)
-                if (tid + u * kPagesThreads < all_blocks && entry[u] < 0) none = tid + u * kPagesThreads;
-        } else {
-            int32_t i = 0;
-            for (int64_t k = tid; k < all_blocks; k += kPagesThreads)
-                if (*entry_of(k, i) < 0) none = min(none, k);
-        }
+    // What goes back has to be there (a request that was released before has no entries), so all entries are looked at before one is
+    // moved: none, if the thread's first block that is not there (none of all: all_blocks) is below.
+    const auto decide = [&](int64_t none) {
         if (none < all_blocks) atomicMin(&s_bad, static_cast<uint32_t>(request_of(s_off, none)) * 8 + kBadEntry);
         __syncthreads();
         bad = s_bad;
         ok = bad == 0xFFFFFFFFu;
-    }
-    if (first && tid == 0) {
+    };
+    const auto report = [&]() {
+        if (!first || tid != 0) return;
         if (!ok) {
             const int i = min(static_cast<int>(bad >> 3), a.B - 1);
             const int64_t count = !COUNTS || i < 0 ? 0 : a.count[i];
@@ -195,19 +172,55 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
                         static_cast<uint32_t>(static_cast<uint64_t>(count) >> 32), bad & 7);
         }
         *a.n_free_out = static_cast<int32_t>(!ok ? n_free : RELEASE ? n_free + all_blocks : n_free - all_blocks);
-    }
-    if (RELEASE) {
-        if (!ok) return;
-        if (held) {
+    };
+    // Up to 16 blocks a thread are looked up once, all searches and loads on their way together (those behind the last look at it again).
+    const auto give_back = [&](auto each) __attribute__((always_inline)) {
+        constexpr int U = decltype(each)::value;
+        int32_t *at[U], entry[U], k[U], i[U];
 #pragma unroll
-            for (int u = 0; u < kHeld; u++) {
-                if (tid + u * kPagesThreads >= all_blocks) break;
-                a.free_blocks[place(tid + u * kPagesThreads)] = entry[u];
-                *at[u] = -1;
-            }
-            return;
+        for (int u = 0; u < U; u++) {
+            k[u] = static_cast<int32_t>(min(static_cast<int64_t>(tid + u * kPagesThreads), all_blocks - 1));
+            i[u] = 0;
         }
+        for (int32_t n = a.B; n > 1; n -= n / 2) {  // request_of, step by step for all
+#pragma unroll
+            for (int u = 0; u < U; u++) i[u] += s_off[i[u] + n / 2] <= k[u] ? n / 2 : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) at[u] = row_of(i[u]) + (k[u] - s_off[i[u]]);
+#pragma unroll
+        for (int u = 0; u < U; u++) entry[u] = *at[u];
+        int64_t none = all_blocks;
+#pragma unroll
+        for (int u = U - 1; u >= 0; u--)
+            if (tid + u * kPagesThreads < all_blocks && entry[u] < 0) none = tid + u * kPagesThreads;
+        decide(none);
+        report();
+        if (!ok) return;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (tid + u * kPagesThreads >= all_blocks) break;
+            a.free_blocks[place(tid + u * kPagesThreads)] = entry[u];
+            *at[u] = -1;
+        }
+    };
+    if (RELEASE && ok && all_blocks > 0) {
+        if (all_blocks <= kPagesThreads) return give_back(std::integral_constant<int, 1>{});
+        if (all_blocks <= 4 * kPagesThreads) return give_back(std::integral_constant<int, 4>{});
+        if (all_blocks <= 16 * kPagesThreads) return give_back(std::integral_constant<int, 16>{});
+        // of more, a request is searched for only where the last one's blocks end
+        const auto entry_of = [&](int64_t k, int32_t& i) {
+            if (i + 1 < a.B && k >= s_off[i + 1]) i = request_of(s_off, k);
+            return row_of(i) + (k - s_off[i]);
+        };
+        int64_t none = all_blocks;
         int32_t i = 0;
+        for (int64_t k = tid; k < all_blocks; k += kPagesThreads)
+            if (*entry_of(k, i) < 0) none = min(none, k);
+        decide(none);
+        report();
+        if (!ok) return;
+        i = 0;
         for (int64_t k = tid; k < all_blocks; k += kPagesThreads) {
             int32_t* e = entry_of(k, i);
             a.free_blocks[place(k)] = *e;
@@ -215,6 +228,8 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
         }
         return;
     }
+    report();
+    if (RELEASE) return;
     if (first) {
         for (int64_t k = tid; k < all_blocks; k += kPagesThreads) {
             const int32_t i = request_of(s_off, k);
