@@ -594,7 +594,8 @@ SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q_stride_t, 
  * is off by (2 + |log2 e|) 2^-23 of itself at most; all that follows is f64. ids, starts, past, out, n_out, kept, dropped: int32.
  * work: workspace of work_bytes >= slhip_draft_verify_work_bytes(...) (enough for every smaller batch too), 16-byte aligned; calls that
  * may overlap each need their own. It needs no initialisation and keeps nothing. requests <= 65536, vocab <= 2^24,
- * tokens * ceil(vocab / 4096) < 2^23, requests * ceil(vocab / 4096) < 2^24. out, n_out, kept, dropped and logp overlap no input.
+ * tokens * ceil(vocab / 4096) < 2^23, requests * ceil(vocab / 4096) < 2^24. starts[0] is 0 and starts never falls. out, n_out, kept, dropped and
+ * logp overlap no input, but kept may be past.
  */
 typedef struct slhip_drafts {
     int64_t requests;               /* B */
@@ -623,7 +624,7 @@ SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64_t target_s
  *   y[t] = add[t] where adapter[i] is -1.
  * A_a [max_rank, K] and B_a [N, max_rank] (rows dense) lie a_stride and b_stride elements after one another; of adapter a only the
  * first rank[a] ranks count (the others may hold anything). x [T, K] f32 or bf16 (dtype_x), add and y [T, N] (dtype_y), row strides
- * in elements; add may be y (in place: rows without an adapter are then not touched) or NULL (0). Rows from starts[B] on are padding: neither
+ * in elements; add may be y (in place: rows without an adapter are then not touched) or NULL (0); y overlaps nothing else. Rows from starts[B] on are padding: neither
  * read nor written. starts[0] is 0 and starts never falls; starts, adapter and rank are int32 on the device.
  * A x is summed and held in f32 (for bf16 y B takes it in two bf16 parts, to 2^-17 of itself); y is rounded once. A row
  * that holds an infinity or a NaN gives no finite values; no other row's change.
@@ -632,7 +633,7 @@ SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64_t target_s
  * work: workspace of work_bytes >= slhip_lora_work_bytes(tokens, max_rank) (enough for fewer tokens and ranks too), 16-byte
  * aligned; calls that may overlap each need their own. It needs no initialisation and keeps nothing.
  * max_rank <= 256, K and N 8 .. 2^24, a matrix of an adapter less than 2^31 bytes, strides of add and y
- * below 2^30, requests <= 4096. Any alignment; rows and adapters of 16-byte steps are fastest.
+ * below 2^30, requests <= 4096, tokens < 2^31 - 2^17. Any alignment; rows and adapters of 16-byte steps are fastest.
  */
 typedef struct slhip_lora_set {
     int32_t dtype; /* of a and b: F32, F16 or BF16 */

@@ -29,6 +29,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kMaxRank = 256;
 constexpr int kMaxRequests = 4096;
+constexpr int64_t kMaxRows = 0x7FFFFFFF - 32 * kMaxRequests;  // the places of their tiles are 32 bits
 constexpr int kUnit = 64;          // inputs that a wave takes together: a line of 16-bit rows
 constexpr int kMostSplits = 16;
 constexpr int64_t kSplitRows = 65536;  // rows times ranges are at most so many, or the rows
@@ -735,7 +736,7 @@ using namespace slhip;
 
 extern "C" SLHIP_API int64_t slhip_lora_work_bytes(int64_t tokens, int64_t max_rank)
 {
-    if (tokens < 0 || tokens > 0x7FFFFFFFll - 65536 || max_rank < 1 || max_rank > kMaxRank) {
+    if (tokens < 0 || tokens > kMaxRows || max_rank < 1 || max_rank > kMaxRank) {
         fail(SLHIP_ERR_INVALID, "lora: bad size");
         return -1;
     }
@@ -757,7 +758,7 @@ extern "C" SLHIP_API int slhip_lora(int dtype_x, int dtype_y, const void* x, int
     if (set->max_rank > kMaxRank) return fail(SLHIP_ERR_UNSUPPORTED, "lora: more than %d ranks", kMaxRank);
     if (rows->requests > kMaxRequests) return fail(SLHIP_ERR_UNSUPPORTED, "lora: more than %d requests", kMaxRequests);
     const int64_t widest = (set->K > set->N ? set->K : set->N) * set->max_rank * (set->dtype == SLHIP_F32 ? 4 : 2);
-    if (set->adapters > 0x7FFFFFFF || widest > 0x7FFFFFFF || set->K > (1 << 24) || set->N > (1 << 24) || rows->tokens > 0x7FFFFFFFll - 65536)
+    if (set->adapters > 0x7FFFFFFF || widest > 0x7FFFFFFF || set->K > (1 << 24) || set->N > (1 << 24) || rows->tokens > kMaxRows)
         return fail(SLHIP_ERR_UNSUPPORTED, "lora: too many adapters, inputs, outputs or rows (a matrix of an adapter has less than 2^31 bytes)");
     if (x_stride < set->K || y_stride < set->N || (add && add_stride < set->N))
         return fail(SLHIP_ERR_INVALID, "lora: a row stride is smaller than the row");

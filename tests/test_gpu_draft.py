@@ -335,6 +335,28 @@ def test_captured_and_replayed(device):
         del g
 
 
+@pytest.mark.parametrize("B", [5, 700])
+@pytest.mark.parametrize("drawn", [True, False])
+def test_lengths_in_place(device, drawn, B):
+    """kept is past: a step's lengths become the next one's; a request that does not fit keeps its own."""
+    c = Case("lengths", ([3, 1, 4, 2, 3] * 140)[:B], 300, "f32", drawn, extra=0)
+    with Dev() as d:
+        (dt, target, draft, dr), more = c.put(d)
+        log(f"draft_verify kept = past B={B} drawn={drawn}")
+        dr.kept = dr.past
+        want = c.statement()
+        native.draft_verify(dt, target, draft, dr, **more)
+        native.synchronize()
+        assert np.array_equal(d.get(dr.past, (B,), np.int32), want[2]) and np.array_equal(d.get(c.at["dropped"], (B,), np.int32), want[3])
+        now = want[2].astype(np.int32)
+        dr.out_stride = 3  # the requests of four rows do not fit
+        native.draft_verify(dt, target, draft, dr, **more)
+        with pytest.raises(native.SlhipCacheError, match="does not fit"):
+            native.synchronize()
+        n_out = np.where(np.diff(c.starts) > 3, 0, want[1])
+        assert np.array_equal(d.get(dr.past, (B,), np.int32), now + n_out)
+
+
 def test_two_streams_at_once(device):
     with Dev() as d:
         cases = [Case(f"stream{i}", [4, 2, 5], 40000, "f32", True) for i in range(2)]

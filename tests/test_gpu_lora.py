@@ -290,6 +290,35 @@ def test_captured_and_replayed_with_other_requests(device):
         del g
 
 
+def test_captured_lists_of_tiles(device):
+    """More than 64 requests in a captured step: it replays with other adapters, lengths and numbers of tiles."""
+    rng = rng_of("graph of lists")
+    B, T = 100, 260
+    st = native.Stream()
+    with Dev() as d:
+        c = Case("lists", [1] * B, [0] * B, 40, 16, 128, 192, "bf16", "bf16", "bf16", padding=T - B)
+        args, more = c.put(d)
+        log("lora capture, 100 requests")
+        g = native.Graph(st, lambda: native.lora(*args, **more, stream=st.handle))
+        for rep in range(6):
+            new = rng.integers(0, 4, B) if rep % 3 else np.full(B, 1)
+            if rep == 4:
+                new[:] = 0
+                new[77] = T
+            while new.sum() > T:
+                new[rng.integers(0, B)] = 0
+            adapter = rng.integers(-1, [40, 2, 1][rep % 3], B)
+            c.starts, c.adapter = np.concatenate([[0], np.cumsum(new)]).astype(np.int32), adapter.astype(np.int32)
+            for p, v in ((args[6].starts, c.starts), (args[6].adapter, c.adapter), (args[4], c.before)):
+                native.call("slhip_memcpy_h2d", p, v.ctypes.data, v.nbytes, st.handle)
+            st.sync()
+            log(f"lora replay {rep}: {int(new.sum())} rows")
+            g.launch(st)
+            st.sync()
+            c.check(d)
+        del g
+
+
 def test_two_streams_at_once(device):
     """Calls that overlap, each with its workspace; and the results do not change from call to call."""
     with Dev() as d:

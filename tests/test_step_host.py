@@ -69,6 +69,8 @@ def _rows(**kw):
     (dict(b_stride=255), {}, {}, ValueError, "adapter stride"), ({}, {}, dict(work=None), ValueError, "workspace"),
     ({}, {}, dict(work=FAKE + 4), ValueError, "workspace"), ({}, {}, dict(work_bytes=64), ValueError, "workspace"),
     ({}, {}, dict(add=FAKE, y=FAKE, y_stride=40), ValueError, "another stride"),
+    ({}, {}, dict(y_stride=1 << 30), NotImplementedError, "2\\^30"), ({}, {}, dict(add_stride=1 << 30), NotImplementedError, "2\\^30"),
+    ({}, dict(tokens=(1 << 31) - (1 << 17)), {}, NotImplementedError, "too many"),
 ])
 def test_lora_refusals(sets, rows, call, error, match):
     a = dict(dtype_x="f32", dtype_y="f32", x=FAKE, add=FAKE, y=FAKE + 4096, work=FAKE, work_bytes=1 << 40)
