@@ -19,9 +19,10 @@
 namespace slhip {
 
 constexpr int kThreads = 256, kWaves = 4;
-constexpr int kVecs = 4;  // 16-byte vectors of a thread: a chunk is 16 KB
+constexpr int kDrawThreads = 1024, kDrawWaves = 16;  // of what follows the rows' sums: few thread blocks, so a latency
+constexpr int kChunkVecs = 1024;                     // 16-byte vectors of a chunk: 16 KB
 constexpr int64_t kMaxVocab = 1 << 24;
-template <int DT> constexpr int kChunk = kThreads * kVecs * Vec<DT>::N;  // logits of a chunk
+template <int DT> constexpr int kChunk = kChunkVecs * Vec<DT>::N;  // logits of a chunk
 
 struct ChunkStat {
     float m;      // the largest logit; NaN where the chunk holds a NaN or an infinity above
@@ -71,12 +72,12 @@ __device__ __forceinline__ Heat heat_of(const float* tau, int32_t i)
     return h;
 }
 
-// A thread's logits of a chunk: vectors of 16 bytes, a block's threads side by side, in the order of the vocabulary from one step
+// A thread's logits of a chunk: vectors of 16 bytes, a block's TH threads side by side, in the order of the vocabulary from one step
 // to the next. Places past the vocabulary are -inf.
-template <int DT> struct Logits {
-    static constexpr int N = Vec<DT>::N, kEach = kVecs * N;
+template <int DT, int TH> struct Logits {
+    static constexpr int N = Vec<DT>::N, kVecs = kChunkVecs / TH, kEach = kVecs * N;
     uint4 w[kVecs];
-    __device__ static __forceinline__ int32_t place(int32_t chunk, int j) { return chunk * kChunk<DT> + (j * kThreads + static_cast<int>(threadIdx.x)) * N; }
+    __device__ static __forceinline__ int32_t place(int32_t chunk, int j) { return chunk * kChunk<DT> + (j * TH + static_cast<int>(threadIdx.x)) * N; }
     __device__ __forceinline__ void load(const void* rows, int64_t row, int64_t stride, int32_t V, int32_t chunk)
     {
         const char* p = static_cast<const char*>(rows) + row * stride * Vec<DT>::BYTES;
@@ -97,7 +98,6 @@ template <int DT> struct Logits {
             }
         }
     }
-    __device__ __forceinline__ void vec(int j, float (&z)[N]) const { Vec<DT>::unpack(w[j], z); }
 };
 
 // v of another lane by a DPP move, 0 where there is none.
@@ -184,11 +184,12 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
     __shared__ float s_m[kWaves];
     __shared__ double s_s[kWaves];
     __shared__ int32_t s_arg[kWaves];
-    constexpr int N = Logits<DT>::N, kMats = DRAFT ? 2 : 1;
+    typedef Logits<DT, kThreads> Mine;
+    constexpr int N = Mine::N, kVecs = Mine::kVecs, kMats = DRAFT ? 2 : 1;
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int64_t item = blockIdx.x, t = item / (a.chunks * kMats);
     const int32_t rest = static_cast<int32_t>(item - t * (a.chunks * kMats)), mat = rest / a.chunks, chunk = rest - mat * a.chunks;
-    Logits<DT> x;
+    Mine x;
     if (mat == 0) x.load(a.target, t, a.zs, a.V, chunk);
     if (t >= a.starts[a.B]) return;
     const int32_t i = row_request(a.starts, a.B, t);
@@ -197,7 +198,7 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
         if (target.greedy || h.greedy || t == a.starts[i + 1] - 1) return;
         x.load(a.draft, t, a.qs, a.V, chunk);
     }
-    float z[Logits<DT>::kEach];
+    float z[Mine::kEach];
 #pragma unroll
     for (int j = 0; j < kVecs; j++) Vec<DT>::unpack(x.w[j], &z[j * N]);
     float m = z[0];
@@ -219,7 +220,7 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
     if (target.greedy) {
 #pragma unroll
         for (int j = kVecs * N - 1; j >= 0; j--)
-            if (z[j] == m) arg = Logits<DT>::place(chunk, j / N) + j % N;
+            if (z[j] == m) arg = Mine::place(chunk, j / N) + j % N;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) arg = min(arg, __shfl_xor(arg, o, 64));
     }
@@ -322,7 +323,7 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
         const bool row = lane < count && mine < n - 1;  // the lane's row has a draft
         const int32_t x = row ? a.ids[s0 + mine + 1] : 0;
         const double u = row ? a.accept[s0 + mine] : 0.0;
-        if (place < n && (mat == 0 || place < n - 1)) {
+        if (group < 16 && place < n && (mat == 0 || place < n - 1)) {
             const int64_t t = s0 + place;
             const int32_t v = place < n - 1 ? a.ids[t + 1] : 0;
             float z = -INFINITY;
@@ -376,9 +377,11 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
             k.mp = p.m;
             k.cp = cp;
             k.ip = 1.0 / p.s;
-            k.mq = q.m;
-            k.cq = cq;
-            k.iq = 1.0 / q.s;
+            if (k.kind == kFromRest) {
+                k.mq = q.m;
+                k.cq = cq;
+                k.iq = 1.0 / q.s;
+            }
             k.px = p.share;
             k.held = SHARES ? (stop - first) * mats : -1;
         }
@@ -396,7 +399,7 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
             raise_error(a.err, kErrKvRequest, static_cast<uint32_t>(i), static_cast<uint32_t>(i), a.past ? static_cast<uint32_t>(a.past[i]) : 0,
                         static_cast<uint32_t>(s1 - s0), static_cast<uint32_t>(static_cast<uint64_t>(s1 - s0) >> 32), 0);
     }
-    for (int64_t j = (n > 0 ? stop + 1 : 0) + tid; j < a.out_stride; j += kThreads) {
+    for (int64_t j = (n > 0 ? stop + 1 : 0) + tid; j < a.out_stride; j += kDrawThreads) {
         out[j] = -1;
         if (logp) logp[j] = 0.0f;
     }
@@ -431,69 +434,58 @@ struct Share {
     }
 };
 
-// The weights of a thread's logits of a chunk, as the pick's kind says, vector by vector: put(j, w).
-template <int DT, class Put> __device__ __forceinline__ void weights(const DraftArgs& a, const Pick& k, int32_t kind, int32_t chunk, const Put& put)
+// The weights of a thread's logits of a chunk, as the pick's kind says.
+template <int DT> __device__ __forceinline__ void weights(const DraftArgs& a, const Pick& k, int32_t kind, int32_t chunk, double (&w)[Vec<DT>::N])
 {
 #pragma clang fp contract(off)  // p - q of equal numbers is 0, not the rounding of a product
-    constexpr int N = Logits<DT>::N;
-    Logits<DT> x, y;
+    constexpr int N = Vec<DT>::N;
+    typedef Logits<DT, kDrawThreads> Mine;
+    static_assert(Mine::kVecs == 1);
+    Mine x, y;
     x.load(a.target, k.row, a.zs, a.V, chunk);
     if (kind == kFromRest) y.load(a.draft, k.row, a.qs, a.V, chunk);
-    const Share p(k.mp, k.cp), q(k.mq, k.cq);
+    float z[N];
+    Vec<DT>::unpack(x.w[0], z);
+    Share(k.mp, k.cp).of(z, w);
 #pragma unroll
-    for (int j = 0; j < kVecs; j++) {
-        float z[N];
-        double w[N];
-        x.vec(j, z);
-        p.of(z, w);
+    for (int e = 0; e < N; e++) w[e] *= k.ip;
+    const int32_t at = Mine::place(chunk, 0);
+    if (kind == kFromOthers) {
 #pragma unroll
-        for (int e = 0; e < N; e++) w[e] *= k.ip;
-        const int32_t at = Logits<DT>::place(chunk, j);
-        if (kind == kFromOthers) {
+        for (int e = 0; e < N; e++) w[e] = at + e == k.token ? 0.0 : w[e];
+    } else if (kind == kFromRest) {
+        double u[N];
+        Vec<DT>::unpack(y.w[0], z);
+        Share(k.mq, k.cq).of(z, u);
 #pragma unroll
-            for (int e = 0; e < N; e++) w[e] = at + e == k.token ? 0.0 : w[e];
-        } else if (kind == kFromRest) {
-            double u[N];
-            y.vec(j, z);
-            q.of(z, u);
-#pragma unroll
-            for (int e = 0; e < N; e++) w[e] = fmax(w[e] - u[e] * k.iq, 0.0);
-        }
-        put(j, w);
+        for (int e = 0; e < N; e++) w[e] = fmax(w[e] - u[e] * k.iq, 0.0);
     }
 }
 
-// The sum over the thread block, in every thread. lds: of this sum alone.
-__device__ __forceinline__ double block_sum(double v, double (&lds)[kWaves])
+// A chunk's sum, in the first thread.
+template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a, const Pick& k, int32_t chunk, double (&lds)[kDrawWaves])
 {
-    v = wave_sum64(v);
-    if ((threadIdx.x & 63) == 0) lds[wave_id()] = v;
-    __syncthreads();
-    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
-}
-
-template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a, const Pick& k, int32_t chunk, double (&lds)[kWaves])
-{
-    double s = 0.0;
-    weights<DT>(a, k, k.kind, chunk, [&](int, const double (&w)[Logits<DT>::N]) __attribute__((always_inline)) {
+    double w[Vec<DT>::N], s = 0.0;
+    weights<DT>(a, k, k.kind, chunk, w);
 #pragma unroll
-        for (int e = 0; e < Logits<DT>::N; e++) s += w[e];
-    });
-    return block_sum(s, lds);
+    for (int e = 0; e < Vec<DT>::N; e++) s += w[e];
+    s = wave_sum64(s);
+    if ((threadIdx.x & 63) == 0) lds[wave_id()] = s;
+    __syncthreads();
+    return row_sum64(lds[threadIdx.x & (kDrawWaves - 1)]);
 }
 
 // The draw itself, by the whole block. Chunk c's weight is sums[c], or where there are none p's, of the target's chunk sums: of the chunk that
 // holds the refused draft without that. (Which is off by 2^-24 of the draft's p at most, as are the sums themselves.)
+// Every wave finds the chunk for itself, a lane for one or more neighbours, and all of them the place in it, 16 bytes a thread.
 template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32_t i, const Pick& k, const double* sums, const double* shares)
 {
-    constexpr int N = Logits<DT>::N;
-    __shared__ double s_total[kWaves], s_up[2][kWaves], s_part[kVecs][kWaves], s_before;
-    __shared__ int32_t s_chunk, s_last, s_place;
+    constexpr int N = Vec<DT>::N;
+    __shared__ double s_part[kDrawWaves];
+    __shared__ int32_t s_place[kDrawWaves], s_last[kDrawWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const ChunkStat* st = a.stats + static_cast<int64_t>(k.row) * 2 * a.chunks;
     const float u = a.sample[i];
-    if (tid == 0) s_chunk = s_place = 0x7FFFFFFF;
-    if (tid == 0) s_last = 0;
     int32_t kind = k.kind;
     const int32_t other = kind == kFromOthers && k.token >= 0 && k.token < a.V ? k.token / kChunk<DT> : -1;
     const auto target = [&](int32_t c) {
@@ -501,87 +493,81 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
         const ChunkStat x = st[c];
         return x.m > -INFINITY ? x.s * exp2_64((static_cast<double>(x.m) - k.mp) * k.cp) * k.ip : 0.0;
     };
-    const auto weight = [&](int32_t c) { return c >= a.chunks ? 0.0 : sums ? sums[c] : c == other ? fmax(target(c) - k.px, 0.0) : target(c); };
-    const double first = weight(tid);  // of the thread's first chunk, mostly the only one
-    double mine = first;
-    for (int32_t c = tid + kThreads; c < a.chunks; c += kThreads) mine += weight(c);
-    double total = block_sum(mine, s_total);
-    const bool none = !(total > 0.0);  // p and q are equal, or the draft has all of p: p
-    if (none) {
-        kind = kFromTarget;
-        mine = 0.0;
-        for (int32_t c = tid; c < a.chunks; c += kThreads) mine += target(c);
-        __syncthreads();
-        total = block_sum(mine, s_total);
-    }
-    const double r = total * (u > 0.0f ? u : 0.0f);
-    // the chunk: the first whose inclusive sum is above r, or the last one with a weight
-    double base = 0.0;
-    int32_t chunk = 0x7FFFFFFF;
-    for (int32_t c0 = 0, turn = 0; c0 < a.chunks && chunk == 0x7FFFFFFF; c0 += kThreads, turn ^= 1) {
-        const int32_t c = c0 + tid;
-        const double v = c >= a.chunks ? 0.0 : none ? target(c) : c0 == 0 ? first : weight(c);
-        double up = wave_scan64(v);
-        if (lane == 63) s_up[turn][wave] = up;
-        __syncthreads();
-        for (int w = 0; w < kWaves; w++) {
-            if (w == wave) up += base;
-            base += s_up[turn][w];
-        }
-        const uint64_t some = __ballot(v > 0.0), above = __ballot(v > 0.0 && up > r);
-        if (lane == 0 && some) atomicMax(&s_last, c + 63 - __clzll(static_cast<long long>(some)));
-        if (lane == 0 && above) atomicMin(&s_chunk, c + __ffsll(static_cast<long long>(above)) - 1);
-        __syncthreads();
-        chunk = s_chunk;
-        if (c == chunk) s_before = up - v;
-    }
-    __syncthreads();
-    const bool end = chunk == 0x7FFFFFFF;  // rounding: the last weight of all
-    if (end) chunk = s_last;
-    base = end ? 0.0 : s_before;
-    __syncthreads();
-    if (tid == 0) s_last = 0;
-    double w[kVecs][N], up[kVecs];
-    weights<DT>(a, k, kind, chunk, [&](int j, const double (&v)[N]) __attribute__((always_inline)) {
+    const auto weight = [&](int32_t c) {
+        if (kind == kFromTarget) return target(c);
+        if (sums) return sums[c];
+        const double v = target(c), rest = v - k.px;
+        return c != other ? v : rest > 0x1p-40 * v ? rest : 0.0;  // (the roundings of a draft that is alone there are no weight)
+    };
+    const int32_t each = (a.chunks + 63) / 64, c0 = min(lane * each, a.chunks), c1 = min(c0 + each, a.chunks);
+    const auto sum_of = [&]() {
         double s = 0.0;
-#pragma unroll
-        for (int e = 0; e < N; e++) {
-            w[j][e] = v[e];
-            s += v[e];
-        }
-        up[j] = wave_scan64(s);
-        if (lane == 63) s_part[j][wave] = up[j];
-        up[j] -= s;
-    });
-    __syncthreads();
-    int32_t last = -1, place = 0x7FFFFFFF;
-#pragma unroll
-    for (int j = 0; j < kVecs; j++) {
-        double c = base;
-        for (int v = 0; v < kWaves; v++) {
-            if (v == wave) c = base + up[j];
-            base += s_part[j][v];
-        }
-        const int32_t at = Logits<DT>::place(chunk, j);
-#pragma unroll
-        for (int e = 0; e < N; e++) {
-            c += w[j][e];
-            if (w[j][e] > 0.0) {
-                last = at + e;
-                if (c > r && place == 0x7FFFFFFF) place = at + e;
+        for (int32_t c = c0; c < c1; c++) s += weight(c);
+        return s;
+    };
+    double mine = sum_of(), up = wave_scan64(mine);
+    if (!(lane64(up, 63) > 0.0)) {  // p and q are equal, or the draft has all of p: p
+        kind = kFromTarget;
+        mine = sum_of();
+        up = wave_scan64(mine);
+    }
+    const double r = lane64(up, 63) * (u > 0.0f ? u : 0.0f);
+    // the chunk: the first whose inclusive sum is above r, or the last one with a weight
+    const uint64_t some = __ballot(mine > 0.0), above = __ballot(mine > 0.0 && up > r);
+    const bool end = !above;  // rounding: the last weight of all
+    const int from = above ? __ffsll(static_cast<long long>(above)) - 1 : some ? 63 - __clzll(static_cast<long long>(some)) : 0;
+    double base = lane64(up - mine, from);
+    int32_t chunk = min(from * each, a.chunks - 1);
+    if (each > 1) {
+        double sum = base;
+        for (int32_t c = chunk, last = min(chunk + each, a.chunks); c < last; c++) {
+            const double v = weight(c);
+            if (v > 0.0) {
+                base = sum;
+                chunk = c;
             }
+            sum += v;
+            if (!end && v > 0.0 && sum > r) break;
         }
     }
+    double w[N], s = 0.0;
+    weights<DT>(a, k, kind, chunk, w);
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        last = max(last, __shfl_xor(last, o, 64));
-        place = min(place, __shfl_xor(place, o, 64));
+    for (int e = 0; e < N; e++) s += w[e];
+    double c = wave_scan64(s);
+    if (lane == 63) s_part[wave] = c;
+    c -= s;
+    __syncthreads();
+    {  // the waves before
+        const double v = s_part[lane & (kDrawWaves - 1)];
+        c += base + row_sum64((lane & (kDrawWaves - 1)) < wave ? v : 0.0);
     }
-    if (lane == 0 && last >= 0) atomicMax(&s_last, last);
-    if (lane == 0) atomicMin(&s_place, place);
+    const int32_t at = Logits<DT, kDrawThreads>::place(chunk, 0);
+    int32_t last = -1, place = -1;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        c += w[e];
+        if (w[e] > 0.0) {
+            last = at + e;
+            if (c > r && place < 0) place = at + e;
+        }
+    }
+    const uint64_t found = __ballot(place >= 0), held = __ballot(last >= 0);
+    if (lane == 0) {
+        s_place[wave] = -1;
+        s_last[wave] = -1;
+    }
+    if (found && lane == __ffsll(static_cast<long long>(found)) - 1) s_place[wave] = place;
+    if (held && lane == 63 - __clzll(static_cast<long long>(held))) s_last[wave] = last;
     __syncthreads();
     if (tid == 0) {
-        const int32_t token = !end && s_place != 0x7FFFFFFF ? s_place : s_last;
+        int32_t token = -1;
+        last = 0;
+        for (int v = 0; v < kDrawWaves; v++) {
+            if (token < 0) token = s_place[v];
+            last = max(last, s_last[v]);
+        }
+        if (end || token < 0) token = last;
         a.out[i * a.out_stride + k.place] = token;
         if (a.logp)
             a.logp[i * a.out_stride + k.place] =
@@ -590,7 +576,7 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
 }
 
 // Drafts that were chosen, or none: the sums of p are there, a thread block a request does the rest.
-template <int DT> __global__ __launch_bounds__(kThreads) void draft_choose(DraftArgs a)
+template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_choose(DraftArgs a)
 {
     __shared__ DecideLds lds;
     const Pick k = decide<DT, true>(a, blockIdx.x, true, lds);
@@ -599,7 +585,7 @@ template <int DT> __global__ __launch_bounds__(kThreads) void draft_choose(Draft
 
 // Drafts that were drawn: what is accepted, then a thread block for each chunk of the row that is drawn from. Few chunks in all (kDecides) are
 // a latency: each then decides for itself, in one launch.
-template <int DT> __global__ __launch_bounds__(kThreads) void draft_decide(DraftArgs a)
+template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_decide(DraftArgs a)
 {
     __shared__ DecideLds lds;
     const Pick k = decide<DT, false>(a, blockIdx.x, true, lds);
@@ -608,9 +594,9 @@ template <int DT> __global__ __launch_bounds__(kThreads) void draft_decide(Draft
 
 constexpr int64_t kDecides = 512;
 
-template <int DT, bool DECIDES> __global__ __launch_bounds__(kThreads) void draft_sums(DraftArgs a)
+template <int DT, bool DECIDES> __global__ __launch_bounds__(kDrawThreads) void draft_sums(DraftArgs a)
 {
-    __shared__ double s_sum[kWaves];
+    __shared__ double s_sum[kDrawWaves];
     const int32_t i = blockIdx.x / a.chunks, chunk = blockIdx.x - i * a.chunks;
     Pick k;
     if constexpr (DECIDES) {
@@ -625,7 +611,7 @@ template <int DT, bool DECIDES> __global__ __launch_bounds__(kThreads) void draf
     if (threadIdx.x == 0) a.sums[static_cast<int64_t>(i) * a.chunks + chunk] = s;
 }
 
-template <int DT> __global__ __launch_bounds__(kThreads) void draft_pick(DraftArgs a)
+template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_pick(DraftArgs a)
 {
     const Pick k = a.picks[blockIdx.x];
     if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, k.kind == kFromRest ? a.sums + static_cast<int64_t>(blockIdx.x) * a.chunks : nullptr, nullptr);
@@ -664,20 +650,20 @@ template <int DT> static int launch(DraftArgs& a, hipStream_t st)
         if (e) return e;
     }
     if (!a.draft) {
-        draft_choose<DT><<<B, kThreads, 0, st>>>(a);
+        draft_choose<DT><<<B, kDrawThreads, 0, st>>>(a);
         return check_launch("draft_choose");
     }
     if (static_cast<int64_t>(B) * a.chunks <= kDecides) {
-        draft_sums<DT, true><<<B * a.chunks, kThreads, 0, st>>>(a);
+        draft_sums<DT, true><<<B * a.chunks, kDrawThreads, 0, st>>>(a);
     } else {
-        draft_decide<DT><<<B, kThreads, 0, st>>>(a);
+        draft_decide<DT><<<B, kDrawThreads, 0, st>>>(a);
         const int e = check_launch("draft_decide");
         if (e) return e;
-        draft_sums<DT, false><<<B * a.chunks, kThreads, 0, st>>>(a);
+        draft_sums<DT, false><<<B * a.chunks, kDrawThreads, 0, st>>>(a);
     }
     const int e = check_launch("draft_sums");
     if (e) return e;
-    draft_pick<DT><<<B, kThreads, 0, st>>>(a);
+    draft_pick<DT><<<B, kDrawThreads, 0, st>>>(a);
     return check_launch("draft_pick");
 }
 
