@@ -9,9 +9,15 @@
 // of a request's sums. The sums of p's chunks are there already; those of max(p - q, 0) take that one row of both a second time. The
 // place in a chunk takes it once more.
 //
-// Numbers. A choice changes where a sum passes a random number, so what two implementations may differ in is kept small: chunk
-// sums are f32 exponentials of arguments with one rounding (log2(e) / tau in two parts, or all terms of a sum would be off the same
-// way), everything behind them f64: the rows' sums, p(x), q(x), and the drawn row's weights, whose differences p - q cancel.
+// Numbers. A choice changes where a sum passes a random number, so what two implementations may differ in is kept small:
+// exponentials are f32 of arguments with one rounding (log2(e) / tau in two parts, or all terms of a sum would be off the same
+// way), a chunk's are added in f32, everything behind them in f64: the rows' sums, p(x), q(x), and the weights drawn from, whose differences
+// p - q are of f64 exponentials where they may cancel.
+//
+// Measured: the sums of 257 rows of 151936 f32 logits and of 193 draft rows (273 MB) 45.5 us, 6.0 TB/s; of 256 rows of 50257 bf16 logits
+// (25.7 MB) 11.4 us, of which some 3.5 are exponentials that the loads, all on their way at once, do not hide, of 64 rows 5.9. What follows is a
+// latency: 256 or 64 draws 6.9 to 7.2 us in one launch (choose); 64 requests with draft logits 5.4 (decide), 12.8 (2432 chunks of p and q,
+// 78 MB out of the last-level cache) and 6.4 (pick); one request with drafts 6.2 (38 chunks that decide for themselves) and 4.7.
 #include <math.h>
 
 #include "step.hpp"
@@ -242,9 +248,9 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
 
 // ---- what is accepted ----------------------------------------------------------------------------------------------
 
-// A row of a matrix: its maximum and sum, the lowest place of the maximum, whether it can be used; and its draft's logit and share.
+// A row of a matrix: its maximum, its sum and 1 / sum, the lowest place of the maximum, whether it can be used; and its draft's logit and share.
 struct RowStat {
-    double m, s, share;
+    double m, s, inv, share;
     int32_t arg;
     bool fine;
     float z;
@@ -332,7 +338,8 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
             RowStat r = row_stat(a.stats + (t * 2 + mat) * a.chunks, a.chunks, c, hp.greedy, SHARES ? lds.shares[group] : nullptr);
             r.fine &= !(mat ? hq.bad : hp.bad);
             r.z = z;
-            r.share = share_of(z, r.m, c) / r.s;
+            r.inv = 1.0 / r.s;
+            r.share = share_of(z, r.m, c) * r.inv;
             if ((tid & 15) == 0) lds.row[group] = r;
         }
         __syncthreads();
@@ -376,11 +383,11 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
             k.kind = last ? kFromTarget : !drawn ? kFromOthers : q.fine ? kFromRest : kFromTarget;
             k.mp = p.m;
             k.cp = cp;
-            k.ip = 1.0 / p.s;
+            k.ip = p.inv;
             if (k.kind == kFromRest) {
                 k.mq = q.m;
                 k.cq = cq;
-                k.iq = 1.0 / q.s;
+                k.iq = q.inv;
             }
             k.px = p.share;
             k.held = SHARES ? (stop - first) * mats : -1;
@@ -408,14 +415,15 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
 
 // ---- the draw ------------------------------------------------------------------------------------------------------
 
-// e^((z - m) / tau): as f32 where it is below 2^-6 (its roundings are then below those of the sums), f64 above, where p - q may cancel.
-// (A vector of four takes 160 instructions more for f64: with a border of 2^-12 the sums of 38 chunks took 8 us.)
+// e^((z - m) / tau): as f32, like the sums; where p - q may cancel (exact), f64 above 2^-6. (Below, f32's roundings are below those of the
+// sums. A vector of four takes 160 instructions more for f64: with a border of 2^-12 the sums of 38 chunks took 8 us instead of 6.2; with f64 for
+// p alone 256 draws 8.0 us instead of 6.9.)
 struct Share {
     double m, c;
     float mf;
     Factor f;
     __device__ __forceinline__ Share(double m_, double c_) : m(m_), c(c_), mf(static_cast<float>(m_)), f(c_) {}
-    template <int N> __device__ __forceinline__ void of(const float (&z)[N], double (&w)[N]) const
+    template <int N> __device__ __forceinline__ void of(const float (&z)[N], bool exact, double (&w)[N]) const
     {
         float e[N], most = 0.0f;
 #pragma unroll
@@ -424,7 +432,7 @@ struct Share {
             most = fmaxf(most, e[j]);
             w[j] = e[j];
         }
-        if (__any(most > 0x1p-6f)) {
+        if (exact && __any(most > 0x1p-6f)) {
 #pragma unroll
             for (int j = 0; j < N; j++) {  // (all of them: a lane's powers take turns then)
                 const double v = exp2_64((static_cast<double>(z[j]) - m) * c);
@@ -434,39 +442,47 @@ struct Share {
     }
 };
 
-// The weights of a thread's logits of a chunk, as the pick's kind says.
-template <int DT> __device__ __forceinline__ void weights(const DraftArgs& a, const Pick& k, int32_t kind, int32_t chunk, double (&w)[Vec<DT>::N])
-{
-#pragma clang fp contract(off)  // p - q of equal numbers is 0, not the rounding of a product
-    constexpr int N = Vec<DT>::N;
+// A thread's 16 bytes of a chunk, and their weights as the kind says.
+template <int DT> struct Draws {
+    static constexpr int N = Vec<DT>::N;
     typedef Logits<DT, kDrawThreads> Mine;
     static_assert(Mine::kVecs == 1);
     Mine x, y;
-    x.load(a.target, k.row, a.zs, a.V, chunk);
-    if (kind == kFromRest) y.load(a.draft, k.row, a.qs, a.V, chunk);
-    float z[N];
-    Vec<DT>::unpack(x.w[0], z);
-    Share(k.mp, k.cp).of(z, w);
-#pragma unroll
-    for (int e = 0; e < N; e++) w[e] *= k.ip;
-    const int32_t at = Mine::place(chunk, 0);
-    if (kind == kFromOthers) {
-#pragma unroll
-        for (int e = 0; e < N; e++) w[e] = at + e == k.token ? 0.0 : w[e];
-    } else if (kind == kFromRest) {
-        double u[N];
-        Vec<DT>::unpack(y.w[0], z);
-        Share(k.mq, k.cq).of(z, u);
-#pragma unroll
-        for (int e = 0; e < N; e++) w[e] = fmax(w[e] - u[e] * k.iq, 0.0);
+    __device__ __forceinline__ void load(const DraftArgs& a, const Pick& k, int32_t kind, int32_t chunk)
+    {
+        x.load(a.target, k.row, a.zs, a.V, chunk);
+        if (kind == kFromRest) y.load(a.draft, k.row, a.qs, a.V, chunk);
     }
-}
+    __device__ __forceinline__ void logits(float (&z)[N]) const { Vec<DT>::unpack(x.w[0], z); }
+    __device__ __forceinline__ void weights(const Pick& k, int32_t kind, int32_t chunk, double (&w)[N]) const
+    {
+#pragma clang fp contract(off)  // p - q of equal numbers is 0, not the rounding of a product
+        float z[N];
+        logits(z);
+        Share(k.mp, k.cp).of(z, kind == kFromRest, w);
+#pragma unroll
+        for (int e = 0; e < N; e++) w[e] *= k.ip;
+        const int32_t at = Mine::place(chunk, 0);
+        if (kind == kFromOthers) {
+#pragma unroll
+            for (int e = 0; e < N; e++) w[e] = at + e == k.token ? 0.0 : w[e];
+        } else if (kind == kFromRest) {
+            double u[N];
+            Vec<DT>::unpack(y.w[0], z);
+            Share(k.mq, k.cq).of(z, true, u);
+#pragma unroll
+            for (int e = 0; e < N; e++) w[e] = fmax(w[e] - u[e] * k.iq, 0.0);
+        }
+    }
+};
 
 // A chunk's sum, in the first thread.
 template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a, const Pick& k, int32_t chunk, double (&lds)[kDrawWaves])
 {
     double w[Vec<DT>::N], s = 0.0;
-    weights<DT>(a, k, k.kind, chunk, w);
+    Draws<DT> mine;
+    mine.load(a, k, k.kind, chunk);
+    mine.weights(k, k.kind, chunk, w);
 #pragma unroll
     for (int e = 0; e < Vec<DT>::N; e++) s += w[e];
     s = wave_sum64(s);
@@ -478,14 +494,14 @@ template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a
 // The draw itself, by the whole block. Chunk c's weight is sums[c], or where there are none p's, of the target's chunk sums: of the chunk that
 // holds the refused draft without that. (Which is off by 2^-24 of the draft's p at most, as are the sums themselves.)
 // Every wave finds the chunk for itself, a lane for one or more neighbours, and all of them the place in it, 16 bytes a thread.
-template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32_t i, const Pick& k, const double* sums, const double* shares)
+template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32_t i, const Pick& k, float u, const double* sums, const double* shares)
 {
     constexpr int N = Vec<DT>::N;
     __shared__ double s_part[kDrawWaves];
     __shared__ int32_t s_place[kDrawWaves], s_last[kDrawWaves];
+    __shared__ float s_place_z[kDrawWaves], s_last_z[kDrawWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const ChunkStat* st = a.stats + static_cast<int64_t>(k.row) * 2 * a.chunks;
-    const float u = a.sample[i];
     int32_t kind = k.kind;
     const int32_t other = kind == kFromOthers && k.token >= 0 && k.token < a.V ? k.token / kChunk<DT> : -1;
     const auto target = [&](int32_t c) {
@@ -531,7 +547,12 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
         }
     }
     double w[N], s = 0.0;
-    weights<DT>(a, k, kind, chunk, w);
+    float z[N];
+    Draws<DT> of;
+    of.load(a, k, kind, chunk);
+    const double log_s = a.logp && wave == 0 ? log(k.ip) : 0.0;  // while the loads are on their way
+    of.logits(z);
+    of.weights(k, kind, chunk, w);
 #pragma unroll
     for (int e = 0; e < N; e++) s += w[e];
     double c = wave_scan64(s);
@@ -544,43 +565,49 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
     }
     const int32_t at = Logits<DT, kDrawThreads>::place(chunk, 0);
     int32_t last = -1, place = -1;
+    float last_z = 0.0f, place_z = 0.0f;
 #pragma unroll
     for (int e = 0; e < N; e++) {
         c += w[e];
         if (w[e] > 0.0) {
             last = at + e;
-            if (c > r && place < 0) place = at + e;
+            last_z = z[e];
+            if (c > r && place < 0) {
+                place = last;
+                place_z = last_z;
+            }
         }
     }
-    const uint64_t found = __ballot(place >= 0), held = __ballot(last >= 0);
-    if (lane == 0) {
-        s_place[wave] = -1;
-        s_last[wave] = -1;
+    // the first place of the wave's, and its last with a weight
+    const auto lowest = [](uint64_t lanes) { return lanes ? __ffsll(static_cast<long long>(lanes)) - 1 : 0; };
+    const auto highest = [](uint64_t lanes) { return lanes ? 63 - __clzll(static_cast<long long>(lanes)) : 0; };
+    if (lane == lowest(__ballot(place >= 0))) {
+        s_place[wave] = place;
+        s_place_z[wave] = place_z;
     }
-    if (found && lane == __ffsll(static_cast<long long>(found)) - 1) s_place[wave] = place;
-    if (held && lane == 63 - __clzll(static_cast<long long>(held))) s_last[wave] = last;
+    if (lane == highest(__ballot(last >= 0))) {
+        s_last[wave] = last;
+        s_last_z[wave] = last_z;
+    }
     __syncthreads();
-    if (tid == 0) {
-        int32_t token = -1;
-        last = 0;
-        for (int v = 0; v < kDrawWaves; v++) {
-            if (token < 0) token = s_place[v];
-            last = max(last, s_last[v]);
-        }
-        if (end || token < 0) token = last;
-        a.out[i * a.out_stride + k.place] = token;
-        if (a.logp)
-            a.logp[i * a.out_stride + k.place] =
-                static_cast<float>((static_cast<double>(Vec<DT>::load1(a.target, k.row * a.zs + token)) - k.mp) * (k.cp / kLog2e64) + log(k.ip));
-    }
+    if (tid >= 64) return;
+    const bool in = lane < kDrawWaves;
+    const uint64_t found = __ballot(in && s_place[lane & (kDrawWaves - 1)] >= 0), held = __ballot(in && s_last[lane & (kDrawWaves - 1)] >= 0);
+    if (lane > 0) return;
+    const bool ends = end || !found;
+    const int from_wave = ends ? highest(held) : lowest(found);
+    const int32_t token = max(ends ? s_last[from_wave] : s_place[from_wave], 0);
+    a.out[i * a.out_stride + k.place] = token;
+    if (a.logp) a.logp[i * a.out_stride + k.place] = static_cast<float>(((ends ? s_last_z : s_place_z)[from_wave] - k.mp) * (k.cp / kLog2e64) + log_s);
 }
 
 // Drafts that were chosen, or none: the sums of p are there, a thread block a request does the rest.
 template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_choose(DraftArgs a)
 {
     __shared__ DecideLds lds;
+    const float u = a.T > 0 ? a.sample[blockIdx.x] : 0.0f;
     const Pick k = decide<DT, true>(a, blockIdx.x, true, lds);
-    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, nullptr, lds.shares[k.held]);
+    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, u, nullptr, lds.shares[k.held]);
 }
 
 // Drafts that were drawn: what is accepted, then a thread block for each chunk of the row that is drawn from. Few chunks in all (kDecides) are
@@ -613,8 +640,9 @@ template <int DT, bool DECIDES> __global__ __launch_bounds__(kDrawThreads) void 
 
 template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_pick(DraftArgs a)
 {
+    const float u = a.T > 0 ? a.sample[blockIdx.x] : 0.0f;
     const Pick k = a.picks[blockIdx.x];
-    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, k.kind == kFromRest ? a.sums + static_cast<int64_t>(blockIdx.x) * a.chunks : nullptr, nullptr);
+    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, u, k.kind == kFromRest ? a.sums + static_cast<int64_t>(blockIdx.x) * a.chunks : nullptr, nullptr);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
