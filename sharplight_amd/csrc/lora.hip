@@ -59,6 +59,24 @@ struct LoraArgs {
     uint32_t* err;
 };
 
+// How many thread blocks share out the columns of all tiles. A tile's beginning (its rows, h) costs a thread block as much as some of its
+// steps. Thread blocks that all run at once are few, with even shares of steps: 32-row tiles' 640 (a prompt of 2048 into 14336 outputs, 16
+// ranks: 520 thread blocks 36 us with the first product, 910 39.7, 3640 43.5; 64 ranks: 520 54 us, 715 with uneven shares 66), 16-row
+// tiles' 512 (64 requests of an adapter each: 512 18.7 us, 2048 22.5). Many steps end more evenly in several rounds of up to 16 ranks (a prompt of 8192
+// into 14336: 2056 114 us, 3855 110; with 64 ranks 514 179 us, 4096 192).
+SLHIP_HD int64_t expand_blocks(int64_t tiles, int64_t cols, int mt, int32_t r16) { return mt == 1 ? 512 : r16 <= 16 && tiles * cols > 4096 ? 4096 : 640; }
+SLHIP_HD int32_t columns_shared(int64_t tiles, int64_t cols, int mt, int32_t r16)
+{
+    const int64_t blocks = expand_blocks(tiles, cols, mt, r16);
+    int64_t most = blocks / tiles;
+    most = most < 1 ? 1 : most > cols ? cols : most;
+    if (blocks != 4096) {
+        const int64_t steps = (cols + most - 1) / most;
+        most = (cols + steps - 1) / steps;
+    }
+    return static_cast<int32_t>(most);
+}
+
 // ---- rows ----------------------------------------------------------------------------------------------------------
 
 constexpr int32_t kNoTile = -2;
@@ -105,7 +123,7 @@ constexpr int kPlanThreads = 1024, kSlots = 2 * kMaxRequests, kEach = kMaxReques
 constexpr int32_t kEmpty = -0x7FFFFFFF;
 constexpr int kPlanLds = (2 * kSlots + kPlanThreads / 64) * 4;
 
-template <int TM> __global__ __launch_bounds__(kPlanThreads) void lora_plan(LoraArgs a, int32_t blocks1, int32_t blocks2)
+template <int TM> __global__ __launch_bounds__(kPlanThreads) void lora_plan(LoraArgs a, int32_t blocks1)
 {
     extern __shared__ int32_t s_slots[];
     int32_t *s_key = s_slots, *s_count = s_slots + kSlots, *s_wave = s_slots + 2 * kSlots;
@@ -179,7 +197,7 @@ template <int TM> __global__ __launch_bounds__(kPlanThreads) void lora_plan(Lora
     }
     if (tid == 0) {  // the tiles share out the thread blocks that there are
         const int32_t some = max(tiles, 1);
-        *a.plan = Plan{tiles, max(min(a.splits, blocks1 / (some * a.rank_blocks)), 1), max(min(a.cols, blocks2 / some), 1), 0};
+        *a.plan = Plan{tiles, max(min(a.splits, blocks1 / (some * a.rank_blocks)), 1), columns_shared(some, a.cols, TM / 16, a.R16), 0};
     }
 }
 
@@ -682,10 +700,10 @@ template <int YT, int WT, int MT> static int expand(const LoraArgs& a, int64_t b
     return check_launch("lora_expand");
 }
 
-template <int MT> static int plan(const LoraArgs& a, int64_t blocks1, int64_t blocks2, hipStream_t st)
+template <int MT> static int plan(const LoraArgs& a, int64_t blocks1, hipStream_t st)
 {
     SLHIP_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&lora_plan<16 * MT>), hipFuncAttributeMaxDynamicSharedMemorySize, kPlanLds));
-    lora_plan<16 * MT><<<1, kPlanThreads, kPlanLds, st>>>(a, static_cast<int32_t>(blocks1), static_cast<int32_t>(blocks2));
+    lora_plan<16 * MT><<<1, kPlanThreads, kPlanLds, st>>>(a, static_cast<int32_t>(blocks1));
     return check_launch("lora_plan");
 }
 
@@ -702,18 +720,13 @@ template <int WT, int MT> static int launch(int dtype_x, int dtype_y, LoraArgs& 
     if (splits > kSplitRows / a.T) splits = kSplitRows / a.T;
     if (!planned && splits > 1024 / (tiles * a.rank_blocks)) splits = 1024 / (tiles * a.rank_blocks);
     a.splits = splits < 1 ? 1 : static_cast<int32_t>(splits);
-    // How many thread blocks share out the columns of all tiles. A tile's beginning (its rows, h) costs a thread block as much as some of its
-    // steps, the more the more ranks there are; many thread blocks end more evenly. (64 requests of an adapter each, 16 ranks, 14336 outputs: 512
-    // thread blocks 18.7 us with the first product, 2048 22.5, 4096 26.9; a prompt of 8192: 512 140 us, 1024 119, 4096 110; of 64 ranks
-    // 768 178, 4096 192.)
-    const int64_t blocks2 = MT == 1 ? 512 : a.R16 <= 16 ? 4096 : 768;
-    const int64_t most = blocks2 / tiles;
-    a.col_blocks = planned || most >= a.cols ? a.cols : most < 1 ? 1 : static_cast<int32_t>(most);
+    a.col_blocks = columns_shared(tiles, a.cols, MT, a.R16);
     int64_t first = tiles * a.splits * a.rank_blocks, second = tiles * a.col_blocks;
     if (planned) {
         if (first > 1024) first = 1024;
-        if (second > blocks2) second = blocks2;
-        const int e = plan<MT>(a, first, second, st);
+        second = tiles * a.cols;  // the most that there could be
+        if (second > expand_blocks(tiles, a.cols, MT, a.R16)) second = expand_blocks(tiles, a.cols, MT, a.R16);
+        const int e = plan<MT>(a, first, st);
         if (e) return e;
     } else {
         a.plan = nullptr;
