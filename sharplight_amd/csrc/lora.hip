@@ -141,7 +141,7 @@ template <int TM> __global__ __launch_bounds__(kPlanThreads) void lora_plan(Lora
     unsigned long long rows_mine = 0;
 #pragma unroll
     for (int e = 0; e < kEach; e++) {
-        const int32_t j = tid + e * kPlanThreads;
+        const int32_t j = lane * (kPlanThreads / 64) + wave + e * kPlanThreads;  // few requests, too, are shared out over the waves
         const bool in = j < a.B;
         s0[e] = in ? a.starts[j] : 0;
         n[e] = in ? rows_of(a, j) : 0;
