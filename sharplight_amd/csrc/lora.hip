@@ -69,8 +69,9 @@ struct LoraArgs {
 // steps. Thread blocks that all run at once are few, with even shares of steps: 32-row tiles' 640 (a prompt of 2048 into 14336 outputs, 16
 // ranks: 520 thread blocks 36 us with the first product, 910 39.7, 3640 43.5; 64 ranks: 520 54 us, 715 with uneven shares 66), 16-row
 // tiles' 512 (64 requests of an adapter each: 512 18.7 us, 2048 22.5). Many steps end more evenly in several rounds of up to 16 ranks (a prompt of 8192
-// into 14336: 2056 114 us, 3855 110; with 64 ranks 514 179 us, 4096 192).
-SLHIP_HD int64_t expand_blocks(int64_t tiles, int64_t cols, int mt, int32_t r16) { return mt == 1 ? 512 : r16 <= 16 && tiles * cols > 4096 ? 4096 : 640; }
+// into 14336: 514 125 us, 3855 110; into 8192: 79 and 73; 4096 into 14336, 7224 steps: 69.5 and 69.8; into 8192: 43 and 52; with 64 ranks
+// 8192 into 14336 take 514 179 us, 4096 192).
+SLHIP_HD int64_t expand_blocks(int64_t tiles, int64_t cols, int mt, int32_t r16) { return mt == 1 ? 512 : r16 <= 16 && tiles * cols > 6144 ? 4096 : 640; }
 SLHIP_HD int32_t columns_shared(int64_t tiles, int64_t cols, int mt, int32_t r16)
 {
     const int64_t blocks = expand_blocks(tiles, cols, mt, r16);
