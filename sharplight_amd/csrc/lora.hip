@@ -339,7 +339,7 @@ template <int DT, int N> struct Run {
 template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads) void lora_shrink(LoraArgs a)
 {
     constexpr int TM = 16 * MT, PX = kParts<XT>, PW = kParts<WT>;
-    constexpr int U = MT * RB == 1 ? 4 : MT == 1 || XT == SLHIP_BF16 ? 2 : 1;  // units whose loads are on their way together
+    constexpr int U = MT * RB == 1 ? 4 : MT * RB == 8 && WT == SLHIP_F32 ? 1 : MT == 1 || XT == SLHIP_BF16 ? 2 : 1;  // units whose loads are on their way together
     __shared__ int32_t s_rows[TM];
     __shared__ f32x4 s_acc[kWaves / 2][MT * RB][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), c = lane & 15, g = lane >> 4;
@@ -543,8 +543,7 @@ template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThrea
 #pragma unroll
         for (int u = 0; u < E; u++) w[u].shift(max(at + u * a.R - last, 0));
     };
-    const auto fetch = [&](int32_t n0) __attribute__((always_inline)) {
-        if (key >= 0) fetch_w(n0, 0);
+    const auto fetch_add = [&](int32_t n0) __attribute__((always_inline)) {
         const char* const at = static_cast<const char*>(a.add) + static_cast<uint32_t>(column(n0)) * Vec<YT>::BYTES;
 #pragma unroll
         for (int m = 0; m < MT; m++)
@@ -555,6 +554,8 @@ template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThrea
                 else add[m][r].w = 0;
             }
     };
+    // thread blocks that run together take neighbouring columns: the same columns of many rows lie in few memory channels
+    const int32_t first = (cb * kWaves + wave) * kColumns, step = col_blocks * kWaves * kColumns;
     const int32_t rank = key < 0 ? 0 : rank_of(a, key), tiles = (rank + RC - 1) / RC, all = (a.R + RC - 1) / RC;
     const auto finish = [&](int32_t n0) __attribute__((always_inline)) {
         f32x4 acc[MT][E];
@@ -568,6 +569,7 @@ template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThrea
 #pragma unroll
             for (int u = 0; u < E; u++) w[u].parts(0, pw[u]);
             if (WIDE && q + 1 < tiles) fetch_w(n0, q + 1);
+            else if (WIDE && n0 + step < a.N) fetch_w(n0 + step, 0);
             bf16x8 x[MT][H];
 #pragma unroll
             for (int m = 0; m < MT; m++)
@@ -614,9 +616,10 @@ template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThrea
                 }
             }
     };
-    // thread blocks that run together take neighbouring columns: the same columns of many rows lie in few memory channels
-    const int32_t first = (cb * kWaves + wave) * kColumns, step = col_blocks * kWaves * kColumns;
-    if (first < a.N) fetch(first);
+    if (first < a.N) {
+        if (key >= 0) fetch_w(first, 0);
+        fetch_add(first);
+    }
     const float scale = key < 0 || !a.scale ? 1.0f : a.scale[key];
     const int32_t splits = a.plan ? a.plan->splits : a.splits;
     // h, ranges of K added up: `parts` lanes share eight ranks of a row
@@ -667,7 +670,10 @@ template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThrea
     }
     __syncthreads();
     for (int32_t n0 = first; n0 < a.N; n0 += step) {
-        if (n0 > first) fetch(n0);
+        if (n0 > first) {
+            if (!WIDE && key >= 0) fetch_w(n0, 0);
+            fetch_add(n0);
+        }
         finish(n0);
     }
     };
@@ -721,11 +727,13 @@ template <int WT, int MT> static int launch(int dtype_x, int dtype_y, LoraArgs& 
     constexpr int64_t wide = kWaves * 16 * kLane;
     a.rank_blocks = a.R16 <= 32 ? 1 : (a.R16 + 63) / 64;
     a.cols = static_cast<int32_t>((a.N + wide - 1) / wide);
-    // ranges of K of 512 inputs at least, as far as they give the machine work
+    // ranges of K of 512 inputs at least, as far as they give the machine work; of 32-row tiles, whose h is more, beyond 8 only for 256 thread blocks
+    // (a prompt of 1500 rows, 64 ranks, 14336 inputs, 13312 outputs: 8 ranges 67.8 us, 16 73.7)
     int64_t splits = a.K / 512;
     if (splits > kMostSplits) splits = kMostSplits;
     if (splits > kSplitRows / a.T) splits = kSplitRows / a.T;
     if (!planned && splits > 1024 / (tiles * a.rank_blocks)) splits = 1024 / (tiles * a.rank_blocks);
+    if (!planned && MT == 2 && splits > 8 && splits * tiles > 256) splits = 256 / tiles > 8 ? 256 / tiles : 8;
     a.splits = splits < 1 ? 1 : static_cast<int32_t>(splits);
     a.col_blocks = columns_shared(tiles, a.cols, MT, a.R16);
     int64_t first = tiles * a.splits * a.rank_blocks, second = tiles * a.col_blocks;
