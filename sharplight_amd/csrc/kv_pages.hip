@@ -75,7 +75,8 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
 {
     constexpr bool RELEASE = OP != kAdvance, COUNTS = OP != kRelease;  // blocks go back; requests have a count
     __shared__ int32_t s_start[kMaxRequests + 1], s_off[kMaxRequests + 1];
-    __shared__ uint32_t s_seen[kMaxSlots / 32];
+    __shared__ uint32_t s_seen[kMaxSlots / 32];  // (of as many words as there are requests at most)
+    static_assert(kMaxSlots / 32 >= kMaxRequests);
     __shared__ int64_t s_wave[2][kPagesThreads / 64];
     __shared__ uint32_t s_bad;  // the first bad request * 8 + what is wrong with it
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
@@ -137,8 +138,13 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     bool ok = bad == 0xFFFFFFFFu;
     if (!ok) all_tokens = all_blocks = 0;
     for (int i = i0; i < i1; i++) {
-        s_start[i] = static_cast<int32_t>(st);
         s_off[i] = static_cast<int32_t>(so);
+        if (RELEASE) {  // block k of all is request i's entry k + s_seen[i] of table row s_start[i]
+            s_start[i] = i == i0 ? slot0 : slot_of(i);
+            s_seen[i] = static_cast<uint32_t>((OP == kTrim ? blocks_of(i == i0 ? past0 : a.past[i], a.shift) : 0) - so);
+        } else {
+            s_start[i] = static_cast<int32_t>(st);
+        }
         if (!RELEASE && first) a.starts[i] = ok ? static_cast<int32_t>(st) : 0;
         if (!ok) continue;
         const int64_t past = i == i0 ? past0 : a.past[i], count = !COUNTS ? 0 : i == i0 ? count0 : a.count[i];
@@ -150,9 +156,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     const auto request_of = [&](const int32_t* sums, int64_t k) {
         return static_cast<int32_t>(item_request([&](int64_t r) { return sums[r]; }, a.B, k, 1, 0));
     };
-    const auto row_of = [&](int32_t i) {  // the first table entry that the request gives back
-        return a.pages + slot_of(i) * a.bps + (OP == kTrim ? blocks_of(a.past[i], a.shift) : 0);
-    };
+    const auto entry_at = [&](int32_t i, int64_t k) { return a.pages + s_start[i] * a.bps + (k + static_cast<int32_t>(s_seen[i])); };
     // where block k of all goes on the stack
     const auto place = [&](int64_t k) { return n_free + (OP == kTrim ? all_blocks - 1 - k : k); };
     // What goes back has to be there (a request that was released before has no entries), so all entries are looked at before one is
@@ -187,7 +191,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
             for (int u = 0; u < U; u++) i[u] += s_off[i[u] + n / 2] <= k[u] ? n / 2 : 0;
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) at[u] = row_of(i[u]) + (k[u] - s_off[i[u]]);
+        for (int u = 0; u < U; u++) at[u] = entry_at(i[u], k[u]);
 #pragma unroll
         for (int u = 0; u < U; u++) entry[u] = *at[u];
         int64_t none = all_blocks;
@@ -211,7 +215,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
         // of more, a request is searched for only where the last one's blocks end
         const auto entry_of = [&](int64_t k, int32_t& i) {
             if (i + 1 < a.B && k >= s_off[i + 1]) i = request_of(s_off, k);
-            return row_of(i) + (k - s_off[i]);
+            return entry_at(i, k);
         };
         int64_t none = all_blocks;
         int32_t i = 0;
