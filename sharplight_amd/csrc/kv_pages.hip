@@ -11,9 +11,10 @@
 // place); a step of many rows then has its rows in a second launch.
 // Measured: 64 requests of a token 4.4 us, 333 requests of 1 to 200 tokens (some 33000 rows) 6.2 us; an empty launch takes 2.5.
 // With kBlockRows = 4096 the latter took 10.4 us, and with the rows in a second launch 10.0. A release is one thread block's too: 64
-// requests of 256 blocks 19 us, of 8192 432.
+// requests of 256 blocks 7.5 us, of 8192 412.
 // A trim is a release that leaves each request's first blocks, and it fills the stack from the other end, so that it undoes an
-// advance. Its few blocks' chain is the release's: lengths -> scan -> table entries -> stores.
+// advance. Its few blocks' chain is the release's: lengths -> scan -> table entries -> stores. 64 requests with up to 4 refused drafts each 3.3 us,
+// 333 that give back 10400 blocks 7.9 (with a search of each block's request in the sums, of ten steps, 10.2).
 #include <type_traits>
 
 #include "common.hpp"
@@ -25,6 +26,7 @@ constexpr int kPagesThreads = 1024;
 constexpr int kMaxRequests = 4096;
 constexpr int kMaxSlots = 131072;
 constexpr int64_t kBlockRows = 1024;
+constexpr int kListed = 16 * kPagesThreads;  // blocks that a release looks up at once
 
 struct KvPagesArgs {
     int32_t B;
@@ -77,6 +79,9 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     __shared__ int32_t s_start[kMaxRequests + 1], s_off[kMaxRequests + 1];
     __shared__ uint32_t s_seen[kMaxSlots / 32];  // (of as many words as there are requests at most)
     static_assert(kMaxSlots / 32 >= kMaxRequests);
+    __shared__ uint32_t s_bits[RELEASE ? kListed / 32 : 1];  // of blocks that go back: a request's first one
+    __shared__ int32_t s_base[RELEASE ? kListed / 32 : 1];   // bits in the words before
+    __shared__ uint16_t s_list[RELEASE ? kMaxRequests : 1];  // the requests of the bits
     __shared__ int64_t s_wave[2][kPagesThreads / 64];
     __shared__ uint32_t s_bad;  // the first bad request * 8 + what is wrong with it
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
@@ -88,6 +93,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     // the thread's first request: most steps have no more than one a thread
     const int32_t past0 = i0 < i1 ? a.past[i0] : 0, count0 = i0 < i1 && COUNTS ? a.count[i0] : 0, slot0 = i0 < i1 ? slot_of(i0) : 0;
     for (int64_t w = tid; w < (a.page_slots + 31) / 32; w += kPagesThreads) s_seen[w] = 0;
+    if (RELEASE && tid < kListed / 32) s_bits[tid] = 0;
     if (tid == 0) s_bad = 0xFFFFFFFFu;
     __syncthreads();
 
@@ -148,8 +154,10 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
         if (!RELEASE && first) a.starts[i] = ok ? static_cast<int32_t>(st) : 0;
         if (!ok) continue;
         const int64_t past = i == i0 ? past0 : a.past[i], count = !COUNTS ? 0 : i == i0 ? count0 : a.count[i];
+        const int64_t blocks_here = moved(past, count);
+        if (RELEASE && blocks_here > 0 && all_blocks <= kListed) atomicOr(&s_bits[so >> 5], 1u << (so & 31));
         st += count;
-        so += moved(past, count);
+        so += blocks_here;
     }
     if (!RELEASE && first && tid == 0) a.starts[a.B] = static_cast<int32_t>(all_tokens);
     __syncthreads();
@@ -186,9 +194,22 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
             k[u] = static_cast<int32_t>(min(static_cast<int64_t>(tid + u * kPagesThreads), all_blocks - 1));
             i[u] = 0;
         }
-        for (int32_t n = a.B; n > 1; n -= n / 2) {  // request_of, step by step for all
+        if (U == 1) {
+            for (int32_t n = a.B; n > 1; n -= n / 2) i[0] += s_off[i[0] + n / 2] <= k[0] ? n / 2 : 0;  // request_of
+        } else {  // a block's request is the one of the last bit up to it: three reads of neighbours, where a search is ten of any
+            const int32_t ones = tid < kListed / 32 ? __popc(s_bits[tid]) : 0;
+            int32_t up = wave_scan(ones);
+            if (lane == 63) s_wave[0][wave] = up;
+            __syncthreads();
+            for (int w = 0; w < wave && w < kListed / 32 / 64; w++) up += static_cast<int32_t>(s_wave[0][w]);
+            if (tid < kListed / 32) s_base[tid] = up - ones;
+            __syncthreads();
+            const auto bit_of = [&](int32_t at) { return s_base[at >> 5] + __popc(s_bits[at >> 5] & (0xFFFFFFFFu >> (31 - (at & 31)))) - 1; };
+            for (int j = i0; j < i1; j++)
+                if ((j + 1 < a.B ? s_off[j + 1] : all_blocks) > s_off[j]) s_list[bit_of(s_off[j])] = static_cast<uint16_t>(j);
+            __syncthreads();
 #pragma unroll
-            for (int u = 0; u < U; u++) i[u] += s_off[i[u] + n / 2] <= k[u] ? n / 2 : 0;
+            for (int u = 0; u < U; u++) i[u] = s_list[bit_of(k[u])];
         }
 #pragma unroll
         for (int u = 0; u < U; u++) at[u] = entry_at(i[u], k[u]);
@@ -211,7 +232,7 @@ __global__ __launch_bounds__(kPagesThreads) void kv_pages_tables(KvPagesArgs a)
     if (RELEASE && ok && all_blocks > 0) {
         if (all_blocks <= kPagesThreads) return give_back(std::integral_constant<int, 1>{});
         if (all_blocks <= 4 * kPagesThreads) return give_back(std::integral_constant<int, 4>{});
-        if (all_blocks <= 16 * kPagesThreads) return give_back(std::integral_constant<int, 16>{});
+        if (all_blocks <= kListed) return give_back(std::integral_constant<int, 16>{});
         // of more, a request is searched for only where the last one's blocks end
         const auto entry_of = [&](int64_t k, int32_t& i) {
             if (i + 1 < a.B && k >= s_off[i + 1]) i = request_of(s_off, k);
