@@ -152,3 +152,35 @@ def test_an_advance_taken_back(device, B):
         assert d.get(n, (1,), np.int32)[0] == n2
         held = p2[p2 >= 0]
         assert len(set(held)) == len(held) and not set(held) & set(f2[:n2])
+
+
+@pytest.mark.parametrize("total", [1, 1023, 1024, 1025, 4096, 4097, 16384, 16385])
+@pytest.mark.parametrize("B", [5, 900, 4096])
+def test_numbers_of_blocks(device, B, total):
+    """Trims and releases of exactly so many blocks, spread over few and many requests, empty ones among them."""
+    rng = rng_of("numbers", B, total)
+    back = np.bincount(rng.choice(np.append(rng.permutation(B)[: B // 2], B - 1), total), minlength=B)
+    keep = rng.integers(0, 3, B)
+    bs, bps = 16, int((back + keep).max()) + 1
+    past = (keep * bs).astype(np.int32)
+    count = (back * bs - np.where(back > 0, rng.integers(0, bs, B), 0)).astype(np.int32)
+    slot = rng.permutation(B + 5)[:B].astype(np.int32)
+    pages = np.full((B + 5, bps), -1, np.int32)
+    ids = iter(rng.permutation(int((back + keep).sum()) + 3).astype(np.int32))
+    for i in range(B):
+        for j in range(int(back[i] + keep[i])):
+            pages[slot[i], j] = next(ids)
+    with Dev() as d:
+        free = np.full(total + 4, -7, np.int32)
+        free[:2] = [next(ids) for _ in range(2)]
+        log(f"kv_pages_trim of {total} blocks, B={B}")
+        p, at = _trim(d, past, count, slot, pages, bs, free, 2)
+        native.kv_pages_trim(p)
+        native.synchronize()
+        assert _check(d, at, step_ref.trim(past, count, slot, pages, bs, free, 2))
+        past = (back * bs - np.where(back > 0, rng.integers(0, bs, B), 0)).astype(np.int32)
+        log(f"kv_pages_release of {total} blocks, B={B}")
+        p, at = _trim(d, past, count, slot, pages, bs, free, 2)
+        native.kv_pages_release(p)
+        native.synchronize()
+        assert _check(d, at, kv8_ref.release(past, slot, pages, bs, free, 2))
