@@ -350,3 +350,31 @@ def test_a_long_prompt(device):
         native.lora(*args, **more)
         native.synchronize()
         c.check(d)
+
+
+@pytest.mark.parametrize("requests", [1, 3, 70])
+def test_many_rows_and_columns(device, requests):
+    """So many column steps that thread blocks take turns; a sample of the rows is compared, in every column."""
+    rng = rng_of("turns", requests)
+    T, K, N, R, padding = 4190, 64, 12540, 16, 6
+    cuts = np.sort(rng.choice(np.arange(1, T - padding), requests - 1, replace=False))
+    starts = np.concatenate([[0], cuts, [T - padding]]).astype(np.int32)
+    adapter = rng.integers(0, 2, requests).astype(np.int32)
+    x, vx = held(rng.standard_normal((T, K)), "bf16")
+    a, va = held(rng.standard_normal((2, R, K)) / np.sqrt(K), "bf16")
+    b, vb = held(rng.standard_normal((2, N, R)) / np.sqrt(R), "bf16")
+    add = oracle.to_bf16(rng.standard_normal((T, N), dtype=np.float32))
+    with Dev() as d:
+        at = d.put(add)
+        size = native.lora_work_bytes(T, R)
+        log(f"lora T={T} N={N} requests={requests}")
+        native.lora("bf16", "bf16", d.put(x), at, at, native.lora_set("bf16", d.put(a), d.put(b), 2, R, K, N),
+                    native.lora_rows(requests, T, d.put(starts), d.put(adapter)), work=d.empty(size), work_bytes=size)
+        native.synchronize()
+        got = d.get(at, (T, N), np.uint16)
+    assert np.array_equal(got[T - padding:], add[T - padding:])
+    rows = np.unique(np.concatenate([rng.integers(0, T - padding, 150), np.arange(T - padding - 33, T - padding), cuts, starts[:-1]]))
+    which = np.searchsorted(starts, rows, side="right") - 1
+    y, bound = step_ref.lora(vx[rows], values(add[rows], "bf16"), va, vb, np.arange(len(rows) + 1), adapter[which], bf16_parts=True)
+    off = np.abs(values(got[rows], "bf16") - y)
+    assert np.all(off <= step_ref.rounded_bound(y, bound, "bf16"))
