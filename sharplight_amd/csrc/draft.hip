@@ -624,18 +624,23 @@ constexpr int64_t kDecides = 512;
 template <int DT, bool DECIDES> __global__ __launch_bounds__(kDrawThreads) void draft_sums(DraftArgs a)
 {
     __shared__ double s_sum[kDrawWaves];
-    const int32_t i = blockIdx.x / a.chunks, chunk = blockIdx.x - i * a.chunks;
-    Pick k;
-    if constexpr (DECIDES) {
-        __shared__ DecideLds lds;
-        k = decide<DT, false>(a, i, chunk == 0, lds);
-        if (chunk == 0 && threadIdx.x == 0) a.picks[i] = k;
-    } else {
-        k = a.picks[i];
+    for (int32_t item = blockIdx.x; item < a.B * a.chunks; item += gridDim.x) {
+        const int32_t i = item / a.chunks, chunk = item - i * a.chunks;
+        Pick k;
+        if constexpr (DECIDES) {  // of one chunk
+            __shared__ DecideLds lds;
+            k = decide<DT, false>(a, i, chunk == 0, lds);
+            if (chunk == 0 && threadIdx.x == 0) a.picks[i] = k;
+        } else {
+            k = a.picks[i];
+        }
+        if (k.kind == kFromRest) {
+            const double s = chunk_sum<DT>(a, k, chunk, s_sum);
+            if (threadIdx.x == 0) a.sums[static_cast<int64_t>(i) * a.chunks + chunk] = s;
+        }
+        if constexpr (DECIDES) return;
+        if (item + static_cast<int32_t>(gridDim.x) < a.B * a.chunks) __syncthreads();  // the next chunk's sums
     }
-    if (k.kind != kFromRest) return;
-    const double s = chunk_sum<DT>(a, k, chunk, s_sum);
-    if (threadIdx.x == 0) a.sums[static_cast<int64_t>(i) * a.chunks + chunk] = s;
 }
 
 template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_pick(DraftArgs a)
@@ -687,7 +692,8 @@ template <int DT> static int launch(DraftArgs& a, hipStream_t st)
         draft_decide<DT><<<B, kDrawThreads, 0, st>>>(a);
         const int e = check_launch("draft_decide");
         if (e) return e;
-        draft_sums<DT, false><<<B * a.chunks, kDrawThreads, 0, st>>>(a);
+        const unsigned most = 1 << 21;  // a launch has less than 2^32 threads
+        draft_sums<DT, false><<<B * a.chunks < most ? B * a.chunks : most, kDrawThreads, 0, st>>>(a);
     }
     const int e = check_launch("draft_sums");
     if (e) return e;

@@ -357,6 +357,23 @@ def test_lengths_in_place(device, drawn, B):
         assert np.array_equal(d.get(dr.past, (B,), np.int32), now + n_out)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_most_requests_times_chunks(device, dtype):
+    """More chunks of all requests than a launch has thread blocks; few of the requests have rows, the last one among them."""
+    B, V = 40000, 1 << 20
+    new = np.zeros(B, int)
+    new[[0, 20011, B - 2, B - 1]] = [2, 1, 2, 2]
+    c = Case("most", new.tolist(), V, dtype, True, good=0.0, size=12.0)
+    with Dev() as d:
+        run(d, c)
+
+
+def test_one_token_in_the_vocabulary(device):
+    for drawn in (True, False):
+        with Dev() as d:
+            run(d, Case("single", [1, 3, 2], 1, "f32", drawn))
+
+
 def test_two_streams_at_once(device):
     with Dev() as d:
         cases = [Case(f"stream{i}", [4, 2, 5], 40000, "f32", True) for i in range(2)]
