@@ -620,27 +620,24 @@ template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_decide(D
 }
 
 constexpr int64_t kDecides = 512;
+constexpr unsigned kRequestsY = 32768;  // of a launch's second dimension
 
 template <int DT, bool DECIDES> __global__ __launch_bounds__(kDrawThreads) void draft_sums(DraftArgs a)
 {
     __shared__ double s_sum[kDrawWaves];
-    for (int32_t item = blockIdx.x; item < a.B * a.chunks; item += gridDim.x) {
-        const int32_t i = item / a.chunks, chunk = item - i * a.chunks;
-        Pick k;
-        if constexpr (DECIDES) {  // of one chunk
-            __shared__ DecideLds lds;
-            k = decide<DT, false>(a, i, chunk == 0, lds);
-            if (chunk == 0 && threadIdx.x == 0) a.picks[i] = k;
-        } else {
-            k = a.picks[i];
-        }
-        if (k.kind == kFromRest) {
-            const double s = chunk_sum<DT>(a, k, chunk, s_sum);
-            if (threadIdx.x == 0) a.sums[static_cast<int64_t>(i) * a.chunks + chunk] = s;
-        }
-        if constexpr (DECIDES) return;
-        if (item + static_cast<int32_t>(gridDim.x) < a.B * a.chunks) __syncthreads();  // the next chunk's sums
+    const int32_t i = blockIdx.z * kRequestsY + blockIdx.y, chunk = blockIdx.x;
+    if (i >= a.B) return;
+    Pick k;
+    if constexpr (DECIDES) {
+        __shared__ DecideLds lds;
+        k = decide<DT, false>(a, i, chunk == 0, lds);
+        if (chunk == 0 && threadIdx.x == 0) a.picks[i] = k;
+    } else {
+        k = a.picks[i];
     }
+    if (k.kind != kFromRest) return;
+    const double s = chunk_sum<DT>(a, k, chunk, s_sum);
+    if (threadIdx.x == 0) a.sums[static_cast<int64_t>(i) * a.chunks + chunk] = s;
 }
 
 template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_pick(DraftArgs a)
@@ -674,6 +671,8 @@ template <int DT> static int launch(DraftArgs& a, hipStream_t st)
 {
     a.chunks = (a.V + kChunk<DT> - 1) / kChunk<DT>;
     const unsigned rows = static_cast<unsigned>(a.T * a.chunks), B = static_cast<unsigned>(a.B);
+    // a request's chunks after one another (with the requests first, 2432 chunks take 18.6 us instead of 12.9); in one dimension they could have 2^32 threads
+    const dim3 chunks(static_cast<unsigned>(a.chunks), B < kRequestsY ? B : kRequestsY, (B + kRequestsY - 1) / kRequestsY);
     if (rows > 0) {
         if (a.draft)
             draft_stats<DT, true><<<rows * 2, kThreads, 0, st>>>(a);
@@ -687,13 +686,12 @@ template <int DT> static int launch(DraftArgs& a, hipStream_t st)
         return check_launch("draft_choose");
     }
     if (static_cast<int64_t>(B) * a.chunks <= kDecides) {
-        draft_sums<DT, true><<<B * a.chunks, kDrawThreads, 0, st>>>(a);
+        draft_sums<DT, true><<<chunks, kDrawThreads, 0, st>>>(a);
     } else {
         draft_decide<DT><<<B, kDrawThreads, 0, st>>>(a);
         const int e = check_launch("draft_decide");
         if (e) return e;
-        const unsigned most = 1 << 21;  // a launch has less than 2^32 threads
-        draft_sums<DT, false><<<B * a.chunks < most ? B * a.chunks : most, kDrawThreads, 0, st>>>(a);
+        draft_sums<DT, false><<<chunks, kDrawThreads, 0, st>>>(a);
     }
     const int e = check_launch("draft_sums");
     if (e) return e;

@@ -359,7 +359,7 @@ def test_lengths_in_place(device, drawn, B):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_most_requests_times_chunks(device, dtype):
-    """More chunks of all requests than a launch has thread blocks; few of the requests have rows, the last one among them."""
+    """More chunks of all requests than one dimension of a launch takes; few of the requests have rows, the last one among them."""
     B, V = 40000, 1 << 20
     new = np.zeros(B, int)
     new[[0, 20011, B - 2, B - 1]] = [2, 1, 2, 2]
