@@ -16,7 +16,7 @@
 //
 // Measured: the sums of 257 rows of 151936 f32 logits and of 193 draft rows (273 MB) 45.5 us, 6.0 TB/s; of 256 rows of 50257 bf16 logits
 // (25.7 MB) 11.4 us, of which some 3.5 are exponentials that the loads, all on their way at once, do not hide, of 64 rows 5.9. What follows is a
-// latency: 256 or 64 draws 6.9 to 7.2 us in one launch (choose); 64 requests with draft logits 5.4 (decide), 13 to 14 (2432 chunks of p and q,
+// latency: 256 or 64 draws 6.6 to 6.7 us in one launch (choose); 64 requests with draft logits 5.4 (decide), 13 to 14 (2432 chunks of p and q,
 // 78 MB out of the last-level cache) and 6.4 (pick); one request with drafts 6.2 (38 chunks that decide for themselves) and 4.7.
 #include <math.h>
 
@@ -415,7 +415,7 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
 
 // ---- the draw ------------------------------------------------------------------------------------------------------
 
-// e^((z - m) / tau): as f32, like the sums; where p - q may cancel (exact), f64 above 2^-6. (Below, f32's roundings are below those of the
+// e^((z - m) / tau): as f32, like the sums; where p - q may cancel, f64 above 2^-6. (Below, f32's roundings are below those of the
 // sums. A vector of four takes 160 instructions more for f64: with a border of 2^-12 the sums of 38 chunks took 8 us instead of 6.2; with f64 for
 // p alone 256 draws 8.0 us instead of 6.9.)
 struct Share {
@@ -423,16 +423,21 @@ struct Share {
     float mf;
     Factor f;
     __device__ __forceinline__ Share(double m_, double c_) : m(m_), c(c_), mf(static_cast<float>(m_)), f(c_) {}
-    template <int N> __device__ __forceinline__ void of(const float (&z)[N], bool exact, double (&w)[N]) const
+    template <int N> __device__ __forceinline__ void near(const float (&z)[N], float (&w)[N]) const
+    {
+#pragma unroll
+        for (int j = 0; j < N; j++) w[j] = f.power(z[j] - mf);
+    }
+    template <int N> __device__ __forceinline__ void exact(const float (&z)[N], double (&w)[N]) const
     {
         float e[N], most = 0.0f;
+        near(z, e);
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            e[j] = f.power(z[j] - mf);
             most = fmaxf(most, e[j]);
             w[j] = e[j];
         }
-        if (exact && __any(most > 0x1p-6f)) {
+        if (__any(most > 0x1p-6f)) {
 #pragma unroll
             for (int j = 0; j < N; j++) {  // (all of them: a lane's powers take turns then)
                 const double v = exp2_64((static_cast<double>(z[j]) - m) * c);
@@ -442,7 +447,7 @@ struct Share {
     }
 };
 
-// A thread's 16 bytes of a chunk, and their weights as the kind says.
+// A thread's 16 bytes of a chunk, and their weights as the kind says: of max(p - q, 0), or of p in units of the row's sum.
 template <int DT> struct Draws {
     static constexpr int N = Vec<DT>::N;
     typedef Logits<DT, kDrawThreads> Mine;
@@ -454,38 +459,44 @@ template <int DT> struct Draws {
         if (kind == kFromRest) y.load(a.draft, k.row, a.qs, a.V, chunk);
     }
     __device__ __forceinline__ void logits(float (&z)[N]) const { Vec<DT>::unpack(x.w[0], z); }
-    __device__ __forceinline__ void weights(const Pick& k, int32_t kind, int32_t chunk, double (&w)[N]) const
+    __device__ __forceinline__ double rest(const Pick& k, double (&w)[N]) const
     {
 #pragma clang fp contract(off)  // p - q of equal numbers is 0, not the rounding of a product
         float z[N];
+        double u[N], s = 0.0;
         logits(z);
-        Share(k.mp, k.cp).of(z, kind == kFromRest, w);
+        Share(k.mp, k.cp).exact(z, w);
+        Vec<DT>::unpack(y.w[0], z);
+        Share(k.mq, k.cq).exact(z, u);
 #pragma unroll
-        for (int e = 0; e < N; e++) w[e] *= k.ip;
-        const int32_t at = Mine::place(chunk, 0);
-        if (kind == kFromOthers) {
-#pragma unroll
-            for (int e = 0; e < N; e++) w[e] = at + e == k.token ? 0.0 : w[e];
-        } else if (kind == kFromRest) {
-            double u[N];
-            Vec<DT>::unpack(y.w[0], z);
-            Share(k.mq, k.cq).of(z, true, u);
-#pragma unroll
-            for (int e = 0; e < N; e++) w[e] = fmax(w[e] - u[e] * k.iq, 0.0);
+        for (int e = 0; e < N; e++) {
+            w[e] = fmax(w[e] * k.ip - u[e] * k.iq, 0.0);
+            s += w[e];
         }
+        return s;
+    }
+    __device__ __forceinline__ float own(const Pick& k, int32_t kind, int32_t at, float (&w)[N]) const
+    {
+        float z[N], s = 0.0f;
+        logits(z);
+        Share(k.mp, k.cp).near(z, w);
+        if (kind == kFromOthers && k.token >= at && k.token < at + N) {
+#pragma unroll
+            for (int e = 0; e < N; e++) w[e] = at + e == k.token ? 0.0f : w[e];
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) s += w[e];
+        return s;
     }
 };
 
 // A chunk's sum, in the first thread.
 template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a, const Pick& k, int32_t chunk, double (&lds)[kDrawWaves])
 {
-    double w[Vec<DT>::N], s = 0.0;
+    double w[Vec<DT>::N];
     Draws<DT> mine;
     mine.load(a, k, k.kind, chunk);
-    mine.weights(k, k.kind, chunk, w);
-#pragma unroll
-    for (int e = 0; e < Vec<DT>::N; e++) s += w[e];
-    s = wave_sum64(s);
+    const double s = wave_sum64(mine.rest(k, w));
     if ((threadIdx.x & 63) == 0) lds[wave_id()] = s;
     __syncthreads();
     return row_sum64(lds[threadIdx.x & (kDrawWaves - 1)]);
@@ -497,9 +508,8 @@ template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a
 template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32_t i, const Pick& k, float u, const double* sums, const double* shares)
 {
     constexpr int N = Vec<DT>::N;
-    __shared__ double s_part[kDrawWaves];
-    __shared__ int32_t s_place[kDrawWaves], s_last[kDrawWaves];
-    __shared__ float s_place_z[kDrawWaves], s_last_z[kDrawWaves];
+    __shared__ double s_part[kDrawWaves], s_log;
+    __shared__ int32_t s_flags[kDrawWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
     const ChunkStat* st = a.stats + static_cast<int64_t>(k.row) * 2 * a.chunks;
     int32_t kind = k.kind;
@@ -546,15 +556,17 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
             if (!end && v > 0.0 && sum > r) break;
         }
     }
-    double w[N], s = 0.0;
-    float z[N];
     Draws<DT> of;
     of.load(a, k, kind, chunk);
-    const double log_s = a.logp && wave == 0 ? log(k.ip) : 0.0;  // while the loads are on their way
-    of.logits(z);
-    of.weights(k, kind, chunk, w);
-#pragma unroll
-    for (int e = 0; e < N; e++) s += w[e];
+    if (a.logp && wave == 0) s_log = log(k.ip);  // while the loads are on their way
+    const int32_t at = Logits<DT, kDrawThreads>::place(chunk, 0);
+    double w[N], s;
+    float e[N];
+    if (kind == kFromRest) {
+        s = of.rest(k, w);
+    } else {
+        s = of.own(k, kind, at, e) * k.ip;
+    }
     double c = wave_scan64(s);
     if (lane == 63) s_part[wave] = c;
     c -= s;
@@ -563,42 +575,32 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
         const double v = s_part[lane & (kDrawWaves - 1)];
         c += base + row_sum64((lane & (kDrawWaves - 1)) < wave ? v : 0.0);
     }
-    const int32_t at = Logits<DT, kDrawThreads>::place(chunk, 0);
-    int32_t last = -1, place = -1;
-    float last_z = 0.0f, place_z = 0.0f;
+    // the first thread whose inclusive sum is above r, or the last one with a weight, and the place among its own
+    const uint64_t found = __ballot(s > 0.0 && c + s > r), held = __ballot(s > 0.0);
+    if (lane == 0) s_flags[wave] = (found && !end ? 1 : 0) + (held ? 2 : 0);
+    __syncthreads();
+    const int32_t flags = s_flags[lane & (kDrawWaves - 1)];
+    const uint64_t waves = (uint64_t{1} << kDrawWaves) - 1, finds = __ballot(flags & 1) & waves, holds = __ballot(flags & 2) & waves;
+    const auto highest = [](uint64_t lanes) { return lanes ? 63 - __clzll(static_cast<long long>(lanes)) : 0; };
+    if (wave != (finds ? __ffsll(static_cast<long long>(finds)) - 1 : highest(holds))) return;
+    if (lane != (finds ? __ffsll(static_cast<long long>(found)) - 1 : highest(held))) return;
+    float z[N];
+    of.logits(z);
+    int32_t token = at;
+    float logit = z[0];
+    bool there = false;
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-        c += w[e];
-        if (w[e] > 0.0) {
-            last = at + e;
-            last_z = z[e];
-            if (c > r && place < 0) {
-                place = last;
-                place_z = last_z;
-            }
+    for (int n = 0; n < N; n++) {
+        const double v = kind == kFromRest ? w[n] : e[n] * k.ip;
+        c += v;
+        if (v > 0.0 && !there) {
+            token = at + n;
+            logit = z[n];
+            there = finds && c > r;
         }
     }
-    // the first place of the wave's, and its last with a weight
-    const auto lowest = [](uint64_t lanes) { return lanes ? __ffsll(static_cast<long long>(lanes)) - 1 : 0; };
-    const auto highest = [](uint64_t lanes) { return lanes ? 63 - __clzll(static_cast<long long>(lanes)) : 0; };
-    if (lane == lowest(__ballot(place >= 0))) {
-        s_place[wave] = place;
-        s_place_z[wave] = place_z;
-    }
-    if (lane == highest(__ballot(last >= 0))) {
-        s_last[wave] = last;
-        s_last_z[wave] = last_z;
-    }
-    __syncthreads();
-    if (tid >= 64) return;
-    const bool in = lane < kDrawWaves;
-    const uint64_t found = __ballot(in && s_place[lane & (kDrawWaves - 1)] >= 0), held = __ballot(in && s_last[lane & (kDrawWaves - 1)] >= 0);
-    if (lane > 0) return;
-    const bool ends = end || !found;
-    const int from_wave = ends ? highest(held) : lowest(found);
-    const int32_t token = max(ends ? s_last[from_wave] : s_place[from_wave], 0);
     a.out[i * a.out_stride + k.place] = token;
-    if (a.logp) a.logp[i * a.out_stride + k.place] = static_cast<float>(((ends ? s_last_z : s_place_z)[from_wave] - k.mp) * (k.cp / kLog2e64) + log_s);
+    if (a.logp) a.logp[i * a.out_stride + k.place] = static_cast<float>((logit - k.mp) * (k.cp / kLog2e64) + s_log);
 }
 
 // Drafts that were chosen, or none: the sums of p are there, a thread block a request does the rest.
