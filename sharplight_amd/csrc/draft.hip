@@ -16,8 +16,8 @@
 //
 // Measured: the sums of 257 rows of 151936 f32 logits and of 193 draft rows (273 MB) 45.5 us, 6.0 TB/s; of 256 rows of 50257 bf16 logits
 // (25.7 MB) 11.4 us, of which some 3.5 are exponentials that the loads, all on their way at once, do not hide, of 64 rows 5.9. What follows is a
-// latency: 256 or 64 draws 6.6 to 6.7 us in one launch (choose); 64 requests with draft logits 5.4 (decide), 13 to 14 (2432 chunks of p and q,
-// 78 MB out of the last-level cache) and 6.4 (pick); one request with drafts 6.2 (38 chunks that decide for themselves) and 4.7.
+// latency: 256 or 64 draws 6.6 to 6.7 us in one launch (choose); 64 requests with draft logits 5.4 (decide), 12.6 (2432 chunks of p and q,
+// 78 MB out of the last-level cache) and 6.2 (pick); one request with drafts 6.2 (38 chunks that decide for themselves) and 4.7.
 #include <math.h>
 
 #include "step.hpp"
