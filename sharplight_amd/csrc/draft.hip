@@ -663,8 +663,9 @@ static int64_t work_of(int64_t B, int64_t T, int64_t chunks)
 static int check_sizes(int64_t B, int64_t T, int64_t V, int64_t* chunks)
 {
     if (B < 0 || T < 0 || V < 1) return fail(SLHIP_ERR_INVALID, "draft_verify: bad size");
-    *chunks = (V + kChunk<SLHIP_F32> - 1) / kChunk<SLHIP_F32>;
-    if (B > 65536 || V > kMaxVocab || T * *chunks * 2 > 0xFFFFFF || B * *chunks > 0xFFFFFF)
+    *chunks = V > kMaxVocab ? 0 : (V + kChunk<SLHIP_F32> - 1) / kChunk<SLHIP_F32>;
+    // (products of what is below 2^24 only: any numbers may come)
+    if (B > 65536 || V > kMaxVocab || T > 0xFFFFFF || T * *chunks * 2 > 0xFFFFFF || B * *chunks > 0xFFFFFF)
         return fail(SLHIP_ERR_UNSUPPORTED, "draft_verify: too many requests, rows or tokens of the vocabulary");
     return SLHIP_OK;
 }
