@@ -580,7 +580,8 @@ SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q_stride_t, 
  *   drawn from. Without draft logits, or where draft_temperature[i] <= 0, the draft was chosen: q_t is 1 there.
  *   Draft x of row t is accepted while accept[t] * q_t(x) < p_t(x). Behind the accepted ones comes one more token, from the row
  *   of the first refused draft or the last row: of weights max(p - q, 0) (the last row, or weights that are all 0: p) it is the
- *   first v whose sum over 0 .. v is above sample[i] times the sum of all, or the last one with a weight.
+ *   first v whose sum over 0 .. v is above sample[i] times the sum of all, or the last one with a weight. (What has less than 2^-100 of the
+ *   row's largest probability may count as 0 here. A logit of -inf is never drawn.)
  *   temperature[i] <= 0: a draft is accepted while it is the lowest v with the largest logit, and that is the token behind; no random
  *   number and no draft logits count. Logits of -inf have the probability 0. Temperatures count as 2^-40 .. 2^40.
  *   out[i, 0 ..]: the accepted drafts and the token, then -1 up to out_stride; n_out[i] their number (0 for a request of no rows);

@@ -502,6 +502,10 @@ template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a
     return row_sum64(lds[threadIdx.x & (kDrawWaves - 1)]);
 }
 
+// A chunk that has less of the row's largest exponential has no weight: the places of one that has are f32 powers of the same
+// largest, so one of its at most 2^13 is above 2^-123 and not 0 (a random number of 0 would be above none of them).
+constexpr double kLeastShare = 0x1p-110;
+
 // The draw itself, by the whole block. Chunk c's weight is sums[c], or where there are none p's, of the target's chunk sums: of the chunk that
 // holds the refused draft without that. (Which is off by 2^-24 of the draft's p at most, as are the sums themselves.)
 // Every wave finds the chunk for itself, a lane for one or more neighbours, and all of them the place in it, 16 bytes a thread.
@@ -515,9 +519,14 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
     int32_t kind = k.kind;
     const int32_t other = kind == kFromOthers && k.token >= 0 && k.token < a.V ? k.token / kChunk<DT> : -1;
     const auto target = [&](int32_t c) {
-        if (shares && c < 16 * kHeld) return shares[c] * k.ip;
-        const ChunkStat x = st[c];
-        return x.m > -INFINITY ? x.s * exp2_64((static_cast<double>(x.m) - k.mp) * k.cp) * k.ip : 0.0;
+        double v;
+        if (shares && c < 16 * kHeld) {
+            v = shares[c];
+        } else {
+            const ChunkStat x = st[c];
+            v = x.m > -INFINITY ? x.s * exp2_64((static_cast<double>(x.m) - k.mp) * k.cp) : 0.0;
+        }
+        return v > kLeastShare ? v * k.ip : 0.0;
     };
     const auto weight = [&](int32_t c) {
         if (kind == kFromTarget) return target(c);
