@@ -32,7 +32,7 @@ template <int DT> constexpr int kChunk = kChunkVecs * Vec<DT>::N;  // logits of 
 
 struct ChunkStat {
     float m;      // the largest logit; NaN where the chunk holds a NaN or an infinity above
-    int32_t arg;  // its first place (rows of greedy requests)
+    int32_t arg;  // its first place (rows of greedy requests); the bits of the f32 sum without the row's draft (chosen drafts, of its chunk)
     double s;     // sum of e^((z - m) / tau)
 };
 
@@ -41,7 +41,7 @@ enum : int32_t { kDone = 0, kFromTarget = 1, kFromRest = 2, kFromOthers = 3 };  
 struct Pick {
     int32_t kind, row, place, token;  // the row, its place in the request, its draft
     double mp, cp, ip, mq, cq, iq;    // maxima, log2(e) / tau, 1 / sums
-    double px;                        // p of the draft
+    double rest;                      // sum of the draft's chunk without it, before the division
     int32_t held, reserved;           // where its chunks' shares are held in LDS (-1: nowhere)
 };
 
@@ -204,6 +204,10 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
         if (target.greedy || h.greedy || t == a.starts[i + 1] - 1) return;
         x.load(a.draft, t, a.qs, a.V, chunk);
     }
+    // where drafts are chosen, the chunk that holds the row's is summed without it, and its own power added at the end
+    int32_t drafted = -1;
+    if (mat == 0 && !target.greedy && t + 1 < min(static_cast<int64_t>(a.starts[i + 1]), a.T) && (!DRAFT || (a.tau_q && a.tau_q[i] <= 0.0f))) drafted = a.ids[t + 1];
+    const bool holds = drafted >= 0 && drafted / kChunk<DT> == chunk;
     float z[Mine::kEach];
 #pragma unroll
     for (int j = 0; j < kVecs; j++) Vec<DT>::unpack(x.w[j], &z[j * N]);
@@ -218,7 +222,12 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
     m = s_m[0];
     for (int w = 1; w < kWaves; w++) m = fmaxf(m, s_m[w]);
     const Factor c(kLog2e64 / h.tau);
-    float s = 0.0f;
+    float s = 0.0f, own = 0.0f;
+    if (holds) {
+        own = Vec<DT>::load1(static_cast<const char*>(a.target) + t * a.zs * Vec<DT>::BYTES, drafted);
+#pragma unroll
+        for (int j = 0; j < kVecs * N; j++) z[j] = Mine::place(chunk, j / N) + j % N == drafted ? -INFINITY : z[j];
+    }
 #pragma unroll
     for (int j = 0; j < kVecs * N; j++) s += c.power(z[j] - m);
     const double sum = wave_sum64(s);
@@ -241,6 +250,10 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
             o.s += s_s[w];
             o.arg = min(o.arg, s_arg[w]);
         }
+        if (holds) {
+            o.arg = __float_as_int(static_cast<float>(o.s));
+            o.s += c.power(own - m);
+        }
         if (m == -INFINITY) o.s = 0.0;
         a.stats[(t * 2 + mat) * a.chunks + chunk] = o;
     }
@@ -258,8 +271,9 @@ struct RowStat {
 
 constexpr int kHeld = 4;  // chunks of a lane that it looks at once: a vocabulary of 262144
 
-// The chunks of a row together, by 16 lanes. shares: of the first 64 chunks, in units of the row's sum before its division.
-__device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks, double c, bool arg, double* shares)
+// The chunks of a row together, by 16 lanes. arg: its first place is wanted. In units of the row's sum before its division, shares: of the first 64
+// chunks; rest: of chunk `holds` without the chosen draft in it (-1: there is none).
+__device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks, double c, bool arg, int32_t holds, double* rest, double* shares)
 {
     const int lane = threadIdx.x & 15;
     ChunkStat x[kHeld];
@@ -283,18 +297,19 @@ __device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks,
     r.m = m;
     double s = 0.0;
     int32_t first = 0x7FFFFFFF;
-    const auto take = [&](const ChunkStat& v) {
-        const double part = v.m > -INFINITY ? v.s * exp2_64((static_cast<double>(v.m) - r.m) * c) : 0.0;
+    const auto take = [&](const ChunkStat& v, int32_t k) {
+        const double unit = exp2_64((static_cast<double>(v.m) - r.m) * c), part = v.m > -INFINITY ? v.s * unit : 0.0;
         s += part;
+        if (k == holds) *rest = v.m > -INFINITY ? __int_as_float(v.arg) * unit : 0.0;
         if (v.m == m) first = min(first, v.arg);
         return part;
     };
 #pragma unroll
     for (int j = 0; j < kHeld; j++) {
-        const double part = take(x[j]);
+        const double part = take(x[j], lane + 16 * j);
         if (shares) shares[lane + 16 * j] = part;
     }
-    for (int32_t k = lane + 16 * kHeld; k < chunks; k += 16) take(st[k]);
+    for (int32_t k = lane + 16 * kHeld; k < chunks; k += 16) take(st[k], k);
     r.s = row_sum64(s);
     if (arg) {
 #pragma unroll
@@ -306,6 +321,7 @@ __device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks,
 
 struct DecideLds {
     RowStat row[16];        // of a pass: target's rows, or target's and draft's in turns
+    double rest[16];        // of a refused draft's chunk
     double shares[16][64];  // of their first chunks, target's rows where no drafts were drawn
 };
 
@@ -335,7 +351,8 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
             float z = -INFINITY;
             if (v >= 0 && v < a.V) z = Vec<DT>::load1(mat ? a.draft : a.target, t * (mat ? a.qs : a.zs) + v);
             const double c = mat ? cq : cp;
-            RowStat r = row_stat(a.stats + (t * 2 + mat) * a.chunks, a.chunks, c, hp.greedy, SHARES ? lds.shares[group] : nullptr);
+            const int32_t holds = !drawn && !hp.greedy && place < n - 1 && v >= 0 && v < a.V ? v / kChunk<DT> : -1;
+            RowStat r = row_stat(a.stats + (t * 2 + mat) * a.chunks, a.chunks, c, hp.greedy, holds, &lds.rest[group], SHARES ? lds.shares[group] : nullptr);
             r.fine &= !(mat ? hq.bad : hp.bad);
             r.z = z;
             r.inv = 1.0 / r.s;
@@ -389,7 +406,7 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
                 k.cq = cq;
                 k.iq = q.inv;
             }
-            k.px = p.share;
+            k.rest = lds.rest[(stop - first) * mats];
             k.held = SHARES ? (stop - first) * mats : -1;
         }
     }
@@ -507,7 +524,7 @@ template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a
 constexpr double kLeastShare = 0x1p-110;
 
 // The draw itself, by the whole block. Chunk c's weight is sums[c], or where there are none p's, of the target's chunk sums: of the chunk that
-// holds the refused draft without that. (Which is off by 2^-24 of the draft's p at most, as are the sums themselves.)
+// holds the refused draft the one that was made without it (a difference would leave nothing beside a draft of nearly all).
 // Every wave finds the chunk for itself, a lane for one or more neighbours, and all of them the place in it, 16 bytes a thread.
 template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32_t i, const Pick& k, float u, const double* sums, const double* shares)
 {
@@ -520,7 +537,9 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
     const int32_t other = kind == kFromOthers && k.token >= 0 && k.token < a.V ? k.token / kChunk<DT> : -1;
     const auto target = [&](int32_t c) {
         double v;
-        if (shares && c < 16 * kHeld) {
+        if (kind == kFromOthers && c == other) {
+            v = k.rest;
+        } else if (shares && c < 16 * kHeld) {
             v = shares[c];
         } else {
             const ChunkStat x = st[c];
@@ -528,12 +547,7 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
         }
         return v > kLeastShare ? v * k.ip : 0.0;
     };
-    const auto weight = [&](int32_t c) {
-        if (kind == kFromTarget) return target(c);
-        if (sums) return sums[c];
-        const double v = target(c), rest = v - k.px;
-        return c != other ? v : rest > 0x1p-40 * v ? rest : 0.0;  // (the roundings of a draft that is alone there are no weight)
-    };
+    const auto weight = [&](int32_t c) { return sums && kind != kFromTarget ? sums[c] : target(c); };
     const int32_t each = (a.chunks + 63) / 64, c0 = min(lane * each, a.chunks), c1 = min(c0 + each, a.chunks);
     const auto sum_of = [&]() {
         double s = 0.0;

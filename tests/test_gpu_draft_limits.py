@@ -57,3 +57,69 @@ def test_ends_beside_chunks_far_below(device, low, drafts, dtype):
             assert x <= weighty[0]
         else:
             assert x >= weighty[-1]
+
+
+# ---- drafts that hold nearly all of p ------------------------------------------------------------------------------
+
+def _others(c, at, places, weights):
+    """Rows of one draft at `at` (logit 0) and others of the given weights; all else is masked. Returns the places and what they weigh."""
+    z = np.full((c.T, c.V), -np.inf)
+    z[:, at] = 0.0
+    z[:, places] = np.log(weights)
+    c.target, c.z = held(z, c.dtype)
+    c.ids[:] = at
+    c.accept[:] = 1 - 2.0 ** -24
+    order = np.sort(places)
+    return order, np.exp(c.z[0, order])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("by_temperature", [False, True])
+@pytest.mark.parametrize("at,places", [(5, [4, 6, 7]), (5, [0, 1, 2, 3, 4, 6, 7]), (4101, [4100, 4102, 4103]), (9, [8, 10, 11, 2060, 2061])])
+def test_a_refused_draft_of_nearly_all_is_not_drawn(device, at, places, by_temperature, dtype):
+    """The others weigh less than half of 2^-24 each: all of them vanish in f32 beside the draft's 1."""
+    c = Case("nearly all", [2] * len(places), 5000, dtype, by_temperature, [1.0], [0.0], settle=False)
+    order, w = _others(c, at, places, np.full(len(places), 0.45 * 2.0 ** -24) if len(places) > 5 else np.full(len(places), 0.8 * 2.0 ** -24))
+    share = np.cumsum(w) / w.sum()
+    c.sample = np.float32(share - 0.5 * w / w.sum())  # the middle of each one's part
+    with Dev() as d:
+        out, n, logp = _call(d, c, f"a draft of nearly all at {at} {dtype}")
+    assert (n == 1).all() and np.array_equal(out[:, 0], order), out[:, 0]
+    want = np.log(step_ref.probabilities(c.z[0], 1.0)[order])
+    assert np.all(np.abs(logp[:, 0] - want) <= [step_ref.logp_bound(c.z[0], 1.0, v) for v in want])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("by_temperature", [False, True])
+@pytest.mark.parametrize("at,total", [(5, 2.0 ** -20), (4999, 2.0 ** -17), (4097, 2.0 ** -14), (100, 2.0 ** -10)])
+def test_what_is_left_of_a_chunk_is_summed_without_the_draft(device, at, total, by_temperature, dtype):
+    """p(x) = 1 - total, the rest over x's chunk and the others: every one of them is drawn by the middle of its part, whose halves are 2^-9 of
+    the rest or more."""
+    V, n = 12000, 100
+    c = Case("left", [2] * n, V, dtype, by_temperature, [1.0], [0.0], settle=False)
+    chunk = 4096 if dtype == "f32" else 8192
+    inside = np.arange(at // chunk * chunk, min((at // chunk + 1) * chunk, V))
+    inside = inside[inside != at]
+    rest = np.setdiff1d(np.arange(V), np.append(inside, at))
+    places = np.concatenate([c.rng.choice(inside, 80, replace=False), c.rng.choice(rest, 20, replace=False)])
+    order, w = _others(c, at, places, total / n * (0.7 + 0.6 * c.rng.random(n)))
+    share = np.cumsum(w) / w.sum()
+    c.sample = np.float32(share - 0.5 * w / w.sum())
+    assert (0.5 * w / w.sum()).min() > 2.0 ** -9
+    with Dev() as d:
+        out, got, _ = _call(d, c, f"what is left beside {at} {total} {dtype}")
+    assert (got == 1).all() and np.array_equal(out[:, 0], order), np.nonzero(out[:, 0] != order)[0]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_what_is_left_in_a_large_vocabulary(device, dtype):
+    """Drafts in chunks behind the first 64."""
+    V, n = 600000, 40
+    c = Case("left, large", [2] * n, V, dtype, False, settle=False)
+    at = 590001
+    places = np.concatenate([np.arange(at - 20, at), np.arange(at + 1, at + 11), c.rng.choice(500000, 10, replace=False)])
+    order, w = _others(c, at, places, 2.0 ** -22 / n * (0.7 + 0.6 * c.rng.random(n)))
+    c.sample = np.float32(np.cumsum(w) / w.sum() - 0.5 * w / w.sum())
+    with Dev() as d:
+        out, got, _ = _call(d, c, f"what is left of a large vocabulary {dtype}")
+    assert (got == 1).all() and np.array_equal(out[:, 0], order)
