@@ -11,7 +11,7 @@
 //
 // Numbers. A choice changes where a sum passes a random number, so what two implementations may differ in is kept small:
 // exponentials are f32 of arguments with one rounding (log2(e) / tau in two parts, or all terms of a sum would be off the same
-// way), a chunk's are added in f32, everything behind them in f64: the rows' sums, p(x), q(x), and the weights drawn from, whose differences
+// way), 16 of them are added in f32, everything behind them in f64: the rows' sums, p(x), q(x), and the weights drawn from, whose differences
 // p - q are of f64 exponentials where they may cancel.
 //
 // Measured: the sums of 257 rows of 151936 f32 logits and of 193 draft rows (273 MB) 45.5 us, 6.0 TB/s; of 256 rows of 50257 bf16 logits
@@ -27,6 +27,7 @@ namespace slhip {
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kDrawThreads = 1024, kDrawWaves = 16;  // of what follows the rows' sums: few thread blocks, so a latency
 constexpr int kChunkVecs = 1024;                     // 16-byte vectors of a chunk: 16 KB
+constexpr int kTerms = 16;                           // powers that are added in f32
 constexpr int64_t kMaxVocab = 1 << 24;
 template <int DT> constexpr int kChunk = kChunkVecs * Vec<DT>::N;  // logits of a chunk
 
@@ -222,15 +223,19 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
     m = s_m[0];
     for (int w = 1; w < kWaves; w++) m = fmaxf(m, s_m[w]);
     const Factor c(kLog2e64 / h.tau);
-    float s = 0.0f, own = 0.0f;
+    float own = 0.0f;
     if (holds) {
         own = Vec<DT>::load1(static_cast<const char*>(a.target) + t * a.zs * Vec<DT>::BYTES, drafted);
 #pragma unroll
         for (int j = 0; j < kVecs * N; j++) z[j] = Mine::place(chunk, j / N) + j % N == drafted ? -INFINITY : z[j];
     }
+    float s[kVecs * N / kTerms] = {};
 #pragma unroll
-    for (int j = 0; j < kVecs * N; j++) s += c.power(z[j] - m);
-    const double sum = wave_sum64(s);
+    for (int j = 0; j < kVecs * N; j++) s[j / kTerms] += c.power(z[j] - m);
+    double mine = s[0];
+#pragma unroll
+    for (int j = 1; j < kVecs * N / kTerms; j++) mine += s[j];
+    const double sum = wave_sum64(mine);
     int32_t arg = 0x7FFFFFFF;
     if (target.greedy) {
 #pragma unroll

@@ -123,3 +123,22 @@ def test_what_is_left_in_a_large_vocabulary(device, dtype):
     with Dev() as d:
         out, got, _ = _call(d, c, f"what is left of a large vocabulary {dtype}")
     assert (got == 1).all() and np.array_equal(out[:, 0], order)
+
+
+# ---- sums ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,far,step", [("f32", 1024, 4), ("bf16", 2048, 8)])
+def test_small_terms_beside_a_large_one(device, dtype, far, step):
+    """All logits that one thread adds are just below half a unit of its first one: the row's sum stays within the bound that 16 f32 terms give."""
+    c = Case("small terms", [1], 20000, dtype, False, settle=False)
+    c.z[:] = -np.inf
+    for j in range(4):
+        c.z[:, far * j:far * j + step] = -16.75  # e^-16.75 = 0.89 * 2^-24
+    c.z[:, 0] = 0.0
+    c.target, c.z = held(c.z, dtype)
+    c.sample[:] = 0.0
+    with Dev() as d:
+        out, n, logp = _call(d, c, f"small terms {dtype}")
+    want = np.log(step_ref.probabilities(c.z[0], 1.0)[0])
+    assert n[0] == 1 and out[0, 0] == 0
+    assert abs(logp[0, 0] - want) <= step_ref.logp_bound(c.z[0], 1.0, want), (logp[0, 0], want)
