@@ -176,7 +176,7 @@ struct Factor {
     {
         const float near = static_cast<float>(c);
         hi = near > c ? __uint_as_float(__float_as_uint(near) - 1) : near;
-        lo = fmaxf(static_cast<float>(c - hi), 0x1p-60f);
+        lo = fmaxf(static_cast<float>(c - hi), 0x1p-100f);  // (c is above 2^-40)
     }
     // 2^(d c) for d <= 0, -inf included.
     __device__ __forceinline__ float power(float d) const { return __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo)); }

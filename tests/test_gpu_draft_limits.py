@@ -142,3 +142,22 @@ def test_small_terms_beside_a_large_one(device, dtype, far, step):
     want = np.log(step_ref.probabilities(c.z[0], 1.0)[0])
     assert n[0] == 1 and out[0, 0] == 0
     assert abs(logp[0, 0] - want) <= step_ref.logp_bound(c.z[0], 1.0, want), (logp[0, 0], want)
+
+
+@pytest.mark.parametrize("tau", [2.0 ** 40, 2.0 ** 60, 2.0 ** 38, 2.0 ** 20, 2.0 ** -20, 2.0 ** -40, 2.0 ** -60])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_temperatures_at_the_ends(device, tau, dtype):
+    """One token, and 4000 of the same chunk that weigh as much together: an exponent's error counts half."""
+    V = 4001
+    c = Case("temperatures", [1], V, dtype, False, [tau], settle=False)
+    heat = min(max(tau, 2.0 ** -40), 2.0 ** 40)
+    c.z[:] = np.log(1 / 4000) * heat
+    c.z[:, 77] = 0.0
+    c.target, c.z = held(c.z, dtype)
+    p = step_ref.probabilities(c.z[0], tau)
+    c.sample[:] = p[:77].sum() + 0.5 * p[77]
+    with Dev() as d:
+        out, n, logp = _call(d, c, f"temperature {tau} {dtype}")
+    want = np.log(p[77])
+    assert n[0] == 1 and out[0, 0] == 77
+    assert abs(logp[0, 0] - want) <= step_ref.logp_bound(c.z[0], tau, want), (logp[0, 0], want)
