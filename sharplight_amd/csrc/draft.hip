@@ -381,7 +381,7 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
                 out[mine] = x;
                 if (logp) logp[mine] = static_cast<float>((static_cast<double>(p.z) - p.m) * (cp / kLog2e64) - log(p.s));
             }
-            if (row && p.fine && !known && mine == stop)
+            if (row && !known && mine == stop)
                 raise_error(a.err, kErrDraftToken, static_cast<uint32_t>(i), static_cast<uint32_t>(mine), static_cast<uint32_t>(x), static_cast<uint32_t>(a.V), 0, 0);
         }
         if (stop < n) break;

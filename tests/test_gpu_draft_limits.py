@@ -161,3 +161,27 @@ def test_temperatures_at_the_ends(device, tau, dtype):
     want = np.log(p[77])
     assert n[0] == 1 and out[0, 0] == 77
     assert abs(logp[0, 0] - want) <= step_ref.logp_bound(c.z[0], tau, want), (logp[0, 0], want)
+
+
+# ---- rows, drafts and temperatures that cannot be used -------------------------------------------------------------
+
+@pytest.mark.parametrize("drawn", [True, False])
+@pytest.mark.parametrize("why", ["nan", "inf", "masked", "temperature"])
+@pytest.mark.parametrize("x", [5000, -1, 1 << 30])
+def test_a_bad_draft_of_a_row_that_cannot_be_used_is_reported(device, x, why, drawn):
+    c = Case("bad both", [1, 3, 2], 5000, "f32", drawn, [1.0], settle=False)
+    c.ids[2] = x  # the draft of request 1's first row
+    if why == "temperature":
+        c.tau[1] = np.nan
+    else:
+        c.z[1, 17 if why != "masked" else slice(None)] = {"nan": np.nan, "inf": np.inf, "masked": -np.inf}[why]
+    c.target, c.z = held(c.z, "f32")
+    with Dev() as d:
+        args, more = c.put(d)
+        log(f"draft_verify bad draft {x} of a row that cannot be used: {why} drawn={drawn}")
+        native.draft_verify(*args, **more)
+        with pytest.raises(IndexError, match="number 0 of request 1"):
+            native.synchronize()
+        native.synchronize()
+        out, n = d.get(c.at["out"], (3, 3), np.int32), d.get(c.at["n_out"], (3,), np.int32)
+    assert n[1] == 1 and (out[1] == -1).all()
