@@ -335,7 +335,7 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
 {
     const int tid = threadIdx.x, lane = tid & 63, group = tid >> 4;
     const int64_t s0 = a.starts[i], s1 = a.starts[i + 1];
-    const bool fits = s0 >= 0 && s1 >= s0 && s1 <= a.T && s1 - s0 <= a.out_stride;
+    const bool inside = s0 >= 0 && s1 >= s0 && s1 <= a.T, fits = inside && s1 - s0 <= a.out_stride;
     const int32_t n = fits ? static_cast<int32_t>(s1 - s0) : 0;
     const Heat hp = heat_of(a.tau, i), hq = a.tau_q ? heat_of(a.tau_q, i) : hp;
     const double cp = kLog2e64 / hp.tau, cq = kLog2e64 / hq.tau;
@@ -423,7 +423,7 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
         }
         a.n_out[i] = n > 0 ? stop + 1 : 0;
         if (a.kept) a.kept[i] = (a.past ? a.past[i] : 0) + (n > 0 ? stop + 1 : 0);
-        if (a.dropped) a.dropped[i] = n > 0 ? n - stop - 1 : 0;
+        if (a.dropped) a.dropped[i] = n > 0 ? n - stop - 1 : inside ? static_cast<int32_t>(s1 - s0) : 0;  // (too many rows: all of them)
         if (!fits)
             raise_error(a.err, kErrKvRequest, static_cast<uint32_t>(i), static_cast<uint32_t>(i), a.past ? static_cast<uint32_t>(a.past[i]) : 0,
                         static_cast<uint32_t>(s1 - s0), static_cast<uint32_t>(static_cast<uint64_t>(s1 - s0) >> 32), 0);

@@ -185,3 +185,37 @@ def test_a_bad_draft_of_a_row_that_cannot_be_used_is_reported(device, x, why, dr
         native.synchronize()
         out, n = d.get(c.at["out"], (3, 3), np.int32), d.get(c.at["n_out"], (3,), np.int32)
     assert n[1] == 1 and (out[1] == -1).all()
+
+
+# ---- lengths -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("drawn", [True, False])
+def test_requests_of_too_many_rows_give_their_blocks_back(device, drawn):
+    """A request with more rows than out_stride gets no token and drops all of its rows: the trim behind takes all their blocks back."""
+    B, bs, bps = 4, 16, 6
+    new, past = [40, 3, 33, 1], np.int32([7, 16, 0, 31])
+    c = Case("too many rows", new, 300, "f32", drawn, settle=False)
+    c.stride, c.past = 3, past
+    pages = np.full((B, bps), -1, np.int32)
+    ids = iter(range(100))
+    for i in range(B):
+        for j in range(-(-int(past[i]) // bs)):
+            pages[i, j] = next(ids)
+    free = np.int32([next(ids) for _ in range(12)])
+    with Dev() as d:
+        pp, pf, n, count, starts = d.put(pages), d.put(free), d.put(np.int32([12])), d.put(np.int32(new)), d.empty(4 * (B + 1))
+        args, more = c.put(d)
+        dr = args[3]
+        log(f"advance, draft_verify of too many rows, trim; drawn={drawn}")
+        native.kv_pages_advance(native.kv_pages(B, dr.past, count, pp, B, bps, bs, pf, 12, n, n, c.T, starts))
+        native.draft_verify(*args, **more)
+        native.kv_pages_trim(native.kv_pages(B, dr.kept, dr.dropped, pp, B, bps, bs, pf, 12, n, n))
+        with pytest.raises(native.SlhipCacheError, match="does not fit"):
+            native.synchronize()
+        native.synchronize()
+        n_out, kept, dropped = (d.get(c.at[k], (B,), np.int32) for k in ("n_out", "kept", "dropped"))
+        assert n_out[0] == n_out[2] == 0 and n_out[3] == 1
+        assert np.array_equal(kept, past + n_out) and np.array_equal(dropped, np.int32(new) - n_out)
+        held_now = d.get(pp, (B, bps), np.int32)
+        assert np.array_equal((held_now >= 0).sum(1), -(-kept // bs))
+        assert d.get(n, (1,), np.int32)[0] == 12 - int((-(-kept // bs)).sum() - (-(-past // bs)).sum())
