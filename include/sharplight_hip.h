@@ -587,10 +587,12 @@ SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q_stride_t, 
  *   out[i, 0 ..]: the accepted drafts and the token, then -1 up to out_stride; n_out[i] their number (0 for a request of no rows);
  *   logp (NULL: none): the logarithms of their p (greedy: at temperature 1), then 0. kept[i] = past[i] + n_out[i], the tokens that
  *   the cache keeps of past[i] and the step's; dropped[i] = the request's rows - n_out[i]: what slhip_kv_pages_trim takes as past and count.
- * Where a row's target logits hold a NaN or +inf, or nothing above -inf, or a temperature is NaN, its draft is refused and its
- * token is -1 with a NaN; where its draft logits do, the draft is refused and the token drawn from p. A draft outside the vocabulary
- * that is reached is refused and reported (SLHIP_ERR_INDEX) by the next slhip_stream_sync. A request that does not fit the rows, or has more of them
- * than out_stride, gets no tokens and is reported (SLHIP_ERR_CACHE); one with too many rows drops them all, of one that does not fit dropped is 0.
+ * Where a row's target logits hold a NaN or +inf, or nothing above -inf, or its temperature is NaN, its draft is refused and its
+ * token is -1 with a NaN; where its draft logits do, or their draft_temperature is NaN, the draft is refused and the token drawn from
+ * p (without draft logits no draft_temperature counts). A draft outside the vocabulary that is reached is refused and reported
+ * (SLHIP_ERR_INDEX) by the next slhip_stream_sync. A request that does not fit the rows, or has more of them than out_stride, gets no
+ * tokens and is reported (SLHIP_ERR_CACHE); one with too many rows drops them all, of one that does not fit dropped is 0.
+ * Without requests nothing is read or written.
  * target, draft: f32 or bf16 (dtype), rows of `vocab` logits with a stride; a row's sum and its weights are of f32 exponentials, of which
  * e is off by (2 + |log2 e|) 2^-23 of itself at most (above 2^-6 of f64 ones where p - q is taken); all that follows is f64. ids, starts, past, out, n_out, kept, dropped: int32.
  * work: workspace of work_bytes >= slhip_draft_verify_work_bytes(...) (enough for every smaller batch too), 16-byte aligned; calls that

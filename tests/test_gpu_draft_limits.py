@@ -1,11 +1,13 @@
-"""Draft verification where its numbers are at their ends."""
+"""Draft verification where its numbers are at their ends: random numbers of 0 and 1 beside tokens far below the others, drafts that hold nearly
+all of p, sums of many small terms, the largest temperature, rows and temperatures that cannot be used. The 64-bit statement is
+tests/step_ref.py's."""
 import numpy as np
 import pytest
 
 from sharplight_amd import native
 from tests import step_ref
 from tests.devutil import Dev, log
-from tests.test_gpu_draft import Case
+from tests.test_gpu_draft import NEAR, Case
 from tests.test_gpu_lora import held
 
 pytestmark = pytest.mark.gpu
@@ -185,6 +187,30 @@ def test_a_bad_draft_of_a_row_that_cannot_be_used_is_reported(device, x, why, dr
         native.synchronize()
         out, n = d.get(c.at["out"], (3, 3), np.int32), d.get(c.at["n_out"], (3,), np.int32)
     assert n[1] == 1 and (out[1] == -1).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_draft_temperature_that_is_not_a_number(device, dtype):
+    """Counts as draft logits that cannot be used: the draft is refused, the token drawn from p. Without draft logits none is looked at."""
+    c = Case("nan draft temperature", [3, 2, 1], 5000, dtype, True, [1.0], [1.0], good=1.0, size=5.0, settle=False)
+    c.tau_q[:2] = np.nan
+    c.accept[:], c.sample[:] = 0.0, 0.6
+    want = c.statement()
+    assert want[5] > NEAR and want[1].tolist() == [1, 1, 1]
+    with Dev() as d:
+        args, more = c.put(d)
+        log(f"draft_verify NaN draft temperature {dtype}")
+        native.draft_verify(*args, **more)
+        native.synchronize()
+        c.check(d, want=want)
+        c.q, c.draft = None, None
+        want = c.statement(tau_q=None)
+        assert want[5] > NEAR and want[1].tolist() == [3, 2, 1]
+        args, more = c.put(d)
+        log(f"draft_verify NaN draft temperature, no draft logits {dtype}")
+        native.draft_verify(*args, **more)
+        native.synchronize()
+        c.check(d, want=want)
 
 
 # ---- lengths -------------------------------------------------------------------------------------------------------
