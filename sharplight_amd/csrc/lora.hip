@@ -336,7 +336,7 @@ template <int DT, int N> struct Run {
 
 // ---- h = A x -------------------------------------------------------------------------------------------------------
 
-template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads) void lora_shrink(LoraArgs a)
+template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads) void lora_shrink(LoraArgs a, int32_t pieces)
 {
     constexpr int TM = 16 * MT, PX = kParts<XT>, PW = kParts<WT>;
     constexpr int U = MT * RB == 1 ? 4 : MT * RB == 8 && WT == SLHIP_F32 ? 1 : MT == 1 || XT == SLHIP_BF16 ? 2 : 1;  // units whose loads are on their way together
@@ -352,7 +352,7 @@ template <int XT, int WT, int MT, int RB> __global__ __launch_bounds__(kThreads)
                 raise_error(a.err, kErrAdapter, static_cast<uint32_t>(i), static_cast<uint32_t>(a.adapter[i]), static_cast<uint32_t>(a.adapters), 0, 0, 0);
         }
     }
-    const int32_t splits = a.plan ? a.plan->splits : a.splits, work = a.plan ? a.plan->tiles * splits * a.rank_blocks : gridDim.x;
+    const int32_t splits = a.plan ? a.plan->splits : a.splits, work = a.plan ? a.plan->tiles * splits * a.rank_blocks : pieces;
     const auto piece = [&](int32_t item) __attribute__((always_inline)) {
     const int32_t rb = item % a.rank_blocks, rest = item / a.rank_blocks, split = rest % splits;
     const int32_t key = find_tile<TM>(a, rest / splits, s_rows);
@@ -499,7 +499,7 @@ constexpr int kLane = 4;  // columns of a lane: 8 of bf16 take 256 registers wit
 // Rows are the first operand here and columns the second. A wave has 64 columns of its rows: product u the columns 4 c + u, so that a
 // lane's sums of the four products are neighbours in a row, and 16 lanes load and store whole lines of it. Row 4 r + g of 16 stands in the operand's
 // place 4 g + r: lane (c, g) has it in element r, and of up to four rows (a decode step's, most often one) all lie in element 0.
-template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThreads) void lora_expand(LoraArgs a)
+template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThreads) void lora_expand(LoraArgs a, int32_t pieces)
 {
     constexpr int TM = 16 * MT, PW = kParts<WT>, E = kLane, kColumns = 16 * E;
     // h's parts of RC ranks are the first operands of H instructions: up to 16 ranks two parts share one, more have one each
@@ -507,7 +507,7 @@ template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThrea
     __shared__ int32_t s_rows[TM];
     extern __shared__ uint4 s_h[];  // [MT][all][H][64]
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), c = lane & 15, g = lane >> 4;
-    const int32_t col_blocks = a.plan ? a.plan->col_blocks : a.col_blocks, work = a.plan ? a.plan->tiles * col_blocks : gridDim.x;
+    const int32_t col_blocks = a.plan ? a.plan->col_blocks : a.col_blocks, work = a.plan ? a.plan->tiles * col_blocks : pieces;
     const auto piece = [&](int32_t item) __attribute__((always_inline)) {
     const int32_t cb = item % col_blocks;
     const int32_t key = find_tile<TM>(a, item / col_blocks, s_rows);
@@ -697,19 +697,22 @@ static int64_t work_of(int64_t T, int64_t R)
     return (T * kMostSplits < most ? T * kMostSplits : most) * round16(R) * 4 + plan_of(T);
 }
 
-template <int XT, int WT, int MT> static int shrink(const LoraArgs& a, int64_t blocks, hipStream_t st)
+// A launch has less than 2^32 threads: beyond that thread blocks take turns. (Pieces are 2^28 at most: 2^31 rows in tiles of 32, by four ranges of ranks.)
+static unsigned blocks_of(int64_t pieces) { return static_cast<unsigned>(pieces < 0xFFFFFF ? pieces : 0xFFFFFF); }
+
+template <int XT, int WT, int MT> static int shrink(const LoraArgs& a, int64_t pieces, hipStream_t st)
 {
     const auto kernel = a.R16 <= 16 ? lora_shrink<XT, WT, MT, 1> : a.R16 <= 32 ? lora_shrink<XT, WT, MT, 2> : lora_shrink<XT, WT, MT, 4>;
-    kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(a);
+    kernel<<<blocks_of(pieces), kThreads, 0, st>>>(a, static_cast<int32_t>(pieces));
     return check_launch("lora_shrink");
 }
 
-template <int YT, int WT, int MT> static int expand(const LoraArgs& a, int64_t blocks, hipStream_t st)
+template <int YT, int WT, int MT> static int expand(const LoraArgs& a, int64_t pieces, hipStream_t st)
 {
     constexpr int P = YT == SLHIP_BF16 ? 2 : 3;
     const int lds = MT * 1024 * (a.R16 <= 16 ? P - 1 : (a.R + 31) / 32 * P);  // at most 48 KB
     const auto kernel = a.R16 <= 16 ? lora_expand<YT, WT, MT, false> : lora_expand<YT, WT, MT, true>;
-    kernel<<<static_cast<unsigned>(blocks), kThreads, lds, st>>>(a);
+    kernel<<<blocks_of(pieces), kThreads, lds, st>>>(a, static_cast<int32_t>(pieces));
     return check_launch("lora_expand");
 }
 
@@ -746,7 +749,6 @@ template <int WT, int MT> static int launch(int dtype_x, int dtype_y, LoraArgs& 
     } else {
         a.plan = nullptr;
     }
-    if (first > 0xFFFFFF || second > 0xFFFFFF) return fail(SLHIP_ERR_UNSUPPORTED, "lora: too many rows");
     const int e = dtype_x == SLHIP_F32 ? shrink<SLHIP_F32, WT, MT>(a, first, st) : shrink<SLHIP_BF16, WT, MT>(a, first, st);
     if (e) return e;
     return dtype_y == SLHIP_F32 ? expand<SLHIP_F32, WT, MT>(a, second, st) : expand<SLHIP_BF16, WT, MT>(a, second, st);
