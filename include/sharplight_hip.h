@@ -629,7 +629,7 @@ SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64_t target_s
  * first rank[a] ranks count (the others may hold anything). x [T, K] f32 or bf16 (dtype_x), add and y [T, N] (dtype_y), row strides
  * in elements; add may be y (in place: rows without an adapter are then not touched) or NULL (0); y overlaps nothing else. Rows from starts[B] on are padding: neither
  * read nor written. starts[0] is 0 and starts never falls; starts, adapter and rank are int32 on the device.
- * A x is summed and held in f32 (for bf16 y B takes it in two bf16 parts, to 2^-17 of itself); y is rounded once. A row
+ * A x is summed and held in f32, all bits of which B is multiplied with; y is rounded once. A row
  * that holds an infinity or a NaN gives no finite values; no other row's change.
  * An adapter outside [-1, adapters) counts as -1 and is reported (SLHIP_ERR_INDEX) by the next slhip_stream_sync; a request
  * that does not fit the rows is left as it was and reported (SLHIP_ERR_CACHE).

@@ -19,9 +19,8 @@
 // Made in one launch, each thread block its own h, a row takes 10.5 and the 64 requests 22.
 //
 // Numbers. All products are of bf16 numbers on the matrix cores, with f32 sums. A number of another type is the sum of bf16 ones, exactly:
-// f16 of two, f32 of three, each the last one's remainder cut to 8 bits; a product takes all pairs. h stays f32; for f32
-// results it goes on in three parts, for bf16 ones in two (2^-17 of itself, against the result's 2^-8). Two parts of 16 ranks fill the two
-// halves of one instruction's 32 products.
+// f16 of two, f32 of three, each the last one's remainder cut to 8 bits; a product takes all pairs. h is f32 and goes on in three
+// parts. Two parts of 16 ranks fill the two halves of one instruction's 32 products.
 #include <type_traits>
 
 #include "kv8_map.hpp"
@@ -491,9 +490,6 @@ template <int DT, int E> struct Piece {
     }
 };
 
-// The two bf16 parts of v, rounded: what is left of an infinity is 0.
-__device__ __forceinline__ float low_part(float v, float hi) { return fabsf(hi) < INFINITY ? v - hi : 0.0f; }
-
 constexpr int kLane = 4;  // columns of a lane: 8 of bf16 take 256 registers with their sums, and two waves a SIMD are too few
 
 // Rows are the first operand here and columns the second. A wave has 64 columns of its rows: product u the columns 4 c + u, so that a
@@ -502,8 +498,8 @@ constexpr int kLane = 4;  // columns of a lane: 8 of bf16 take 256 registers wit
 template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThreads) void lora_expand(LoraArgs a, int32_t pieces)
 {
     constexpr int TM = 16 * MT, PW = kParts<WT>, E = kLane, kColumns = 16 * E;
-    // h's parts of RC ranks are the first operands of H instructions: up to 16 ranks two parts share one, more have one each
-    constexpr int P = YT == SLHIP_BF16 ? 2 : 3, H = WIDE ? P : P - 1, RC = WIDE ? 32 : 16;
+    // h's three parts of RC ranks are the first operands of H instructions: up to 16 ranks two of them share one, more have one each
+    constexpr int H = WIDE ? kParts<SLHIP_F32> : 2, RC = WIDE ? 32 : 16;
     __shared__ int32_t s_rows[TM];
     extern __shared__ uint4 s_h[];  // [MT][all][H][64]
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id(), c = lane & 15, g = lane >> 4;
@@ -653,20 +649,11 @@ template <int YT, int WT, int MT, bool WIDE> __global__ __launch_bounds__(kThrea
         if (part > 0) continue;
         uint4* const put = s_h + ((m * all + q) * H) * 64 + l;  // WIDE: an operand a part, else lanes l and l + 32 of one
         constexpr int kNext = WIDE ? 64 : 32;
-        if constexpr (P == 2) {
-            float lo[8];
-            put[0] = Vec<SLHIP_BF16>::pack(f);
-            Vec<SLHIP_BF16>::unpack(put[0], lo);
+        bf16x8 p[kParts<SLHIP_F32>];
+        cut(f, p);
 #pragma unroll
-            for (int e = 0; e < 8; e++) lo[e] = low_part(f[e], lo[e]);
-            put[kNext] = Vec<SLHIP_BF16>::pack(lo);
-        } else {
-            bf16x8 p[3];
-            cut(f, p);
-#pragma unroll
-            for (int i = 0; i < 3; i++) put[kNext * i] = __builtin_bit_cast(uint4, p[i]);
-            if (!WIDE) put[96] = make_uint4(0, 0, 0, 0);
-        }
+        for (int i = 0; i < kParts<SLHIP_F32>; i++) put[kNext * i] = __builtin_bit_cast(uint4, p[i]);
+        if (!WIDE) put[kNext * kParts<SLHIP_F32>] = make_uint4(0, 0, 0, 0);
     }
     __syncthreads();
     for (int32_t n0 = first; n0 < a.N; n0 += step) {
@@ -709,8 +696,7 @@ template <int XT, int WT, int MT> static int shrink(const LoraArgs& a, int64_t p
 
 template <int YT, int WT, int MT> static int expand(const LoraArgs& a, int64_t pieces, hipStream_t st)
 {
-    constexpr int P = YT == SLHIP_BF16 ? 2 : 3;
-    const int lds = MT * 1024 * (a.R16 <= 16 ? P - 1 : (a.R + 31) / 32 * P);  // at most 48 KB
+    const int lds = MT * 1024 * (a.R16 <= 16 ? 2 : (a.R + 31) / 32 * kParts<SLHIP_F32>);  // at most 48 KB
     const auto kernel = a.R16 <= 16 ? lora_expand<YT, WT, MT, false> : lora_expand<YT, WT, MT, true>;
     kernel<<<blocks_of(pieces), kThreads, lds, st>>>(a, static_cast<int32_t>(pieces));
     return check_launch("lora_expand");

@@ -5,9 +5,48 @@ import pytest
 from sharplight_amd import native
 from tests import step_ref
 from tests.devutil import Dev, log
-from tests.test_gpu_lora import held, values
+from tests.test_gpu_lora import NP, TYPES, Case, held, values
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("x,w,y", TYPES)
+@pytest.mark.parametrize("new,rank", [(1, 16), (3, 40), (70, 16), (70, 33)])
+def test_h_keeps_its_24_bits(device, new, rank, x, w, y):
+    """h = (1 + 2^-10 + 2^-20, -1, -2^-10) whose sum is 2^-20: what is held of h in 16 bits leaves 0 of it."""
+    K, N = 64, 72
+    c = Case("bits", [new], [0], 1, rank, K, N, x, w, y)
+    c.vx[:], c.va[:], c.vb[:], c.vadd[:] = 0, 0, 0, 0
+    c.vx[:, :3] = [1.0, 2.0 ** -10, 2.0 ** -20]
+    c.va[0, 0, :3], c.va[0, 1, 0], c.va[0, rank - 1, 1] = 1.0, -1.0, -1.0
+    c.vb[0, :, [0, 1, rank - 1]] = 1.0
+    (c.x, c.vx), (c.a, c.va), (c.b, c.vb), (c.add, c.vadd) = (held(v, t) for v, t in ((c.vx, x), (c.va, w), (c.vb, w), (c.vadd, y)))
+    with Dev() as d:
+        args, more = c.put(d)
+        log(f"lora bits of h {x}/{w}/{y} rank={rank} rows={new}")
+        native.lora(*args, **more)
+        native.synchronize()
+        got = values(d.get(c.py, (c.T, N), NP[y]), y)
+    assert (got == 2.0 ** -20).all(), got[0, :4]
+
+
+@pytest.mark.parametrize("x,w,y", TYPES)
+def test_rows_beside_ones_that_are_not_finite(device, x, w, y):
+    """Within the bound of their own type's result."""
+    c = Case("beside", [40, 1, 1], [0, 1, 1], 2, 16, 64, 48, x, w, y)
+    clean, bound = c.expected()
+    bad = {7: np.inf, 20: np.nan, 41: -np.inf}
+    for r, v in bad.items():
+        c.x[r, 3] = held(np.float64([v]), x)[0][0]
+    with Dev() as d:
+        args, more = c.put(d)
+        log(f"lora beside rows that are not finite {x}/{w}/{y}")
+        native.lora(*args, **more)
+        native.synchronize()
+        got = values(d.get(c.py, (c.T, c.N), NP[y]), y)
+    others = [t for t in range(c.T) if t not in bad]
+    assert (np.abs(got - clean)[others] <= step_ref.rounded_bound(clean, bound, y)[others]).all()
+    assert not np.isfinite(got[list(bad)]).any()
 
 
 def test_more_rows_than_a_launch_has_thread_blocks(device):
