@@ -464,7 +464,9 @@ SLHIP_API int slhip_cache_write(int dtype_in, int dtype_cache, const void* x, in
  *   keep(i) = ceil(past[i] / block_size), back(i) = ceil((past[i] + count[i]) / block_size) - keep(i) of them, o(i) = back(0) + ..
  *   + back(i-1), go back on the stack: free_blocks[*n_free + o(B) - 1 - (o(i) + j)] = pages[slot, keep(i) + j] for j < back(i),
  *   their table entries become -1, and *n_free_out = *n_free + o(B). Where all that an advance took goes back in the same
- *   order of requests, the free list is as it was before. starts, seq, pos and tokens are not used.
+ *   order of requests, the free list is as it was before. starts, seq, pos and tokens are not used. Only the tables step back: a block
+ *   of the 8-bit cache that keeps some of its tokens keeps what the others did to it (a larger scale, to which its codes were rounded;
+ *   NaN where one of them was not finite), until its tokens are written again from its first one on.
  *
  * n_free_out may be n_free itself (one counter that the steps of a captured loop advance) or another word (the old count
  * stays, to step back to). All or nothing, for each of the three: where a length is negative, a context would outgrow its table row or the rows
