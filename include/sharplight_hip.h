@@ -632,9 +632,9 @@ SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64_t target_s
  * in elements; add may be y (in place: rows without an adapter are then not touched) or NULL (0); y overlaps nothing else. Rows from starts[B] on are padding: neither
  * read nor written. starts[0] is 0 and starts never falls; starts, adapter and rank are int32 on the device.
  * A x is summed and held in f32, all bits of which B is multiplied with; y is rounded once. A row
- * that holds an infinity or a NaN gives no finite values; no other row's change.
+ * that holds an infinity or a NaN gives no finite values where its adapter has a rank; no other row's change.
  * An adapter outside [-1, adapters) counts as -1 and is reported (SLHIP_ERR_INDEX) by the next slhip_stream_sync; a request
- * that does not fit the rows is left as it was and reported (SLHIP_ERR_CACHE).
+ * that does not fit the rows is left as it was and reported (SLHIP_ERR_CACHE). Without rows (tokens 0) or requests nothing is looked at.
  * work: workspace of work_bytes >= slhip_lora_work_bytes(tokens, max_rank) (enough for fewer tokens and ranks too), 16-byte
  * aligned; calls that may overlap each need their own. It needs no initialisation and keeps nothing.
  * max_rank <= 256, K and N 8 .. 2^24, a matrix of an adapter less than 2^31 bytes, strides of add and y

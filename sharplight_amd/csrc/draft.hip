@@ -14,10 +14,11 @@
 // way), 16 of them are added in f32, everything behind them in f64: the rows' sums, p(x), q(x), and the weights drawn from, whose differences
 // p - q are of f64 exponentials where they may cancel.
 //
-// Measured: the sums of 257 rows of 151936 f32 logits and of 193 draft rows (273 MB) 45.5 us, 6.0 TB/s; of 256 rows of 50257 bf16 logits
-// (25.7 MB) 11.4 us, of which some 3.5 are exponentials that the loads, all on their way at once, do not hide, of 64 rows 5.9. What follows is a
-// latency: 256 or 64 draws 6.6 to 6.7 us in one launch (choose); 64 requests with draft logits 5.4 (decide), 12.6 (2432 chunks of p and q,
-// 78 MB out of the last-level cache) and 6.2 (pick); one request with drafts 6.2 (38 chunks that decide for themselves) and 4.7.
+// Measured: the sums of 257 rows of 151936 f32 logits and of 193 draft rows (273 MB) 45.6 us, 6.0 TB/s, in bf16 (137 MB) 30.3, of which the vector
+// unit works 89%; of 256 rows of 50257 bf16 logits (25.7 MB) 11.4 us, of which some 3.5 are exponentials that the loads, all on their way at once, do not
+// hide, of 64 rows 5.9. What follows is a latency: 256 or 64 draws 6.7 us in one launch (choose), 16 requests' looked-up drafts 7.1; 64 requests with draft
+// logits 5.5 (decide), 13.2 (2432 chunks of p and q, 78 MB out of the last-level cache; bf16 14.0) and 6.2 (pick; bf16 8.1); one request with drafts 6.4 (38
+// chunks that decide for themselves) and 4.3.
 #include <math.h>
 
 #include "step.hpp"

@@ -9,14 +9,16 @@
 // (no more than its rows alone would make), so a launch is sized from rows and requests (item_base). Up to 64
 // requests a wave looks at all of them at once, a lane each, and every thread block finds its rows so; of more, a launch before (lora_plan)
 // lists the tiles, and the others share out what there is: 256 requests that share 8 adapters are 17 tiles, of 272 that there might be.
-// With mfma 16x16x32 (A[m][8g+j], B[8g+j][n], C[4g+r][n] in lane (n or m) + 16 g) adapters are the first operand and rows the
-// second one, so that a lane's sums are four neighbours of one row: h is stored and y made without an exchange.
+// With mfma 16x16x32 (A[m][8g+j], B[8g+j][n], C[4g+r][n] in lane (n or m) + 16 g) the first product has adapters as the first operand and rows
+// as the second one, so that a lane's sums are four neighbours of one row of h; the second product has rows first (lora_expand).
 //
-// Measured, in us: one row of 16 ranks, [4096, 4096] in bf16: 5.0 + 6.0 (latencies: lengths -> adapter -> weights, twice); 64 requests with
-// an adapter each into 14336 outputs: 6.4 + 13.7 (38 MB of adapters); 256 requests that share 8 of 64 ranks, f32 [4096, 14336]: 5.4 for the list, 12.8
-// + 9.1; 23 requests' 2194 rows, f32 with f16 adapters of 24 ranks [4104, 2880]: 12.1 + 24.6 (25 and 70 MB); a prompt of 8192 into
-// 14336 outputs in bf16: 16.5 (69 MB) + 97 (470 MB, 4.8 TB/s; a kernel that only copies rows in pieces as short as these takes 81 to 95).
-// Made in one launch, each thread block its own h, a row takes 10.5 and the 64 requests 22.
+// Measured, in us: one row of 16 ranks, [4096, 4096] in bf16: 4.6 + 6.0 (latencies: lengths -> adapter -> weights, twice); 64 requests with
+// an adapter each into 14336 outputs: 6.4 + 13.4 (38 MB of adapters), with f32 adapters 8.3 + 21.7 (75 MB); 256 requests that share 8 of 64 ranks, f32
+// [4096, 14336]: 4.8 for the list, 12.2 + 8.8; 23 requests' 2194 rows, f32 with f16 adapters of 24 ranks [4104, 2880]: 11.7 + 23.8 (25 and 70 MB); a prompt
+// of 8192 into 14336 outputs in bf16: 16.2 (69 MB) + 96.8 (470 MB, 4.9 TB/s; a kernel that only copies rows in pieces as short as these takes 81 to 95).
+// Made in one launch, each thread block its own h, a row takes 10.5 and the 64 requests 22. One thread block writes the list, and one lane of it the keys of an
+// adapter's tiles: of long requests that share an adapter it takes more than products of [64, 64] (100 requests of 184 rows 20 us, the products 12; 300 of 3700
+// 916 and 345).
 //
 // Numbers. All products are of bf16 numbers on the matrix cores, with f32 sums. A number of another type is the sum of bf16 ones, exactly:
 // f16 of two, f32 of three, each the last one's remainder cut to 8 bits; a product takes all pairs. h is f32 and goes on in three
