@@ -209,7 +209,7 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
     // where drafts are chosen, the chunk that holds the row's is summed without it, and its own power added at the end
     int32_t drafted = -1;
     if (mat == 0 && !target.greedy && t + 1 < min(static_cast<int64_t>(a.starts[i + 1]), a.T) && (!DRAFT || (a.tau_q && a.tau_q[i] <= 0.0f))) drafted = a.ids[t + 1];
-    const bool holds = drafted >= 0 && drafted / kChunk<DT> == chunk;
+    const bool holds = drafted >= 0 && drafted < a.V && drafted / kChunk<DT> == chunk;
     float z[Mine::kEach];
 #pragma unroll
     for (int j = 0; j < kVecs; j++) Vec<DT>::unpack(x.w[j], &z[j * N]);

@@ -190,6 +190,27 @@ def test_a_bad_draft_of_a_row_that_cannot_be_used_is_reported(device, x, why, dr
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [1, 7, 5000, 8191])
+@pytest.mark.parametrize("behind", [0, 1, 8])
+def test_a_chosen_draft_behind_the_vocabulary(device, behind, V, dtype):
+    """In what would be the last chunk: refused and reported, and what lies behind the row's logits (NaN, or nothing) is not looked at."""
+    c = Case("behind", [2, 2, 2], V, dtype, False, [1.0, 0.6], settle=False)
+    c.ids[1::2] = V + behind
+    c.sample[:] = [0.2, 0.5, 0.9]
+    want = c.statement()
+    assert want[5] > NEAR and (want[1] == 1).all()
+    for stride in (V, V + 24):
+        with Dev() as d:
+            args, more = c.put(d, target_stride=stride)
+            log(f"draft_verify chosen draft {V + behind} of {V}, stride {stride} {dtype}")
+            native.draft_verify(*args, **more)
+            with pytest.raises(IndexError, match="number 0 of request"):
+                native.synchronize()
+            native.synchronize()
+            c.check(d, want=want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_a_draft_temperature_that_is_not_a_number(device, dtype):
     """Counts as draft logits that cannot be used: the draft is refused, the token drawn from p. Without draft logits none is looked at."""
     c = Case("nan draft temperature", [3, 2, 1], 5000, dtype, True, [1.0], [1.0], good=1.0, size=5.0, settle=False)
