@@ -582,8 +582,8 @@ SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q_stride_t, 
  *   drawn from. Without draft logits, or where draft_temperature[i] <= 0, the draft was chosen: q_t is 1 there.
  *   Draft x of row t is accepted while accept[t] * q_t(x) < p_t(x). Behind the accepted ones comes one more token, from the row
  *   of the first refused draft or the last row: of weights max(p - q, 0) (the last row, or weights that are all 0: p) it is the
- *   first v whose sum over 0 .. v is above sample[i] times the sum of all, or the last one with a weight. (What has less than 2^-100 of the
- *   row's largest probability may count as 0 here. A logit of -inf is never drawn.)
+ *   first v whose sum over 0 .. v is above sample[i] times the sum of all, or the last one with a weight. (What has less than 2^-900 of the
+ *   row's largest probability may count as 0 here, and so may 4096 or 8192 neighbours' p - q below 2^-36 of their p. A logit of -inf is never drawn.)
  *   temperature[i] <= 0: a draft is accepted while it is the lowest v with the largest logit, and that is the token behind; no random
  *   number and no draft logits count. Logits of -inf have the probability 0. Temperatures count as 2^-40 .. 2^40.
  *   out[i, 0 ..]: the accepted drafts and the token, then -1 up to out_stride; n_out[i] their number (0 for a request of no rows);
@@ -595,8 +595,8 @@ SLHIP_API int slhip_kv8_attention(int dtype, const void* q, int64_t q_stride_t, 
  * (SLHIP_ERR_INDEX) by the next slhip_stream_sync. A request that does not fit the rows, or has more of them than out_stride, gets no
  * tokens and is reported (SLHIP_ERR_CACHE); one with too many rows drops them all, of one that does not fit dropped is 0.
  * Without requests nothing is read or written.
- * target, draft: f32 or bf16 (dtype), rows of `vocab` logits with a stride; a row's sum and its weights are of f32 exponentials, of which
- * e is off by (2 + |log2 e|) 2^-23 of itself at most (above 2^-6 of f64 ones where p - q is taken); all that follows is f64. ids, starts, past, out, n_out, kept, dropped: int32.
+ * target, draft: f32 or bf16 (dtype), rows of `vocab` logits with a stride. What is drawn by is f64, of exponentials that are off by 2^-39 of
+ * themselves at most; p and q that a drawn draft is accepted by are of f32 exponentials, of which e is off by (2 + |log2 e|) 2^-23 of itself at most. ids, starts, past, out, n_out, kept, dropped: int32.
  * work: workspace of work_bytes >= slhip_draft_verify_work_bytes(...) (enough for every smaller batch too), 16-byte aligned; calls that
  * may overlap each need their own. It needs no initialisation and keeps nothing. requests <= 65536, vocab <= 2^24,
  * tokens * ceil(vocab / 4096) < 2^23, requests * ceil(vocab / 4096) < 2^24. starts[0] is 0 and starts never falls. out, n_out, kept, dropped and

@@ -5,14 +5,16 @@
 // max(p - q, 0) of the refused draft's row, or p of the last row: the first v whose inclusive sum is above w times the sum of all.
 //
 // Every row's S is needed for its p(x), so the rows are read once for their sums (HBM bounds it), in chunks that lie in
-// registers: a chunk's maximum first, then one exponential a logit, no running rescale. Which row is drawn from follows from all
+// registers: a wave's maximum first, then one exponential a logit, no running rescale. Which row is drawn from follows from all
 // of a request's sums. The sums of p's chunks are there already; those of max(p - q, 0) take that one row of both a second time. The
 // place in a chunk takes it once more.
 //
-// Numbers. A choice changes where a sum passes a random number, so what two implementations may differ in is kept small:
-// exponentials are f32 of arguments with one rounding (log2(e) / tau in two parts, or all terms of a sum would be off the same
-// way), 16 of them are added in f32, everything behind them in f64: the rows' sums, p(x), q(x), and the weights drawn from, whose differences
-// p - q are of f64 exponentials where they may cancel.
+// Numbers. A choice changes where a sum passes a random number. An acceptance has one such border, p(x): f32 exponentials (of arguments with one rounding:
+// log2(e) / tau in two parts, or all terms of a sum would be off the same way), 16 of them added in f32 and the rest in f64, move it by some 2^-24, and are what rows
+// that are compared with draft logits have. A draw has as many borders as there are tokens, so that one of them lies within 2^-26 of the random number in one
+// draw of some thousands (sums of f32 exponentials gave another token than f64's in 2e-4 to 3e-4 of the draws from 50257 to 151936 tokens): all that is drawn by is of f64
+// exponentials to 2^-39. Those are the sums of the rows that may be drawn from as they are (a request's last one, and all without draft logits), and what is made of
+// the one row behind a refused draft.
 //
 // Measured: the sums of 257 rows of 151936 f32 logits and of 193 draft rows (273 MB) 45.6 us, 6.0 TB/s, in bf16 (137 MB) 30.3, of which the vector
 // unit works 89%; of 256 rows of 50257 bf16 logits (25.7 MB) 11.4 us, of which some 3.5 are exponentials that the loads, all on their way at once, do not
@@ -34,17 +36,23 @@ template <int DT> constexpr int kChunk = kChunkVecs * Vec<DT>::N;  // logits of 
 
 struct ChunkStat {
     float m;      // the largest logit; NaN where the chunk holds a NaN or an infinity above
-    int32_t arg;  // its first place (rows of greedy requests); the bits of the f32 sum without the row's draft (chosen drafts, of its chunk)
-    double s;     // sum of e^((z - m) / tau)
+    int32_t arg;  // its first place (rows of greedy requests)
+    double s;     // sum of e^((z - m) / tau), without the row's draft where that was chosen
 };
 
 // What is drawn for a request, and from what.
 enum : int32_t { kDone = 0, kFromTarget = 1, kFromRest = 2, kFromOthers = 3 };  // nothing; p; max(p - q, 0); p without the draft
 struct Pick {
     int32_t kind, row, place, token;  // the row, its place in the request, its draft
-    double mp, cp, ip, mq, cq, iq;    // maxima, log2(e) / tau, 1 / sums
-    double rest;                      // sum of the draft's chunk without it, before the division
-    int32_t held, reserved;           // where its chunks' shares are held in LDS (-1: nowhere)
+    double mp, cp, sum, mq, cq, ratio;  // maxima, log2(e) / tau, the sum of p's powers, that sum / q's
+    double own;                       // the draft's power of p
+    int32_t held;                     // where its chunks' shares are held in LDS (-1: nowhere)
+    int32_t exact;                    // its sums of all rows are the ones to draw by
+};
+
+// A chunk of the drawn row, where drafts were drawn: sums of its powers of p and of q, of p - ratio q where that is above 0, and of q there.
+struct ChunkSums {
+    double p, q, rest, above;
 };
 
 struct DraftArgs {
@@ -61,7 +69,7 @@ struct DraftArgs {
     float* logp;
     ChunkStat* stats;  // [T][2][chunks]
     Pick* picks;       // [B]
-    double* sums;      // [B][chunks]
+    ChunkSums* sums;   // [B][chunks]
     uint32_t* err;
 };
 
@@ -151,39 +159,95 @@ __device__ __forceinline__ double wave_scan64(double v)
     return v + dpp64<0x143, 0xC>(v);
 }
 
-// 2^y to 2^-36 of itself for y <= 0 (0 below -1000): the series of 2^f, |f| <= 1/2.
-__device__ __forceinline__ double exp2_64(double y)
+// Of lanes that are alike in l & 3, in every one of them.
+__device__ __forceinline__ double sum_by_four(double v)
 {
-    const double n = rint(y), f = (y - n) * 0.693147180559945309417;
-    double r = 1.0 / 362880.0;
-    r = fma(r, f, 1.0 / 40320.0);
-    r = fma(r, f, 1.0 / 5040.0);
-    r = fma(r, f, 1.0 / 720.0);
-    r = fma(r, f, 1.0 / 120.0);
-    r = fma(r, f, 1.0 / 24.0);
-    r = fma(r, f, 1.0 / 6.0);
-    r = fma(r, f, 0.5);
-    r = fma(r, f, 1.0);
-    r = fma(r, f, 1.0);
-    return y < -1000.0 ? 0.0 : ldexp(r, static_cast<int>(n));
+    v += dpp64<0x124>(v);  // a row's quads: it turned by 4 and by 8
+    v += dpp64<0x128>(v);
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+// Four sums over the wave together, number l & 3 in lane l: each step over lanes also halves what a lane holds.
+__device__ __forceinline__ double wave_sums64(const double (&s)[4])
+{
+    const int lane = threadIdx.x & 63;
+    const bool odd = lane & 1, high = lane & 2;
+    const double a = (odd ? s[1] : s[0]) + dpp64<0xB1>(odd ? s[0] : s[1]), b = (odd ? s[3] : s[2]) + dpp64<0xB1>(odd ? s[2] : s[3]);
+    return sum_by_four((high ? b : a) + dpp64<0x4E>(high ? a : b));
 }
 
 constexpr double kLog2e64 = 1.44269504088896340736;
 
-// log2(e) / tau as f32 parts, the second one positive: -inf times it is -inf.
-struct Factor {
-    float hi, lo;
-    __device__ __forceinline__ explicit Factor(double c)
+// e^((z - m) / tau) = 2^((z - m) c) of z <= m, to 2^-39 of itself, and not below 2^-1000. 2^f, |f| <= 1/2, is the polynomial of degree 8 that is 1 at 0 and whose
+// largest relative error is least (2^-39.7; found by exchange of that error's extrema).
+constexpr int kTogether = 4;
+constexpr double kNone = 0x1p-999;  // 2^-1000, of a rounded factor
+struct Power {
+    double m, c, least;
+    __device__ __forceinline__ Power(double m_, double c_) : m(m_), c(c_), least(-1000.0f * __builtin_amdgcn_rcpf(static_cast<float>(c_))) {}
+    // Of K logits step by step together (a step waits for the one before), as 2^f and the power of two that it is to be multiplied with.
+    template <int K> __device__ __forceinline__ void parts(const float* z, double (&w)[K], double (&scale)[K]) const
+    {
+        // what is added to it is rounded to a whole number, in the lower bits: here with an exponent's bias
+        constexpr double kWhole = 0x1.8p52 + 1023;
+        constexpr double kTerm[] = {0x1.66348837ae4fdp-20, 0x1.00ee071f2a659p-16, 0x1.4306c115fa167p-13, 0x1.5d872975bfeabp-10, 0x1.3b2ab7f3b35e4p-7,
+                                    0x1.c6b08defc2653p-5, 0x1.ebfbdff7c5a77p-3, 0x1.62e42fef7a78bp-1, 1.0};
+        double d[K];
+#pragma unroll
+        for (int e = 0; e < K; e++) d[e] = fmax(z[e] - m, least);
+#pragma unroll
+        for (int e = 0; e < K; e++) {
+            const double n = fma(d[e], c, kWhole);
+            d[e] = fma(d[e], c, kWhole - n);
+            scale[e] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, n) << 52);
+            w[e] = kTerm[0];
+        }
+#pragma unroll
+        for (int t = 1; t < 9; t++)
+#pragma unroll
+            for (int e = 0; e < K; e++) w[e] = fma(w[e], d[e], kTerm[t]);
+    }
+    template <int K> __device__ __forceinline__ void of(const float* z, double (&w)[K]) const
+    {
+        double scale[K];
+        parts(z, w, scale);
+#pragma unroll
+        for (int e = 0; e < K; e++) w[e] *= scale[e];
+    }
+    __device__ __forceinline__ double at(float z) const
+    {
+        double w[1];
+        of(&z, w);
+        return w[0];
+    }
+    // `to` and the power.
+    __device__ __forceinline__ double add(float z, double to) const
+    {
+        double w[1], scale[1];
+        parts(&z, w, scale);
+        return fma(w[0], scale[0], to);
+    }
+    // 0 for all that is as small, -inf among it.
+    __device__ __forceinline__ double or_none(float z) const
+    {
+        const double v = at(z);
+        return v > kNone ? v : 0.0;
+    }
+};
+
+// The same in f32: to (2 + |log2 e|) 2^-23 of itself, 0 below 2^-126. log2(e) / tau is taken as two parts, the second one positive: -inf times it is -inf. (An element
+// takes 8 issue slots so, in f64 18.)
+struct PowerF32 {
+    float m, hi, lo;
+    __device__ __forceinline__ PowerF32(float m_, double c) : m(m_)
     {
         const float near = static_cast<float>(c);
         hi = near > c ? __uint_as_float(__float_as_uint(near) - 1) : near;
         lo = fmaxf(static_cast<float>(c - hi), 0x1p-100f);  // (c is above 2^-40)
     }
-    // 2^(d c) for d <= 0, -inf included.
-    __device__ __forceinline__ float power(float d) const { return __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo)); }
+    __device__ __forceinline__ float at(float z) const { return __builtin_amdgcn_exp2f(fmaf(z - m, hi, (z - m) * lo)); }
 };
-
-__device__ __forceinline__ double share_of(float z, double m, double c) { return z == -INFINITY ? 0.0 : exp2_64((static_cast<double>(z) - m) * c); }
 
 // ---- the sums of all rows ------------------------------------------------------------------------------------------
 
@@ -203,13 +267,13 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
     const int32_t i = row_request(a.starts, a.B, t);
     const Heat target = heat_of(a.tau, i), h = mat == 0 || !a.tau_q ? target : heat_of(a.tau_q, i);
     if (mat == 1) {  // not of greedy requests, nor of the row that has no draft
-        if (target.greedy || h.greedy || t == a.starts[i + 1] - 1) return;
+        if (target.greedy || h.greedy || t + 1 >= a.starts[i + 1]) return;
         x.load(a.draft, t, a.qs, a.V, chunk);
     }
-    // where drafts are chosen, the chunk that holds the row's is summed without it, and its own power added at the end
-    int32_t drafted = -1;
-    if (mat == 0 && !target.greedy && t + 1 < min(static_cast<int64_t>(a.starts[i + 1]), a.T) && (!DRAFT || (a.tau_q && a.tau_q[i] <= 0.0f))) drafted = a.ids[t + 1];
-    const bool holds = drafted >= 0 && drafted < a.V && drafted / kChunk<DT> == chunk;
+    // Where drafts are chosen, the chunk that holds the row's is summed without it. Those rows and requests' last ones may be drawn from by these sums.
+    const bool last = t + 1 >= a.starts[i + 1], chosen = !DRAFT || (a.tau_q && a.tau_q[i] <= 0.0f);
+    const int32_t drafted = mat == 0 && !target.greedy && !last && chosen && t + 1 < a.T ? a.ids[t + 1] : -1;
+    const bool holds = drafted >= 0 && drafted < a.V && drafted / kChunk<DT> == chunk, exact = mat == 0 && !target.greedy && (last || chosen);
     float z[Mine::kEach];
 #pragma unroll
     for (int j = 0; j < kVecs; j++) Vec<DT>::unpack(x.w[j], &z[j * N]);
@@ -219,24 +283,25 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
     const bool bad = !(m < INFINITY);
     m = group_max<64>(m);
     if (__any(bad)) m = INFINITY;
-    if (lane == 0) s_m[wave] = m;
-    __syncthreads();
-    m = s_m[0];
-    for (int w = 1; w < kWaves; w++) m = fmaxf(m, s_m[w]);
-    const Factor c(kLog2e64 / h.tau);
-    float own = 0.0f;
     if (holds) {
-        own = Vec<DT>::load1(static_cast<const char*>(a.target) + t * a.zs * Vec<DT>::BYTES, drafted);
 #pragma unroll
         for (int j = 0; j < kVecs * N; j++) z[j] = Mine::place(chunk, j / N) + j % N == drafted ? -INFINITY : z[j];
     }
-    float s[kVecs * N / kTerms] = {};
+    const double c = kLog2e64 / h.tau;
+    double sum = 0.0;
+    if (!exact) {
+        const PowerF32 power(m, c);
+        float s[kVecs * N / kTerms] = {};
 #pragma unroll
-    for (int j = 0; j < kVecs * N; j++) s[j / kTerms] += c.power(z[j] - m);
-    double mine = s[0];
+        for (int j = 0; j < kVecs * N; j++) s[j / kTerms] += power.at(z[j]);
 #pragma unroll
-    for (int j = 1; j < kVecs * N / kTerms; j++) mine += s[j];
-    const double sum = wave_sum64(mine);
+        for (int j = 0; j < kVecs * N / kTerms; j++) sum += s[j];
+    } else {
+        const Power power(m, c);
+#pragma unroll
+        for (int j = 0; j < kVecs * N; j++) sum = power.add(z[j], sum);
+    }
+    sum = wave_sum64(sum);
     int32_t arg = 0x7FFFFFFF;
     if (target.greedy) {
 #pragma unroll
@@ -246,22 +311,21 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
         for (int o = 1; o < 64; o <<= 1) arg = min(arg, __shfl_xor(arg, o, 64));
     }
     if (lane == 0) {
+        s_m[wave] = m;
         s_s[wave] = sum;
         s_arg[wave] = arg;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        ChunkStat o{m == INFINITY ? NAN : m, s_arg[0], s_s[0]};
-        for (int w = 1; w < kWaves; w++) {
-            o.s += s_s[w];
-            o.arg = min(o.arg, s_arg[w]);
-        }
-        if (holds) {
-            o.arg = __float_as_int(static_cast<float>(o.s));
-            o.s += c.power(own - m);
-        }
-        if (m == -INFINITY) o.s = 0.0;
-        a.stats[(t * 2 + mat) * a.chunks + chunk] = o;
+    if (threadIdx.x < 64) {  // each wave's sum is of its own maximum; a lane each
+        const float mine = lane < kWaves ? s_m[lane] : -INFINITY;
+        m = group_max_dpp<16>(mine);
+        double v = mine > -INFINITY ? s_s[lane & (kWaves - 1)] * Power(m, c).at(mine) : 0.0;
+        v += dpp64<0xB1>(v);
+        v += dpp64<0x4E>(v);
+        arg = 0x7FFFFFFF;
+        for (int w = 0; w < kWaves; w++)
+            if (s_m[w] == m) arg = min(arg, s_arg[w]);
+        if (lane == 0) a.stats[(t * 2 + mat) * a.chunks + chunk] = ChunkStat{m == INFINITY ? NAN : m, arg, v};
     }
 }
 
@@ -269,7 +333,7 @@ template <int DT, bool DRAFT> __global__ __launch_bounds__(kThreads) void draft_
 
 // A row of a matrix: its maximum, its sum and 1 / sum, the lowest place of the maximum, whether it can be used; and its draft's logit and share.
 struct RowStat {
-    double m, s, inv, share;
+    double m, s, inv, share;  // (share: of its draft)
     int32_t arg;
     bool fine;
     float z;
@@ -277,9 +341,8 @@ struct RowStat {
 
 constexpr int kHeld = 4;  // chunks of a lane that it looks at once: a vocabulary of 262144
 
-// The chunks of a row together, by 16 lanes. arg: its first place is wanted. In units of the row's sum before its division, shares: of the first 64
-// chunks; rest: of chunk `holds` without the chosen draft in it (-1: there is none).
-__device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks, double c, bool arg, int32_t holds, double* rest, double* shares)
+// The chunks of a row together, by 16 lanes. arg: its first place is wanted; shares: of the first 64 chunks, in units of the row's sum before its division.
+__device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks, double c, bool arg, double* shares)
 {
     const int lane = threadIdx.x & 15;
     ChunkStat x[kHeld];
@@ -303,19 +366,19 @@ __device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks,
     r.m = m;
     double s = 0.0;
     int32_t first = 0x7FFFFFFF;
-    const auto take = [&](const ChunkStat& v, int32_t k) {
-        const double unit = exp2_64((static_cast<double>(v.m) - r.m) * c), part = v.m > -INFINITY ? v.s * unit : 0.0;
+    const Power power(r.m, c);
+    const auto take = [&](const ChunkStat& v) {
+        const double part = v.m > -INFINITY ? v.s * power.at(v.m) : 0.0;
         s += part;
-        if (k == holds) *rest = v.m > -INFINITY ? __int_as_float(v.arg) * unit : 0.0;
         if (v.m == m) first = min(first, v.arg);
         return part;
     };
 #pragma unroll
     for (int j = 0; j < kHeld; j++) {
-        const double part = take(x[j], lane + 16 * j);
+        const double part = take(x[j]);
         if (shares) shares[lane + 16 * j] = part;
     }
-    for (int32_t k = lane + 16 * kHeld; k < chunks; k += 16) take(st[k], k);
+    for (int32_t k = lane + 16 * kHeld; k < chunks; k += 16) take(st[k]);
     r.s = row_sum64(s);
     if (arg) {
 #pragma unroll
@@ -327,7 +390,6 @@ __device__ __forceinline__ RowStat row_stat(const ChunkStat* st, int32_t chunks,
 
 struct DecideLds {
     RowStat row[16];        // of a pass: target's rows, or target's and draft's in turns
-    double rest[16];        // of a refused draft's chunk
     double shares[16][64];  // of their first chunks, target's rows where no drafts were drawn
 };
 
@@ -357,12 +419,14 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
             float z = -INFINITY;
             if (v >= 0 && v < a.V) z = Vec<DT>::load1(mat ? a.draft : a.target, t * (mat ? a.qs : a.zs) + v);
             const double c = mat ? cq : cp;
-            const int32_t holds = !drawn && !hp.greedy && place < n - 1 && v >= 0 && v < a.V ? v / kChunk<DT> : -1;
-            RowStat r = row_stat(a.stats + (t * 2 + mat) * a.chunks, a.chunks, c, hp.greedy, holds, &lds.rest[group], SHARES ? lds.shares[group] : nullptr);
+            RowStat r = row_stat(a.stats + (t * 2 + mat) * a.chunks, a.chunks, c, hp.greedy, SHARES ? lds.shares[group] : nullptr);
             r.fine &= !(mat ? hq.bad : hp.bad);
             r.z = z;
+            const Power power(r.m, c);
+            const double own = power.or_none(z);
+            if (!drawn && !hp.greedy && place < n - 1) r.s += own;  // (its chunk's sum is without it)
             r.inv = 1.0 / r.s;
-            r.share = share_of(z, r.m, c) * r.inv;
+            r.share = own * r.inv;
             if ((tid & 15) == 0) lds.row[group] = r;
         }
         __syncthreads();
@@ -406,13 +470,14 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
             k.kind = last ? kFromTarget : !drawn ? kFromOthers : q.fine ? kFromRest : kFromTarget;
             k.mp = p.m;
             k.cp = cp;
-            k.ip = p.inv;
+            k.sum = p.s;
             if (k.kind == kFromRest) {
                 k.mq = q.m;
                 k.cq = cq;
-                k.iq = q.inv;
+                k.ratio = p.s * q.inv;
             }
-            k.rest = lds.rest[(stop - first) * mats];
+            k.exact = last || !drawn;
+            k.own = p.share * p.s;
             k.held = SHARES ? (stop - first) * mats : -1;
         }
     }
@@ -438,39 +503,7 @@ template <int DT, bool SHARES> __device__ __forceinline__ Pick decide(const Draf
 
 // ---- the draw ------------------------------------------------------------------------------------------------------
 
-// e^((z - m) / tau): as f32, like the sums; where p - q may cancel, f64 above 2^-6. (Below, f32's roundings are below those of the
-// sums. A vector of four takes 160 instructions more for f64: with a border of 2^-12 the sums of 38 chunks took 8 us instead of 6.2; with f64 for
-// p alone 256 draws 8.0 us instead of 6.9.)
-struct Share {
-    double m, c;
-    float mf;
-    Factor f;
-    __device__ __forceinline__ Share(double m_, double c_) : m(m_), c(c_), mf(static_cast<float>(m_)), f(c_) {}
-    template <int N> __device__ __forceinline__ void near(const float (&z)[N], float (&w)[N]) const
-    {
-#pragma unroll
-        for (int j = 0; j < N; j++) w[j] = f.power(z[j] - mf);
-    }
-    template <int N> __device__ __forceinline__ void exact(const float (&z)[N], double (&w)[N]) const
-    {
-        float e[N], most = 0.0f;
-        near(z, e);
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-            most = fmaxf(most, e[j]);
-            w[j] = e[j];
-        }
-        if (__any(most > 0x1p-6f)) {
-#pragma unroll
-            for (int j = 0; j < N; j++) {  // (all of them: a lane's powers take turns then)
-                const double v = exp2_64((static_cast<double>(z[j]) - m) * c);
-                w[j] = e[j] > 0x1p-6f ? v : w[j];
-            }
-        }
-    }
-};
-
-// A thread's 16 bytes of a chunk, and their weights as the kind says: of max(p - q, 0), or of p in units of the row's sum.
+// A thread's 16 bytes of a chunk, and their weights as the kind says: of max(p - q, 0) or of p, in units of p's powers.
 template <int DT> struct Draws {
     static constexpr int N = Vec<DT>::N;
     typedef Logits<DT, kDrawThreads> Mine;
@@ -482,30 +515,34 @@ template <int DT> struct Draws {
         if (kind == kFromRest) y.load(a.draft, k.row, a.qs, a.V, chunk);
     }
     __device__ __forceinline__ void logits(float (&z)[N]) const { Vec<DT>::unpack(x.w[0], z); }
+    __device__ static __forceinline__ void powers(const uint4& w, double m, double c, double (&p)[N])
+    {
+        float z[N];
+        Vec<DT>::unpack(w, z);
+        Power(m, c).of(z, p);
+#pragma unroll
+        for (int e = 0; e < N; e++) p[e] = p[e] > kNone ? p[e] : 0.0;
+    }
     __device__ __forceinline__ double rest(const Pick& k, double (&w)[N]) const
     {
 #pragma clang fp contract(off)  // p - q of equal numbers is 0, not the rounding of a product
-        float z[N];
-        double u[N], s = 0.0;
-        logits(z);
-        Share(k.mp, k.cp).exact(z, w);
-        Vec<DT>::unpack(y.w[0], z);
-        Share(k.mq, k.cq).exact(z, u);
+        double q[N], s = 0.0;
+        powers(x.w[0], k.mp, k.cp, w);
+        powers(y.w[0], k.mq, k.cq, q);
 #pragma unroll
         for (int e = 0; e < N; e++) {
-            w[e] = fmax(w[e] * k.ip - u[e] * k.iq, 0.0);
+            w[e] = fmax(w[e] - q[e] * k.ratio, 0.0);
             s += w[e];
         }
         return s;
     }
-    __device__ __forceinline__ float own(const Pick& k, int32_t kind, int32_t at, float (&w)[N]) const
+    __device__ __forceinline__ double own(const Pick& k, int32_t kind, int32_t at, double (&w)[N]) const
     {
-        float z[N], s = 0.0f;
-        logits(z);
-        Share(k.mp, k.cp).near(z, w);
+        double s = 0.0;
+        powers(x.w[0], k.mp, k.cp, w);
         if (kind == kFromOthers && k.token >= at && k.token < at + N) {
 #pragma unroll
-            for (int e = 0; e < N; e++) w[e] = at + e == k.token ? 0.0f : w[e];
+            for (int e = 0; e < N; e++) w[e] = at + e == k.token ? 0.0 : w[e];
         }
 #pragma unroll
         for (int e = 0; e < N; e++) s += w[e];
@@ -513,48 +550,100 @@ template <int DT> struct Draws {
     }
 };
 
-// A chunk's sum, in the first thread.
-template <int DT> __device__ __forceinline__ double chunk_sum(const DraftArgs& a, const Pick& k, int32_t chunk, double (&lds)[kDrawWaves])
+// A chunk's sums, by a block of TH threads, number j in thread j. ratio is of the rows' f32 sums: where that puts a place on the wrong side of 0, p - ratio q is
+// 2^-20 of p or less, and `rest` is corrected by the ratio's error times `above`.
+template <int DT, int TH> __device__ __forceinline__ double chunk_sums(const DraftArgs& a, const Pick& k, int32_t chunk, double (&lds)[TH / 64][4])
 {
-    double w[Vec<DT>::N];
-    Draws<DT> mine;
-    mine.load(a, k, k.kind, chunk);
-    const double s = wave_sum64(mine.rest(k, w));
-    if ((threadIdx.x & 63) == 0) lds[wave_id()] = s;
+    typedef Logits<DT, TH> Mine;
+    constexpr int N = Vec<DT>::N, kWavesHere = TH / 64;
+    const bool both = k.kind == kFromRest;
+    double s[4] = {};
+    Mine x, y;
+    x.load(a.target, k.row, a.zs, a.V, chunk);
+    if (both) y.load(a.draft, k.row, a.qs, a.V, chunk);
+    const Power of_p(k.mp, k.cp), of_q(k.mq, k.cq);
+#pragma unroll
+    for (int j = 0; j < Mine::kVecs; j++) {
+        float z[N], v[N];
+        Vec<DT>::unpack(x.w[j], z);
+        Vec<DT>::unpack(y.w[j], v);
+#pragma unroll
+        for (int e = 0; e < N; e += kTogether) {
+            double p[kTogether], q[kTogether];
+            of_p.of(&z[e], p);
+#pragma unroll
+            for (int i = 0; i < kTogether; i++) s[0] += p[i];
+            if (both) {
+                of_q.of(&v[e], q);
+#pragma unroll
+                for (int i = 0; i < kTogether; i++) {
+                    const double rest = fma(-k.ratio, q[i], p[i]);
+                    s[1] += q[i];
+                    s[2] += fmax(rest, 0.0);
+                    s[3] += rest > 0.0 ? q[i] : 0.0;
+                }
+            }
+        }
+    }
+    const int lane = threadIdx.x & 63;
+    double v = wave_sums64(s);
+    if (lane < 4) lds[wave_id()][lane] = v;
     __syncthreads();
-    return row_sum64(lds[threadIdx.x & (kDrawWaves - 1)]);
+    v = lane >> 2 < kWavesHere ? lds[lane >> 2 & (kWavesHere - 1)][lane & 3] : 0.0;
+    return sum_by_four(v);
 }
 
-// A chunk that has less of the row's largest exponential has no weight: the places of one that has are f32 powers of the same
-// largest, so one of its at most 2^13 is above 2^-123 and not 0 (a random number of 0 would be above none of them).
-constexpr double kLeastShare = 0x1p-110;
+// What is below it counts as 0: a chunk that is above has a place that is above 2^-1000 (a random number of 0 is above no other's sum).
+constexpr double kLeastShare = 0x1p-900;
 
-// The draw itself, by the whole block. Chunk c's weight is sums[c], or where there are none p's, of the target's chunk sums: of the chunk that
-// holds the refused draft the one that was made without it (a difference would leave nothing beside a draft of nearly all).
+// The draw itself, by the whole block, in units of p's powers. Where the draft was drawn and refused, chunk c's weight is of its sums[c]; else of the target's chunk
+// sums, which leave a chosen draft out (a difference would leave nothing beside a draft of nearly all).
 // Every wave finds the chunk for itself, a lane for one or more neighbours, and all of them the place in it, 16 bytes a thread.
-template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32_t i, const Pick& k, float u, const double* sums, const double* shares)
+template <int DT, bool DRAWN> __device__ __forceinline__ void pick(const DraftArgs& a, int32_t i, Pick k, float u, const double* shares)
 {
     constexpr int N = Vec<DT>::N;
     __shared__ double s_part[kDrawWaves], s_log;
     __shared__ int32_t s_flags[kDrawWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+    const int32_t each = (a.chunks + 63) / 64, c0 = min(lane * each, a.chunks), c1 = min(c0 + each, a.chunks);
     const ChunkStat* st = a.stats + static_cast<int64_t>(k.row) * 2 * a.chunks;
+    const ChunkSums* sums = a.sums + static_cast<int64_t>(i) * a.chunks;
     int32_t kind = k.kind;
     const int32_t other = kind == kFromOthers && k.token >= 0 && k.token < a.V ? k.token / kChunk<DT> : -1;
-    const auto target = [&](int32_t c) {
-        double v;
-        if (kind == kFromOthers && c == other) {
-            v = k.rest;
-        } else if (shares && c < 16 * kHeld) {
+    const bool summed = DRAWN && !k.exact;
+    double correct = 0.0;  // of the ratio
+    ChunkSums near{};      // of the lane's first chunk
+    if (summed) {
+        if (c0 < c1) near = sums[c0];
+        double p = near.p, q = near.q;
+        for (int32_t c = c0 + 1; c < c1; c++) {
+            p += sums[c].p;
+            q += sums[c].q;
+        }
+        k.sum = wave_sum64(p);
+        if (kind == kFromRest) {
+            const double exact = k.sum / wave_sum64(q);
+            correct = exact - k.ratio;
+            k.ratio = exact;
+        }
+    }
+    const auto weight = [&](int32_t c) {
+        double v, least = kLeastShare;
+        if (summed) {
+            const ChunkSums x = c == c0 ? near : sums[c];
+            v = x.p;
+            if (kind == kFromRest) {
+                v = x.rest - correct * x.above;
+                least = fmax(least, 0x1p-36 * (v + k.ratio * x.above));  // (below it are roundings: there may be no place that has a weight)
+            }
+        } else if (!DRAWN && c < 16 * kHeld) {
             v = shares[c];
         } else {
             const ChunkStat x = st[c];
-            v = x.m > -INFINITY ? x.s * exp2_64((static_cast<double>(x.m) - k.mp) * k.cp) : 0.0;
+            v = x.m > -INFINITY ? x.s * Power(k.mp, k.cp).at(x.m) : 0.0;
         }
-        return v > kLeastShare ? v * k.ip : 0.0;
+        return (v > least ? v : 0.0) + (kind == kFromTarget && c == other ? k.own : 0.0);
     };
-    const auto weight = [&](int32_t c) { return sums && kind != kFromTarget ? sums[c] : target(c); };
-    const int32_t each = (a.chunks + 63) / 64, c0 = min(lane * each, a.chunks), c1 = min(c0 + each, a.chunks);
     const auto sum_of = [&]() {
         double s = 0.0;
         for (int32_t c = c0; c < c1; c++) s += weight(c);
@@ -587,15 +676,10 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
     }
     Draws<DT> of;
     of.load(a, k, kind, chunk);
-    if (a.logp && wave == 0) s_log = log(k.ip);  // while the loads are on their way
+    if (a.logp && wave == 0) s_log = log(k.sum);  // while the loads are on their way
     const int32_t at = Logits<DT, kDrawThreads>::place(chunk, 0);
-    double w[N], s;
-    float e[N];
-    if (kind == kFromRest) {
-        s = of.rest(k, w);
-    } else {
-        s = of.own(k, kind, at, e) * k.ip;
-    }
+    double w[N];
+    const double s = kind == kFromRest ? of.rest(k, w) : of.own(k, kind, at, w);
     double c = wave_scan64(s);
     if (lane == 63) s_part[wave] = c;
     c -= s;
@@ -620,7 +704,7 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
     bool there = false;
 #pragma unroll
     for (int n = 0; n < N; n++) {
-        const double v = kind == kFromRest ? w[n] : e[n] * k.ip;
+        const double v = w[n];
         c += v;
         if (v > 0.0 && !there) {
             token = at + n;
@@ -629,7 +713,7 @@ template <int DT> __device__ __forceinline__ void pick(const DraftArgs& a, int32
         }
     }
     a.out[i * a.out_stride + k.place] = token;
-    if (a.logp) a.logp[i * a.out_stride + k.place] = static_cast<float>((logit - k.mp) * (k.cp / kLog2e64) + s_log);
+    if (a.logp) a.logp[i * a.out_stride + k.place] = static_cast<float>((logit - k.mp) * (k.cp / kLog2e64) - s_log);
 }
 
 // Drafts that were chosen, or none: the sums of p are there, a thread block a request does the rest.
@@ -638,7 +722,7 @@ template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_choose(D
     __shared__ DecideLds lds;
     const float u = a.T > 0 ? a.sample[blockIdx.x] : 0.0f;
     const Pick k = decide<DT, true>(a, blockIdx.x, true, lds);
-    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, u, nullptr, lds.shares[k.held]);
+    if (k.kind != kDone) pick<DT, false>(a, blockIdx.x, k, u, lds.shares[k.held]);
 }
 
 // Drafts that were drawn: what is accepted, then a thread block for each chunk of the row that is drawn from. Few chunks in all (kDecides) are
@@ -653,9 +737,10 @@ template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_decide(D
 constexpr int64_t kDecides = 512;
 constexpr unsigned kRequestsY = 32768;  // of a launch's second dimension
 
-template <int DT, bool DECIDES> __global__ __launch_bounds__(kDrawThreads) void draft_sums(DraftArgs a)
+template <int DT, bool DECIDES> __global__ __launch_bounds__(DECIDES ? kDrawThreads : kThreads) void draft_sums(DraftArgs a)
 {
-    __shared__ double s_sum[kDrawWaves];
+    constexpr int TH = DECIDES ? kDrawThreads : kThreads;
+    __shared__ double s_sum[TH / 64][4];
     const int32_t i = blockIdx.z * kRequestsY + blockIdx.y, chunk = blockIdx.x;
     if (i >= a.B) return;
     Pick k;
@@ -666,16 +751,16 @@ template <int DT, bool DECIDES> __global__ __launch_bounds__(kDrawThreads) void 
     } else {
         k = a.picks[i];
     }
-    if (k.kind != kFromRest) return;
-    const double s = chunk_sum<DT>(a, k, chunk, s_sum);
-    if (threadIdx.x == 0) a.sums[static_cast<int64_t>(i) * a.chunks + chunk] = s;
+    if (k.kind == kDone || k.exact) return;
+    const double s = chunk_sums<DT, TH>(a, k, chunk, s_sum);
+    if (threadIdx.x < 4) reinterpret_cast<double*>(a.sums + static_cast<int64_t>(i) * a.chunks + chunk)[threadIdx.x] = s;
 }
 
 template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_pick(DraftArgs a)
 {
     const float u = a.T > 0 ? a.sample[blockIdx.x] : 0.0f;
     const Pick k = a.picks[blockIdx.x];
-    if (k.kind != kDone) pick<DT>(a, blockIdx.x, k, u, k.kind == kFromRest ? a.sums + static_cast<int64_t>(blockIdx.x) * a.chunks : nullptr, nullptr);
+    if (k.kind != kDone) pick<DT, true>(a, blockIdx.x, k, u, nullptr);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------
@@ -685,7 +770,7 @@ static int64_t round16(int64_t n) { return (n + 15) & ~int64_t{15}; }
 // The workspace: chunk sums of all rows, the picks, their chunks' sums.
 static int64_t work_of(int64_t B, int64_t T, int64_t chunks)
 {
-    return T * 2 * chunks * static_cast<int64_t>(sizeof(ChunkStat)) + round16(B * static_cast<int64_t>(sizeof(Pick))) + round16(B * chunks * 8);
+    return T * 2 * chunks * static_cast<int64_t>(sizeof(ChunkStat)) + round16(B * static_cast<int64_t>(sizeof(Pick))) + B * chunks * static_cast<int64_t>(sizeof(ChunkSums));
 }
 
 // chunks: of the smaller kind, f32's.
@@ -723,7 +808,7 @@ template <int DT> static int launch(DraftArgs& a, hipStream_t st)
         draft_decide<DT><<<B, kDrawThreads, 0, st>>>(a);
         const int e = check_launch("draft_decide");
         if (e) return e;
-        draft_sums<DT, false><<<chunks, kDrawThreads, 0, st>>>(a);
+        draft_sums<DT, false><<<chunks, kThreads, 0, st>>>(a);
     }
     const int e = check_launch("draft_sums");
     if (e) return e;
@@ -784,7 +869,7 @@ extern "C" SLHIP_API int slhip_draft_verify(int dtype, const void* target, int64
     a.logp = d->logp;
     a.stats = static_cast<ChunkStat*>(work);
     a.picks = reinterpret_cast<Pick*>(a.stats + a.T * 2 * chunks);
-    a.sums = reinterpret_cast<double*>(reinterpret_cast<char*>(a.picks) + round16(a.B * static_cast<int64_t>(sizeof(Pick))));
+    a.sums = reinterpret_cast<ChunkSums*>(reinterpret_cast<char*>(a.picks) + round16(a.B * static_cast<int64_t>(sizeof(Pick))));
     e = error_word(&a.err);
     if (e) return e;
     return dtype == SLHIP_F32 ? launch<SLHIP_F32>(a, to_stream(stream)) : launch<SLHIP_BF16>(a, to_stream(stream));
