@@ -550,47 +550,41 @@ template <int DT> struct Draws {
     }
 };
 
-// A chunk's sums, by a block of TH threads, number j in thread j. ratio is of the rows' f32 sums: where that puts a place on the wrong side of 0, p - ratio q is
+// A chunk's sums, by the whole block, number j in thread j. ratio is of the rows' f32 sums: where that puts a place on the wrong side of 0, p - ratio q is
 // 2^-20 of p or less, and `rest` is corrected by the ratio's error times `above`.
-template <int DT, int TH> __device__ __forceinline__ double chunk_sums(const DraftArgs& a, const Pick& k, int32_t chunk, double (&lds)[TH / 64][4])
+template <int DT> __device__ __forceinline__ double chunk_sums(const DraftArgs& a, const Pick& k, int32_t chunk, double (&lds)[kDrawWaves][4])
 {
-    typedef Logits<DT, TH> Mine;
-    constexpr int N = Vec<DT>::N, kWavesHere = TH / 64;
+    constexpr int N = Vec<DT>::N;
     const bool both = k.kind == kFromRest;
     double s[4] = {};
-    Mine x, y;
-    x.load(a.target, k.row, a.zs, a.V, chunk);
-    if (both) y.load(a.draft, k.row, a.qs, a.V, chunk);
+    float z[N], v[N];
+    Draws<DT> mine;
+    mine.load(a, k, k.kind, chunk);
+    Vec<DT>::unpack(mine.x.w[0], z);
+    if (both) Vec<DT>::unpack(mine.y.w[0], v);
     const Power of_p(k.mp, k.cp), of_q(k.mq, k.cq);
 #pragma unroll
-    for (int j = 0; j < Mine::kVecs; j++) {
-        float z[N], v[N];
-        Vec<DT>::unpack(x.w[j], z);
-        Vec<DT>::unpack(y.w[j], v);
+    for (int e = 0; e < N; e += kTogether) {
+        double p[kTogether], q[kTogether];
+        of_p.of(&z[e], p);
 #pragma unroll
-        for (int e = 0; e < N; e += kTogether) {
-            double p[kTogether], q[kTogether];
-            of_p.of(&z[e], p);
+        for (int i = 0; i < kTogether; i++) s[0] += p[i];
+        if (both) {
+            of_q.of(&v[e], q);
 #pragma unroll
-            for (int i = 0; i < kTogether; i++) s[0] += p[i];
-            if (both) {
-                of_q.of(&v[e], q);
-#pragma unroll
-                for (int i = 0; i < kTogether; i++) {
-                    const double rest = fma(-k.ratio, q[i], p[i]);
-                    s[1] += q[i];
-                    s[2] += fmax(rest, 0.0);
-                    s[3] += rest > 0.0 ? q[i] : 0.0;
-                }
+            for (int i = 0; i < kTogether; i++) {
+                const double rest = fma(-k.ratio, q[i], p[i]);
+                s[1] += q[i];
+                s[2] += fmax(rest, 0.0);
+                s[3] += rest > 0.0 ? q[i] : 0.0;
             }
         }
     }
     const int lane = threadIdx.x & 63;
-    double v = wave_sums64(s);
-    if (lane < 4) lds[wave_id()][lane] = v;
+    const double sum = wave_sums64(s);
+    if (lane < 4) lds[wave_id()][lane] = sum;
     __syncthreads();
-    v = lane >> 2 < kWavesHere ? lds[lane >> 2 & (kWavesHere - 1)][lane & 3] : 0.0;
-    return sum_by_four(v);
+    return sum_by_four(lds[lane >> 2][lane & 3]);
 }
 
 // What is below it counts as 0: a chunk that is above has a place that is above 2^-1000 (a random number of 0 is above no other's sum).
@@ -737,10 +731,9 @@ template <int DT> __global__ __launch_bounds__(kDrawThreads) void draft_decide(D
 constexpr int64_t kDecides = 512;
 constexpr unsigned kRequestsY = 32768;  // of a launch's second dimension
 
-template <int DT, bool DECIDES> __global__ __launch_bounds__(DECIDES ? kDrawThreads : kThreads) void draft_sums(DraftArgs a)
+template <int DT, bool DECIDES> __global__ __launch_bounds__(kDrawThreads) void draft_sums(DraftArgs a)
 {
-    constexpr int TH = DECIDES ? kDrawThreads : kThreads;
-    __shared__ double s_sum[TH / 64][4];
+    __shared__ double s_sum[kDrawWaves][4];
     const int32_t i = blockIdx.z * kRequestsY + blockIdx.y, chunk = blockIdx.x;
     if (i >= a.B) return;
     Pick k;
@@ -752,7 +745,7 @@ template <int DT, bool DECIDES> __global__ __launch_bounds__(DECIDES ? kDrawThre
         k = a.picks[i];
     }
     if (k.kind == kDone || k.exact) return;
-    const double s = chunk_sums<DT, TH>(a, k, chunk, s_sum);
+    const double s = chunk_sums<DT>(a, k, chunk, s_sum);
     if (threadIdx.x < 4) reinterpret_cast<double*>(a.sums + static_cast<int64_t>(i) * a.chunks + chunk)[threadIdx.x] = s;
 }
 
@@ -808,7 +801,7 @@ template <int DT> static int launch(DraftArgs& a, hipStream_t st)
         draft_decide<DT><<<B, kDrawThreads, 0, st>>>(a);
         const int e = check_launch("draft_decide");
         if (e) return e;
-        draft_sums<DT, false><<<chunks, kThreads, 0, st>>>(a);
+        draft_sums<DT, false><<<chunks, kDrawThreads, 0, st>>>(a);
     }
     const int e = check_launch("draft_sums");
     if (e) return e;
