@@ -16,11 +16,11 @@
 // exponentials to 2^-39. Those are the sums of the rows that may be drawn from as they are (a request's last one, and all without draft logits), and what is made of
 // the one row behind a refused draft.
 //
-// Measured: the sums of 257 rows of 151936 f32 logits and of 193 draft rows (273 MB) 45.6 us, 6.0 TB/s, in bf16 (137 MB) 30.3, of which the vector
-// unit works 89%; of 256 rows of 50257 bf16 logits (25.7 MB) 11.4 us, of which some 3.5 are exponentials that the loads, all on their way at once, do not
-// hide, of 64 rows 5.9. What follows is a latency: 256 or 64 draws 6.7 us in one launch (choose), 16 requests' looked-up drafts 7.1; 64 requests with draft
-// logits 5.5 (decide), 13.2 (2432 chunks of p and q, 78 MB out of the last-level cache; bf16 14.0) and 6.2 (pick; bf16 8.1); one request with drafts 6.4 (38
-// chunks that decide for themselves) and 4.3.
+// Measured: the sums of 257 rows of 151936 f32 logits and of 193 draft rows (273 MB) 47.0 us, 5.8 TB/s (with f32 exponentials alone 45.6), in bf16 (137 MB) 34.2, of
+// which the vector unit works 91%; of 256 rows of 50257 bf16 logits (25.7 MB) 15.7 us (f32 11.4; without any 9.8: the loads, all on their way at once, do not hide the
+// exponentials, and two chunks a thread block, the second one loaded behind the first, take 17.4), of 64 rows 7.0. What follows is a latency: 256 draws 7.7 us in one
+// launch (choose), 64 7.2, 16 requests' looked-up drafts 7.1; 64 requests with draft logits 5.6 (decide), 13.7 (2432 chunks of p and q, 78 MB out of the last-level
+// cache; bf16 13.0) and 6.8 (pick; bf16 7.9); one request with drafts 6.6 (38 chunks that decide for themselves) and 5.4.
 #include <math.h>
 
 #include "step.hpp"
